@@ -370,12 +370,12 @@ def own_cache(s):
     case, ctx = s["case"], context()
     before, new = lengths(case)
     pages = [-(-(a + b) // PAGE) for a, b in zip(before, new)]
-    kv = ctx.kv_cache_q4(1, case["kv"], case["dim"], sum(pages), case["seqs"], max(pages))
+    kv = ctx.kv_cache_q4(1, case["heads"], case["kv"], case["dim"], sum(pages), case["seqs"], max(pages), dtype=case["type"])
     seqs = [kv.seq_alloc() for _ in before]
     torch.cuda.synchronize()
     if sum(before):
         kv.batch(seqs, [0] * len(seqs), before)
-        kv.write_dev(0, s["old_k"].data_ptr(), s["old_v"].data_ptr(), dtype=case["type"])
+        kv.write_dev(0, s["old_k"].data_ptr(), s["old_v"].data_ptr())
     kv.batch(seqs, before, new)
     ctx.synchronize()
     s["kv"] = kv
@@ -384,8 +384,8 @@ def own_cache(s):
 
 
 def attend_own(s):
-    case, k, v = s["case"], *s["held"]
-    s["kv"].attend_dev(0, s["q"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), case["heads"], s["scale"], s["out"].data_ptr(), dtype=case["type"], k_held=k.data_ptr(), v_held=v.data_ptr())
+    k, v = s["held"]
+    s["kv"].attend_dev(0, s["q"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), s["scale"], s["out"].data_ptr(), k_held=k.data_ptr(), v_held=v.data_ptr())
     return {"out": s["out"], "k": k, "v": v}
 
 
