@@ -42,6 +42,7 @@ struct dc_ctx {
     size_t scratch_bytes = 0;
     void* pinned = nullptr;        // small pinned staging area for host<->device results
     size_t pinned_bytes = 0;
+    int stage_off = 0;             // block table entries staged in `pinned` so far (kv.cu)
     int use_pdl = 1;
     int route_mode = 0;            // router variant of the op-level MoE calls (DC_ROUTE_*)
 };

@@ -14,6 +14,7 @@ struct dc_kv_seq {
     std::vector<int> blocks;     // logical block -> physical block
 };
 
+struct dc_q4;
 struct dc_kv_cache {
     dc_ctx* ctx = nullptr;
     int n_layer = 0, n_kv = 0, head_dim = 0;
@@ -29,10 +30,11 @@ struct dc_kv_cache {
     std::vector<plane> planes;
     uint8_t* state = nullptr;    // [max_seqs][state_bytes]
     size_t state_bytes = 0;
+    struct dc_q4* q4 = nullptr;  // of a cache in 4 bits (planes of its layers)
+    uint64_t edits = 0;          // changes of sequences and their blocks
     std::vector<int> free_list;
     std::vector<int> ref;        // references per physical block (sequences sharing it after a fork)
     std::vector<dc_kv_seq> seqs;
-    int stage_off = 0;
     // Prefix cache (core/include/densecore/memory/kv_cache.h:176-213): a full block can be registered under
     // the hash of the whole token prefix that ends with it; the cache then holds one reference of its own, so
     // the block outlives its sequence until it is evicted (least recently used first) to satisfy an allocation.
@@ -49,6 +51,7 @@ int dc_kv_init(dc_ctx* ctx, dc_kv_cache* kv, int n_layer, int n_kv_head, int hea
 int dc_kv_init_planes(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<size_t>& row_bytes, size_t state_bytes, int max_blocks, int max_seqs,
                       int max_blocks_per_seq);
 void dc_kv_release(dc_kv_cache* kv);
+DC_PART void dc_q4_release(dc_kv_cache* kv);
 int dc_kv_seq_alloc(dc_kv_cache* kv, int* out_seq);
 int dc_kv_seq_free(dc_kv_cache* kv, int seq);
 int dc_kv_seq_reserve(dc_kv_cache* kv, int seq, int n_tokens);

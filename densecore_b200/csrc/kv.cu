@@ -97,6 +97,7 @@ static int take_block(dc_kv_cache* kv) {
 }
 
 void dc_kv_release(dc_kv_cache* kv) {
+    if (dc_q4_release) dc_q4_release(kv);
     if (kv->k_arena) cudaFree(kv->k_arena);
     if (kv->v_arena) cudaFree(kv->v_arena);
     if (kv->d_tables) cudaFree(kv->d_tables);
@@ -125,6 +126,7 @@ int dc_kv_seq_alloc(dc_kv_cache* kv, int* out_seq) {
 int dc_kv_seq_free(dc_kv_cache* kv, int seq) {
     if (seq < 0 || seq >= kv->max_seqs || !kv->seqs[seq].used)
         return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv: sequence %d is not allocated", seq);
+    ++kv->edits;
     // a block returns to the free list when its last reference goes (kv_cache.h:140)
     for (int b : kv->seqs[seq].blocks)
         if (--kv->ref[b] <= 0) {
@@ -149,16 +151,22 @@ static int upload_table(dc_kv_cache* kv, int seq, int first, int n) {
     if (n <= 0) return DC_B200_OK;
     int32_t* stage = (int32_t*)dc_pinned(kv->ctx, 64 * 1024);
     if (!stage) return DC_B200_OUT_OF_MEMORY;
-    if (n > 16 * 1024) return dc_fail(kv->ctx, DC_B200_UNSUPPORTED, "kv: too many new blocks at once");
-    if (kv->stage_off + n > 16 * 1024) {   // a small pinned ring keeps the async copy source valid
-        cudaStreamSynchronize(kv->ctx->stream);
-        kv->stage_off = 0;
+    int& off = kv->ctx->stage_off;      // a small pinned ring, shared by the context's caches, keeps the async copy source valid
+    while (n > 0) {
+        const int c = n < 16 * 1024 ? n : 16 * 1024;
+        if (off + c > 16 * 1024) {
+            cudaStreamSynchronize(kv->ctx->stream);
+            off = 0;
+        }
+        memcpy(stage + off, kv->seqs[seq].blocks.data() + first, (size_t)c * sizeof(int32_t));
+        cudaError_t e = cudaMemcpyAsync(kv->d_tables + (size_t)seq * kv->max_blocks_per_seq + first, stage + off, (size_t)c * sizeof(int32_t),
+                                        cudaMemcpyHostToDevice, kv->ctx->stream);
+        off += c;
+        if (e != cudaSuccess) return dc_check_cuda(kv->ctx, e, "kv: block table upload");
+        first += c;
+        n -= c;
     }
-    memcpy(stage + kv->stage_off, kv->seqs[seq].blocks.data() + first, (size_t)n * sizeof(int32_t));
-    cudaError_t e = cudaMemcpyAsync(kv->d_tables + (size_t)seq * kv->max_blocks_per_seq + first, stage + kv->stage_off,
-                                    (size_t)n * sizeof(int32_t), cudaMemcpyHostToDevice, kv->ctx->stream);
-    kv->stage_off += n;
-    return dc_check_cuda(kv->ctx, e, "kv: block table upload");
+    return DC_B200_OK;
 }
 
 // New sequence that shares every block of src (Fork, kv_cache.h:151-156): nothing is copied now; a shared
@@ -166,6 +174,7 @@ static int upload_table(dc_kv_cache* kv, int seq, int first, int n) {
 int dc_kv_seq_fork(dc_kv_cache* kv, int src_seq, int* out_seq) {
     if (src_seq < 0 || src_seq >= kv->max_seqs || !kv->seqs[src_seq].used)
         return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv: sequence %d is not allocated", src_seq);
+    ++kv->edits;
     int dst = -1;
     int st = dc_kv_seq_alloc(kv, &dst);
     if (st != DC_B200_OK) return st;
@@ -190,6 +199,7 @@ int dc_kv_seq_fork(dc_kv_cache* kv, int src_seq, int* out_seq) {
 int dc_kv_seq_reserve(dc_kv_cache* kv, int seq, int n_tokens) {
     if (seq < 0 || seq >= kv->max_seqs || !kv->seqs[seq].used)
         return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv: sequence %d is not allocated", seq);
+    ++kv->edits;
     dc_kv_seq& s = kv->seqs[seq];
     const int need = (n_tokens + DC_KV_BLOCK - 1) / DC_KV_BLOCK;
     if (need > kv->max_blocks_per_seq)
@@ -247,6 +257,7 @@ int dc_kv_prefix_attach(dc_kv_cache* kv, int seq, const int32_t* tokens, int n_t
     dc_kv_seq& s = kv->seqs[seq];
     if (s.len != 0 || !s.blocks.empty())
         return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv: prefix lookup needs an empty sequence (sequence %d holds %d tokens)", seq, s.len);
+    ++kv->edits;
     ++kv->prefix_lookups;
     if (kv->state_bytes) return DC_B200_OK;     // cached blocks alone do not bring a recurrent state back
     if (!tokens || n_tokens <= DC_KV_BLOCK) return DC_B200_OK;
@@ -277,6 +288,7 @@ int dc_kv_prefix_register(dc_kv_cache* kv, int seq, const int32_t* tokens, int n
     if (seq < 0 || seq >= kv->max_seqs || !kv->seqs[seq].used || !tokens)
         return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv: sequence %d is not allocated", seq);
     if (kv->state_bytes) return DC_B200_OK;
+    ++kv->edits;
     dc_kv_seq& s = kv->seqs[seq];
     if (n_tokens > s.len) n_tokens = s.len;
     uint64_t h = 14695981039346656037ULL;
