@@ -110,6 +110,12 @@ def _signatures() -> dict:
         "dc_b200_flash_attn_decode": (i32, [vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, f32, vp]),
         "dc_b200_flash_attn_prefill": (i32, [vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, f32, vp]),
         "dc_b200_kv_read_block": (i32, [vp, i32, i32, vp, vp]),
+        "dc_b200_kv_create_q4": (i32, [vp, i32, i32, i32, i32, i32, i32, i32, i32, pp]),
+        "dc_b200_kv_batch": (i32, [vp, i32, vp, vp, vp]),
+        "dc_b200_kv_q4_write_dev": (i32, [vp, vp, i32, vp, vp, i32, vp, vp]),
+        "dc_b200_flash_attn_q4_dev": (i32, [vp, vp, i32, vp, i32, vp, vp, i32, f32, vp, i32, vp, vp]),
+        "dc_b200_flash_attn_q4": (i32, [vp, vp, i32, vp, vp, vp, f32, vp]),
+        "dc_b200_kv_q4_read_block": (i32, [vp, i32, i32, vp, vp]),
         "dc_b200_argmax": (i32, [vp, vp, i32, i32, vp]),
         "dc_b200_verify_accept": (i32, [vp, vp, vp, vp, vp, u64, u32, i32, i32, i32, f32, pi, pi]),
         "dc_b200_verify_uniforms": (i32, [vp, u64, u32, i32, vp]),

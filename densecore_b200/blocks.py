@@ -17,6 +17,7 @@ GGML_TYPE_F32 = 0
 GGML_TYPE_F16 = 1
 GGML_TYPE_Q4_K = 12
 GGML_TYPE_Q6_K = 14
+GGML_TYPE_BF16 = 30
 QK_K = 256
 BLOCK_BYTES = {GGML_TYPE_Q4_K: 144, GGML_TYPE_Q6_K: 210}
 Q8K_BYTES = 292

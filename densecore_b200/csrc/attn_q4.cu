@@ -1,0 +1,699 @@
+// Attention over a paged cache that holds keys and values in 4 bits.
+//
+// A cached row of a head is held in groups of 64 values: m = fp16(least), d = fp16((largest - least) * fp32(1/15)), codes
+// q = rint((x - m) / d) within 0..15 (0 where d is 0), all in fp32; a code stands for fp32(d q + m).  A group with a value that is not
+// finite or beyond +-65504 is held with d = m = NaN, and reads back so.  Blocks, tables, sharing and copy-on-write are kv.cu's, on planes of
+// one record per (page, key head) (dc_q4.h).  A step is planned once (dc_b200_kv_batch) and then run for every layer.
+//
+// Scores of a token: sum over groups of d (q . codes) + m (sum of q): the codes go to the tensor cores as they are (fp16 subnormals c 2^-24 and
+// c 2^-20, exact), queries as two fp16 terms, and the scale is applied to the f32 sum.  Values: sum over tokens of (p d) codes, the weights
+// p d as two fp16 terms, plus the sum of p m in f32.  The two terms are rows h and h + 8 of one m16 operand, so that they cost no extra product.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "dc_common.cuh"
+#include "dc_internal.h"
+#include "dc_launch.cuh"
+#include "dc_q4.h"
+
+using namespace dc;
+
+#define DC_TRY(expr)                       \
+    do {                                   \
+        int _st = (expr);                  \
+        if (_st != DC_B200_OK) return _st; \
+    } while (0)
+
+namespace {
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void put(float* p, float x) { *p = x; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_h2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ---------------------------------------------------------------- new rows into the cache
+struct WriteParams {
+    const uint8_t* plan;
+    const void *k, *v;
+    int ldkv, n_kv, max_blocks;
+    const int32_t* tables;
+    uint8_t* arena;
+    float *k_held, *v_held;      // [T][n_kv][HD], may be null
+};
+
+// One warp per (token, key head, key or value).  Bound: latency (a step's rows are some KB).
+template <int HD, typename TX>
+__global__ void __launch_bounds__(128) k_q4_write(const WriteParams p) {
+    using R = dc_q4_rec<HD>;
+    constexpr int PER = HD / 32;      // neighbouring values of a lane
+    __shared__ uint8_t codes[4][HD];
+    pdl_wait();
+    pdl_launch_dependents();      // (not before the wait: what the next kernel reads ahead of its own wait has to be complete)
+    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
+    const int32_t* tok = reinterpret_cast<const int32_t*>(p.plan) + hd->tokens;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = hd->T * p.n_kv * 2;
+    for (int u = blockIdx.x * 4 + warp; u < units; u += gridDim.x * 4) {
+        const int t = u / (2 * p.n_kv), w = u - t * 2 * p.n_kv, head = w >> 1, is_v = w & 1;
+        const int seq = tok[2 * t], pos = tok[2 * t + 1], slot = pos % DC_KV_BLOCK;
+        const TX* src = reinterpret_cast<const TX*>(is_v ? p.v : p.k) + (size_t)t * p.ldkv + head * HD + PER * lane;
+        float x[PER], lo = INFINITY, hi = -INFINITY;
+        bool fine = true;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            x[i] = to_f32(src[i]);
+            fine = fine && fabsf(x[i]) <= 65504.0f;
+            lo = fminf(lo, x[i]);
+            hi = fmaxf(hi, x[i]);
+        }
+        constexpr int LANES = 64 / PER;      // of a group
+#pragma unroll
+        for (int s = LANES / 2; s > 0; s >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+        }
+        const uint32_t bad = __ballot_sync(0xffffffffu, !fine) >> (lane / LANES * LANES);
+        __half d = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), m = __float2half_rn(lo);
+        const float df = __half2float(d), mf = __half2float(m);
+        const bool nan = (LANES == 32 ? bad : bad & ((1u << (LANES & 31)) - 1u)) != 0;
+        int q[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) q[i] = !nan && df > 0.0f ? (int)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mf), df)), 0.0f), 15.0f) : 0;
+        if (nan) d = m = __ushort_as_half((unsigned short)0x7FFF);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) codes[warp][PER * lane + i] = (uint8_t)q[i];
+        __syncwarp();
+        const int block = p.tables[(size_t)seq * p.max_blocks + pos / DC_KV_BLOCK];
+        uint8_t* rec = p.arena + ((size_t)block * p.n_kv + head) * R::BYTES;
+        if (lane % LANES == 0)
+            reinterpret_cast<__half2*>(rec + (is_v ? R::V_SCALES : R::K_SCALES))[slot * R::GROUPS + lane / LANES] = __halves2half2(d, m);
+        const uint8_t* c = codes[warp];
+        if (!is_v) {
+            if (lane < HD / 8) {
+                const int t4 = lane & 3, i = lane >> 2;
+                uint32_t word = 0;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) word |= (uint32_t)c[32 * i + 8 * (n & 3) + 2 * t4 + (n >> 2)] << (4 * n);
+                *reinterpret_cast<uint32_t*>(rec + R::k_word(slot, t4, i)) = word;
+            }
+        } else {
+#pragma unroll
+            for (int b = lane; b < HD / 2; b += 32) {
+                const int d8 = b & 7, i = b >> 3;
+                rec[R::v_byte(slot, d8, i)] = c[16 * i + d8] | (uint8_t)(c[16 * i + 8 + d8] << 4);
+            }
+        }
+        float* held = is_v ? p.v_held : p.k_held;
+        if (held) {
+            const float ds = __half2float(d), ms = __half2float(m);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) held[((size_t)t * p.n_kv + head) * HD + PER * lane + i] = fmaf(ds, (float)q[i], ms);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- attention, eight rows at a time
+struct RowsParams {
+    const uint8_t* plan;
+    const void* q;
+    int ldq, ldo, heads, n_kv, max_blocks;
+    const int32_t* tables;
+    const uint8_t* arena;
+    float scale;
+    void* out;
+    int early;      // the kernel before this one wrote the step's rows and waited for all before it: older pages may be read ahead of the wait
+    int* err;
+};
+
+constexpr int RW = DC_Q4_WARPS;
+constexpr int RW_STAGES = 4;      // pages in flight, per warp
+template <int HD>
+constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BYTES + RW * RW_STAGES * 8 + (size_t)RW * 8 * (HD + 2) * 4; }
+
+// One CTA per (item, key head): its warps take the item's pages in turn, each with a running maximum of its own, and join at the end; the last CTA of a tile joins
+// the tile's splits in their order, so that results do not depend on who comes last.
+// A lane has row h = lane / 4 of the tile, tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page and dimensions 8 j + 2 t, + 1 of the answers (t = lane % 4).
+template <int HD, typename TX>
+__global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
+    using R = dc_q4_rec<HD>;
+    constexpr int GR = R::GROUPS, KW = HD / 32, VW = HD / 16;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int s_last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t4 = lane & 3, kvh = blockIdx.y, G = p.heads / p.n_kv;
+    const uint32_t ring = smem_u32(smem) + warp * RW_STAGES * R::BYTES, bars = smem_u32(smem) + RW * RW_STAGES * R::BYTES + warp * RW_STAGES * 8;
+    float* part = reinterpret_cast<float*>(smem + RW * RW_STAGES * R::BYTES + RW * RW_STAGES * 8);      // [RW][8][HD], then maxima and sums
+    float* part_ml = part + RW * 8 * HD;
+    if (lane == 0) {
+        for (int s = 0; s < RW_STAGES; ++s) mbar_init(bars + 8 * s, 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
+    bool waited = !p.early;
+    if (waited) pdl_wait();
+    pdl_launch_dependents();
+    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
+    const int32_t* words = reinterpret_cast<const int32_t*>(p.plan);
+    const int n_items = hd->n_items;
+    uint32_t n_full = 0;      // pages that this warp has waited for
+    for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+        const dc_q4_item im = reinterpret_cast<const dc_q4_item*>(words + hd->items)[it];
+        const int r = im.tile * 8 + h, j = r / G, g = r - j * G;
+        const bool row = j < im.count;
+        const int qpos = im.pos0 + j, first_new = im.pos0 / DC_KV_BLOCK, all_see = im.pos0 + im.tile * 8 / G;      // positions up to all_see: seen by every row
+        const int n_my = (im.page1 - im.page0 - warp + RW - 1) / RW;
+        const int32_t* table = p.tables + (size_t)im.seq * p.max_blocks;
+        int entry = 0;      // lane i: the block of page (i + a multiple of 32) of this warp
+        auto issue = [&](int i) {
+            const int page = im.page0 + warp + i * RW;
+            if (i % 32 == 0) entry = i + lane < n_my ? table[page + lane * RW] : 0;
+            if (!waited && page >= first_new) pdl_wait(), waited = true;
+            const int block = __shfl_sync(0xffffffffu, entry, i % 32);
+            if (lane == 0) {
+                const uint32_t s = (n_full + i) % RW_STAGES;
+                mbar_expect_tx(bars + 8 * s, R::BYTES);
+                bulk_g2s(ring + s * R::BYTES, p.arena + ((size_t)block * p.n_kv + kvh) * R::BYTES, R::BYTES, bars + 8 * s);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < RW_STAGES; ++i)
+            if (i < n_my) issue(i);
+        // ---- queries: times scale log2 e, two fp16 terms of q 2^(10 - e) with 2^e <= largest of the row < 2^(e + 1); a third nibble's codes come
+        // sixteenfold, so that the dimensions they meet are divided by 16
+        uint32_t qa[HD / 16][4];
+        float qsum[GR], F;
+        {
+            float x[HD / 16][4], most = 0.0f;
+            const TX* src = reinterpret_cast<const TX*>(p.q) + (size_t)(im.tok0 + (row ? j : 0)) * p.ldq + (size_t)(kvh * G + (row ? g : 0)) * HD + 2 * t4;
+            const float mul = row ? p.scale * 1.4426950408889634f : 0.0f;
+#pragma unroll
+            for (int s = 0; s < GR; ++s) qsum[s] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < HD / 16; ++s) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[s][i] = row ? to_f32(src[16 * s + 8 * (i >> 1) + (i & 1)]) * mul : 0.0f;
+                    most = fmaxf(most, fabsf(x[s][i]));
+                    qsum[s / 4] += x[s][i];
+                }
+            }
+#pragma unroll
+            for (int s = 1; s < 4; s <<= 1) {
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+#pragma unroll
+                for (int i = 0; i < GR; ++i) qsum[i] += __shfl_xor_sync(0xffffffffu, qsum[i], s);
+            }
+            const int e = max(-100, min(100, (int)(__float_as_uint(most) >> 23) - 127));
+            const float up = __uint_as_float((uint32_t)(137 - e) << 23);
+            F = __uint_as_float((uint32_t)(141 + e) << 23);
+#pragma unroll
+            for (int s = 0; s < HD / 16; ++s) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float a = x[s][2 * i] * (i ? up * 0.0625f : up), b = x[s][2 * i + 1] * (i ? up * 0.0625f : up);
+                    const uint32_t hi = pack_h2(a, b);
+                    const float2 f = unpack_h2(hi);
+                    qa[s][2 * i] = hi;
+                    qa[s][2 * i + 1] = pack_h2(a - f.x, b - f.y);
+                }
+            }
+        }
+        float o[HD / 8][4], om[GR], m_run = -1e30f, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < GR; ++i) om[i] = 0.0f;
+
+        for (int i = 0; i < n_my; ++i) {
+            const uint32_t s = (n_full + i) % RW_STAGES, at = ring + s * R::BYTES;
+            mbar_wait(bars + 8 * s, ((n_full + i) / RW_STAGES) & 1, p.err);
+            // ---- the page into registers, its stage to the next one
+            uint32_t kw[2][KW], vw[VW], kd[2][2][GR], vd[2][2][GR];      // [half][token of two]
+            if constexpr (HD == 128) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const uint4 x = lds128(at + a * 512 + lane * 16), y = lds128(at + R::V_CODES + a * 512 + lane * 16);
+                    kw[a][0] = x.x, kw[a][1] = x.y, kw[a][2] = x.z, kw[a][3] = x.w;
+                    vw[4 * a] = y.x, vw[4 * a + 1] = y.y, vw[4 * a + 2] = y.z, vw[4 * a + 3] = y.w;
+                    const uint4 u = lds128(at + R::K_SCALES + (8 * a + 2 * t4) * 8), w = lds128(at + R::V_SCALES + (8 * a + 2 * t4) * 8);
+                    kd[a][0][0] = u.x, kd[a][0][1] = u.y, kd[a][1][0] = u.z, kd[a][1][1] = u.w;
+                    vd[a][0][0] = w.x, vd[a][0][1] = w.y, vd[a][1][0] = w.z, vd[a][1][1] = w.w;
+                }
+            } else {
+                const uint4 x = lds128(at + lane * 16), y = lds128(at + R::V_CODES + lane * 16);
+                kw[0][0] = x.x, kw[0][1] = x.y, kw[1][0] = x.z, kw[1][1] = x.w;
+                vw[0] = y.x, vw[1] = y.y, vw[2] = y.z, vw[3] = y.w;
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const uint2 u = lds64(at + R::K_SCALES + (8 * a + 2 * t4) * 4), w = lds64(at + R::V_SCALES + (8 * a + 2 * t4) * 4);
+                    kd[a][0][0] = u.x, kd[a][1][0] = u.y, vd[a][0][0] = w.x, vd[a][1][0] = w.y;
+                }
+            }
+            __syncwarp();
+            if (i + RW_STAGES < n_my) issue(i + RW_STAGES);
+            // ---- scores
+            float sc[2][2], mx = -INFINITY;
+            const int pos = (im.page0 + warp + i * RW) * DC_KV_BLOCK;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                float acc[GR][4];
+#pragma unroll
+                for (int c = 0; c < GR; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < KW; ++c) {
+                    const uint32_t w = kw[a][c], w8 = w >> 8;
+                    mma_f16(acc[c / 2], qa[2 * c], w & 0x000F000Fu, w & 0x00F000F0u);
+                    mma_f16(acc[c / 2], qa[2 * c + 1], w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    float x = 0.0f, y = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < GR; ++c) {
+                        const float2 dm = unpack_h2(kd[a][b][c]);
+                        x = fmaf(dm.x, acc[c][b] + acc[c][2 + b], x);
+                        y = fmaf(dm.y, qsum[c], y);
+                    }
+                    sc[a][b] = fmaf(x, F, y);
+                }
+            }
+            if (pos + DC_KV_BLOCK - 1 > all_see) {      // some row does not see all of the page; what lies there may be anything
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        if (pos + 8 * a + 2 * t4 + b > qpos) {
+                            sc[a][b] = -INFINITY;
+#pragma unroll
+                            for (int c = 0; c < GR; ++c) vd[a][b][c] = 0;
+                        }
+            }
+#pragma unroll
+            for (int a = 0; a < 2; ++a) mx = fmaxf(mx, fmaxf(sc[a][0], sc[a][1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            if (__any_sync(0xffffffffu, mx > m_run)) {
+                const float m_new = fmaxf(m_run, mx), corr = ex2(m_run - m_new);
+                m_run = m_new;
+                l *= corr;
+#pragma unroll
+                for (int c = 0; c < GR; ++c) om[c] *= corr;
+#pragma unroll
+                for (int c = 0; c < HD / 8; ++c) o[c][0] *= corr, o[c][1] *= corr, o[c][2] *= corr, o[c][3] *= corr;
+            }
+            // ---- weights times scales in two terms (the second one 2^11 fold), values
+            uint32_t pa[GR][4];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const float p0 = ex2(sc[a][0] - m_run), p1 = ex2(sc[a][1] - m_run);
+                l += p0 + p1;
+#pragma unroll
+                for (int c = 0; c < GR; ++c) {
+                    const float2 d0 = unpack_h2(vd[a][0][c]), d1 = unpack_h2(vd[a][1][c]);
+                    om[c] = fmaf(p0, d0.y, om[c]);
+                    om[c] = fmaf(p1, d1.y, om[c]);
+                    const float w0 = p0 * d0.x, w1 = p1 * d1.x;
+                    const uint32_t hi = pack_h2(w0, w1);
+                    const float2 f = unpack_h2(hi);
+                    pa[c][2 * a] = hi;
+                    pa[c][2 * a + 1] = pack_h2((w0 - f.x) * 2048.0f, (w1 - f.y) * 2048.0f);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < VW; ++c) {
+                const uint32_t w = vw[c], w8 = w >> 8;
+                mma_f16(o[2 * c], pa[c / 4], w & 0x000F000Fu, w8 & 0x000F000Fu);
+                mma_f16(o[2 * c + 1], pa[c / 4], w & 0x00F000F0u, w8 & 0x00F000F0u);
+            }
+        }
+        n_full += max(0, n_my);
+        // ---- the warps' parts
+#pragma unroll
+        for (int s = 1; s < 4; s <<= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, s);
+#pragma unroll
+            for (int c = 0; c < GR; ++c) om[c] += __shfl_xor_sync(0xffffffffu, om[c], s);
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+            const float f = c & 1 ? 1048576.0f : 16777216.0f;
+            float2 x;
+            x.x = fmaf(fmaf(o[c][2], 1.0f / 2048.0f, o[c][0]), f, om[c / 8]);
+            x.y = fmaf(fmaf(o[c][3], 1.0f / 2048.0f, o[c][1]), f, om[c / 8]);
+            *reinterpret_cast<float2*>(part + (warp * 8 + h) * HD + 8 * c + 2 * t4) = x;
+        }
+        if (t4 == 0) part_ml[2 * (warp * 8 + h)] = m_run, part_ml[2 * (warp * 8 + h) + 1] = l;
+        if (!waited) pdl_wait(), waited = true;      // (ahead of the first store)
+        __syncthreads();
+        const bool alone = im.n_splits == 1;
+        float* ws = reinterpret_cast<float*>(const_cast<int32_t*>(words) + hd->ws) + ((size_t)im.ws * p.n_kv + (size_t)im.n_splits * kvh) * (8 * (HD + 2));
+        TX* out = reinterpret_cast<TX*>(p.out);
+        for (int x = threadIdx.x; x < 8 * HD; x += RW * 32) {
+            const int rr = x / HD, d = x - rr * HD;
+            float M = -1e30f, L = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < RW; ++w) M = fmaxf(M, part_ml[2 * (w * 8 + rr)]);
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                const float f = ex2(part_ml[2 * (w * 8 + rr)] - M);
+                L = fmaf(part_ml[2 * (w * 8 + rr) + 1], f, L);
+                v = fmaf(part[(w * 8 + rr) * HD + d], f, v);
+            }
+            if (alone) {
+                const int ro = im.tile * 8 + rr, jo = ro / G, go = ro - jo * G;
+                if (jo < im.count) put(out + (size_t)(im.tok0 + jo) * p.ldo + (size_t)(kvh * G + go) * HD + d, __fdividef(v, L));
+            } else {
+                float* to = ws + (size_t)im.split * (8 * (HD + 2));
+                to[x] = v;
+                if (d == 0) to[8 * HD + 2 * rr] = M, to[8 * HD + 2 * rr + 1] = L;
+            }
+        }
+        if (!alone) {
+            int* ticket = const_cast<int*>(words) + hd->tickets + im.ticket * p.n_kv + kvh;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                s_last = atomicAdd(ticket, 1) == im.n_splits - 1;
+                if (s_last) *ticket = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (s_last) {
+                for (int x = threadIdx.x; x < 8 * HD; x += RW * 32) {
+                    const int rr = x / HD, d = x - rr * HD, ro = im.tile * 8 + rr, jo = ro / G, go = ro - jo * G;
+                    if (jo >= im.count) continue;
+                    float M = -1e30f, L = 0.0f, v = 0.0f;
+                    for (int s = 0; s < im.n_splits; ++s) M = fmaxf(M, __ldcg(ws + (size_t)s * (8 * (HD + 2)) + 8 * HD + 2 * rr));
+                    for (int s = 0; s < im.n_splits; ++s) {
+                        const float* from = ws + (size_t)s * (8 * (HD + 2));
+                        const float f = ex2(__ldcg(from + 8 * HD + 2 * rr) - M);
+                        L = fmaf(__ldcg(from + 8 * HD + 2 * rr + 1), f, L);
+                        v = fmaf(__ldcg(from + x), f, v);
+                    }
+                    put(out + (size_t)(im.tok0 + jo) * p.ldo + (size_t)(kvh * G + go) * HD + d, __fdividef(v, L));
+                }
+            }
+        }
+        __syncthreads();      // the parts are free for the next item
+    }
+    if (!waited) pdl_wait();
+}
+
+template <int HD, typename TX>
+int launch_rows(dc_ctx* ctx, const dc_q4_call& c) {
+    const dc_q4& z = *c.kv->q4;
+    DC_TRY(dc_kernel_setup(ctx, (const void*)k_q4_rows<HD, TX>, (int)rows_smem<HD>(), "k_q4_rows"));
+    RowsParams p = {z.plan, c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.after_write ? 1 : 0, ctx->d_err};
+    return dc_launch(ctx, "k_q4_rows", k_q4_rows<HD, TX>, dim3(z.n_items, z.kv), dim3(RW * 32), rows_smem<HD>(), p);
+}
+
+template <int HD, typename TX>
+int launch_write(dc_ctx* ctx, const WriteParams& p, int units) {
+    return dc_launch(ctx, "k_q4_write", k_q4_write<HD, TX>, dim3(std::min((units + 3) / 4, ctx->num_sms * 8)), dim3(128), 0, p);
+}
+
+}  // namespace
+
+int dc_launch_q4_rows(dc_ctx* ctx, const dc_q4_call& c) {
+    const dc_q4& z = *c.kv->q4;
+    if (z.n_items == 0) return DC_B200_OK;
+    if (z.dim == 128) return z.type == DC_TYPE_F32 ? launch_rows<128, float>(ctx, c) : launch_rows<128, __nv_bfloat16>(ctx, c);
+    return z.type == DC_TYPE_F32 ? launch_rows<64, float>(ctx, c) : launch_rows<64, __nv_bfloat16>(ctx, c);
+}
+
+// ---------------------------------------------------------------- plans
+void dc_q4_release(dc_kv_cache* kv) {
+    dc_q4* z = kv->q4;
+    if (!z) return;
+    if (z->plan) cudaFree(z->plan);
+    for (uint8_t* p : z->retired) cudaFree(p);
+    if (z->stage) cudaFreeHost(z->stage);
+    if (z->uploaded) cudaEventDestroy(z->uploaded);
+    delete z;
+    kv->q4 = nullptr;
+}
+
+namespace {
+
+bool capturing(dc_ctx* ctx) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(ctx->stream, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+
+// Blocks that the entries need beside the ones they hold: new ones, and copies of the ones they are about to write that someone else holds too.
+int blocks_needed(const dc_kv_cache* kv, const std::vector<dc_q4_entry>& es) {
+    std::vector<std::pair<int, int>> given;      // (block, references already given up)
+    int n = 0;
+    for (const dc_q4_entry& e : es) {
+        const dc_kv_seq& s = kv->seqs[e.seq];
+        const int need = (e.pos0 + e.count + DC_KV_BLOCK - 1) / DC_KV_BLOCK, have = (int)s.blocks.size();
+        for (int b = e.pos0 / DC_KV_BLOCK; b < need && b < have; ++b) {
+            if (kv->ref[s.blocks[b]] <= 1) continue;
+            auto it = std::find_if(given.begin(), given.end(), [&](const std::pair<int, int>& x) { return x.first == s.blocks[b]; });
+            if (it == given.end()) it = given.insert(given.end(), {s.blocks[b], 0});
+            if (kv->ref[s.blocks[b]] - it->second <= 1) continue;
+            ++it->second;
+            ++n;
+        }
+        n += std::max(0, need - have);
+    }
+    return n;
+}
+
+int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, int T) {
+    dc_q4& z = *kv->q4;
+    std::vector<int32_t> tokens(2 * (size_t)T);
+    std::vector<dc_q4_item> items;
+    std::vector<dc_q4_tile> tiles;
+    for (const dc_q4_entry& e : es)
+        for (int i = 0; i < e.count; ++i) tokens[2 * (size_t)(e.tok0 + i)] = e.seq, tokens[2 * (size_t)(e.tok0 + i) + 1] = e.pos0 + i;
+    int n_tickets, n_ws;
+    dc_q4_items(es, z.heads / z.kv, z.kv, ctx->num_sms, &items, &n_tickets, &n_ws);
+    // ---- one allocation: header, arrays, tickets (zero, and left so by every call), partial results
+    auto up = [](size_t n) { return (n + 63) / 64 * 64; };
+    dc_q4_head hd = {};
+    hd.T = T, hd.n_items = (int)items.size(), hd.n_tiles = (int)tiles.size();
+    size_t at = up(sizeof(hd));
+    hd.tokens = (int32_t)(at / 4), at += up(tokens.size() * 4);
+    hd.items = (int32_t)(at / 4), at += up(items.size() * sizeof(dc_q4_item));
+    hd.tiles = (int32_t)(at / 4), at += up(tiles.size() * sizeof(dc_q4_tile));
+    const size_t copied = at;
+    hd.tickets = (int32_t)(at / 4), at += up((size_t)n_tickets * z.kv * 4);
+    hd.ws = (int32_t)(at / 4), at += up((size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4);
+    if (at > ((size_t)1 << 33) - 64) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: the step's plan takes %zu bytes", at);
+    if (at > z.plan_bytes) {
+        uint8_t* fresh = nullptr;
+        const size_t want = at + at / 2 + (1 << 16);
+        DC_TRY(dc_check_cuda(ctx, cudaMalloc(&fresh, want), "kv_batch: plan"));
+        if (z.plan) {      // a captured call that still names it finds a step without tokens
+            z.retired.push_back(z.plan);
+            DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.plan, 0, sizeof(hd), ctx->stream), "kv_batch: old plan"));
+        }
+        z.plan = fresh, z.plan_bytes = want;
+    }
+    if (!z.uploaded) DC_TRY(dc_check_cuda(ctx, cudaEventCreateWithFlags(&z.uploaded, cudaEventDisableTiming), "kv_batch: event"));
+    else DC_TRY(dc_check_cuda(ctx, cudaEventSynchronize(z.uploaded), "kv_batch: staging"));
+    if (copied > z.stage_bytes) {
+        if (z.stage) cudaFreeHost(z.stage);
+        z.stage = nullptr, z.stage_bytes = 0;
+        DC_TRY(dc_check_cuda(ctx, cudaMallocHost(&z.stage, copied * 2), "kv_batch: staging"));
+        z.stage_bytes = copied * 2;
+    }
+    memcpy(z.stage, &hd, sizeof(hd));
+    memcpy(z.stage + 4 * (size_t)hd.tokens, tokens.data(), tokens.size() * 4);
+    memcpy(z.stage + 4 * (size_t)hd.items, items.data(), items.size() * sizeof(dc_q4_item));
+    memcpy(z.stage + 4 * (size_t)hd.tiles, tiles.data(), tiles.size() * sizeof(dc_q4_tile));
+    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.plan, z.stage, copied, cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
+    DC_TRY(dc_check_cuda(ctx, cudaEventRecord(z.uploaded, ctx->stream), "kv_batch: plan"));
+    if (n_tickets) DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.plan + 4 * (size_t)hd.tickets, 0, (size_t)n_tickets * z.kv * 4, ctx->stream), "kv_batch: tickets"));
+    z.T = T, z.n_items = hd.n_items, z.n_tiles = hd.n_tiles;
+    return DC_B200_OK;
+}
+
+int check_call(dc_ctx* ctx, const dc_kv_cache* kv, int layer, const char* name) {
+    if (!ctx || !kv) return DC_B200_INVALID_ARGUMENT;
+    if (!kv->q4) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "%s: not a cache in 4 bits", name);
+    if (kv->ctx != ctx) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "%s: the cache belongs to another context", name);
+    if (layer < 0 || layer >= kv->q4->n_layer) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "%s: layer %d of %d", name, layer, kv->q4->n_layer);
+    if (!kv->q4->planned) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "%s: no batch (dc_b200_kv_batch)", name);
+    if (kv->q4->edits != kv->edits)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "%s: a sequence was freed, forked, reserved or looked up in the prefix cache since dc_b200_kv_batch", name);
+    return DC_B200_OK;
+}
+
+int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held) {
+    const dc_q4& z = *kv->q4;
+    const WriteParams p = {z.plan, k, v, ldkv, z.kv, kv->max_blocks_per_seq, kv->d_tables, kv->planes[layer].arena, k_held, v_held};
+    const int units = (int)std::min<long long>((long long)z.T * z.kv * 2, 1 << 30);
+    if (z.dim == 128) return z.type == DC_TYPE_F32 ? launch_write<128, float>(ctx, p, units) : launch_write<128, __nv_bfloat16>(ctx, p, units);
+    return z.type == DC_TYPE_F32 ? launch_write<64, float>(ctx, p, units) : launch_write<64, __nv_bfloat16>(ctx, p, units);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_b200_kv_create_q4(dc_ctx* ctx, int n_layer, int n_head, int n_kv_head, int head_dim, int row_type, int max_blocks, int max_seqs,
+                         int max_blocks_per_seq, dc_kv_cache** out) {
+    if (!ctx || !out) return DC_B200_INVALID_ARGUMENT;
+    *out = nullptr;
+    if (n_layer < 1 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || n_kv_head > 65535 || max_blocks < 1 || max_seqs < 1 || max_blocks_per_seq < 1)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_create_q4: bad shape (%d heads, %d key heads)", n_head, n_kv_head);
+    if (head_dim != 64 && head_dim != 128) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_create_q4: head size %d (64 and 128 are supported)", head_dim);
+    if (row_type != DC_TYPE_F32 && row_type != DC_TYPE_BF16) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_create_q4: row type %d (F32 and BF16 are supported)", row_type);
+    if (n_head > (1 << 20) || (long long)max_blocks_per_seq * DC_KV_BLOCK > (1 << 30) || (long long)max_seqs * max_blocks_per_seq > (1LL << 31) - 1)
+        return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_create_q4: %d sequences of %d pages, %d heads", max_seqs, max_blocks_per_seq, n_head);
+    cudaSetDevice(ctx->device);
+    dc_kv_cache* kv = new dc_kv_cache();
+    kv->q4 = new dc_q4();
+    kv->q4->n_layer = n_layer, kv->q4->heads = n_head, kv->q4->kv = n_kv_head, kv->q4->dim = head_dim, kv->q4->type = row_type;
+    const size_t row = (size_t)n_kv_head * 18 * head_dim / DC_KV_BLOCK;
+    const int st = dc_kv_init_planes(ctx, kv, std::vector<size_t>(n_layer, row), 0, max_blocks, max_seqs, max_blocks_per_seq);
+    if (st != DC_B200_OK) {
+        dc_kv_release(kv);
+        delete kv;
+        return st;
+    }
+    *out = kv;
+    return DC_B200_OK;
+}
+
+int dc_b200_kv_batch(dc_kv_cache* kv, int n_entries, const int32_t* seqs, const int32_t* pos0, const int32_t* counts) {
+    if (!kv) return DC_B200_INVALID_ARGUMENT;
+    dc_ctx* ctx = kv->ctx;
+    if (!kv->q4) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: not a cache in 4 bits");
+    if (n_entries < 0 || (n_entries && (!seqs || !pos0 || !counts))) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: bad argument (%d entries)", n_entries);
+    cudaSetDevice(ctx->device);
+    if (capturing(ctx)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: not within a stream capture");
+    std::vector<dc_q4_entry> es;
+    std::vector<char> seen(kv->max_seqs, 0);
+    long long T = 0;
+    const int G = kv->q4->heads / kv->q4->kv;
+    for (int i = 0; i < n_entries; ++i) {
+        const int s = seqs[i];
+        if (s < 0 || s >= kv->max_seqs || !kv->seqs[s].used) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d is not allocated", s);
+        if (seen[s]) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d is named twice", s);
+        seen[s] = 1;
+        if (counts[i] < 0 || pos0[i] < 0 || pos0[i] > kv->seqs[s].len)
+            return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d holds %d tokens, asked are %d from position %d on", s, kv->seqs[s].len, counts[i], pos0[i]);
+        if ((long long)pos0[i] + counts[i] > (long long)kv->max_blocks_per_seq * DC_KV_BLOCK)
+            return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: sequence %d needs %lld positions, its table holds %d pages", s, (long long)pos0[i] + counts[i], kv->max_blocks_per_seq);
+        if (counts[i]) es.push_back({s, pos0[i], counts[i], (int)T});
+        T += counts[i];
+        if (T * G > (1 << 24)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: too many new tokens at once");
+    }
+    const int need = blocks_needed(kv, es), there = dc_kv_available_blocks(kv);
+    if (need > there) return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: out of blocks (%d free, %d needed)", there, need);
+    kv->q4->planned = false;
+    for (const dc_q4_entry& e : es) {
+        kv->seqs[e.seq].len = e.pos0;      // rows from there on are written anew (what others share is copied first)
+        DC_TRY(dc_kv_seq_reserve(kv, e.seq, e.pos0 + e.count));
+        kv->seqs[e.seq].len = e.pos0 + e.count;
+    }
+    DC_TRY(make_plan(ctx, kv, es, (int)T));
+    kv->q4->edits = kv->edits;
+    kv->q4->planned = true;
+    return DC_B200_OK;
+}
+
+int dc_b200_kv_q4_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k_dev, const void* v_dev, int ld_kv, float* k_held_dev, float* v_held_dev) {
+    DC_TRY(check_call(ctx, kv, layer, "kv_q4_write_dev"));
+    const dc_q4& z = *kv->q4;
+    if (ld_kv == 0) ld_kv = z.kv * z.dim;
+    if (z.T == 0) return DC_B200_OK;
+    if (!k_dev || !v_dev || ld_kv < z.kv * z.dim) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_q4_write_dev: bad argument (row stride %d)", ld_kv);
+    cudaSetDevice(ctx->device);
+    return write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev);
+}
+
+int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_dev, int ld_q, const void* k_dev, const void* v_dev, int ld_kv, float scale,
+                              void* out_dev, int ld_out, float* k_held_dev, float* v_held_dev) {
+    DC_TRY(check_call(ctx, kv, layer, "flash_attn_q4_dev"));
+    const dc_q4& z = *kv->q4;
+    if (ld_q == 0) ld_q = z.heads * z.dim;
+    if (ld_kv == 0) ld_kv = z.kv * z.dim;
+    if (ld_out == 0) ld_out = z.heads * z.dim;
+    if (z.T == 0) return DC_B200_OK;
+    if (!q_dev || !out_dev || (!k_dev != !v_dev) || ld_q < z.heads * z.dim || ld_out < z.heads * z.dim || ld_kv < z.kv * z.dim || (!k_dev && (k_held_dev || v_held_dev)))
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: bad argument (row strides %d, %d, %d)", ld_q, ld_kv, ld_out);
+    if (!isfinite(scale)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: scale is not finite");
+    cudaSetDevice(ctx->device);
+    if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev));
+    const dc_q4_call c = {kv, kv->planes[layer].arena, q_dev, ld_q, ld_out, scale, out_dev, k_dev != nullptr};
+    return dc_launch_q4_rows(ctx, c);
+}
+
+int dc_b200_flash_attn_q4(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_host, const void* k_host, const void* v_host, float scale, void* out_host) {
+    if (!ctx) return DC_B200_INVALID_ARGUMENT;
+    const bool known = kv && kv->q4 && kv->q4->planned;
+    const size_t es = known && kv->q4->type == DC_TYPE_F32 ? 4 : 2, q_bytes = known ? (size_t)kv->q4->T * kv->q4->heads * kv->q4->dim * es : 0;
+    auto fail_closed = [&](int st) {
+        if (out_host && q_bytes) memset(out_host, 0, q_bytes);
+        return st;
+    };
+    int st = check_call(ctx, kv, layer, "flash_attn_q4");
+    if (st != DC_B200_OK) return fail_closed(st);
+    if (kv->q4->T == 0) return DC_B200_OK;
+    if (!q_host || !out_host || (!k_host != !v_host)) return fail_closed(dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4: bad argument"));
+    cudaSetDevice(ctx->device);
+    const size_t kv_bytes = (size_t)kv->q4->T * kv->q4->kv * kv->q4->dim * es, pad_q = (q_bytes + 255) / 256 * 256, pad_kv = (kv_bytes + 255) / 256 * 256;
+    uint8_t* s = dc_scratch(ctx, 2 * pad_q + 2 * pad_kv);
+    if (!s) return fail_closed(DC_B200_OUT_OF_MEMORY);
+    uint8_t *q = s, *o = s + pad_q, *k = o + pad_q, *v = k + pad_kv;
+    auto copy = [&](void* to, const void* from, size_t n, cudaMemcpyKind how) { return dc_check_cuda(ctx, cudaMemcpyAsync(to, from, n, how, ctx->stream), "flash_attn_q4"); };
+    st = copy(q, q_host, q_bytes, cudaMemcpyHostToDevice);
+    if (st == DC_B200_OK && k_host) st = copy(k, k_host, kv_bytes, cudaMemcpyHostToDevice);
+    if (st == DC_B200_OK && k_host) st = copy(v, v_host, kv_bytes, cudaMemcpyHostToDevice);
+    if (st == DC_B200_OK) st = dc_b200_flash_attn_q4_dev(ctx, kv, layer, q, 0, k_host ? k : nullptr, k_host ? v : nullptr, 0, scale, o, 0, nullptr, nullptr);
+    if (st == DC_B200_OK) st = copy(out_host, o, q_bytes, cudaMemcpyDeviceToHost);
+    if (st == DC_B200_OK) st = dc_b200_synchronize(ctx);
+    return st == DC_B200_OK ? st : fail_closed(st);
+}
+
+int dc_b200_kv_q4_read_block(dc_kv_cache* kv, int layer, int block, float* k_host, float* v_host) {
+    if (!kv || !kv->q4 || layer < 0 || layer >= kv->q4->n_layer || block < 0 || block >= kv->max_blocks) return DC_B200_INVALID_ARGUMENT;
+    cudaSetDevice(kv->ctx->device);
+    const int n_kv = kv->q4->kv, HD = kv->q4->dim, GR = HD / 64, rec = 18 * HD;
+    std::vector<uint8_t> page((size_t)n_kv * rec);
+    cudaError_t e = cudaStreamSynchronize(kv->ctx->stream);
+    if (e == cudaSuccess) e = cudaMemcpy(page.data(), kv->planes[layer].arena + page.size() * block, page.size(), cudaMemcpyDeviceToHost);
+    DC_TRY(dc_check_cuda(kv->ctx, e, "kv_q4_read_block"));
+    auto half = [&](const uint8_t* at) {
+        uint16_t b;
+        memcpy(&b, at, 2);
+        return __half2float(__ushort_as_half(b));
+    };
+    for (int tok = 0; tok < DC_KV_BLOCK; ++tok)
+        for (int h = 0; h < n_kv; ++h)
+            for (int d = 0; d < HD; ++d) {
+                const uint8_t* r = page.data() + (size_t)h * rec;
+                const int i = d >> 5, t = (d & 7) >> 1, nib = ((d >> 3) & 3) + 4 * (d & 1);
+                uint32_t w;
+                memcpy(&w, r + (HD == 128 ? dc_q4_rec<128>::k_word(tok, t, i) : dc_q4_rec<64>::k_word(tok, t, i)), 4);
+                const uint8_t b = r[HD == 128 ? dc_q4_rec<128>::v_byte(tok, d & 7, d >> 4) : dc_q4_rec<64>::v_byte(tok, d & 7, d >> 4)];
+                const uint8_t *ks = r + 8 * HD + (tok * GR + d / 64) * 4, *vs = r + 17 * HD + (tok * GR + d / 64) * 4;
+                const size_t to = ((size_t)tok * n_kv + h) * HD + d;
+                if (k_host) k_host[to] = fmaf(half(ks), (float)((w >> (4 * nib)) & 15), half(ks + 2));
+                if (v_host) v_host[to] = fmaf(half(vs), (float)(d & 8 ? b >> 4 : b & 15), half(vs + 2));
+            }
+    return DC_B200_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,98 @@
+// A cache of keys and values in 4 bits: where everything lies, and the plan of a step.  Shared by attn_q4.cu and attn_q4_prompt.cu.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "dc_kv.h"
+
+// A page of a key head is one record of 18 HD bytes, so that one bulk copy brings it:
+//   key codes     8 HD   words of eight codes of one token, in the order in which lanes of mma.m16n8k16 take a second operand of 16 dimensions x 8 tokens
+//   key scales      HD   [16 tokens][HD / 64] pairs (scale, least value) of fp16
+//   value codes   8 HD   the same for 16 tokens x 8 dimensions; a byte is two dimensions (d, d + 8) of one token
+//   value scales    HD
+// Every byte belongs to one token: tokens are written one by one, by different warps, without reading what is there.
+template <int HD>
+struct dc_q4_rec {
+    static constexpr int GROUPS = HD / 64, K_SCALES = 8 * HD, V_CODES = 9 * HD, V_SCALES = 17 * HD, BYTES = 18 * HD;
+    // word i (dimensions 32 i ..) of lane t's part of a token's key: nibble q + 4 o holds dimension 32 i + 8 q + 2 t + o
+    static constexpr int __host__ __device__ k_word(int tok, int t, int i) {
+        return HD == 128 ? (tok >> 3) * 512 + ((tok & 7) * 4 + t) * 16 + 4 * i : ((tok & 7) * 4 + t) * 16 + (tok >> 3) * 8 + 4 * i;
+    }
+    // byte of dimensions 16 i + d8 (low nibble) and 16 i + 8 + d8 (high nibble) of a token's value
+    static constexpr int __host__ __device__ v_byte(int tok, int d8, int i) {
+        const int lane = d8 * 4 + ((tok & 7) >> 1);
+        return V_CODES + (HD == 128 ? (i >> 2) * 512 + lane * 16 + (i & 3) * 4 : lane * 16 + i * 4) + (tok >> 3) + 2 * (tok & 1);
+    }
+};
+
+// The plan of a step in device memory, one allocation: this header, then the arrays that it names (offsets in words).
+// Kernels read the header's counts and loop, so that a captured call takes later plans too.
+struct dc_q4_head {
+    int32_t T, n_items, n_tiles, tokens, items, tiles, tickets, ws;
+    int32_t pad[8];
+};
+// One CTA's work in k_q4_rows: pages page0 .. page1 - 1 for one tile of eight rows (row r: new token r / G of the entry, query head r % G of the key head).
+struct dc_q4_item {
+    int32_t seq, pos0, tok0, count, tile, page0, page1;
+    int32_t split, n_splits, ws;      // of the tile; partial results at ws + split
+    int32_t ticket, pad;
+};
+// One CTA's work in the prompt kernel: `rows` rows from `row0` of the entry on.
+struct dc_q4_tile {
+    int32_t seq, pos0, tok0, count, row0, pad[3];
+};
+
+// `count` new tokens of a sequence from position pos0 on; the step's tokens tok0 ..
+struct dc_q4_entry {
+    int32_t seq, pos0, count, tok0;
+};
+constexpr int DC_Q4_WARPS = 4;      // of a CTA of k_q4_rows
+
+// The items of all tiles of the entries; *n_ws: partial results, *n_tickets: tiles that more than one CTA works on.
+inline void dc_q4_items(const std::vector<dc_q4_entry>& es, int G, int n_kv, int num_sms, std::vector<dc_q4_item>* items, int* n_tickets, int* n_ws) {
+    auto tiles_of = [&](const dc_q4_entry& e) { return (int)(((long long)e.count * G + 7) / 8); };
+    auto pages_of = [&](const dc_q4_entry& e, int tile) { return (e.pos0 + std::min(e.count - 1, (tile * 8 + 7) / G)) / 16 + 1; };
+    long long work = 0;
+    for (const dc_q4_entry& e : es)
+        for (int t = 0; t < tiles_of(e); ++t) work += pages_of(e, t);
+    // pages of an item: four rounds of three CTAs an SM where there is that much, two pages a warp at least
+    const long long slots = (long long)num_sms * 3 * 4;
+    const int per = (int)std::max<long long>(2 * DC_Q4_WARPS, (work * n_kv + slots - 1) / slots);
+    *n_tickets = *n_ws = 0;
+    for (const dc_q4_entry& e : es)
+        for (int t = 0; t < tiles_of(e); ++t) {
+            const int pages = pages_of(e, t), n = (pages + per - 1) / per;
+            for (int s = 0; s < n; ++s)
+                items->push_back({e.seq, e.pos0, e.tok0, e.count, t, s * per, std::min(pages, (s + 1) * per), s, n, n > 1 ? *n_ws : 0, n > 1 ? *n_tickets : 0, 0});
+            if (n > 1) ++*n_tickets, *n_ws += n;
+        }
+}
+
+struct dc_q4 {
+    int n_layer = 0, heads = 0, kv = 0, dim = 0, type = 0;
+    // the newest plan: host copies of what launches need, and the block manager's state that it was made for
+    bool planned = false;
+    uint64_t edits = 0;
+    int T = 0, n_items = 0, n_tiles = 0;
+    uint8_t* plan = nullptr;
+    size_t plan_bytes = 0;
+    std::vector<uint8_t*> retired;      // outgrown plans, emptied; captured calls may still read them
+    uint8_t* stage = nullptr;           // pinned copy of the plan being uploaded
+    size_t stage_bytes = 0;
+    cudaEvent_t uploaded = nullptr;
+};
+
+struct dc_q4_call {
+    const dc_kv_cache* kv;
+    const uint8_t* arena;      // one layer
+    const void* q;
+    int ldq, ldo;
+    float scale;
+    void* out;
+    bool after_write;          // the kernel before it in the stream is this call's k_q4_write
+};
+int dc_launch_q4_rows(dc_ctx* ctx, const dc_q4_call& c);
+int dc_launch_q4_prompt(dc_ctx* ctx, const dc_q4_call& c);

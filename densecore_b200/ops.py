@@ -12,7 +12,21 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .blocks import BLOCK_BYTES, GGML_TYPE_Q4_K, GGML_TYPE_Q6_K, Q8K_BYTES, QK_K, row_bytes
+from .blocks import (BLOCK_BYTES, GGML_TYPE_BF16, GGML_TYPE_F16, GGML_TYPE_F32, GGML_TYPE_Q4_K, GGML_TYPE_Q6_K, Q8K_BYTES, QK_K,
+                     row_bytes)
+
+ROW_TYPES = {"f32": GGML_TYPE_F32, "bf16": GGML_TYPE_BF16, "f16": GGML_TYPE_F16}
+_HOST_ROWS = {"f32": np.float32, "bf16": np.uint16, "f16": np.float16}      # bf16 rows on the host: their bits
+
+
+def _row_type(dtype: str) -> int:
+    if dtype not in ROW_TYPES:
+        raise ValueError(f"row type {dtype!r} (one of {', '.join(ROW_TYPES)})")
+    return ROW_TYPES[dtype]
+
+
+def _dev(p: int):
+    return C.c_void_p(p) if p else None
 
 
 def _vp(a: np.ndarray | None):
@@ -205,6 +219,11 @@ class Context:
                  max_blocks_per_seq: int) -> "KVCache":
         return KVCache(self, n_layer, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq)
 
+    def kv_cache_q4(self, n_layer: int, n_head: int, n_kv_head: int, head_dim: int, max_blocks: int, max_seqs: int, max_blocks_per_seq: int,
+                    dtype: str = "f32") -> "KVCacheQ4":
+        """Cache in 4 bits for layers of n_head query heads; dtype: rows of queries, keys, values and results ("f32", "bf16")."""
+        return KVCacheQ4(self, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, dtype)
+
 
 class KVCache:
     """Paged fp16 KV cache with 16-token blocks (dc_b200_kv_*)."""
@@ -272,3 +291,68 @@ class KVCache:
         self.ctx._check(_lib.lib().dc_b200_flash_attn_prefill(self.ctx.handle, self.handle, layer, _vp(q), _vp(k), _vp(v), seq,
                                                               pos0, n, n_head, scale, _vp(out)))
         return out
+
+
+class KVCacheQ4(KVCache):
+    """Paged KV cache in 4 bits (dc_b200_kv_create_q4); sequences, forks and block tables as in KVCache."""
+
+    def __init__(self, ctx: Context, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, dtype="f32"):
+        self.handle = None
+        self.ctx, self.n_layer, self.n_head, self.n_kv, self.head_dim, self.dtype = ctx, n_layer, n_head, n_kv_head, head_dim, dtype
+        self.n_tokens = 0
+        h = C.c_void_p()
+        ctx._check(_lib.lib().dc_b200_kv_create_q4(ctx.handle, n_layer, n_head, n_kv_head, head_dim, _row_type(dtype), max_blocks, max_seqs,
+                                                   max_blocks_per_seq, C.byref(h)))
+        self.handle = h
+
+    def __del__(self):
+        try:
+            if self.ctx.handle:
+                self.close()
+        except Exception:
+            pass
+
+    def seq_fork(self, seq: int) -> int:
+        """New sequence sharing seq's blocks (copy-on-write)."""
+        s = C.c_int(-1)
+        self.ctx._check(_lib.lib().dc_b200_kv_seq_fork(self.handle, seq, C.byref(s)))
+        return s.value
+
+    def batch(self, seqs, pos0, counts):
+        """Begins a step: counts[e] new tokens of seqs[e] from position pos0[e] on."""
+        a = [np.ascontiguousarray(x, dtype=np.int32).reshape(-1) for x in (seqs, pos0, counts)]
+        if not a[0].size == a[1].size == a[2].size:
+            raise ValueError("seqs, pos0 and counts differ in length")
+        self.ctx._check(_lib.lib().dc_b200_kv_batch(self.handle, a[0].size, *(_vp(x) for x in a)))
+        self.n_tokens = int(a[2].sum())
+
+    def write_dev(self, layer: int, k: int, v: int, ld: int = 0, k_held: int = 0, v_held: int = 0):
+        """Writes the step's rows (device addresses) into one layer."""
+        self.ctx._check(_lib.lib().dc_b200_kv_q4_write_dev(self.ctx.handle, self.handle, layer, _dev(k), _dev(v), ld, _dev(k_held), _dev(v_held)))
+
+    def attend_dev(self, layer: int, q: int, k: int, v: int, scale: float, out: int, ld_q: int = 0, ld_kv: int = 0, ld_out: int = 0, k_held: int = 0,
+                   v_held: int = 0):
+        """Writes the step's rows (k = v = 0: they stand there already), then attends; device addresses, enqueue only."""
+        self.ctx._check(_lib.lib().dc_b200_flash_attn_q4_dev(self.ctx.handle, self.handle, layer, _dev(q), ld_q, _dev(k), _dev(v), ld_kv, scale, _dev(out),
+                                                             ld_out, _dev(k_held), _dev(v_held)))
+
+    def attend(self, layer: int, q, k, v, scale: float) -> np.ndarray:
+        """The same on host arrays: q [T, n_head, hd], k and v [T, n_kv, hd] (both None: written already); bf16 rows as their bits (uint16)."""
+        t = _HOST_ROWS[self.dtype]
+        q = np.ascontiguousarray(q, dtype=t)
+        if q.shape != (self.n_tokens, self.n_head, self.head_dim):
+            raise ValueError(f"q has shape {q.shape}, the step has {self.n_tokens} tokens")
+        k, v = (None if x is None else np.ascontiguousarray(x, dtype=t) for x in (k, v))
+        for x in (k, v):
+            if x is not None and x.shape != (self.n_tokens, self.n_kv, self.head_dim):
+                raise ValueError(f"keys or values have shape {x.shape}, the step has {self.n_tokens} tokens")
+        out = np.empty_like(q)
+        self.ctx._check(_lib.lib().dc_b200_flash_attn_q4(self.ctx.handle, self.handle, layer, _vp(q), _vp(k), _vp(v), scale, _vp(out)))
+        return out
+
+    def read_block(self, layer: int, block: int):
+        """The values that a block stands for: K and V, [16, n_kv, hd] f32."""
+        k = np.zeros((16, self.n_kv, self.head_dim), dtype=np.float32)
+        v = np.zeros_like(k)
+        self.ctx._check(_lib.lib().dc_b200_kv_q4_read_block(self.handle, layer, block, _vp(k), _vp(v)))
+        return k, v

@@ -47,7 +47,7 @@ enum {
 };
 
 /* ggml type ids of the tensors this library accepts */
-enum { DC_GGML_TYPE_F32 = 0, DC_GGML_TYPE_F16 = 1, DC_GGML_TYPE_Q4_K = 12, DC_GGML_TYPE_Q6_K = 14 };
+enum { DC_GGML_TYPE_F32 = 0, DC_GGML_TYPE_F16 = 1, DC_GGML_TYPE_Q4_K = 12, DC_GGML_TYPE_Q6_K = 14, DC_GGML_TYPE_BF16 = 30 };
 
 typedef struct dc_ctx dc_ctx;
 typedef struct dc_weight dc_weight;
@@ -220,6 +220,42 @@ DC_B200_API int dc_b200_flash_attn_prefill(dc_ctx* ctx, dc_kv_cache* kv, int lay
                                            int n_head, float scale, float* out_host);
 /* Raw fp16 contents of one block of one layer (K then V planes), for tests. */
 DC_B200_API int dc_b200_kv_read_block(dc_kv_cache* kv, int layer, int block, void* k_host, void* v_host);
+
+/* ---- paged KV cache in 4 bits + attention over it ---------------------------- */
+/* A cache whose rows are held in 4 bits, for serving many requests or long ones (no counterpart in DenseCore's
+ * decode path).  A row of a key head is cut into groups of 64 values; a group has m = fp16(least value),
+ * d = fp16((largest - least) * fp32(1/15)), codes q = rint((x - m) / d) within 0..15 in fp32 arithmetic (0 where d
+ * is 0), and stands for fp32(d q + m).  A group with a value that is not finite or beyond +-65504 reads back as NaN.
+ * Head sizes 64 (36 bytes a row) and 128 (72).  n_head query heads share n_kv_head key heads evenly.  row_type: type
+ * of queries, new rows and results, DC_GGML_TYPE_F32 or DC_GGML_TYPE_BF16; attention over F32 rows is exact to f32
+ * rounding, over BF16 rows to bf16's.  All calls of the block manager above (sequences, fork, prefix cache, block
+ * tables) serve such a cache; dc_b200_flash_attn_decode / _prefill and dc_b200_kv_read_block refuse it. */
+DC_B200_API int dc_b200_kv_create_q4(dc_ctx* ctx, int n_layer, int n_head, int n_kv_head, int head_dim, int row_type, int max_blocks, int max_seqs,
+                                     int max_blocks_per_seq, dc_kv_cache** out);
+/* Begins a step: counts[e] new tokens of sequence seqs[e] at positions pos0[e] .. pos0[e] + counts[e] - 1, for any
+ * mixture of decoded tokens, drafted ones and prompt portions (host arrays; a sequence once at most; 0 tokens: the entry is left out).  pos0 is
+ * the sequence's length, or less: what stood from there on is then written anew.  Reserves blocks (copying the
+ * shared ones about to be written), sets the lengths and uploads the step's plan, which all later calls of the cache
+ * take: once per step, then one call per layer.  Refused without effect if blocks do not suffice; not allowed within a
+ * stream capture.  A call of dc_b200_kv_seq_free / _fork / _reserve / _prefix_* ends the step.  The calls below may
+ * be captured into a graph; a replay works on the newest plan at that time if its step needs no more plan memory than
+ * any before the capture (otherwise it does nothing), and is subject to the same rules as a call. */
+DC_B200_API int dc_b200_kv_batch(dc_kv_cache* kv, int n_entries, const int32_t* seqs, const int32_t* pos0, const int32_t* counts);
+/* Writes the step's rows into one layer.  k_dev, v_dev: [T][n_kv_head][head_dim] rows ld_kv elements apart (0: dense),
+ * T the step's new tokens, entry after entry.  k_held_dev, v_held_dev (may be NULL): f32 [T][n_kv_head][head_dim], the
+ * values that the cache now stands for. */
+DC_B200_API int dc_b200_kv_q4_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k_dev, const void* v_dev, int ld_kv, float* k_held_dev,
+                                        float* v_held_dev);
+/* Writes the step's rows (k_dev and v_dev both NULL: they stand there already), then attends: the token at position p
+ * of a sequence over positions 0..p.  q_dev: [T][n_head][head_dim] rows ld_q elements apart, out_dev the same with
+ * ld_out (0: dense); any alignment of the elements' own size.  out_dev must not overlap the inputs.  Only enqueues. */
+DC_B200_API int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_dev, int ld_q, const void* k_dev, const void* v_dev,
+                                          int ld_kv, float scale, void* out_dev, int ld_out, float* k_held_dev, float* v_held_dev);
+/* The same on host arrays (dense rows); out is zero-filled on failure. */
+DC_B200_API int dc_b200_flash_attn_q4(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_host, const void* k_host, const void* v_host, float scale,
+                                      void* out_host);
+/* The values that one block of one layer stands for: f32 [16][n_kv_head][head_dim] each (either may be NULL). */
+DC_B200_API int dc_b200_kv_q4_read_block(dc_kv_cache* kv, int layer, int block, float* k_host, float* v_host);
 
 /* ---- sampling / speculative verify ----------------------------------------- */
 /* Greedy pick, first maximum wins (ArgmaxScalar, core/src/sampler/sampler.cpp:42-57). */
