@@ -5,9 +5,14 @@
 // finite or beyond +-65504 is held with d = m = NaN, and reads back so.  Blocks, tables, sharing and copy-on-write are kv.cu's, on planes of
 // one record per (page, key head) (dc_q4.h).  A step is planned once (dc_b200_kv_batch) and then run for every layer.
 //
-// Scores of a token: sum over groups of d (q . codes) + m (sum of q): the codes go to the tensor cores as they are (fp16 subnormals c 2^-24 and
-// c 2^-20, exact), queries as two fp16 terms, and the scale is applied to the f32 sum.  Values: sum over tokens of (p d) codes, the weights
-// p d as two fp16 terms, plus the sum of p m in f32.  The two terms are rows h and h + 8 of one m16 operand, so that they cost no extra product.
+// Scores of a token: sum over groups of d (q . codes) + m (sum of q); answers: sum over tokens of (p d) codes, plus the sum of p m.  Codes go to the
+// tensor cores as fp16, the scales are applied to f32 sums and weights.
+//   bf16 rows: codes as they lie (fp16 subnormals c 2^-24 and c 2^-20, exact), queries as fp16 (exact: 8 bits), weights p d rounded to fp16 (half a step, 2^-11 relative,
+//   an eighth of a bf16 result's own).  Answers are made transposed, 16 dimensions x 8 rows, which fills the operand's sixteen rows with one word of codes a lane.
+// The running reference of a row's exponentials is the largest of score + log2 d (d of the token's value, at least 2^-24), not of the scores: the weights p d stay
+// within 1 whatever the values' size, and clear of fp16's least numbers.
+//   f32 rows: queries and weights as two fp16 terms (22 bits), rows h and h + 8 of one sixteen-row operand, so that they cost no extra product; codes as c - 8
+//   with m + 8 d in place of m: sums around zero, where c and m alone would leave answers as small differences of large sums (measured: 5e-5 of the result, now below 1e-6).
 #include <math.h>
 #include <string.h>
 
@@ -34,6 +39,11 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
@@ -47,6 +57,23 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight codes of a word as four pairs: nibbles (0, 4) and (2, 6) times 1, (1, 5) and (3, 7) times 16; EXACT: c - 8, else c 2^-24.
+template <bool EXACT>
+__device__ __forceinline__ void codes_of(uint32_t w, uint32_t (&c)[4]) {
+    const uint32_t w8 = w >> 8;
+    if constexpr (EXACT) {
+        const __half2 lo = __floats2half2_rn(-1032.0f, -1032.0f), hi = __floats2half2_rn(-1152.0f, -1152.0f);
+        auto add = [](uint32_t x, __half2 y) {
+            const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&x), y);
+            return *reinterpret_cast<const uint32_t*>(&r);
+        };
+        c[0] = add((w & 0x000F000Fu) | 0x64006400u, lo), c[1] = add((w & 0x00F000F0u) | 0x64006400u, hi);
+        c[2] = add((w8 & 0x000F000Fu) | 0x64006400u, lo), c[3] = add((w8 & 0x00F000F0u) | 0x64006400u, hi);
+    } else {
+        c[0] = w & 0x000F000Fu, c[1] = w & 0x00F000F0u, c[2] = w8 & 0x000F000Fu, c[3] = w8 & 0x00F000F0u;
+    }
 }
 
 // ---------------------------------------------------------------- new rows into the cache
@@ -150,11 +177,12 @@ constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BY
 
 // One CTA per (item, key head): its warps take the item's pages in turn, each with a running maximum of its own, and join at the end; the last CTA of a tile joins
 // the tile's splits in their order, so that results do not depend on who comes last.
-// A lane has row h = lane / 4 of the tile, tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page and dimensions 8 j + 2 t, + 1 of the answers (t = lane % 4).
+// A lane has row h = lane / 4 of the tile and tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page (t = lane % 4).
 template <int HD, typename TX>
-__global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
+__global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(const RowsParams p) {
     using R = dc_q4_rec<HD>;
-    constexpr int GR = R::GROUPS, KW = HD / 32, VW = HD / 16;
+    constexpr bool EXACT = sizeof(TX) == 4;
+    constexpr int GR = R::GROUPS, KW = HD / 32, VW = HD / 16, OT = EXACT ? HD / 8 : HD / 16, PART = 8 * (HD + 2);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int s_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t4 = lane & 3, kvh = blockIdx.y, G = p.heads / p.n_kv;
@@ -195,21 +223,21 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
 #pragma unroll
         for (int i = 0; i < RW_STAGES; ++i)
             if (i < n_my) issue(i);
-        // ---- queries: times scale log2 e, two fp16 terms of q 2^(10 - e) with 2^e <= largest of the row < 2^(e + 1); a third nibble's codes come
-        // sixteenfold, so that the dimensions they meet are divided by 16
-        uint32_t qa[HD / 16][4];
+        // ---- queries as fp16 terms of q 2^(10 - e), 2^e <= largest of the row < 2^(e + 1); dimensions that meet codes times 16 are divided by 16.
+        // F turns the products' sums into scores in units of log2 e; qsum: sums of a group's queries in these units
+        uint32_t qa[HD / 16][EXACT ? 4 : 2];
         float qsum[GR], F;
         {
             float x[HD / 16][4], most = 0.0f;
             const TX* src = reinterpret_cast<const TX*>(p.q) + (size_t)(im.tok0 + (row ? j : 0)) * p.ldq + (size_t)(kvh * G + (row ? g : 0)) * HD + 2 * t4;
-            const float mul = row ? p.scale * 1.4426950408889634f : 0.0f;
+            const float mul = p.scale * 1.4426950408889634f;
 #pragma unroll
             for (int s = 0; s < GR; ++s) qsum[s] = 0.0f;
 #pragma unroll
             for (int s = 0; s < HD / 16; ++s) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[s][i] = row ? to_f32(src[16 * s + 8 * (i >> 1) + (i & 1)]) * mul : 0.0f;
+                    x[s][i] = row ? to_f32(src[16 * s + 8 * (i >> 1) + (i & 1)]) : 0.0f;
                     most = fmaxf(most, fabsf(x[s][i]));
                     qsum[s / 4] += x[s][i];
                 }
@@ -220,24 +248,31 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
 #pragma unroll
                 for (int i = 0; i < GR; ++i) qsum[i] += __shfl_xor_sync(0xffffffffu, qsum[i], s);
             }
+#pragma unroll
+            for (int i = 0; i < GR; ++i) qsum[i] *= mul;
             const int e = max(-100, min(100, (int)(__float_as_uint(most) >> 23) - 127));
             const float up = __uint_as_float((uint32_t)(137 - e) << 23);
-            F = __uint_as_float((uint32_t)(141 + e) << 23);
+            F = __uint_as_float((uint32_t)((EXACT ? 117 : 141) + e) << 23) * mul;
 #pragma unroll
             for (int s = 0; s < HD / 16; ++s) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float a = x[s][2 * i] * (i ? up * 0.0625f : up), b = x[s][2 * i + 1] * (i ? up * 0.0625f : up);
                     const uint32_t hi = pack_h2(a, b);
-                    const float2 f = unpack_h2(hi);
-                    qa[s][2 * i] = hi;
-                    qa[s][2 * i + 1] = pack_h2(a - f.x, b - f.y);
+                    if constexpr (EXACT) {
+                        const float2 f = unpack_h2(hi);
+                        qa[s][2 * i] = hi;
+                        qa[s][2 * i + 1] = pack_h2(a - f.x, b - f.y);
+                    } else {
+                        qa[s][i] = hi;
+                    }
                 }
             }
         }
-        float o[HD / 8][4], om[GR], m_run = -1e30f, l = 0.0f;
+        // EXACT: tile c of o has dimensions 8 c + 2 t, + 1 of rows h (first terms) and h (second terms); else dimensions 16 c + h and + 8 of rows 2 t, + 1
+        float o[OT][4], om[GR], m_run = -1e30f, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll
         for (int i = 0; i < GR; ++i) om[i] = 0.0f;
 
@@ -278,9 +313,16 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
                 for (int c = 0; c < GR; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < KW; ++c) {
-                    const uint32_t w = kw[a][c], w8 = w >> 8;
-                    mma_f16(acc[c / 2], qa[2 * c], w & 0x000F000Fu, w & 0x00F000F0u);
-                    mma_f16(acc[c / 2], qa[2 * c + 1], w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+                    uint32_t b[4];
+                    codes_of<EXACT>(kw[a][c], b);
+                    if constexpr (EXACT) {
+                        mma_f16(acc[c / 2], qa[2 * c], b[0], b[1]);
+                        mma_f16(acc[c / 2], qa[2 * c + 1], b[2], b[3]);
+                    } else {
+                        const uint32_t q0[4] = {qa[2 * c][0], 0u, qa[2 * c][1], 0u}, q1[4] = {qa[2 * c + 1][0], 0u, qa[2 * c + 1][1], 0u};
+                        mma_f16(acc[c / 2], q0, b[0], b[1]);
+                        mma_f16(acc[c / 2], q1, b[2], b[3]);
+                    }
                 }
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -288,8 +330,8 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
 #pragma unroll
                     for (int c = 0; c < GR; ++c) {
                         const float2 dm = unpack_h2(kd[a][b][c]);
-                        x = fmaf(dm.x, acc[c][b] + acc[c][2 + b], x);
-                        y = fmaf(dm.y, qsum[c], y);
+                        x = fmaf(dm.x, EXACT ? acc[c][b] + acc[c][2 + b] : acc[c][b], x);
+                        y = fmaf(EXACT ? fmaf(8.0f, dm.x, dm.y) : dm.y, qsum[c], y);
                     }
                     sc[a][b] = fmaf(x, F, y);
                 }
@@ -305,8 +347,20 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
                             for (int c = 0; c < GR; ++c) vd[a][b][c] = 0;
                         }
             }
+            float2 dm[2][2][GR];      // values' scales and least ones (EXACT: the middle, m + 8 d)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) mx = fmaxf(mx, fmaxf(sc[a][0], sc[a][1]));
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    float most = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < GR; ++c) {
+                        dm[a][b][c] = unpack_h2(vd[a][b][c]);
+                        if constexpr (EXACT) dm[a][b][c].y = fmaf(8.0f, dm[a][b][c].x, dm[a][b][c].y);
+                        most = fmaxf(most, dm[a][b][c].x);
+                    }
+                    mx = fmaxf(mx, sc[a][b] + fmaxf(lg2(most), -24.0f));
+                }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             if (__any_sync(0xffffffffu, mx > m_run)) {
@@ -315,32 +369,47 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
                 l *= corr;
 #pragma unroll
                 for (int c = 0; c < GR; ++c) om[c] *= corr;
+                if constexpr (EXACT) {
 #pragma unroll
-                for (int c = 0; c < HD / 8; ++c) o[c][0] *= corr, o[c][1] *= corr, o[c][2] *= corr, o[c][3] *= corr;
+                    for (int c = 0; c < OT; ++c) o[c][0] *= corr, o[c][1] *= corr, o[c][2] *= corr, o[c][3] *= corr;
+                } else {
+                    const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t4), c1 = __shfl_sync(0xffffffffu, corr, 8 * t4 + 4);
+#pragma unroll
+                    for (int c = 0; c < OT; ++c) o[c][0] *= c0, o[c][1] *= c1, o[c][2] *= c0, o[c][3] *= c1;
+                }
             }
-            // ---- weights times scales in two terms (the second one 2^11 fold), values
-            uint32_t pa[GR][4];
+            // ---- weights times scales, values
+            uint32_t pa[GR][EXACT ? 4 : 2];
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const float p0 = ex2(sc[a][0] - m_run), p1 = ex2(sc[a][1] - m_run);
                 l += p0 + p1;
 #pragma unroll
                 for (int c = 0; c < GR; ++c) {
-                    const float2 d0 = unpack_h2(vd[a][0][c]), d1 = unpack_h2(vd[a][1][c]);
+                    const float2 d0 = dm[a][0][c], d1 = dm[a][1][c];
                     om[c] = fmaf(p0, d0.y, om[c]);
                     om[c] = fmaf(p1, d1.y, om[c]);
                     const float w0 = p0 * d0.x, w1 = p1 * d1.x;
                     const uint32_t hi = pack_h2(w0, w1);
-                    const float2 f = unpack_h2(hi);
-                    pa[c][2 * a] = hi;
-                    pa[c][2 * a + 1] = pack_h2((w0 - f.x) * 2048.0f, (w1 - f.y) * 2048.0f);
+                    if constexpr (EXACT) {      // the second term 2^11 fold: it stays clear of fp16's least numbers
+                        const float2 f = unpack_h2(hi);
+                        pa[c][2 * a] = hi;
+                        pa[c][2 * a + 1] = pack_h2((w0 - f.x) * 2048.0f, (w1 - f.y) * 2048.0f);
+                    } else {
+                        pa[c][a] = hi;
+                    }
                 }
             }
 #pragma unroll
             for (int c = 0; c < VW; ++c) {
-                const uint32_t w = vw[c], w8 = w >> 8;
-                mma_f16(o[2 * c], pa[c / 4], w & 0x000F000Fu, w8 & 0x000F000Fu);
-                mma_f16(o[2 * c + 1], pa[c / 4], w & 0x00F000F0u, w8 & 0x00F000F0u);
+                uint32_t b[4];
+                codes_of<EXACT>(vw[c], b);
+                if constexpr (EXACT) {
+                    mma_f16(o[2 * c], pa[c / 4], b[0], b[2]);
+                    mma_f16(o[2 * c + 1], pa[c / 4], b[1], b[3]);
+                } else {
+                    mma_f16(o[c], b, pa[c / 4][0], pa[c / 4][1]);
+                }
             }
         }
         n_full += max(0, n_my);
@@ -351,38 +420,60 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
 #pragma unroll
             for (int c = 0; c < GR; ++c) om[c] += __shfl_xor_sync(0xffffffffu, om[c], s);
         }
+        if constexpr (EXACT) {
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-            const float f = c & 1 ? 1048576.0f : 16777216.0f;
-            float2 x;
-            x.x = fmaf(fmaf(o[c][2], 1.0f / 2048.0f, o[c][0]), f, om[c / 8]);
-            x.y = fmaf(fmaf(o[c][3], 1.0f / 2048.0f, o[c][1]), f, om[c / 8]);
-            *reinterpret_cast<float2*>(part + (warp * 8 + h) * HD + 8 * c + 2 * t4) = x;
+            for (int c = 0; c < OT; ++c) {
+                const float f = c & 1 ? 0.0625f : 1.0f;
+                float2 x;
+                x.x = fmaf(fmaf(o[c][2], 1.0f / 2048.0f, o[c][0]), f, om[c / 8]);
+                x.y = fmaf(fmaf(o[c][3], 1.0f / 2048.0f, o[c][1]), f, om[c / 8]);
+                *reinterpret_cast<float2*>(part + (warp * 8 + h) * HD + 8 * c + 2 * t4) = x;
+            }
+        } else {
+            float om2[GR][2];
+#pragma unroll
+            for (int c = 0; c < GR; ++c) om2[c][0] = __shfl_sync(0xffffffffu, om[c], 8 * t4), om2[c][1] = __shfl_sync(0xffffffffu, om[c], 8 * t4 + 4);
+#pragma unroll
+            for (int c = 0; c < OT; ++c) {
+                float* to = part + (warp * 8 + 2 * t4) * HD + 16 * c + h;
+                to[0] = fmaf(o[c][0], 16777216.0f, om2[c / 4][0]);
+                to[HD] = fmaf(o[c][1], 16777216.0f, om2[c / 4][1]);
+                to[8] = fmaf(o[c][2], 1048576.0f, om2[c / 4][0]);
+                to[HD + 8] = fmaf(o[c][3], 1048576.0f, om2[c / 4][1]);
+            }
         }
         if (t4 == 0) part_ml[2 * (warp * 8 + h)] = m_run, part_ml[2 * (warp * 8 + h) + 1] = l;
         if (!waited) pdl_wait(), waited = true;      // (ahead of the first store)
         __syncthreads();
+        // ---- joined: a thread has four neighbouring dimensions of a row at a time
         const bool alone = im.n_splits == 1;
-        float* ws = reinterpret_cast<float*>(const_cast<int32_t*>(words) + hd->ws) + ((size_t)im.ws * p.n_kv + (size_t)im.n_splits * kvh) * (8 * (HD + 2));
-        TX* out = reinterpret_cast<TX*>(p.out);
-        for (int x = threadIdx.x; x < 8 * HD; x += RW * 32) {
-            const int rr = x / HD, d = x - rr * HD;
-            float M = -1e30f, L = 0.0f, v = 0.0f;
+        float* ws = reinterpret_cast<float*>(const_cast<int32_t*>(words) + hd->ws) + ((size_t)im.ws * p.n_kv + (size_t)im.n_splits * kvh) * PART;
+        auto store = [&](int x4, const float4& v, float inv) {
+            const int ro = im.tile * 8 + x4 / (HD / 4), jo = ro / G, go = ro - jo * G;
+            if (jo >= im.count) return;
+            TX* to = reinterpret_cast<TX*>(p.out) + (size_t)(im.tok0 + jo) * p.ldo + (size_t)(kvh * G + go) * HD + 4 * (x4 % (HD / 4));
+            put(to, v.x * inv), put(to + 1, v.y * inv), put(to + 2, v.z * inv), put(to + 3, v.w * inv);
+        };
+#pragma unroll
+        for (int x4 = threadIdx.x; x4 < 8 * HD / 4; x4 += RW * 32) {
+            const int rr = x4 / (HD / 4);
+            float M = -1e30f, L = 0.0f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < RW; ++w) M = fmaxf(M, part_ml[2 * (w * 8 + rr)]);
 #pragma unroll
             for (int w = 0; w < RW; ++w) {
                 const float f = ex2(part_ml[2 * (w * 8 + rr)] - M);
+                const float4 x = reinterpret_cast<const float4*>(part + w * 8 * HD)[x4];
                 L = fmaf(part_ml[2 * (w * 8 + rr) + 1], f, L);
-                v = fmaf(part[(w * 8 + rr) * HD + d], f, v);
+                v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
             }
             if (alone) {
-                const int ro = im.tile * 8 + rr, jo = ro / G, go = ro - jo * G;
-                if (jo < im.count) put(out + (size_t)(im.tok0 + jo) * p.ldo + (size_t)(kvh * G + go) * HD + d, __fdividef(v, L));
+                store(x4, v, __fdividef(1.0f, L));
             } else {
-                float* to = ws + (size_t)im.split * (8 * (HD + 2));
-                to[x] = v;
-                if (d == 0) to[8 * HD + 2 * rr] = M, to[8 * HD + 2 * rr + 1] = L;
+                float* to = ws + (size_t)im.split * PART;
+                reinterpret_cast<float4*>(to)[x4] = v;
+                if (x4 % (HD / 4) == 0) to[8 * HD + rr] = M, to[8 * HD + 8 + rr] = L;
             }
         }
         if (!alone) {
@@ -396,18 +487,35 @@ __global__ void __launch_bounds__(RW * 32, 3) k_q4_rows(const RowsParams p) {
             }
             __syncthreads();
             if (s_last) {
-                for (int x = threadIdx.x; x < 8 * HD; x += RW * 32) {
-                    const int rr = x / HD, d = x - rr * HD, ro = im.tile * 8 + rr, jo = ro / G, go = ro - jo * G;
-                    if (jo >= im.count) continue;
-                    float M = -1e30f, L = 0.0f, v = 0.0f;
-                    for (int s = 0; s < im.n_splits; ++s) M = fmaxf(M, __ldcg(ws + (size_t)s * (8 * (HD + 2)) + 8 * HD + 2 * rr));
-                    for (int s = 0; s < im.n_splits; ++s) {
-                        const float* from = ws + (size_t)s * (8 * (HD + 2));
-                        const float f = ex2(__ldcg(from + 8 * HD + 2 * rr) - M);
-                        L = fmaf(__ldcg(from + 8 * HD + 2 * rr + 1), f, L);
-                        v = fmaf(__ldcg(from + x), f, v);
+                // the splits' factors in place of the parts: [split][8 rows], DC_Q4_SPLITS at most; then rows' sums
+                static_assert(DC_Q4_SPLITS * 8 + 8 <= RW * 8 * 64, "factors take the parts' place");
+                float *f = part, *inv = part + DC_Q4_SPLITS * 8;
+                if (threadIdx.x < 32) {
+                    const int rr = lane & 7;      // four lanes a row
+                    float M = -1e30f, L = 0.0f;
+                    for (int s = lane >> 3; s < im.n_splits; s += 4) M = fmaxf(M, f[8 * s + rr] = __ldcg(ws + (size_t)s * PART + 8 * HD + rr));
+                    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
+                    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+                    for (int s = lane >> 3; s < im.n_splits; s += 4) {
+                        const float x = ex2(f[8 * s + rr] - M);
+                        f[8 * s + rr] = x;
+                        L = fmaf(__ldcg(ws + (size_t)s * PART + 8 * HD + 8 + rr), x, L);
                     }
-                    put(out + (size_t)(im.tok0 + jo) * p.ldo + (size_t)(kvh * G + go) * HD + d, __fdividef(v, L));
+                    L += __shfl_xor_sync(0xffffffffu, L, 8);
+                    L += __shfl_xor_sync(0xffffffffu, L, 16);
+                    if (lane < 8) inv[rr] = __fdividef(1.0f, L);
+                }
+                __syncthreads();
+                for (int x4 = threadIdx.x; x4 < 8 * HD / 4; x4 += RW * 32) {
+                    const int rr = x4 / (HD / 4);
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                    for (int s = 0; s < im.n_splits; ++s) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + x4);
+                        const float w = f[8 * s + rr];
+                        v.x = fmaf(x.x, w, v.x), v.y = fmaf(x.y, w, v.y), v.z = fmaf(x.z, w, v.z), v.w = fmaf(x.w, w, v.w);
+                    }
+                    store(x4, v, inv[rr]);
                 }
             }
         }

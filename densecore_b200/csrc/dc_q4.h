@@ -50,6 +50,7 @@ struct dc_q4_entry {
     int32_t seq, pos0, count, tok0;
 };
 constexpr int DC_Q4_WARPS = 4;      // of a CTA of k_q4_rows
+constexpr int DC_Q4_SPLITS = 240;   // of a tile, at most
 
 // The items of all tiles of the entries; *n_ws: partial results, *n_tickets: tiles that more than one CTA works on.
 inline void dc_q4_items(const std::vector<dc_q4_entry>& es, int G, int n_kv, int num_sms, std::vector<dc_q4_item>* items, int* n_tickets, int* n_ws) {
@@ -64,9 +65,9 @@ inline void dc_q4_items(const std::vector<dc_q4_entry>& es, int G, int n_kv, int
     *n_tickets = *n_ws = 0;
     for (const dc_q4_entry& e : es)
         for (int t = 0; t < tiles_of(e); ++t) {
-            const int pages = pages_of(e, t), n = (pages + per - 1) / per;
+            const int pages = pages_of(e, t), mine = std::max(per, (pages + DC_Q4_SPLITS - 1) / DC_Q4_SPLITS), n = (pages + mine - 1) / mine;
             for (int s = 0; s < n; ++s)
-                items->push_back({e.seq, e.pos0, e.tok0, e.count, t, s * per, std::min(pages, (s + 1) * per), s, n, n > 1 ? *n_ws : 0, n > 1 ? *n_tickets : 0, 0});
+                items->push_back({e.seq, e.pos0, e.tok0, e.count, t, s * mine, std::min(pages, (s + 1) * mine), s, n, n > 1 ? *n_ws : 0, n > 1 ? *n_tickets : 0, 0});
             if (n > 1) ++*n_tickets, *n_ws += n;
         }
 }
