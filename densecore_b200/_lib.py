@@ -120,6 +120,14 @@ def _signatures() -> dict:
         "dc_b200_verify_accept": (i32, [vp, vp, vp, vp, vp, u64, u32, i32, i32, i32, f32, pi, pi]),
         "dc_b200_verify_uniforms": (i32, [vp, u64, u32, i32, vp]),
         "dc_b200_verify_accept_dev": (i32, [vp, vp, vp, vp, vp, u64, u32, i32, i32, i32, f32, pi, pi]),
+        "dc_b200_sample_rows_dev": (i32, [vp, vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "dc_b200_sample_rows": (i32, [vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "dc_b200_lora_create": (i32, [vp, i64, i64, i32, i32, i32, pp]),
+        "dc_b200_lora_destroy": (None, [vp]),
+        "dc_b200_lora_set": (i32, [vp, i32, i32, vp, vp, f32]),
+        "dc_b200_lora_set_dev": (i32, [vp, i32, i32, vp, vp, f32]),
+        "dc_b200_lora_add_dev": (i32, [vp, vp, vp, i64, i32, vp, vp, i64, vp, i64]),
+        "dc_b200_mul_mat_lora_dev": (i32, [vp, vp, vp, vp, i32, vp, vp]),
         "dc_b200_softmax": (i32, [vp, vp, i32, i32, f32, vp]),
         "dc_b200_sample_dev": (i32, [vp, vp, i32, f32, f32, vp, pi]),
         "dc_b200_model_create": (i32, [vp, C.POINTER(ModelConfig), pp]),

@@ -1,0 +1,402 @@
+// Low-rank adapters of many requests beside a shared product: y[t] = base[t] + s_a (x[t] A_a^T) B_a^T with a = ids[t], rows of other ids (none, unknown, empty)
+// y[t] = base[t].  Two kernels: h = s x A^T (few rows: a warp per rank of a row; many: tiles of 16 rows), then y = base + h B^T in tiles of rows.
+//
+// Rows x and h are f32 and enter the tensor cores as two terms of 11 bits (tf32, 22 bits together; products of m16n8k8 with f32 sums), matrices are bf16 or
+// fp16, which tf32 holds exactly.  A tile whose rows have several adapters takes one after the other: each
+// adapter's matrices are read once per tile, whatever the order of rows.
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "dc_common.cuh"
+#include "dc_internal.h"
+#include "dc_launch.cuh"
+
+using namespace dc;
+
+#define DC_TRY(expr)                       \
+    do {                                   \
+        int _st = (expr);                  \
+        if (_st != DC_B200_OK) return _st; \
+    } while (0)
+
+struct dc_lora {
+    dc_ctx* ctx = nullptr;
+    int64_t K = 0, N = 0, Kp = 0, Np = 0;      // padded to 16 and 8
+    int slots = 0, max_rank = 0, Rp = 0, type = 0;      // ranks padded to 16
+    uint16_t *a = nullptr, *b = nullptr;      // [slot][Rp][Kp] and [slot][Np][Rp], zero where there is nothing
+    int32_t* rank = nullptr;                  // [slot], 0: empty
+    float* scale = nullptr;
+    float* h = nullptr;                       // workspace [rows][Rp]
+    int64_t h_rows = 0;
+    std::vector<float*> retired;              // outgrown workspaces, which captured calls may still name
+};
+
+namespace {
+
+struct LoraParams {
+    const uint16_t *a, *b;
+    const int32_t* rank;
+    const float* scale;
+    int slots, Rp;
+    int64_t K, N, Kp, Np;
+    const float* x;
+    int64_t ldx;
+    int M;
+    const int32_t* ids;
+    float* h;
+    const float* base;
+    float* y;
+    int64_t ldb, ldy;
+};
+
+__device__ __forceinline__ int slot_of(const LoraParams& p, int row) {      // -1: none
+    if (row >= p.M) return -1;
+    const int a = p.ids[row];
+    return a >= 0 && a < p.slots && p.rank[a] > 0 ? a : -1;
+}
+template <bool BF>
+__device__ __forceinline__ float2 two(uint32_t w) {
+    if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The product of 16 neighbours along k: lane (h, t) holds rows h, h + 8 of the first operand and column h of the second, k = 4 t .. 4 t + 3.  Two steps of
+// k8 (4 t and 4 t + 1 stand for t and t + 4 of the first, 4 t + 2 and 4 t + 3 of the second), the low terms first.
+struct Terms {
+    uint32_t hi[2][4], lo[2][4];
+    __device__ __forceinline__ Terms(const float4& u, const float4& v) {
+        const float r[2][4] = {{u.x, u.y, u.z, u.w}, {v.x, v.y, v.z, v.w}};
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {      // rows h, h + 8 at k = t, then at t + 4
+                const float f = r[i & 1][2 * s + (i >> 1)];
+                hi[s][i] = __float_as_uint(f) & 0xFFFFE000u;
+                lo[s][i] = __float_as_uint(f - __uint_as_float(hi[s][i]));
+            }
+    }
+    __device__ __forceinline__ void times(float (&d)[4], const float2& b01, const float2& b23) const {
+        mma_tf32(d, lo[0], __float_as_uint(b01.x), __float_as_uint(b01.y));
+        mma_tf32(d, lo[1], __float_as_uint(b23.x), __float_as_uint(b23.y));
+        mma_tf32(d, hi[0], __float_as_uint(b01.x), __float_as_uint(b01.y));
+        mma_tf32(d, hi[1], __float_as_uint(b23.x), __float_as_uint(b23.y));
+    }
+};
+__device__ __forceinline__ float4 load_x4(const float* row, int64_t k, int64_t K, bool vec, bool in) {
+    if (!in || k >= K) return make_float4(0.f, 0.f, 0.f, 0.f);
+    if (vec && k + 4 <= K) return __ldg(reinterpret_cast<const float4*>(row + k));
+    return make_float4(row[k], k + 1 < K ? row[k + 1] : 0.f, k + 2 < K ? row[k + 2] : 0.f, k + 3 < K ? row[k + 3] : 0.f);
+}
+
+// Few rows: a warp per rank of a row.  Bound: latency of the matrix' rows.
+template <bool BF>
+__global__ void __launch_bounds__(256) k_lora_down(const LoraParams p, int vec) {
+    const int row = blockIdx.x, r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int a = slot_of(p, row);
+    if (a < 0 || r >= (p.rank[a] + 15) / 16 * 16) return;      // (the padding's rows of the matrix are zero, so are its sums)
+    const uint16_t* w = p.a + ((size_t)a * p.Rp + r) * p.Kp;
+    const float* x = p.x + (size_t)row * p.ldx;
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll 4
+    for (int64_t k = 4 * lane; k < p.Kp; k += 128) {
+        const uint2 c = __ldg(reinterpret_cast<const uint2*>(w + k));
+        const float4 v = load_x4(x, k, p.K, vec, true);
+        const float2 c0 = two<BF>(c.x), c1 = two<BF>(c.y);
+        s0 = fmaf(v.x, c0.x, s0), s1 = fmaf(v.y, c0.y, s1);
+        s0 = fmaf(v.z, c1.x, s0), s1 = fmaf(v.w, c1.y, s1);
+    }
+    s0 += s1;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, s);
+    if (lane == 0) p.h[(size_t)row * p.Rp + r] = s0 * p.scale[a];
+}
+
+// Adapters of a tile's rows, one after the other: `f(slot, mask)` with the rows (bits) that have it.
+template <typename F>
+__device__ __forceinline__ void each_adapter(int mine, uint32_t rows, F f) {      // mine: lane i's row's slot; rows: bits to look at
+    uint32_t todo = __ballot_sync(0xffffffffu, mine >= 0) & rows;
+    while (todo) {
+        const int a = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+        const uint32_t mask = __ballot_sync(0xffffffffu, mine == a) & rows;
+        f(a, mask);
+        todo &= ~mask;
+    }
+}
+
+// A row's sums are its own adapter's; the others' passes may leave anything there (zero times an infinite matrix).
+template <int N>
+__device__ __forceinline__ void keep_rows(float (&acc)[N][4], const float (&sum)[N][4], bool u, bool v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (u) acc[i][0] = sum[i][0], acc[i][1] = sum[i][1];
+        if (v) acc[i][2] = sum[i][2], acc[i][3] = sum[i][3];
+    }
+}
+
+constexpr int DT_R = 64;      // ranks of a CTA of k_lora_down_tile
+
+// Many rows: a CTA per (16 rows, 64 ranks), its warps share out k in steps of 16 and add up in the end.
+template <bool BF>
+__global__ void __launch_bounds__(256) k_lora_down_tile(const LoraParams p, int vec) {
+    __shared__ float part[8][16][DT_R + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.x * 16, r0 = blockIdx.y * DT_R;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int mine = slot_of(p, row0 + (lane & 15));
+    float acc[DT_R / 8][4];
+#pragma unroll
+    for (int i = 0; i < DT_R / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+    each_adapter(mine, 0xFFFFu, [&](int a, uint32_t mask) {
+        const int tiles = min(DT_R / 8, ((p.rank[a] + 15) / 16 * 16 - r0) / 8);
+        if (tiles <= 0) return;
+        float sum[DT_R / 8][4];
+#pragma unroll
+        for (int i = 0; i < DT_R / 8; ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.0f;
+        const bool u = mask >> h & 1, v = mask >> (h + 8) & 1;
+        const float *xu = p.x + (size_t)(row0 + (u ? h : 0)) * p.ldx, *xv = p.x + (size_t)(row0 + (v ? h + 8 : 0)) * p.ldx;
+        const uint16_t* w = p.a + ((size_t)a * p.Rp + r0 + h) * p.Kp + 4 * t;
+#pragma unroll 2
+        for (int64_t k = 16 * warp; k < p.Kp; k += 128) {
+            const Terms x(load_x4(xu, k + 4 * t, p.K, vec, u), load_x4(xv, k + 4 * t, p.K, vec, v));
+#pragma unroll
+            for (int i = 0; i < DT_R / 8; ++i)
+                if (i < tiles) {
+                    const uint2 c = __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Kp + k));
+                    x.times(sum[i], two<BF>(c.x), two<BF>(c.y));
+                }
+        }
+        keep_rows(acc, sum, u, v);
+    });
+#pragma unroll
+    for (int i = 0; i < DT_R / 8; ++i) {
+        part[warp][h][8 * i + 2 * t] = acc[i][0], part[warp][h][8 * i + 2 * t + 1] = acc[i][1];
+        part[warp][h + 8][8 * i + 2 * t] = acc[i][2], part[warp][h + 8][8 * i + 2 * t + 1] = acc[i][3];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * DT_R; i += 256) {
+        const int row = i / DT_R, r = i % DT_R, a = slot_of(p, row0 + row);
+        if (a < 0 || r0 + r >= p.Rp) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += part[w][row][r];
+        p.h[(size_t)(row0 + row) * p.Rp + r0 + r] = s * p.scale[a];
+    }
+}
+
+// y = base + h B^T: a CTA per (16 MT rows, 64 NP columns), a warp has 8 NP columns.  Bound: base and y for many rows, the matrices' latency for few.
+template <bool BF, int MT, int NP>
+__global__ void __launch_bounds__(256) k_lora_up(const LoraParams p, int vec) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.y * 16 * MT;
+    const int64_t n0 = ((int64_t)blockIdx.x * 8 + warp) * 8 * NP;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (n0 >= p.N) return;
+    const int mine = slot_of(p, row0 + (lane & (16 * MT - 1)));
+    float acc[MT][NP][4] = {};
+    each_adapter(mine, MT == 1 ? 0xFFFFu : 0xFFFFFFFFu, [&](int a, uint32_t mask) {
+        const int ranks = p.rank[a];
+        const uint16_t* w = p.b + ((size_t)a * p.Np + n0 + h) * p.Rp + 4 * t;
+        const float* hh = p.h + (size_t)row0 * p.Rp + 4 * t;
+        float sum[MT][NP][4] = {};
+#pragma unroll 1
+        for (int r = 0; r < ranks; r += 16) {
+            uint2 c[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) c[i] = n0 + 8 * i < p.Np ? __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Rp + r)) : make_uint2(0, 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if (!(mask >> (16 * m) & 0xFFFFu)) continue;
+                float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+                if (mask >> (16 * m + h) & 1) u = __ldcg(reinterpret_cast<const float4*>(hh + (size_t)(16 * m + h) * p.Rp + r));
+                if (mask >> (16 * m + h + 8) & 1) v = __ldcg(reinterpret_cast<const float4*>(hh + (size_t)(16 * m + h + 8) * p.Rp + r));
+                const Terms x(u, v);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) x.times(sum[m][i], two<BF>(c[i].x), two<BF>(c[i].y));
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) keep_rows(acc[m], sum[m], mask >> (16 * m + h) & 1, mask >> (16 * m + h + 8) & 1);
+    });
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int row = row0 + 16 * m + h + 8 * q;
+            if (row >= p.M) continue;
+            const float* from = p.base + (size_t)row * p.ldb;
+            float* to = p.y + (size_t)row * p.ldy;
+            float2 f[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int64_t n = n0 + 8 * i + 2 * t;
+                if (vec && n + 1 < p.N) f[i] = *reinterpret_cast<const float2*>(from + n);
+                else f[i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int64_t n = n0 + 8 * i + 2 * t;
+                f[i].x += acc[m][i][2 * q], f[i].y += acc[m][i][2 * q + 1];
+                if (vec && n + 1 < p.N) {
+                    *reinterpret_cast<float2*>(to + n) = f[i];
+                } else {
+                    if (n < p.N) to[n] = f[i].x;
+                    if (n + 1 < p.N) to[n + 1] = f[i].y;
+                }
+            }
+        }
+}
+
+// One adapter's matrices into their padded places; `rank` 0 empties the slot.
+__global__ void __launch_bounds__(256) k_lora_set(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b, uint16_t* __restrict__ to_a, uint16_t* __restrict__ to_b, int rank, int Rp,
+                                                  int64_t K, int64_t Kp, int64_t N, int64_t Np, int32_t* rank_at, float* scale_at, float scale) {
+    pdl_wait();
+    const int64_t all_a = (int64_t)Rp * Kp, all = all_a + Np * Rp;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        if (i < all_a) {
+            const int64_t r = i / Kp, k = i - r * Kp;
+            to_a[i] = r < rank && k < K ? a[r * K + k] : (uint16_t)0;
+        } else {
+            const int64_t n = (i - all_a) / Rp, r = (i - all_a) - n * Rp;
+            to_b[i - all_a] = r < rank && n < N ? b[n * rank + r] : (uint16_t)0;
+        }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *rank_at = rank, *scale_at = scale;
+}
+
+// Rows from which x A^T runs in tiles of sixteen: below, a warp a rank has more CTAs; above, tiles read the matrix once for sixteen rows.
+constexpr int LORA_TILE_ROWS = 129;
+// Rows from which y takes 32 rows and 256 columns a CTA instead of 16 and 64.
+constexpr int LORA_WIDE_ROWS = 129;
+
+template <bool BF>
+int launch_add(dc_ctx* ctx, const LoraParams& p, int max_rank) {
+    const int vx = ((uintptr_t)p.x & 15) == 0 && p.ldx % 4 == 0, vy = ((uintptr_t)p.base & 7) == 0 && ((uintptr_t)p.y & 7) == 0 && p.ldb % 2 == 0 && p.ldy % 2 == 0;
+    if (p.M < LORA_TILE_ROWS)
+        DC_TRY(dc_launch(ctx, "k_lora_down", k_lora_down<BF>, dim3(p.M, (max_rank + 15) / 16 * 2), dim3(256), 0, p, vx));
+    else
+        DC_TRY(dc_launch(ctx, "k_lora_down_tile", k_lora_down_tile<BF>, dim3((p.M + 15) / 16, (p.Rp + DT_R - 1) / DT_R), dim3(256), 0, p, vx));
+    if (p.M < LORA_WIDE_ROWS)
+        return dc_launch(ctx, "k_lora_up", k_lora_up<BF, 1, 1>, dim3((unsigned)((p.N + 63) / 64), (p.M + 15) / 16), dim3(256), 0, p, vy);
+    return dc_launch(ctx, "k_lora_up", k_lora_up<BF, 2, 4>, dim3((unsigned)((p.N + 255) / 256), (p.M + 31) / 32), dim3(256), 0, p, vy);
+}
+
+int grow(dc_ctx* ctx, dc_lora* l, int64_t rows) {
+    if (rows <= l->h_rows) return DC_B200_OK;
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone)
+        return dc_fail(ctx, DC_B200_UNSUPPORTED, "lora_add: the first call with %lld rows or more cannot be captured", (long long)rows);
+    float* fresh = nullptr;
+    const int64_t want = std::max<int64_t>(rows + rows / 2, 64);
+    DC_TRY(dc_check_cuda(ctx, cudaMalloc(&fresh, (size_t)want * l->Rp * 4), "lora workspace"));
+    if (l->h) l->retired.push_back(l->h);
+    l->h = fresh, l->h_rows = want;
+    return DC_B200_OK;
+}
+
+int check_set(dc_lora* l, int slot, int rank, const void* a, const void* b, float scale) {
+    if (slot < 0 || slot >= l->slots || rank < 0 || rank > l->max_rank || (rank && (!a || !b)) || !isfinite(scale))
+        return dc_fail(l->ctx, DC_B200_INVALID_ARGUMENT, "lora_set: slot %d of %d, rank %d of at most %d", slot, l->slots, rank, l->max_rank);
+    return DC_B200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_b200_lora_create(dc_ctx* ctx, int64_t K, int64_t N, int max_adapters, int max_rank, int type, dc_lora** out) {
+    if (!ctx || !out) return DC_B200_INVALID_ARGUMENT;
+    *out = nullptr;
+    if (K < 1 || N < 1 || K > (1 << 24) || N > (1 << 24) || max_adapters < 1 || max_rank < 1 || max_rank > 4096)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_create: bad shape (%lld x %lld, %d adapters of rank %d)", (long long)K, (long long)N, max_adapters, max_rank);
+    if (type != DC_TYPE_BF16 && type != DC_TYPE_F16) return dc_fail(ctx, DC_B200_UNSUPPORTED, "lora_create: matrices of type %d (BF16 and F16 are supported)", type);
+    cudaSetDevice(ctx->device);
+    dc_lora* l = new dc_lora();
+    l->ctx = ctx, l->K = K, l->N = N, l->Kp = (K + 15) / 16 * 16, l->Np = (N + 7) / 8 * 8;
+    l->slots = max_adapters, l->max_rank = max_rank, l->Rp = (max_rank + 15) / 16 * 16, l->type = type;
+    cudaError_t e = cudaMalloc(&l->a, (size_t)max_adapters * l->Rp * l->Kp * 2);
+    if (e == cudaSuccess) e = cudaMalloc(&l->b, (size_t)max_adapters * l->Np * l->Rp * 2);
+    if (e == cudaSuccess) e = cudaMalloc(&l->rank, (size_t)max_adapters * 4);
+    if (e == cudaSuccess) e = cudaMalloc(&l->scale, (size_t)max_adapters * 4);
+    if (e == cudaSuccess) e = cudaMemsetAsync(l->rank, 0, (size_t)max_adapters * 4, ctx->stream);
+    if (e != cudaSuccess) {
+        const int st = dc_check_cuda(ctx, e, "lora_create");
+        cudaFree(l->a), cudaFree(l->b), cudaFree(l->rank), cudaFree(l->scale);
+        delete l;
+        return st;
+    }
+    *out = l;
+    return DC_B200_OK;
+}
+
+void dc_b200_lora_destroy(dc_lora* l) {
+    if (!l) return;
+    cudaSetDevice(l->ctx->device);
+    cudaStreamSynchronize(l->ctx->stream);
+    cudaFree(l->a), cudaFree(l->b), cudaFree(l->rank), cudaFree(l->scale);
+    if (l->h) cudaFree(l->h);
+    for (float* h : l->retired) cudaFree(h);
+    delete l;
+}
+
+int dc_b200_lora_set_dev(dc_lora* l, int slot, int rank, const void* a_dev, const void* b_dev, float scale) {
+    if (!l) return DC_B200_INVALID_ARGUMENT;
+    DC_TRY(check_set(l, slot, rank, a_dev, b_dev, scale));
+    dc_ctx* ctx = l->ctx;
+    cudaSetDevice(ctx->device);
+    const int64_t all = (int64_t)l->Rp * (l->Kp + l->Np);
+    return dc_launch(ctx, "k_lora_set", k_lora_set, dim3((unsigned)std::min<int64_t>((all + 255) / 256, ctx->num_sms * 16)), dim3(256), 0, (const uint16_t*)a_dev, (const uint16_t*)b_dev,
+                     l->a + (size_t)slot * l->Rp * l->Kp, l->b + (size_t)slot * l->Np * l->Rp, rank, l->Rp, l->K, l->Kp, l->N, l->Np, l->rank + slot, l->scale + slot, scale);
+}
+
+int dc_b200_lora_set(dc_lora* l, int slot, int rank, const void* a_host, const void* b_host, float scale) {
+    if (!l) return DC_B200_INVALID_ARGUMENT;
+    DC_TRY(check_set(l, slot, rank, a_host, b_host, scale));
+    dc_ctx* ctx = l->ctx;
+    cudaSetDevice(ctx->device);
+    const size_t na = (size_t)rank * l->K * 2, nb = (size_t)rank * l->N * 2, pad = (na + 255) / 256 * 256;
+    uint8_t* s = dc_scratch(ctx, pad + nb + 256);
+    if (!s) return DC_B200_OUT_OF_MEMORY;
+    if (rank) DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(s, a_host, na, cudaMemcpyHostToDevice, ctx->stream), "lora_set"));
+    if (rank) DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(s + pad, b_host, nb, cudaMemcpyHostToDevice, ctx->stream), "lora_set"));
+    DC_TRY(dc_b200_lora_set_dev(l, slot, rank, s, s + pad, scale));
+    return dc_b200_synchronize(ctx);
+}
+
+int dc_b200_lora_add_dev(dc_ctx* ctx, dc_lora* l, const float* x_dev, int64_t ld_x, int M, const int32_t* ids_dev, const float* base_dev, int64_t ld_base, float* y_dev, int64_t ld_y) {
+    if (!ctx || !l) return DC_B200_INVALID_ARGUMENT;
+    if (l->ctx != ctx) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: the adapters belong to another context");
+    if (ld_x == 0) ld_x = l->K;
+    if (ld_base == 0) ld_base = l->N;
+    if (ld_y == 0) ld_y = l->N;
+    if (M < 0 || M > (1 << 20) || ld_x < l->K || ld_base < l->N || ld_y < l->N)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: bad argument (%d rows, strides %lld, %lld, %lld)", M, (long long)ld_x, (long long)ld_base, (long long)ld_y);
+    if (M == 0) return DC_B200_OK;
+    if (!x_dev || !ids_dev || !y_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: null buffer");
+    if (!base_dev) base_dev = y_dev, ld_base = ld_y;
+    cudaSetDevice(ctx->device);
+    DC_TRY(grow(ctx, l, M));
+    const LoraParams p = {l->a, l->b, l->rank, l->scale, l->slots, l->Rp, l->K, l->N, l->Kp, l->Np, x_dev, ld_x, M, ids_dev, l->h, base_dev, y_dev, ld_base, ld_y};
+    return l->type == DC_TYPE_BF16 ? launch_add<true>(ctx, p, l->max_rank) : launch_add<false>(ctx, p, l->max_rank);
+}
+
+int dc_b200_mul_mat_lora_dev(dc_ctx* ctx, const dc_weight* w, dc_lora* l, const float* x_dev, int M, const int32_t* ids_dev, float* y_dev) {
+    if (!ctx || !w || !l) return DC_B200_INVALID_ARGUMENT;
+    if (w->K != l->K || w->N != l->N || w->E != 1)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: adapters of %lld x %lld beside a matrix of %lld x %lld", (long long)l->K, (long long)l->N, (long long)w->K, (long long)w->N);
+    if (M < 1 || !x_dev || !ids_dev || !y_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: bad argument");
+    const uintptr_t x0 = (uintptr_t)x_dev, x1 = (uintptr_t)(x_dev + (size_t)M * l->K), y0 = (uintptr_t)y_dev, y1 = (uintptr_t)(y_dev + (size_t)M * l->N);
+    if (!(x1 <= y0 || y1 <= x0)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: x and y overlap");
+    if (l->ctx != ctx) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: the adapters belong to another context");
+    DC_TRY(dc_b200_mul_mat_dev(ctx, w, x_dev, M, y_dev));
+    return dc_b200_lora_add_dev(ctx, l, x_dev, 0, M, ids_dev, nullptr, 0, y_dev, 0);
+}
+
+}  // extern "C"

@@ -1,0 +1,649 @@
+// Sampling of one token a row by temperature, top-k, top-p and min-p from given uniform numbers (the order of DenseCore's sampler: temperature, top-k, top-p,
+// core/src/sampler/sampler.cpp:235-262; min-p after them).
+//
+// The order of a row's tokens is by falling logit, equal ones by rising index; every filter keeps a beginning of it, so that one comparison with the last kept
+// token's key (value, index) decides.  Weights exp((x - largest) / T) are whole numbers of 2^-44 (made in 64 bits): their sums do not depend on the order of
+// additions, so that atomics in any order give the same result, and a border between two tokens moves by 2^-44 times the number of tokens at most.
+//
+// One cluster of CTAs per row: the row lies in their shared memory, a contiguous part each, and is read from HBM once.
+//   1. the largest token;  2. a histogram of 2048 bins of falling value (numbers, and weights where the cut goes by weight) finds the bin with the cut;
+//   3. up to 1024 tokens down to that bin: they are sorted in one CTA, which applies all filters and draws;
+//   else the bin is refined to the cut's key, and 4. all CTAs sum the kept weights of their parts and the part with the draw is searched.
+#include <cooperative_groups.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "dc_common.cuh"
+#include "dc_internal.h"
+#include "dc_launch.cuh"
+
+namespace cg = cooperative_groups;
+using namespace dc;
+
+#define DC_TRY(expr)                       \
+    do {                                   \
+        int _st = (expr);                  \
+        if (_st != DC_B200_OK) return _st; \
+    } while (0)
+
+namespace {
+
+typedef unsigned long long u64;
+constexpr int SF_T = 512, SF_W = SF_T / 32, SF_BINS = 2048, SF_LIST = 1024, SF_CLUSTER = 8;
+constexpr int SF_MOST = 48 * 1024;      // tokens of a CTA
+constexpr u64 SF_ONE = 1ull << 44;
+
+struct SampleParams {
+    const void* logits;
+    size_t ld;
+    int V, seg;      // seg: tokens of a warp, contiguous
+    const float* temperature;
+    const int32_t* top_k;
+    const float *top_p, *min_p, *u;
+    int32_t* token;
+    float *p, *dist;
+};
+
+__device__ __forceinline__ uint32_t sort_key(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+__device__ __forceinline__ u64 token_key(float x, int index) { return ((u64)sort_key(x + 0.0f) << 32) | (uint32_t)~index; }      // (-0 and 0 are equal)
+__device__ __forceinline__ int key_index(u64 k) { return (int)~(uint32_t)k; }
+
+// exp2 in 64 bits: 2^(k / 64) from a table times a polynomial of degree 4 (Taylor, |r| <= 1/128: 4e-14), rounded to whole numbers of 2^-44.
+struct Weigher {
+    double most, c;      // largest logit, log2(e) / T
+    const double* table;
+    bool infinite;
+    __device__ __forceinline__ u64 operator()(float x) const {
+        if (infinite) return x == INFINITY ? SF_ONE : 0ull;
+        if (!(x > -INFINITY)) return 0ull;
+        const double y = ((double)x - most) * c;
+        if (!(y > -46.0)) return 0ull;
+        const double t = y + 105553116266496.0;      // 1.5 2^46: to the nearest 64th
+        const int k = __double2loint(t);
+        const double r = y - (t - 105553116266496.0);
+        const double q = fma(r, fma(r, fma(r, fma(r, 0.0096181291076284772, 0.055504108664821580), 0.24022650695910071), 0.69314718055994531), 1.0);
+        const double v = table[k & 63] * q;
+        const double w = __hiloint2double(__double2hiint(v) + ((k >> 6) << 20), __double2loint(v)) + 256.0;      // units of 2^-44
+        return (u64)__double_as_longlong(w) - 0x4070000000000000ull;
+    }
+};
+
+struct Shared {      // beside the row and the histogram
+    double table[64];
+    u64 best[SF_CLUSTER], warp[SF_W], part[SF_CLUSTER];
+    u64 cut, total, before, in_before;
+    uint32_t lo[SF_CLUSTER], hi[SF_CLUSTER];
+    int bin, upto, inside, n_list, found, counts[SF_CLUSTER];
+};
+
+template <typename TX>
+struct Sampler {
+    cg::cluster_group cl = cg::this_cluster();
+    const SampleParams& p;
+    float* xs;
+    uint32_t* cnt;
+    u64* wh;
+    Shared* sh;
+    int rank, n_cta, warp, lane, base;      // base: token index of xs[0]
+    Weigher w;
+    float to_bin;
+    u64 best;
+
+    __device__ Sampler(const SampleParams& p_) : p(p_) {}
+
+    __device__ __forceinline__ int bin_of(float x) const { return (int)fminf((key_value((uint32_t)(best >> 32)) - x) * to_bin, (float)(SF_BINS - 1)); }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {      // f(value, index) of this warp's tokens that have a value; whole warps
+        const float* x = xs + warp * p.seg;
+        for (int i = lane; i < p.seg; i += 32) f(x[i], base + warp * p.seg + i);
+    }
+    __device__ u64 block_sum(u64 v) const {      // in all threads
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+        __syncthreads();
+        if (lane == 0) sh->warp[warp] = v;
+        __syncthreads();
+        v = 0;
+        for (int i = 0; i < SF_W; ++i) v += sh->warp[i];
+        return v;
+    }
+    __device__ u64 cluster_sum(u64 v) {
+        v = block_sum(v);
+        cl.sync();      // (nobody still reads an earlier sum)
+        if (threadIdx.x < n_cta) cl.map_shared_rank(sh, threadIdx.x)->part[rank] = v;
+        cl.sync();
+        v = 0;
+        for (int i = 0; i < n_cta; ++i) v += sh->part[i];
+        return v;
+    }
+    template <typename T>
+    __device__ void everywhere(T Shared::* at, T v) {      // (one thread)
+        for (int i = 0; i < n_cta; ++i) cl.map_shared_rank(sh, i)->*at = v;
+    }
+    // inclusive sums of a value a thread, over the CTA
+    __device__ u64 scan(u64 v) const {
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const u64 o = __shfl_up_sync(0xffffffffu, v, s);
+            if (lane >= s) v += o;
+        }
+        __syncthreads();
+        if (lane == 31) sh->warp[warp] = v;
+        __syncthreads();
+        for (int i = 0; i < warp; ++i) v += sh->warp[i];
+        return v;
+    }
+
+    // Numbers (and weights) per bin of the tokens that `bin` gives a bin >= 0; their sums in CTA 0, which looks for the bin with the cut: the one that holds the
+    // count-th token (count > 0), or the one where `goal` is reached by the weights on top of `before`.  Everyone then has bin, upto (tokens down to
+    // and with the bin), inside (tokens in it), before (weights ahead of it) and in_before (tokens ahead of it).
+    template <typename F>
+    __device__ void histogram(bool weights, F bin, long long count, float top_p, u64 before, u64* total, bool total_wanted) {
+        for (int i = threadIdx.x; i < SF_BINS; i += SF_T) cnt[i] = 0, wh[i] = 0;
+        __syncthreads();
+        each([&](float x, int i) {
+            const int b = bin(x, i);
+            if (b >= 0) {
+                atomicAdd(cnt + b, 1u);
+                if (weights) {
+                    const u64 v = w(x);
+                    if (v) atomicAdd(wh + b, v);
+                }
+            }
+        });
+        cl.sync();
+        for (int b = rank + n_cta * threadIdx.x; b < SF_BINS; b += n_cta * SF_T) {      // every CTA sums up its share of the bins
+            uint32_t n = 0;
+            u64 v = 0;
+            for (int i = 0; i < n_cta; ++i) {
+                n += cl.map_shared_rank(cnt, i)[b];
+                if (weights) v += cl.map_shared_rank(wh, i)[b];
+            }
+            cl.map_shared_rank(cnt, 0)[b] = n;
+            if (weights) cl.map_shared_rank(wh, 0)[b] = v;
+        }
+        cl.sync();
+        if (rank == 0) {
+            constexpr int B = SF_BINS / SF_T;
+            uint32_t n[B];
+            u64 v[B], sn = 0, sv = 0;
+            for (int i = 0; i < B; ++i) {
+                n[i] = cnt[B * threadIdx.x + i], v[i] = weights ? wh[B * threadIdx.x + i] : 0;
+                sn += n[i], sv += v[i];
+            }
+            u64 an = scan(sn) - sn, av = scan(sv);
+            const u64 all = block_sum(sv);
+            av -= sv;
+            if (total_wanted && threadIdx.x == 0) everywhere(&Shared::total, all);
+            const double goal = (double)top_p * (double)(total_wanted ? all : *total);
+            int last = -1;      // of the CTA's last bin with a token: taken if no bin reaches the cut
+            for (int i = 0; i < B; ++i)
+                if (n[i]) last = B * (int)threadIdx.x + i;
+            __syncthreads();
+            if (threadIdx.x == 0) sh->found = -1;
+            __syncthreads();
+            if (last >= 0) atomicMax(&sh->found, last);
+            __syncthreads();
+            const int fall_back = sh->found;
+            for (int i = 0; i < B; ++i) {
+                const int b = B * (int)threadIdx.x + i;
+                bool here;
+                if (count > 0) here = (long long)an < count && (long long)(an + n[i]) >= count;
+                else here = n[i] && (double)(before + av) < goal && (double)(before + av + v[i]) >= goal;
+                if (count > 0 ? here || (b == fall_back && (long long)(an + n[i]) < count) : here || (b == fall_back && (double)(before + av + v[i]) < goal)) {
+                    everywhere(&Shared::bin, b);
+                    everywhere(&Shared::upto, (int)(an + n[i]));
+                    everywhere(&Shared::inside, (int)n[i]);
+                    everywhere(&Shared::before, before + av);
+                    everywhere(&Shared::in_before, an);
+                }
+                an += n[i], av += v[i];
+            }
+        }
+        cl.sync();
+    }
+
+    // The keys of tokens that `take` names, into CTA 0's list (unordered); its length in CTA 0's n_list.
+    template <typename F>
+    __device__ void gather(F take) {
+        if (rank == 0 && threadIdx.x == 0) sh->n_list = 0;
+        cl.sync();
+        u64* list = cl.map_shared_rank(wh, 0);
+        int* n = &cl.map_shared_rank(sh, 0)->n_list;
+        each([&](float x, int i) {
+            if (take(x, i)) {
+                const int at = atomicAdd(n, 1);
+                if (at < SF_LIST) list[at] = token_key(x, i);
+            }
+        });
+        cl.sync();
+    }
+    // CTA 0: list[0 .. n) sorted, largest first; n <= SF_LIST
+    __device__ void sort(u64* list, int n) const {
+        int size = 2;
+        while (size < n) size <<= 1;
+        for (int i = n + threadIdx.x; i < size; i += SF_T) list[i] = 0;
+        __syncthreads();
+        for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                for (int i = threadIdx.x; i < size / 2; i += SF_T) {
+                    const int a = 2 * i - (i & (j - 1)), b = a + j;
+                    const u64 x = list[a], y = list[b];
+                    if ((x < y) == ((a & k) == 0)) list[a] = y, list[b] = x;
+                }
+                __syncthreads();
+            }
+    }
+    // CTA 0: token i of the sorted list's weights ahead of it; two tokens a thread.  pre[0], pre[1]: of tokens 2 t and 2 t + 1; own: theirs
+    __device__ void ahead(const u64* list, int n, u64 (&own)[2], u64 (&pre)[2]) const {
+        const int t = threadIdx.x;
+        own[0] = 2 * t < n ? w(key_value((uint32_t)(list[2 * t] >> 32))) : 0;
+        own[1] = 2 * t + 1 < n ? w(key_value((uint32_t)(list[2 * t + 1] >> 32))) : 0;
+        pre[0] = scan(own[0] + own[1]) - own[0] - own[1];
+        pre[1] = pre[0] + own[0];
+    }
+
+    // The key of the last token that a cut by number (count > 0) or by weight keeps, among the tokens at or above `from`; `total`: the sum of their weights if the
+    // caller wants it or the cut goes by weight.
+    __device__ u64 cut_at(u64 from, long long count, float top_p, u64* total) {
+        const bool weights = count <= 0;
+        histogram(weights, [&](float x, int i) { return x > -INFINITY && token_key(x, i) >= from ? bin_of(x) : -1; }, count, top_p, 0, total, weights);
+        if (weights) *total = sh->total;
+        const int b = sh->bin;
+        uint32_t lo = 0, hi = 0xFFFFFFFFu;
+        bool by_bin = true;
+        auto in = [&](float x, int i) {
+            if (!(x > -INFINITY) || token_key(x, i) < from) return false;
+            const uint32_t k = sort_key(x + 0.0f);
+            return by_bin ? bin_of(x) == b : k >= lo && k <= hi;
+        };
+        u64 before = sh->before;      // weights and tokens surely kept
+        long long kept = (long long)sh->in_before;
+        int inside = sh->inside;
+        for (;;) {
+            if (inside <= SF_LIST) {
+                gather(in);
+                if (rank == 0) {
+                    const int n = min(sh->n_list, SF_LIST);
+                    sort(wh, n);
+                    u64 own[2], pre[2];
+                    ahead(wh, n, own, pre);
+                    int last = -1;
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = 2 * threadIdx.x + i;
+                        if (at < n && (weights ? at == 0 || (double)(before + pre[i]) < (double)top_p * (double)*total : kept + at < count)) last = at;
+                    }
+                    if (threadIdx.x == 0) sh->found = 0;
+                    __syncthreads();
+                    if (last > 0) atomicMax(&sh->found, last);
+                    __syncthreads();
+                    if (threadIdx.x == 0) everywhere(&Shared::cut, wh[sh->found]);
+                }
+                cl.sync();
+                return sh->cut;
+            }
+            // ---- the values' range in the bin
+            uint32_t a = 0xFFFFFFFFu, z = 0;
+            each([&](float x, int i) {
+                if (in(x, i)) a = min(a, sort_key(x + 0.0f)), z = max(z, sort_key(x + 0.0f));
+            });
+            a = __reduce_min_sync(0xffffffffu, a), z = __reduce_max_sync(0xffffffffu, z);
+            __syncthreads();
+            if (lane == 0) sh->warp[warp] = ((u64)a << 32) | z;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                for (int i = 0; i < SF_W; ++i) a = min(a, (uint32_t)(sh->warp[i] >> 32)), z = max(z, (uint32_t)sh->warp[i]);
+                for (int i = 0; i < n_cta; ++i) cl.map_shared_rank(sh, i)->lo[rank] = a, cl.map_shared_rank(sh, i)->hi[rank] = z;
+            }
+            cl.sync();
+            for (int i = 0; i < n_cta; ++i) a = min(a, sh->lo[i]), z = max(z, sh->hi[i]);
+            lo = a, hi = z, by_bin = false;
+            if (lo == hi) {      // equal values: so many of them by index
+                long long q = count - kept;
+                if (weights) {
+                    const u64 one = w(key_value(lo));
+                    const double left = (double)top_p * (double)*total - (double)before;
+                    q = one ? (long long)ceil(left / (double)one) : inside;
+                }
+                q = min((long long)inside, max(1ll, q));
+                int mine = 0;
+                each([&](float x, int i) { mine += in(x, i); });
+                mine = __reduce_add_sync(0xffffffffu, mine);
+                __syncthreads();
+                if (lane == 0) sh->warp[warp] = mine;
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    int n = 0;
+                    for (int i = 0; i < SF_W; ++i) n += (int)sh->warp[i];
+                    for (int i = 0; i < n_cta; ++i) cl.map_shared_rank(sh, i)->counts[rank] = n;
+                }
+                cl.sync();
+                long long ahead_of_me = 0;
+                for (int i = 0; i < rank; ++i) ahead_of_me += sh->counts[i];
+                for (int i = 0; i < warp; ++i) ahead_of_me += (long long)sh->warp[i];
+                if (ahead_of_me < q && ahead_of_me + mine >= q) {
+                    const float* x = xs + warp * p.seg;
+                    for (int i = lane; i < p.seg; i += 32) {
+                        const int index = base + warp * p.seg + i;
+                        const uint32_t there = __ballot_sync(0xffffffffu, in(x[i], index));
+                        if (ahead_of_me + __popc(there) >= q) {
+                            if ((there >> lane & 1) && ahead_of_me + __popc(there & ((2u << lane) - 1u)) == q) everywhere(&Shared::cut, token_key(x[i], index));
+                            break;
+                        }
+                        ahead_of_me += __popc(there);
+                    }
+                }
+                cl.sync();
+                return sh->cut;
+            }
+            // ---- 2048 parts of that range, falling
+            const u64 width = (u64)hi - lo + 1;
+            u64 t = *total;
+            histogram(weights, [&](float x, int i) { return in(x, i) ? (int)((u64)(hi - sort_key(x + 0.0f)) * SF_BINS / width) : -1; }, weights ? 0 : count - kept, top_p, before, &t, false);
+            const int part = sh->bin;
+            before = sh->before;
+            kept += (long long)sh->in_before;
+            inside = sh->inside;
+            // keys k with (hi - k) 2048 / width == part
+            const u64 first = ((u64)part * width + SF_BINS - 1) / SF_BINS, next = ((u64)(part + 1) * width + SF_BINS - 1) / SF_BINS;
+            const uint32_t top = hi;
+            hi = (uint32_t)(top - first), lo = (uint32_t)(top - (next - 1));
+        }
+    }
+
+    // Token, its probability and the distribution of the tokens at or above `cut` with weights of `least` at least (the first one always).
+    __device__ void draw(int row, u64 cut, u64 least, float u) {
+        auto kept = [&](float x, int i) -> u64 {
+            const u64 k = token_key(x, i);
+            if (!(x > -INFINITY) || k < cut) return 0ull;
+            const u64 v = w(x);
+            return v >= least || k == best ? v : 0ull;
+        };
+        u64 mine = 0;
+        each([&](float x, int i) { mine += kept(x, i); });
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, s);
+        __syncthreads();
+        if (lane == 0) sh->warp[warp] = mine;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            u64 v = 0;
+            for (int i = 0; i < SF_W; ++i) v += sh->warp[i];
+            for (int i = 0; i < n_cta; ++i) cl.map_shared_rank(sh, i)->part[rank] = v;
+        }
+        cl.sync();
+        u64 total = 0, ahead_of_me = 0;
+        for (int i = 0; i < n_cta; ++i) {
+            if (i < rank) ahead_of_me += sh->part[i];
+            total += sh->part[i];
+        }
+        for (int i = 0; i < warp; ++i) ahead_of_me += sh->warp[i];
+        const u64 goal = goal_of(u, total);
+        if (ahead_of_me <= goal && goal < ahead_of_me + mine) {
+            const float* x = xs + warp * p.seg;
+            for (int i = lane; i < p.seg; i += 32) {
+                const int index = base + warp * p.seg + i;
+                const u64 own = kept(x[i], index);
+                u64 v = own;
+#pragma unroll
+                for (int s = 1; s < 32; s <<= 1) {
+                    const u64 o = __shfl_up_sync(0xffffffffu, v, s);
+                    if (lane >= s) v += o;
+                }
+                if (own && ahead_of_me + v - own <= goal && goal < ahead_of_me + v) put(row, index, own, total);
+                ahead_of_me += __shfl_sync(0xffffffffu, v, 31);
+                if (ahead_of_me > goal) break;
+            }
+        }
+        if (p.dist) distribution(row, cut, least, total);
+    }
+    // floor(u total): the draw is the first token up to which the sum is above it
+    __device__ static u64 goal_of(float u, u64 total) {
+        const float c = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+        return __umul64hi((u64)((double)c * 18446744073709551616.0), total);
+    }
+    __device__ void put(int row, int index, u64 own, u64 total) const {
+        p.token[row] = index;
+        if (p.p) p.p[row] = (float)((double)own / (double)total);
+    }
+    __device__ void distribution(int row, u64 cut, u64 least, u64 total) const {
+        const double inv = 1.0 / (double)total;
+        float* to = p.dist + (size_t)row * p.V;
+        each([&](float x, int i) {
+            if (i >= p.V) return;
+            const u64 k = token_key(x, i);
+            u64 v = 0;
+            if (x > -INFINITY && k >= cut) {
+                v = w(x);
+                if (v < least && k != best) v = 0;
+            }
+            to[i] = (float)((double)v * inv);
+        });
+    }
+
+    // CTA 0's sorted list holds all tokens down to the cut by number, or by weight of `total`: the filters and the draw.
+    __device__ void draw_list(int row, long long count, float top_p, u64 total, u64 least, float u) {
+        u64* list = wh;
+        u64* other = wh + SF_LIST;
+        const int n = min(sh->n_list, SF_LIST), t = threadIdx.x;
+        sort(list, n);
+        u64 own[2], pre[2];
+        ahead(list, n, own, pre);
+        if (count > 0) {      // the first `count` are the whole
+            const u64 in = (2 * t < count ? own[0] : 0) + (2 * t + 1 < count ? own[1] : 0);
+            total = block_sum(in);
+        }
+        const double goal = (double)top_p * (double)total;
+        int last = 0;
+        for (int i = 0; i < 2; ++i) {
+            const int at = 2 * t + i;
+            if (at < n && (count <= 0 || at < count) && (top_p >= 1.0f || (double)pre[i] < goal) && own[i] >= least) last = at;
+        }
+        __syncthreads();
+        if (t == 0) sh->found = 0;
+        __syncthreads();
+        if (last > 0) atomicMax(&sh->found, last);
+        __syncthreads();
+        const int keep = sh->found + 1;
+        const u64 whole = block_sum((2 * t < keep ? own[0] : 0) + (2 * t + 1 < keep ? own[1] : 0));
+        if (t == 0) sh->cut = list[keep - 1], sh->total = whole;
+        // the kept ones by rising index: largest first of (~index, place)
+        for (int i = t; i < keep; i += SF_T) other[i] = ((u64)(uint32_t)list[i] << 32) | (uint32_t)i;
+        sort(other, keep);
+        for (int i = 0; i < 2; ++i) own[i] = 2 * t + i < keep ? w(key_value((uint32_t)(list[(uint32_t)other[2 * t + i]] >> 32))) : 0;
+        const u64 upto = scan(own[0] + own[1]), target = goal_of(u, whole);
+        u64 a = upto - own[0] - own[1];
+        for (int i = 0; i < 2; ++i) {
+            if (own[i] && a <= target && target < a + own[i]) put(row, (int)~(uint32_t)(other[2 * t + i] >> 32), own[i], whole);
+            a += own[i];
+        }
+        __syncthreads();
+    }
+};
+
+template <typename TX>
+__global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    Sampler<TX> s(p);
+    s.rank = (int)s.cl.block_rank(), s.n_cta = (int)s.cl.num_blocks(), s.warp = threadIdx.x >> 5, s.lane = threadIdx.x & 31;
+    s.wh = reinterpret_cast<u64*>(smem);
+    s.cnt = reinterpret_cast<uint32_t*>(s.wh + SF_BINS);
+    s.sh = reinterpret_cast<Shared*>(s.cnt + SF_BINS);
+    s.xs = reinterpret_cast<float*>(s.sh + 1);
+    s.base = s.rank * SF_W * p.seg;
+    const int row = blockIdx.x / s.n_cta;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (threadIdx.x < 64) s.sh->table[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
+    // ---- the row's part, NaN as -inf; its largest token
+    const TX* src = reinterpret_cast<const TX*>(p.logits) + (size_t)row * p.ld;
+    u64 best = 0;
+    {
+        float* x = s.xs + s.warp * p.seg;
+        const int at0 = s.base + s.warp * p.seg;
+        auto take = [&](float v, int i) {
+            if (!(v > -INFINITY)) v = -INFINITY;
+            x[i] = v;
+            const u64 k = token_key(v, at0 + i);
+            if (v > -INFINITY && k > best) best = k;
+        };
+        constexpr int PER = 16 / sizeof(TX);
+        const bool vec = ((uintptr_t)(src + at0) & 15) == 0;
+        if (vec) {
+            for (int i = s.lane * PER; i < p.seg; i += 32 * PER) {
+                TX v[PER];
+                if (at0 + i + PER <= p.V) {
+                    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + at0 + i);
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) take((float)v[j], i + j);
+                } else {
+                    for (int j = 0; j < PER; ++j) take(at0 + i + j < p.V ? (float)src[at0 + i + j] : -INFINITY, i + j);
+                }
+            }
+        } else {
+            for (int i = s.lane; i < p.seg; i += 32) take(at0 + i < p.V ? (float)src[at0 + i] : -INFINITY, i);
+        }
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) {
+        const u64 o = __shfl_xor_sync(0xffffffffu, best, k);
+        best = o > best ? o : best;
+    }
+    if (s.lane == 0) s.sh->warp[s.warp] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < SF_W; ++i) best = s.sh->warp[i] > best ? s.sh->warp[i] : best;
+        for (int i = 0; i < s.n_cta; ++i) s.cl.map_shared_rank(s.sh, i)->best[s.rank] = best;
+    }
+    s.cl.sync();
+    best = 0;
+    for (int i = 0; i < s.n_cta; ++i) best = s.sh->best[i] > best ? s.sh->best[i] : best;
+    s.best = best;
+    const float T = p.temperature ? p.temperature[row] : 1.0f, top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.0f, u = p.u[row];
+    const int top_k = p.top_k ? p.top_k[row] : 0;
+    if (best == 0) {      // no token has a weight
+        if (s.rank == 0 && threadIdx.x == 0) {
+            p.token[row] = -1;
+            if (p.p) p.p[row] = 0.0f;
+        }
+        if (p.dist)
+            s.each([&](float, int i) { if (i < p.V) p.dist[(size_t)row * p.V + i] = 0.0f; });
+        s.cl.sync();
+        return;
+    }
+    const float most = key_value((uint32_t)(best >> 32));
+    s.w.most = (double)most, s.w.c = 1.4426950408889634 / (double)T, s.w.table = s.sh->table, s.w.infinite = most == INFINITY;
+    const long long count = top_k > 0 && top_k < p.V ? top_k : 0;
+    const bool by_weight = top_p < 1.0f;
+    const u64 least = min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 1.0f) * (double)SF_ONE) : 0ull;
+    if (!(T > 0.0f) || count == 1 || top_p <= 0.0f || min_p > 1.0f) {      // the first token alone
+        if (s.rank == 0 && threadIdx.x == 0) s.put(row, key_index(best), 1, 1);
+        if (p.dist) s.each([&](float x, int i) { if (i < p.V) p.dist[(size_t)row * p.V + i] = token_key(x, i) == best && x > -INFINITY ? 1.0f : 0.0f; });
+        s.cl.sync();
+        return;
+    }
+    if (!count && !by_weight) {
+        s.draw(row, 0, least, u);
+        s.cl.sync();
+        return;
+    }
+    // bins: 64 to a unit of the logits where the cut goes by number, 32 to a power of two of the weights where it goes by weight
+    s.to_bin = count ? 64.0f : fminf(32.0f * 1.44269504f / T, 1e30f);
+    if (s.w.infinite) s.to_bin = 0.0f;
+    u64 total = 0;
+    s.histogram(!count, [&](float x, int i) { return x > -INFINITY ? s.bin_of(x) : -1; }, count, top_p, 0, &total, !count);
+    total = s.sh->total;
+    const int bin = s.sh->bin;
+    if (s.sh->upto <= SF_LIST) {
+        s.gather([&](float x, int i) { return x > -INFINITY && s.bin_of(x) <= bin; });
+        if (s.rank == 0) s.draw_list(row, count, top_p, total, least, u);
+        if (p.dist) {
+            if (s.rank == 0 && threadIdx.x == 0) {
+                const u64 cut = s.sh->cut, whole = s.sh->total;
+                s.everywhere(&Shared::cut, cut);
+                s.everywhere(&Shared::total, whole);
+            }
+            s.cl.sync();
+            s.distribution(row, s.sh->cut, 0, s.sh->total);
+        }
+        s.cl.sync();
+        return;
+    }
+    u64 cut = 0;
+    if (count) cut = s.cut_at(0, count, 1.0f, &total);
+    if (by_weight) {
+        s.to_bin = s.w.infinite ? 0.0f : fminf(32.0f * 1.44269504f / T, 1e30f);
+        cut = s.cut_at(cut, 0, top_p, &total);
+    }
+    s.draw(row, cut, least, u);
+    s.cl.sync();
+}
+
+size_t sample_smem(int seg) { return SF_BINS * 12 + sizeof(Shared) + (size_t)SF_W * seg * 4; }
+
+template <typename TX>
+int launch_sample(dc_ctx* ctx, SampleParams p, int rows) {
+    // eight CTAs a row: two of them fit into an SM up to some 140 000 tokens
+    const int n = SF_CLUSTER;
+    p.seg = ((p.V + n * SF_W - 1) / (n * SF_W) + 31) / 32 * 32;
+    const size_t smem = sample_smem(p.seg);
+    DC_TRY(dc_kernel_setup(ctx, (const void*)k_sample_filter<TX>, (int)sample_smem(SF_MOST / SF_W), "k_sample_filter"));
+    return dc_launch_cluster(ctx, "k_sample_filter", k_sample_filter<TX>, dim3(rows * n), dim3(SF_T), smem, n, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_b200_sample_rows_dev(dc_ctx* ctx, const void* logits_dev, int type, int rows, int vocab, int64_t ld, const float* temperature_dev, const int32_t* top_k_dev,
+                            const float* top_p_dev, const float* min_p_dev, const float* uniforms_dev, int32_t* tokens_dev, float* p_dev, float* dist_dev) {
+    if (!ctx) return DC_B200_INVALID_ARGUMENT;
+    if (ld == 0) ld = vocab;
+    if (rows < 0 || vocab < 1 || ld < vocab) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "sample_rows: bad shape (%d rows of %d, stride %lld)", rows, vocab, (long long)ld);
+    if (type != DC_TYPE_F32 && type != DC_TYPE_BF16) return dc_fail(ctx, DC_B200_UNSUPPORTED, "sample_rows: logits of type %d (F32 and BF16 are supported)", type);
+    if (vocab > SF_MOST * SF_CLUSTER - SF_CLUSTER * SF_W * 32 || rows > (1 << 20)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "sample_rows: %d rows of %d tokens", rows, vocab);
+    if (rows == 0) return DC_B200_OK;
+    if (!logits_dev || !uniforms_dev || !tokens_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "sample_rows: null buffer");
+    cudaSetDevice(ctx->device);
+    SampleParams p = {logits_dev, (size_t)ld, vocab, 0, temperature_dev, top_k_dev, top_p_dev, min_p_dev, uniforms_dev, tokens_dev, p_dev, dist_dev};
+    return type == DC_TYPE_F32 ? launch_sample<float>(ctx, p, rows) : launch_sample<__nv_bfloat16>(ctx, p, rows);
+}
+
+int dc_b200_sample_rows(dc_ctx* ctx, const float* logits_host, int rows, int vocab, const float* temperature, const int32_t* top_k, const float* top_p,
+                        const float* min_p, const float* uniforms, int32_t* tokens_out, float* p_out, float* dist_out) {
+    if (!ctx) return DC_B200_INVALID_ARGUMENT;
+    if (!logits_host || !uniforms || !tokens_out || rows < 1 || vocab < 1) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "sample_rows: bad argument");
+    for (int i = 0; i < rows; ++i)
+        if (!(uniforms[i] >= 0.0f && uniforms[i] < 1.0f) || (temperature && !(temperature[i] >= 0.0f)) || (top_p && !(top_p[i] > 0.0f)) || (min_p && !(min_p[i] >= 0.0f && min_p[i] <= 1.0f)) ||
+            (top_k && top_k[i] < 0))
+            return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "sample_rows: row %d has a setting out of range", i);
+    cudaSetDevice(ctx->device);
+    const size_t big = (size_t)rows * vocab * 4, small = ((size_t)rows * 4 + 255) / 256 * 256, pad = (big + 255) / 256 * 256;
+    uint8_t* s = dc_scratch(ctx, pad * (dist_out ? 2 : 1) + 7 * small);
+    if (!s) return DC_B200_OUT_OF_MEMORY;
+    float* l = (float*)s;
+    uint8_t* at = s + pad + (dist_out ? pad : 0);
+    auto up = [&](const void* from) -> uint8_t* {      // (pageable sources: the copy is done with them when it returns)
+        uint8_t* to = at;
+        at += small;
+        if (from && cudaMemcpyAsync(to, from, (size_t)rows * 4, cudaMemcpyHostToDevice, ctx->stream) != cudaSuccess) return nullptr;
+        return from ? to : nullptr;
+    };
+    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(l, logits_host, big, cudaMemcpyHostToDevice, ctx->stream), "sample_rows"));
+    uint8_t *dt = up(temperature), *dk = up(top_k), *dp = up(top_p), *dm = up(min_p), *du = up(uniforms), *tok = at, *pr = at + small;
+    DC_TRY(dc_check_cuda(ctx, cudaGetLastError(), "sample_rows"));
+    DC_TRY(dc_b200_sample_rows_dev(ctx, l, DC_TYPE_F32, rows, vocab, 0, (float*)dt, (int32_t*)dk, (float*)dp, (float*)dm, (float*)du, (int32_t*)tok, (float*)pr,
+                                   dist_out ? (float*)(s + pad) : nullptr));
+    auto down = [&](void* to, const void* from, size_t n) { return to ? dc_check_cuda(ctx, cudaMemcpyAsync(to, from, n, cudaMemcpyDeviceToHost, ctx->stream), "sample_rows") : DC_B200_OK; };
+    DC_TRY(down(tokens_out, tok, (size_t)rows * 4));
+    DC_TRY(down(p_out, pr, (size_t)rows * 4));
+    DC_TRY(down(dist_out, s + pad, big));
+    return dc_b200_synchronize(ctx);
+}
+
+}  // extern "C"

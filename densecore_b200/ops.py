@@ -214,6 +214,39 @@ class Context:
                                                      gamma, vocab, mode, temperature, C.byref(n), C.byref(t)))
         return n.value, t.value
 
+    def sample_rows_dev(self, logits: int, rows: int, vocab: int, temperature: int, top_k: int, top_p: int, min_p: int, uniforms: int, tokens: int, p: int = 0,
+                        dist: int = 0, ld: int = 0, dtype: str = "f32"):
+        """One token a row from device-resident logits; settings and results are device addresses (settings 0: not used), enqueue only."""
+        self._check(_lib.lib().dc_b200_sample_rows_dev(self.handle, _dev(logits), _row_type(dtype), rows, vocab, ld, _dev(temperature), _dev(top_k), _dev(top_p),
+                                                       _dev(min_p), _dev(uniforms), _dev(tokens), _dev(p), _dev(dist)))
+
+    def sample_rows(self, logits: np.ndarray, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, want_dist: bool = False):
+        """One token a row by temperature, top-k, top-p and min-p (scalars or one value a row).  Returns (tokens, probabilities[, distributions])."""
+        logits = np.ascontiguousarray(np.atleast_2d(logits), dtype=np.float32)
+        rows, vocab = logits.shape
+
+        def per_row(v, t):
+            return None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype=t), (rows,)))
+
+        s = [per_row(temperature, np.float32), per_row(top_k, np.int32), per_row(top_p, np.float32), per_row(min_p, np.float32), per_row(uniforms, np.float32)]
+        tokens, p = np.zeros(rows, dtype=np.int32), np.zeros(rows, dtype=np.float32)
+        dist = np.empty_like(logits) if want_dist else None
+        self._check(_lib.lib().dc_b200_sample_rows(self.handle, _vp(logits), rows, vocab, *(_vp(x) for x in s), _vp(tokens), _vp(p), _vp(dist)))
+        return (tokens, p, dist) if want_dist else (tokens, p)
+
+    # ---- adapters
+    def lora(self, K: int, N: int, max_adapters: int, max_rank: int, dtype: str = "bf16") -> "LoraSet":
+        """Low-rank adapters of a matrix of N x K; dtype: type of their matrices ("bf16", "f16")."""
+        return LoraSet(self, K, N, max_adapters, max_rank, dtype)
+
+    def lora_add_dev(self, lora: "LoraSet", x: int, M: int, ids: int, y: int, base_dev: int = 0, ld_x: int = 0, ld_base: int = 0, ld_y: int = 0):
+        """y = base + each row's adapter of x (base 0: y holds it); device addresses, enqueue only."""
+        self._check(_lib.lib().dc_b200_lora_add_dev(self.handle, lora.handle, _dev(x), ld_x, M, _dev(ids), _dev(base_dev), ld_base, _dev(y), ld_y))
+
+    def mul_mat_lora_dev(self, w: Weight, lora: "LoraSet", x: int, M: int, ids: int, y: int):
+        """mul_mat_dev with each row's adapter on top."""
+        self._check(_lib.lib().dc_b200_mul_mat_lora_dev(self.handle, w.handle, lora.handle, _dev(x), M, _dev(ids), _dev(y)))
+
     # ---- paged KV
     def kv_cache(self, n_layer: int, n_kv_head: int, head_dim: int, max_blocks: int, max_seqs: int,
                  max_blocks_per_seq: int) -> "KVCache":
@@ -223,6 +256,46 @@ class Context:
                     dtype: str = "f32") -> "KVCacheQ4":
         """Cache in 4 bits for layers of n_head query heads; dtype: rows of queries, keys, values and results ("f32", "bf16")."""
         return KVCacheQ4(self, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, dtype)
+
+
+class LoraSet:
+    """Adapters of one matrix for many requests (dc_b200_lora_*)."""
+
+    def __init__(self, ctx: Context, K: int, N: int, max_adapters: int, max_rank: int, dtype: str = "bf16"):
+        self.handle = None
+        self.ctx, self.K, self.N, self.dtype = ctx, K, N, dtype
+        h = C.c_void_p()
+        ctx._check(_lib.lib().dc_b200_lora_create(ctx.handle, K, N, max_adapters, max_rank, _row_type(dtype), C.byref(h)))
+        self.handle = h
+
+    def close(self):
+        if self.handle:
+            _lib.lib().dc_b200_lora_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self.ctx.handle:
+                self.close()
+        except Exception:
+            pass
+
+    def set(self, slot: int, A: np.ndarray, B: np.ndarray, scale: float = 1.0):
+        """A [rank, K] and B [N, rank]: float16 for "f16", bits (uint16) for "bf16"."""
+        t = _HOST_ROWS[self.dtype]
+        if A.dtype != t or B.dtype != t:
+            raise ValueError(f"matrices of type {A.dtype}, {B.dtype}; {np.dtype(t)} is wanted")
+        if A.ndim != 2 or A.shape[1] != self.K or B.shape != (self.N, A.shape[0]):
+            raise ValueError(f"matrices of shape {A.shape}, {B.shape} beside one of {self.N} x {self.K}")
+        A, B = np.ascontiguousarray(A), np.ascontiguousarray(B)
+        self.ctx._check(_lib.lib().dc_b200_lora_set(self.handle, slot, A.shape[0], _vp(A), _vp(B), scale))
+
+    def set_dev(self, slot: int, rank: int, A: int, B: int, scale: float = 1.0):
+        """The same from device addresses, enqueue only."""
+        self.ctx._check(_lib.lib().dc_b200_lora_set_dev(self.handle, slot, rank, _dev(A), _dev(B), scale))
+
+    def clear(self, slot: int):
+        self.ctx._check(_lib.lib().dc_b200_lora_set_dev(self.handle, slot, 0, None, None, 0.0))
 
 
 class KVCache:

@@ -287,6 +287,44 @@ DC_B200_API int dc_b200_sample_dev(dc_ctx* ctx, const float* logits_dev, int voc
 DC_B200_API int dc_b200_softmax(dc_ctx* ctx, const float* logits_host, int rows, int n, float temperature,
                                 float* probs_host);
 
+/* One token for each of many rows of logits, every row with settings of its own (SampleToken's temperature, top-k and
+ * top-p, core/src/sampler/sampler.cpp:235-262, and min-p).  The order of a row's tokens is by falling logit, equal ones by
+ * rising index.  Kept is a beginning of it: the first top_k (0 or less: all); of these the shortest beginning that holds a share top_p
+ * of their weights exp((logit - largest) / temperature) (1 or more: all, 0 or less: the first); of these the ones with weights of min_p
+ * at least; the first token always.  The draw is the first kept token, by index, up to which the kept weights' sum is above
+ * uniform times their whole sum.  A temperature that is not above 0 takes the first token.  -inf and NaN have no
+ * weight; a row without any weight gives token -1.  Weights are whole numbers of 2^-44, so that results do not
+ * depend on the order of sums.  logits_dev: [rows][vocab], rows ld elements apart (0: dense), type DC_GGML_TYPE_F32 or
+ * DC_GGML_TYPE_BF16, at most 389120 tokens a row.  temperature, top_k, top_p, min_p: [rows], each may be NULL (1, all, all, none).  uniforms_dev:
+ * [rows] in [0, 1).  Results: tokens_dev [rows]; p_dev [rows] (may be NULL), the token's probability among the kept; dist_dev
+ * [rows][vocab] f32 (may be NULL), the distribution drawn from, as a later dc_b200_verify_accept_dev (mode 1) needs it.  Only enqueues. */
+DC_B200_API int dc_b200_sample_rows_dev(dc_ctx* ctx, const void* logits_dev, int type, int rows, int vocab, int64_t ld, const float* temperature_dev,
+                                        const int32_t* top_k_dev, const float* top_p_dev, const float* min_p_dev, const float* uniforms_dev,
+                                        int32_t* tokens_dev, float* p_dev, float* dist_dev);
+/* The same on host arrays (dense f32 rows); refuses settings out of range: temperature < 0, top_k < 0, top_p <= 0, min_p
+ * outside [0, 1], uniforms outside [0, 1), NaN. */
+DC_B200_API int dc_b200_sample_rows(dc_ctx* ctx, const float* logits_host, int rows, int vocab, const float* temperature, const int32_t* top_k,
+                                    const float* top_p, const float* min_p, const float* uniforms, int32_t* tokens_out, float* p_out,
+                                    float* dist_out);
+
+/* ---- low-rank adapters beside a shared product -------------------------------- */
+/* A set of adapters of one matrix [N, K] for many requests at once (no counterpart in DenseCore): slot a holds A [rank, K]
+ * and B [N, rank], DC_GGML_TYPE_BF16 or DC_GGML_TYPE_F16, and a scale; ranks may differ, max_rank at most.  Matrices are copied into a layout of the set's own. */
+typedef struct dc_lora dc_lora;
+DC_B200_API int dc_b200_lora_create(dc_ctx* ctx, int64_t K, int64_t N, int max_adapters, int max_rank, int type, dc_lora** out);
+DC_B200_API void dc_b200_lora_destroy(dc_lora* l);
+/* Fills a slot (rank 0: empties it).  The _dev form only enqueues: the matrices have to stay until the stream has got there. */
+DC_B200_API int dc_b200_lora_set(dc_lora* l, int slot, int rank, const void* a_host, const void* b_host, float scale);
+DC_B200_API int dc_b200_lora_set_dev(dc_lora* l, int slot, int rank, const void* a_dev, const void* b_dev, float scale);
+/* y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T with a = ids_dev[t]; a row whose id names no filled slot gives base[t].  x [M][K], base and y
+ * [M][N] f32, rows ld_* elements apart (0: dense).  base_dev NULL: y_dev holds it; base and y are the same rows or do not overlap, x and y
+ * do not overlap.  Sums and the rank-sized rows between the two products are f32, each row's result depends on its own adapter alone.  Only enqueues; the set's workspace
+ * grows with M (a call that needs more than any before cannot be captured), and calls on one set must not overlap in time. */
+DC_B200_API int dc_b200_lora_add_dev(dc_ctx* ctx, dc_lora* l, const float* x_dev, int64_t ld_x, int M, const int32_t* ids_dev, const float* base_dev,
+                                     int64_t ld_base, float* y_dev, int64_t ld_y);
+/* dc_b200_mul_mat_dev, then the rows' adapters on top (x and y must not overlap). */
+DC_B200_API int dc_b200_mul_mat_lora_dev(dc_ctx* ctx, const dc_weight* w, dc_lora* l, const float* x_dev, int M, const int32_t* ids_dev, float* y_dev);
+
 /* ---- decoder: the ops above chained into one model step --------------------- */
 /* The graph BuildTransformerGraph lays out for a Qwen3-style decoder
  * (core/src/llm/graph/decoder.cpp:1085-1100 QKV, :1265-1343 Q/K norm, :1422-1450
