@@ -6,9 +6,11 @@
 // additions, so that atomics in any order give the same result, and a border between two tokens moves by 2^-44 times the number of tokens at most.
 //
 // One cluster of CTAs per row: the row lies in their shared memory, a contiguous part each, and is read from HBM once.
-//   1. the largest token;  2. a histogram of 2048 bins of falling value (numbers, and weights where the cut goes by weight) finds the bin with the cut;
-//   3. up to 1024 tokens down to that bin: they are sorted in one CTA, which applies all filters and draws;
-//   else the bin is refined to the cut's key, and 4. all CTAs sum the kept weights of their parts and the part with the draw is searched.
+//   a cut by number: the threads' largest tokens, in a histogram of 2048 bins of falling value, give a bin that the cut cannot lie beyond;
+//   a cut by weight: a histogram of numbers (32-bit atomics; sums of 64 bits in shared memory took ten times as long) bounds the weights ahead of every bin from both
+//   sides, between which the cut lies;
+//   up to 1024 tokens down to there: they are sorted in one CTA, which applies all filters and draws;
+//   else the bins between the bounds are refined until 1024 tokens or one value is left, and the part of the row with the draw is searched.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -53,32 +55,37 @@ __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(
 __device__ __forceinline__ u64 token_key(float x, int index) { return ((u64)sort_key(x + 0.0f) << 32) | (uint32_t)~index; }      // (-0 and 0 are equal)
 __device__ __forceinline__ int key_index(u64 k) { return (int)~(uint32_t)k; }
 
-// exp2 in 64 bits: 2^(k / 64) from a table times a polynomial of degree 4 (Taylor, |r| <= 1/128: 4e-14), rounded to whole numbers of 2^-44.
+// exp2 in 64 bits: 2^(k / 256) from a table times a polynomial of degree 3 (Taylor, |r| <= 1/512: 1.4e-13), rounded to whole numbers of 2^-44.
 struct Weigher {
     double most, c;      // largest logit, log2(e) / T
     const double* table;
     bool infinite;
     __device__ __forceinline__ u64 operator()(float x) const {
         if (infinite) return x == INFINITY ? SF_ONE : 0ull;
-        if (!(x > -INFINITY)) return 0ull;
-        const double y = ((double)x - most) * c;
-        if (!(y > -46.0)) return 0ull;
-        const double t = y + 105553116266496.0;      // 1.5 2^46: to the nearest 64th
+        const double d = (double)x - most;
+        const double t = fma(d, c, 26388279066624.0);      // 1.5 2^44: to the nearest 256th
+        if (!(t > 26388279066624.0 - 46.0) || !(x > -INFINITY)) return 0ull;
         const int k = __double2loint(t);
-        const double r = y - (t - 105553116266496.0);
-        const double q = fma(r, fma(r, fma(r, fma(r, 0.0096181291076284772, 0.055504108664821580), 0.24022650695910071), 0.69314718055994531), 1.0);
-        const double v = table[k & 63] * q;
-        const double w = __hiloint2double(__double2hiint(v) + ((k >> 6) << 20), __double2loint(v)) + 256.0;      // units of 2^-44
+        const double r = fma(d, c, 26388279066624.0 - t);
+        const double q = fma(r, fma(r, fma(r, 0.055504108664821580, 0.24022650695910071), 0.69314718055994531), 1.0);
+        const double v = table[k & 255];
+        const double w = fma(__hiloint2double(__double2hiint(v) + ((k >> 8) << 20), __double2loint(v)), q, 256.0);      // units of 2^-44
         return (u64)__double_as_longlong(w) - 0x4070000000000000ull;
     }
+    // bounds on weights in a bin of `per` bins to a power of two, the rounding of the bin's number included (2048 / per 2^-22 < 2^-14 of the exponent)
+    __device__ __forceinline__ static double above(float b, float per) { return exp2((double)(-b / per) + 0.0001) * (double)SF_ONE + 1.0; }
+    __device__ __forceinline__ static double below(float b, float per) { return fmax(exp2((double)(-(b + 1.0f) / per) - 0.0001) * (double)SF_ONE - 1.0, 0.0); }
 };
 
-struct Shared {      // beside the row and the histogram
-    double table[64];
+struct alignas(16) Shared {      // beside the row and the histogram
+    double table[256];
     u64 best[SF_CLUSTER], warp[SF_W], part[SF_CLUSTER];
-    u64 cut, total, before, in_before;
+    u64 cut, total, in_before;
     uint32_t lo[SF_CLUSTER], hi[SF_CLUSTER];
-    int bin, upto, inside, n_list, found, counts[SF_CLUSTER];
+    double dwarp[SF_W];
+    int first[2];
+    int bin, bin2, upto, inside, n_list, drawn, counts[SF_CLUSTER];
+    float drawn_p;
 };
 
 template <typename TX>
@@ -91,7 +98,7 @@ struct Sampler {
     Shared* sh;
     int rank, n_cta, warp, lane, base;      // base: token index of xs[0]
     Weigher w;
-    float to_bin;
+    float to_bin, top;      // top: the largest of this thread's tokens as they were read
     u64 best;
 
     __device__ Sampler(const SampleParams& p_) : p(p_) {}
@@ -100,6 +107,7 @@ struct Sampler {
     template <typename F>
     __device__ __forceinline__ void each(F f) const {      // f(value, index) of this warp's tokens that have a value; whole warps
         const float* x = xs + warp * p.seg;
+#pragma unroll 4
         for (int i = lane; i < p.seg; i += 32) f(x[i], base + warp * p.seg + i);
     }
     __device__ u64 block_sum(u64 v) const {      // in all threads
@@ -125,6 +133,27 @@ struct Sampler {
     __device__ void everywhere(T Shared::* at, T v) {      // (one thread)
         for (int i = 0; i < n_cta; ++i) cl.map_shared_rank(sh, i)->*at = v;
     }
+    __device__ int block_last(int v) const {      // the largest, in all threads
+        v = __reduce_max_sync(0xffffffffu, v);
+        __syncthreads();
+        if (lane == 0) sh->warp[warp] = (u64)(v + 1);
+        __syncthreads();
+        u64 m = 0;
+        for (int i = 0; i < SF_W; ++i) m = sh->warp[i] > m ? sh->warp[i] : m;
+        return (int)m - 1;
+    }
+    __device__ double scan(double v) const {
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const double o = __shfl_up_sync(0xffffffffu, v, s);
+            if (lane >= s) v += o;
+        }
+        __syncthreads();
+        if (lane == 31) sh->dwarp[warp] = v;
+        __syncthreads();
+        for (int i = 0; i < warp; ++i) v += sh->dwarp[i];
+        return v;
+    }
     // inclusive sums of a value a thread, over the CTA
     __device__ u64 scan(u64 v) const {
 #pragma unroll
@@ -139,73 +168,119 @@ struct Sampler {
         return v;
     }
 
-    // Numbers (and weights) per bin of the tokens that `bin` gives a bin >= 0; their sums in CTA 0, which looks for the bin with the cut: the one that holds the
-    // count-th token (count > 0), or the one where `goal` is reached by the weights on top of `before`.  Everyone then has bin, upto (tokens down to
-    // and with the bin), inside (tokens in it), before (weights ahead of it) and in_before (tokens ahead of it).
+    // Numbers of `fill`'s calls per bin, summed up over the cluster in CTA 0's cnt.
     template <typename F>
-    __device__ void histogram(bool weights, F bin, long long count, float top_p, u64 before, u64* total, bool total_wanted) {
-        for (int i = threadIdx.x; i < SF_BINS; i += SF_T) cnt[i] = 0, wh[i] = 0;
+    __device__ void histogram(F fill) {
+        for (int i = threadIdx.x; i < SF_BINS; i += SF_T) cnt[i] = 0;
         __syncthreads();
-        each([&](float x, int i) {
-            const int b = bin(x, i);
-            if (b >= 0) {
-                atomicAdd(cnt + b, 1u);
-                if (weights) {
-                    const u64 v = w(x);
-                    if (v) atomicAdd(wh + b, v);
-                }
-            }
-        });
+        fill();
         cl.sync();
         for (int b = rank + n_cta * threadIdx.x; b < SF_BINS; b += n_cta * SF_T) {      // every CTA sums up its share of the bins
-            uint32_t n = 0;
-            u64 v = 0;
-            for (int i = 0; i < n_cta; ++i) {
-                n += cl.map_shared_rank(cnt, i)[b];
-                if (weights) v += cl.map_shared_rank(wh, i)[b];
-            }
-            cl.map_shared_rank(cnt, 0)[b] = n;
-            if (weights) cl.map_shared_rank(wh, 0)[b] = v;
+            uint32_t n[SF_CLUSTER], all = 0;
+#pragma unroll
+            for (int i = 0; i < SF_CLUSTER; ++i) n[i] = i < n_cta ? cl.map_shared_rank(cnt, i)[b] : 0;
+#pragma unroll
+            for (int i = 0; i < SF_CLUSTER; ++i) all += n[i];
+            cl.map_shared_rank(cnt, 0)[b] = all;
         }
         cl.sync();
-        if (rank == 0) {
-            constexpr int B = SF_BINS / SF_T;
-            uint32_t n[B];
-            u64 v[B], sn = 0, sv = 0;
-            for (int i = 0; i < B; ++i) {
-                n[i] = cnt[B * threadIdx.x + i], v[i] = weights ? wh[B * threadIdx.x + i] : 0;
-                sn += n[i], sv += v[i];
+    }
+    // CTA 0, after histogram(): to everyone, bin = the first bin at which the number of tokens reaches `count` (or the last one with a token), upto = the number of
+    // tokens down to and with it, in_before = ahead of it, inside = in it.
+    __device__ void find_count(long long count) {
+        constexpr int B = SF_BINS / SF_T;
+        uint32_t n[B];
+        u64 sn = 0;
+        int last = -1;      // of the CTA's last bin with a token
+        for (int i = 0; i < B; ++i) {
+            n[i] = cnt[B * threadIdx.x + i];
+            sn += n[i];
+            if (n[i]) last = B * (int)threadIdx.x + i;
+        }
+        u64 an = scan(sn) - sn;
+        last = block_last(last);
+        for (int i = 0; i < B; ++i) {
+            const int b = B * (int)threadIdx.x + i;
+            if (((long long)an < count && (long long)(an + n[i]) >= count) || (b == last && (long long)(an + n[i]) < count)) {
+                everywhere(&Shared::bin, b);
+                everywhere(&Shared::bin2, b);
+                everywhere(&Shared::upto, (int)(an + n[i]));
+                everywhere(&Shared::inside, (int)n[i]);
+                everywhere(&Shared::in_before, an);
             }
-            u64 an = scan(sn) - sn, av = scan(sv);
-            const u64 all = block_sum(sv);
-            av -= sv;
-            if (total_wanted && threadIdx.x == 0) everywhere(&Shared::total, all);
-            const double goal = (double)top_p * (double)(total_wanted ? all : *total);
-            int last = -1;      // of the CTA's last bin with a token: taken if no bin reaches the cut
-            for (int i = 0; i < B; ++i)
-                if (n[i]) last = B * (int)threadIdx.x + i;
-            __syncthreads();
-            if (threadIdx.x == 0) sh->found = -1;
-            __syncthreads();
-            if (last >= 0) atomicMax(&sh->found, last);
-            __syncthreads();
-            const int fall_back = sh->found;
-            for (int i = 0; i < B; ++i) {
-                const int b = B * (int)threadIdx.x + i;
-                bool here;
-                if (count > 0) here = (long long)an < count && (long long)(an + n[i]) >= count;
-                else here = n[i] && (double)(before + av) < goal && (double)(before + av + v[i]) >= goal;
-                if (count > 0 ? here || (b == fall_back && (long long)(an + n[i]) < count) : here || (b == fall_back && (double)(before + av + v[i]) < goal)) {
-                    everywhere(&Shared::bin, b);
-                    everywhere(&Shared::upto, (int)(an + n[i]));
-                    everywhere(&Shared::inside, (int)n[i]);
-                    everywhere(&Shared::before, before + av);
-                    everywhere(&Shared::in_before, an);
+            an += n[i];
+        }
+    }
+    // The same for a cut where the weights' sum on top of `before` reaches `goal`, hi(b) and lo(b) bounds on a weight in bin b: bin = the first bin that may reach it,
+    // bin2 = the first one that does for sure (or the last one with a token); upto = tokens down to bin2, inside = in bin .. bin2, in_before = ahead of bin.
+    template <typename H, typename L>
+    __device__ void find_weight(double before, double goal, H hi, L lo) {
+        constexpr int B = SF_BINS / SF_T;
+        uint32_t n[B];
+        double uh = 0.0, ul = 0.0;
+        u64 sn = 0;
+        int last = -1;
+        for (int i = 0; i < B; ++i) {
+            const int b = B * (int)threadIdx.x + i;
+            n[i] = cnt[b];
+            sn += n[i];
+            if (n[i]) uh += n[i] * hi(b), ul += n[i] * lo(b), last = b;
+        }
+        u64 an = scan(sn) - sn;
+        double ah = scan(uh) - uh + before, al = scan(ul) - ul + before;
+        last = block_last(last);
+        const double may = goal * (1.0 - 1e-9), sure = goal * (1.0 + 1e-9);      // (these sums are rounded)
+        if (threadIdx.x == 0) sh->first[0] = sh->first[1] = SF_BINS;
+        __syncthreads();
+        int f[2] = {SF_BINS, SF_BINS};
+        double h = ah, l = al;
+        for (int i = 0; i < B; ++i) {
+            const int b = B * (int)threadIdx.x + i;
+            if (!n[i]) continue;
+            h += n[i] * hi(b), l += n[i] * lo(b);
+            if (h >= may && f[0] == SF_BINS) f[0] = b;
+            if (l >= sure && f[1] == SF_BINS) f[1] = b;
+        }
+        for (int i = 0; i < 2; ++i) {
+            f[i] = __reduce_min_sync(0xffffffffu, f[i]);
+            if (lane == 0 && f[i] < SF_BINS) atomicMin(&sh->first[i], f[i]);
+        }
+        __syncthreads();
+        const int b0 = min(sh->first[0], last), b1 = min(sh->first[1], last);
+        for (int i = 0; i < B; ++i) {
+            const int b = B * (int)threadIdx.x + i;
+            if (b == b0) {
+                everywhere(&Shared::bin, b);
+                everywhere(&Shared::in_before, an);
+            }
+            an += n[i];
+            if (b == b1) {
+                everywhere(&Shared::bin2, b);
+                everywhere(&Shared::upto, (int)an);
+            }
+        }
+    }
+
+    // For a cut by weight among the tokens at or above `from`: their number per bin and the sum of their weights (returned), then find_weight().
+    __device__ u64 weigh_and_count(u64 from, float per_unit, float top_p) {
+        u64 sum = 0;
+        histogram([&] {
+            each([&](float x, int i) {
+                if (x > -INFINITY && token_key(x, i) >= from) {
+                    atomicAdd(cnt + bin_of(x), 1u);
+                    sum += w(x);
                 }
-                an += n[i], av += v[i];
-            }
+            });
+        });
+        sum = cluster_sum(sum);
+        if (rank == 0) {
+            // (bins that are not 32 to a power of two, at extreme temperatures, bound nothing from below)
+            const bool bounded = per_unit < 1e30f && !w.infinite;
+            find_weight(0.0, (double)top_p * (double)sum, [&](int b) { return bounded ? w.above((float)b, 32.0f) : (double)SF_ONE; },
+                        [&](int b) { return bounded && b < SF_BINS - 1 ? w.below((float)b, 32.0f) : 0.0; });
         }
         cl.sync();
+        return sum;
     }
 
     // The keys of tokens that `take` names, into CTA 0's list (unordered); its length in CTA 0's n_list.
@@ -248,24 +323,34 @@ struct Sampler {
         pre[1] = pre[0] + own[0];
     }
 
-    // The key of the last token that a cut by number (count > 0) or by weight keeps, among the tokens at or above `from`; `total`: the sum of their weights if the
-    // caller wants it or the cut goes by weight.
-    __device__ u64 cut_at(u64 from, long long count, float top_p, u64* total) {
+    // The key of the last token that a cut by number (count > 0) or by weight keeps, among the tokens at or above `from`, once histogram() and find_*() have
+    // run.  total: the sum of their weights, for a cut by weight.  *mine: weights of this thread's tokens that are kept, ahead of the cut's own bin.
+    __device__ u64 cut_at(u64 from, long long count, float top_p, u64 total, u64* mine) {
         const bool weights = count <= 0;
-        histogram(weights, [&](float x, int i) { return x > -INFINITY && token_key(x, i) >= from ? bin_of(x) : -1; }, count, top_p, 0, total, weights);
-        if (weights) *total = sh->total;
-        const int b = sh->bin;
+        const double goal = (double)top_p * (double)total;
+        const int b0 = sh->bin, b1 = sh->bin2;
         uint32_t lo = 0, hi = 0xFFFFFFFFu;
         bool by_bin = true;
         auto in = [&](float x, int i) {
             if (!(x > -INFINITY) || token_key(x, i) < from) return false;
+            if (by_bin) {
+                const int b = bin_of(x);
+                return b >= b0 && b <= b1;
+            }
             const uint32_t k = sort_key(x + 0.0f);
-            return by_bin ? bin_of(x) == b : k >= lo && k <= hi;
+            return k >= lo && k <= hi;
         };
-        u64 before = sh->before;      // weights and tokens surely kept
-        long long kept = (long long)sh->in_before;
-        int inside = sh->inside;
-        for (;;) {
+        long long kept = (long long)sh->in_before;      // tokens surely kept
+        int inside = weights ? sh->upto - (int)kept : sh->inside;
+        u64 before = 0;                                 // their weights
+        *mine = 0;
+        if (weights) {
+            u64 sum = 0;
+            each([&](float x, int i) { if (x > -INFINITY && token_key(x, i) >= from && bin_of(x) < b0) sum += w(x); });
+            *mine = sum;
+            before = cluster_sum(sum);
+        }
+        for (int round = 0; round < 64; ++round) {      // (each leaves half of 2^32 values at most; equal ones end it)
             if (inside <= SF_LIST) {
                 gather(in);
                 if (rank == 0) {
@@ -276,18 +361,15 @@ struct Sampler {
                     int last = -1;
                     for (int i = 0; i < 2; ++i) {
                         const int at = 2 * threadIdx.x + i;
-                        if (at < n && (weights ? at == 0 || (double)(before + pre[i]) < (double)top_p * (double)*total : kept + at < count)) last = at;
+                        if (at < n && (weights ? at == 0 || (double)(before + pre[i]) < goal : kept + at < count)) last = at;
                     }
-                    if (threadIdx.x == 0) sh->found = 0;
-                    __syncthreads();
-                    if (last > 0) atomicMax(&sh->found, last);
-                    __syncthreads();
-                    if (threadIdx.x == 0) everywhere(&Shared::cut, wh[sh->found]);
+                    last = block_last(last);
+                    if (threadIdx.x == 0) everywhere(&Shared::cut, wh[max(last, 0)]);
                 }
                 cl.sync();
-                return sh->cut;
+                break;
             }
-            // ---- the values' range in the bin
+            // ---- the values' range
             uint32_t a = 0xFFFFFFFFu, z = 0;
             each([&](float x, int i) {
                 if (in(x, i)) a = min(a, sort_key(x + 0.0f)), z = max(z, sort_key(x + 0.0f));
@@ -307,26 +389,25 @@ struct Sampler {
                 long long q = count - kept;
                 if (weights) {
                     const u64 one = w(key_value(lo));
-                    const double left = (double)top_p * (double)*total - (double)before;
-                    q = one ? (long long)ceil(left / (double)one) : inside;
+                    q = one ? (long long)ceil((goal - (double)before) / (double)one) : inside;
                 }
                 q = min((long long)inside, max(1ll, q));
-                int mine = 0;
-                each([&](float x, int i) { mine += in(x, i); });
-                mine = __reduce_add_sync(0xffffffffu, mine);
+                int n = 0;
+                each([&](float x, int i) { n += in(x, i); });
+                n = __reduce_add_sync(0xffffffffu, n);
                 __syncthreads();
-                if (lane == 0) sh->warp[warp] = mine;
+                if (lane == 0) sh->warp[warp] = n;
                 __syncthreads();
                 if (threadIdx.x == 0) {
-                    int n = 0;
-                    for (int i = 0; i < SF_W; ++i) n += (int)sh->warp[i];
-                    for (int i = 0; i < n_cta; ++i) cl.map_shared_rank(sh, i)->counts[rank] = n;
+                    int all = 0;
+                    for (int i = 0; i < SF_W; ++i) all += (int)sh->warp[i];
+                    for (int i = 0; i < n_cta; ++i) cl.map_shared_rank(sh, i)->counts[rank] = all;
                 }
                 cl.sync();
                 long long ahead_of_me = 0;
                 for (int i = 0; i < rank; ++i) ahead_of_me += sh->counts[i];
                 for (int i = 0; i < warp; ++i) ahead_of_me += (long long)sh->warp[i];
-                if (ahead_of_me < q && ahead_of_me + mine >= q) {
+                if (ahead_of_me < q && ahead_of_me + n >= q) {
                     const float* x = xs + warp * p.seg;
                     for (int i = lane; i < p.seg; i += 32) {
                         const int index = base + warp * p.seg + i;
@@ -339,25 +420,71 @@ struct Sampler {
                     }
                 }
                 cl.sync();
-                return sh->cut;
+                break;
             }
-            // ---- 2048 parts of that range, falling
+            // ---- 2048 parts of that range, falling: keys k with (hi - k) 2048 / width == part
             const u64 width = (u64)hi - lo + 1;
-            u64 t = *total;
-            histogram(weights, [&](float x, int i) { return in(x, i) ? (int)((u64)(hi - sort_key(x + 0.0f)) * SF_BINS / width) : -1; }, weights ? 0 : count - kept, top_p, before, &t, false);
-            const int part = sh->bin;
-            before = sh->before;
-            kept += (long long)sh->in_before;
-            inside = sh->inside;
-            // keys k with (hi - k) 2048 / width == part
-            const u64 first = ((u64)part * width + SF_BINS - 1) / SF_BINS, next = ((u64)(part + 1) * width + SF_BINS - 1) / SF_BINS;
             const uint32_t top = hi;
-            hi = (uint32_t)(top - first), lo = (uint32_t)(top - (next - 1));
+            auto edge = [&](int part) { return (uint32_t)(((u64)part * width + SF_BINS - 1) / SF_BINS); };      // least top - k of a part
+            histogram([&] {
+                each([&](float x, int i) {
+                    if (in(x, i)) atomicAdd(cnt + (int)((u64)(top - sort_key(x + 0.0f)) * SF_BINS / width), 1u);
+                });
+            });
+            if (rank == 0) {
+                if (weights)
+                    find_weight((double)before, goal, [&](int b) { return (double)w(key_value(top - edge(b))); }, [&](int b) { return (double)w(key_value(top - (edge(b + 1) - 1))); });
+                else
+                    find_count(count - kept);
+            }
+            cl.sync();
+            // ---- the bounds' parts; where they are far apart (weights that fall from 1 to 0 within a part), the half of them that has the cut: a round leaves
+            // half of the values' range at most
+            int p0 = sh->bin, p1 = sh->bin2;
+            kept += (long long)sh->in_before;
+            inside = sh->upto - (int)sh->in_before;
+            cl.sync();      // (what find_*() wrote has been read)
+            if (weights) {
+                uint32_t above = top - edge(p0);      // keys above it are surely kept
+                u64 sum = 0;
+                each([&](float x, int i) { if (in(x, i) && sort_key(x + 0.0f) > above) sum += w(x); });
+                *mine += sum;
+                before += cluster_sum(sum);
+                if (p1 - p0 >= SF_BINS / 8) {
+                    const int half = (p0 + p1) / 2;
+                    const uint32_t mid = top - (edge(half + 1) - 1);      // least key of the upper half
+                    int n = 0;
+                    sum = 0;
+                    each([&](float x, int i) {
+                        const uint32_t k = sort_key(x + 0.0f);
+                        if (in(x, i) && k <= above && k >= mid) sum += w(x), ++n;
+                    });
+                    const u64 upper = cluster_sum(sum);
+                    const int n_upper = (int)cluster_sum((u64)n);
+                    if ((double)(before + upper) >= goal) {
+                        p1 = half, inside = n_upper;
+                    } else {
+                        *mine += sum;
+                        before += upper;
+                        p0 = half + 1, inside -= n_upper;
+                    }
+                }
+            }
+            const uint32_t new_hi = top - edge(p0), new_lo = top - (edge(p1 + 1) - 1);
+            hi = new_hi, lo = new_lo;
         }
+        const u64 cut = sh->cut;
+        if (weights) {
+            u64 sum = 0;
+            each([&](float x, int i) { if (in(x, i) && token_key(x, i) >= cut) sum += w(x); });
+            *mine += sum;
+        }
+        return cut;
     }
 
-    // Token, its probability and the distribution of the tokens at or above `cut` with weights of `least` at least (the first one always).
-    __device__ void draw(int row, u64 cut, u64 least, float u) {
+    // Token, its probability and the distribution of the tokens at or above `cut` with weights of `least` at least (the first one always).  mine: the sum of
+    // the weights of this thread's kept tokens, if known.
+    __device__ void draw(int row, u64 cut, u64 least, float u, const u64* known) {
         auto kept = [&](float x, int i) -> u64 {
             const u64 k = token_key(x, i);
             if (!(x > -INFINITY) || k < cut) return 0ull;
@@ -365,10 +492,11 @@ struct Sampler {
             return v >= least || k == best ? v : 0ull;
         };
         u64 mine = 0;
-        each([&](float x, int i) { mine += kept(x, i); });
+        if (known) mine = *known;
+        else each([&](float x, int i) { mine += kept(x, i); });
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, s);
-        __syncthreads();
+        cl.sync();      // (nobody still reads an earlier sum)
         if (lane == 0) sh->warp[warp] = mine;
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -384,6 +512,8 @@ struct Sampler {
         }
         for (int i = 0; i < warp; ++i) ahead_of_me += sh->warp[i];
         const u64 goal = goal_of(u, total);
+        int drawn = -1;      // in the warp that has it
+        float drawn_p = 0.0f;
         if (ahead_of_me <= goal && goal < ahead_of_me + mine) {
             const float* x = xs + warp * p.seg;
             for (int i = lane; i < p.seg; i += 32) {
@@ -395,34 +525,51 @@ struct Sampler {
                     const u64 o = __shfl_up_sync(0xffffffffu, v, s);
                     if (lane >= s) v += o;
                 }
-                if (own && ahead_of_me + v - own <= goal && goal < ahead_of_me + v) put(row, index, own, total);
+                if (own && ahead_of_me + v - own <= goal && goal < ahead_of_me + v) drawn = index, drawn_p = put(row, index, own, total);
                 ahead_of_me += __shfl_sync(0xffffffffu, v, 31);
                 if (ahead_of_me > goal) break;
             }
         }
-        if (p.dist) distribution(row, cut, least, total);
+        if (!p.dist) return;
+        const int has = __ffs(__ballot_sync(0xffffffffu, drawn >= 0)) - 1;
+        if (has >= 0) drawn = __shfl_sync(0xffffffffu, drawn, has), drawn_p = __shfl_sync(0xffffffffu, drawn_p, has);
+        distribution(row, cut, least, total, drawn, drawn_p);
     }
     // floor(u total): the draw is the first token up to which the sum is above it
     __device__ static u64 goal_of(float u, u64 total) {
         const float c = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
         return __umul64hi((u64)((double)c * 18446744073709551616.0), total);
     }
-    __device__ void put(int row, int index, u64 own, u64 total) const {
+    __device__ float put(int row, int index, u64 own, u64 total) const {
+        const float f = (float)((double)own / (double)total);
         p.token[row] = index;
-        if (p.p) p.p[row] = (float)((double)own / (double)total);
+        if (p.p) p.p[row] = f;
+        return f;
     }
-    __device__ void distribution(int row, u64 cut, u64 least, u64 total) const {
-        const double inv = 1.0 / (double)total;
+    // Probabilities are f32 results: exp2 in f32, its argument in two terms (2^-22 relative in all); the drawn token's is the one in p.
+    __device__ void distribution(int row, u64 cut, u64 least, u64 total, int drawn, float drawn_p) const {
+        const float inv = (float)((double)SF_ONE / (double)total), most = (float)w.most, c0 = (float)w.c, c1 = (float)(w.c - (double)c0);
+        const uint32_t cut_key = (uint32_t)(cut >> 32);
         float* to = p.dist + (size_t)row * p.V;
+        const bool plain = fabsf(c0) < 1e30f && fabsf(most) < 1e30f && c0 > 1e-30f && !w.infinite;
         each([&](float x, int i) {
             if (i >= p.V) return;
-            const u64 k = token_key(x, i);
-            u64 v = 0;
-            if (x > -INFINITY && k >= cut) {
-                v = w(x);
-                if (v < least && k != best) v = 0;
+            float f = 0.0f;
+            const uint32_t k = sort_key(x + 0.0f);
+            if (x > -INFINITY && k >= cut_key && (k > cut_key || token_key(x, i) >= cut)) {
+                if (plain && least == 0) {
+                    // x - most = d + e exactly
+                    const float d = x - most, b = d - x, e = (x - (d - b)) + (-most - b), y = d * c0;
+                    const float n = rintf(y), z = (y - n) + fmaf(e, c0, fmaf(d, c1, fmaf(d, c0, -y)));
+                    float g;
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(g) : "f"(z));
+                    f = n > -126.0f ? g * inv * __int_as_float(((int)n + 127) << 23) : 0.0f;
+                } else {
+                    const u64 v = w(x);
+                    f = v < least && token_key(x, i) != best ? 0.0f : (float)((double)v / (double)total);
+                }
             }
-            to[i] = (float)((double)v * inv);
+            to[i] = i == drawn ? drawn_p : f;
         });
     }
 
@@ -444,12 +591,7 @@ struct Sampler {
             const int at = 2 * t + i;
             if (at < n && (count <= 0 || at < count) && (top_p >= 1.0f || (double)pre[i] < goal) && own[i] >= least) last = at;
         }
-        __syncthreads();
-        if (t == 0) sh->found = 0;
-        __syncthreads();
-        if (last > 0) atomicMax(&sh->found, last);
-        __syncthreads();
-        const int keep = sh->found + 1;
+        const int keep = block_last(last) + 1;
         const u64 whole = block_sum((2 * t < keep ? own[0] : 0) + (2 * t + 1 < keep ? own[1] : 0));
         if (t == 0) sh->cut = list[keep - 1], sh->total = whole;
         // the kept ones by rising index: largest first of (~index, place)
@@ -459,7 +601,10 @@ struct Sampler {
         const u64 upto = scan(own[0] + own[1]), target = goal_of(u, whole);
         u64 a = upto - own[0] - own[1];
         for (int i = 0; i < 2; ++i) {
-            if (own[i] && a <= target && target < a + own[i]) put(row, (int)~(uint32_t)(other[2 * t + i] >> 32), own[i], whole);
+            if (own[i] && a <= target && target < a + own[i]) {
+                sh->drawn = (int)~(uint32_t)(other[2 * t + i] >> 32);
+                sh->drawn_p = put(row, sh->drawn, own[i], whole);
+            }
             a += own[i];
         }
         __syncthreads();
@@ -477,37 +622,53 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
     s.xs = reinterpret_cast<float*>(s.sh + 1);
     s.base = s.rank * SF_W * p.seg;
     const int row = blockIdx.x / s.n_cta;
+    for (int i = threadIdx.x; i < 256; i += SF_T) s.sh->table[i] = exp2((double)i * 0.00390625);
     pdl_wait();
     pdl_launch_dependents();
-    if (threadIdx.x < 64) s.sh->table[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
     // ---- the row's part, NaN as -inf; its largest token
     const TX* src = reinterpret_cast<const TX*>(p.logits) + (size_t)row * p.ld;
     u64 best = 0;
     {
         float* x = s.xs + s.warp * p.seg;
         const int at0 = s.base + s.warp * p.seg;
+        float top = -INFINITY;
+        int top_at = 0;
         auto take = [&](float v, int i) {
             if (!(v > -INFINITY)) v = -INFINITY;
-            x[i] = v;
-            const u64 k = token_key(v, at0 + i);
-            if (v > -INFINITY && k > best) best = k;
+            if (v > top) top = v, top_at = at0 + i;      // (a lane's tokens come by rising index)
+            return v;
         };
-        constexpr int PER = 16 / sizeof(TX);
-        const bool vec = ((uintptr_t)(src + at0) & 15) == 0;
-        if (vec) {
-            for (int i = s.lane * PER; i < p.seg; i += 32 * PER) {
-                TX v[PER];
-                if (at0 + i + PER <= p.V) {
-                    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + at0 + i);
+        constexpr int PER = 16 / sizeof(TX), IN_FLIGHT = 4;
+        if (((uintptr_t)(src + at0) & 15) == 0) {
+            for (int i0 = s.lane * PER; i0 < p.seg; i0 += IN_FLIGHT * 32 * PER) {
+                TX v[IN_FLIGHT][PER];
 #pragma unroll
-                    for (int j = 0; j < PER; ++j) take((float)v[j], i + j);
-                } else {
-                    for (int j = 0; j < PER; ++j) take(at0 + i + j < p.V ? (float)src[at0 + i + j] : -INFINITY, i + j);
+                for (int c = 0; c < IN_FLIGHT; ++c) {
+                    const int i = i0 + c * 32 * PER;
+                    if (i < p.seg && at0 + i + PER <= p.V) *reinterpret_cast<uint4*>(v[c]) = __ldg(reinterpret_cast<const uint4*>(src + at0 + i));
+                }
+#pragma unroll
+                for (int c = 0; c < IN_FLIGHT; ++c) {
+                    const int i = i0 + c * 32 * PER;
+                    if (i >= p.seg) break;
+                    float f[PER];
+                    if (at0 + i + PER <= p.V) {
+#pragma unroll
+                        for (int j = 0; j < PER; ++j) f[j] = take((float)v[c][j], i + j);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < PER; ++j) f[j] = take(at0 + i + j < p.V ? (float)src[at0 + i + j] : -INFINITY, i + j);
+                    }
+#pragma unroll
+                    for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(x + i + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
                 }
             }
         } else {
-            for (int i = s.lane; i < p.seg; i += 32) take(at0 + i < p.V ? (float)src[at0 + i] : -INFINITY, i);
+#pragma unroll 4
+            for (int i = s.lane; i < p.seg; i += 32) x[i] = take(at0 + i < p.V ? (float)src[at0 + i] : -INFINITY, i);
         }
+        s.top = top;
+        if (top > -INFINITY) best = token_key(top, top_at);
     }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) {
@@ -548,39 +709,70 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
         return;
     }
     if (!count && !by_weight) {
-        s.draw(row, 0, least, u);
+        s.draw(row, 0, least, u, nullptr);
         s.cl.sync();
         return;
     }
     // bins: 64 to a unit of the logits where the cut goes by number, 32 to a power of two of the weights where it goes by weight
-    s.to_bin = count ? 64.0f : fminf(32.0f * 1.44269504f / T, 1e30f);
-    if (s.w.infinite) s.to_bin = 0.0f;
+    const float weight_bins = s.w.infinite ? 0.0f : fminf(32.0f * 1.44269504f / T, 1e30f);
+    s.to_bin = s.w.infinite ? 0.0f : count ? 64.0f : weight_bins;
     u64 total = 0;
-    s.histogram(!count, [&](float x, int i) { return x > -INFINITY ? s.bin_of(x) : -1; }, count, top_p, 0, &total, !count);
-    total = s.sh->total;
-    const int bin = s.sh->bin;
-    if (s.sh->upto <= SF_LIST) {
-        s.gather([&](float x, int i) { return x > -INFINITY && s.bin_of(x) <= bin; });
+    bool listed = false;
+    if (count) {
+        // `count` threads have a token of a bin or a higher one: so have the first `count` tokens
+        if (count <= SF_LIST / 2) {
+            s.histogram([&] { if (s.top > -INFINITY) atomicAdd(s.cnt + s.bin_of(s.top), 1u); });
+            if (s.rank == 0) s.find_count(count);
+            s.cl.sync();
+            if (s.sh->upto >= count || s.sh->bin == SF_BINS - 1) {
+                const int bin = s.sh->bin;
+                s.gather([&](float x, int) { return x > -INFINITY && s.bin_of(x) <= bin; });
+                listed = *s.cl.map_shared_rank(&s.sh->n_list, 0) <= SF_LIST;
+            }
+            s.cl.sync();
+        }
+        if (!listed) {
+            s.histogram([&] { s.each([&](float x, int) { if (x > -INFINITY) atomicAdd(s.cnt + s.bin_of(x), 1u); }); });
+            if (s.rank == 0) s.find_count(count);
+            s.cl.sync();
+        }
+    } else {
+        total = s.weigh_and_count(0, weight_bins, top_p);
+    }
+    if (!listed && s.sh->upto <= SF_LIST) {
+        const int bin = s.sh->bin2;
+        s.gather([&](float x, int) { return x > -INFINITY && s.bin_of(x) <= bin; });
+        listed = true;
+    }
+    if (listed) {
         if (s.rank == 0) s.draw_list(row, count, top_p, total, least, u);
         if (p.dist) {
             if (s.rank == 0 && threadIdx.x == 0) {
-                const u64 cut = s.sh->cut, whole = s.sh->total;
-                s.everywhere(&Shared::cut, cut);
-                s.everywhere(&Shared::total, whole);
+                const Shared& z = *s.sh;
+                s.everywhere(&Shared::cut, z.cut);
+                s.everywhere(&Shared::total, z.total);
+                s.everywhere(&Shared::drawn, z.drawn);
+                s.everywhere(&Shared::drawn_p, z.drawn_p);
             }
             s.cl.sync();
-            s.distribution(row, s.sh->cut, 0, s.sh->total);
+            s.distribution(row, s.sh->cut, 0, s.sh->total, s.sh->drawn, s.sh->drawn_p);
         }
         s.cl.sync();
         return;
     }
-    u64 cut = 0;
-    if (count) cut = s.cut_at(0, count, 1.0f, &total);
-    if (by_weight) {
-        s.to_bin = s.w.infinite ? 0.0f : fminf(32.0f * 1.44269504f / T, 1e30f);
-        cut = s.cut_at(cut, 0, top_p, &total);
+    u64 cut = 0, mine = 0;
+    if (count) {
+        cut = s.cut_at(0, count, 1.0f, 0, &mine);
+        if (by_weight) {
+            s.cl.sync();
+            s.to_bin = weight_bins;
+            total = s.weigh_and_count(cut, weight_bins, top_p);
+            cut = s.cut_at(cut, 0, top_p, total, &mine);
+        }
+    } else {
+        cut = s.cut_at(0, 0, top_p, total, &mine);
     }
-    s.draw(row, cut, least, u);
+    s.draw(row, cut, least, u, by_weight && least == 0 ? &mine : nullptr);
     s.cl.sync();
 }
 
