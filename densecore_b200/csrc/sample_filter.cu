@@ -32,8 +32,9 @@ using namespace dc;
 namespace {
 
 typedef unsigned long long u64;
-constexpr int SF_T = 512, SF_W = SF_T / 32, SF_BINS = 2048, SF_LIST = 1024, SF_CLUSTER = 8;
-constexpr int SF_MOST = 48 * 1024;      // tokens of a CTA
+constexpr int SF_T = 512, SF_W = SF_T / 32, SF_BINS = 2048, SF_LIST = 1024, SF_CLUSTER = 16;
+constexpr int SF_MOST = 48 * 1024;      // f32 tokens of a CTA
+constexpr int SF_VOCAB = 8 * (SF_MOST - 32 * SF_W);
 constexpr u64 SF_ONE = 1ull << 44;
 
 struct SampleParams {
@@ -72,9 +73,9 @@ struct Weigher {
         const double w = fma(__hiloint2double(__double2hiint(v) + ((k >> 8) << 20), __double2loint(v)), q, 256.0);      // units of 2^-44
         return (u64)__double_as_longlong(w) - 0x4070000000000000ull;
     }
-    // bounds on weights in a bin of `per` bins to a power of two, the rounding of the bin's number included (2048 / per 2^-22 < 2^-14 of the exponent)
-    __device__ __forceinline__ static double above(float b, float per) { return exp2((double)(-b / per) + 0.0001) * (double)SF_ONE + 1.0; }
-    __device__ __forceinline__ static double below(float b, float per) { return fmax(exp2((double)(-(b + 1.0f) / per) - 0.0001) * (double)SF_ONE - 1.0, 0.0); }
+    // bounds on weights in a bin of 32 to a power of two: the rounding of the bin's number (2048 / 32 2^-22 of the exponent) and of exp2 (2^-22) are less than 1e-4 of the exponent
+    __device__ __forceinline__ static float above(float b) { return exp2f(fmaf(b, -0.03125f, 44.0001f)) + 1.0f; }
+    __device__ __forceinline__ static float below(float b) { return fmaxf(exp2f(fmaf(b, -0.03125f, 43.9686f)) - 1.0f, 0.0f); }
 };
 
 struct alignas(16) Shared {      // beside the row and the histogram
@@ -92,7 +93,7 @@ template <typename TX>
 struct Sampler {
     cg::cluster_group cl = cg::this_cluster();
     const SampleParams& p;
-    float* xs;
+    TX* xs;      // NaN as -inf
     uint32_t* cnt;
     u64* wh;
     Shared* sh;
@@ -106,9 +107,9 @@ struct Sampler {
     __device__ __forceinline__ int bin_of(float x) const { return (int)fminf((key_value((uint32_t)(best >> 32)) - x) * to_bin, (float)(SF_BINS - 1)); }
     template <typename F>
     __device__ __forceinline__ void each(F f) const {      // f(value, index) of this warp's tokens that have a value; whole warps
-        const float* x = xs + warp * p.seg;
+        const TX* x = xs + warp * p.seg;
 #pragma unroll 4
-        for (int i = lane; i < p.seg; i += 32) f(x[i], base + warp * p.seg + i);
+        for (int i = lane; i < p.seg; i += 32) f((float)x[i], base + warp * p.seg + i);
     }
     __device__ u64 block_sum(u64 v) const {      // in all threads
 #pragma unroll
@@ -176,11 +177,9 @@ struct Sampler {
         fill();
         cl.sync();
         for (int b = rank + n_cta * threadIdx.x; b < SF_BINS; b += n_cta * SF_T) {      // every CTA sums up its share of the bins
-            uint32_t n[SF_CLUSTER], all = 0;
-#pragma unroll
-            for (int i = 0; i < SF_CLUSTER; ++i) n[i] = i < n_cta ? cl.map_shared_rank(cnt, i)[b] : 0;
-#pragma unroll
-            for (int i = 0; i < SF_CLUSTER; ++i) all += n[i];
+            uint32_t all = 0;
+#pragma unroll 8
+            for (int i = 0; i < n_cta; ++i) all += cl.map_shared_rank(cnt, i)[b];
             cl.map_shared_rank(cnt, 0)[b] = all;
         }
         cl.sync();
@@ -217,14 +216,17 @@ struct Sampler {
     __device__ void find_weight(double before, double goal, H hi, L lo) {
         constexpr int B = SF_BINS / SF_T;
         uint32_t n[B];
-        double uh = 0.0, ul = 0.0;
+        double uh = 0.0, ul = 0.0, vh[B], vl[B];
         u64 sn = 0;
         int last = -1;
+#pragma unroll
         for (int i = 0; i < B; ++i) {
             const int b = B * (int)threadIdx.x + i;
             n[i] = cnt[b];
             sn += n[i];
-            if (n[i]) uh += n[i] * hi(b), ul += n[i] * lo(b), last = b;
+            vh[i] = n[i] ? n[i] * hi(b) : 0.0, vl[i] = n[i] ? n[i] * lo(b) : 0.0;
+            uh += vh[i], ul += vl[i];
+            if (n[i]) last = b;
         }
         u64 an = scan(sn) - sn;
         double ah = scan(uh) - uh + before, al = scan(ul) - ul + before;
@@ -237,7 +239,7 @@ struct Sampler {
         for (int i = 0; i < B; ++i) {
             const int b = B * (int)threadIdx.x + i;
             if (!n[i]) continue;
-            h += n[i] * hi(b), l += n[i] * lo(b);
+            h += vh[i], l += vl[i];
             if (h >= may && f[0] == SF_BINS) f[0] = b;
             if (l >= sure && f[1] == SF_BINS) f[1] = b;
         }
@@ -266,7 +268,7 @@ struct Sampler {
         u64 sum = 0;
         histogram([&] {
             each([&](float x, int i) {
-                if (x > -INFINITY && token_key(x, i) >= from) {
+                if (x > -INFINITY && (!from || token_key(x, i) >= from)) {
                     atomicAdd(cnt + bin_of(x), 1u);
                     sum += w(x);
                 }
@@ -276,8 +278,8 @@ struct Sampler {
         if (rank == 0) {
             // (bins that are not 32 to a power of two, at extreme temperatures, bound nothing from below)
             const bool bounded = per_unit < 1e30f && !w.infinite;
-            find_weight(0.0, (double)top_p * (double)sum, [&](int b) { return bounded ? w.above((float)b, 32.0f) : (double)SF_ONE; },
-                        [&](int b) { return bounded && b < SF_BINS - 1 ? w.below((float)b, 32.0f) : 0.0; });
+            find_weight(0.0, (double)top_p * (double)sum, [&](int b) { return bounded ? (double)w.above((float)b) : (double)SF_ONE; },
+                        [&](int b) { return bounded && b < SF_BINS - 1 ? (double)w.below((float)b) : 0.0; });
         }
         cl.sync();
         return sum;
@@ -304,6 +306,20 @@ struct Sampler {
         while (size < n) size <<= 1;
         for (int i = n + threadIdx.x; i < size; i += SF_T) list[i] = 0;
         __syncthreads();
+        if (size <= 128) {      // one warp is faster than all of them with barriers
+            if (warp == 0)
+                for (int k = 2; k <= size; k <<= 1)
+                    for (int j = k >> 1; j > 0; j >>= 1) {
+                        for (int i = lane; i < size / 2; i += 32) {
+                            const int a = 2 * i - (i & (j - 1)), b = a + j;
+                            const u64 x = list[a], y = list[b];
+                            if ((x < y) == ((a & k) == 0)) list[a] = y, list[b] = x;
+                        }
+                        __syncwarp();
+                    }
+            __syncthreads();
+            return;
+        }
         for (int k = 2; k <= size; k <<= 1)
             for (int j = k >> 1; j > 0; j >>= 1) {
                 for (int i = threadIdx.x; i < size / 2; i += SF_T) {
@@ -332,7 +348,7 @@ struct Sampler {
         uint32_t lo = 0, hi = 0xFFFFFFFFu;
         bool by_bin = true;
         auto in = [&](float x, int i) {
-            if (!(x > -INFINITY) || token_key(x, i) < from) return false;
+            if (!(x > -INFINITY) || (from && token_key(x, i) < from)) return false;
             if (by_bin) {
                 const int b = bin_of(x);
                 return b >= b0 && b <= b1;
@@ -346,7 +362,7 @@ struct Sampler {
         *mine = 0;
         if (weights) {
             u64 sum = 0;
-            each([&](float x, int i) { if (x > -INFINITY && token_key(x, i) >= from && bin_of(x) < b0) sum += w(x); });
+            each([&](float x, int i) { if (x > -INFINITY && bin_of(x) < b0 && (!from || token_key(x, i) >= from)) sum += w(x); });
             *mine = sum;
             before = cluster_sum(sum);
         }
@@ -408,12 +424,12 @@ struct Sampler {
                 for (int i = 0; i < rank; ++i) ahead_of_me += sh->counts[i];
                 for (int i = 0; i < warp; ++i) ahead_of_me += (long long)sh->warp[i];
                 if (ahead_of_me < q && ahead_of_me + n >= q) {
-                    const float* x = xs + warp * p.seg;
+                    const TX* x = xs + warp * p.seg;
                     for (int i = lane; i < p.seg; i += 32) {
                         const int index = base + warp * p.seg + i;
-                        const uint32_t there = __ballot_sync(0xffffffffu, in(x[i], index));
+                        const uint32_t there = __ballot_sync(0xffffffffu, in((float)x[i], index));
                         if (ahead_of_me + __popc(there) >= q) {
-                            if ((there >> lane & 1) && ahead_of_me + __popc(there & ((2u << lane) - 1u)) == q) everywhere(&Shared::cut, token_key(x[i], index));
+                            if ((there >> lane & 1) && ahead_of_me + __popc(there & ((2u << lane) - 1u)) == q) everywhere(&Shared::cut, token_key((float)x[i], index));
                             break;
                         }
                         ahead_of_me += __popc(there);
@@ -510,15 +526,26 @@ struct Sampler {
             if (i < rank) ahead_of_me += sh->part[i];
             total += sh->part[i];
         }
-        for (int i = 0; i < warp; ++i) ahead_of_me += sh->warp[i];
         const u64 goal = goal_of(u, total);
         int drawn = -1;      // in the warp that has it
         float drawn_p = 0.0f;
-        if (ahead_of_me <= goal && goal < ahead_of_me + mine) {
-            const float* x = xs + warp * p.seg;
-            for (int i = lane; i < p.seg; i += 32) {
-                const int index = base + warp * p.seg + i;
-                const u64 own = kept(x[i], index);
+        if (ahead_of_me <= goal && goal < ahead_of_me + sh->part[rank]) {      // in this CTA: the warp's part that has it is searched by all warps, 32 tokens each in turn
+            int found = 0;
+            while (found < SF_W - 1 && goal >= ahead_of_me + sh->warp[found]) ahead_of_me += sh->warp[found++];
+            const TX* x = xs + found * p.seg;
+            const int at = base + found * p.seg, lines = p.seg / 32;
+            for (int c = warp; c < lines; c += SF_W) {
+                u64 v = kept((float)x[32 * c + lane], at + 32 * c + lane);
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+                if (lane == 0) wh[c] = v;
+            }
+            __syncthreads();
+            if (warp == found) {
+                int line = 0;
+                while (line < lines - 1 && goal >= ahead_of_me + wh[line]) ahead_of_me += wh[line++];
+                const int index = at + 32 * line + lane;
+                const u64 own = kept((float)x[32 * line + lane], index);
                 u64 v = own;
 #pragma unroll
                 for (int s = 1; s < 32; s <<= 1) {
@@ -526,8 +553,6 @@ struct Sampler {
                     if (lane >= s) v += o;
                 }
                 if (own && ahead_of_me + v - own <= goal && goal < ahead_of_me + v) drawn = index, drawn_p = put(row, index, own, total);
-                ahead_of_me += __shfl_sync(0xffffffffu, v, 31);
-                if (ahead_of_me > goal) break;
             }
         }
         if (!p.dist) return;
@@ -619,7 +644,7 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
     s.wh = reinterpret_cast<u64*>(smem);
     s.cnt = reinterpret_cast<uint32_t*>(s.wh + SF_BINS);
     s.sh = reinterpret_cast<Shared*>(s.cnt + SF_BINS);
-    s.xs = reinterpret_cast<float*>(s.sh + 1);
+    s.xs = reinterpret_cast<TX*>(s.sh + 1);
     s.base = s.rank * SF_W * p.seg;
     const int row = blockIdx.x / s.n_cta;
     for (int i = threadIdx.x; i < 256; i += SF_T) s.sh->table[i] = exp2((double)i * 0.00390625);
@@ -629,7 +654,7 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
     const TX* src = reinterpret_cast<const TX*>(p.logits) + (size_t)row * p.ld;
     u64 best = 0;
     {
-        float* x = s.xs + s.warp * p.seg;
+        TX* x = s.xs + s.warp * p.seg;
         const int at0 = s.base + s.warp * p.seg;
         float top = -INFINITY;
         int top_at = 0;
@@ -660,12 +685,13 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
                         for (int j = 0; j < PER; ++j) f[j] = take(at0 + i + j < p.V ? (float)src[at0 + i + j] : -INFINITY, i + j);
                     }
 #pragma unroll
-                    for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(x + i + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+                    for (int j = 0; j < PER; ++j) v[c][j] = (TX)f[j];
+                    *reinterpret_cast<uint4*>(x + i) = *reinterpret_cast<const uint4*>(v[c]);
                 }
             }
         } else {
 #pragma unroll 4
-            for (int i = s.lane; i < p.seg; i += 32) x[i] = take(at0 + i < p.V ? (float)src[at0 + i] : -INFINITY, i);
+            for (int i = s.lane; i < p.seg; i += 32) x[i] = (TX)take(at0 + i < p.V ? (float)src[at0 + i] : -INFINITY, i);
         }
         s.top = top;
         if (top > -INFINITY) best = token_key(top, top_at);
@@ -776,15 +802,19 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
     s.cl.sync();
 }
 
-size_t sample_smem(int seg) { return SF_BINS * 12 + sizeof(Shared) + (size_t)SF_W * seg * 4; }
+size_t sample_smem(int seg, size_t type) { return SF_BINS * 12 + sizeof(Shared) + (size_t)SF_W * seg * type; }
 
 template <typename TX>
 int launch_sample(dc_ctx* ctx, SampleParams p, int rows) {
-    // eight CTAs a row: two of them fit into an SM up to some 140 000 tokens
-    const int n = SF_CLUSTER;
-    p.seg = ((p.V + n * SF_W - 1) / (n * SF_W) + 31) / 32 * 32;
-    const size_t smem = sample_smem(p.seg);
-    DC_TRY(dc_kernel_setup(ctx, (const void*)k_sample_filter<TX>, (int)sample_smem(SF_MOST / SF_W), "k_sample_filter"));
+    auto seg_of = [&](int n) { return ((p.V + n * SF_W - 1) / (n * SF_W) + 31) / 32 * 32; };
+    // few CTAs a row (fewer meetings), but two of them fit into an SM, and all SMs have work as long as a CTA has 4096 tokens
+    int n = 1;
+    while (n < 8 && sample_smem(seg_of(n), sizeof(TX)) > 112 * 1024) n *= 2;
+    while (n < SF_CLUSTER && rows * n * 2 <= ctx->num_sms && p.V / n > 4096) n *= 2;
+    p.seg = seg_of(n);
+    const size_t smem = sample_smem(p.seg, sizeof(TX));
+    DC_TRY(dc_kernel_setup(ctx, (const void*)k_sample_filter<TX>, (int)sample_smem(SF_MOST / SF_W, 4), "k_sample_filter"));
+    if (n > 8) DC_TRY(dc_check_cuda(ctx, cudaFuncSetAttribute((const void*)k_sample_filter<TX>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "k_sample_filter"));
     return dc_launch_cluster(ctx, "k_sample_filter", k_sample_filter<TX>, dim3(rows * n), dim3(SF_T), smem, n, p);
 }
 
@@ -798,7 +828,7 @@ int dc_b200_sample_rows_dev(dc_ctx* ctx, const void* logits_dev, int type, int r
     if (ld == 0) ld = vocab;
     if (rows < 0 || vocab < 1 || ld < vocab) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "sample_rows: bad shape (%d rows of %d, stride %lld)", rows, vocab, (long long)ld);
     if (type != DC_TYPE_F32 && type != DC_TYPE_BF16) return dc_fail(ctx, DC_B200_UNSUPPORTED, "sample_rows: logits of type %d (F32 and BF16 are supported)", type);
-    if (vocab > SF_MOST * SF_CLUSTER - SF_CLUSTER * SF_W * 32 || rows > (1 << 20)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "sample_rows: %d rows of %d tokens", rows, vocab);
+    if (vocab > SF_VOCAB || rows > (1 << 20)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "sample_rows: %d rows of %d tokens", rows, vocab);
     if (rows == 0) return DC_B200_OK;
     if (!logits_dev || !uniforms_dev || !tokens_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "sample_rows: null buffer");
     cudaSetDevice(ctx->device);
