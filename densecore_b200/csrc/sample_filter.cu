@@ -32,7 +32,8 @@ using namespace dc;
 namespace {
 
 typedef unsigned long long u64;
-constexpr int SF_T = 512, SF_W = SF_T / 32, SF_BINS = 2048, SF_LIST = 1024, SF_CLUSTER = 16;
+constexpr int SF_T = 512, SF_W = SF_T / 32, SF_BINS = 2048, SF_LIST = 1024, SF_SHORT = 256, SF_CLUSTER = 16;
+constexpr int SF_GROUPS = 256;          // of a row's threads, 2 n_cta neighbours each
 constexpr int SF_MOST = 48 * 1024;      // f32 tokens of a CTA
 constexpr int SF_VOCAB = 8 * (SF_MOST - 32 * SF_W);
 constexpr u64 SF_ONE = 1ull << 44;
@@ -80,8 +81,9 @@ struct Weigher {
 
 struct alignas(16) Shared {      // beside the row and the histogram
     double table[256];
-    u64 best[SF_CLUSTER], warp[SF_W], part[SF_CLUSTER];
-    u64 cut, total, in_before;
+    u64 warp[SF_W], part[SF_CLUSTER];
+    u64 cut, total, in_before, sum;
+    u64 group[SF_GROUPS], least;
     uint32_t lo[SF_CLUSTER], hi[SF_CLUSTER];
     double dwarp[SF_W];
     int first[2];
@@ -143,44 +145,43 @@ struct Sampler {
         for (int i = 0; i < SF_W; ++i) m = sh->warp[i] > m ? sh->warp[i] : m;
         return (int)m - 1;
     }
-    __device__ double scan(double v) const {
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const double o = __shfl_up_sync(0xffffffffu, v, s);
-            if (lane >= s) v += o;
-        }
-        __syncthreads();
-        if (lane == 31) sh->dwarp[warp] = v;
-        __syncthreads();
-        for (int i = 0; i < warp; ++i) v += sh->dwarp[i];
-        return v;
-    }
     // inclusive sums of a value a thread, over the CTA
-    __device__ u64 scan(u64 v) const {
+    template <typename V>
+    __device__ V scan_in(V v, V* of_warp) const {
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
-            const u64 o = __shfl_up_sync(0xffffffffu, v, s);
+            const V o = __shfl_up_sync(0xffffffffu, v, s);
             if (lane >= s) v += o;
         }
         __syncthreads();
-        if (lane == 31) sh->warp[warp] = v;
+        if (lane == 31) of_warp[warp] = v;
         __syncthreads();
-        for (int i = 0; i < warp; ++i) v += sh->warp[i];
-        return v;
+        V w = lane < SF_W ? of_warp[lane] : V(0);
+#pragma unroll
+        for (int s = 1; s < SF_W; s <<= 1) {
+            const V o = __shfl_up_sync(0xffffffffu, w, s);
+            if (lane >= s) w += o;
+        }
+        w = __shfl_sync(0xffffffffu, w, warp - 1 & 31);
+        return warp ? v + w : v;
     }
+    __device__ u64 scan(u64 v) const { return scan_in(v, sh->warp); }
+    __device__ double scan(double v) const { return scan_in(v, sh->dwarp); }
 
-    // Numbers of `fill`'s calls per bin, summed up over the cluster in CTA 0's cnt.
+    // Numbers per bin of the cluster's tokens, as `fill` counts them in cnt, and the sum of what it returns a thread, in CTA 0's cnt and sum.
     template <typename F>
     __device__ void histogram(F fill) {
         for (int i = threadIdx.x; i < SF_BINS; i += SF_T) cnt[i] = 0;
-        __syncthreads();
-        fill();
-        cl.sync();
-        for (int b = rank + n_cta * threadIdx.x; b < SF_BINS; b += n_cta * SF_T) {      // every CTA sums up its share of the bins
-            uint32_t all = 0;
-#pragma unroll 8
-            for (int i = 0; i < n_cta; ++i) all += cl.map_shared_rank(cnt, i)[b];
-            cl.map_shared_rank(cnt, 0)[b] = all;
+        if (threadIdx.x == 0) sh->sum = 0;
+        cl.sync();      // (CTA 0's are clear before others add to them)
+        u64 v = fill();
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+        if (lane == 0 && v) atomicAdd(&cl.map_shared_rank(sh, 0)->sum, v);
+        if (rank != 0) {
+            __syncthreads();
+            for (int b = threadIdx.x; b < SF_BINS; b += SF_T)
+                if (cnt[b]) atomicAdd(cl.map_shared_rank(cnt, 0) + b, cnt[b]);
         }
         cl.sync();
     }
@@ -265,31 +266,31 @@ struct Sampler {
 
     // For a cut by weight among the tokens at or above `from`: their number per bin and the sum of their weights (returned), then find_weight().
     __device__ u64 weigh_and_count(u64 from, float per_unit, float top_p) {
-        u64 sum = 0;
-        histogram([&] {
+        histogram([&]() -> u64 {
+            u64 sum = 0;
             each([&](float x, int i) {
                 if (x > -INFINITY && (!from || token_key(x, i) >= from)) {
                     atomicAdd(cnt + bin_of(x), 1u);
                     sum += w(x);
                 }
             });
+            return sum;
         });
-        sum = cluster_sum(sum);
         if (rank == 0) {
+            const u64 sum = sh->sum;
+            if (threadIdx.x == 0) everywhere(&Shared::total, sum);
             // (bins that are not 32 to a power of two, at extreme temperatures, bound nothing from below)
             const bool bounded = per_unit < 1e30f && !w.infinite;
             find_weight(0.0, (double)top_p * (double)sum, [&](int b) { return bounded ? (double)w.above((float)b) : (double)SF_ONE; },
                         [&](int b) { return bounded && b < SF_BINS - 1 ? (double)w.below((float)b) : 0.0; });
         }
         cl.sync();
-        return sum;
+        return sh->total;
     }
 
-    // The keys of tokens that `take` names, into CTA 0's list (unordered); its length in CTA 0's n_list.
+    // The keys of tokens that `take` names, into CTA 0's list (unordered); its length in CTA 0's n_list, which is 0 before.
     template <typename F>
     __device__ void gather(F take) {
-        if (rank == 0 && threadIdx.x == 0) sh->n_list = 0;
-        cl.sync();
         u64* list = cl.map_shared_rank(wh, 0);
         int* n = &cl.map_shared_rank(sh, 0)->n_list;
         each([&](float x, int i) {
@@ -299,6 +300,9 @@ struct Sampler {
             }
         });
         cl.sync();
+    }
+    __device__ void clear_list() {      // with a meeting of the cluster between it and gather()
+        if (rank == 0 && threadIdx.x == 0) sh->n_list = 0;
     }
     // CTA 0: list[0 .. n) sorted, largest first; n <= SF_LIST
     __device__ void sort(u64* list, int n) const {
@@ -368,6 +372,8 @@ struct Sampler {
         }
         for (int round = 0; round < 64; ++round) {      // (each leaves half of 2^32 values at most; equal ones end it)
             if (inside <= SF_LIST) {
+                clear_list();
+                cl.sync();
                 gather(in);
                 if (rank == 0) {
                     const int n = min(sh->n_list, SF_LIST);
@@ -442,10 +448,11 @@ struct Sampler {
             const u64 width = (u64)hi - lo + 1;
             const uint32_t top = hi;
             auto edge = [&](int part) { return (uint32_t)(((u64)part * width + SF_BINS - 1) / SF_BINS); };      // least top - k of a part
-            histogram([&] {
+            histogram([&]() -> u64 {
                 each([&](float x, int i) {
                     if (in(x, i)) atomicAdd(cnt + (int)((u64)(top - sort_key(x + 0.0f)) * SF_BINS / width), 1u);
                 });
+                return 0;
             });
             if (rank == 0) {
                 if (weights)
@@ -598,6 +605,49 @@ struct Sampler {
         });
     }
 
+    // The same as draw_list() for up to 256 tokens: places and sums by comparing each with all.
+    __device__ void draw_short(int row, long long count, float top_p, u64 total, u64 least, float u) {
+        const int n = sh->n_list, t = threadIdx.x;
+        u64 *key = wh, *weight = wh + SF_LIST;
+        const u64 mine = t < n ? key[t] : 0, own = t < n ? w(key_value((uint32_t)(mine >> 32))) : 0;
+        if (t < n) weight[t] = own;
+        if (t == n) key[t] = 0, weight[t] = 0;      // (read in pairs)
+        __syncthreads();
+        u64 pre = 0;
+        int place = 0;
+        if (t < n) {
+#pragma unroll 2
+            for (int j = 0; j < n; j += 2) {
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(key + j), v = *reinterpret_cast<const ulonglong2*>(weight + j);
+                if (k.x > mine) pre += v.x, ++place;
+                if (k.y > mine) pre += v.y, ++place;
+            }
+            if (count > 0 && place == min((long long)n, count) - 1) sh->total = pre + own;
+        }
+        __syncthreads();
+        if (count > 0) total = sh->total;
+        const bool in = t < n && (place == 0 || ((count <= 0 || place < count) && (top_p >= 1.0f || (double)pre < (double)top_p * (double)total) && own >= least));
+        const int keep = __syncthreads_count(in);
+        if (t < n && place == keep - 1) sh->total = pre + own, sh->cut = mine;
+        if (t < n && place >= keep) weight[t] = 0;
+        __syncthreads();
+        const u64 whole = sh->total, goal = goal_of(u, whole);
+        if (in && own) {
+            u64 ahead = 0;      // kept ones of lower index: larger low words
+#pragma unroll 2
+            for (int j = 0; j < n; j += 2) {
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(key + j), v = *reinterpret_cast<const ulonglong2*>(weight + j);
+                if ((uint32_t)k.x > (uint32_t)mine) ahead += v.x;
+                if ((uint32_t)k.y > (uint32_t)mine) ahead += v.y;
+            }
+            if (ahead <= goal && goal < ahead + own) {
+                sh->drawn = key_index(mine);
+                sh->drawn_p = put(row, sh->drawn, own, whole);
+            }
+        }
+        __syncthreads();
+    }
+
     // CTA 0's sorted list holds all tokens down to the cut by number, or by weight of `total`: the filters and the draw.
     __device__ void draw_list(int row, long long count, float top_p, u64 total, u64 least, float u) {
         u64* list = wh;
@@ -696,20 +746,27 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
         s.top = top;
         if (top > -INFINITY) best = token_key(top, top_at);
     }
+    // ---- the largest token of each of 256 groups of threads, in all CTAs
+    const int lanes = 2 * s.n_cta, per_cta = SF_GROUPS / s.n_cta;
+    for (int k = 1; k < lanes; k <<= 1) {
+        const u64 o = __shfl_xor_sync(0xffffffffu, best, k);
+        best = o > best ? o : best;
+    }
+    if (s.lane % lanes == 0) {
+        const int g = s.rank * per_cta + threadIdx.x / lanes;
+        for (int i = 0; i < s.n_cta; ++i) s.cl.map_shared_rank(s.sh, i)->group[g] = best;
+    }
+    s.clear_list();
+    if (threadIdx.x == 0) s.sh->least = 0;
+    s.cl.sync();
+    best = 0;
+#pragma unroll
+    for (int i = 0; i < SF_GROUPS / 32; ++i) best = s.sh->group[s.lane + 32 * i] > best ? s.sh->group[s.lane + 32 * i] : best;
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) {
         const u64 o = __shfl_xor_sync(0xffffffffu, best, k);
         best = o > best ? o : best;
     }
-    if (s.lane == 0) s.sh->warp[s.warp] = best;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < SF_W; ++i) best = s.sh->warp[i] > best ? s.sh->warp[i] : best;
-        for (int i = 0; i < s.n_cta; ++i) s.cl.map_shared_rank(s.sh, i)->best[s.rank] = best;
-    }
-    s.cl.sync();
-    best = 0;
-    for (int i = 0; i < s.n_cta; ++i) best = s.sh->best[i] > best ? s.sh->best[i] : best;
     s.best = best;
     const float T = p.temperature ? p.temperature[row] : 1.0f, top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.0f, u = p.u[row];
     const int top_k = p.top_k ? p.top_k[row] : 0;
@@ -745,20 +802,32 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
     u64 total = 0;
     bool listed = false;
     if (count) {
-        // `count` threads have a token of a bin or a higher one: so have the first `count` tokens
-        if (count <= SF_LIST / 2) {
-            s.histogram([&] { if (s.top > -INFINITY) atomicAdd(s.cnt + s.bin_of(s.top), 1u); });
-            if (s.rank == 0) s.find_count(count);
-            s.cl.sync();
-            if (s.sh->upto >= count || s.sh->bin == SF_BINS - 1) {
-                const int bin = s.sh->bin;
-                s.gather([&](float x, int) { return x > -INFINITY && s.bin_of(x) <= bin; });
-                listed = *s.cl.map_shared_rank(&s.sh->n_list, 0) <= SF_LIST;
+        if (count <= SF_GROUPS * 3 / 4) {
+            // `count` groups have a token at or above the count-th largest of the groups' largest ones: so lie the first `count` tokens
+            const u64 mine = s.sh->group[threadIdx.x % SF_GROUPS];
+            int place = 0;
+            if (threadIdx.x < SF_GROUPS) {
+#pragma unroll 8
+                for (int j = 0; j < SF_GROUPS; j += 2) {
+                    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(s.sh->group + j);
+                    place += (k.x > mine) + (k.y > mine);
+                }
+                if (place == count - 1 && mine) s.sh->least = mine;      // (groups without a token are 0)
             }
-            s.cl.sync();
+            __syncthreads();
+            const u64 from = s.sh->least;
+            if (from) {
+                s.gather([&](float x, int i) { return x > -INFINITY && token_key(x, i) >= from; });
+                listed = *s.cl.map_shared_rank(&s.sh->n_list, 0) <= SF_LIST;
+                s.cl.sync();
+            }
         }
         if (!listed) {
-            s.histogram([&] { s.each([&](float x, int) { if (x > -INFINITY) atomicAdd(s.cnt + s.bin_of(x), 1u); }); });
+            s.clear_list();
+            s.histogram([&]() -> u64 {
+                s.each([&](float x, int) { if (x > -INFINITY) atomicAdd(s.cnt + s.bin_of(x), 1u); });
+                return 0;
+            });
             if (s.rank == 0) s.find_count(count);
             s.cl.sync();
         }
@@ -771,7 +840,10 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
         listed = true;
     }
     if (listed) {
-        if (s.rank == 0) s.draw_list(row, count, top_p, total, least, u);
+        if (s.rank == 0) {
+            if (s.sh->n_list <= SF_SHORT) s.draw_short(row, count, top_p, total, least, u);
+            else s.draw_list(row, count, top_p, total, least, u);
+        }
         if (p.dist) {
             if (s.rank == 0 && threadIdx.x == 0) {
                 const Shared& z = *s.sh;
@@ -783,7 +855,6 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
             s.cl.sync();
             s.distribution(row, s.sh->cut, 0, s.sh->total, s.sh->drawn, s.sh->drawn_p);
         }
-        s.cl.sync();
         return;
     }
     u64 cut = 0, mine = 0;
