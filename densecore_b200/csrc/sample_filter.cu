@@ -62,17 +62,16 @@ struct Weigher {
     double most, c;      // largest logit, log2(e) / T
     const double* table;
     bool infinite;
-    __device__ __forceinline__ u64 operator()(float x) const {
-        if (infinite) return x == INFINITY ? SF_ONE : 0ull;
+    __device__ __forceinline__ u64 operator()(float x) const {      // (without branches: several in flight)
         const double d = (double)x - most;
         const double t = fma(d, c, 26388279066624.0);      // 1.5 2^44: to the nearest 256th
-        if (!(t > 26388279066624.0 - 46.0) || !(x > -INFINITY)) return 0ull;
         const int k = __double2loint(t);
         const double r = fma(d, c, 26388279066624.0 - t);
         const double q = fma(r, fma(r, fma(r, 0.055504108664821580, 0.24022650695910071), 0.69314718055994531), 1.0);
         const double v = table[k & 255];
         const double w = fma(__hiloint2double(__double2hiint(v) + ((k >> 8) << 20), __double2loint(v)), q, 256.0);      // units of 2^-44
-        return (u64)__double_as_longlong(w) - 0x4070000000000000ull;
+        const u64 whole = t > 26388279066624.0 - 46.0 ? (u64)__double_as_longlong(w) - 0x4070000000000000ull : 0ull;      // (none for -inf and NaN)
+        return infinite ? (x == INFINITY ? SF_ONE : 0ull) : whole;
     }
     // bounds on weights in a bin of 32 to a power of two: the rounding of the bin's number (2048 / 32 2^-22 of the exponent) and of exp2 (2^-22) are less than 1e-4 of the exponent
     __device__ __forceinline__ static float above(float b) { return exp2f(fmaf(b, -0.03125f, 44.0001f)) + 1.0f; }
@@ -268,12 +267,19 @@ struct Sampler {
     __device__ u64 weigh_and_count(u64 from, float per_unit, float top_p) {
         histogram([&]() -> u64 {
             u64 sum = 0;
-            each([&](float x, int i) {
-                if (x > -INFINITY && (!from || token_key(x, i) >= from)) {
-                    atomicAdd(cnt + bin_of(x), 1u);
-                    sum += w(x);
-                }
-            });
+            if (!from)
+                each([&](float x, int) {
+                    const u64 v = w(x);
+                    if (x > -INFINITY) atomicAdd(cnt + bin_of(x), 1u);
+                    sum += v;
+                });
+            else
+                each([&](float x, int i) {
+                    if (x > -INFINITY && token_key(x, i) >= from) {
+                        atomicAdd(cnt + bin_of(x), 1u);
+                        sum += w(x);
+                    }
+                });
             return sum;
         });
         if (rank == 0) {
@@ -516,6 +522,7 @@ struct Sampler {
         };
         u64 mine = 0;
         if (known) mine = *known;
+        else if (!cut && !least) each([&](float x, int) { mine += w(x); });
         else each([&](float x, int i) { mine += kept(x, i); });
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, s);
