@@ -2,7 +2,7 @@
 //
 // A cached row of a head is held in groups of 64 values: m = fp16(least), d = fp16((largest - least) * fp32(1/15)), codes
 // q = rint((x - m) / d) within 0..15 (0 where d is 0), all in fp32; a code stands for fp32(d q + m).  A group with a value that is not
-// finite or beyond +-65504 is held with d = m = NaN, and reads back so.  Blocks, tables, sharing and copy-on-write are kv.cu's, on planes of
+// finite or beyond +-32768 (above it d c + m may leave fp16's range) is held with d = m = NaN, and reads back so.  Blocks, tables, sharing and copy-on-write are kv.cu's, on planes of
 // one record per (page, key head) (dc_q4.h).  A step is planned once (dc_b200_kv_batch) and then run for every layer.
 //
 // Scores of a token: sum over groups of d (q . codes) + m (sum of q); answers: sum over tokens of (p d) codes, plus the sum of p m.  Codes go to the
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(128) k_q4_write(const WriteParams p) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             x[i] = to_f32(src[i]);
-            fine = fine && fabsf(x[i]) <= 65504.0f;
+            fine = fine && fabsf(x[i]) <= 32768.0f;
             lo = fminf(lo, x[i]);
             hi = fmaxf(hi, x[i]);
         }
@@ -592,8 +592,12 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
     std::vector<dc_q4_tile> tiles;
     for (const dc_q4_entry& e : es)
         for (int i = 0; i < e.count; ++i) tokens[2 * (size_t)(e.tok0 + i)] = e.seq, tokens[2 * (size_t)(e.tok0 + i) + 1] = e.pos0 + i;
-    int n_tickets, n_ws;
-    dc_q4_items(es, z.heads / z.kv, z.kv, ctx->num_sms, &items, &n_tickets, &n_ws);
+    const int G = z.heads / z.kv;
+    std::vector<dc_q4_entry> few, many;
+    for (const dc_q4_entry& e : es) (z.type == DC_TYPE_BF16 && (long long)e.count * G >= DC_Q4_PROMPT_ROWS ? many : few).push_back(e);
+    int n_tickets, n_ws, n_parts;
+    dc_q4_items(few, G, z.kv, ctx->num_sms, &items, &n_tickets, &n_ws);
+    dc_q4_tiles(many, G, z.kv, ctx->num_sms, &tiles, &n_parts);
     // ---- one allocation: header, arrays, tickets (zero, and left so by every call), partial results
     auto up = [](size_t n) { return (n + 63) / 64 * 64; };
     dc_q4_head hd = {};
@@ -604,7 +608,8 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
     hd.tiles = (int32_t)(at / 4), at += up(tiles.size() * sizeof(dc_q4_tile));
     const size_t copied = at;
     hd.tickets = (int32_t)(at / 4), at += up((size_t)n_tickets * z.kv * 4);
-    hd.ws = (int32_t)(at / 4), at += up((size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4);
+    // (one kernel's parts after the other's: the rows kernel has joined its own when the next one starts)
+    hd.ws = (int32_t)(at / 4), at += up(std::max((size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4, (size_t)n_parts * z.kv * 256 * (z.dim + 4) * 4));
     if (at > ((size_t)1 << 33) - 64) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: the step's plan takes %zu bytes", at);
     if (at > z.plan_bytes) {
         uint8_t* fresh = nullptr;
@@ -631,7 +636,7 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
     DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.plan, z.stage, copied, cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
     DC_TRY(dc_check_cuda(ctx, cudaEventRecord(z.uploaded, ctx->stream), "kv_batch: plan"));
     if (n_tickets) DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.plan + 4 * (size_t)hd.tickets, 0, (size_t)n_tickets * z.kv * 4, ctx->stream), "kv_batch: tickets"));
-    z.T = T, z.n_items = hd.n_items, z.n_tiles = hd.n_tiles;
+    z.T = T, z.n_items = hd.n_items, z.n_tiles = hd.n_tiles, z.split_tiles = n_parts > 0;
     return DC_B200_OK;
 }
 
@@ -745,7 +750,8 @@ int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const voi
     cudaSetDevice(ctx->device);
     if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev));
     const dc_q4_call c = {kv, kv->planes[layer].arena, q_dev, ld_q, ld_out, scale, out_dev, k_dev != nullptr};
-    return dc_launch_q4_rows(ctx, c);
+    DC_TRY(dc_launch_q4_rows(ctx, c));
+    return dc_launch_q4_prompt(ctx, c);
 }
 
 int dc_b200_flash_attn_q4(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_host, const void* k_host, const void* v_host, float scale, void* out_host) {

@@ -1,0 +1,448 @@
+// Attention of prompt-sized portions over the cache in 4 bits, bf16 rows, on the 5th-generation tensor cores.
+//
+// One CTA per (256 rows of an entry, key head, part of the keys): row r is new token r / G and query head r % G of the key head, so that any number of query heads a key
+// head fills the tiles.  Two sets of 128 rows share key and value tiles of 64 keys.  Scores and P V are tcgen05.mma with f32 accumulators in tensor memory: per
+// set two tiles of scores of 64 columns, whose first 32 then hold the weights as fp16 pairs, and HD columns of answers; the next tile's scores are made while a
+// thread per row weights this one's.
+//   warps 0-7    weights: four a set, thread = row = tensor-memory lane
+//   warps 8-11   pages by bulk copies, codes turned into fp16 rows of the operands' 128-byte swizzle (d c + m, rounded once: 2^-11 relative)
+//   warp 12      issues the products
+// Queries are bf16 rows times a power of two (exact in fp16), weights fp16 (2^-11): together below a bf16 result's own 2^-8.
+// A value that is not a number (d = m = NaN) enters the tiles as 0, or the products would carry it to rows that do not see it; the CTA keeps the first
+// position of such a value per group of 64 dimensions, and rows that see it end as NaN there.
+// Bound: the weights' arithmetic and the chain scores, weights, answers of a tile, one CTA per SM.
+// Keys are split over CTAs where there are fewer row tiles than SMs (dc_q4_tiles); k_q4_join adds the parts up.
+#include <math.h>
+
+#include "dc_common.cuh"
+#include "dc_internal.h"
+#include "dc_launch.cuh"
+#include "dc_q4.h"
+#include "dc_tcgen05.cuh"
+
+using namespace dc;
+
+#define DC_TRY(expr)                       \
+    do {                                   \
+        int _st = (expr);                  \
+        if (_st != DC_B200_OK) return _st; \
+    } while (0)
+
+namespace {
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// two codes in the halves' low four bits, anything above: d c + m
+__device__ __forceinline__ uint32_t value2(uint32_t w, __half2 d, __half2 m) {
+    const uint32_t x = (w & 0x000F000Fu) | 0x64006400u;      // 1024 + c
+    const __half2 v = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(-1024.0f, -1024.0f)), d, m);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+struct PromptParams {
+    const uint8_t* plan;
+    const __nv_bfloat16* q;
+    int ldq, ldo, heads, n_kv, max_blocks;
+    const int32_t* tables;
+    const uint8_t* arena;
+    float scale;
+    __nv_bfloat16* out;
+};
+
+constexpr int QP_ROWS = 128, QP_KEYS = 64, QP_STAGES = 4, QP_RAW = 3, QP_THREADS = 13 * 32;
+enum QpBar { QP_FULL = 0, QP_FREE = 4, QP_S = 8, QP_P = 12, QP_O = 16, QP_DRAIN = 18, QP_PAGES = 19, QP_READ = 22, QP_NBARS = 25 };
+template <int HD>
+struct Lay {
+    static constexpr uint32_t SET = QP_ROWS * HD * 2, TILE = QP_KEYS * HD * 2;      // a set's queries; keys or values of a tile: halves of 64 columns
+    static constexpr uint32_t KV = 2 * SET, RAW = KV + QP_STAGES * 2 * TILE, RAW_BYTES = 4 * dc_q4_rec<HD>::BYTES, BARS = RAW + QP_RAW * RAW_BYTES;
+    static constexpr size_t SMEM = BARS + QP_NBARS * 8 + 1024;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams p, int* err) {
+    using L = Lay<HD>;
+    using R = dc_q4_rec<HD>;
+    constexpr int GR = R::GROUPS;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_nan[2];
+    __shared__ float s_pow[2 * QP_ROWS];      // 2^e of a row
+    pdl_wait();
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.y, G = p.heads / p.n_kv;
+    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
+    if ((int)blockIdx.x >= hd->n_tiles) return;      // (a replay on a smaller step)
+    const dc_q4_tile tl = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles)[blockIdx.x];
+    const int rows = min(2 * QP_ROWS, tl.count * G - tl.row0), sets = rows > QP_ROWS ? 2 : 1;
+    const int last = tl.pos0 + (tl.row0 + rows - 1) / G, first_tile = tl.tile0, n_tiles = tl.tile1 - tl.tile0;
+    const uint32_t sm = (smem_u32(smem) + 1023u) & ~1023u;
+    auto bar = [sm](int which, int i = 0) -> uint32_t { return sm + L::BARS + 8u * (uint32_t)(which + i); };
+    if (warp == 12) {
+        tmem_alloc(smem_u32(&s_tmem), 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int i = 0; i < QP_NBARS; ++i) mbar_init(bar(i), i < QP_FREE || i >= QP_READ ? 128 : i >= QP_P && i < QP_O ? 4 : 1);
+        mbar_fence_init();
+        s_nan[0] = s_nan[1] = 0x7fffffff;
+    }
+    auto row_of = [&](int r) -> const __nv_bfloat16* {      // a row's query, or null
+        if (r >= rows) return nullptr;
+        const int x = tl.row0 + r, j = x / G;
+        return p.q + (size_t)(tl.tok0 + j) * p.ldq + (size_t)(kvh * G + x - j * G) * HD;
+    };
+    // ---- queries: a row times 2^-e, 2^e <= its largest < 2^(e + 1), four threads a row
+    if (tid < 384) {
+        constexpr int PER = HD / 4;
+        const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+        for (int r = tid >> 2; r < 2 * QP_ROWS; r += 96) {
+            const __nv_bfloat16* src = row_of(r);
+            float x[PER], most = 0.0f;
+            const int d0 = (tid & 3) * PER;
+            if (src && (((uintptr_t)(src + d0)) & 3) == 0) {
+#pragma unroll
+                for (int i = 0; i < PER; i += 2) {
+                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + d0 + i));
+                    x[i] = f.x, x[i + 1] = f.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) x[i] = src ? __bfloat162float(src[d0 + i]) : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) most = fmaxf(most, fabsf(x[i]));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int e = max(-100, min(100, (int)(__float_as_uint(most) >> 23) - 127));
+            const float up = __uint_as_float((uint32_t)(127 - e) << 23) * sign;
+            if ((tid & 3) == 0) s_pow[r] = __uint_as_float((uint32_t)(127 + e) << 23);
+            const uint32_t base = sm + (r >> 7) * L::SET + (r & 127) * 128;
+#pragma unroll
+            for (int c = 0; c < PER / 8; ++c) {
+                const int col = (d0 >> 3) + c;
+                sts128(base + (col >> 3) * (QP_ROWS * 128) + (((col & 7) ^ (r & 7)) << 4), pack_h2(x[8 * c] * up, x[8 * c + 1] * up), pack_h2(x[8 * c + 2] * up, x[8 * c + 3] * up),
+                       pack_h2(x[8 * c + 4] * up, x[8 * c + 5] * up), pack_h2(x[8 * c + 6] * up, x[8 * c + 7] * up));
+            }
+        }
+    }
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_launch_dependents();      // (not before the tensor memory is there: a successor that held some and waited for this kernel would never give it back)
+    const uint32_t tmem = s_tmem;
+    auto wait = [&](uint32_t b, uint32_t parity) {      // (a role that gives up lets the others run into limits of their own)
+        const bool is = mbar_wait_warp(b, parity);
+        if (!is && err) atomicExch(err, DC_ERR_MBAR_TIMEOUT);
+        return is;
+    };
+    if (warp < 8) {
+        // ------------------------------------------------------------------ weights
+        const int u = warp >> 2, row = 32 * (warp & 3) + lane, r = QP_ROWS * u + row;
+        if (u < sets) {
+            const uint32_t t_unit = tmem + u * 256 + ((uint32_t)(32 * (warp & 3)) << 16), t_o = t_unit + 128;
+            const bool in = r < rows;
+            const int qp = in ? tl.pos0 + (tl.row0 + r) / G : -1, all_see = tl.pos0 + (tl.row0 + QP_ROWS * u + 32 * (warp & 3)) / G;
+            const float sl2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f * s_pow[r], 1e-35f);      // (above 0: minus infinity stays so)
+            float m_run = -1e30f, l_run[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            bool ok = true;
+            __syncwarp();
+            {
+                const uint32_t zero[16] = {};
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) tmem_st16(t_o + 16 * c, zero);      // (complete and ordered with the first tile's weights)
+            }
+            for (int t = 0; t < n_tiles; ++t) {
+                const uint32_t t_s = t_unit + 64 * (t & 1);
+                ok = wait(bar(QP_S, 2 * u + (t & 1)), (t >> 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                int x[4][16];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld16(t_s + 16 * c, x[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
+                auto s = [&](int i) -> float { return __int_as_float(x[i >> 4][i & 15]); };
+                const int k0 = (first_tile + t) * QP_KEYS;
+                if (k0 + QP_KEYS - 1 > all_see) {
+#pragma unroll
+                    for (int i = 0; i < QP_KEYS; ++i)
+                        if (k0 + i > qp) x[i >> 4][i & 15] = __float_as_int(-INFINITY);
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    mx[c] = s(16 * c);
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], s(16 * c + i));
+                }
+                const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
+                if (__any_sync(0xffffffffu, m_new > m_run)) {
+                    const float corr = ex2(m_run - m_new);
+                    m_run = m_new;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) l_run[i] *= corr;
+                    if (t > 0) {
+                        ok = wait(bar(QP_O, u), (t - 1) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD / 16; ++c) {
+                            int o[16];
+                            uint32_t w[16];
+                            tmem_ld16(t_o + 16 * c, o);
+                            tmem_ld_wait(o);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__int_as_float(o[i]) * corr);
+                            tmem_st16(t_o + 16 * c, w);
+                        }
+                    }
+                }
+                __syncwarp();      // masks are a lane's own, the stores are the whole warp's
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float a = ex2(fmaf(s(32 * h + 2 * i), sl2, -m_run)), b = ex2(fmaf(s(32 * h + 2 * i + 1), sl2, -m_run));
+                        l_run[i & 3] += a + b;
+                        w[i] = pack_h2(a, b);
+                    }
+                    tmem_st16(t_s + 16 * h, w);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(QP_P, 2 * u + (t & 1)));      // (two barriers: a warp may be done with the next tile before another is with this one)
+            }
+            // (phase by phase: the parity of the last alone also stands for the one before the last but one; tile t's scores come behind phase t - 2)
+            if (ok && n_tiles > 1) ok = wait(bar(QP_O, u), (n_tiles - 2) & 1);
+            if (ok) ok = wait(bar(QP_O, u), (n_tiles - 1) & 1);
+            if (ok) {
+                tc_fence_after();
+                const float l = (l_run[0] + l_run[1]) + (l_run[2] + l_run[3]);
+                const bool whole = tl.n_splits == 1;
+                const float mul = whole ? 1.0f / l : 1.0f;
+                const int x = tl.row0 + r, j = x / G;
+                __nv_bfloat16* dst = p.out + (size_t)(tl.tok0 + (in ? j : 0)) * p.ldo + (size_t)(kvh * G + (in ? x - j * G : 0)) * HD;
+                float* part = reinterpret_cast<float*>(const_cast<uint8_t*>(p.plan) + 4 * (size_t)hd->ws) +
+                              (((size_t)tl.ws * p.n_kv + (size_t)tl.n_splits * kvh + tl.split) * (2 * QP_ROWS) + r) * (HD + 4);
+                const bool vec = ((uintptr_t)dst & 15) == 0;
+                if (in && !whole) *reinterpret_cast<float2*>(part + HD) = make_float2(m_run, l);
+#pragma unroll 1
+                for (int c = 0; c < HD / 16; ++c) {
+                    int o[16];
+                    __syncwarp();      // lanes without a row have skipped the last stores: the load is the whole warp's
+                    tmem_ld16(t_o + 16 * c, o);
+                    tmem_ld_wait(o);
+                    if (in) {
+                        const float f = s_nan[c / 4] <= qp ? NAN : mul;
+                        auto v = [&](int i) { return __int_as_float(o[i]) * f; };
+                        if (!whole) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + 16 * c + i) = make_float4(v(i), v(i + 1), v(i + 2), v(i + 3));
+                        } else if (vec) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 8)
+                                *reinterpret_cast<uint4*>(dst + 16 * c + i) = make_uint4(pack_bf2(v(i), v(i + 1)), pack_bf2(v(i + 2), v(i + 3)), pack_bf2(v(i + 4), v(i + 5)), pack_bf2(v(i + 6), v(i + 7)));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) dst[16 * c + i] = __float2bfloat16_rn(v(i));
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ------------------------------------------------------------------ key and value tiles
+        const int lt = tid - 256, lw = lt >> 5;
+        const int32_t* table = p.tables + (size_t)tl.seq * p.max_blocks;
+        const int last_page = last / DC_KV_BLOCK;
+        auto fetch = [&](int t) {      // one thread: the four pages of a tile (those beyond the last token: the last page, for something finite)
+            const uint32_t b = bar(QP_PAGES, t % QP_RAW);
+            mbar_expect_tx(b, L::RAW_BYTES);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int page = min((first_tile + t) * 4 + i, last_page);
+                bulk_g2s(sm + L::RAW + (t % QP_RAW) * L::RAW_BYTES + i * R::BYTES, p.arena + ((size_t)table[page] * p.n_kv + kvh) * R::BYTES, R::BYTES, b);
+            }
+        };
+        int fetched = 0, t = 0;
+        if (lt == 0)
+            for (; fetched < QP_RAW && fetched < n_tiles; ++fetched) fetch(fetched);
+        for (; t < n_tiles; ++t) {
+            bool ok = wait(bar(QP_PAGES, t % QP_RAW), (t / QP_RAW) & 1);
+            if (ok && t >= QP_STAGES) ok = wait(bar(QP_FREE, t % QP_STAGES), (t / QP_STAGES - 1) & 1);
+            if (!ok) break;
+            const uint32_t to = sm + L::KV + (t % QP_STAGES) * (2 * L::TILE);
+            const uint32_t raw = sm + L::RAW + (t % QP_RAW) * L::RAW_BYTES + lw * R::BYTES;      // a warp has one page
+            const int pos = (first_tile + t) * QP_KEYS + lw * DC_KV_BLOCK;
+            // ---- keys: a lane takes 32 dimensions of one token, from four words that lie 16 bytes apart
+#pragma unroll
+            for (int x = 0; x < 16 * (HD / 32) / 32; ++x) {
+                const int id = lane + 32 * x, i = id % (HD / 32), tok = id / (HD / 32), key = lw * 16 + tok;
+                const uint32_t sc = lds32(raw + R::K_SCALES + (tok * GR + i / 2) * 4);
+                const __half2 dm = *reinterpret_cast<const __half2*>(&sc), d = __low2half2(dm), m = __high2half2(dm);
+                uint32_t w[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) w[c] = lds32(raw + R::k_word(tok, c, i));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int col = 4 * i + c;
+                    sts128(to + (col >> 3) * (QP_KEYS * 128) + key * 128 + (((col & 7) ^ (key & 7)) << 4), value2(w[0] >> (4 * c), d, m), value2(w[1] >> (4 * c), d, m),
+                           value2(w[2] >> (4 * c), d, m), value2(w[3] >> (4 * c), d, m));
+                }
+            }
+            // ---- values: a lane takes 16 dimensions of four tokens, from eight words of eight codes; what is not a number or beyond the last token is 0
+            if (lane < 4 * (HD / 16)) {
+                const int t4 = lane & 3, i = lane >> 2;
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = lds32(raw + (R::v_byte(2 * t4, e, i) & ~3));
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {      // byte b: token 2 t, 2 t + 8, 2 t + 1, 2 t + 9
+                    const int tok = 2 * t4 + 8 * (b & 1) + (b >> 1), key = lw * 16 + tok;
+                    uint32_t sc = lds32(raw + R::V_SCALES + (tok * GR + i / 4) * 4);
+                    const bool nan = (sc & 0x7FFFu) > 0x7C00u;
+                    if (pos + tok > last || nan) {
+                        if (nan && pos + tok <= last) atomicMin(&s_nan[i / 4], pos + tok);
+                        sc = 0;
+                    }
+                    const __half2 dm = *reinterpret_cast<const __half2*>(&sc), d = __low2half2(dm), m = __high2half2(dm);
+                    uint32_t pair[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pair[e] = __byte_perm(w[2 * e], w[2 * e + 1], b | (4 + b) << 8 | b << 4 | (4 + b) << 12);      // bytes (x, x, y, y)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int col = 2 * i + h;
+                        sts128(to + L::TILE + (col >> 3) * (QP_KEYS * 128) + key * 128 + (((col & 7) ^ (key & 7)) << 4), value2(pair[0] >> (4 * h), d, m), value2(pair[1] >> (4 * h), d, m),
+                               value2(pair[2] >> (4 * h), d, m), value2(pair[3] >> (4 * h), d, m));
+                    }
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(bar(QP_FULL, t % QP_STAGES));
+            mbar_arrive(bar(QP_READ, t % QP_RAW));
+            if (lw == 0 && t + QP_RAW < n_tiles) {      // the pages' place is free once all have read them
+                if (!wait(bar(QP_READ, t % QP_RAW), (t / QP_RAW) & 1)) break;
+                if (lt == 0) fetch(fetched++);
+            }
+        }
+        if (lt == 0)
+            for (; t < fetched; ++t) mbar_wait(bar(QP_PAGES, t % QP_RAW), (t / QP_RAW) & 1, nullptr);      // (given up: copies in flight)
+    } else {
+        // ------------------------------------------------------------------ products
+        const bool one = elect_one();
+        constexpr uint32_t id_s = umma_idesc_f16(QP_ROWS, QP_KEYS), id_o = umma_idesc_f16(QP_ROWS, HD) | (1u << 16);      // a value tile's rows are keys: N-major
+        auto scores = [&](int u, int t) {
+            if (one) {
+                const uint64_t q = umma_desc_sw128(sm + u * L::SET, 1024), k = umma_desc_sw128(sm + L::KV + (t % QP_STAGES) * (2 * L::TILE), 1024);
+                const uint32_t d = tmem + u * 256 + 64 * (t & 1);
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) umma_f16(d, q + ((i >> 2) * (QP_ROWS * 128) + 32 * (i & 3)) / 16, k + ((i >> 2) * (QP_KEYS * 128) + 32 * (i & 3)) / 16, id_s, i > 0);
+                umma_commit(bar(QP_S, 2 * u + (t & 1)));
+            }
+        };
+        auto values = [&](int u, int t) {
+            if (one) {
+                const uint64_t v = umma_desc_sw128_n(sm + L::KV + (t % QP_STAGES) * (2 * L::TILE) + L::TILE, QP_KEYS * 128, 1024);
+                const uint32_t d = tmem + u * 256 + 128, w = tmem + u * 256 + 64 * (t & 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) umma_f16_ts(d, w + 8 * i, v + (16 * 128 * i) / 16, id_o, 1);
+                umma_commit(bar(QP_O, u));
+            }
+        };
+        bool ok = wait(bar(QP_FULL, 0), 0);
+        if (ok) {
+            tc_fence_after();
+            for (int u = 0; u < sets; ++u) scores(u, 0);
+        }
+        // scores of tile t + 1 go where the weights of tile t - 1 were, once the product that reads those is complete
+        for (int t = 0; t < n_tiles && ok; ++t) {
+#pragma unroll 1
+            for (int u = 0; u < sets; ++u) {
+                if (ok && t + 1 < n_tiles) {
+                    if (u == 0) ok = wait(bar(QP_FULL, (t + 1) % QP_STAGES), ((t + 1) / QP_STAGES) & 1);
+                    if (ok && t > 0) ok = wait(bar(QP_O, u), (t - 1) & 1);
+                    tc_fence_after();
+                    if (ok) scores(u, t + 1);
+                }
+                ok = ok && wait(bar(QP_P, 2 * u + (t & 1)), (t >> 1) & 1);
+                tc_fence_after();
+                if (ok) values(u, t);
+            }
+            if (ok && one) umma_commit(bar(QP_FREE, t % QP_STAGES));
+        }
+        if (!ok) {      // products in flight still read shared and tensor memory
+            if (one) umma_commit(bar(QP_DRAIN));
+            mbar_wait_warp(bar(QP_DRAIN), 0);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// The parts of rows whose keys were split, added up: a warp per row of a tile, in the order of the parts.
+template <int HD>
+__global__ void __launch_bounds__(256) k_q4_join(const PromptParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
+    const int lane = threadIdx.x & 31, G = p.heads / p.n_kv, kvh = blockIdx.y, r = blockIdx.z * 8 + (threadIdx.x >> 5);
+    if ((int)blockIdx.x >= hd->n_tiles) return;
+    const dc_q4_tile tl = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles)[blockIdx.x];
+    if (tl.n_splits == 1 || tl.split != 0 || r >= tl.count * G - tl.row0) return;
+    constexpr size_t ROW = HD + 4, PART = 2 * QP_ROWS * ROW;
+    const float* from = reinterpret_cast<const float*>(p.plan + 4 * (size_t)hd->ws) + ((size_t)tl.ws * p.n_kv + (size_t)tl.n_splits * kvh) * PART + r * ROW;
+    constexpr int PER = HD / 32;
+    float M = -1e30f, l = 0.0f, v[PER] = {};
+    for (int s = 0; s < tl.n_splits; ++s) M = fmaxf(M, __ldcg(from + s * PART + HD));
+    for (int s = 0; s < tl.n_splits; ++s) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + s * PART + HD));
+        const float f = ex2(ml.x - M);
+        l = fmaf(ml.y, f, l);
+        if constexpr (PER == 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(from + s * PART) + lane);
+            v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]), v[2] = fmaf(x.z, f, v[2]), v[3] = fmaf(x.w, f, v[3]);
+        } else {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(from + s * PART) + lane);
+            v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]);
+        }
+    }
+    const float inv = 1.0f / l;
+    const int x = tl.row0 + r, j = x / G;
+    __nv_bfloat16* dst = p.out + (size_t)(tl.tok0 + j) * p.ldo + (size_t)(kvh * G + x - j * G) * HD + PER * lane;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) dst[i] = __float2bfloat16_rn(v[i] * inv);
+}
+
+template <int HD>
+int launch(dc_ctx* ctx, const dc_q4_call& c) {
+    const dc_q4& z = *c.kv->q4;
+    DC_TRY(dc_kernel_setup_unspilled(ctx, (const void*)k_q4_prompt<HD>, (int)Lay<HD>::SMEM, "k_q4_prompt"));
+    PromptParams p = {z.plan, (const __nv_bfloat16*)c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, (__nv_bfloat16*)c.out};
+    DC_TRY(dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(z.n_tiles, z.kv), dim3(QP_THREADS), Lay<HD>::SMEM, p, ctx->d_err));
+    if (!z.split_tiles) return DC_B200_OK;
+    return dc_launch(ctx, "k_q4_join", k_q4_join<HD>, dim3(z.n_tiles, z.kv, 2 * QP_ROWS / 8), dim3(256), 0, p);
+}
+
+}  // namespace
+
+int dc_launch_q4_prompt(dc_ctx* ctx, const dc_q4_call& c) {
+    if (c.kv->q4->n_tiles == 0) return DC_B200_OK;
+    return c.kv->q4->dim == 128 ? launch<128>(ctx, c) : launch<64>(ctx, c);
+}

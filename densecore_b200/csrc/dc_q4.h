@@ -40,9 +40,9 @@ struct dc_q4_item {
     int32_t split, n_splits, ws;      // of the tile; partial results at ws + split
     int32_t ticket, pad;
 };
-// One CTA's work in the prompt kernel: `rows` rows from `row0` of the entry on.
+// One CTA's work in k_q4_prompt: up to 256 rows from row0 of the entry on, key tiles (64 keys) tile0 .. tile1 - 1 of the ones that they see; partial results at ws + split.
 struct dc_q4_tile {
-    int32_t seq, pos0, tok0, count, row0, pad[3];
+    int32_t seq, pos0, tok0, count, row0, tile0, tile1, split, n_splits, ws, pad[2];
 };
 
 // `count` new tokens of a sequence from position pos0 on; the step's tokens tok0 ..
@@ -72,12 +72,32 @@ inline void dc_q4_items(const std::vector<dc_q4_entry>& es, int G, int n_kv, int
         }
 }
 
+// Entries of that many rows (new tokens times query heads of a key head) take the tensor-core kernel, for bf16 rows.
+constexpr int DC_Q4_PROMPT_ROWS = 64;
+
+// Tiles of the entries for k_q4_prompt, those with most keys first.  Keys are split where there are fewer tiles than SMs, into parts of eight key tiles at least.
+inline void dc_q4_tiles(const std::vector<dc_q4_entry>& es, int G, int n_kv, int num_sms, std::vector<dc_q4_tile>* tiles, int* n_ws) {
+    *n_ws = 0;
+    long long n = 0;
+    for (const dc_q4_entry& e : es) n += ((long long)e.count * G + 255) / 256;
+    const int most = n ? (int)std::max<long long>(1, num_sms / (n * n_kv)) : 1;
+    for (const dc_q4_entry& e : es)
+        for (int r = 0; r < e.count * G; r += 256) {
+            const int keys = (e.pos0 + (std::min(r + 256, e.count * G) - 1) / G) / 64 + 1, parts = std::max(1, std::min(most, keys / 8));
+            for (int s = 0; s < parts; ++s)
+                tiles->push_back({e.seq, e.pos0, e.tok0, e.count, r, (int)((long long)keys * s / parts), (int)((long long)keys * (s + 1) / parts), s, parts, parts > 1 ? *n_ws : 0, {0, 0}});
+            if (parts > 1) *n_ws += parts;
+        }
+    std::stable_sort(tiles->begin(), tiles->end(), [](const dc_q4_tile& a, const dc_q4_tile& b) { return a.tile1 - a.tile0 > b.tile1 - b.tile0; });
+}
+
 struct dc_q4 {
     int n_layer = 0, heads = 0, kv = 0, dim = 0, type = 0;
     // the newest plan: host copies of what launches need, and the block manager's state that it was made for
     bool planned = false;
     uint64_t edits = 0;
     int T = 0, n_items = 0, n_tiles = 0;
+    bool split_tiles = false;
     uint8_t* plan = nullptr;
     size_t plan_bytes = 0;
     std::vector<uint8_t*> retired;      // outgrown plans, emptied; captured calls may still read them

@@ -225,7 +225,7 @@ DC_B200_API int dc_b200_kv_read_block(dc_kv_cache* kv, int layer, int block, voi
 /* A cache whose rows are held in 4 bits, for serving many requests or long ones (no counterpart in DenseCore's
  * decode path).  A row of a key head is cut into groups of 64 values; a group has m = fp16(least value),
  * d = fp16((largest - least) * fp32(1/15)), codes q = rint((x - m) / d) within 0..15 in fp32 arithmetic (0 where d
- * is 0), and stands for fp32(d q + m).  A group with a value that is not finite or beyond +-65504 reads back as NaN.
+ * is 0), and stands for fp32(d q + m).  A group with a value that is not finite or beyond +-32768 reads back as NaN.
  * Head sizes 64 (36 bytes a row) and 128 (72).  n_head query heads share n_kv_head key heads evenly.  row_type: type
  * of queries, new rows and results, DC_GGML_TYPE_F32 or DC_GGML_TYPE_BF16; attention over F32 rows is exact to f32
  * rounding, over BF16 rows to bf16's.  All calls of the block manager above (sequences, fork, prefix cache, block

@@ -77,6 +77,49 @@ int main(int, char** v) {
     assert not tiles
 
 
+@pytest.mark.parametrize("G,n_kv", [(1, 1), (3, 2), (8, 4), (16, 1)])
+def test_prompt_tiles_cover_every_row_and_key_once(tmp_path, G, n_kv):
+    exe = _program(tmp_path, r"""
+int main(int, char** v) {
+    std::vector<dc_q4_entry> es = {{3, 0, 64, 0}, {0, 15, 2000, 64}, {1, 100000, 300, 2064}, {2, 63, 1, 2364}};
+    if (atoi(v[3])) es.resize(1), es.push_back({1, 100000, 300, 64});
+    std::vector<dc_q4_tile> tiles;
+    int ws;
+    dc_q4_tiles(es, atoi(v[1]), atoi(v[2]), 148, &tiles, &ws);
+    printf("%d\n", ws);
+    for (auto& t : tiles) printf("%d %d %d %d %d %d %d %d %d %d\n", t.seq, t.pos0, t.tok0, t.count, t.row0, t.tile0, t.tile1, t.split, t.n_splits, t.ws);
+}
+""")
+    for short in (0, 1):
+        lines = [[int(x) for x in line.split()] for line in subprocess.check_output([exe, str(G), str(n_kv), str(short)], text=True).splitlines()]
+        ws, taken, got = lines[0][0], set(), {}
+        for seq, pos0, tok0, count, row0, t0, t1, split, n, at in lines[1:]:
+            assert t0 < t1
+            got.setdefault((seq, pos0, count, row0), []).append((t0, t1, split, n))
+            if n > 1:
+                assert 0 <= at + split < ws and (at + split) not in taken
+                taken.add(at + split)
+        assert len(taken) == ws
+        sizes = [line[6] - line[5] for line in lines[1:]]
+        assert sizes == sorted(sizes, reverse=True)
+        for seq, pos0, count in ([(3, 0, 64), (0, 15, 2000), (1, 100000, 300), (2, 63, 1)] if not short else [(3, 0, 64), (1, 100000, 300)]):
+            for row0 in range(0, count * G, 256):
+                parts = sorted(got.pop((seq, pos0, count, row0)))
+                last = pos0 + (min(row0 + 256, count * G) - 1) // G
+                assert parts[0][0] == 0 and parts[-1][1] == last // 64 + 1 and all(x[1] == y[0] for x, y in zip(parts, parts[1:]))
+                assert [x[2] for x in parts] == list(range(len(parts))) and {x[3] for x in parts} == {len(parts)}
+        assert not got
+
+
+def test_the_prompt_kernel_is_built_without_spills(tmp_path):
+    """It loads from tensor memory: the launcher refuses a build that spills."""
+    import re
+    cmd = [B.nvcc(), "-Xptxas", "-v", *B.NVCC_FLAGS, "-I", os.path.join(B.ROOT, "include"), "-c", os.path.join(B.CSRC, "attn_q4_prompt.cu"), "-o", str(tmp_path / "o.o")]
+    out = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, check=True).stdout
+    seen = [body for name, body in re.findall(r"Compiling entry function '(\w+)'(.*?)(?=Compiling entry|\Z)", out, re.S) if "k_q4_prompt" in name]
+    assert len(seen) == 2 and all("0 bytes stack frame, 0 bytes spill stores, 0 bytes spill loads" in body for body in seen)
+
+
 def test_null_arguments_are_refused():
     import ctypes as C
     from densecore_b200 import _lib

@@ -3,7 +3,9 @@
 Rounding that the bounds count: a score is off by at most a (2^-22 of the two fp16 terms of a query + 2^-20 of its sums in f32), a = scale sum |q_i k_i|, and
 by 2^-22 of its own size in units of log2 e; a weight by that and 2^-21 of the exponential and the two terms; the answer, a mean of values, by twice the
 weights' relative error times the largest value.  bf16 rows: weights p d are rounded to fp16, by 2^-11 of themselves or 2^-25 of the row's largest, and codes d q
-reach no further than 2 max |v| (largest less least of a group): 2^-11 (2 max |v|) + n 2^-25 (2 max |v|) for n tokens; results add half a step, eps / 2 relative."""
+reach no further than 2 max |v| (largest less least of a group): 2^-11 (2 max |v|) + n 2^-25 (2 max |v|) for n tokens; results add half a step, eps / 2 relative.  Portions of 64 rows or more (new tokens times query heads of a key head) of bf16 rows take
+keys, values and weights as fp16: 2^-11 of a score's sum of magnitudes, and twice 2^-11 max |v|; over a whole result these are of random sign, so that its error's norm
+stays below bf16's own 2^-8 of the result's."""
 import numpy as np
 import pytest
 import torch
@@ -37,7 +39,7 @@ def unbits(x):
     return torch.from_numpy(x).view(torch.bfloat16).float().numpy()
 
 
-def attention(q, K, V, pos0, scale):
+def attention(q, K, V, pos0, scale, halves=False):
     """One sequence: q [n, heads, hd], K, V [pos0 + n, kv, hd].  Returns answers and the bound on their error, [n, heads, hd] both."""
     n, heads, hd = q.shape
     G = heads // K.shape[1]
@@ -51,7 +53,7 @@ def attention(q, K, V, pos0, scale):
             a = float(np.abs(scale) * (np.abs(k[:c]) @ np.abs(x)).max())
             w = np.exp(z - z.max())
             y[i, h] = w @ v[:c] / w.sum()
-            ds = a * (2.0 ** -22 + 2.0 ** -20) + 1.5 * float(np.abs(z).max()) * 2.0 ** -22
+            ds = a * (2.0 ** -22 + 2.0 ** -20 + halves * 2.0 ** -11) + 1.5 * float(np.abs(z).max()) * 2.0 ** -22
             tol[i, h] = (2 * (2 * ds + 2.0 ** -21) + 2.0 ** -20) * np.abs(v[:c]).max()
     return y, tol
 
@@ -88,7 +90,10 @@ class Mirror:
         return out
 
     def compare(self, out, q, s, p, scale, layer=0):
-        y, tol = attention(q, self.k[layer][s], self.v[layer][s], p, scale)
+        halves = self.dtype == "bf16" and len(q) * (self.heads // self.n_kv) >= 64
+        y, tol = attention(q, self.k[layer][s], self.v[layer][s], p, scale, halves)
+        if halves:
+            assert np.linalg.norm(out - y) <= 2.0 ** -8 * np.linalg.norm(y)
         if self.dtype == "bf16":
             v = np.abs(self.v[layer][s]).max()
             tol = tol + 2 * v * (2.0 ** -11 + len(self.v[layer][s]) * 2.0 ** -25)
@@ -133,6 +138,66 @@ def test_long_sequences_are_split_and_joined(ctx, dtype, hd, context):
     m.step(rng, [a, b], [0, 0], [context, 77], check=False)
     m.step(rng, [a, b], [context, 77], [1, 1])
     m.step(rng, [b, a], [78, context + 1], [2, 3])
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(4, 4, 128), (6, 2, 128), (8, 1, 128), (32, 4, 128), (16, 1, 64), (5, 1, 64)])
+def test_prompts(ctx, heads, kv, hd):
+    """Portions around the sizes of tiles (64 keys, 128 and 256 rows), first ones and later ones, beside decoded tokens and alone."""
+    rng = np.random.default_rng(heads + hd)
+    m = Mirror(ctx, "bf16", heads, kv, hd, 3, 160)
+    a, b, c = (m.cache.seq_alloc() for _ in range(3))
+    m.step(rng, [a], [0], [64])
+    m.step(rng, [b, a], [0, 64], [257, 1])
+    m.step(rng, [c, a, b], [0, 65, 257], [129, 128, 63])
+    m.step(rng, [b, c], [320, 129], [1, 300])
+    m.step(rng, [a], [193], [90])
+    for x in (a, b, c):
+        m.check_blocks(x)
+
+
+@pytest.mark.parametrize("heads,kv,hd,context,count", [(8, 4, 128, 2222, 40), (2, 1, 64, 3001, 70), (16, 2, 128, 1500, 200)])
+def test_prompts_behind_long_contexts_are_split(ctx, heads, kv, hd, context, count):
+    rng = np.random.default_rng(context)
+    m = Mirror(ctx, "bf16", heads, kv, hd, 2, (context + count) // 16 + 2)
+    a, b = m.cache.seq_alloc(), m.cache.seq_alloc()
+    m.step(rng, [a, b], [0, 0], [context, 500], check=False)
+    rows = m.rows(rng, count + 1)
+    first = m.step(rng, [a, b], [context, 500], [count, 1], rows=rows)
+    assert np.array_equal(m.step(rng, [a, b], [context, 500], [count, 1], rows=rows, check=False), first)
+    m.step(rng, [b], [501], [32], scale=-0.1)
+    m.step(rng, [b], [533], [64], scale=0.0)
+
+
+def test_a_nan_in_a_prompt_reaches_later_tokens_and_its_group_alone(ctx):
+    rng = np.random.default_rng(30)
+    m = Mirror(ctx, "bf16", 4, 2, 128, 1, 30)
+    a = m.cache.seq_alloc()
+    rows = m.rows(rng, 400)
+    rows[2][333, 1, 70] = np.nan         # a value: second group of head 1
+    rows[1][350, 0, 5] = np.inf          # a key of head 0
+    out = m.step(rng, [a], [0], [400], rows=rows, check=False)
+    want = np.zeros(out.shape, bool)
+    want[333:, 2:, 64:] = True
+    want[350:, :2] = True
+    assert np.array_equal(np.isnan(out), want)
+    k, v = held(rows[1]), held(rows[2])
+    y, _ = attention(rows[0][:333], k[:333], v[:333], 0, 128 ** -0.5)
+    assert np.linalg.norm(out[:333] - y) <= 2.0 ** -8 * np.linalg.norm(y)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_range_of_values(ctx, dtype):
+    """Up to 32768 in magnitude is held, beyond it a group is NaN."""
+    rng = np.random.default_rng(31)
+    m = Mirror(ctx, dtype, 2, 1, 64, 1, 10)
+    a = m.cache.seq_alloc()
+    q, k, v = m.rows(rng, 70)
+    k[3, 0, :2], v[5, 0, :2] = (32768, -32768), (32768, -32768)
+    m.step(rng, [a], [0], [70], rows=(q, k, v), scale=1e-6)
+    m.check_blocks(a)
+    v[5, 0, 0] = 33024
+    out = m.step(rng, [a], [0], [70], rows=(q, k, v), scale=1e-6, check=False)
+    assert np.all(np.isnan(out[5:])) and np.all(np.isfinite(out[:5]))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
