@@ -10,7 +10,7 @@
 //   bf16 rows: codes as they lie (fp16 subnormals c 2^-24 and c 2^-20, exact), queries as fp16 (exact: 8 bits), weights p d rounded to fp16 (half a step, 2^-11 relative,
 //   an eighth of a bf16 result's own).  Answers are made transposed, 16 dimensions x 8 rows, which fills the operand's sixteen rows with one word of codes a lane.
 // The running reference of a row's exponentials is the largest of score + log2 d (d of the token's value, at least 2^-24), not of the scores: the weights p d stay
-// within 1 whatever the values' size, and clear of fp16's least numbers.
+// within 64 whatever the values' size, and clear of fp16's least numbers.
 //   f32 rows: queries and weights as two fp16 terms (22 bits), rows h and h + 8 of one sixteen-row operand, so that they cost no extra product; codes as c - 8
 //   with m + 8 d in place of m: sums around zero, where c and m alone would leave answers as small differences of large sums (measured: 5e-5 of the result, now below 1e-6).
 #include <math.h>
@@ -363,7 +363,8 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
                 }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (__any_sync(0xffffffffu, mx > m_run)) {
+            // (the reference follows once it is 2^6 behind: weights up to 64 are as exact, and the answers' factors are rare)
+            if (__any_sync(0xffffffffu, mx > m_run + 6.0f)) {
                 const float m_new = fmaxf(m_run, mx), corr = ex2(m_run - m_new);
                 m_run = m_new;
                 l *= corr;

@@ -5,8 +5,9 @@
 // set two tiles of scores of 64 columns, whose first 32 then hold the weights as fp16 pairs, and HD columns of answers; the next tile's scores are made while a
 // thread per row weights this one's.
 //   warps 0-7    weights: four a set, thread = row = tensor-memory lane
-//   warps 8-11   pages by bulk copies, codes turned into fp16 rows of the operands' 128-byte swizzle (d c + m, rounded once: 2^-11 relative)
-//   warp 12      issues the products
+//   warps 8-15   pages by bulk copies, codes turned into fp16 rows of the operands' 128-byte swizzle (d c + m, rounded once: 2^-11 relative); a warp has the keys
+//                or the values of one page
+//   warp 16      issues the products
 // Queries are bf16 rows times a power of two (exact in fp16), weights fp16 (2^-11): together below a bf16 result's own 2^-8.
 // A value that is not a number (d = m = NaN) enters the tiles as 0, or the products would carry it to rows that do not see it; the CTA keeps the first
 // position of such a value per group of 64 dimensions, and rows that see it end as NaN there.
@@ -63,7 +64,7 @@ struct PromptParams {
     __nv_bfloat16* out;
 };
 
-constexpr int QP_ROWS = 128, QP_KEYS = 64, QP_STAGES = 4, QP_RAW = 3, QP_THREADS = 13 * 32;
+constexpr int QP_ROWS = 128, QP_KEYS = 64, QP_STAGES = 4, QP_RAW = 3, QP_THREADS = 17 * 32;
 enum QpBar { QP_FULL = 0, QP_FREE = 4, QP_S = 8, QP_P = 12, QP_O = 16, QP_DRAIN = 18, QP_PAGES = 19, QP_READ = 22, QP_NBARS = 25 };
 template <int HD>
 struct Lay {
@@ -82,20 +83,20 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
     __shared__ int s_nan[2];
     __shared__ float s_pow[2 * QP_ROWS];      // 2^e of a row
     pdl_wait();
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.y, G = p.heads / p.n_kv;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.x, G = p.heads / p.n_kv;
     const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
-    if ((int)blockIdx.x >= hd->n_tiles) return;      // (a replay on a smaller step)
-    const dc_q4_tile tl = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles)[blockIdx.x];
+    if ((int)blockIdx.y >= hd->n_tiles) return;      // (a replay on a smaller step)
+    const dc_q4_tile tl = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles)[blockIdx.y];
     const int rows = min(2 * QP_ROWS, tl.count * G - tl.row0), sets = rows > QP_ROWS ? 2 : 1;
     const int last = tl.pos0 + (tl.row0 + rows - 1) / G, first_tile = tl.tile0, n_tiles = tl.tile1 - tl.tile0;
     const uint32_t sm = (smem_u32(smem) + 1023u) & ~1023u;
     auto bar = [sm](int which, int i = 0) -> uint32_t { return sm + L::BARS + 8u * (uint32_t)(which + i); };
-    if (warp == 12) {
+    if (warp == 16) {
         tmem_alloc(smem_u32(&s_tmem), 512);
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < QP_NBARS; ++i) mbar_init(bar(i), i < QP_FREE || i >= QP_READ ? 128 : i >= QP_P && i < QP_O ? 4 : 1);
+        for (int i = 0; i < QP_NBARS; ++i) mbar_init(bar(i), i < QP_FREE || i >= QP_READ ? 256 : i >= QP_P && i < QP_O ? 4 : 1);
         mbar_fence_init();
         s_nan[0] = s_nan[1] = 0x7fffffff;
     }
@@ -170,27 +171,32 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                 ok = wait(bar(QP_S, 2 * u + (t & 1)), (t >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
-                int x[4][16];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld16(t_s + 16 * c, x[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
-                auto s = [&](int i) -> float { return __int_as_float(x[i >> 4][i & 15]); };
                 const int k0 = (first_tile + t) * QP_KEYS;
-                if (k0 + QP_KEYS - 1 > all_see) {
+                const bool masked = k0 + QP_KEYS - 1 > all_see;
+                int x[2][16];      // 32 scores at a time, once for their largest and once for the weights: all 64 would not stay in registers
+                auto s = [&](int i) -> float { return __int_as_float(x[i >> 4][i & 15]); };
+                auto load = [&](int h) {
+                    tmem_ld16(t_s + 32 * h, x[0]);
+                    tmem_ld16(t_s + 32 * h + 16, x[1]);
+                    tmem_ld_wait(x[0]);
+                    tmem_ld_wait(x[1]);
+                    if (masked) {
 #pragma unroll
-                    for (int i = 0; i < QP_KEYS; ++i)
-                        if (k0 + i > qp) x[i >> 4][i & 15] = __float_as_int(-INFINITY);
-                }
-                float mx[4];
+                        for (int i = 0; i < 32; ++i)
+                            if (k0 + 32 * h + i > qp) x[i >> 4][i & 15] = __float_as_int(-INFINITY);
+                    }
+                };
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    mx[c] = s(16 * c);
+                for (int h = 0; h < 2; ++h) {
+                    __syncwarp();
+                    load(h);
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) mx[c] = fmaxf(mx[c], s(16 * c + i));
+                    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s(i));
                 }
                 const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
-                if (__any_sync(0xffffffffu, m_new > m_run)) {
+                // the reference follows the largest score once that is 2^8 above it: weights up to 256 are as exact, and the answers' factors are rare
+                if (__any_sync(0xffffffffu, m_new > m_run + 8.0f)) {
                     const float corr = ex2(m_run - m_new);
                     m_run = m_new;
 #pragma unroll
@@ -211,17 +217,19 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                         }
                     }
                 }
-                __syncwarp();      // masks are a lane's own, the stores are the whole warp's
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t w[16];
+                    __syncwarp();      // masks are a lane's own, loads and stores are the whole warp's
+                    load(h);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float a = ex2(fmaf(s(32 * h + 2 * i), sl2, -m_run)), b = ex2(fmaf(s(32 * h + 2 * i + 1), sl2, -m_run));
+                        const float a = ex2(fmaf(s(2 * i), sl2, -m_run)), b = ex2(fmaf(s(2 * i + 1), sl2, -m_run));
                         l_run[i & 3] += a + b;
                         w[i] = pack_h2(a, b);
                     }
-                    tmem_st16(t_s + 16 * h, w);
+                    __syncwarp();
+                    tmem_st16(t_s + 16 * h, w);      // (columns whose scores have been read)
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -266,9 +274,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                 }
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         // ------------------------------------------------------------------ key and value tiles
-        const int lt = tid - 256, lw = lt >> 5;
+        const int lt = tid - 256, lw = lt >> 5 & 3;      // a warp has one page
         const int32_t* table = p.tables + (size_t)tl.seq * p.max_blocks;
         const int last_page = last / DC_KV_BLOCK;
         auto fetch = [&](int t) {      // one thread: the four pages of a tile (those beyond the last token: the last page, for something finite)
@@ -288,55 +296,60 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
             if (ok && t >= QP_STAGES) ok = wait(bar(QP_FREE, t % QP_STAGES), (t / QP_STAGES - 1) & 1);
             if (!ok) break;
             const uint32_t to = sm + L::KV + (t % QP_STAGES) * (2 * L::TILE);
-            const uint32_t raw = sm + L::RAW + (t % QP_RAW) * L::RAW_BYTES + lw * R::BYTES;      // a warp has one page
+            const uint32_t raw = sm + L::RAW + (t % QP_RAW) * L::RAW_BYTES + lw * R::BYTES;
             const int pos = (first_tile + t) * QP_KEYS + lw * DC_KV_BLOCK;
-            // ---- keys: a lane takes 32 dimensions of one token, from four words that lie 16 bytes apart
+            if (warp < 12) {
+                // ---- keys: a lane takes 32 dimensions of one token at a time, from four words that lie 16 bytes apart
+                constexpr int N = HD / 64;
+                uint32_t w[N][4], sc[N];
 #pragma unroll
-            for (int x = 0; x < 16 * (HD / 32) / 32; ++x) {
-                const int id = lane + 32 * x, i = id % (HD / 32), tok = id / (HD / 32), key = lw * 16 + tok;
-                const uint32_t sc = lds32(raw + R::K_SCALES + (tok * GR + i / 2) * 4);
-                const __half2 dm = *reinterpret_cast<const __half2*>(&sc), d = __low2half2(dm), m = __high2half2(dm);
-                uint32_t w[4];
+                for (int x = 0; x < N; ++x) {      // (all loads ahead of the stores, which they may not pass)
+                    const int id = lane + 32 * x, i = id % (HD / 32), tok = id / (HD / 32);
+                    sc[x] = lds32(raw + R::K_SCALES + (tok * GR + i / 2) * 4);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) w[c] = lds32(raw + R::k_word(tok, c, i));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int col = 4 * i + c;
-                    sts128(to + (col >> 3) * (QP_KEYS * 128) + key * 128 + (((col & 7) ^ (key & 7)) << 4), value2(w[0] >> (4 * c), d, m), value2(w[1] >> (4 * c), d, m),
-                           value2(w[2] >> (4 * c), d, m), value2(w[3] >> (4 * c), d, m));
+                    for (int c = 0; c < 4; ++c) w[x][c] = lds32(raw + R::k_word(tok, c, i));
                 }
-            }
-            // ---- values: a lane takes 16 dimensions of four tokens, from eight words of eight codes; what is not a number or beyond the last token is 0
-            if (lane < 4 * (HD / 16)) {
+#pragma unroll
+                for (int x = 0; x < N; ++x) {
+                    const int id = lane + 32 * x, i = id % (HD / 32), tok = id / (HD / 32), key = lw * 16 + tok;
+                    const __half2 dm = *reinterpret_cast<const __half2*>(&sc[x]), d = __low2half2(dm), m = __high2half2(dm);
+                    const uint32_t at = to + (i >> 1) * (QP_KEYS * 128) + key * 128;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        sts128(at + (((4 * (i & 1) + c) ^ (key & 7)) << 4), value2(w[x][0] >> (4 * c), d, m), value2(w[x][1] >> (4 * c), d, m), value2(w[x][2] >> (4 * c), d, m),
+                               value2(w[x][3] >> (4 * c), d, m));
+                }
+            } else if (lane < 4 * (HD / 16)) {
+                // ---- values: a lane takes 16 dimensions of four tokens, from eight words of eight codes; what is not a number or beyond the last token is 0
                 const int t4 = lane & 3, i = lane >> 2;
-                uint32_t w[8];
+                uint32_t w[8], sc[4];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = lds32(raw + (R::v_byte(2 * t4, e, i) & ~3));
 #pragma unroll
+                for (int b = 0; b < 4; ++b) sc[b] = lds32(raw + R::V_SCALES + ((2 * t4 + 8 * (b & 1) + (b >> 1)) * GR + i / 4) * 4);
+#pragma unroll
                 for (int b = 0; b < 4; ++b) {      // byte b: token 2 t, 2 t + 8, 2 t + 1, 2 t + 9
                     const int tok = 2 * t4 + 8 * (b & 1) + (b >> 1), key = lw * 16 + tok;
-                    uint32_t sc = lds32(raw + R::V_SCALES + (tok * GR + i / 4) * 4);
-                    const bool nan = (sc & 0x7FFFu) > 0x7C00u;
+                    const bool nan = (sc[b] & 0x7FFFu) > 0x7C00u;
                     if (pos + tok > last || nan) {
                         if (nan && pos + tok <= last) atomicMin(&s_nan[i / 4], pos + tok);
-                        sc = 0;
+                        sc[b] = 0;
                     }
-                    const __half2 dm = *reinterpret_cast<const __half2*>(&sc), d = __low2half2(dm), m = __high2half2(dm);
+                    const __half2 dm = *reinterpret_cast<const __half2*>(&sc[b]), d = __low2half2(dm), m = __high2half2(dm);
                     uint32_t pair[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) pair[e] = __byte_perm(w[2 * e], w[2 * e + 1], b | (4 + b) << 8 | b << 4 | (4 + b) << 12);      // bytes (x, x, y, y)
+                    const uint32_t at = to + L::TILE + (i >> 2) * (QP_KEYS * 128) + key * 128;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int col = 2 * i + h;
-                        sts128(to + L::TILE + (col >> 3) * (QP_KEYS * 128) + key * 128 + (((col & 7) ^ (key & 7)) << 4), value2(pair[0] >> (4 * h), d, m), value2(pair[1] >> (4 * h), d, m),
-                               value2(pair[2] >> (4 * h), d, m), value2(pair[3] >> (4 * h), d, m));
-                    }
+                    for (int h = 0; h < 2; ++h)
+                        sts128(at + (((2 * (i & 3) + h) ^ (key & 7)) << 4), value2(pair[0] >> (4 * h), d, m), value2(pair[1] >> (4 * h), d, m), value2(pair[2] >> (4 * h), d, m),
+                               value2(pair[3] >> (4 * h), d, m));
                 }
             }
             fence_async_smem();
             mbar_arrive(bar(QP_FULL, t % QP_STAGES));
             mbar_arrive(bar(QP_READ, t % QP_RAW));
-            if (lw == 0 && t + QP_RAW < n_tiles) {      // the pages' place is free once all have read them
+            if (warp == 8 && t + QP_RAW < n_tiles) {      // the pages' place is free once all have read them
                 if (!wait(bar(QP_READ, t % QP_RAW), (t / QP_RAW) & 1)) break;
                 if (lt == 0) fetch(fetched++);
             }
@@ -393,7 +406,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 // The parts of rows whose keys were split, added up: a warp per row of a tile, in the order of the parts.
@@ -435,7 +448,7 @@ int launch(dc_ctx* ctx, const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
     DC_TRY(dc_kernel_setup_unspilled(ctx, (const void*)k_q4_prompt<HD>, (int)Lay<HD>::SMEM, "k_q4_prompt"));
     PromptParams p = {z.plan, (const __nv_bfloat16*)c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, (__nv_bfloat16*)c.out};
-    DC_TRY(dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(z.n_tiles, z.kv), dim3(QP_THREADS), Lay<HD>::SMEM, p, ctx->d_err));
+    DC_TRY(dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(z.kv, z.n_tiles), dim3(QP_THREADS), Lay<HD>::SMEM, p, ctx->d_err));
     if (!z.split_tiles) return DC_B200_OK;
     return dc_launch(ctx, "k_q4_join", k_q4_join<HD>, dim3(z.n_tiles, z.kv, 2 * QP_ROWS / 8), dim3(256), 0, p);
 }
