@@ -6,7 +6,7 @@
 // thread per row weights this one's.
 //   warps 0-7    weights: four a set, thread = row = tensor-memory lane
 //   warps 8-15   pages by bulk copies, codes turned into fp16 rows of the operands' 128-byte swizzle (d c + m, rounded once: 2^-11 relative); a warp has the keys
-//                or the values of one page
+//                or the values of one page, values turned (rows are dimensions: products with keys along the rows took three times as long to issue)
 //   warp 16      issues the products
 // Queries are bf16 rows times a power of two (exact in fp16), weights fp16 (2^-11): together below a bf16 result's own 2^-8.
 // A value that is not a number (d = m = NaN) enters the tiles as 0, or the products would carry it to rows that do not see it; the CTA keeps the first
@@ -47,11 +47,20 @@ __device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ __half2 as_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 // two codes in the halves' low four bits, anything above: d c + m
 __device__ __forceinline__ uint32_t value2(uint32_t w, __half2 d, __half2 m) {
-    const uint32_t x = (w & 0x000F000Fu) | 0x64006400u;      // 1024 + c
-    const __half2 v = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(-1024.0f, -1024.0f)), d, m);
+    const __half2 v = __hfma2(__hadd2(as_h2((w & 0x000F000Fu) | 0x64006400u), __floats2half2_rn(-1024.0f, -1024.0f)), d, m);      // 1024 + c - 1024
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Four words 16 bytes apart, from lanes whose places differ by 64 bytes: each lane starts at another one of the four, so that the lanes meet in no bank.
+__device__ __forceinline__ void lds_turned(uint32_t at, int turn, uint32_t (&w)[4]) {
+    uint32_t x[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) x[c] = lds32(at + ((c + turn) & 3) * 16);
+    const bool odd = turn & 1, two = turn & 2;
+    const uint32_t y0 = odd ? x[3] : x[0], y1 = odd ? x[0] : x[1], y2 = odd ? x[1] : x[2], y3 = odd ? x[2] : x[3];
+    w[0] = two ? y2 : y0, w[1] = two ? y3 : y1, w[2] = two ? y0 : y2, w[3] = two ? y1 : y3;
 }
 
 struct PromptParams {
@@ -276,21 +285,26 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
         }
     } else if (warp < 16) {
         // ------------------------------------------------------------------ key and value tiles
-        const int lt = tid - 256, lw = lt >> 5 & 3;      // a warp has one page
+        const int lw = warp & 3;      // a warp has one page
         const int32_t* table = p.tables + (size_t)tl.seq * p.max_blocks;
         const int last_page = last / DC_KV_BLOCK;
-        auto fetch = [&](int t) {      // one thread: the four pages of a tile (those beyond the last token: the last page, for something finite)
-            const uint32_t b = bar(QP_PAGES, t % QP_RAW);
-            mbar_expect_tx(b, L::RAW_BYTES);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int page = min((first_tile + t) * 4 + i, last_page);
-                bulk_g2s(sm + L::RAW + (t % QP_RAW) * L::RAW_BYTES + i * R::BYTES, p.arena + ((size_t)table[page] * p.n_kv + kvh) * R::BYTES, R::BYTES, b);
-            }
+        // warp 8, lanes 0-3: a page each of a tile (those beyond the last token: the last page, for something finite); the block of the next fetch is read ahead
+        int fetched = 0, t = 0, block = 0;
+        auto look_up = [&](int t) {
+            if (lane < 4 && t < n_tiles) block = table[min((first_tile + t) * 4 + lane, last_page)];
         };
-        int fetched = 0, t = 0;
-        if (lt == 0)
-            for (; fetched < QP_RAW && fetched < n_tiles; ++fetched) fetch(fetched);
+        auto fetch = [&] {
+            const uint32_t b = bar(QP_PAGES, fetched % QP_RAW);
+            if (lane == 0) mbar_expect_tx(b, L::RAW_BYTES);
+            __syncwarp();
+            if (lane < 4)
+                bulk_g2s(sm + L::RAW + (fetched % QP_RAW) * L::RAW_BYTES + lane * R::BYTES, p.arena + ((size_t)block * p.n_kv + kvh) * R::BYTES, R::BYTES, b);
+            look_up(++fetched);
+        };
+        if (warp == 8) {
+            look_up(0);
+            while (fetched < QP_RAW && fetched < n_tiles) fetch();
+        }
         for (; t < n_tiles; ++t) {
             bool ok = wait(bar(QP_PAGES, t % QP_RAW), (t / QP_RAW) & 1);
             if (ok && t >= QP_STAGES) ok = wait(bar(QP_FREE, t % QP_STAGES), (t / QP_STAGES - 1) & 1);
@@ -299,70 +313,85 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
             const uint32_t raw = sm + L::RAW + (t % QP_RAW) * L::RAW_BYTES + lw * R::BYTES;
             const int pos = (first_tile + t) * QP_KEYS + lw * DC_KV_BLOCK;
             if (warp < 12) {
-                // ---- keys: a lane takes 32 dimensions of one token at a time, from four words that lie 16 bytes apart
+                // ---- keys: rows of the operand are tokens; a lane takes 32 dimensions of one token at a time
                 constexpr int N = HD / 64;
                 uint32_t w[N][4], sc[N];
+                const int i = HD == 128 ? lane >> 3 : lane >> 4;
 #pragma unroll
                 for (int x = 0; x < N; ++x) {      // (all loads ahead of the stores, which they may not pass)
-                    const int id = lane + 32 * x, i = id % (HD / 32), tok = id / (HD / 32);
+                    const int tok = HD == 128 ? (lane & 7) + 8 * x : lane & 15;
                     sc[x] = lds32(raw + R::K_SCALES + (tok * GR + i / 2) * 4);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) w[x][c] = lds32(raw + R::k_word(tok, c, i));
+                    lds_turned(raw + R::k_word(tok, 0, i), (tok & 7) >> 1, w[x]);
                 }
 #pragma unroll
                 for (int x = 0; x < N; ++x) {
-                    const int id = lane + 32 * x, i = id % (HD / 32), tok = id / (HD / 32), key = lw * 16 + tok;
-                    const __half2 dm = *reinterpret_cast<const __half2*>(&sc[x]), d = __low2half2(dm), m = __high2half2(dm);
+                    const int tok = HD == 128 ? (lane & 7) + 8 * x : lane & 15, key = lw * 16 + tok;
+                    const __half2 dm = as_h2(sc[x]), d = __low2half2(dm), m = __high2half2(dm);
                     const uint32_t at = to + (i >> 1) * (QP_KEYS * 128) + key * 128;
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
                         sts128(at + (((4 * (i & 1) + c) ^ (key & 7)) << 4), value2(w[x][0] >> (4 * c), d, m), value2(w[x][1] >> (4 * c), d, m), value2(w[x][2] >> (4 * c), d, m),
                                value2(w[x][3] >> (4 * c), d, m));
                 }
-            } else if (lane < 4 * (HD / 16)) {
-                // ---- values: a lane takes 16 dimensions of four tokens, from eight words of eight codes; what is not a number or beyond the last token is 0
-                const int t4 = lane & 3, i = lane >> 2;
-                uint32_t w[8], sc[4];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = lds32(raw + (R::v_byte(2 * t4, e, i) & ~3));
-#pragma unroll
-                for (int b = 0; b < 4; ++b) sc[b] = lds32(raw + R::V_SCALES + ((2 * t4 + 8 * (b & 1) + (b >> 1)) * GR + i / 4) * 4);
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {      // byte b: token 2 t, 2 t + 8, 2 t + 1, 2 t + 9
-                    const int tok = 2 * t4 + 8 * (b & 1) + (b >> 1), key = lw * 16 + tok;
-                    const bool nan = (sc[b] & 0x7FFFu) > 0x7C00u;
+            } else {
+                // ---- values: rows of the operand are dimensions; a lane takes the page's 16 tokens of two dimensions, 8 apart, at a time
+                const uint32_t scales = raw + R::V_SCALES;
+                if (lane < 16 * GR) {      // what is not a number or beyond the last token is 0
+                    const int tok = lane / GR;
+                    const bool nan = (lds32(scales + 4 * lane) & 0x7FFFu) > 0x7C00u;
                     if (pos + tok > last || nan) {
-                        if (nan && pos + tok <= last) atomicMin(&s_nan[i / 4], pos + tok);
-                        sc[b] = 0;
+                        if (nan && pos + tok <= last) atomicMin(&s_nan[lane % GR], pos + tok);
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(scales + 4 * lane), "r"(0) : "memory");
                     }
-                    const __half2 dm = *reinterpret_cast<const __half2*>(&sc[b]), d = __low2half2(dm), m = __high2half2(dm);
-                    uint32_t pair[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) pair[e] = __byte_perm(w[2 * e], w[2 * e + 1], b | (4 + b) << 8 | b << 4 | (4 + b) << 12);      // bytes (x, x, y, y)
-                    const uint32_t at = to + L::TILE + (i >> 2) * (QP_KEYS * 128) + key * 128;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        sts128(at + (((2 * (i & 3) + h) ^ (key & 7)) << 4), value2(pair[0] >> (4 * h), d, m), value2(pair[1] >> (4 * h), d, m), value2(pair[2] >> (4 * h), d, m),
-                               value2(pair[3] >> (4 * h), d, m));
                 }
+                __syncwarp();
+                constexpr int N = HD / 64;
+                const int d8 = lane & 7;
+                uint32_t w[N][4], sc[16 * GR];
+#pragma unroll
+                for (int x = 0; x < N; ++x) lds_turned(raw + (R::v_byte(0, d8, (lane >> 3) + 4 * x)), d8 >> 1, w[x]);
+#pragma unroll
+                for (int x = 0; x < 16 * GR / 4; ++x) {
+                    const uint4 f = lds128(scales + 16 * x);
+                    sc[4 * x] = f.x, sc[4 * x + 1] = f.y, sc[4 * x + 2] = f.z, sc[4 * x + 3] = f.w;
+                }
+#pragma unroll
+                for (int x = 0; x < N; ++x)
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {      // tokens 8 a .. 8 a + 7
+                        __half2 d[4], m[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t u = sc[(8 * a + 2 * c) * GR + x], v = sc[(8 * a + 2 * c + 1) * GR + x];
+                            d[c] = as_h2(__byte_perm(u, v, 0x5410)), m[c] = as_h2(__byte_perm(u, v, 0x7632));
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int dim = 16 * ((lane >> 3) + 4 * x) + 8 * h + d8, sh = 8 * a + 4 * h;
+                            sts128(to + L::TILE + dim * 128 + (((2 * lw + a) ^ d8) << 4), value2(w[x][0] >> sh, d[0], m[0]), value2(w[x][1] >> sh, d[1], m[1]), value2(w[x][2] >> sh, d[2], m[2]),
+                                   value2(w[x][3] >> sh, d[3], m[3]));
+                        }
+                    }
             }
             fence_async_smem();
             mbar_arrive(bar(QP_FULL, t % QP_STAGES));
             mbar_arrive(bar(QP_READ, t % QP_RAW));
             if (warp == 8 && t + QP_RAW < n_tiles) {      // the pages' place is free once all have read them
                 if (!wait(bar(QP_READ, t % QP_RAW), (t / QP_RAW) & 1)) break;
-                if (lt == 0) fetch(fetched++);
+                fetch();
             }
         }
-        if (lt == 0)
+        if (warp == 8 && lane == 0)
             for (; t < fetched; ++t) mbar_wait(bar(QP_PAGES, t % QP_RAW), (t / QP_RAW) & 1, nullptr);      // (given up: copies in flight)
     } else {
         // ------------------------------------------------------------------ products
         const bool one = elect_one();
-        constexpr uint32_t id_s = umma_idesc_f16(QP_ROWS, QP_KEYS), id_o = umma_idesc_f16(QP_ROWS, HD) | (1u << 16);      // a value tile's rows are keys: N-major
+        constexpr uint32_t id_s = umma_idesc_f16(QP_ROWS, QP_KEYS), id_o = umma_idesc_f16(QP_ROWS, HD);
+        // descriptors of both sets' queries and of every stage's keys and values differ in the address alone: made once, added to
+        const uint64_t dq = umma_desc_sw128(sm, 1024), dk = umma_desc_sw128(sm + L::KV, 1024), dv = umma_desc_sw128(sm + L::KV + L::TILE, 1024);
         auto scores = [&](int u, int t) {
             if (one) {
-                const uint64_t q = umma_desc_sw128(sm + u * L::SET, 1024), k = umma_desc_sw128(sm + L::KV + (t % QP_STAGES) * (2 * L::TILE), 1024);
+                const uint64_t q = dq + u * (L::SET / 16), k = dk + (t % QP_STAGES) * (2 * L::TILE / 16);
                 const uint32_t d = tmem + u * 256 + 64 * (t & 1);
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i) umma_f16(d, q + ((i >> 2) * (QP_ROWS * 128) + 32 * (i & 3)) / 16, k + ((i >> 2) * (QP_KEYS * 128) + 32 * (i & 3)) / 16, id_s, i > 0);
@@ -371,22 +400,24 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
         };
         auto values = [&](int u, int t) {
             if (one) {
-                const uint64_t v = umma_desc_sw128_n(sm + L::KV + (t % QP_STAGES) * (2 * L::TILE) + L::TILE, QP_KEYS * 128, 1024);
+                const uint64_t v = dv + (t % QP_STAGES) * (2 * L::TILE / 16);
                 const uint32_t d = tmem + u * 256 + 128, w = tmem + u * 256 + 64 * (t & 1);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) umma_f16_ts(d, w + 8 * i, v + (16 * 128 * i) / 16, id_o, 1);
+                for (int i = 0; i < 4; ++i) umma_f16_ts(d, w + 8 * i, v + 2 * i, id_o, 1);
                 umma_commit(bar(QP_O, u));
             }
         };
         bool ok = wait(bar(QP_FULL, 0), 0);
         if (ok) {
             tc_fence_after();
-            for (int u = 0; u < sets; ++u) scores(u, 0);
+            scores(0, 0);
+            if (sets > 1) scores(1, 0);
         }
         // scores of tile t + 1 go where the weights of tile t - 1 were, once the product that reads those is complete
         for (int t = 0; t < n_tiles && ok; ++t) {
-#pragma unroll 1
-            for (int u = 0; u < sets; ++u) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (u == 1 && sets == 1) break;
                 if (ok && t + 1 < n_tiles) {
                     if (u == 0) ok = wait(bar(QP_FULL, (t + 1) % QP_STAGES), ((t + 1) / QP_STAGES) & 1);
                     if (ok && t > 0) ok = wait(bar(QP_O, u), (t - 1) & 1);
