@@ -74,7 +74,7 @@ struct PromptParams {
 };
 
 constexpr int QP_ROWS = 128, QP_KEYS = 64, QP_STAGES = 4, QP_RAW = 3, QP_THREADS = 17 * 32;
-enum QpBar { QP_FULL = 0, QP_FREE = 4, QP_S = 8, QP_P = 12, QP_O = 16, QP_DRAIN = 18, QP_PAGES = 19, QP_READ = 22, QP_NBARS = 25 };
+enum QpBar { QP_FULL = 0, QP_FREE = 4, QP_S = 8, QP_P = 12, QP_O = 16, QP_DRAIN = 18, QP_PAGES = 19, QP_READ = 22, QP_QUERY = 25, QP_NBARS = 26 };
 template <int HD>
 struct Lay {
     static constexpr uint32_t SET = QP_ROWS * HD * 2, TILE = QP_KEYS * HD * 2;      // a set's queries; keys or values of a tile: halves of 64 columns
@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.x, G = p.heads / p.n_kv;
     const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
     if ((int)blockIdx.y >= hd->n_tiles) return;      // (a replay on a smaller step)
-    const dc_q4_tile tl = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles)[blockIdx.y];
+    const dc_q4_tile* tp = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles) + blockIdx.y;
+    const dc_q4_tile tl = *tp;
     const int rows = min(2 * QP_ROWS, tl.count * G - tl.row0), sets = rows > QP_ROWS ? 2 : 1;
     const int last = tl.pos0 + (tl.row0 + rows - 1) / G, first_tile = tl.tile0, n_tiles = tl.tile1 - tl.tile0;
     const uint32_t sm = (smem_u32(smem) + 1023u) & ~1023u;
@@ -105,50 +106,10 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < QP_NBARS; ++i) mbar_init(bar(i), i < QP_FREE || i >= QP_READ ? 256 : i >= QP_P && i < QP_O ? 4 : 1);
+        for (int i = 0; i < QP_NBARS; ++i) mbar_init(bar(i), i == QP_QUERY ? sets * QP_ROWS : i < QP_FREE || i >= QP_READ ? 256 : i >= QP_P && i < QP_O ? 4 : 1);
         mbar_fence_init();
         s_nan[0] = s_nan[1] = 0x7fffffff;
     }
-    auto row_of = [&](int r) -> const __nv_bfloat16* {      // a row's query, or null
-        if (r >= rows) return nullptr;
-        const int x = tl.row0 + r, j = x / G;
-        return p.q + (size_t)(tl.tok0 + j) * p.ldq + (size_t)(kvh * G + x - j * G) * HD;
-    };
-    // ---- queries: a row times 2^-e, 2^e <= its largest < 2^(e + 1), four threads a row
-    if (tid < 384) {
-        constexpr int PER = HD / 4;
-        const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
-        for (int r = tid >> 2; r < 2 * QP_ROWS; r += 96) {
-            const __nv_bfloat16* src = row_of(r);
-            float x[PER], most = 0.0f;
-            const int d0 = (tid & 3) * PER;
-            if (src && (((uintptr_t)(src + d0)) & 3) == 0) {
-#pragma unroll
-                for (int i = 0; i < PER; i += 2) {
-                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + d0 + i));
-                    x[i] = f.x, x[i + 1] = f.y;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < PER; ++i) x[i] = src ? __bfloat162float(src[d0 + i]) : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < PER; ++i) most = fmaxf(most, fabsf(x[i]));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int e = max(-100, min(100, (int)(__float_as_uint(most) >> 23) - 127));
-            const float up = __uint_as_float((uint32_t)(127 - e) << 23) * sign;
-            if ((tid & 3) == 0) s_pow[r] = __uint_as_float((uint32_t)(127 + e) << 23);
-            const uint32_t base = sm + (r >> 7) * L::SET + (r & 127) * 128;
-#pragma unroll
-            for (int c = 0; c < PER / 8; ++c) {
-                const int col = (d0 >> 3) + c;
-                sts128(base + (col >> 3) * (QP_ROWS * 128) + (((col & 7) ^ (r & 7)) << 4), pack_h2(x[8 * c] * up, x[8 * c + 1] * up), pack_h2(x[8 * c + 2] * up, x[8 * c + 3] * up),
-                       pack_h2(x[8 * c + 4] * up, x[8 * c + 5] * up), pack_h2(x[8 * c + 6] * up, x[8 * c + 7] * up));
-            }
-        }
-    }
-    fence_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -165,9 +126,65 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
         if (u < sets) {
             const uint32_t t_unit = tmem + u * 256 + ((uint32_t)(32 * (warp & 3)) << 16), t_o = t_unit + 128;
             const bool in = r < rows;
-            const int qp = in ? tl.pos0 + (tl.row0 + r) / G : -1, all_see = tl.pos0 + (tl.row0 + QP_ROWS * u + 32 * (warp & 3)) / G;
+            auto token = [&](const dc_q4_tile& z) { return (z.row0 + r) / G; };
+            const int my_token = token(tl);
+            const int qp = in ? tl.pos0 + my_token : -1, all_see = tl.pos0 + (tl.row0 + QP_ROWS * u + 32 * (warp & 3)) / G;
+            // ---- the warp's queries, neighbouring lanes along a row: a row times 2^-e, 2^e <= its largest < 2^(e + 1)
+            const uint32_t own = sm + u * L::SET + 32 * (warp & 3) * 128;      // the warp's 32 rows; after the last product they hold its results
+            constexpr int LANES = HD / 8, PER = 32 / LANES, BATCH = 4;          // lanes of a row, rows at a time
+            const int c8 = lane % LANES;
+            auto row_at = [&](int i) { return PER * i + lane / LANES; };       // (of the warp's 32)
+            auto place = [&](int rr, int c) { return own + (c >> 3) * (QP_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4); };
+            // the lane's own row: its token and head; a row's first element in rows of queries or results, from the lane that has it (whole warps)
+            auto element = [&](const dc_q4_tile& z, int j, int rr, int ld) {
+                const int jr = __shfl_sync(0xffffffffu, j, rr), g = z.row0 + QP_ROWS * u + 32 * (warp & 3) + rr - jr * G;
+                return (size_t)(z.tok0 + jr) * ld + (size_t)(kvh * G + g) * HD;
+            };
+            const int n_first = rows - (QP_ROWS * u + 32 * (warp & 3));          // rows that there are, of the warp's 32
+            auto f2 = [](uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); };
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32 / PER; i0 += BATCH) {
+                uint4 v[BATCH];
+                float most[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int rr = row_at(i0 + i);
+                    const __nv_bfloat16* src = p.q + element(tl, my_token, rr, p.ldq) + 8 * c8;
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (rr < n_first) {
+                        if (((uintptr_t)src & 15) == 0) {
+                            v[i] = __ldg(reinterpret_cast<const uint4*>(src));
+                        } else {
+                            const uint16_t* at = reinterpret_cast<const uint16_t*>(src);
+                            v[i] = make_uint4(at[0] | (uint32_t)at[1] << 16, at[2] | (uint32_t)at[3] << 16, at[4] | (uint32_t)at[5] << 16, at[6] | (uint32_t)at[7] << 16);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                    most[i] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) most[i] = fmaxf(most[i], fmaxf(fabsf(f2(w[k]).x), fabsf(f2(w[k]).y)));
+                }
+#pragma unroll
+                for (int k = 1; k < LANES; k <<= 1)
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], k));
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int rr = row_at(i0 + i), e = max(-100, min(100, (int)(__float_as_uint(most[i]) >> 23) - 127));
+                    const float up = __uint_as_float((uint32_t)(127 - e) << 23) * (p.scale < 0.0f ? -1.0f : 1.0f);
+                    auto half = [&](uint32_t x) { return pack_h2(f2(x).x * up, f2(x).y * up); };
+                    sts128(place(rr, c8), half(v[i].x), half(v[i].y), half(v[i].z), half(v[i].w));
+                    if (c8 == 0) s_pow[QP_ROWS * u + 32 * (warp & 3) + rr] = __uint_as_float((uint32_t)(127 + e) << 23);
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(bar(QP_QUERY));
+            __syncwarp();
             const float sl2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f * s_pow[r], 1e-35f);      // (above 0: minus infinity stays so)
-            float m_run = -1e30f, l_run[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float m_run = -1e30f, l_run[2] = {0.0f, 0.0f};
             bool ok = true;
             __syncwarp();
             {
@@ -209,7 +226,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                     const float corr = ex2(m_run - m_new);
                     m_run = m_new;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) l_run[i] *= corr;
+                    for (int i = 0; i < 2; ++i) l_run[i] *= corr;
                     if (t > 0) {
                         ok = wait(bar(QP_O, u), (t - 1) & 1);
                         if (!ok) break;
@@ -234,7 +251,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float a = ex2(fmaf(s(2 * i), sl2, -m_run)), b = ex2(fmaf(s(2 * i + 1), sl2, -m_run));
-                        l_run[i & 3] += a + b;
+                        l_run[i & 1] += a + b;
                         w[i] = pack_h2(a, b);
                     }
                     __syncwarp();
@@ -250,34 +267,65 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
             if (ok) ok = wait(bar(QP_O, u), (n_tiles - 1) & 1);
             if (ok) {
                 tc_fence_after();
-                const float l = (l_run[0] + l_run[1]) + (l_run[2] + l_run[3]);
-                const bool whole = tl.n_splits == 1;
-                const float mul = whole ? 1.0f / l : 1.0f;
-                const int x = tl.row0 + r, j = x / G;
-                __nv_bfloat16* dst = p.out + (size_t)(tl.tok0 + (in ? j : 0)) * p.ldo + (size_t)(kvh * G + (in ? x - j * G : 0)) * HD;
-                float* part = reinterpret_cast<float*>(const_cast<uint8_t*>(p.plan) + 4 * (size_t)hd->ws) +
-                              (((size_t)tl.ws * p.n_kv + (size_t)tl.n_splits * kvh + tl.split) * (2 * QP_ROWS) + r) * (HD + 4);
-                const bool vec = ((uintptr_t)dst & 15) == 0;
-                if (in && !whole) *reinterpret_cast<float2*>(part + HD) = make_float2(m_run, l);
+                const float l = l_run[0] + l_run[1];
+                const dc_q4_tile te = *tp;      // (again: what stays in registers meanwhile spills)
+                const bool whole = te.n_splits == 1;
+                const int n_own = te.count * G - te.row0 - (QP_ROWS * u + 32 * (warp & 3));
+                const float mul = 1.0f / l;
+                // rows by way of shared memory, so that neighbouring lanes store along a row; f32 parts 64 dimensions at a time
+                if (whole) {
 #pragma unroll 1
-                for (int c = 0; c < HD / 16; ++c) {
-                    int o[16];
-                    __syncwarp();      // lanes without a row have skipped the last stores: the load is the whole warp's
-                    tmem_ld16(t_o + 16 * c, o);
-                    tmem_ld_wait(o);
-                    if (in) {
+                    for (int c = 0; c < HD / 16; ++c) {
+                        int o[16];
+                        __syncwarp();
+                        tmem_ld16(t_o + 16 * c, o);
+                        tmem_ld_wait(o);
                         const float f = s_nan[c / 4] <= qp ? NAN : mul;
                         auto v = [&](int i) { return __int_as_float(o[i]) * f; };
-                        if (!whole) {
 #pragma unroll
-                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + 16 * c + i) = make_float4(v(i), v(i + 1), v(i + 2), v(i + 3));
-                        } else if (vec) {
-#pragma unroll
-                            for (int i = 0; i < 16; i += 8)
-                                *reinterpret_cast<uint4*>(dst + 16 * c + i) = make_uint4(pack_bf2(v(i), v(i + 1)), pack_bf2(v(i + 2), v(i + 3)), pack_bf2(v(i + 4), v(i + 5)), pack_bf2(v(i + 6), v(i + 7)));
+                        for (int i = 0; i < 2; ++i)
+                            sts128(place(lane, 2 * c + i), pack_bf2(v(8 * i), v(8 * i + 1)), pack_bf2(v(8 * i + 2), v(8 * i + 3)), pack_bf2(v(8 * i + 4), v(8 * i + 5)), pack_bf2(v(8 * i + 6), v(8 * i + 7)));
+                    }
+                    __syncwarp();
+                    const int own_token = token(te);
+#pragma unroll 8
+                    for (int i = 0; i < 32 / PER; ++i) {
+                        const int rr = row_at(i);
+                        __nv_bfloat16* dst = p.out + element(te, own_token, rr, p.ldo) + 8 * c8;
+                        const uint4 v = lds128(place(rr, c8));
+                        if (rr >= n_own) continue;
+                        if (((uintptr_t)dst & 15) == 0) {
+                            *reinterpret_cast<uint4*>(dst) = v;
                         } else {
+                            uint16_t* at = reinterpret_cast<uint16_t*>(dst);
+                            at[0] = v.x & 0xFFFF, at[1] = v.x >> 16, at[2] = v.y & 0xFFFF, at[3] = v.y >> 16, at[4] = v.z & 0xFFFF, at[5] = v.z >> 16, at[6] = v.w & 0xFFFF, at[7] = v.w >> 16;
+                        }
+                    }
+                } else {
+                    float* part = reinterpret_cast<float*>(const_cast<uint8_t*>(p.plan) + 4 * (size_t)hd->ws) +
+                                  (((size_t)te.ws * p.n_kv + (size_t)te.n_splits * kvh + te.split) * (2 * QP_ROWS) + QP_ROWS * u + 32 * (warp & 3)) * (HD + 4);
+                    if (in) *reinterpret_cast<float2*>(part + (size_t)lane * (HD + 4) + HD) = make_float2(m_run, l);
+                    constexpr int LN = HD == 128 ? 16 : 8;      // lanes of a row: 64 dimensions of four bytes, or 32
+#pragma unroll 1
+                    for (int g = 0; g < HD / (4 * LN); ++g) {
+#pragma unroll 1
+                        for (int c = 0; c < LN / 4; ++c) {
+                            int o[16];
+                            __syncwarp();
+                            tmem_ld16(t_o + 4 * LN * g + 16 * c, o);
+                            tmem_ld_wait(o);
+                            const float f = s_nan[(4 * LN * g + 16 * c) / 64] <= qp ? NAN : 1.0f;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) dst[16 * c + i] = __float2bfloat16_rn(v(i));
+                            for (int i = 0; i < 4; ++i)
+                                sts128(place(lane, 4 * c + i), __float_as_uint(__int_as_float(o[4 * i]) * f), __float_as_uint(__int_as_float(o[4 * i + 1]) * f),
+                                       __float_as_uint(__int_as_float(o[4 * i + 2]) * f), __float_as_uint(__int_as_float(o[4 * i + 3]) * f));
+                        }
+                        __syncwarp();
+#pragma unroll 4
+                        for (int i = 0; i < 32 / PER; ++i) {
+                            const int rr = row_at(i);
+                            const uint4 v = lds128(place(rr, c8));
+                            if (rr < n_own) *reinterpret_cast<uint4*>(part + (size_t)rr * (HD + 4) + 4 * LN * g + 4 * c8) = v;
                         }
                     }
                 }
@@ -407,7 +455,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                 umma_commit(bar(QP_O, u));
             }
         };
-        bool ok = wait(bar(QP_FULL, 0), 0);
+        bool ok = wait(bar(QP_QUERY), 0) && wait(bar(QP_FULL, 0), 0);
         if (ok) {
             tc_fence_after();
             scores(0, 0);
