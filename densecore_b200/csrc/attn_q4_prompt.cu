@@ -7,7 +7,7 @@
 //   warps 0-7    weights: four a set, thread = row = tensor-memory lane
 //   warps 8-15   pages by bulk copies, codes turned into fp16 rows of the operands' 128-byte swizzle (d c + m, rounded once: 2^-11 relative); a warp has the keys
 //                or the values of one page, values turned (rows are dimensions: products with keys along the rows took three times as long to issue)
-//   warp 16      issues the products
+//   warps 16-17  issue a set's products each (one warp for both was the bound: some 50 cycles a product)
 // Queries are bf16 rows times a power of two (exact in fp16), weights fp16 (2^-11): together below a bf16 result's own 2^-8.
 // A value that is not a number (d = m = NaN) enters the tiles as 0, or the products would carry it to rows that do not see it; the CTA keeps the first
 // position of such a value per group of 64 dimensions, and rows that see it end as NaN there.
@@ -73,8 +73,8 @@ struct PromptParams {
     __nv_bfloat16* out;
 };
 
-constexpr int QP_ROWS = 128, QP_KEYS = 64, QP_STAGES = 4, QP_RAW = 3, QP_THREADS = 17 * 32;
-enum QpBar { QP_FULL = 0, QP_FREE = 4, QP_S = 8, QP_P = 12, QP_O = 16, QP_DRAIN = 18, QP_PAGES = 19, QP_READ = 22, QP_QUERY = 25, QP_NBARS = 26 };
+constexpr int QP_ROWS = 128, QP_KEYS = 64, QP_STAGES = 4, QP_RAW = 3, QP_THREADS = 18 * 32;
+enum QpBar { QP_FULL = 0, QP_FREE = 4, QP_S = 8, QP_P = 12, QP_O = 16, QP_DRAIN = 18, QP_PAGES = 20, QP_READ = 23, QP_QUERY = 26, QP_NBARS = 27 };
 template <int HD>
 struct Lay {
     static constexpr uint32_t SET = QP_ROWS * HD * 2, TILE = QP_KEYS * HD * 2;      // a set's queries; keys or values of a tile: halves of 64 columns
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < QP_NBARS; ++i) mbar_init(bar(i), i == QP_QUERY ? sets * QP_ROWS : i < QP_FREE || i >= QP_READ ? 256 : i >= QP_P && i < QP_O ? 4 : 1);
+        for (int i = 0; i < QP_NBARS; ++i) mbar_init(bar(i), i == QP_QUERY ? sets * QP_ROWS : i >= QP_FREE && i < QP_S ? sets : i < QP_FREE || i >= QP_READ ? 256 : i >= QP_P && i < QP_O ? 4 : 1);
         mbar_fence_init();
         s_nan[0] = s_nan[1] = 0x7fffffff;
     }
@@ -431,56 +431,52 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
         }
         if (warp == 8 && lane == 0)
             for (; t < fetched; ++t) mbar_wait(bar(QP_PAGES, t % QP_RAW), (t / QP_RAW) & 1, nullptr);      // (given up: copies in flight)
-    } else {
+    } else if (warp - 16 < sets) {
         // ------------------------------------------------------------------ products
+        const int u = warp - 16;
         const bool one = elect_one();
         constexpr uint32_t id_s = umma_idesc_f16(QP_ROWS, QP_KEYS), id_o = umma_idesc_f16(QP_ROWS, HD);
-        // descriptors of both sets' queries and of every stage's keys and values differ in the address alone: made once, added to
-        const uint64_t dq = umma_desc_sw128(sm, 1024), dk = umma_desc_sw128(sm + L::KV, 1024), dv = umma_desc_sw128(sm + L::KV + L::TILE, 1024);
-        auto scores = [&](int u, int t) {
+        const uint64_t q = umma_desc_sw128(sm + u * L::SET, 1024), dk = umma_desc_sw128(sm + L::KV, 1024), dv = umma_desc_sw128(sm + L::KV + L::TILE, 1024);
+        const uint32_t t_unit = tmem + u * 256;
+        auto scores = [&](int t) {
             if (one) {
-                const uint64_t q = dq + u * (L::SET / 16), k = dk + (t % QP_STAGES) * (2 * L::TILE / 16);
-                const uint32_t d = tmem + u * 256 + 64 * (t & 1);
+                const uint64_t k = dk + (t % QP_STAGES) * (2 * L::TILE / 16);
+                const uint32_t d = t_unit + 64 * (t & 1);
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i) umma_f16(d, q + ((i >> 2) * (QP_ROWS * 128) + 32 * (i & 3)) / 16, k + ((i >> 2) * (QP_KEYS * 128) + 32 * (i & 3)) / 16, id_s, i > 0);
                 umma_commit(bar(QP_S, 2 * u + (t & 1)));
             }
         };
-        auto values = [&](int u, int t) {
+        auto values = [&](int t) {
             if (one) {
                 const uint64_t v = dv + (t % QP_STAGES) * (2 * L::TILE / 16);
-                const uint32_t d = tmem + u * 256 + 128, w = tmem + u * 256 + 64 * (t & 1);
+                const uint32_t w = t_unit + 64 * (t & 1);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) umma_f16_ts(d, w + 8 * i, v + 2 * i, id_o, 1);
+                for (int i = 0; i < 4; ++i) umma_f16_ts(t_unit + 128, w + 8 * i, v + 2 * i, id_o, 1);
                 umma_commit(bar(QP_O, u));
+                umma_commit(bar(QP_FREE, t % QP_STAGES));
             }
         };
         bool ok = wait(bar(QP_QUERY), 0) && wait(bar(QP_FULL, 0), 0);
         if (ok) {
             tc_fence_after();
-            scores(0, 0);
-            if (sets > 1) scores(1, 0);
+            scores(0);
         }
-        // scores of tile t + 1 go where the weights of tile t - 1 were, once the product that reads those is complete
+        // scores of tile t + 1 go where the weights of tile t - 1 were, once the product that reads those is complete; ahead of the wait for tile t's weights
         for (int t = 0; t < n_tiles && ok; ++t) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (u == 1 && sets == 1) break;
-                if (ok && t + 1 < n_tiles) {
-                    if (u == 0) ok = wait(bar(QP_FULL, (t + 1) % QP_STAGES), ((t + 1) / QP_STAGES) & 1);
-                    if (ok && t > 0) ok = wait(bar(QP_O, u), (t - 1) & 1);
-                    tc_fence_after();
-                    if (ok) scores(u, t + 1);
-                }
-                ok = ok && wait(bar(QP_P, 2 * u + (t & 1)), (t >> 1) & 1);
+            if (t + 1 < n_tiles) {
+                ok = wait(bar(QP_FULL, (t + 1) % QP_STAGES), ((t + 1) / QP_STAGES) & 1);
+                if (ok && t > 0) ok = wait(bar(QP_O, u), (t - 1) & 1);
                 tc_fence_after();
-                if (ok) values(u, t);
+                if (ok) scores(t + 1);
             }
-            if (ok && one) umma_commit(bar(QP_FREE, t % QP_STAGES));
+            ok = ok && wait(bar(QP_P, 2 * u + (t & 1)), (t >> 1) & 1);
+            tc_fence_after();
+            if (ok) values(t);
         }
         if (!ok) {      // products in flight still read shared and tensor memory
-            if (one) umma_commit(bar(QP_DRAIN));
-            mbar_wait_warp(bar(QP_DRAIN), 0);
+            if (one) umma_commit(bar(QP_DRAIN, u));
+            mbar_wait_warp(bar(QP_DRAIN, u), 0);
         }
     }
     tc_fence_before();
