@@ -78,88 +78,102 @@ __device__ __forceinline__ void codes_of(uint32_t w, uint32_t (&c)[4]) {
 
 // ---------------------------------------------------------------- new rows into the cache
 struct WriteParams {
-    const uint8_t* plan;
+    const dc_q4_head* head;
+    const dc_q4_token* tokens;
     const void *k, *v;
-    int ldkv, n_kv, max_blocks;
-    const int32_t* tables;
+    int ldkv, n_kv;
     uint8_t* arena;
     float *k_held, *v_held;      // [T][n_kv][HD], may be null
 };
 
-// One warp per (token, key head, key or value).  Bound: latency (a step's rows are some KB).
+// rint(x / d) as the division rounds it, x within 16 d: by the reciprocal, and by the division itself where the product lies near a border
+__device__ __forceinline__ float rounded_quotient(float x, float d, float inv) {
+    const float t = x * inv, q = rintf(t);
+    return fabsf(fabsf(t - q) - 0.5f) < 1e-4f ? rintf(__fdiv_rn(x, d)) : q;
+}
+
+// One warp per (token, key head), its key and value side by side.  Bound: latency (a step's rows are some KB); a prompt's by its rows.
 template <int HD, typename TX>
 __global__ void __launch_bounds__(128) k_q4_write(const WriteParams p) {
     using R = dc_q4_rec<HD>;
-    constexpr int PER = HD / 32;      // neighbouring values of a lane
-    __shared__ uint8_t codes[4][HD];
+    constexpr int PER = HD / 32, LANES = 64 / PER;      // neighbouring values of a lane, lanes of a group
+    __shared__ uint8_t codes[4][2][HD];
     pdl_wait();
     pdl_launch_dependents();      // (not before the wait: what the next kernel reads ahead of its own wait has to be complete)
-    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
-    const int32_t* tok = reinterpret_cast<const int32_t*>(p.plan) + hd->tokens;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = hd->T * p.n_kv * 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = p.head->T * p.n_kv;
     for (int u = blockIdx.x * 4 + warp; u < units; u += gridDim.x * 4) {
-        const int t = u / (2 * p.n_kv), w = u - t * 2 * p.n_kv, head = w >> 1, is_v = w & 1;
-        const int seq = tok[2 * t], pos = tok[2 * t + 1], slot = pos % DC_KV_BLOCK;
-        const TX* src = reinterpret_cast<const TX*>(is_v ? p.v : p.k) + (size_t)t * p.ldkv + head * HD + PER * lane;
-        float x[PER], lo = INFINITY, hi = -INFINITY;
-        bool fine = true;
+        const int t = u / p.n_kv, head = u - t * p.n_kv;
+        const dc_q4_token tok = p.tokens[t];
+        float x[2][PER], lo[2], hi[2];
+        bool fine[2];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            x[i] = to_f32(src[i]);
-            fine = fine && fabsf(x[i]) <= 32768.0f;
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
+        for (int w = 0; w < 2; ++w) {
+            const TX* src = reinterpret_cast<const TX*>(w ? p.v : p.k) + (size_t)t * p.ldkv + head * HD + PER * lane;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) x[w][i] = to_f32(src[i]);
         }
-        constexpr int LANES = 64 / PER;      // of a group
 #pragma unroll
-        for (int s = LANES / 2; s > 0; s >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+        for (int w = 0; w < 2; ++w) {
+            lo[w] = INFINITY, hi[w] = -INFINITY, fine[w] = true;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) fine[w] = fine[w] && fabsf(x[w][i]) <= 32768.0f, lo[w] = fminf(lo[w], x[w][i]), hi[w] = fmaxf(hi[w], x[w][i]);
         }
-        const uint32_t bad = __ballot_sync(0xffffffffu, !fine) >> (lane / LANES * LANES);
-        __half d = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), m = __float2half_rn(lo);
-        const float df = __half2float(d), mf = __half2float(m);
-        const bool nan = (LANES == 32 ? bad : bad & ((1u << (LANES & 31)) - 1u)) != 0;
-        int q[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) q[i] = !nan && df > 0.0f ? (int)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mf), df)), 0.0f), 15.0f) : 0;
-        if (nan) d = m = __ushort_as_half((unsigned short)0x7FFF);
+        for (int s = LANES / 2; s > 0; s >>= 1)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                lo[w] = fminf(lo[w], __shfl_xor_sync(0xffffffffu, lo[w], s));
+                hi[w] = fmaxf(hi[w], __shfl_xor_sync(0xffffffffu, hi[w], s));
+            }
+        uint8_t* rec = p.arena + ((size_t)tok.block * p.n_kv + head) * R::BYTES;
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < PER; ++i) codes[warp][PER * lane + i] = (uint8_t)q[i];
-        __syncwarp();
-        const int block = p.tables[(size_t)seq * p.max_blocks + pos / DC_KV_BLOCK];
-        uint8_t* rec = p.arena + ((size_t)block * p.n_kv + head) * R::BYTES;
-        if (lane % LANES == 0)
-            reinterpret_cast<__half2*>(rec + (is_v ? R::V_SCALES : R::K_SCALES))[slot * R::GROUPS + lane / LANES] = __halves2half2(d, m);
-        const uint8_t* c = codes[warp];
-        if (!is_v) {
-            if (lane < HD / 8) {
-                const int t4 = lane & 3, i = lane >> 2;
-                uint32_t word = 0;
-#pragma unroll
-                for (int n = 0; n < 8; ++n) word |= (uint32_t)c[32 * i + 8 * (n & 3) + 2 * t4 + (n >> 2)] << (4 * n);
-                *reinterpret_cast<uint32_t*>(rec + R::k_word(slot, t4, i)) = word;
-            }
-        } else {
-#pragma unroll
-            for (int b = lane; b < HD / 2; b += 32) {
-                const int d8 = b & 7, i = b >> 3;
-                rec[R::v_byte(slot, d8, i)] = c[16 * i + d8] | (uint8_t)(c[16 * i + 8 + d8] << 4);
-            }
-        }
-        float* held = is_v ? p.v_held : p.k_held;
-        if (held) {
+        for (int w = 0; w < 2; ++w) {
+            const uint32_t bad = __ballot_sync(0xffffffffu, !fine[w]) >> (lane / LANES * LANES);
+            const bool nan = (LANES == 32 ? bad : bad & ((1u << (LANES & 31)) - 1u)) != 0;
+            __half d = __float2half_rn(__fmul_rn(__fsub_rn(hi[w], lo[w]), 1.0f / 15.0f)), m = __float2half_rn(lo[w]);
+            const float df = __half2float(d), mf = __half2float(m), inv = __fdividef(1.0f, df);
+            const bool steps = !nan && df > 0.0f;
+            if (nan) d = m = __ushort_as_half((unsigned short)0x7FFF);
             const float ds = __half2float(d), ms = __half2float(m);
+            float* held = w ? p.v_held : p.k_held;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) held[((size_t)t * p.n_kv + head) * HD + PER * lane + i] = fmaf(ds, (float)q[i], ms);
+            for (int i = 0; i < PER; ++i) {
+                const float q = steps ? fminf(fmaxf(rounded_quotient(__fsub_rn(x[w][i], mf), df, inv), 0.0f), 15.0f) : 0.0f;
+                codes[warp][w][PER * lane + i] = (uint8_t)q;
+                x[w][i] = fmaf(ds, q, ms);
+            }
+            if (held) {
+                float* to = held + ((size_t)t * p.n_kv + head) * HD + PER * lane;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) to[i] = x[w][i];
+            }
+            if (lane % LANES == 0) reinterpret_cast<__half2*>(rec + (w ? R::V_SCALES : R::K_SCALES))[tok.slot * R::GROUPS + lane / LANES] = __halves2half2(d, m);
+        }
+        __syncwarp();
+        if (lane < HD / 8) {
+            const uint8_t* c = codes[warp][0];
+            const int t4 = lane & 3, i = lane >> 2;
+            uint32_t word = 0;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) word |= (uint32_t)c[32 * i + 8 * (n & 3) + 2 * t4 + (n >> 2)] << (4 * n);
+            *reinterpret_cast<uint32_t*>(rec + R::k_word(tok.slot, t4, i)) = word;
+        }
+        const uint8_t* c = codes[warp][1];
+#pragma unroll
+        for (int b = lane; b < HD / 2; b += 32) {
+            const int d8 = b & 7, i = b >> 3;
+            rec[R::v_byte(tok.slot, d8, i)] = c[16 * i + d8] | (uint8_t)(c[16 * i + 8 + d8] << 4);
         }
     }
 }
 
 // ---------------------------------------------------------------- attention, eight rows at a time
 struct RowsParams {
-    const uint8_t* plan;
+    const dc_q4_head* head;
+    const dc_q4_item* items;
+    int* tickets;
+    float* ws;
     const void* q;
     int ldq, ldo, heads, n_kv, max_blocks;
     const int32_t* tables;
@@ -197,12 +211,11 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
     bool waited = !p.early;
     if (waited) pdl_wait();
     pdl_launch_dependents();
-    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
-    const int32_t* words = reinterpret_cast<const int32_t*>(p.plan);
-    const int n_items = hd->n_items;
+    dc_q4_item im = p.items[blockIdx.x];      // (within the plan's room even if a later plan has fewer: it need not wait for their number)
+    const int n_items = p.head->n_items;
     uint32_t n_full = 0;      // pages that this warp has waited for
     for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
-        const dc_q4_item im = reinterpret_cast<const dc_q4_item*>(words + hd->items)[it];
+        if (it != (int)blockIdx.x) im = p.items[it];
         const int r = im.tile * 8 + h, j = r / G, g = r - j * G;
         const bool row = j < im.count;
         const int qpos = im.pos0 + j, first_new = im.pos0 / DC_KV_BLOCK, all_see = im.pos0 + im.tile * 8 / G;      // positions up to all_see: seen by every row
@@ -448,7 +461,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
         __syncthreads();
         // ---- joined: a thread has four neighbouring dimensions of a row at a time
         const bool alone = im.n_splits == 1;
-        float* ws = reinterpret_cast<float*>(const_cast<int32_t*>(words) + hd->ws) + ((size_t)im.ws * p.n_kv + (size_t)im.n_splits * kvh) * PART;
+        float* ws = p.ws + ((size_t)im.ws * p.n_kv + (size_t)im.n_splits * kvh) * PART;
         auto store = [&](int x4, const float4& v, float inv) {
             const int ro = im.tile * 8 + x4 / (HD / 4), jo = ro / G, go = ro - jo * G;
             if (jo >= im.count) return;
@@ -478,7 +491,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             }
         }
         if (!alone) {
-            int* ticket = const_cast<int*>(words) + hd->tickets + im.ticket * p.n_kv + kvh;
+            int* ticket = p.tickets + im.ticket * p.n_kv + kvh;
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -488,16 +501,27 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             }
             __syncthreads();
             if (s_last) {
-                // the splits' factors in place of the parts: [split][8 rows], DC_Q4_SPLITS at most; then rows' sums
+                // the splits' factors in place of the parts: [split][8 rows], DC_Q4_SPLITS at most; then rows' sums.  The first splits' sums are on their way meanwhile
                 static_assert(DC_Q4_SPLITS * 8 + 8 <= RW * 8 * 64, "factors take the parts' place");
+                constexpr int AHEAD = 2, X4 = 8 * HD / 4 / (RW * 32);
+                float4 first[X4][AHEAD];
+#pragma unroll
+                for (int k = 0; k < X4; ++k)
+#pragma unroll
+                    for (int s = 0; s < AHEAD; ++s)
+                        if (s < im.n_splits) first[k][s] = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + threadIdx.x + k * RW * 32);
                 float *f = part, *inv = part + DC_Q4_SPLITS * 8;
                 if (threadIdx.x < 32) {
                     const int rr = lane & 7;      // four lanes a row
                     float M = -1e30f, L = 0.0f;
-                    for (int s = lane >> 3; s < im.n_splits; s += 4) M = fmaxf(M, f[8 * s + rr] = __ldcg(ws + (size_t)s * PART + 8 * HD + rr));
+                    const float m0 = lane >> 3 < im.n_splits ? __ldcg(ws + (size_t)(lane >> 3) * PART + 8 * HD + rr) : -1e30f;
+                    const float l0 = lane >> 3 < im.n_splits ? __ldcg(ws + (size_t)(lane >> 3) * PART + 8 * HD + 8 + rr) : 0.0f;
+                    M = m0;
+                    for (int s = (lane >> 3) + 4; s < im.n_splits; s += 4) M = fmaxf(M, f[8 * s + rr] = __ldcg(ws + (size_t)s * PART + 8 * HD + rr));
                     M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
                     M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
-                    for (int s = lane >> 3; s < im.n_splits; s += 4) {
+                    if (lane >> 3 < im.n_splits) L = l0 * (f[lane] = ex2(m0 - M));
+                    for (int s = (lane >> 3) + 4; s < im.n_splits; s += 4) {
                         const float x = ex2(f[8 * s + rr] - M);
                         f[8 * s + rr] = x;
                         L = fmaf(__ldcg(ws + (size_t)s * PART + 8 * HD + 8 + rr), x, L);
@@ -507,11 +531,19 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
                     if (lane < 8) inv[rr] = __fdividef(1.0f, L);
                 }
                 __syncthreads();
-                for (int x4 = threadIdx.x; x4 < 8 * HD / 4; x4 += RW * 32) {
-                    const int rr = x4 / (HD / 4);
+#pragma unroll
+                for (int k = 0; k < X4; ++k) {
+                    const int x4 = threadIdx.x + k * RW * 32, rr = x4 / (HD / 4);
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int s = 0; s < im.n_splits; ++s) {
+#pragma unroll
+                    for (int s = 0; s < AHEAD; ++s)
+                        if (s < im.n_splits) {
+                            const float4 x = first[k][s];
+                            const float w = f[8 * s + rr];
+                            v.x = fmaf(x.x, w, v.x), v.y = fmaf(x.y, w, v.y), v.z = fmaf(x.z, w, v.z), v.w = fmaf(x.w, w, v.w);
+                        }
+#pragma unroll 4
+                    for (int s = AHEAD; s < im.n_splits; ++s) {
                         const float4 x = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + x4);
                         const float w = f[8 * s + rr];
                         v.x = fmaf(x.x, w, v.x), v.y = fmaf(x.y, w, v.y), v.z = fmaf(x.z, w, v.z), v.w = fmaf(x.w, w, v.w);
@@ -529,7 +561,7 @@ template <int HD, typename TX>
 int launch_rows(dc_ctx* ctx, const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
     DC_TRY(dc_kernel_setup(ctx, (const void*)k_q4_rows<HD, TX>, (int)rows_smem<HD>(), "k_q4_rows"));
-    RowsParams p = {z.plan, c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.after_write ? 1 : 0, ctx->d_err};
+    RowsParams p = {(const dc_q4_head*)z.plan, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.after_write ? 1 : 0, ctx->d_err};
     return dc_launch(ctx, "k_q4_rows", k_q4_rows<HD, TX>, dim3(z.n_items, z.kv), dim3(RW * 32), rows_smem<HD>(), p);
 }
 
@@ -588,56 +620,65 @@ int blocks_needed(const dc_kv_cache* kv, const std::vector<dc_q4_entry>& es) {
 
 int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, int T) {
     dc_q4& z = *kv->q4;
-    std::vector<int32_t> tokens(2 * (size_t)T);
+    std::vector<dc_q4_token> tokens(T);
     std::vector<dc_q4_item> items;
     std::vector<dc_q4_tile> tiles;
-    for (const dc_q4_entry& e : es)
-        for (int i = 0; i < e.count; ++i) tokens[2 * (size_t)(e.tok0 + i)] = e.seq, tokens[2 * (size_t)(e.tok0 + i) + 1] = e.pos0 + i;
+    std::vector<int32_t> joins;      // tiles whose keys are split: their first part
     const int G = z.heads / z.kv;
     std::vector<dc_q4_entry> few, many;
-    for (const dc_q4_entry& e : es) (z.type == DC_TYPE_BF16 && (long long)e.count * G >= DC_Q4_PROMPT_ROWS ? many : few).push_back(e);
+    for (const dc_q4_entry& e : es) {
+        for (int i = 0; i < e.count; ++i) tokens[e.tok0 + i] = {kv->seqs[e.seq].blocks[(e.pos0 + i) / DC_KV_BLOCK], (e.pos0 + i) % DC_KV_BLOCK};
+        (z.type == DC_TYPE_BF16 && (long long)e.count * G >= DC_Q4_PROMPT_ROWS ? many : few).push_back(e);
+    }
     int n_tickets, n_ws, n_parts;
     dc_q4_items(few, G, z.kv, ctx->num_sms, &items, &n_tickets, &n_ws);
     dc_q4_tiles(many, G, z.kv, ctx->num_sms, &tiles, &n_parts);
-    // ---- one allocation: header, arrays, tickets (zero, and left so by every call), partial results
-    auto up = [](size_t n) { return (n + 63) / 64 * 64; };
-    dc_q4_head hd = {};
-    hd.T = T, hd.n_items = (int)items.size(), hd.n_tiles = (int)tiles.size();
-    size_t at = up(sizeof(hd));
-    hd.tokens = (int32_t)(at / 4), at += up(tokens.size() * 4);
-    hd.items = (int32_t)(at / 4), at += up(items.size() * sizeof(dc_q4_item));
-    hd.tiles = (int32_t)(at / 4), at += up(tiles.size() * sizeof(dc_q4_tile));
-    const size_t copied = at;
-    hd.tickets = (int32_t)(at / 4), at += up((size_t)n_tickets * z.kv * 4);
-    // (one kernel's parts after the other's: the rows kernel has joined its own when the next one starts)
-    hd.ws = (int32_t)(at / 4), at += up(std::max((size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4, (size_t)n_parts * z.kv * 256 * (z.dim + 4) * 4));
-    if (at > ((size_t)1 << 33) - 64) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: the step's plan takes %zu bytes", at);
-    if (at > z.plan_bytes) {
+    for (size_t i = 0; i < tiles.size(); ++i)
+        if (tiles[i].n_splits > 1 && tiles[i].split == 0) joins.push_back((int32_t)i);
+    // ---- header, arrays, tickets (zero, and left so by every call), partial results (one kernel's after the other's: the rows kernel has joined its own when the next starts)
+    const size_t need[6] = {tokens.size() * sizeof(dc_q4_token), items.size() * sizeof(dc_q4_item), tiles.size() * sizeof(dc_q4_tile), joins.size() * 4, (size_t)n_tickets * z.kv * 4,
+                            std::max((size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4, (size_t)n_parts * z.kv * 256 * (z.dim + 4) * 4)};
+    bool fits = z.plan != nullptr;
+    for (int i = 0; i < 6; ++i) fits = fits && need[i] <= z.cap[i];
+    if (!fits) {
+        size_t cap[6], at[6], bytes = 256;
+        for (int i = 0; i < 6; ++i) {
+            cap[i] = std::max(z.cap[i], (need[i] + need[i] / 2 + 4096) / 256 * 256);
+            at[i] = bytes;
+            bytes += cap[i];
+        }
         uint8_t* fresh = nullptr;
-        const size_t want = at + at / 2 + (1 << 16);
-        DC_TRY(dc_check_cuda(ctx, cudaMalloc(&fresh, want), "kv_batch: plan"));
+        DC_TRY(dc_check_cuda(ctx, cudaMalloc(&fresh, bytes), "kv_batch: plan"));
         if (z.plan) {      // a captured call that still names it finds a step without tokens
             z.retired.push_back(z.plan);
-            DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.plan, 0, sizeof(hd), ctx->stream), "kv_batch: old plan"));
+            DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.plan, 0, sizeof(dc_q4_head), ctx->stream), "kv_batch: old plan"));
         }
-        z.plan = fresh, z.plan_bytes = want;
+        DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(fresh, 0, at[DC_Q4_WS], ctx->stream), "kv_batch: plan"));
+        z.plan = fresh, z.plan_bytes = bytes;
+        std::copy(cap, cap + 6, z.cap), std::copy(at, at + 6, z.at);
     }
     if (!z.uploaded) DC_TRY(dc_check_cuda(ctx, cudaEventCreateWithFlags(&z.uploaded, cudaEventDisableTiming), "kv_batch: event"));
     else DC_TRY(dc_check_cuda(ctx, cudaEventSynchronize(z.uploaded), "kv_batch: staging"));
-    if (copied > z.stage_bytes) {
+    const size_t staged = 256 + need[0] + need[1] + need[2] + need[3];
+    if (staged > z.stage_bytes) {
         if (z.stage) cudaFreeHost(z.stage);
         z.stage = nullptr, z.stage_bytes = 0;
-        DC_TRY(dc_check_cuda(ctx, cudaMallocHost(&z.stage, copied * 2), "kv_batch: staging"));
-        z.stage_bytes = copied * 2;
+        DC_TRY(dc_check_cuda(ctx, cudaMallocHost(&z.stage, staged * 2), "kv_batch: staging"));
+        z.stage_bytes = staged * 2;
     }
+    const dc_q4_head hd = {T, (int)items.size(), (int)tiles.size(), (int)joins.size()};
+    const void* from[4] = {tokens.data(), items.data(), tiles.data(), joins.data()};
     memcpy(z.stage, &hd, sizeof(hd));
-    memcpy(z.stage + 4 * (size_t)hd.tokens, tokens.data(), tokens.size() * 4);
-    memcpy(z.stage + 4 * (size_t)hd.items, items.data(), items.size() * sizeof(dc_q4_item));
-    memcpy(z.stage + 4 * (size_t)hd.tiles, tiles.data(), tiles.size() * sizeof(dc_q4_tile));
-    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.plan, z.stage, copied, cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
+    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.plan, z.stage, sizeof(hd), cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
+    size_t off = 256;
+    for (int i = 0; i < 4; ++i) {
+        if (!need[i]) continue;
+        memcpy(z.stage + off, from[i], need[i]);
+        DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.plan + z.at[i], z.stage + off, need[i], cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
+        off += need[i];
+    }
     DC_TRY(dc_check_cuda(ctx, cudaEventRecord(z.uploaded, ctx->stream), "kv_batch: plan"));
-    if (n_tickets) DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.plan + 4 * (size_t)hd.tickets, 0, (size_t)n_tickets * z.kv * 4, ctx->stream), "kv_batch: tickets"));
-    z.T = T, z.n_items = hd.n_items, z.n_tiles = hd.n_tiles, z.split_tiles = n_parts > 0;
+    z.T = T, z.n_items = hd.n_items, z.n_tiles = hd.n_tiles, z.n_joins = hd.n_joins;
     return DC_B200_OK;
 }
 
@@ -654,8 +695,8 @@ int check_call(dc_ctx* ctx, const dc_kv_cache* kv, int layer, const char* name) 
 
 int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held) {
     const dc_q4& z = *kv->q4;
-    const WriteParams p = {z.plan, k, v, ldkv, z.kv, kv->max_blocks_per_seq, kv->d_tables, kv->planes[layer].arena, k_held, v_held};
-    const int units = (int)std::min<long long>((long long)z.T * z.kv * 2, 1 << 30);
+    const WriteParams p = {(const dc_q4_head*)z.plan, (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), k, v, ldkv, z.kv, kv->planes[layer].arena, k_held, v_held};
+    const int units = (int)std::min<long long>((long long)z.T * z.kv, 1 << 30);
     if (z.dim == 128) return z.type == DC_TYPE_F32 ? launch_write<128, float>(ctx, p, units) : launch_write<128, __nv_bfloat16>(ctx, p, units);
     return z.type == DC_TYPE_F32 ? launch_write<64, float>(ctx, p, units) : launch_write<64, __nv_bfloat16>(ctx, p, units);
 }

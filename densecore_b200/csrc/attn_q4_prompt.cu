@@ -64,7 +64,10 @@ __device__ __forceinline__ void lds_turned(uint32_t at, int turn, uint32_t (&w)[
 }
 
 struct PromptParams {
-    const uint8_t* plan;
+    const dc_q4_head* head;
+    const dc_q4_tile* tiles;
+    const int32_t* joins;
+    float* ws;
     const __nv_bfloat16* q;
     int ldq, ldo, heads, n_kv, max_blocks;
     const int32_t* tables;
@@ -93,10 +96,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
     __shared__ float s_pow[2 * QP_ROWS];      // 2^e of a row
     pdl_wait();
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.x, G = p.heads / p.n_kv;
-    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
-    if ((int)blockIdx.y >= hd->n_tiles) return;      // (a replay on a smaller step)
-    const dc_q4_tile* tp = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles) + blockIdx.y;
+    const dc_q4_tile* tp = p.tiles + blockIdx.y;
     const dc_q4_tile tl = *tp;
+    if ((int)blockIdx.y >= p.head->n_tiles) return;      // (a replay on a smaller step)
     const int rows = min(2 * QP_ROWS, tl.count * G - tl.row0), sets = rows > QP_ROWS ? 2 : 1;
     const int last = tl.pos0 + (tl.row0 + rows - 1) / G, first_tile = tl.tile0, n_tiles = tl.tile1 - tl.tile0;
     const uint32_t sm = (smem_u32(smem) + 1023u) & ~1023u;
@@ -302,8 +304,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                         }
                     }
                 } else {
-                    float* part = reinterpret_cast<float*>(const_cast<uint8_t*>(p.plan) + 4 * (size_t)hd->ws) +
-                                  (((size_t)te.ws * p.n_kv + (size_t)te.n_splits * kvh + te.split) * (2 * QP_ROWS) + QP_ROWS * u + 32 * (warp & 3)) * (HD + 4);
+                    float* part = p.ws + (((size_t)te.ws * p.n_kv + (size_t)te.n_splits * kvh + te.split) * (2 * QP_ROWS) + QP_ROWS * u + 32 * (warp & 3)) * (HD + 4);
                     if (in) *reinterpret_cast<float2*>(part + (size_t)lane * (HD + 4) + HD) = make_float2(m_run, l);
                     constexpr int LN = HD == 128 ? 16 : 8;      // lanes of a row: 64 dimensions of four bytes, or 32
 #pragma unroll 1
@@ -489,13 +490,12 @@ template <int HD>
 __global__ void __launch_bounds__(256) k_q4_join(const PromptParams p) {
     pdl_wait();
     pdl_launch_dependents();
-    const dc_q4_head* hd = reinterpret_cast<const dc_q4_head*>(p.plan);
     const int lane = threadIdx.x & 31, G = p.heads / p.n_kv, kvh = blockIdx.y, r = blockIdx.z * 8 + (threadIdx.x >> 5);
-    if ((int)blockIdx.x >= hd->n_tiles) return;
-    const dc_q4_tile tl = reinterpret_cast<const dc_q4_tile*>(reinterpret_cast<const int32_t*>(p.plan) + hd->tiles)[blockIdx.x];
-    if (tl.n_splits == 1 || tl.split != 0 || r >= tl.count * G - tl.row0) return;
+    if ((int)blockIdx.x >= p.head->n_joins) return;
+    const dc_q4_tile tl = p.tiles[p.joins[blockIdx.x]];
+    if (r >= tl.count * G - tl.row0) return;
     constexpr size_t ROW = HD + 4, PART = 2 * QP_ROWS * ROW;
-    const float* from = reinterpret_cast<const float*>(p.plan + 4 * (size_t)hd->ws) + ((size_t)tl.ws * p.n_kv + (size_t)tl.n_splits * kvh) * PART + r * ROW;
+    const float* from = p.ws + ((size_t)tl.ws * p.n_kv + (size_t)tl.n_splits * kvh) * PART + r * ROW;
     constexpr int PER = HD / 32;
     float M = -1e30f, l = 0.0f, v[PER] = {};
     for (int s = 0; s < tl.n_splits; ++s) M = fmaxf(M, __ldcg(from + s * PART + HD));
@@ -522,10 +522,10 @@ template <int HD>
 int launch(dc_ctx* ctx, const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
     DC_TRY(dc_kernel_setup_unspilled(ctx, (const void*)k_q4_prompt<HD>, (int)Lay<HD>::SMEM, "k_q4_prompt"));
-    PromptParams p = {z.plan, (const __nv_bfloat16*)c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, (__nv_bfloat16*)c.out};
+    PromptParams p = {(const dc_q4_head*)z.plan, (const dc_q4_tile*)(z.plan + z.at[DC_Q4_TILES]), (const int32_t*)(z.plan + z.at[DC_Q4_JOINS]), (float*)(z.plan + z.at[DC_Q4_WS]), (const __nv_bfloat16*)c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, (__nv_bfloat16*)c.out};
     DC_TRY(dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(z.kv, z.n_tiles), dim3(QP_THREADS), Lay<HD>::SMEM, p, ctx->d_err));
-    if (!z.split_tiles) return DC_B200_OK;
-    return dc_launch(ctx, "k_q4_join", k_q4_join<HD>, dim3(z.n_tiles, z.kv, 2 * QP_ROWS / 8), dim3(256), 0, p);
+    if (!z.n_joins) return DC_B200_OK;
+    return dc_launch(ctx, "k_q4_join", k_q4_join<HD>, dim3(z.n_joins, z.kv, 2 * QP_ROWS / 8), dim3(256), 0, p);
 }
 
 }  // namespace

@@ -28,11 +28,13 @@ struct dc_q4_rec {
     }
 };
 
-// The plan of a step in device memory, one allocation: this header, then the arrays that it names (offsets in words).
-// Kernels read the header's counts and loop, so that a captured call takes later plans too.
+// The plan of a step in device memory, one allocation: this header, then arrays at places that stay where they are as long as the allocation does.  Kernels
+// get the places and read the counts, so that a captured call takes later plans too.
 struct dc_q4_head {
-    int32_t T, n_items, n_tiles, tokens, items, tiles, tickets, ws;
-    int32_t pad[8];
+    int32_t T, n_items, n_tiles, n_joins;
+};
+struct dc_q4_token {
+    int32_t block, slot;
 };
 // One CTA's work in k_q4_rows: pages page0 .. page1 - 1 for one tile of eight rows (row r: new token r / G of the entry, query head r % G of the key head).
 struct dc_q4_item {
@@ -96,15 +98,17 @@ struct dc_q4 {
     // the newest plan: host copies of what launches need, and the block manager's state that it was made for
     bool planned = false;
     uint64_t edits = 0;
-    int T = 0, n_items = 0, n_tiles = 0;
-    bool split_tiles = false;
+    int T = 0, n_items = 0, n_tiles = 0, n_joins = 0;
     uint8_t* plan = nullptr;
     size_t plan_bytes = 0;
+    size_t cap[6] = {}, at[6] = {};     // room for the arrays and where they begin: tokens, items, tiles, joins, tickets, partial results
     std::vector<uint8_t*> retired;      // outgrown plans, emptied; captured calls may still read them
     uint8_t* stage = nullptr;           // pinned copy of the plan being uploaded
     size_t stage_bytes = 0;
     cudaEvent_t uploaded = nullptr;
 };
+
+enum { DC_Q4_TOKENS = 0, DC_Q4_ITEMS, DC_Q4_TILES, DC_Q4_JOINS, DC_Q4_TICKETS, DC_Q4_WS };
 
 struct dc_q4_call {
     const dc_kv_cache* kv;

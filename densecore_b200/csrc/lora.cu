@@ -1,7 +1,9 @@
 // Low-rank adapters of many requests beside a shared product: y[t] = base[t] + s_a (x[t] A_a^T) B_a^T with a = ids[t], rows of other ids (none, unknown, empty)
-// y[t] = base[t].  Two kernels: h = s x A^T (few rows: a warp per rank of a row; many: tiles of 16 rows), then y = base + h B^T in tiles of rows.
+// y[t] = base[t].  Two kernels: h = s x A^T, then y = base + h B^T.
+// Few rows: a warp per rank of a row, then a thread per column of a row; what counts is the number of loads that wait for one another (id, rank, matrix), and
+// every matrix row is in flight at once.  Many rows: tiles of rows on the tensor cores.
 //
-// Rows x and h are f32 and enter the tensor cores as two terms of 11 bits (tf32, 22 bits together; products of m16n8k8 with f32 sums), matrices are bf16 or
+// Tiles: rows x and h are f32 and enter the tensor cores as two terms of 11 bits (tf32, 22 bits together; products of m16n8k8 with f32 sums), matrices are bf16 or
 // fp16, which tf32 holds exactly.  A tile whose rows have several adapters takes one after the other: each
 // adapter's matrices are read once per tile, whatever the order of rows.
 #include <math.h>
@@ -28,7 +30,7 @@ struct dc_lora {
     uint16_t *a = nullptr, *b = nullptr;      // [slot][Rp][Kp] and [slot][Np][Rp], zero where there is nothing
     int32_t* rank = nullptr;                  // [slot], 0: empty
     float* scale = nullptr;
-    float* h = nullptr;                       // workspace [rows][Rp]
+    float* h = nullptr;                       // workspace [parts][rows][Rp]
     int64_t h_rows = 0;
     std::vector<float*> retired;              // outgrown workspaces, which captured calls may still name
 };
@@ -94,7 +96,7 @@ __device__ __forceinline__ float4 load_x4(const float* row, int64_t k, int64_t K
     return make_float4(row[k], k + 1 < K ? row[k + 1] : 0.f, k + 2 < K ? row[k + 2] : 0.f, k + 3 < K ? row[k + 3] : 0.f);
 }
 
-// Few rows: a warp per rank of a row.  Bound: latency of the matrix' rows.
+// Few rows: a warp per rank of a row.
 template <bool BF>
 __global__ void __launch_bounds__(256) k_lora_down(const LoraParams p, int vec) {
     const int row = blockIdx.x, r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -104,19 +106,51 @@ __global__ void __launch_bounds__(256) k_lora_down(const LoraParams p, int vec) 
     if (a < 0 || r >= (p.rank[a] + 15) / 16 * 16) return;      // (the padding's rows of the matrix are zero, so are its sums)
     const uint16_t* w = p.a + ((size_t)a * p.Rp + r) * p.Kp;
     const float* x = p.x + (size_t)row * p.ldx;
+    const float scale = p.scale[a];
     float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll 4
-    for (int64_t k = 4 * lane; k < p.Kp; k += 128) {
-        const uint2 c = __ldg(reinterpret_cast<const uint2*>(w + k));
-        const float4 v = load_x4(x, k, p.K, vec, true);
-        const float2 c0 = two<BF>(c.x), c1 = two<BF>(c.y);
-        s0 = fmaf(v.x, c0.x, s0), s1 = fmaf(v.y, c0.y, s1);
-        s0 = fmaf(v.z, c1.x, s0), s1 = fmaf(v.w, c1.y, s1);
+#pragma unroll 8
+    for (int64_t k = 8 * lane; k < p.Kp; k += 256) {
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(w + k));
+        const float4 u = load_x4(x, k, p.K, vec, true), v = load_x4(x, k + 4, p.K, vec, true);
+        const float2 c0 = two<BF>(c.x), c1 = two<BF>(c.y), c2 = two<BF>(c.z), c3 = two<BF>(c.w);
+        s0 = fmaf(u.x, c0.x, s0), s1 = fmaf(u.y, c0.y, s1), s0 = fmaf(u.z, c1.x, s0), s1 = fmaf(u.w, c1.y, s1);
+        s0 = fmaf(v.x, c2.x, s0), s1 = fmaf(v.y, c2.y, s1), s0 = fmaf(v.z, c3.x, s0), s1 = fmaf(v.w, c3.y, s1);
     }
     s0 += s1;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, s);
-    if (lane == 0) p.h[(size_t)row * p.Rp + r] = s0 * p.scale[a];
+    if (lane == 0) p.h[(size_t)row * p.Rp + r] = s0 * scale;
+}
+
+// Few rows: a thread per column of a row, sixteen ranks (two loads of its row of the matrix) at a time.
+template <bool BF>
+__global__ void __launch_bounds__(128) k_lora_up_rows(const LoraParams p) {
+    const int row = blockIdx.y;
+    const int64_t n = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (n >= p.N) return;
+    const int a = slot_of(p, row);
+    float sum = p.base[(size_t)row * p.ldb + n], add = 0.0f;
+    if (a >= 0) {
+        const int ranks = p.rank[a];
+        const uint16_t* w = p.b + ((size_t)a * p.Np + n) * p.Rp;
+        const float* h = p.h + (size_t)row * p.Rp;
+#pragma unroll 2
+        for (int r = 0; r < ranks; r += 16) {
+            const uint4 c[2] = {__ldg(reinterpret_cast<const uint4*>(w + r)), __ldg(reinterpret_cast<const uint4*>(w + r + 8))};
+            float4 u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = __ldcg(reinterpret_cast<const float4*>(h + r) + i);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 c0 = two<BF>(c[i].x), c1 = two<BF>(c[i].y), c2 = two<BF>(c[i].z), c3 = two<BF>(c[i].w);
+                add = fmaf(u[2 * i].x, c0.x, add), add = fmaf(u[2 * i].y, c0.y, add), add = fmaf(u[2 * i].z, c1.x, add), add = fmaf(u[2 * i].w, c1.y, add);
+                add = fmaf(u[2 * i + 1].x, c2.x, add), add = fmaf(u[2 * i + 1].y, c2.y, add), add = fmaf(u[2 * i + 1].z, c3.x, add), add = fmaf(u[2 * i + 1].w, c3.y, add);
+            }
+        }
+    }
+    p.y[(size_t)row * p.ldy + n] = sum + add;
 }
 
 // Adapters of a tile's rows, one after the other: `f(slot, mask)` with the rows (bits) that have it.
@@ -143,7 +177,7 @@ __device__ __forceinline__ void keep_rows(float (&acc)[N][4], const float (&sum)
 
 constexpr int DT_R = 64;      // ranks of a CTA of k_lora_down_tile
 
-// Many rows: a CTA per (16 rows, 64 ranks), its warps share out k in steps of 16 and add up in the end.
+// Many rows: a CTA per (16 rows, 64 ranks, part of k), its warps share out the part in steps of 16 and add up in the end; the parts are added by the next kernel.
 template <bool BF>
 __global__ void __launch_bounds__(256) k_lora_down_tile(const LoraParams p, int vec) {
     __shared__ float part[8][16][DT_R + 1];
@@ -163,8 +197,9 @@ __global__ void __launch_bounds__(256) k_lora_down_tile(const LoraParams p, int 
         const bool u = mask >> h & 1, v = mask >> (h + 8) & 1;
         const float *xu = p.x + (size_t)(row0 + (u ? h : 0)) * p.ldx, *xv = p.x + (size_t)(row0 + (v ? h + 8 : 0)) * p.ldx;
         const uint16_t* w = p.a + ((size_t)a * p.Rp + r0 + h) * p.Kp + 4 * t;
+        const int64_t per = (p.Kp / 16 + gridDim.z - 1) / gridDim.z * 16, k0 = blockIdx.z * per, k1 = min(p.Kp, k0 + per);
 #pragma unroll 2
-        for (int64_t k = 16 * warp; k < p.Kp; k += 128) {
+        for (int64_t k = k0 + 16 * warp; k < k1; k += 128) {
             const Terms x(load_x4(xu, k + 4 * t, p.K, vec, u), load_x4(xv, k + 4 * t, p.K, vec, v));
 #pragma unroll
             for (int i = 0; i < DT_R / 8; ++i)
@@ -187,37 +222,57 @@ __global__ void __launch_bounds__(256) k_lora_down_tile(const LoraParams p, int 
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) s += part[w][row][r];
-        p.h[(size_t)(row0 + row) * p.Rp + r0 + r] = s * p.scale[a];
+        p.h[((size_t)blockIdx.z * p.M + row0 + row) * p.Rp + r0 + r] = s * p.scale[a];
     }
 }
 
-// y = base + h B^T: a CTA per (16 MT rows, 64 NP columns), a warp has 8 NP columns.  Bound: base and y for many rows, the matrices' latency for few.
-template <bool BF, int MT, int NP>
-__global__ void __launch_bounds__(256) k_lora_up(const LoraParams p, int vec) {
+// Many rows: y = base + h B^T, a CTA per (32 rows, 128 columns), a warp has 16 columns.  h comes in `parts` sums.  Bound: base and y.
+template <bool BF>
+__global__ void __launch_bounds__(256) k_lora_up(const LoraParams p, int vec, int parts) {
+    constexpr int MT = 2, NP = 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.y * 16 * MT;
     const int64_t n0 = ((int64_t)blockIdx.x * 8 + warp) * 8 * NP;
     pdl_wait();
     pdl_launch_dependents();
     if (n0 >= p.N) return;
-    const int mine = slot_of(p, row0 + (lane & (16 * MT - 1)));
+    // base first: it is on its way during the products
+    float2 f[MT][2][NP];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int row = row0 + 16 * m + h + 8 * q;
+            const float* from = p.base + (size_t)(row < p.M ? row : 0) * p.ldb;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int64_t n = n0 + 8 * i + 2 * t;
+                if (vec && n + 1 < p.N) f[m][q][i] = *reinterpret_cast<const float2*>(from + n);
+                else f[m][q][i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
+            }
+        }
+    const int mine = slot_of(p, row0 + lane);
     float acc[MT][NP][4] = {};
-    each_adapter(mine, MT == 1 ? 0xFFFFu : 0xFFFFFFFFu, [&](int a, uint32_t mask) {
+    each_adapter(mine, 0xFFFFFFFFu, [&](int a, uint32_t mask) {
         const int ranks = p.rank[a];
         const uint16_t* w = p.b + ((size_t)a * p.Np + n0 + h) * p.Rp + 4 * t;
         const float* hh = p.h + (size_t)row0 * p.Rp + 4 * t;
         float sum[MT][NP][4] = {};
-#pragma unroll 1
+#pragma unroll 2
         for (int r = 0; r < ranks; r += 16) {
             uint2 c[NP];
 #pragma unroll
             for (int i = 0; i < NP; ++i) c[i] = n0 + 8 * i < p.Np ? __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Rp + r)) : make_uint2(0, 0);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                if (!(mask >> (16 * m) & 0xFFFFu)) continue;
-                float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-                if (mask >> (16 * m + h) & 1) u = __ldcg(reinterpret_cast<const float4*>(hh + (size_t)(16 * m + h) * p.Rp + r));
-                if (mask >> (16 * m + h + 8) & 1) v = __ldcg(reinterpret_cast<const float4*>(hh + (size_t)(16 * m + h + 8) * p.Rp + r));
-                const Terms x(u, v);
+                float4 u[2] = {};
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if (mask >> (16 * m + h + 8 * q) & 1)
+                        for (int z = 0; z < parts; ++z) {
+                            const float4 v = __ldcg(reinterpret_cast<const float4*>(hh + ((size_t)z * p.M + 16 * m + h + 8 * q) * p.Rp + r));
+                            u[q].x += v.x, u[q].y += v.y, u[q].z += v.z, u[q].w += v.w;
+                        }
+                const Terms x(u[0], u[1]);
 #pragma unroll
                 for (int i = 0; i < NP; ++i) x.times(sum[m][i], two<BF>(c[i].x), two<BF>(c[i].y));
             }
@@ -231,24 +286,17 @@ __global__ void __launch_bounds__(256) k_lora_up(const LoraParams p, int vec) {
         for (int q = 0; q < 2; ++q) {
             const int row = row0 + 16 * m + h + 8 * q;
             if (row >= p.M) continue;
-            const float* from = p.base + (size_t)row * p.ldb;
             float* to = p.y + (size_t)row * p.ldy;
-            float2 f[NP];
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int64_t n = n0 + 8 * i + 2 * t;
-                if (vec && n + 1 < p.N) f[i] = *reinterpret_cast<const float2*>(from + n);
-                else f[i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
-            }
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int64_t n = n0 + 8 * i + 2 * t;
-                f[i].x += acc[m][i][2 * q], f[i].y += acc[m][i][2 * q + 1];
+                float2 v = f[m][q][i];
+                v.x += acc[m][i][2 * q], v.y += acc[m][i][2 * q + 1];
                 if (vec && n + 1 < p.N) {
-                    *reinterpret_cast<float2*>(to + n) = f[i];
+                    *reinterpret_cast<float2*>(to + n) = v;
                 } else {
-                    if (n < p.N) to[n] = f[i].x;
-                    if (n + 1 < p.N) to[n + 1] = f[i].y;
+                    if (n < p.N) to[n] = v.x;
+                    if (n + 1 < p.N) to[n + 1] = v.y;
                 }
             }
         }
@@ -271,21 +319,26 @@ __global__ void __launch_bounds__(256) k_lora_set(const uint16_t* __restrict__ a
     if (blockIdx.x == 0 && threadIdx.x == 0) *rank_at = rank, *scale_at = scale;
 }
 
-// Rows from which x A^T runs in tiles of sixteen: below, a warp a rank has more CTAs; above, tiles read the matrix once for sixteen rows.
-constexpr int LORA_TILE_ROWS = 129;
-// Rows from which y takes 32 rows and 256 columns a CTA instead of 16 and 64.
-constexpr int LORA_WIDE_ROWS = 129;
+// Rows from which tiles are taken: they read a matrix once for 16 or 32 rows; below, one warp a rank and one thread a column have shorter chains of loads.
+constexpr int LORA_TILE_ROWS = 97;
+constexpr int LORA_PARTS = 4;      // of k, at most
+
+int parts_of(const dc_ctx* ctx, int M, int64_t Kp) {      // until the CTAs fill the SMs three times, a warp keeping two steps
+    int n = 1;
+    while (n < LORA_PARTS && (M + 15) / 16 * n < 3 * ctx->num_sms && Kp / (16 * 8 * 2 * n) >= 2) n *= 2;
+    return n;
+}
 
 template <bool BF>
 int launch_add(dc_ctx* ctx, const LoraParams& p, int max_rank) {
     const int vx = ((uintptr_t)p.x & 15) == 0 && p.ldx % 4 == 0, vy = ((uintptr_t)p.base & 7) == 0 && ((uintptr_t)p.y & 7) == 0 && p.ldb % 2 == 0 && p.ldy % 2 == 0;
-    if (p.M < LORA_TILE_ROWS)
+    if (p.M < LORA_TILE_ROWS) {
         DC_TRY(dc_launch(ctx, "k_lora_down", k_lora_down<BF>, dim3(p.M, (max_rank + 15) / 16 * 2), dim3(256), 0, p, vx));
-    else
-        DC_TRY(dc_launch(ctx, "k_lora_down_tile", k_lora_down_tile<BF>, dim3((p.M + 15) / 16, (p.Rp + DT_R - 1) / DT_R), dim3(256), 0, p, vx));
-    if (p.M < LORA_WIDE_ROWS)
-        return dc_launch(ctx, "k_lora_up", k_lora_up<BF, 1, 1>, dim3((unsigned)((p.N + 63) / 64), (p.M + 15) / 16), dim3(256), 0, p, vy);
-    return dc_launch(ctx, "k_lora_up", k_lora_up<BF, 2, 4>, dim3((unsigned)((p.N + 255) / 256), (p.M + 31) / 32), dim3(256), 0, p, vy);
+        return dc_launch(ctx, "k_lora_up_rows", k_lora_up_rows<BF>, dim3((unsigned)((p.N + 127) / 128), p.M), dim3(128), 0, p);
+    }
+    const int parts = parts_of(ctx, p.M, p.Kp);
+    DC_TRY(dc_launch(ctx, "k_lora_down_tile", k_lora_down_tile<BF>, dim3((p.M + 15) / 16, (p.Rp + DT_R - 1) / DT_R, parts), dim3(256), 0, p, vx));
+    return dc_launch(ctx, "k_lora_up", k_lora_up<BF>, dim3((unsigned)((p.N + 127) / 128), (p.M + 31) / 32), dim3(256), 0, p, vy, parts);
 }
 
 int grow(dc_ctx* ctx, dc_lora* l, int64_t rows) {
@@ -382,7 +435,7 @@ int dc_b200_lora_add_dev(dc_ctx* ctx, dc_lora* l, const float* x_dev, int64_t ld
     if (!x_dev || !ids_dev || !y_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: null buffer");
     if (!base_dev) base_dev = y_dev, ld_base = ld_y;
     cudaSetDevice(ctx->device);
-    DC_TRY(grow(ctx, l, M));
+    DC_TRY(grow(ctx, l, M < LORA_TILE_ROWS ? M : (int64_t)M * parts_of(ctx, M, l->Kp)));
     const LoraParams p = {l->a, l->b, l->rank, l->scale, l->slots, l->Rp, l->K, l->N, l->Kp, l->Np, x_dev, ld_x, M, ids_dev, l->h, base_dev, y_dev, ld_base, ld_y};
     return l->type == DC_TYPE_BF16 ? launch_add<true>(ctx, p, l->max_rank) : launch_add<false>(ctx, p, l->max_rank);
 }
