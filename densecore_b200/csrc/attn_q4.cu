@@ -46,6 +46,8 @@ __device__ __forceinline__ float lg2(float x) {
 }
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float2 pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 pair(const __nv_bfloat16* p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p)); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
@@ -54,7 +56,7 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 }
 __device__ __forceinline__ float2 unpack_h2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -185,15 +187,15 @@ struct RowsParams {
 };
 
 constexpr int RW = DC_Q4_WARPS;
-constexpr int RW_STAGES = 4;      // pages in flight, per warp
+constexpr int RW_STAGES = 3;      // pages in flight, per warp
 template <int HD>
-constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BYTES + RW * RW_STAGES * 8 + (size_t)RW * 8 * (HD + 2) * 4; }
+constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BYTES + RW * RW_STAGES * 8 + (size_t)RW * 8 * (HD + 2) * 4 + HD / 16 * 512; }
 
 // One CTA per (item, key head): its warps take the item's pages in turn, each with a running maximum of its own, and join at the end; the last CTA of a tile joins
 // the tile's splits in their order, so that results do not depend on who comes last.
 // A lane has row h = lane / 4 of the tile and tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page (t = lane % 4).
 template <int HD, typename TX>
-__global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(const RowsParams p) {
+__global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
     using R = dc_q4_rec<HD>;
     constexpr bool EXACT = sizeof(TX) == 4;
     constexpr int GR = R::GROUPS, KW = HD / 32, VW = HD / 16, OT = EXACT ? HD / 8 : HD / 16, PART = 8 * (HD + 2);
@@ -203,6 +205,8 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
     const uint32_t ring = smem_u32(smem) + warp * RW_STAGES * R::BYTES, bars = smem_u32(smem) + RW * RW_STAGES * R::BYTES + warp * RW_STAGES * 8;
     float* part = reinterpret_cast<float*>(smem + RW * RW_STAGES * R::BYTES + RW * RW_STAGES * 8);      // [RW][8][HD], then maxima and sums
     float* part_ml = part + RW * 8 * HD;
+    // EXACT: the queries as operands, [16 dimensions][lane]: they would take 4 HD / 16 registers of every warp
+    const uint32_t sq = smem_u32(part_ml + RW * 16) + lane * 16;
     if (lane == 0) {
         for (int s = 0; s < RW_STAGES; ++s) mbar_init(bars + 8 * s, 1);
         mbar_fence_init();
@@ -238,19 +242,30 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             if (i < n_my) issue(i);
         // ---- queries as fp16 terms of q 2^(10 - e), 2^e <= largest of the row < 2^(e + 1); dimensions that meet codes times 16 are divided by 16.
         // F turns the products' sums into scores in units of log2 e; qsum: sums of a group's queries in these units
-        uint32_t qa[HD / 16][EXACT ? 4 : 2];
+        uint32_t qa[EXACT ? 1 : HD / 16][2];
         float qsum[GR], F;
         {
             float x[HD / 16][4], most = 0.0f;
             const TX* src = reinterpret_cast<const TX*>(p.q) + (size_t)(im.tok0 + (row ? j : 0)) * p.ldq + (size_t)(kvh * G + (row ? g : 0)) * HD + 2 * t4;
             const float mul = p.scale * 1.4426950408889634f;
+            if (((uintptr_t)src & (2 * sizeof(TX) - 1)) == 0) {
+#pragma unroll
+                for (int s = 0; s < HD / 8; ++s) {
+                    const float2 f = row ? pair(src + 8 * s) : make_float2(0.0f, 0.0f);
+                    x[s / 2][2 * (s & 1)] = f.x, x[s / 2][2 * (s & 1) + 1] = f.y;
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[s][i] = row ? to_f32(src[16 * s + 8 * (i >> 1) + (i & 1)]) : 0.0f;
+            }
 #pragma unroll
             for (int s = 0; s < GR; ++s) qsum[s] = 0.0f;
 #pragma unroll
             for (int s = 0; s < HD / 16; ++s) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[s][i] = row ? to_f32(src[16 * s + 8 * (i >> 1) + (i & 1)]) : 0.0f;
                     most = fmaxf(most, fabsf(x[s][i]));
                     qsum[s / 4] += x[s][i];
                 }
@@ -268,19 +283,22 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             F = __uint_as_float((uint32_t)((EXACT ? 117 : 141) + e) << 23) * mul;
 #pragma unroll
             for (int s = 0; s < HD / 16; ++s) {
+                uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float a = x[s][2 * i] * (i ? up * 0.0625f : up), b = x[s][2 * i + 1] * (i ? up * 0.0625f : up);
-                    const uint32_t hi = pack_h2(a, b);
+                    w[2 * i] = pack_h2(a, b);
                     if constexpr (EXACT) {
-                        const float2 f = unpack_h2(hi);
-                        qa[s][2 * i] = hi;
-                        qa[s][2 * i + 1] = pack_h2(a - f.x, b - f.y);
+                        const float2 f = unpack_h2(w[2 * i]);
+                        w[2 * i + 1] = pack_h2(a - f.x, b - f.y);
                     } else {
-                        qa[s][i] = hi;
+                        qa[s][i] = w[2 * i];
                     }
                 }
+                if constexpr (EXACT)
+                    if (warp == s % RW) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + 512 * s), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
             }
+            if constexpr (EXACT) __syncthreads();
         }
         // EXACT: tile c of o has dimensions 8 c + 2 t, + 1 of rows h (first terms) and h (second terms); else dimensions 16 c + h and + 8 of rows 2 t, + 1
         float o[OT][4], om[GR], m_run = -1e30f, l = 0.0f;
@@ -319,31 +337,42 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             // ---- scores
             float sc[2][2], mx = -INFINITY;
             const int pos = (im.page0 + warp + i * RW) * DC_KV_BLOCK;
+            float acc[2][GR][4];
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int c = 0; c < GR; ++c) acc[a][c][0] = acc[a][c][1] = acc[a][c][2] = acc[a][c][3] = 0.0f;
+            // (groups and halves in turn: a product does not wait for the one before)
+#pragma unroll
+            for (int k = 0; k < KW / GR; ++k)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int g = 0; g < GR; ++g) {
+                        const int c = g * (KW / GR) + k;
+                        uint32_t q4[4];
+                        if constexpr (EXACT) {
+                            const uint4 f = lds128(sq + 512 * (2 * c + half));
+                            q4[0] = f.x, q4[1] = f.y, q4[2] = f.z, q4[3] = f.w;
+                        } else {
+                            q4[0] = qa[2 * c + half][0], q4[1] = 0u, q4[2] = qa[2 * c + half][1], q4[3] = 0u;
+                        }
+#pragma unroll
+                        for (int a = 0; a < 2; ++a) {
+                            uint32_t b[4];
+                            codes_of<EXACT>(kw[a][c], b);
+                            mma_f16(acc[a][g], q4, b[2 * half], b[2 * half + 1]);
+                        }
+                    }
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                float acc[GR][4];
-#pragma unroll
-                for (int c = 0; c < GR; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
-#pragma unroll
-                for (int c = 0; c < KW; ++c) {
-                    uint32_t b[4];
-                    codes_of<EXACT>(kw[a][c], b);
-                    if constexpr (EXACT) {
-                        mma_f16(acc[c / 2], qa[2 * c], b[0], b[1]);
-                        mma_f16(acc[c / 2], qa[2 * c + 1], b[2], b[3]);
-                    } else {
-                        const uint32_t q0[4] = {qa[2 * c][0], 0u, qa[2 * c][1], 0u}, q1[4] = {qa[2 * c + 1][0], 0u, qa[2 * c + 1][1], 0u};
-                        mma_f16(acc[c / 2], q0, b[0], b[1]);
-                        mma_f16(acc[c / 2], q1, b[2], b[3]);
-                    }
-                }
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     float x = 0.0f, y = 0.0f;
 #pragma unroll
                     for (int c = 0; c < GR; ++c) {
                         const float2 dm = unpack_h2(kd[a][b][c]);
-                        x = fmaf(dm.x, EXACT ? acc[c][b] + acc[c][2 + b] : acc[c][b], x);
+                        x = fmaf(dm.x, EXACT ? acc[a][c][b] + acc[a][c][2 + b] : acc[a][c][b], x);
                         y = fmaf(EXACT ? fmaf(8.0f, dm.x, dm.y) : dm.y, qsum[c], y);
                     }
                     sc[a][b] = fmaf(x, F, y);
@@ -468,8 +497,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             TX* to = reinterpret_cast<TX*>(p.out) + (size_t)(im.tok0 + jo) * p.ldo + (size_t)(kvh * G + go) * HD + 4 * (x4 % (HD / 4));
             put(to, v.x * inv), put(to + 1, v.y * inv), put(to + 2, v.z * inv), put(to + 3, v.w * inv);
         };
-#pragma unroll
-        for (int x4 = threadIdx.x; x4 < 8 * HD / 4; x4 += RW * 32) {
+        if (const int x4 = threadIdx.x; x4 < 8 * HD / 4) {
             const int rr = x4 / (HD / 4);
             float M = -1e30f, L = 0.0f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -502,14 +530,14 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             __syncthreads();
             if (s_last) {
                 // the splits' factors in place of the parts: [split][8 rows], DC_Q4_SPLITS at most; then rows' sums.  The first splits' sums are on their way meanwhile
-                static_assert(DC_Q4_SPLITS * 8 + 8 <= RW * 8 * 64, "factors take the parts' place");
-                constexpr int AHEAD = 2, X4 = 8 * HD / 4 / (RW * 32);
-                float4 first[X4][AHEAD];
+                static_assert(DC_Q4_SPLITS * 8 + 8 <= RW * 8 * 64 && RW * 32 >= 256, "factors take the parts' place");
+                constexpr int AHEAD = 4;
+                const int x4 = threadIdx.x, rr4 = x4 / (HD / 4);
+                const bool has = x4 < 8 * HD / 4;
+                float4 first[AHEAD];
 #pragma unroll
-                for (int k = 0; k < X4; ++k)
-#pragma unroll
-                    for (int s = 0; s < AHEAD; ++s)
-                        if (s < im.n_splits) first[k][s] = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + threadIdx.x + k * RW * 32);
+                for (int s = 0; s < AHEAD; ++s)
+                    if (has && s < im.n_splits) first[s] = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + x4);
                 float *f = part, *inv = part + DC_Q4_SPLITS * 8;
                 if (threadIdx.x < 32) {
                     const int rr = lane & 7;      // four lanes a row
@@ -531,24 +559,21 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
                     if (lane < 8) inv[rr] = __fdividef(1.0f, L);
                 }
                 __syncthreads();
-#pragma unroll
-                for (int k = 0; k < X4; ++k) {
-                    const int x4 = threadIdx.x + k * RW * 32, rr = x4 / (HD / 4);
+                if (has) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int s = 0; s < AHEAD; ++s)
                         if (s < im.n_splits) {
-                            const float4 x = first[k][s];
-                            const float w = f[8 * s + rr];
-                            v.x = fmaf(x.x, w, v.x), v.y = fmaf(x.y, w, v.y), v.z = fmaf(x.z, w, v.z), v.w = fmaf(x.w, w, v.w);
+                            const float w = f[8 * s + rr4];
+                            v.x = fmaf(first[s].x, w, v.x), v.y = fmaf(first[s].y, w, v.y), v.z = fmaf(first[s].z, w, v.z), v.w = fmaf(first[s].w, w, v.w);
                         }
 #pragma unroll 4
                     for (int s = AHEAD; s < im.n_splits; ++s) {
                         const float4 x = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + x4);
-                        const float w = f[8 * s + rr];
+                        const float w = f[8 * s + rr4];
                         v.x = fmaf(x.x, w, v.x), v.y = fmaf(x.y, w, v.y), v.z = fmaf(x.z, w, v.z), v.w = fmaf(x.w, w, v.w);
                     }
-                    store(x4, v, inv[rr]);
+                    store(x4, v, inv[rr4]);
                 }
             }
         }

@@ -165,16 +165,7 @@ __device__ __forceinline__ void each_adapter(int mine, uint32_t rows, F f) {    
     }
 }
 
-// A row's sums are its own adapter's; the others' passes may leave anything there (zero times an infinite matrix).
-template <int N>
-__device__ __forceinline__ void keep_rows(float (&acc)[N][4], const float (&sum)[N][4], bool u, bool v) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (u) acc[i][0] = sum[i][0], acc[i][1] = sum[i][1];
-        if (v) acc[i][2] = sum[i][2], acc[i][3] = sum[i][3];
-    }
-}
-
+// A row's sums are stored by its own adapter's pass; the others' may leave anything there (zero times an infinite matrix).
 constexpr int DT_R = 64;      // ranks of a CTA of k_lora_down_tile
 
 // Many rows: a CTA per (16 rows, 64 ranks, part of k), its warps share out the part in steps of 16 and add up in the end; the parts are added by the next kernel.
@@ -185,121 +176,124 @@ __global__ void __launch_bounds__(256) k_lora_down_tile(const LoraParams p, int 
     pdl_wait();
     pdl_launch_dependents();
     const int mine = slot_of(p, row0 + (lane & 15));
-    float acc[DT_R / 8][4];
-#pragma unroll
-    for (int i = 0; i < DT_R / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-    each_adapter(mine, 0xFFFFu, [&](int a, uint32_t mask) {
+    const int64_t per = (p.Kp / 16 + gridDim.z - 1) / gridDim.z * 16, k0 = blockIdx.z * per, k1 = min(p.Kp, k0 + per);
+    each_adapter(mine, 0xFFFFu, [&](int a, uint32_t mask) {      // (the same ones in all warps)
         const int tiles = min(DT_R / 8, ((p.rank[a] + 15) / 16 * 16 - r0) / 8);
         if (tiles <= 0) return;
-        float sum[DT_R / 8][4];
-#pragma unroll
-        for (int i = 0; i < DT_R / 8; ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.0f;
+        const float scale = p.scale[a];
+        float sum[DT_R / 8][4] = {};
         const bool u = mask >> h & 1, v = mask >> (h + 8) & 1;
         const float *xu = p.x + (size_t)(row0 + (u ? h : 0)) * p.ldx, *xv = p.x + (size_t)(row0 + (v ? h + 8 : 0)) * p.ldx;
         const uint16_t* w = p.a + ((size_t)a * p.Rp + r0 + h) * p.Kp + 4 * t;
-        const int64_t per = (p.Kp / 16 + gridDim.z - 1) / gridDim.z * 16, k0 = blockIdx.z * per, k1 = min(p.Kp, k0 + per);
 #pragma unroll 2
         for (int64_t k = k0 + 16 * warp; k < k1; k += 128) {
+            uint2 c[DT_R / 8];
+#pragma unroll
+            for (int i = 0; i < DT_R / 8; ++i) c[i] = i < tiles ? __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Kp + k)) : make_uint2(0, 0);
             const Terms x(load_x4(xu, k + 4 * t, p.K, vec, u), load_x4(xv, k + 4 * t, p.K, vec, v));
 #pragma unroll
             for (int i = 0; i < DT_R / 8; ++i)
-                if (i < tiles) {
-                    const uint2 c = __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Kp + k));
-                    x.times(sum[i], two<BF>(c.x), two<BF>(c.y));
-                }
+                if (i < tiles) x.times(sum[i], two<BF>(c[i].x), two<BF>(c[i].y));
         }
-        keep_rows(acc, sum, u, v);
+        __syncthreads();      // (the last adapter's sums have been read)
+#pragma unroll
+        for (int i = 0; i < DT_R / 8; ++i) {
+            part[warp][h][8 * i + 2 * t] = sum[i][0], part[warp][h][8 * i + 2 * t + 1] = sum[i][1];
+            part[warp][h + 8][8 * i + 2 * t] = sum[i][2], part[warp][h + 8][8 * i + 2 * t + 1] = sum[i][3];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * DT_R; i += 256) {
+            const int row = i / DT_R, r = i % DT_R;
+            if (!(mask >> row & 1) || r >= 8 * tiles) continue;
+            float s = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s += part[q][row][r];
+            p.h[((size_t)blockIdx.z * p.M + row0 + row) * p.Rp + r0 + r] = s * scale;
+        }
     });
-#pragma unroll
-    for (int i = 0; i < DT_R / 8; ++i) {
-        part[warp][h][8 * i + 2 * t] = acc[i][0], part[warp][h][8 * i + 2 * t + 1] = acc[i][1];
-        part[warp][h + 8][8 * i + 2 * t] = acc[i][2], part[warp][h + 8][8 * i + 2 * t + 1] = acc[i][3];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * DT_R; i += 256) {
-        const int row = i / DT_R, r = i % DT_R, a = slot_of(p, row0 + row);
-        if (a < 0 || r0 + r >= p.Rp) continue;
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) s += part[w][row][r];
-        p.h[((size_t)blockIdx.z * p.M + row0 + row) * p.Rp + r0 + r] = s * p.scale[a];
-    }
 }
 
-// Many rows: y = base + h B^T, a CTA per (32 rows, 128 columns), a warp has 16 columns.  h comes in `parts` sums.  Bound: base and y.
+// Many rows: y = base + h B^T, a CTA per (32 rows, 256 columns), a warp has 32 columns.  h comes in `parts` sums, 128 ranks of it at a time.  Bound: base and y.
+constexpr int UP_R = 128;
 template <bool BF>
 __global__ void __launch_bounds__(256) k_lora_up(const LoraParams p, int vec, int parts) {
-    constexpr int MT = 2, NP = 2;
+    constexpr int MT = 2, NP = 4;
+    __shared__ __align__(16) float sh[16 * MT][UP_R + 4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.y * 16 * MT;
     const int64_t n0 = ((int64_t)blockIdx.x * 8 + warp) * 8 * NP;
     pdl_wait();
     pdl_launch_dependents();
-    if (n0 >= p.N) return;
-    // base first: it is on its way during the products
-    float2 f[MT][2][NP];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int row = row0 + 16 * m + h + 8 * q;
-            const float* from = p.base + (size_t)(row < p.M ? row : 0) * p.ldb;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int64_t n = n0 + 8 * i + 2 * t;
-                if (vec && n + 1 < p.N) f[m][q][i] = *reinterpret_cast<const float2*>(from + n);
-                else f[m][q][i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
-            }
-        }
     const int mine = slot_of(p, row0 + lane);
-    float acc[MT][NP][4] = {};
-    each_adapter(mine, 0xFFFFFFFFu, [&](int a, uint32_t mask) {
-        const int ranks = p.rank[a];
-        const uint16_t* w = p.b + ((size_t)a * p.Np + n0 + h) * p.Rp + 4 * t;
-        const float* hh = p.h + (size_t)row0 * p.Rp + 4 * t;
-        float sum[MT][NP][4] = {};
-#pragma unroll 2
-        for (int r = 0; r < ranks; r += 16) {
-            uint2 c[NP];
+    auto store = [&](const float (&sum)[MT][NP][4], uint32_t mask) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) c[i] = n0 + 8 * i < p.Np ? __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Rp + r)) : make_uint2(0, 0);
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                float4 u[2] = {};
+            for (int q = 0; q < 2; ++q) {
+                const int row = row0 + 16 * m + h + 8 * q;
+                if (!(mask >> (16 * m + h + 8 * q) & 1)) continue;
+                const float* from = p.base + (size_t)row * p.ldb;
+                float* to = p.y + (size_t)row * p.ldy;
+                float2 f[NP];
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
-                    if (mask >> (16 * m + h + 8 * q) & 1)
-                        for (int z = 0; z < parts; ++z) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4*>(hh + ((size_t)z * p.M + 16 * m + h + 8 * q) * p.Rp + r));
-                            u[q].x += v.x, u[q].y += v.y, u[q].z += v.z, u[q].w += v.w;
-                        }
-                const Terms x(u[0], u[1]);
+                for (int i = 0; i < NP; ++i) {
+                    const int64_t n = n0 + 8 * i + 2 * t;
+                    if (vec && n + 1 < p.N) f[i] = *reinterpret_cast<const float2*>(from + n);
+                    else f[i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
+                }
 #pragma unroll
-                for (int i = 0; i < NP; ++i) x.times(sum[m][i], two<BF>(c[i].x), two<BF>(c[i].y));
+                for (int i = 0; i < NP; ++i) {
+                    const int64_t n = n0 + 8 * i + 2 * t;
+                    f[i].x += sum[m][i][2 * q], f[i].y += sum[m][i][2 * q + 1];
+                    if (vec && n + 1 < p.N) {
+                        *reinterpret_cast<float2*>(to + n) = f[i];
+                    } else {
+                        if (n < p.N) to[n] = f[i].x;
+                        if (n + 1 < p.N) to[n + 1] = f[i].y;
+                    }
+                }
             }
-        }
+    };
+    uint32_t rest = p.M - row0 >= 32 ? 0xFFFFFFFFu : (1u << (p.M - row0)) - 1u;
+    each_adapter(mine, rest, [&](int a, uint32_t mask) {      // (the same ones in all warps)
+        const int ranks = (p.rank[a] + 15) / 16 * 16;
+        const uint16_t* w = p.b + ((size_t)a * p.Np + n0 + h) * p.Rp + 4 * t;
+        float sum[MT][NP][4] = {};
+        for (int r0 = 0; r0 < ranks; r0 += UP_R) {
+            const int here = min(UP_R, ranks - r0), per = here / 4;
+            __syncthreads();
+            for (int i = threadIdx.x; i < 16 * MT * per; i += 256) {
+                const int row = i / per, c = i - row * per;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (mask >> row & 1)
+#pragma unroll 4
+                    for (int z = 0; z < parts; ++z) {
+                        const float4 o = __ldcg(reinterpret_cast<const float4*>(p.h + ((size_t)z * p.M + row0 + row) * p.Rp + r0) + c);
+                        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+                    }
+                *reinterpret_cast<float4*>(&sh[row][4 * c]) = v;
+            }
+            __syncthreads();
+#pragma unroll 2
+            for (int r = 0; r < here; r += 16) {
+                uint2 c[NP];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) keep_rows(acc[m], sum[m], mask >> (16 * m + h) & 1, mask >> (16 * m + h + 8) & 1);
-    });
+                for (int i = 0; i < NP; ++i) c[i] = n0 + 8 * i < p.Np ? __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Rp + r0 + r)) : make_uint2(0, 0);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+                for (int m = 0; m < MT; ++m) {
+                    if (!(mask >> (16 * m) & 0xFFFFu)) continue;
+                    const Terms x(*reinterpret_cast<const float4*>(&sh[16 * m + h][r + 4 * t]), *reinterpret_cast<const float4*>(&sh[16 * m + h + 8][r + 4 * t]));
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int row = row0 + 16 * m + h + 8 * q;
-            if (row >= p.M) continue;
-            float* to = p.y + (size_t)row * p.ldy;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int64_t n = n0 + 8 * i + 2 * t;
-                float2 v = f[m][q][i];
-                v.x += acc[m][i][2 * q], v.y += acc[m][i][2 * q + 1];
-                if (vec && n + 1 < p.N) {
-                    *reinterpret_cast<float2*>(to + n) = v;
-                } else {
-                    if (n < p.N) to[n] = v.x;
-                    if (n + 1 < p.N) to[n + 1] = v.y;
+                    for (int i = 0; i < NP; ++i) x.times(sum[m][i], two<BF>(c[i].x), two<BF>(c[i].y));
                 }
             }
         }
+        store(sum, mask);
+        rest &= ~mask;
+    });
+    if (rest && (p.y != p.base || p.ldy != p.ldb)) {      // rows without an adapter
+        const float none[MT][NP][4] = {};
+        store(none, rest);
+    }
 }
 
 // One adapter's matrices into their padded places; `rank` 0 empties the slot.
@@ -338,7 +332,7 @@ int launch_add(dc_ctx* ctx, const LoraParams& p, int max_rank) {
     }
     const int parts = parts_of(ctx, p.M, p.Kp);
     DC_TRY(dc_launch(ctx, "k_lora_down_tile", k_lora_down_tile<BF>, dim3((p.M + 15) / 16, (p.Rp + DT_R - 1) / DT_R, parts), dim3(256), 0, p, vx));
-    return dc_launch(ctx, "k_lora_up", k_lora_up<BF>, dim3((unsigned)((p.N + 127) / 128), (p.M + 31) / 32), dim3(256), 0, p, vy, parts);
+    return dc_launch(ctx, "k_lora_up", k_lora_up<BF>, dim3((unsigned)((p.N + 255) / 256), (p.M + 31) / 32), dim3(256), 0, p, vy, parts);
 }
 
 int grow(dc_ctx* ctx, dc_lora* l, int64_t rows) {
