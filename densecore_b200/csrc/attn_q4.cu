@@ -205,8 +205,9 @@ __global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
     const uint32_t ring = smem_u32(smem) + warp * RW_STAGES * R::BYTES, bars = smem_u32(smem) + RW * RW_STAGES * R::BYTES + warp * RW_STAGES * 8;
     float* part = reinterpret_cast<float*>(smem + RW * RW_STAGES * R::BYTES + RW * RW_STAGES * 8);      // [RW][8][HD], then maxima and sums
     float* part_ml = part + RW * 8 * HD;
-    // EXACT: the queries as operands, [16 dimensions][lane]: they would take 4 HD / 16 registers of every warp
-    const uint32_t sq = smem_u32(part_ml + RW * 16) + lane * 16;
+    // the queries as operands, [16 dimensions][lane]: they would take HD / 8 or HD / 4 registers of every warp
+    constexpr int QB = EXACT ? 16 : 8;
+    const uint32_t sq = smem_u32(part_ml + RW * 16) + lane * QB;
     if (lane == 0) {
         for (int s = 0; s < RW_STAGES; ++s) mbar_init(bars + 8 * s, 1);
         mbar_fence_init();
@@ -242,7 +243,6 @@ __global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
             if (i < n_my) issue(i);
         // ---- queries as fp16 terms of q 2^(10 - e), 2^e <= largest of the row < 2^(e + 1); dimensions that meet codes times 16 are divided by 16.
         // F turns the products' sums into scores in units of log2 e; qsum: sums of a group's queries in these units
-        uint32_t qa[EXACT ? 1 : HD / 16][2];
         float qsum[GR], F;
         {
             float x[HD / 16][4], most = 0.0f;
@@ -291,14 +291,14 @@ __global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
                     if constexpr (EXACT) {
                         const float2 f = unpack_h2(w[2 * i]);
                         w[2 * i + 1] = pack_h2(a - f.x, b - f.y);
-                    } else {
-                        qa[s][i] = w[2 * i];
                     }
                 }
-                if constexpr (EXACT)
-                    if (warp == s % RW) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + 512 * s), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                if (warp == s % RW) {
+                    if constexpr (EXACT) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + 32 * QB * s), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    else asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(sq + 32 * QB * s), "r"(w[0]), "r"(w[2]) : "memory");
+                }
             }
-            if constexpr (EXACT) __syncthreads();
+            __syncthreads();
         }
         // EXACT: tile c of o has dimensions 8 c + 2 t, + 1 of rows h (first terms) and h (second terms); else dimensions 16 c + h and + 8 of rows 2 t, + 1
         float o[OT][4], om[GR], m_run = -1e30f, l = 0.0f;
@@ -352,10 +352,11 @@ __global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
                         const int c = g * (KW / GR) + k;
                         uint32_t q4[4];
                         if constexpr (EXACT) {
-                            const uint4 f = lds128(sq + 512 * (2 * c + half));
+                            const uint4 f = lds128(sq + 32 * QB * (2 * c + half));
                             q4[0] = f.x, q4[1] = f.y, q4[2] = f.z, q4[3] = f.w;
                         } else {
-                            q4[0] = qa[2 * c + half][0], q4[1] = 0u, q4[2] = qa[2 * c + half][1], q4[3] = 0u;
+                            const uint2 f = lds64(sq + 32 * QB * (2 * c + half));
+                            q4[0] = f.x, q4[1] = 0u, q4[2] = f.y, q4[3] = 0u;
                         }
 #pragma unroll
                         for (int a = 0; a < 2; ++a) {

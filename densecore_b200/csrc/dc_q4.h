@@ -61,8 +61,8 @@ inline void dc_q4_items(const std::vector<dc_q4_entry>& es, int G, int n_kv, int
     long long work = 0;
     for (const dc_q4_entry& e : es)
         for (int t = 0; t < tiles_of(e); ++t) work += pages_of(e, t);
-    // pages of an item: eight rounds of two CTAs an SM where there is that much, six pages a warp at least (joining parts takes as long as some five pages)
-    const long long slots = (long long)num_sms * 2 * 8;
+    // pages of an item: four rounds of two CTAs an SM where there is that much, six pages a warp at least (joining parts takes as long as some five pages)
+    const long long slots = (long long)num_sms * 2 * 4;
     const int per = (int)std::max<long long>(6 * DC_Q4_WARPS, (work * n_kv + slots - 1) / slots);
     *n_tickets = *n_ws = 0;
     for (const dc_q4_entry& e : es)

@@ -170,7 +170,7 @@ constexpr int DT_R = 64;      // ranks of a CTA of k_lora_down_tile
 
 // Many rows: a CTA per (16 rows, 64 ranks, part of k), its warps share out the part in steps of 16 and add up in the end; the parts are added by the next kernel.
 template <bool BF>
-__global__ void __launch_bounds__(256) k_lora_down_tile(const LoraParams p, int vec) {
+__global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, int vec) {
     __shared__ float part[8][16][DT_R + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.x * 16, r0 = blockIdx.y * DT_R;
     pdl_wait();
@@ -213,47 +213,49 @@ __global__ void __launch_bounds__(256) k_lora_down_tile(const LoraParams p, int 
     });
 }
 
-// Many rows: y = base + h B^T, a CTA per (32 rows, 256 columns), a warp has 32 columns.  h comes in `parts` sums, 128 ranks of it at a time.  Bound: base and y.
+// Many rows: y = base + h B^T, a CTA per (16 rows, 256 columns), a warp has 32 columns.  h comes in `parts` sums, 128 ranks of it at a time; base is on its way
+// meanwhile.  Bound: base and y.
 constexpr int UP_R = 128;
 template <bool BF>
-__global__ void __launch_bounds__(256) k_lora_up(const LoraParams p, int vec, int parts) {
-    constexpr int MT = 2, NP = 4;
+__global__ void __launch_bounds__(256, 3) k_lora_up(const LoraParams p, int vec, int parts) {
+    constexpr int MT = 1, NP = 4;
     __shared__ __align__(16) float sh[16 * MT][UP_R + 4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.y * 16 * MT;
     const int64_t n0 = ((int64_t)blockIdx.x * 8 + warp) * 8 * NP;
     pdl_wait();
     pdl_launch_dependents();
-    const int mine = slot_of(p, row0 + lane);
+    float2 f[2][NP];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int row = row0 + h + 8 * q;
+        const float* from = p.base + (size_t)(row < p.M ? row : 0) * p.ldb;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int64_t n = n0 + 8 * i + 2 * t;
+            if (vec && n + 1 < p.N) f[q][i] = *reinterpret_cast<const float2*>(from + n);
+            else f[q][i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
+        }
+    }
+    const int mine = slot_of(p, row0 + (lane & 15));
     auto store = [&](const float (&sum)[MT][NP][4], uint32_t mask) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int q = 0; q < 2; ++q) {
+            if (!(mask >> (h + 8 * q) & 1)) continue;
+            float* to = p.y + (size_t)(row0 + h + 8 * q) * p.ldy;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int row = row0 + 16 * m + h + 8 * q;
-                if (!(mask >> (16 * m + h + 8 * q) & 1)) continue;
-                const float* from = p.base + (size_t)row * p.ldb;
-                float* to = p.y + (size_t)row * p.ldy;
-                float2 f[NP];
-#pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    const int64_t n = n0 + 8 * i + 2 * t;
-                    if (vec && n + 1 < p.N) f[i] = *reinterpret_cast<const float2*>(from + n);
-                    else f[i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
-                }
-#pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    const int64_t n = n0 + 8 * i + 2 * t;
-                    f[i].x += sum[m][i][2 * q], f[i].y += sum[m][i][2 * q + 1];
-                    if (vec && n + 1 < p.N) {
-                        *reinterpret_cast<float2*>(to + n) = f[i];
-                    } else {
-                        if (n < p.N) to[n] = f[i].x;
-                        if (n + 1 < p.N) to[n + 1] = f[i].y;
-                    }
+            for (int i = 0; i < NP; ++i) {
+                const int64_t n = n0 + 8 * i + 2 * t;
+                const float2 v = make_float2(f[q][i].x + sum[0][i][2 * q], f[q][i].y + sum[0][i][2 * q + 1]);
+                if (vec && n + 1 < p.N) {
+                    *reinterpret_cast<float2*>(to + n) = v;
+                } else {
+                    if (n < p.N) to[n] = v.x;
+                    if (n + 1 < p.N) to[n + 1] = v.y;
                 }
             }
+        }
     };
-    uint32_t rest = p.M - row0 >= 32 ? 0xFFFFFFFFu : (1u << (p.M - row0)) - 1u;
+    uint32_t rest = p.M - row0 >= 16 ? 0xFFFFu : (1u << (p.M - row0)) - 1u;
     each_adapter(mine, rest, [&](int a, uint32_t mask) {      // (the same ones in all warps)
         const int ranks = (p.rank[a] + 15) / 16 * 16;
         const uint16_t* w = p.b + ((size_t)a * p.Np + n0 + h) * p.Rp + 4 * t;
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(256) k_lora_set(const uint16_t* __restrict__ a
     if (blockIdx.x == 0 && threadIdx.x == 0) *rank_at = rank, *scale_at = scale;
 }
 
-// Rows from which tiles are taken: they read a matrix once for 16 or 32 rows; below, one warp a rank and one thread a column have shorter chains of loads.
+// Rows from which tiles are taken: they read a matrix once for 16 rows; below, one warp a rank and one thread a column have shorter chains of loads.
 constexpr int LORA_TILE_ROWS = 97;
 constexpr int LORA_PARTS = 4;      // of k, at most
 
@@ -332,7 +334,7 @@ int launch_add(dc_ctx* ctx, const LoraParams& p, int max_rank) {
     }
     const int parts = parts_of(ctx, p.M, p.Kp);
     DC_TRY(dc_launch(ctx, "k_lora_down_tile", k_lora_down_tile<BF>, dim3((p.M + 15) / 16, (p.Rp + DT_R - 1) / DT_R, parts), dim3(256), 0, p, vx));
-    return dc_launch(ctx, "k_lora_up", k_lora_up<BF>, dim3((unsigned)((p.N + 255) / 256), (p.M + 31) / 32), dim3(256), 0, p, vy, parts);
+    return dc_launch(ctx, "k_lora_up", k_lora_up<BF>, dim3((unsigned)((p.N + 255) / 256), (p.M + 15) / 16), dim3(256), 0, p, vy, parts);
 }
 
 int grow(dc_ctx* ctx, dc_lora* l, int64_t rows) {
