@@ -195,7 +195,7 @@ constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BY
 // the tile's splits in their order, so that results do not depend on who comes last.
 // A lane has row h = lane / 4 of the tile and tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page (t = lane % 4).
 template <int HD, typename TX>
-__global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
+__global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(const RowsParams p) {
     using R = dc_q4_rec<HD>;
     constexpr bool EXACT = sizeof(TX) == 4;
     constexpr int GR = R::GROUPS, KW = HD / 32, VW = HD / 16, OT = EXACT ? HD / 8 : HD / 16, PART = 8 * (HD + 2);
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
             TX* to = reinterpret_cast<TX*>(p.out) + (size_t)(im.tok0 + jo) * p.ldo + (size_t)(kvh * G + go) * HD + 4 * (x4 % (HD / 4));
             put(to, v.x * inv), put(to + 1, v.y * inv), put(to + 2, v.z * inv), put(to + 3, v.w * inv);
         };
-        if (const int x4 = threadIdx.x; x4 < 8 * HD / 4) {
+        for (int x4 = threadIdx.x; x4 < 8 * HD / 4; x4 += RW * 32) {
             const int rr = x4 / (HD / 4);
             float M = -1e30f, L = 0.0f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -531,14 +531,14 @@ __global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
             __syncthreads();
             if (s_last) {
                 // the splits' factors in place of the parts: [split][8 rows], DC_Q4_SPLITS at most; then rows' sums.  The first splits' sums are on their way meanwhile
-                static_assert(DC_Q4_SPLITS * 8 + 8 <= RW * 8 * 64 && RW * 32 >= 256, "factors take the parts' place");
-                constexpr int AHEAD = 4;
-                const int x4 = threadIdx.x, rr4 = x4 / (HD / 4);
-                const bool has = x4 < 8 * HD / 4;
-                float4 first[AHEAD];
+                static_assert(DC_Q4_SPLITS * 8 + 8 <= RW * 8 * 64 && 8 * HD / 4 % (RW * 32) == 0, "factors take the parts' place");
+                constexpr int AHEAD = 2, X4 = 8 * HD / 4 / (RW * 32);
+                float4 first[X4][AHEAD];
 #pragma unroll
-                for (int s = 0; s < AHEAD; ++s)
-                    if (has && s < im.n_splits) first[s] = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + x4);
+                for (int k = 0; k < X4; ++k)
+#pragma unroll
+                    for (int s = 0; s < AHEAD; ++s)
+                        if (s < im.n_splits) first[k][s] = __ldcg(reinterpret_cast<const float4*>(ws + (size_t)s * PART) + threadIdx.x + k * RW * 32);
                 float *f = part, *inv = part + DC_Q4_SPLITS * 8;
                 if (threadIdx.x < 32) {
                     const int rr = lane & 7;      // four lanes a row
@@ -560,13 +560,15 @@ __global__ void __launch_bounds__(RW * 32, 2) k_q4_rows(const RowsParams p) {
                     if (lane < 8) inv[rr] = __fdividef(1.0f, L);
                 }
                 __syncthreads();
-                if (has) {
+#pragma unroll
+                for (int k = 0; k < X4; ++k) {
+                    const int x4 = threadIdx.x + k * RW * 32, rr4 = x4 / (HD / 4);
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int s = 0; s < AHEAD; ++s)
                         if (s < im.n_splits) {
                             const float w = f[8 * s + rr4];
-                            v.x = fmaf(first[s].x, w, v.x), v.y = fmaf(first[s].y, w, v.y), v.z = fmaf(first[s].z, w, v.z), v.w = fmaf(first[s].w, w, v.w);
+                            v.x = fmaf(first[k][s].x, w, v.x), v.y = fmaf(first[k][s].y, w, v.y), v.z = fmaf(first[k][s].z, w, v.z), v.w = fmaf(first[k][s].w, w, v.w);
                         }
 #pragma unroll 4
                     for (int s = AHEAD; s < im.n_splits; ++s) {

@@ -51,7 +51,7 @@ struct dc_q4_tile {
 struct dc_q4_entry {
     int32_t seq, pos0, count, tok0;
 };
-constexpr int DC_Q4_WARPS = 8;      // of a CTA of k_q4_rows
+constexpr int DC_Q4_WARPS = 4;      // of a CTA of k_q4_rows
 constexpr int DC_Q4_SPLITS = 240;   // of a tile, at most
 
 // The items of all tiles of the entries; *n_ws: partial results, *n_tickets: tiles that more than one CTA works on.
@@ -61,8 +61,8 @@ inline void dc_q4_items(const std::vector<dc_q4_entry>& es, int G, int n_kv, int
     long long work = 0;
     for (const dc_q4_entry& e : es)
         for (int t = 0; t < tiles_of(e); ++t) work += pages_of(e, t);
-    // pages of an item: four rounds of two CTAs an SM where there is that much, six pages a warp at least (joining parts takes as long as some five pages)
-    const long long slots = (long long)num_sms * 2 * 4;
+    // pages of an item: four rounds of three CTAs an SM where there is that much, six pages a warp at least (joining parts takes as long as some five pages)
+    const long long slots = (long long)num_sms * 3 * 4;
     const int per = (int)std::max<long long>(6 * DC_Q4_WARPS, (work * n_kv + slots - 1) / slots);
     *n_tickets = *n_ws = 0;
     for (const dc_q4_entry& e : es)
