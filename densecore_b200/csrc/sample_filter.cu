@@ -32,7 +32,7 @@ using namespace dc;
 namespace {
 
 typedef unsigned long long u64;
-constexpr int SF_T = 512, SF_W = SF_T / 32, SF_BINS = 2048, SF_LIST = 1024, SF_SHORT = 256, SF_CLUSTER = 16;
+constexpr int SF_T = 512, SF_W = SF_T / 32, SF_BINS = 2048, SF_LIST = 1024, SF_SHORT = 256, SF_NEAR = 64, SF_CLUSTER = 16;
 constexpr int SF_GROUPS = 256;          // of a row's threads, 2 n_cta neighbours each
 constexpr int SF_MOST = 48 * 1024;      // f32 tokens of a CTA
 constexpr int SF_VOCAB = 8 * (SF_MOST - 32 * SF_W);
@@ -73,9 +73,9 @@ struct Weigher {
         const u64 whole = t > 26388279066624.0 - 46.0 ? (u64)__double_as_longlong(w) - 0x4070000000000000ull : 0ull;      // (none for -inf and NaN)
         return infinite ? (x == INFINITY ? SF_ONE : 0ull) : whole;
     }
-    // bounds on weights in a bin of 32 to a power of two: the rounding of the bin's number (2048 / 32 2^-22 of the exponent) and of exp2 (2^-22) are less than 1e-4 of the exponent
-    __device__ __forceinline__ static float above(float b) { return exp2f(fmaf(b, -0.03125f, 44.0001f)) + 1.0f; }
-    __device__ __forceinline__ static float below(float b) { return fmaxf(exp2f(fmaf(b, -0.03125f, 43.9686f)) - 1.0f, 0.0f); }
+    // bounds on weights in a bin of 64 to a power of two: the rounding of the bin's number (2048 / 64 2^-22 of the exponent) and of exp2 (2^-22) are less than 1e-4 of the exponent
+    __device__ __forceinline__ static float above(float b) { return exp2f(fmaf(b, -0.015625f, 44.0001f)) + 1.0f; }
+    __device__ __forceinline__ static float below(float b) { return fmaxf(exp2f(fmaf(b, -0.015625f, 43.984275f)) - 1.0f, 0.0f); }
 };
 
 struct alignas(16) Shared {      // beside the row and the histogram
@@ -285,7 +285,7 @@ struct Sampler {
         if (rank == 0) {
             const u64 sum = sh->sum;
             if (threadIdx.x == 0) everywhere(&Shared::total, sum);
-            // (bins that are not 32 to a power of two, at extreme temperatures, bound nothing from below)
+            // (bins that are not 64 to a power of two, at extreme temperatures, bound nothing from below)
             const bool bounded = per_unit < 1e30f && !w.infinite;
             find_weight(0.0, (double)top_p * (double)sum, [&](int b) { return bounded ? (double)w.above((float)b) : (double)SF_ONE; },
                         [&](int b) { return bounded && b < SF_BINS - 1 ? (double)w.below((float)b) : 0.0; });
@@ -354,7 +354,7 @@ struct Sampler {
     __device__ u64 cut_at(u64 from, long long count, float top_p, u64 total, u64* mine) {
         const bool weights = count <= 0;
         const double goal = (double)top_p * (double)total;
-        const int b0 = sh->bin, b1 = sh->bin2;
+        int b0 = sh->bin, b1 = sh->bin2;
         uint32_t lo = 0, hi = 0xFFFFFFFFu;
         bool by_bin = true;
         auto in = [&](float x, int i) {
@@ -370,7 +370,53 @@ struct Sampler {
         int inside = weights ? sh->upto - (int)kept : sh->inside;
         u64 before = 0;                                 // their weights
         *mine = 0;
-        if (weights) {
+        if (weights && b1 > b0 && b1 - b0 < SF_NEAR) {
+            // the bounds are few bins apart: the weights of each, a warp's own (its tokens fall into them one by one), then the bin with the cut
+            for (int i = threadIdx.x; i < SF_W * SF_NEAR; i += SF_T) wh[i] = 0;
+            if (threadIdx.x == 0) sh->sum = 0;
+            if (threadIdx.x < SF_NEAR) sh->group[threadIdx.x] = 0;
+            cl.sync();
+            u64 sum = 0;
+            each([&](float x, int i) {
+                const int b = x > -INFINITY && (!from || token_key(x, i) >= from) ? bin_of(x) : SF_BINS;
+                if (b <= b1) {
+                    const u64 v = w(x);
+                    if (b < b0) sum += v;
+                    else atomicAdd(wh + warp * SF_NEAR + b - b0, v);
+                }
+            });
+            *mine = sum;
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+            if (lane == 0 && sum) atomicAdd(&cl.map_shared_rank(sh, 0)->sum, sum);
+            __syncthreads();
+            if (threadIdx.x < SF_NEAR) {
+                u64 v = 0;
+                for (int i = 0; i < SF_W; ++i) v += wh[i * SF_NEAR + threadIdx.x];
+                if (v) atomicAdd(&cl.map_shared_rank(sh, 0)->group[threadIdx.x], v);
+            }
+            cl.sync();
+            if (rank == 0 && threadIdx.x == 0) {
+                u64 at = sh->sum;
+                u64 tokens = sh->in_before;
+                int b = b0;
+                for (; b < b1 && (double)(at + sh->group[b - b0]) < goal; ++b) at += sh->group[b - b0], tokens += cnt[b];
+                const int n = (int)cnt[b];
+                everywhere(&Shared::bin, b);
+                everywhere(&Shared::total, at);
+                everywhere(&Shared::in_before, tokens);
+                everywhere(&Shared::inside, n);
+            }
+            cl.sync();
+            const int b = sh->bin;
+            if (lane == 0)
+                for (int i = b0; i < b; ++i) *mine += wh[warp * SF_NEAR + i - b0];
+            b0 = b1 = b;
+            before = sh->total;
+            kept = (long long)sh->in_before;
+            inside = sh->inside;
+            cl.sync();      // (what was written has been read, and the list's place is free)
+        } else if (weights) {
             u64 sum = 0;
             each([&](float x, int i) { if (x > -INFINITY && bin_of(x) < b0 && (!from || token_key(x, i) >= from)) sum += w(x); });
             *mine = sum;
@@ -803,8 +849,8 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
         s.cl.sync();
         return;
     }
-    // bins: 64 to a unit of the logits where the cut goes by number, 32 to a power of two of the weights where it goes by weight
-    const float weight_bins = s.w.infinite ? 0.0f : fminf(32.0f * 1.44269504f / T, 1e30f);
+    // bins: 64 to a unit of the logits where the cut goes by number, 64 to a power of two of the weights where it goes by weight
+    const float weight_bins = s.w.infinite ? 0.0f : fminf(64.0f * 1.44269504f / T, 1e30f);
     s.to_bin = s.w.infinite ? 0.0f : count ? 64.0f : weight_bins;
     u64 total = 0;
     bool listed = false;
