@@ -182,7 +182,7 @@ struct RowsParams {
     const uint8_t* arena;
     float scale;
     void* out;
-    int early;      // the kernel before this one wrote the step's rows and waited for all before it: older pages may be read ahead of the wait
+    int early;      // dc_q4_call
     int* err;
 };
 
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
         auto issue = [&](int i) {
             const int page = im.page0 + warp + i * RW;
             if (i % 32 == 0) entry = i + lane < n_my ? table[page + lane * RW] : 0;
-            if (!waited && page >= first_new) pdl_wait(), waited = true;
+            if (!waited && p.early == 1 && page >= first_new) pdl_wait(), waited = true;
             const int block = __shfl_sync(0xffffffffu, entry, i % 32);
             if (lane == 0) {
                 const uint32_t s = (n_full + i) % RW_STAGES;
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             }
         }
         if (t4 == 0) part_ml[2 * (warp * 8 + h)] = m_run, part_ml[2 * (warp * 8 + h) + 1] = l;
-        if (!waited) pdl_wait(), waited = true;      // (ahead of the first store)
+        if (!waited && p.early == 1) pdl_wait(), waited = true;      // (ahead of the first store)
         __syncthreads();
         // ---- joined: a thread has four neighbouring dimensions of a row at a time
         const bool alone = im.n_splits == 1;
@@ -582,14 +582,14 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
         }
         __syncthreads();      // the parts are free for the next item
     }
-    if (!waited) pdl_wait();
+    if (!waited) pdl_wait();      // (a successor that waits for this kernel waits for its predecessor too)
 }
 
 template <int HD, typename TX>
 int launch_rows(dc_ctx* ctx, const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
     DC_TRY(dc_kernel_setup(ctx, (const void*)k_q4_rows<HD, TX>, (int)rows_smem<HD>(), "k_q4_rows"));
-    RowsParams p = {(const dc_q4_head*)z.plan, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.after_write ? 1 : 0, ctx->d_err};
+    RowsParams p = {(const dc_q4_head*)z.plan, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.early, ctx->d_err};
     return dc_launch(ctx, "k_q4_rows", k_q4_rows<HD, TX>, dim3(z.n_items, z.kv), dim3(RW * 32), rows_smem<HD>(), p);
 }
 
@@ -663,14 +663,14 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
     dc_q4_tiles(many, G, z.kv, ctx->num_sms, &tiles, &n_parts);
     for (size_t i = 0; i < tiles.size(); ++i)
         if (tiles[i].n_splits > 1 && tiles[i].split == 0) joins.push_back((int32_t)i);
-    // ---- header, arrays, tickets (zero, and left so by every call), partial results (one kernel's after the other's: the rows kernel has joined its own when the next starts)
-    const size_t need[6] = {tokens.size() * sizeof(dc_q4_token), items.size() * sizeof(dc_q4_item), tiles.size() * sizeof(dc_q4_tile), joins.size() * 4, (size_t)n_tickets * z.kv * 4,
-                            std::max((size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4, (size_t)n_parts * z.kv * 256 * (z.dim + 4) * 4)};
+    // ---- header, arrays, tickets (zero, and left so by every call), partial results
+    const size_t need[DC_Q4_ARRAYS] = {tokens.size() * sizeof(dc_q4_token), items.size() * sizeof(dc_q4_item), tiles.size() * sizeof(dc_q4_tile), joins.size() * 4, (size_t)n_tickets * z.kv * 4,
+                                       (size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4, (size_t)n_parts * z.kv * 256 * (z.dim + 4) * 4};
     bool fits = z.plan != nullptr;
-    for (int i = 0; i < 6; ++i) fits = fits && need[i] <= z.cap[i];
+    for (int i = 0; i < DC_Q4_ARRAYS; ++i) fits = fits && need[i] <= z.cap[i];
     if (!fits) {
-        size_t cap[6], at[6], bytes = 256;
-        for (int i = 0; i < 6; ++i) {
+        size_t cap[DC_Q4_ARRAYS], at[DC_Q4_ARRAYS], bytes = 256;
+        for (int i = 0; i < DC_Q4_ARRAYS; ++i) {
             cap[i] = std::max(z.cap[i], (need[i] + need[i] / 2 + 4096) / 256 * 256);
             at[i] = bytes;
             bytes += cap[i];
@@ -683,7 +683,7 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
         }
         DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(fresh, 0, at[DC_Q4_WS], ctx->stream), "kv_batch: plan"));
         z.plan = fresh, z.plan_bytes = bytes;
-        std::copy(cap, cap + 6, z.cap), std::copy(at, at + 6, z.at);
+        std::copy(cap, cap + DC_Q4_ARRAYS, z.cap), std::copy(at, at + DC_Q4_ARRAYS, z.at);
     }
     if (!z.uploaded) DC_TRY(dc_check_cuda(ctx, cudaEventCreateWithFlags(&z.uploaded, cudaEventDisableTiming), "kv_batch: event"));
     else DC_TRY(dc_check_cuda(ctx, cudaEventSynchronize(z.uploaded), "kv_batch: staging"));
@@ -819,9 +819,11 @@ int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const voi
     if (!isfinite(scale)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: scale is not finite");
     cudaSetDevice(ctx->device);
     if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev));
-    const dc_q4_call c = {kv, kv->planes[layer].arena, q_dev, ld_q, ld_out, scale, out_dev, k_dev != nullptr};
+    dc_q4_call c = {kv, kv->planes[layer].arena, q_dev, ld_q, ld_out, scale, out_dev, k_dev ? 1 : 0};
+    DC_TRY(dc_launch_q4_prompt(ctx, c));
+    if (z.n_tiles) c.early = 2;      // the SMs that prompt tiles leave idle take the single tokens meanwhile
     DC_TRY(dc_launch_q4_rows(ctx, c));
-    return dc_launch_q4_prompt(ctx, c);
+    return dc_launch_q4_join(ctx, c);
 }
 
 int dc_b200_flash_attn_q4(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_host, const void* k_host, const void* v_host, float scale, void* out_host) {

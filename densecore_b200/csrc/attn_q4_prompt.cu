@@ -498,17 +498,35 @@ __global__ void __launch_bounds__(256) k_q4_join(const PromptParams p) {
     const float* from = p.ws + ((size_t)tl.ws * p.n_kv + (size_t)tl.n_splits * kvh) * PART + r * ROW;
     constexpr int PER = HD / 32;
     float M = -1e30f, l = 0.0f, v[PER] = {};
-    for (int s = 0; s < tl.n_splits; ++s) M = fmaxf(M, __ldcg(from + s * PART + HD));
-    for (int s = 0; s < tl.n_splits; ++s) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + s * PART + HD));
-        const float f = ex2(ml.x - M);
-        l = fmaf(ml.y, f, l);
-        if constexpr (PER == 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(from + s * PART) + lane);
-            v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]), v[2] = fmaf(x.z, f, v[2]), v[3] = fmaf(x.w, f, v[3]);
-        } else {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(from + s * PART) + lane);
-            v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]);
+    for (int s0 = 0; s0 < tl.n_splits; s0 += 4) {      // four parts' numbers on their way at once
+        float2 ml[4];
+        float x[4][PER];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float* at = from + (size_t)min(s0 + k, tl.n_splits - 1) * PART;
+            ml[k] = __ldcg(reinterpret_cast<const float2*>(at + HD));
+            if constexpr (PER == 4) {
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(at) + lane);
+                x[k][0] = f.x, x[k][1] = f.y, x[k][2] = f.z, x[k][3] = f.w;
+            } else {
+                const float2 f = __ldcg(reinterpret_cast<const float2*>(at) + lane);
+                x[k][0] = f.x, x[k][1] = f.y;
+            }
+        }
+        float m = M;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, ml[k].x);
+        const float old = ex2(M - m);
+        M = m, l *= old;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] *= old;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (s0 + k >= tl.n_splits) break;
+            const float f = ex2(ml[k].x - M);
+            l = fmaf(ml[k].y, f, l);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = fmaf(x[k][i], f, v[i]);
         }
     }
     const float inv = 1.0f / l;
@@ -518,14 +536,16 @@ __global__ void __launch_bounds__(256) k_q4_join(const PromptParams p) {
     for (int i = 0; i < PER; ++i) dst[i] = __float2bfloat16_rn(v[i] * inv);
 }
 
+PromptParams params(const dc_q4_call& c) {
+    const dc_q4& z = *c.kv->q4;
+    return {(const dc_q4_head*)z.plan, (const dc_q4_tile*)(z.plan + z.at[DC_Q4_TILES]), (const int32_t*)(z.plan + z.at[DC_Q4_JOINS]), (float*)(z.plan + z.at[DC_Q4_PARTS]),
+            (const __nv_bfloat16*)c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, (__nv_bfloat16*)c.out};
+}
+
 template <int HD>
 int launch(dc_ctx* ctx, const dc_q4_call& c) {
-    const dc_q4& z = *c.kv->q4;
     DC_TRY(dc_kernel_setup_unspilled(ctx, (const void*)k_q4_prompt<HD>, (int)Lay<HD>::SMEM, "k_q4_prompt"));
-    PromptParams p = {(const dc_q4_head*)z.plan, (const dc_q4_tile*)(z.plan + z.at[DC_Q4_TILES]), (const int32_t*)(z.plan + z.at[DC_Q4_JOINS]), (float*)(z.plan + z.at[DC_Q4_WS]), (const __nv_bfloat16*)c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, (__nv_bfloat16*)c.out};
-    DC_TRY(dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(z.kv, z.n_tiles), dim3(QP_THREADS), Lay<HD>::SMEM, p, ctx->d_err));
-    if (!z.n_joins) return DC_B200_OK;
-    return dc_launch(ctx, "k_q4_join", k_q4_join<HD>, dim3(z.n_joins, z.kv, 2 * QP_ROWS / 8), dim3(256), 0, p);
+    return dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(c.kv->q4->kv, c.kv->q4->n_tiles), dim3(QP_THREADS), Lay<HD>::SMEM, params(c), ctx->d_err);
 }
 
 }  // namespace
@@ -533,4 +553,11 @@ int launch(dc_ctx* ctx, const dc_q4_call& c) {
 int dc_launch_q4_prompt(dc_ctx* ctx, const dc_q4_call& c) {
     if (c.kv->q4->n_tiles == 0) return DC_B200_OK;
     return c.kv->q4->dim == 128 ? launch<128>(ctx, c) : launch<64>(ctx, c);
+}
+
+int dc_launch_q4_join(dc_ctx* ctx, const dc_q4_call& c) {
+    const dc_q4& z = *c.kv->q4;
+    if (z.n_joins == 0) return DC_B200_OK;
+    const dim3 grid(z.n_joins, z.kv, 2 * QP_ROWS / 8);
+    return z.dim == 128 ? dc_launch(ctx, "k_q4_join", k_q4_join<128>, grid, dim3(256), 0, params(c)) : dc_launch(ctx, "k_q4_join", k_q4_join<64>, grid, dim3(256), 0, params(c));
 }

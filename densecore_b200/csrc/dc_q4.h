@@ -101,14 +101,14 @@ struct dc_q4 {
     int T = 0, n_items = 0, n_tiles = 0, n_joins = 0;
     uint8_t* plan = nullptr;
     size_t plan_bytes = 0;
-    size_t cap[6] = {}, at[6] = {};     // room for the arrays and where they begin: tokens, items, tiles, joins, tickets, partial results
+    size_t cap[7] = {}, at[7] = {};     // room for the arrays and where they begin: tokens, items, tiles, joins, tickets, partial results of rows and of prompt tiles
     std::vector<uint8_t*> retired;      // outgrown plans, emptied; captured calls may still read them
     uint8_t* stage = nullptr;           // pinned copy of the plan being uploaded
     size_t stage_bytes = 0;
     cudaEvent_t uploaded = nullptr;
 };
 
-enum { DC_Q4_TOKENS = 0, DC_Q4_ITEMS, DC_Q4_TILES, DC_Q4_JOINS, DC_Q4_TICKETS, DC_Q4_WS };
+enum { DC_Q4_TOKENS = 0, DC_Q4_ITEMS, DC_Q4_TILES, DC_Q4_JOINS, DC_Q4_TICKETS, DC_Q4_WS, DC_Q4_PARTS, DC_Q4_ARRAYS };
 
 struct dc_q4_call {
     const dc_kv_cache* kv;
@@ -117,7 +117,9 @@ struct dc_q4_call {
     int ldq, ldo;
     float scale;
     void* out;
-    bool after_write;          // the kernel before it in the stream is this call's k_q4_write
+    int early;                 // what k_q4_rows may do ahead of its predecessor's end: 0 nothing, 1 all but the step's own pages and stores (k_q4_write), 2 everything
+                               // (k_q4_prompt of the same call, whose CTAs have begun, behind k_q4_write)
 };
 int dc_launch_q4_rows(dc_ctx* ctx, const dc_q4_call& c);
 int dc_launch_q4_prompt(dc_ctx* ctx, const dc_q4_call& c);
+int dc_launch_q4_join(dc_ctx* ctx, const dc_q4_call& c);      // last: adds up the prompt tiles whose keys are split
