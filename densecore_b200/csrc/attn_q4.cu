@@ -17,6 +17,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "dc_common.cuh"
@@ -183,6 +184,7 @@ struct RowsParams {
     float scale;
     void* out;
     int early;      // dc_q4_call
+    int tiles;      // of the call: a replay on a plan with others would leave their rows out
     int* err;
 };
 
@@ -218,6 +220,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
     pdl_launch_dependents();
     dc_q4_item im = p.items[blockIdx.x];      // (within the plan's room even if a later plan has fewer: it need not wait for their number)
     const int n_items = p.head->n_items;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && p.head->n_tiles > 0 && p.tiles == 0) atomicExch(p.err, DC_ERR_REPLAY);
     uint32_t n_full = 0;      // pages that this warp has waited for
     for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
         if (it != (int)blockIdx.x) im = p.items[it];
@@ -589,7 +592,7 @@ template <int HD, typename TX>
 int launch_rows(dc_ctx* ctx, const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
     DC_TRY(dc_kernel_setup(ctx, (const void*)k_q4_rows<HD, TX>, (int)rows_smem<HD>(), "k_q4_rows"));
-    RowsParams p = {(const dc_q4_head*)z.plan, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.early, ctx->d_err};
+    RowsParams p = {(const dc_q4_head*)z.plan, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.early, z.n_tiles, ctx->d_err};
     return dc_launch(ctx, "k_q4_rows", k_q4_rows<HD, TX>, dim3(z.n_items, z.kv), dim3(RW * 32), rows_smem<HD>(), p);
 }
 
@@ -724,9 +727,47 @@ int check_call(dc_ctx* ctx, const dc_kv_cache* kv, int layer, const char* name) 
 int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held) {
     const dc_q4& z = *kv->q4;
     const WriteParams p = {(const dc_q4_head*)z.plan, (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), k, v, ldkv, z.kv, kv->planes[layer].arena, k_held, v_held};
-    const int units = (int)std::min<long long>((long long)z.T * z.kv, 1 << 30);
+    const int units = z.T * z.kv;
     if (z.dim == 128) return z.type == DC_TYPE_F32 ? launch_write<128, float>(ctx, p, units) : launch_write<128, __nv_bfloat16>(ctx, p, units);
     return z.type == DC_TYPE_F32 ? launch_write<64, float>(ctx, p, units) : launch_write<64, __nv_bfloat16>(ctx, p, units);
+}
+
+int create(dc_ctx* ctx, dc_kv_cache* kv, int n_layer, int n_head, int n_kv_head, int head_dim, int row_type, int max_blocks, int max_seqs, int max_blocks_per_seq) {
+    kv->q4->n_layer = n_layer, kv->q4->heads = n_head, kv->q4->kv = n_kv_head, kv->q4->dim = head_dim, kv->q4->type = row_type;
+    return dc_kv_init_planes(ctx, kv, std::vector<size_t>(n_layer, (size_t)n_kv_head * 18 * head_dim / DC_KV_BLOCK), 0, max_blocks, max_seqs, max_blocks_per_seq);
+}
+
+// dc_b200_kv_batch behind its first checks; throws std::bad_alloc.
+int begin_step(dc_ctx* ctx, dc_kv_cache* kv, int n_entries, const int32_t* seqs, const int32_t* pos0, const int32_t* counts) {
+    std::vector<dc_q4_entry> es;
+    std::vector<char> seen(kv->max_seqs, 0);
+    long long T = 0, prompt_tiles = 0;      // (the latter at most: grid.y of k_q4_prompt)
+    for (int i = 0; i < n_entries; ++i) {
+        const int s = seqs[i];
+        if (s < 0 || s >= kv->max_seqs || !kv->seqs[s].used) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d is not allocated", s);
+        if (seen[s]) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d is named twice", s);
+        seen[s] = 1;
+        if (counts[i] < 0 || pos0[i] < 0 || pos0[i] > kv->seqs[s].len)
+            return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d holds %d tokens, asked are %d from position %d on", s, kv->seqs[s].len, counts[i], pos0[i]);
+        if ((long long)pos0[i] + counts[i] > (long long)kv->max_blocks_per_seq * DC_KV_BLOCK)
+            return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: sequence %d needs %lld positions, its table holds %d pages", s, (long long)pos0[i] + counts[i], kv->max_blocks_per_seq);
+        if (counts[i]) es.push_back({s, pos0[i], counts[i], (int)T});
+        T += counts[i];
+        prompt_tiles += ((long long)counts[i] * (kv->q4->heads / kv->q4->kv) + 255) / 256;
+        if (prompt_tiles > 65535 || T * kv->q4->heads > (1 << 24)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: more than 2^24 new rows of queries or 65535 tiles of 256 at once");
+    }
+    const int need = blocks_needed(kv, es), there = dc_kv_available_blocks(kv);
+    if (need > there) return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: out of blocks (%d free, %d needed)", there, need);
+    kv->q4->planned = false;
+    for (const dc_q4_entry& e : es) {
+        kv->seqs[e.seq].len = e.pos0;      // rows from there on are written anew (what others share is copied first)
+        DC_TRY(dc_kv_seq_reserve(kv, e.seq, e.pos0 + e.count));
+        kv->seqs[e.seq].len = e.pos0 + e.count;
+    }
+    DC_TRY(make_plan(ctx, kv, es, (int)T));
+    kv->q4->edits = kv->edits;
+    kv->q4->planned = true;
+    return DC_B200_OK;
 }
 
 }  // namespace
@@ -744,18 +785,22 @@ int dc_b200_kv_create_q4(dc_ctx* ctx, int n_layer, int n_head, int n_kv_head, in
     if (n_head > (1 << 20) || (long long)max_blocks_per_seq * DC_KV_BLOCK > (1 << 30) || (long long)max_seqs * max_blocks_per_seq > (1LL << 31) - 1)
         return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_create_q4: %d sequences of %d pages, %d heads", max_seqs, max_blocks_per_seq, n_head);
     cudaSetDevice(ctx->device);
-    dc_kv_cache* kv = new dc_kv_cache();
-    kv->q4 = new dc_q4();
-    kv->q4->n_layer = n_layer, kv->q4->heads = n_head, kv->q4->kv = n_kv_head, kv->q4->dim = head_dim, kv->q4->type = row_type;
-    const size_t row = (size_t)n_kv_head * 18 * head_dim / DC_KV_BLOCK;
-    const int st = dc_kv_init_planes(ctx, kv, std::vector<size_t>(n_layer, row), 0, max_blocks, max_seqs, max_blocks_per_seq);
-    if (st != DC_B200_OK) {
+    dc_kv_cache* kv = nullptr;
+    int st;
+    try {
+        kv = new dc_kv_cache();
+        kv->q4 = new dc_q4();
+        st = create(ctx, kv, n_layer, n_head, n_kv_head, head_dim, row_type, max_blocks, max_seqs, max_blocks_per_seq);
+    } catch (const std::bad_alloc&) {
+        st = dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_create_q4: out of host memory");
+    }
+    if (st != DC_B200_OK && kv) {
         dc_kv_release(kv);
         delete kv;
-        return st;
+        kv = nullptr;
     }
     *out = kv;
-    return DC_B200_OK;
+    return st;
 }
 
 int dc_b200_kv_batch(dc_kv_cache* kv, int n_entries, const int32_t* seqs, const int32_t* pos0, const int32_t* counts) {
@@ -765,35 +810,11 @@ int dc_b200_kv_batch(dc_kv_cache* kv, int n_entries, const int32_t* seqs, const 
     if (n_entries < 0 || (n_entries && (!seqs || !pos0 || !counts))) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: bad argument (%d entries)", n_entries);
     cudaSetDevice(ctx->device);
     if (capturing(ctx)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: not within a stream capture");
-    std::vector<dc_q4_entry> es;
-    std::vector<char> seen(kv->max_seqs, 0);
-    long long T = 0;
-    const int G = kv->q4->heads / kv->q4->kv;
-    for (int i = 0; i < n_entries; ++i) {
-        const int s = seqs[i];
-        if (s < 0 || s >= kv->max_seqs || !kv->seqs[s].used) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d is not allocated", s);
-        if (seen[s]) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d is named twice", s);
-        seen[s] = 1;
-        if (counts[i] < 0 || pos0[i] < 0 || pos0[i] > kv->seqs[s].len)
-            return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d holds %d tokens, asked are %d from position %d on", s, kv->seqs[s].len, counts[i], pos0[i]);
-        if ((long long)pos0[i] + counts[i] > (long long)kv->max_blocks_per_seq * DC_KV_BLOCK)
-            return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: sequence %d needs %lld positions, its table holds %d pages", s, (long long)pos0[i] + counts[i], kv->max_blocks_per_seq);
-        if (counts[i]) es.push_back({s, pos0[i], counts[i], (int)T});
-        T += counts[i];
-        if (T * G > (1 << 24)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: too many new tokens at once");
+    try {
+        return begin_step(ctx, kv, n_entries, seqs, pos0, counts);
+    } catch (const std::bad_alloc&) {
+        return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: out of host memory");
     }
-    const int need = blocks_needed(kv, es), there = dc_kv_available_blocks(kv);
-    if (need > there) return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: out of blocks (%d free, %d needed)", there, need);
-    kv->q4->planned = false;
-    for (const dc_q4_entry& e : es) {
-        kv->seqs[e.seq].len = e.pos0;      // rows from there on are written anew (what others share is copied first)
-        DC_TRY(dc_kv_seq_reserve(kv, e.seq, e.pos0 + e.count));
-        kv->seqs[e.seq].len = e.pos0 + e.count;
-    }
-    DC_TRY(make_plan(ctx, kv, es, (int)T));
-    kv->q4->edits = kv->edits;
-    kv->q4->planned = true;
-    return DC_B200_OK;
 }
 
 int dc_b200_kv_q4_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k_dev, const void* v_dev, int ld_kv, float* k_held_dev, float* v_held_dev) {
@@ -816,6 +837,7 @@ int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const voi
     if (z.T == 0) return DC_B200_OK;
     if (!q_dev || !out_dev || (!k_dev != !v_dev) || ld_q < z.heads * z.dim || ld_out < z.heads * z.dim || ld_kv < z.kv * z.dim || (!k_dev && (k_held_dev || v_held_dev)))
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: bad argument (row strides %d, %d, %d)", ld_q, ld_kv, ld_out);
+    if (z.n_tiles && capturing(ctx)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "flash_attn_q4_dev: prompt-sized portions cannot be captured (their number of CTAs goes by the positions)");
     if (!isfinite(scale)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: scale is not finite");
     cudaSetDevice(ctx->device);
     if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev));
@@ -857,7 +879,12 @@ int dc_b200_kv_q4_read_block(dc_kv_cache* kv, int layer, int block, float* k_hos
     if (!kv || !kv->q4 || layer < 0 || layer >= kv->q4->n_layer || block < 0 || block >= kv->max_blocks) return DC_B200_INVALID_ARGUMENT;
     cudaSetDevice(kv->ctx->device);
     const int n_kv = kv->q4->kv, HD = kv->q4->dim, GR = HD / 64, rec = 18 * HD;
-    std::vector<uint8_t> page((size_t)n_kv * rec);
+    std::vector<uint8_t> page;
+    try {
+        page.resize((size_t)n_kv * rec);
+    } catch (const std::bad_alloc&) {
+        return dc_fail(kv->ctx, DC_B200_OUT_OF_MEMORY, "kv_q4_read_block: out of host memory");
+    }
     cudaError_t e = cudaStreamSynchronize(kv->ctx->stream);
     if (e == cudaSuccess) e = cudaMemcpy(page.data(), kv->planes[layer].arena + page.size() * block, page.size(), cudaMemcpyDeviceToHost);
     DC_TRY(dc_check_cuda(kv->ctx, e, "kv_q4_read_block"));

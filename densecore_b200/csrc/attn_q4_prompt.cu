@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                 tc_fence_after();
                 const int k0 = (first_tile + t) * QP_KEYS;
                 const bool masked = k0 + QP_KEYS - 1 > all_see;
-                int x[2][16];      // 32 scores at a time, once for their largest and once for the weights: all 64 would not stay in registers
+                int x[2][16] = {};      // 32 scores at a time, once for their largest and once for the weights: all 64 would not stay in registers
                 auto s = [&](int i) -> float { return __int_as_float(x[i >> 4][i & 15]); };
                 auto load = [&](int h) {
                     tmem_ld16(t_s + 32 * h, x[0]);

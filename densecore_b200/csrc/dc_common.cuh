@@ -29,6 +29,7 @@
 // no kernel can hang the GPU.
 #define DC_WAIT_LIMIT (1u << 22)
 #define DC_ERR_MBAR_TIMEOUT 1
+#define DC_ERR_REPLAY 64   // a captured step met a plan that it does not serve
 
 namespace dc {
 

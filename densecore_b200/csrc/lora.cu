@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "dc_common.cuh"
@@ -345,7 +346,12 @@ int grow(dc_ctx* ctx, dc_lora* l, int64_t rows) {
     float* fresh = nullptr;
     const int64_t want = std::max<int64_t>(rows + rows / 2, 64);
     DC_TRY(dc_check_cuda(ctx, cudaMalloc(&fresh, (size_t)want * l->Rp * 4), "lora workspace"));
-    if (l->h) l->retired.push_back(l->h);
+    try {
+        if (l->h) l->retired.push_back(l->h);
+    } catch (const std::bad_alloc&) {
+        cudaFree(fresh);
+        return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "lora workspace: out of host memory");
+    }
     l->h = fresh, l->h_rows = want;
     return DC_B200_OK;
 }
@@ -367,7 +373,8 @@ int dc_b200_lora_create(dc_ctx* ctx, int64_t K, int64_t N, int max_adapters, int
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_create: bad shape (%lld x %lld, %d adapters of rank %d)", (long long)K, (long long)N, max_adapters, max_rank);
     if (type != DC_TYPE_BF16 && type != DC_TYPE_F16) return dc_fail(ctx, DC_B200_UNSUPPORTED, "lora_create: matrices of type %d (BF16 and F16 are supported)", type);
     cudaSetDevice(ctx->device);
-    dc_lora* l = new dc_lora();
+    dc_lora* l = new (std::nothrow) dc_lora();
+    if (!l) return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "lora_create: out of host memory");
     l->ctx = ctx, l->K = K, l->N = N, l->Kp = (K + 15) / 16 * 16, l->Np = (N + 7) / 8 * 8;
     l->slots = max_adapters, l->max_rank = max_rank, l->Rp = (max_rank + 15) / 16 * 16, l->type = type;
     cudaError_t e = cudaMalloc(&l->a, (size_t)max_adapters * l->Rp * l->Kp * 2);

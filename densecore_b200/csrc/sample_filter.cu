@@ -100,7 +100,7 @@ struct Sampler {
     Shared* sh;
     int rank, n_cta, warp, lane, base;      // base: token index of xs[0]
     Weigher w;
-    float to_bin, top;      // top: the largest of this thread's tokens as they were read
+    float to_bin;
     u64 best;
 
     __device__ Sampler(const SampleParams& p_) : p(p_) {}
@@ -796,7 +796,6 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
 #pragma unroll 4
             for (int i = s.lane; i < p.seg; i += 32) x[i] = (TX)take(at0 + i < p.V ? (float)src[at0 + i] : -INFINITY, i);
         }
-        s.top = top;
         if (top > -INFINITY) best = token_key(top, top_at);
     }
     // ---- the largest token of each of 256 groups of threads, in all CTAs

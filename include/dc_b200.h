@@ -238,8 +238,10 @@ DC_B200_API int dc_b200_kv_create_q4(dc_ctx* ctx, int n_layer, int n_head, int n
  * shared ones about to be written), sets the lengths and uploads the step's plan, which all later calls of the cache
  * take: once per step, then one call per layer.  Refused without effect if blocks do not suffice; not allowed within a
  * stream capture.  A call of dc_b200_kv_seq_free / _fork / _reserve / _prefix_* ends the step.  The calls below may
- * be captured into a graph; a replay works on the newest plan at that time if its step needs no more plan memory than
- * any before the capture (otherwise it does nothing), and is subject to the same rules as a call. */
+ * be captured into a graph while no entry is prompt-sized (of BF16 rows, 64 or more new tokens times query heads of a
+ * key head).  A replay works on the newest plan at that time, whatever its entries and positions, if that needs no more plan memory than
+ * any before the capture (otherwise it does nothing), and is subject to the same rules as a call; on a plan with
+ * prompt-sized entries it leaves their rows out, which the next dc_b200_synchronize reports. */
 DC_B200_API int dc_b200_kv_batch(dc_kv_cache* kv, int n_entries, const int32_t* seqs, const int32_t* pos0, const int32_t* counts);
 /* Writes the step's rows into one layer.  k_dev, v_dev: [T][n_kv_head][head_dim] rows ld_kv elements apart (0: dense),
  * T the step's new tokens, entry after entry.  k_held_dev, v_held_dev (may be NULL): f32 [T][n_kv_head][head_dim], the
@@ -296,7 +298,7 @@ DC_B200_API int dc_b200_softmax(dc_ctx* ctx, const float* logits_host, int rows,
  * weight; a row without any weight gives token -1.  Weights are whole numbers of 2^-44, so that results do not
  * depend on the order of sums.  logits_dev: [rows][vocab], rows ld elements apart (0: dense), type DC_GGML_TYPE_F32 or
  * DC_GGML_TYPE_BF16, at most 389120 tokens a row.  temperature, top_k, top_p, min_p: [rows], each may be NULL (1, all, all, none).  uniforms_dev:
- * [rows] in [0, 1).  Results: tokens_dev [rows]; p_dev [rows] (may be NULL), the token's probability among the kept; dist_dev
+ * [rows] in [0, 1) (what lies outside is taken as the nearest within).  Results: tokens_dev [rows]; p_dev [rows] (may be NULL), the token's probability among the kept; dist_dev
  * [rows][vocab] f32 (may be NULL), the distribution drawn from, as a later dc_b200_verify_accept_dev (mode 1) needs it.  Only enqueues. */
 DC_B200_API int dc_b200_sample_rows_dev(dc_ctx* ctx, const void* logits_dev, int type, int rows, int vocab, int64_t ld, const float* temperature_dev,
                                         const int32_t* top_k_dev, const float* top_p_dev, const float* min_p_dev, const float* uniforms_dev,
@@ -318,7 +320,8 @@ DC_B200_API int dc_b200_lora_set(dc_lora* l, int slot, int rank, const void* a_h
 DC_B200_API int dc_b200_lora_set_dev(dc_lora* l, int slot, int rank, const void* a_dev, const void* b_dev, float scale);
 /* y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T with a = ids_dev[t]; a row whose id names no filled slot gives base[t].  x [M][K], base and y
  * [M][N] f32, rows ld_* elements apart (0: dense).  base_dev NULL: y_dev holds it; base and y are the same rows or do not overlap, x and y
- * do not overlap.  Sums and the rank-sized rows between the two products are f32, each row's result depends on its own adapter alone.  Only enqueues; the set's workspace
+ * do not overlap.  Sums and the rank-sized rows between the two products are f32, each row's result depends on its own x and adapter alone
+ * (infinities in them may come out as NaN).  Only enqueues; the set's workspace
  * grows with M (a call that needs more than any before cannot be captured), and calls on one set must not overlap in time. */
 DC_B200_API int dc_b200_lora_add_dev(dc_ctx* ctx, dc_lora* l, const float* x_dev, int64_t ld_x, int M, const int32_t* ids_dev, const float* base_dev,
                                      int64_t ld_base, float* y_dev, int64_t ld_y);

@@ -447,6 +447,42 @@ def test_a_captured_step_replays_on_the_newest_plan(ctx):
     del graph
 
 
+def test_prompt_sized_portions_are_not_captured(ctx):
+    rng = np.random.default_rng(33)
+    m = Mirror(ctx, "bf16", 8, 2, 128, 2, 40)
+    a = m.cache.seq_alloc()
+    m.step(rng, [a], [0], [100])
+    stream = torch.cuda.ExternalStream(dc._lib.lib().dc_b200_stream(ctx.handle))
+    q, k, v = (torch.zeros(40, h, 128, device=GPU, dtype=torch.bfloat16) for h in (8, 2, 2))
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    call = lambda: m.cache.attend_dev(0, q.data_ptr(), k.data_ptr(), v.data_ptr(), 1.0, out.data_ptr())
+    m.cache.batch([a], [100], [16])          # 64 rows
+    ctx.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(dc.DcError) as e:
+            call()
+        assert e.value.status == -7
+    m.cache.batch([a], [100], [15])          # 60 rows
+    call()
+    ctx.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+    m.cache.batch([a], [100], [40])          # a replay on a step that it does not serve is reported
+    with torch.cuda.stream(stream):
+        graph.replay()
+    with pytest.raises(dc.DcError) as e:
+        ctx.synchronize()
+    assert e.value.status == -6
+    m.cache.batch([a], [100], [3])
+    with torch.cuda.stream(stream):
+        graph.replay()
+    ctx.synchronize()
+    del graph
+
+
 def test_refusals(ctx):
     rng = np.random.default_rng(18)
     for bad in (dict(head_dim=96), dict(n_head=3), dict(dtype="f16"), dict(n_layer=0), dict(max_blocks=0)):
