@@ -741,7 +741,7 @@ int create(dc_ctx* ctx, dc_kv_cache* kv, int n_layer, int n_head, int n_kv_head,
 int begin_step(dc_ctx* ctx, dc_kv_cache* kv, int n_entries, const int32_t* seqs, const int32_t* pos0, const int32_t* counts) {
     std::vector<dc_q4_entry> es;
     std::vector<char> seen(kv->max_seqs, 0);
-    long long T = 0, prompt_tiles = 0;      // (the latter at most: grid.y of k_q4_prompt)
+    long long T = 0;
     for (int i = 0; i < n_entries; ++i) {
         const int s = seqs[i];
         if (s < 0 || s >= kv->max_seqs || !kv->seqs[s].used) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_batch: sequence %d is not allocated", s);
@@ -753,8 +753,7 @@ int begin_step(dc_ctx* ctx, dc_kv_cache* kv, int n_entries, const int32_t* seqs,
             return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: sequence %d needs %lld positions, its table holds %d pages", s, (long long)pos0[i] + counts[i], kv->max_blocks_per_seq);
         if (counts[i]) es.push_back({s, pos0[i], counts[i], (int)T});
         T += counts[i];
-        prompt_tiles += ((long long)counts[i] * (kv->q4->heads / kv->q4->kv) + 255) / 256;
-        if (prompt_tiles > 65535 || T * kv->q4->heads > (1 << 24)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: more than 2^24 new rows of queries or 65535 tiles of 256 at once");
+        if (T * kv->q4->heads > (1 << 30)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "kv_batch: more than 2^30 new rows of queries at once");
     }
     const int need = blocks_needed(kv, es), there = dc_kv_available_blocks(kv);
     if (need > there) return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: out of blocks (%d free, %d needed)", there, need);

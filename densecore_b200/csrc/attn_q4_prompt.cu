@@ -95,10 +95,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
     __shared__ int s_nan[2];
     __shared__ float s_pow[2 * QP_ROWS];      // 2^e of a row
     pdl_wait();
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.x, G = p.heads / p.n_kv;
-    const dc_q4_tile* tp = p.tiles + blockIdx.y;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.x % p.n_kv, tile = blockIdx.x / p.n_kv, G = p.heads / p.n_kv;
+    const dc_q4_tile* tp = p.tiles + tile;
     const dc_q4_tile tl = *tp;
-    if ((int)blockIdx.y >= p.head->n_tiles) return;      // (a replay on a smaller step)
     const int rows = min(2 * QP_ROWS, tl.count * G - tl.row0), sets = rows > QP_ROWS ? 2 : 1;
     const int last = tl.pos0 + (tl.row0 + rows - 1) / G, first_tile = tl.tile0, n_tiles = tl.tile1 - tl.tile0;
     const uint32_t sm = (smem_u32(smem) + 1023u) & ~1023u;
@@ -491,7 +490,6 @@ __global__ void __launch_bounds__(256) k_q4_join(const PromptParams p) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, G = p.heads / p.n_kv, kvh = blockIdx.y, r = blockIdx.z * 8 + (threadIdx.x >> 5);
-    if ((int)blockIdx.x >= p.head->n_joins) return;
     const dc_q4_tile tl = p.tiles[p.joins[blockIdx.x]];
     if (r >= tl.count * G - tl.row0) return;
     constexpr size_t ROW = HD + 4, PART = 2 * QP_ROWS * ROW;
@@ -545,7 +543,7 @@ PromptParams params(const dc_q4_call& c) {
 template <int HD>
 int launch(dc_ctx* ctx, const dc_q4_call& c) {
     DC_TRY(dc_kernel_setup_unspilled(ctx, (const void*)k_q4_prompt<HD>, (int)Lay<HD>::SMEM, "k_q4_prompt"));
-    return dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(c.kv->q4->kv, c.kv->q4->n_tiles), dim3(QP_THREADS), Lay<HD>::SMEM, params(c), ctx->d_err);
+    return dc_launch(ctx, "k_q4_prompt", k_q4_prompt<HD>, dim3(c.kv->q4->kv * c.kv->q4->n_tiles), dim3(QP_THREADS), Lay<HD>::SMEM, params(c), ctx->d_err);
 }
 
 }  // namespace

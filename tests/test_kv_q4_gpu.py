@@ -447,6 +447,32 @@ def test_a_captured_step_replays_on_the_newest_plan(ctx):
     del graph
 
 
+def test_a_million_new_tokens_at_once(ctx):
+    """Caches filled in one step: more tiles than a grid's second dimension holds."""
+    n, each = 64, 17000
+    m = Mirror(ctx, "bf16", 16, 1, 64, n, -(-each // 16))
+    seqs = [m.cache.seq_alloc() for _ in range(n)]
+    torch.manual_seed(5)
+    q, k, v = (torch.randn(n * each, h, 64, device=GPU, dtype=torch.bfloat16) for h in (16, 1, 1))
+    kh, vh = (torch.empty(n * each, 1, 64, device=GPU) for _ in "kv")
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    m.cache.batch(seqs, [0] * n, [each] * n)
+    m.cache.attend_dev(0, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0.125, out.data_ptr(), k_held=kh.data_ptr(), v_held=vh.data_ptr())
+    ctx.synchronize()
+    for i in (0, n // 2, n - 1):
+        rows = slice(i * each, (i + 1) * each)
+        new = [bf16(x[rows].float().cpu().numpy()) for x in (k, v)]
+        m.k[0][seqs[i]], m.v[0][seqs[i]] = (held(x) for x in new)
+        assert np.array_equal(kh[rows].cpu().numpy(), m.k[0][seqs[i]]) and np.array_equal(vh[rows].cpu().numpy(), m.v[0][seqs[i]])
+        for p in (0, each // 2, each - 4):
+            at = slice(i * each + p, i * each + p + 4)
+            y, store = m.k[0][seqs[i]], m.v[0][seqs[i]]
+            m.k[0][seqs[i]], m.v[0][seqs[i]] = y[:p + 4], store[:p + 4]
+            m.compare(out[at].float().cpu().numpy(), q[at].float().cpu().numpy(), seqs[i], p, 0.125)
+            m.k[0][seqs[i]], m.v[0][seqs[i]] = y, store
+
+
 def test_prompt_sized_portions_are_not_captured(ctx):
     rng = np.random.default_rng(33)
     m = Mirror(ctx, "bf16", 8, 2, 128, 2, 40)
