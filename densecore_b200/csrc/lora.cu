@@ -316,8 +316,10 @@ __global__ void __launch_bounds__(256) k_lora_set(const uint16_t* __restrict__ a
     if (blockIdx.x == 0 && threadIdx.x == 0) *rank_at = rank, *scale_at = scale;
 }
 
-// Rows from which tiles are taken: they read a matrix once for 16 rows; below, one warp a rank and one thread a column have shorter chains of loads.
-constexpr int LORA_TILE_ROWS = 97;
+// Rows from which tiles are taken: they read a matrix once for 16 rows of one adapter; below, one warp a rank and one thread a column have shorter chains of loads, and do
+// not mind rows of many adapters, each of which costs a tile a pass.  K 2048, N 6144, by rows and tiles, in us: 100 rows of rank 16, four adapters mixed 11 and 29;
+// 200 rows 16 and 38; rank 64: 24 and 35, 41 and 50; 400 rows, each adapter's in a run: 29 and 21, rank 64 60 and 23.
+int tile_rows(int Rp) { return std::max(97, std::min(257, 4096 / Rp)); }
 constexpr int LORA_PARTS = 4;      // of k, at most
 
 int parts_of(const dc_ctx* ctx, int M, int64_t Kp) {      // until the CTAs fill the SMs three times, a warp keeping two steps
@@ -329,7 +331,7 @@ int parts_of(const dc_ctx* ctx, int M, int64_t Kp) {      // until the CTAs fill
 template <bool BF>
 int launch_add(dc_ctx* ctx, const LoraParams& p, int max_rank) {
     const int vx = ((uintptr_t)p.x & 15) == 0 && p.ldx % 4 == 0, vy = ((uintptr_t)p.base & 7) == 0 && ((uintptr_t)p.y & 7) == 0 && p.ldb % 2 == 0 && p.ldy % 2 == 0;
-    if (p.M < LORA_TILE_ROWS) {
+    if (p.M < tile_rows(p.Rp)) {
         DC_TRY(dc_launch(ctx, "k_lora_down", k_lora_down<BF>, dim3(p.M, (max_rank + 15) / 16 * 2), dim3(256), 0, p, vx));
         return dc_launch(ctx, "k_lora_up_rows", k_lora_up_rows<BF>, dim3((unsigned)((p.N + 127) / 128), p.M), dim3(128), 0, p);
     }
@@ -432,13 +434,13 @@ int dc_b200_lora_add_dev(dc_ctx* ctx, dc_lora* l, const float* x_dev, int64_t ld
     if (ld_x == 0) ld_x = l->K;
     if (ld_base == 0) ld_base = l->N;
     if (ld_y == 0) ld_y = l->N;
-    if (M < 0 || M > (1 << 20) || ld_x < l->K || ld_base < l->N || ld_y < l->N)
+    if (M < 0 || M > 65535 * 16 || ld_x < l->K || ld_base < l->N || ld_y < l->N)
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: bad argument (%d rows, strides %lld, %lld, %lld)", M, (long long)ld_x, (long long)ld_base, (long long)ld_y);
     if (M == 0) return DC_B200_OK;
     if (!x_dev || !ids_dev || !y_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: null buffer");
     if (!base_dev) base_dev = y_dev, ld_base = ld_y;
     cudaSetDevice(ctx->device);
-    DC_TRY(grow(ctx, l, M < LORA_TILE_ROWS ? M : (int64_t)M * parts_of(ctx, M, l->Kp)));
+    DC_TRY(grow(ctx, l, M < tile_rows(l->Rp) ? M : (int64_t)M * parts_of(ctx, M, l->Kp)));
     const LoraParams p = {l->a, l->b, l->rank, l->scale, l->slots, l->Rp, l->K, l->N, l->Kp, l->Np, x_dev, ld_x, M, ids_dev, l->h, base_dev, y_dev, ld_base, ld_y};
     return l->type == DC_TYPE_BF16 ? launch_add<true>(ctx, p, l->max_rank) : launch_add<false>(ctx, p, l->max_rank);
 }

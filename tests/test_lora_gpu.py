@@ -75,6 +75,14 @@ def test_shapes(ctx, dtype, K, N, M):
         a.check(*rows(M, K, N, 5, M, order))
 
 
+@pytest.mark.parametrize("rank", [16, 32, 48])
+@pytest.mark.parametrize("M", [96, 97, 127, 128, 255, 256, 257])
+def test_where_tiles_begin(ctx, rank, M):
+    a = Adapters(ctx, 320, 264, [rank, 1, rank // 2], "f16", seed=M)
+    for order in ("any", "runs"):
+        a.check(*rows(M, 320, 264, 3, M, order))
+
+
 @pytest.mark.parametrize("M", [5, 300])
 @pytest.mark.parametrize("rank", [1, 15, 16, 17, 65, 128, 200])
 def test_ranks(ctx, rank, M):
