@@ -407,10 +407,10 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
                     }
                     mx = fmaxf(mx, sc[a][b] + fmaxf(lg2(most), -24.0f));
                 }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // (the reference follows once it is 2^6 behind: weights up to 64 are as exact, and the answers' factors are rare)
+            // (the reference follows once it is 2^6 behind: weights up to 64 are as exact, and the row's maximum and the answers' factors are rare)
             if (__any_sync(0xffffffffu, mx > m_run + 6.0f)) {
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float m_new = fmaxf(m_run, mx), corr = ex2(m_run - m_new);
                 m_run = m_new;
                 l *= corr;
