@@ -5,7 +5,7 @@
 //
 // Tiles: rows x and h are f32 and enter the tensor cores as two terms of 11 bits (tf32, 22 bits together; products of m16n8k8 with f32 sums), matrices are bf16 or
 // fp16, which tf32 holds exactly.  A tile whose rows have several adapters takes one after the other: each
-// adapter's matrices are read once per tile, whatever the order of rows.
+// adapter's matrices are read once per tile, whatever the order of rows; up to 256 rows are put in their adapters' order first.
 #include <math.h>
 
 #include <algorithm>
@@ -33,6 +33,7 @@ struct dc_lora {
     float* scale = nullptr;
     float* h = nullptr;                       // workspace [parts][rows][Rp]
     int64_t h_rows = 0;
+    int32_t* order = nullptr;                 // workspace of k_lora_order
     std::vector<float*> retired;              // outgrown workspaces, which captured calls may still name
 };
 
@@ -52,6 +53,7 @@ struct LoraParams {
     const float* base;
     float* y;
     int64_t ldb, ldy;
+    const int32_t* order;      // rows by adapter (k_lora_order), or NULL: as they come
 };
 
 __device__ __forceinline__ int slot_of(const LoraParams& p, int row) {      // -1: none
@@ -59,6 +61,8 @@ __device__ __forceinline__ int slot_of(const LoraParams& p, int row) {      // -
     const int a = p.ids[row];
     return a >= 0 && a < p.slots && p.rank[a] > 0 ? a : -1;
 }
+// Tiles: place i of all rows has row row_at(i); h is held by places
+__device__ __forceinline__ int row_at(const LoraParams& p, int i) { return i < p.M ? (p.order ? p.order[i] : i) : p.M; }
 template <bool BF>
 __device__ __forceinline__ float2 two(uint32_t w) {
     if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
@@ -154,6 +158,27 @@ __global__ void __launch_bounds__(128) k_lora_up_rows(const LoraParams p) {
     p.y[(size_t)row * p.ldy + n] = sum + add;
 }
 
+// Rows by adapter, those without one last, else as they come: a row's place is the number of rows before it.  One CTA, some 5 us with its launch.
+// A tile of several adapters takes a pass for each: 200 mixed rows of rank 64 40 us as they come, 27 in order; runs of prompts, where nothing is gained, 22 and 28 at 384 rows.
+constexpr int LORA_SORTED = 256;
+__global__ void __launch_bounds__(LORA_SORTED) k_lora_order(const LoraParams p, int32_t* order) {
+    __shared__ __align__(16) int slot[LORA_SORTED];
+    const int i = threadIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int a = slot_of(p, i), mine = a < 0 ? 0x7fffffff : a;
+    slot[i] = mine;      // (places from M on count for nobody: none, and behind all)
+    __syncthreads();
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < (p.M + 3) / 4; ++j) {
+        const int4 s = *reinterpret_cast<const int4*>(slot + 4 * j);
+        place += (s.x < mine || (s.x == mine && 4 * j < i)) + (s.y < mine || (s.y == mine && 4 * j + 1 < i)) + (s.z < mine || (s.z == mine && 4 * j + 2 < i)) +
+                 (s.w < mine || (s.w == mine && 4 * j + 3 < i));
+    }
+    if (i < p.M) order[place] = i;
+}
+
 // Adapters of a tile's rows, one after the other: `f(slot, mask)` with the rows (bits) that have it.
 template <typename F>
 __device__ __forceinline__ void each_adapter(int mine, uint32_t rows, F f) {      // mine: lane i's row's slot; rows: bits to look at
@@ -177,7 +202,8 @@ __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, i
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.x * 16, r0 = blockIdx.y * DT_R;
     pdl_wait();
     pdl_launch_dependents();
-    const int mine = slot_of(p, row0 + (lane & 15));
+    const int mine = slot_of(p, row_at(p, row0 + (lane & 15)));
+    const int row_u = row_at(p, row0 + h), row_v = row_at(p, row0 + h + 8);
     const int64_t per = (p.Kp / 16 + gridDim.z - 1) / gridDim.z * 16, k0 = blockIdx.z * per, k1 = min(p.Kp, k0 + per);
     each_adapter(mine, 0xFFFFu, [&](int a, uint32_t mask) {      // (the same ones in all warps)
         const int tiles = min(DT_R / 8, ((p.rank[a] + 15) / 16 * 16 - r0) / 8);
@@ -185,7 +211,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, i
         const float scale = p.scale[a];
         float sum[DT_R / 8][4] = {};
         const bool u = mask >> h & 1, v = mask >> (h + 8) & 1;
-        const float *xu = p.x + (size_t)(row0 + (u ? h : 0)) * p.ldx, *xv = p.x + (size_t)(row0 + (v ? h + 8 : 0)) * p.ldx;
+        const float *xu = p.x + (size_t)(u ? row_u : 0) * p.ldx, *xv = p.x + (size_t)(v ? row_v : 0) * p.ldx;
         const uint16_t* w = p.a + ((size_t)a * p.Rp + r0 + h) * p.Kp + 4 * t;
 #pragma unroll 2
         for (int64_t k = k0 + 16 * warp; k < k1; k += 128) {
@@ -227,10 +253,11 @@ __global__ void __launch_bounds__(256, 3) k_lora_up(const LoraParams p, int vec,
     const int64_t n0 = ((int64_t)blockIdx.x * 8 + warp) * 8 * NP;
     pdl_wait();
     pdl_launch_dependents();
+    const int rows[2] = {row_at(p, row0 + h), row_at(p, row0 + h + 8)};
     float2 f[2][NP];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-        const int row = row0 + h + 8 * q;
+        const int row = rows[q];
         const float* from = p.base + (size_t)(row < p.M ? row : 0) * p.ldb;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
@@ -239,12 +266,12 @@ __global__ void __launch_bounds__(256, 3) k_lora_up(const LoraParams p, int vec,
             else f[q][i] = make_float2(n < p.N ? from[n] : 0.f, n + 1 < p.N ? from[n + 1] : 0.f);
         }
     }
-    const int mine = slot_of(p, row0 + (lane & 15));
+    const int mine = slot_of(p, row_at(p, row0 + (lane & 15)));
     auto store = [&](const float (&sum)[MT][NP][4], uint32_t mask) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             if (!(mask >> (h + 8 * q) & 1)) continue;
-            float* to = p.y + (size_t)(row0 + h + 8 * q) * p.ldy;
+            float* to = p.y + (size_t)rows[q] * p.ldy;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int64_t n = n0 + 8 * i + 2 * t;
@@ -318,10 +345,10 @@ __global__ void __launch_bounds__(256) k_lora_set(const uint16_t* __restrict__ a
     if (blockIdx.x == 0 && threadIdx.x == 0) *rank_at = rank, *scale_at = scale;
 }
 
-// Rows from which tiles are taken: they read a matrix once for 16 rows of one adapter; below, one warp a rank and one thread a column have shorter chains of loads, and do
-// not mind rows of many adapters, each of which costs a tile a pass.  K 2048, N 6144, by rows and tiles, in us: 100 rows of rank 16, four adapters mixed 11 and 29;
-// 200 rows 16 and 38; rank 64: 24 and 35, 41 and 50; 400 rows, each adapter's in a run: 29 and 21, rank 64 60 and 23.
-int tile_rows(int Rp) { return std::max(97, std::min(257, 4096 / Rp)); }
+// Rows from which tiles are taken: they read a matrix once for 16 rows of one adapter; below, one warp a rank and one thread a column have shorter chains of loads.
+// K 2048, N 6144, four adapters mixed, by rows and by tiles of rows in order, in us: 100 rows of rank 32 13 and 21, 256 22 and 25; 100 rows of rank 64 25 and 23, 256 49 and 28;
+// rank 128 42 and 27, 87 and 34.
+int tile_rows(int Rp) { return Rp <= 32 ? 257 : 97; }
 constexpr int LORA_PARTS = 4;      // of k, at most
 
 int parts_of(const dc_ctx* ctx, int M, int64_t Kp) {      // until the CTAs fill the SMs three times, a warp keeping two steps
@@ -331,13 +358,18 @@ int parts_of(const dc_ctx* ctx, int M, int64_t Kp) {      // until the CTAs fill
 }
 
 template <bool BF>
-int launch_add(dc_ctx* ctx, const LoraParams& p, int max_rank) {
+int launch_add(dc_ctx* ctx, LoraParams p, int max_rank, int32_t* order) {
     const int vx = ((uintptr_t)p.x & 15) == 0 && p.ldx % 4 == 0, vy = ((uintptr_t)p.base & 7) == 0 && ((uintptr_t)p.y & 7) == 0 && p.ldb % 2 == 0 && p.ldy % 2 == 0;
     if (p.M < tile_rows(p.Rp)) {
         DC_TRY(dc_launch(ctx, "k_lora_down", k_lora_down<BF>, dim3(p.M, (max_rank + 15) / 16 * 2), dim3(256), 0, p, vx));
         return dc_launch(ctx, "k_lora_up_rows", k_lora_up_rows<BF>, dim3((unsigned)((p.N + 127) / 128), p.M), dim3(128), 0, p);
     }
     const int parts = parts_of(ctx, p.M, p.Kp);
+    p.order = nullptr;
+    if (p.M <= LORA_SORTED) {      // (more rows than that are prompts' for the most part, which come in runs)
+        DC_TRY(dc_launch(ctx, "k_lora_order", k_lora_order, dim3(1), dim3(LORA_SORTED), 0, p, order));
+        p.order = order;
+    }
     DC_TRY(dc_launch(ctx, "k_lora_down_tile", k_lora_down_tile<BF>, dim3((p.M + 15) / 16, (p.Rp + DT_R - 1) / DT_R, parts), dim3(256), 0, p, vx));
     return dc_launch(ctx, "k_lora_up", k_lora_up<BF>, dim3((unsigned)((p.N + 255) / 256), (p.M + 15) / 16), dim3(256), 0, p, vy, parts);
 }
@@ -384,6 +416,7 @@ int dc_b200_lora_create(dc_ctx* ctx, int64_t K, int64_t N, int max_adapters, int
     cudaError_t e = cudaMalloc(&l->a, (size_t)max_adapters * l->Rp * l->Kp * 2);
     if (e == cudaSuccess) e = cudaMalloc(&l->b, (size_t)max_adapters * l->Np * l->Rp * 2);
     if (e == cudaSuccess) e = cudaMalloc(&l->rank, (size_t)max_adapters * 4);
+    if (e == cudaSuccess) e = cudaMalloc(&l->order, LORA_SORTED * 4);
     if (e == cudaSuccess) e = cudaMalloc(&l->scale, (size_t)max_adapters * 4);
     if (e == cudaSuccess) e = cudaMemsetAsync(l->rank, 0, (size_t)max_adapters * 4, ctx->stream);
     if (e != cudaSuccess) {
@@ -403,6 +436,7 @@ void dc_b200_lora_destroy(dc_lora* l) {
     cudaFree(l->a), cudaFree(l->b), cudaFree(l->rank), cudaFree(l->scale);
     if (l->h) cudaFree(l->h);
     for (float* h : l->retired) cudaFree(h);
+    cudaFree(l->order);
     delete l;
 }
 
@@ -443,8 +477,8 @@ int dc_b200_lora_add_dev(dc_ctx* ctx, dc_lora* l, const float* x_dev, int64_t ld
     if (!base_dev) base_dev = y_dev, ld_base = ld_y;
     cudaSetDevice(ctx->device);
     DC_TRY(grow(ctx, l, M < tile_rows(l->Rp) ? M : (int64_t)M * parts_of(ctx, M, l->Kp)));
-    const LoraParams p = {l->a, l->b, l->rank, l->scale, l->slots, l->Rp, l->K, l->N, l->Kp, l->Np, x_dev, ld_x, M, ids_dev, l->h, base_dev, y_dev, ld_base, ld_y};
-    return l->type == DC_TYPE_BF16 ? launch_add<true>(ctx, p, l->max_rank) : launch_add<false>(ctx, p, l->max_rank);
+    const LoraParams p = {l->a, l->b, l->rank, l->scale, l->slots, l->Rp, l->K, l->N, l->Kp, l->Np, x_dev, ld_x, M, ids_dev, l->h, base_dev, y_dev, ld_base, ld_y, nullptr};
+    return l->type == DC_TYPE_BF16 ? launch_add<true>(ctx, p, l->max_rank, l->order) : launch_add<false>(ctx, p, l->max_rank, l->order);
 }
 
 int dc_b200_mul_mat_lora_dev(dc_ctx* ctx, const dc_weight* w, dc_lora* l, const float* x_dev, int M, const int32_t* ids_dev, float* y_dev) {
