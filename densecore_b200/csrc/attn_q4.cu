@@ -761,12 +761,21 @@ int begin_step(dc_ctx* ctx, dc_kv_cache* kv, int n_entries, const int32_t* seqs,
     const int need = blocks_needed(kv, es), there = dc_kv_available_blocks(kv);
     if (need > there) return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "kv_batch: out of blocks (%d free, %d needed)", there, need);
     kv->q4->planned = false;
+    struct Lengths {      // as they were, should anything fail from here on (blocks reserved meanwhile stay with their sequences)
+        dc_kv_cache* kv;
+        std::vector<std::pair<int, int>> of;
+        ~Lengths() {
+            for (const auto& x : of) kv->seqs[x.first].len = x.second;
+        }
+    } before = {kv, {}};
+    for (const dc_q4_entry& e : es) before.of.push_back({e.seq, kv->seqs[e.seq].len});
     for (const dc_q4_entry& e : es) {
         kv->seqs[e.seq].len = e.pos0;      // rows from there on are written anew (what others share is copied first)
         DC_TRY(dc_kv_seq_reserve(kv, e.seq, e.pos0 + e.count));
         kv->seqs[e.seq].len = e.pos0 + e.count;
     }
     DC_TRY(make_plan(ctx, kv, es, (int)T));
+    before.of.clear();
     kv->q4->edits = kv->edits;
     kv->q4->planned = true;
     return DC_B200_OK;
