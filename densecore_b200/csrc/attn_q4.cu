@@ -727,6 +727,10 @@ int check_call(dc_ctx* ctx, const dc_kv_cache* kv, int layer, const char* name) 
     return DC_B200_OK;
 }
 
+int empty_step(dc_ctx* ctx, const char* name) {      // nothing to do; a capture of it would do nothing for later steps either
+    return capturing(ctx) ? dc_fail(ctx, DC_B200_UNSUPPORTED, "%s: a step without tokens cannot be captured", name) : DC_B200_OK;
+}
+
 int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held) {
     const dc_q4& z = *kv->q4;
     const WriteParams p = {(const dc_q4_head*)z.plan, (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), k, v, ldkv, z.kv, kv->planes[layer].arena, k_held, v_held};
@@ -832,7 +836,7 @@ int dc_b200_kv_q4_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void*
     DC_TRY(check_call(ctx, kv, layer, "kv_q4_write_dev"));
     const dc_q4& z = *kv->q4;
     if (ld_kv == 0) ld_kv = z.kv * z.dim;
-    if (z.T == 0) return DC_B200_OK;
+    if (z.T == 0) return empty_step(ctx, "kv_q4_write_dev");
     if (!k_dev || !v_dev || ld_kv < z.kv * z.dim) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_q4_write_dev: bad argument (row stride %d)", ld_kv);
     cudaSetDevice(ctx->device);
     return write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev);
@@ -845,7 +849,7 @@ int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const voi
     if (ld_q == 0) ld_q = z.heads * z.dim;
     if (ld_kv == 0) ld_kv = z.kv * z.dim;
     if (ld_out == 0) ld_out = z.heads * z.dim;
-    if (z.T == 0) return DC_B200_OK;
+    if (z.T == 0) return empty_step(ctx, "flash_attn_q4_dev");
     if (!q_dev || !out_dev || (!k_dev != !v_dev) || ld_q < z.heads * z.dim || ld_out < z.heads * z.dim || ld_kv < z.kv * z.dim || (!k_dev && (k_held_dev || v_held_dev)))
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: bad argument (row strides %d, %d, %d)", ld_q, ld_kv, ld_out);
     if (z.n_tiles && capturing(ctx)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "flash_attn_q4_dev: prompt-sized portions cannot be captured (their number of CTAs goes by the positions)");

@@ -238,7 +238,7 @@ DC_B200_API int dc_b200_kv_create_q4(dc_ctx* ctx, int n_layer, int n_head, int n
  * shared ones about to be written), sets the lengths and uploads the step's plan, which all later calls of the cache
  * take: once per step, then one call per layer.  Refused without effect if blocks do not suffice; not allowed within a
  * stream capture.  A call of dc_b200_kv_seq_free / _fork / _reserve / _prefix_* ends the step.  The calls below may
- * be captured into a graph while no entry is prompt-sized (of BF16 rows, 64 or more new tokens times query heads of a
+ * be captured into a graph while the step has tokens and no entry is prompt-sized (of BF16 rows, 64 or more new tokens times query heads of a
  * key head).  A replay works on the newest plan at that time, whatever its entries and positions, if that needs no more plan memory than
  * any before the capture (otherwise it does nothing), and is subject to the same rules as a call; on a plan with
  * prompt-sized entries it leaves their rows out, which the next dc_b200_synchronize reports. */
@@ -299,7 +299,8 @@ DC_B200_API int dc_b200_softmax(dc_ctx* ctx, const float* logits_host, int rows,
  * depend on the order of sums.  logits_dev: [rows][vocab], rows ld elements apart (0: dense), type DC_GGML_TYPE_F32 or
  * DC_GGML_TYPE_BF16, at most 389120 tokens a row.  temperature, top_k, top_p, min_p: [rows], each may be NULL (1, all, all, none).  uniforms_dev:
  * [rows] in [0, 1) (what lies outside is taken as the nearest within).  Results: tokens_dev [rows]; p_dev [rows] (may be NULL), the token's probability among the kept; dist_dev
- * [rows][vocab] f32 (may be NULL), the distribution drawn from, as a later dc_b200_verify_accept_dev (mode 1) needs it.  Only enqueues. */
+ * [rows][vocab] f32 (may be NULL), the distribution drawn from, as a later dc_b200_verify_accept_dev (mode 1) needs it; results do not overlap
+ * each other or the inputs.  Only enqueues. */
 DC_B200_API int dc_b200_sample_rows_dev(dc_ctx* ctx, const void* logits_dev, int type, int rows, int vocab, int64_t ld, const float* temperature_dev,
                                         const int32_t* top_k_dev, const float* top_p_dev, const float* min_p_dev, const float* uniforms_dev,
                                         int32_t* tokens_dev, float* p_dev, float* dist_dev);

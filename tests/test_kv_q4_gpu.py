@@ -447,6 +447,25 @@ def test_a_captured_step_replays_on_the_newest_plan(ctx):
     del graph
 
 
+def test_a_step_without_tokens_is_not_captured(ctx):
+    m = Mirror(ctx, "f32", 4, 2, 64, 2, 4)
+    a = m.cache.seq_alloc()
+    stream = torch.cuda.ExternalStream(dc._lib.lib().dc_b200_stream(ctx.handle))
+    x = torch.zeros(1, 4, 64, device=GPU)
+    torch.cuda.synchronize()
+    m.cache.batch([a], [0], [0])
+    m.cache.attend_dev(0, x.data_ptr(), x.data_ptr(), x.data_ptr(), 1.0, x.data_ptr())      # nothing to do
+    ctx.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for call in (lambda: m.cache.attend_dev(0, x.data_ptr(), x.data_ptr(), x.data_ptr(), 1.0, x.data_ptr()),
+                     lambda: m.cache.write_dev(0, x.data_ptr(), x.data_ptr())):
+            with pytest.raises(dc.DcError) as e:
+                call()
+            assert e.value.status == -7
+    del graph
+
+
 def test_a_million_new_tokens_at_once(ctx):
     """Caches filled in one step: more tiles than a grid's second dimension holds."""
     n, each = 64, 17000
