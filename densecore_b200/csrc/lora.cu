@@ -192,12 +192,12 @@ __device__ __forceinline__ void each_adapter(int mine, uint32_t rows, F f) {    
 }
 
 // A row's sums are stored by its own adapter's pass; the others' may leave anything there (zero times an infinite matrix).
-constexpr int DT_R = 64;      // ranks of a CTA of k_lora_down_tile
-
-// Many rows: a CTA per (16 rows, 64 ranks, part of k), its warps share out the part in steps of 16 and add up in the end; the parts are added by the next kernel.
-// Bound: latency of one part's loads and sums (17 to 20 us of that call), and tiles with the rows of two adapters, which take two passes.
-template <bool BF>
+// Many rows: a CTA per (16 rows, 8 NT ranks, part of k), its warps share out the part in steps of 16 and add up in the end; the parts are added by the next kernel.
+// Bound: latency of one part's loads and sums (17 us of 2011 rows, K 2048, rank 64), and tiles with the rows of two adapters, which take two passes.  Sixteen ranks leave registers for
+// eight steps' loads at once, 32 for four: 746 rows, K 7408, N 2656, rank 2 by 16 ranks 28 us, by 64 (two steps) 45; rank 64 by 32 ranks 44, by 64 54, by 16 50.
+template <bool BF, int NT>
 __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, int vec) {
+    constexpr int DT_R = 8 * NT;
     __shared__ float part[8][16][DT_R + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = lane >> 2, t = lane & 3, row0 = blockIdx.x * 16, r0 = blockIdx.y * DT_R;
     pdl_wait();
@@ -206,26 +206,26 @@ __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, i
     const int row_u = row_at(p, row0 + h), row_v = row_at(p, row0 + h + 8);
     const int64_t per = (p.Kp / 16 + gridDim.z - 1) / gridDim.z * 16, k0 = blockIdx.z * per, k1 = min(p.Kp, k0 + per);
     each_adapter(mine, 0xFFFFu, [&](int a, uint32_t mask) {      // (the same ones in all warps)
-        const int tiles = min(DT_R / 8, ((p.rank[a] + 15) / 16 * 16 - r0) / 8);
+        const int tiles = min(NT, ((p.rank[a] + 15) / 16 * 16 - r0) / 8);
         if (tiles <= 0) return;
         const float scale = p.scale[a];
-        float sum[DT_R / 8][4] = {};
+        float sum[NT][4] = {};
         const bool u = mask >> h & 1, v = mask >> (h + 8) & 1;
         const float *xu = p.x + (size_t)(u ? row_u : 0) * p.ldx, *xv = p.x + (size_t)(v ? row_v : 0) * p.ldx;
         const uint16_t* w = p.a + ((size_t)a * p.Rp + r0 + h) * p.Kp + 4 * t;
-#pragma unroll 2
+#pragma unroll (16 / NT)
         for (int64_t k = k0 + 16 * warp; k < k1; k += 128) {
-            uint2 c[DT_R / 8];
+            uint2 c[NT];
 #pragma unroll
-            for (int i = 0; i < DT_R / 8; ++i) c[i] = i < tiles ? __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Kp + k)) : make_uint2(0, 0);
+            for (int i = 0; i < NT; ++i) c[i] = i < tiles ? __ldg(reinterpret_cast<const uint2*>(w + (size_t)(8 * i) * p.Kp + k)) : make_uint2(0, 0);
             const Terms x(load_x4(xu, k + 4 * t, p.K, vec, u), load_x4(xv, k + 4 * t, p.K, vec, v));
 #pragma unroll
-            for (int i = 0; i < DT_R / 8; ++i)
+            for (int i = 0; i < NT; ++i)
                 if (i < tiles) x.times(sum[i], two<BF>(c[i].x), two<BF>(c[i].y));
         }
         __syncthreads();      // (the last adapter's sums have been read)
 #pragma unroll
-        for (int i = 0; i < DT_R / 8; ++i) {
+        for (int i = 0; i < NT; ++i) {
             part[warp][h][8 * i + 2 * t] = sum[i][0], part[warp][h][8 * i + 2 * t + 1] = sum[i][1];
             part[warp][h + 8][8 * i + 2 * t] = sum[i][2], part[warp][h + 8][8 * i + 2 * t + 1] = sum[i][3];
         }
@@ -349,11 +349,13 @@ __global__ void __launch_bounds__(256) k_lora_set(const uint16_t* __restrict__ a
 // K 2048, N 6144, four adapters mixed, by rows and by tiles of rows in order, in us: 100 rows of rank 32 13 and 21, 256 22 and 25; 100 rows of rank 64 25 and 23, 256 49 and 28;
 // rank 128 42 and 27, 87 and 34.
 int tile_rows(int Rp) { return Rp <= 32 ? 257 : 97; }
-constexpr int LORA_PARTS = 4;      // of k, at most
+constexpr int LORA_PARTS = 8;      // of k, at most
 
-int parts_of(const dc_ctx* ctx, int M, int64_t Kp) {      // until the CTAs fill the SMs three times, a warp keeping two steps
+// Until the CTAs fill the SMs three times, a warp keeping two steps, and four from the fifth part on: 400 rows, K 8192, rank 16 in four parts 17.8 us, in eight 15.9; 700 rows, K 2048,
+// rank 64 30.5 and 32.5.
+int parts_of(const dc_ctx* ctx, int M, int64_t Kp) {
     int n = 1;
-    while (n < LORA_PARTS && (M + 15) / 16 * n < 3 * ctx->num_sms && Kp / (16 * 8 * 2 * n) >= 2) n *= 2;
+    while (n < LORA_PARTS && (M + 15) / 16 * n < 3 * ctx->num_sms && Kp / (16 * 8 * 2 * n) >= (n < 4 ? 2 : 4)) n *= 2;
     return n;
 }
 
@@ -370,7 +372,9 @@ int launch_add(dc_ctx* ctx, LoraParams p, int max_rank, int32_t* order) {
         DC_TRY(dc_launch(ctx, "k_lora_order", k_lora_order, dim3(1), dim3(LORA_SORTED), 0, p, order));
         p.order = order;
     }
-    DC_TRY(dc_launch(ctx, "k_lora_down_tile", k_lora_down_tile<BF>, dim3((p.M + 15) / 16, (p.Rp + DT_R - 1) / DT_R, parts), dim3(256), 0, p, vx));
+    const int ranks = p.Rp <= 16 ? 16 : 32;      // of a CTA
+    auto down = ranks == 16 ? k_lora_down_tile<BF, 2> : k_lora_down_tile<BF, 4>;
+    DC_TRY(dc_launch(ctx, "k_lora_down_tile", down, dim3((p.M + 15) / 16, (p.Rp + ranks - 1) / ranks, parts), dim3(256), 0, p, vx));
     return dc_launch(ctx, "k_lora_up", k_lora_up<BF>, dim3((unsigned)((p.N + 255) / 256), (p.M + 15) / 16), dim3(256), 0, p, vy, parts);
 }
 
