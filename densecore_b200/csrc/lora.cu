@@ -242,8 +242,9 @@ __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, i
 }
 
 // Many rows: y = base + h B^T, a CTA per (16 rows, 256 columns), a warp has 32 columns.  h comes in `parts` sums, 128 ranks of it at a time; base is on its way
-// meanwhile.  Bound: base and y, and the two-term products beside them: 2011 rows, N 6144, K 2048, rank 64: 42 of the call's 70 us, 2.3 TB/s; base and y without products would
-// take 22.  (Several tiles a CTA with the matrix in shared memory and base fetched three tiles ahead: 73 us a call; parts of h summed by clusters: 69.)
+// meanwhile.  Bound: base and y, and the two-term products beside them: 2011 rows, N 6144, K 2048, rank 64: some 45 of the call's 68 us, 2.2 TB/s; base and y without products would
+// take 22.  (Several tiles a CTA with the matrix in shared memory and base fetched three tiles ahead: 73 us a call where this took 70; two CTAs an SM with more
+// loads on their way 74 against 68; four with 64 registers spill: 78.)
 constexpr int UP_R = 128;
 template <bool BF>
 __global__ void __launch_bounds__(256, 3) k_lora_up(const LoraParams p, int vec, int parts) {
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(256, 3) k_lora_up(const LoraParams p, int vec,
                 *reinterpret_cast<float4*>(&sh[row][4 * c]) = v;
             }
             __syncthreads();
-#pragma unroll 2
+#pragma unroll 4
             for (int r = 0; r < here; r += 16) {
                 uint2 c[NP];
 #pragma unroll
