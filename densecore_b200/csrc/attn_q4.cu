@@ -681,13 +681,16 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
             at[i] = bytes;
             bytes += cap[i];
         }
+        z.retired.reserve(z.retired.size() + 1);
         uint8_t* fresh = nullptr;
         DC_TRY(dc_check_cuda(ctx, cudaMalloc(&fresh, bytes), "kv_batch: plan"));
-        if (z.plan) {      // a captured call that still names it finds a step without tokens
-            z.retired.push_back(z.plan);
-            DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.plan, 0, sizeof(dc_q4_head), ctx->stream), "kv_batch: old plan"));
+        cudaError_t e = cudaMemsetAsync(fresh, 0, at[DC_Q4_WS], ctx->stream);
+        if (e == cudaSuccess && z.plan) e = cudaMemsetAsync(z.plan, 0, sizeof(dc_q4_head), ctx->stream);      // a captured call that still names it finds a step without tokens
+        if (e != cudaSuccess) {
+            cudaFree(fresh);
+            return dc_check_cuda(ctx, e, "kv_batch: plan");
         }
-        DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(fresh, 0, at[DC_Q4_WS], ctx->stream), "kv_batch: plan"));
+        if (z.plan) z.retired.push_back(z.plan);
         z.plan = fresh, z.plan_bytes = bytes;
         std::copy(cap, cap + DC_Q4_ARRAYS, z.cap), std::copy(at, at + DC_Q4_ARRAYS, z.at);
     }
