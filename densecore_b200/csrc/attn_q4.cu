@@ -82,7 +82,7 @@ __device__ __forceinline__ void codes_of(uint32_t w, uint32_t (&c)[4]) {
 // ---------------------------------------------------------------- new rows into the cache
 struct WriteParams {
     const dc_q4_head* head;
-    const dc_q4_token* tokens;
+    const dc_q4_token* tokens;   // null: the header's
     const void *k, *v;
     int ldkv, n_kv;
     uint8_t* arena;
@@ -104,9 +104,10 @@ __global__ void __launch_bounds__(128) k_q4_write(const WriteParams p) {
     pdl_wait();
     pdl_launch_dependents();      // (not before the wait: what the next kernel reads ahead of its own wait has to be complete)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = p.head->T * p.n_kv;
+    const dc_q4_token* tokens = p.tokens ? p.tokens : p.head->tokens;
     for (int u = blockIdx.x * 4 + warp; u < units; u += gridDim.x * 4) {
         const int t = u / p.n_kv, head = u - t * p.n_kv;
-        const dc_q4_token tok = p.tokens[t];
+        const dc_q4_token tok = tokens[t];
         float x[2][PER], lo[2], hi[2];
         bool fine[2];
 #pragma unroll
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(128) k_q4_write(const WriteParams p) {
 // ---------------------------------------------------------------- attention, eight rows at a time
 struct RowsParams {
     const dc_q4_head* head;
-    const dc_q4_item* items;
+    const dc_q4_item* items;      // these three: not of captured calls
     int* tickets;
     float* ws;
     const void* q;
@@ -199,7 +200,8 @@ constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BY
 // turn codes and scales into operands (59 % of the issue slots): 48 bf16 requests of up to 32000 positions, 533 MB, 162 us, 3.3 TB/s.  Four warps a CTA beat eight (sixteen
 // requests 15 against 23 us): fewer parts to join.
 // A lane has row h = lane / 4 of the tile and tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page (t = lane % 4).
-template <int HD, typename TX>
+// CAPTURED: the arrays' places come from the header, and there may be more CTAs than items.
+template <int HD, typename TX, bool CAPTURED>
 __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(const RowsParams p) {
     using R = dc_q4_rec<HD>;
     constexpr bool EXACT = sizeof(TX) == 4;
@@ -221,12 +223,13 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
     bool waited = !p.early;
     if (waited) pdl_wait();
     pdl_launch_dependents();
-    dc_q4_item im = p.items[blockIdx.x];      // (within the plan's room even if a later plan has fewer: it need not wait for their number)
+    dc_q4_item im;
+    if constexpr (!CAPTURED) im = p.items[blockIdx.x];      // (as many as CTAs: it need not wait for their number)
     const int n_items = p.head->n_items;
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && p.head->n_tiles > 0 && p.tiles == 0) atomicExch(p.err, DC_ERR_REPLAY);
     uint32_t n_full = 0;      // pages that this warp has waited for
     for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
-        if (it != (int)blockIdx.x) im = p.items[it];
+        if (CAPTURED || it != (int)blockIdx.x) im = (CAPTURED ? p.head->items : p.items)[it];
         const int r = im.tile * 8 + h, j = r / G, g = r - j * G;
         const bool row = j < im.count;
         const int qpos = im.pos0 + j, first_new = im.pos0 / DC_KV_BLOCK, all_see = im.pos0 + im.tile * 8 / G;      // positions up to all_see: seen by every row
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
         __syncthreads();
         // ---- joined: a thread has four neighbouring dimensions of a row at a time
         const bool alone = im.n_splits == 1;
-        float* ws = p.ws + ((size_t)im.ws * p.n_kv + (size_t)im.n_splits * kvh) * PART;
+        float* ws = (CAPTURED ? p.head->ws : p.ws) + ((size_t)im.ws * p.n_kv + (size_t)im.n_splits * kvh) * PART;
         auto store = [&](int x4, const float4& v, float inv) {
             const int ro = im.tile * 8 + x4 / (HD / 4), jo = ro / G, go = ro - jo * G;
             if (jo >= im.count) return;
@@ -526,7 +529,7 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
             }
         }
         if (!alone) {
-            int* ticket = p.tickets + im.ticket * p.n_kv + kvh;
+            int* ticket = (CAPTURED ? p.head->tickets : p.tickets) + im.ticket * p.n_kv + kvh;
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -594,9 +597,12 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
 template <int HD, typename TX>
 int launch_rows(dc_ctx* ctx, const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
-    DC_TRY(dc_kernel_setup(ctx, (const void*)k_q4_rows<HD, TX>, (int)rows_smem<HD>(), "k_q4_rows"));
-    RowsParams p = {(const dc_q4_head*)z.plan, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.early, z.n_tiles, ctx->d_err};
-    return dc_launch(ctx, "k_q4_rows", k_q4_rows<HD, TX>, dim3(z.n_items, z.kv), dim3(RW * 32), rows_smem<HD>(), p);
+    const auto kernel = c.captured ? k_q4_rows<HD, TX, true> : k_q4_rows<HD, TX, false>;
+    DC_TRY(dc_kernel_setup(ctx, (const void*)kernel, (int)rows_smem<HD>(), "k_q4_rows"));
+    const RowsParams p = {z.head, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.early, z.n_tiles, ctx->d_err};
+    // (a captured call's later plans may have more items: CTAs for all SMs)
+    const int ctas = c.captured ? std::max(z.n_items, ((sizeof(TX) == 2 ? 4 : 3) * ctx->num_sms + z.kv - 1) / z.kv) : z.n_items;
+    return dc_launch(ctx, "k_q4_rows", kernel, dim3(ctas, z.kv), dim3(RW * 32), rows_smem<HD>(), p);
 }
 
 template <int HD, typename TX>
@@ -619,6 +625,7 @@ void dc_q4_release(dc_kv_cache* kv) {
     if (!z) return;
     if (z->plan) cudaFree(z->plan);
     for (uint8_t* p : z->retired) cudaFree(p);
+    if (z->head) cudaFree(z->head);
     if (z->stage) cudaFreeHost(z->stage);
     if (z->uploaded) cudaEventDestroy(z->uploaded);
     delete z;
@@ -669,13 +676,13 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
     dc_q4_tiles(many, G, z.kv, ctx->num_sms, &tiles, &n_parts);
     for (size_t i = 0; i < tiles.size(); ++i)
         if (tiles[i].n_splits > 1 && tiles[i].split == 0) joins.push_back((int32_t)i);
-    // ---- header, arrays, tickets (zero, and left so by every call), partial results
+    // ---- arrays, tickets (zero, and left so by every call), partial results
     const size_t need[DC_Q4_ARRAYS] = {tokens.size() * sizeof(dc_q4_token), items.size() * sizeof(dc_q4_item), tiles.size() * sizeof(dc_q4_tile), joins.size() * 4, (size_t)n_tickets * z.kv * 4,
                                        (size_t)n_ws * z.kv * 8 * (z.dim + 2) * 4, (size_t)n_parts * z.kv * 256 * (z.dim + 4) * 4};
     bool fits = z.plan != nullptr;
     for (int i = 0; i < DC_Q4_ARRAYS; ++i) fits = fits && need[i] <= z.cap[i];
     if (!fits) {
-        size_t cap[DC_Q4_ARRAYS], at[DC_Q4_ARRAYS], bytes = 256;
+        size_t cap[DC_Q4_ARRAYS], at[DC_Q4_ARRAYS], bytes = 0;
         for (int i = 0; i < DC_Q4_ARRAYS; ++i) {
             cap[i] = std::max(z.cap[i], (need[i] + need[i] / 2 + 4096) / 256 * 256);
             at[i] = bytes;
@@ -684,36 +691,36 @@ int make_plan(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<dc_q4_entry>& es, 
         z.retired.reserve(z.retired.size() + 1);
         uint8_t* fresh = nullptr;
         DC_TRY(dc_check_cuda(ctx, cudaMalloc(&fresh, bytes), "kv_batch: plan"));
-        cudaError_t e = cudaMemsetAsync(fresh, 0, at[DC_Q4_WS], ctx->stream);
-        if (e == cudaSuccess && z.plan) e = cudaMemsetAsync(z.plan, 0, sizeof(dc_q4_head), ctx->stream);      // a captured call that still names it finds a step without tokens
+        const cudaError_t e = cudaMemsetAsync(fresh, 0, at[DC_Q4_WS], ctx->stream);
         if (e != cudaSuccess) {
             cudaFree(fresh);
             return dc_check_cuda(ctx, e, "kv_batch: plan");
         }
         if (z.plan) z.retired.push_back(z.plan);
-        z.plan = fresh, z.plan_bytes = bytes;
+        z.plan = fresh;
         std::copy(cap, cap + DC_Q4_ARRAYS, z.cap), std::copy(at, at + DC_Q4_ARRAYS, z.at);
     }
     if (!z.uploaded) DC_TRY(dc_check_cuda(ctx, cudaEventCreateWithFlags(&z.uploaded, cudaEventDisableTiming), "kv_batch: event"));
     else DC_TRY(dc_check_cuda(ctx, cudaEventSynchronize(z.uploaded), "kv_batch: staging"));
-    const size_t staged = 256 + need[0] + need[1] + need[2] + need[3];
+    const size_t staged = sizeof(dc_q4_head) + need[0] + need[1] + need[2] + need[3];
     if (staged > z.stage_bytes) {
         if (z.stage) cudaFreeHost(z.stage);
         z.stage = nullptr, z.stage_bytes = 0;
         DC_TRY(dc_check_cuda(ctx, cudaMallocHost(&z.stage, staged * 2), "kv_batch: staging"));
         z.stage_bytes = staged * 2;
     }
-    const dc_q4_head hd = {T, (int)items.size(), (int)tiles.size(), (int)joins.size()};
+    const dc_q4_head hd = {T, (int)items.size(), (int)tiles.size(), (int)joins.size(), (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]),
+                           (int32_t*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS])};
     const void* from[4] = {tokens.data(), items.data(), tiles.data(), joins.data()};
-    memcpy(z.stage, &hd, sizeof(hd));
-    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.plan, z.stage, sizeof(hd), cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
-    size_t off = 256;
+    size_t off = sizeof(hd);
     for (int i = 0; i < 4; ++i) {
         if (!need[i]) continue;
         memcpy(z.stage + off, from[i], need[i]);
         DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.plan + z.at[i], z.stage + off, need[i], cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
         off += need[i];
     }
+    memcpy(z.stage, &hd, sizeof(hd));
+    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.head, z.stage, sizeof(hd), cudaMemcpyHostToDevice, ctx->stream), "kv_batch: plan"));
     DC_TRY(dc_check_cuda(ctx, cudaEventRecord(z.uploaded, ctx->stream), "kv_batch: plan"));
     z.T = T, z.n_items = hd.n_items, z.n_tiles = hd.n_tiles, z.n_joins = hd.n_joins;
     return DC_B200_OK;
@@ -734,15 +741,17 @@ int empty_step(dc_ctx* ctx, const char* name) {      // nothing to do; a capture
     return capturing(ctx) ? dc_fail(ctx, DC_B200_UNSUPPORTED, "%s: a step without tokens cannot be captured", name) : DC_B200_OK;
 }
 
-int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held) {
+int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held, bool captured) {
     const dc_q4& z = *kv->q4;
-    const WriteParams p = {(const dc_q4_head*)z.plan, (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), k, v, ldkv, z.kv, kv->planes[layer].arena, k_held, v_held};
+    const WriteParams p = {z.head, captured ? nullptr : (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), k, v, ldkv, z.kv, kv->planes[layer].arena, k_held, v_held};
     const int units = z.T * z.kv;
     if (z.dim == 128) return z.type == DC_TYPE_F32 ? launch_write<128, float>(ctx, p, units) : launch_write<128, __nv_bfloat16>(ctx, p, units);
     return z.type == DC_TYPE_F32 ? launch_write<64, float>(ctx, p, units) : launch_write<64, __nv_bfloat16>(ctx, p, units);
 }
 
 int create(dc_ctx* ctx, dc_kv_cache* kv, int n_layer, int n_head, int n_kv_head, int head_dim, int row_type, int max_blocks, int max_seqs, int max_blocks_per_seq) {
+    DC_TRY(dc_check_cuda(ctx, cudaMalloc(&kv->q4->head, sizeof(dc_q4_head)), "kv_create_q4"));
+    DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(kv->q4->head, 0, sizeof(dc_q4_head), ctx->stream), "kv_create_q4"));
     kv->q4->n_layer = n_layer, kv->q4->heads = n_head, kv->q4->kv = n_kv_head, kv->q4->dim = head_dim, kv->q4->type = row_type;
     return dc_kv_init_planes(ctx, kv, std::vector<size_t>(n_layer, (size_t)n_kv_head * 18 * head_dim / DC_KV_BLOCK), 0, max_blocks, max_seqs, max_blocks_per_seq);
 }
@@ -842,7 +851,7 @@ int dc_b200_kv_q4_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void*
     if (z.T == 0) return empty_step(ctx, "kv_q4_write_dev");
     if (!k_dev || !v_dev || ld_kv < z.kv * z.dim) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_q4_write_dev: bad argument (row stride %d)", ld_kv);
     cudaSetDevice(ctx->device);
-    return write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev);
+    return write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev, capturing(ctx));
 }
 
 int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_dev, int ld_q, const void* k_dev, const void* v_dev, int ld_kv, float scale,
@@ -855,11 +864,12 @@ int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const voi
     if (z.T == 0) return empty_step(ctx, "flash_attn_q4_dev");
     if (!q_dev || !out_dev || (!k_dev != !v_dev) || ld_q < z.heads * z.dim || ld_out < z.heads * z.dim || ld_kv < z.kv * z.dim || (!k_dev && (k_held_dev || v_held_dev)))
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: bad argument (row strides %d, %d, %d)", ld_q, ld_kv, ld_out);
-    if (z.n_tiles && capturing(ctx)) return dc_fail(ctx, DC_B200_UNSUPPORTED, "flash_attn_q4_dev: prompt-sized portions cannot be captured (their number of CTAs goes by the positions)");
+    const bool captured = capturing(ctx);
+    if (z.n_tiles && captured) return dc_fail(ctx, DC_B200_UNSUPPORTED, "flash_attn_q4_dev: prompt-sized portions cannot be captured (their number of CTAs goes by the positions)");
     if (!isfinite(scale)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: scale is not finite");
     cudaSetDevice(ctx->device);
-    if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev));
-    dc_q4_call c = {kv, kv->planes[layer].arena, q_dev, ld_q, ld_out, scale, out_dev, k_dev ? 1 : 0};
+    if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev, captured));
+    dc_q4_call c = {kv, kv->planes[layer].arena, q_dev, ld_q, ld_out, scale, out_dev, k_dev ? 1 : 0, captured};
     DC_TRY(dc_launch_q4_prompt(ctx, c));
     if (z.n_tiles) c.early = 2;      // the SMs that prompt tiles leave idle take the single tokens meanwhile
     DC_TRY(dc_launch_q4_rows(ctx, c));

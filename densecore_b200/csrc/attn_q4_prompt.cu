@@ -66,7 +66,6 @@ __device__ __forceinline__ void lds_turned(uint32_t at, int turn, uint32_t (&w)[
 }
 
 struct PromptParams {
-    const dc_q4_head* head;
     const dc_q4_tile* tiles;
     const int32_t* joins;
     float* ws;
@@ -538,7 +537,7 @@ __global__ void __launch_bounds__(256) k_q4_join(const PromptParams p) {
 
 PromptParams params(const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
-    return {(const dc_q4_head*)z.plan, (const dc_q4_tile*)(z.plan + z.at[DC_Q4_TILES]), (const int32_t*)(z.plan + z.at[DC_Q4_JOINS]), (float*)(z.plan + z.at[DC_Q4_PARTS]),
+    return {(const dc_q4_tile*)(z.plan + z.at[DC_Q4_TILES]), (const int32_t*)(z.plan + z.at[DC_Q4_JOINS]), (float*)(z.plan + z.at[DC_Q4_PARTS]),
             (const __nv_bfloat16*)c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, (__nv_bfloat16*)c.out};
 }
 

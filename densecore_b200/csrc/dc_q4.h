@@ -28,13 +28,19 @@ struct dc_q4_rec {
     }
 };
 
-// The plan of a step in device memory, one allocation: this header, then arrays at places that stay where they are as long as the allocation does.  Kernels
-// get the places and read the counts, so that a captured call takes later plans too.
-struct dc_q4_head {
-    int32_t T, n_items, n_tiles, n_joins;
-};
+// The plan of a step in device memory: arrays in one allocation, which a larger plan replaces, and this header, which stays where it is as long as the cache does.
+// Kernels get the arrays' places from the host and read the counts, so that they need not wait for one to find the other; within a captured call they take the
+// places from the header, so that it serves every later plan, wherever that lies.
 struct dc_q4_token {
     int32_t block, slot;
+};
+struct dc_q4_item;
+struct dc_q4_head {
+    int32_t T, n_items, n_tiles, n_joins;
+    const dc_q4_token* tokens;
+    const dc_q4_item* items;
+    int32_t* tickets;
+    float* ws;
 };
 // One CTA's work in k_q4_rows: pages page0 .. page1 - 1 for one tile of eight rows (row r: new token r / G of the entry, query head r % G of the key head).
 struct dc_q4_item {
@@ -100,10 +106,10 @@ struct dc_q4 {
     bool planned = false;
     uint64_t edits = 0;
     int T = 0, n_items = 0, n_tiles = 0, n_joins = 0;
-    uint8_t* plan = nullptr;
-    size_t plan_bytes = 0;
+    dc_q4_head* head = nullptr;         // device
+    uint8_t* plan = nullptr;            // arrays
     size_t cap[7] = {}, at[7] = {};     // room for the arrays and where they begin: tokens, items, tiles, joins, tickets, partial results of rows and of prompt tiles
-    std::vector<uint8_t*> retired;      // outgrown plans, emptied; captured calls may still read them
+    std::vector<uint8_t*> retired;      // outgrown plans, which calls in flight may still read
     uint8_t* stage = nullptr;           // pinned copy of the plan being uploaded
     size_t stage_bytes = 0;
     cudaEvent_t uploaded = nullptr;
@@ -120,6 +126,7 @@ struct dc_q4_call {
     void* out;
     int early;                 // what k_q4_rows may do ahead of its predecessor's end: 0 nothing, 1 all but the step's own pages and stores (k_q4_write), 2 everything
                                // (k_q4_prompt of the same call, whose CTAs have begun, behind k_q4_write)
+    bool captured;             // the call is being captured: its replays take the newest plan from the header
 };
 int dc_launch_q4_rows(dc_ctx* ctx, const dc_q4_call& c);
 int dc_launch_q4_prompt(dc_ctx* ctx, const dc_q4_call& c);
