@@ -413,6 +413,9 @@ int dc_b200_lora_create(dc_ctx* ctx, int64_t K, int64_t N, int max_adapters, int
     if (K < 1 || N < 1 || K > (1 << 24) || N > (1 << 24) || max_adapters < 1 || max_rank < 1 || max_rank > 4096)
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_create: bad shape (%lld x %lld, %d adapters of rank %d)", (long long)K, (long long)N, max_adapters, max_rank);
     if (type != DC_TYPE_BF16 && type != DC_TYPE_F16) return dc_fail(ctx, DC_B200_UNSUPPORTED, "lora_create: matrices of type %d (BF16 and F16 are supported)", type);
+    // (2^40 numbers a matrix are beyond any device's memory, and their bytes clear of 64 bits' end)
+    if (max_adapters > (int64_t(1) << 40) / ((max_rank + 15) / 16 * 16 * (std::max(K, N) + 15)))
+        return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "lora_create: %d adapters of rank %d beside a matrix of %lld x %lld", max_adapters, max_rank, (long long)N, (long long)K);
     cudaSetDevice(ctx->device);
     dc_lora* l = new (std::nothrow) dc_lora();
     if (!l) return dc_fail(ctx, DC_B200_OUT_OF_MEMORY, "lora_create: out of host memory");

@@ -312,7 +312,8 @@ DC_B200_API int dc_b200_sample_rows(dc_ctx* ctx, const float* logits_host, int r
 
 /* ---- low-rank adapters beside a shared product -------------------------------- */
 /* A set of adapters of one matrix [N, K] for many requests at once (no counterpart in DenseCore): slot a holds A [rank, K]
- * and B [N, rank], DC_GGML_TYPE_BF16 or DC_GGML_TYPE_F16, and a scale; ranks may differ, max_rank at most.  Matrices are copied into a layout of the set's own. */
+ * and B [N, rank], DC_GGML_TYPE_BF16 or DC_GGML_TYPE_F16, and a scale; ranks may differ, max_rank at most.  Matrices are copied into a layout of the set's own.
+ * K and N up to 2^24, max_rank up to 4096, each matrix of all slots together up to 2^40 numbers. */
 typedef struct dc_lora dc_lora;
 DC_B200_API int dc_b200_lora_create(dc_ctx* ctx, int64_t K, int64_t N, int max_adapters, int max_rank, int type, dc_lora** out);
 DC_B200_API void dc_b200_lora_destroy(dc_lora* l);

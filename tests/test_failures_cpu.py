@@ -38,3 +38,25 @@ int main() {
 """)
     r = run(exe)
     assert r.returncode == 0 and int(r.stdout.split()[0]) > 8, r.stdout
+
+
+def test_sets_of_adapters_beyond_any_memory_are_refused(tmp_path):
+    """Sizes whose bytes wrap around 64 bits would get a small allocation and be written far beyond it."""
+    exe = program(tmp_path, ["lora"], r"""
+extern "C" int dc_b200_mul_mat_dev(dc_ctx*, const dc_weight*, const float*, int, float*) { return 0; }
+int main() {
+    dc_ctx ctx;
+    const long long bad[][4] = {{1 << 24, 1 << 24, 1 << 27, 4096}, {1 << 24, 8, 1 << 27, 4096}, {16, 1 << 24, 1 << 30, 2048}, {1 << 24, 1 << 24, 1 << 28, 16}, {1 << 24, 1 << 24, 2147483647, 4096}, {1 << 23, 100, 1 << 28, 4096}};
+    for (auto& b : bad) {
+        dc_lora* l = nullptr;
+        const int st = dc_b200_lora_create(&ctx, b[0], b[1], (int)b[2], (int)b[3], DC_GGML_TYPE_BF16, &l);
+        if (st != DC_B200_OUT_OF_MEMORY || l || fake::calls) return printf("%lld x %lld, %lld adapters of rank %lld: status %d\n", b[0], b[1], b[2], b[3], st), 1;
+    }
+    dc_lora* l = nullptr;
+    if (dc_b200_lora_create(&ctx, 64, 32, 4, 8, DC_GGML_TYPE_BF16, &l)) return printf("a small one\n"), 1;
+    dc_b200_lora_destroy(l);
+    return fake::bad_frees || !fake::live.empty();
+}
+""")
+    r = run(exe)
+    assert r.returncode == 0, r.stdout
