@@ -403,6 +403,12 @@ int check_set(dc_lora* l, int slot, int rank, const void* a, const void* b, floa
     return DC_B200_OK;
 }
 
+void release(dc_lora* l) {      // (what it does not have is null)
+    cudaFree(l->a), cudaFree(l->b), cudaFree(l->rank), cudaFree(l->scale), cudaFree(l->order), cudaFree(l->h);
+    for (float* h : l->retired) cudaFree(h);
+    delete l;
+}
+
 }  // namespace
 
 extern "C" {
@@ -429,8 +435,7 @@ int dc_b200_lora_create(dc_ctx* ctx, int64_t K, int64_t N, int max_adapters, int
     if (e == cudaSuccess) e = cudaMemsetAsync(l->rank, 0, (size_t)max_adapters * 4, ctx->stream);
     if (e != cudaSuccess) {
         const int st = dc_check_cuda(ctx, e, "lora_create");
-        cudaFree(l->a), cudaFree(l->b), cudaFree(l->rank), cudaFree(l->scale);
-        delete l;
+        release(l);
         return st;
     }
     *out = l;
@@ -441,11 +446,7 @@ void dc_b200_lora_destroy(dc_lora* l) {
     if (!l) return;
     cudaSetDevice(l->ctx->device);
     cudaStreamSynchronize(l->ctx->stream);
-    cudaFree(l->a), cudaFree(l->b), cudaFree(l->rank), cudaFree(l->scale);
-    if (l->h) cudaFree(l->h);
-    for (float* h : l->retired) cudaFree(h);
-    cudaFree(l->order);
-    delete l;
+    release(l);
 }
 
 int dc_b200_lora_set_dev(dc_lora* l, int slot, int rank, const void* a_dev, const void* b_dev, float scale) {

@@ -60,3 +60,24 @@ int main() {
 """)
     r = run(exe)
     assert r.returncode == 0, r.stdout
+
+
+def test_a_set_of_adapters_that_fails_to_be_made_leaves_nothing(tmp_path):
+    exe = program(tmp_path, ["lora"], r"""
+extern "C" int dc_b200_mul_mat_dev(dc_ctx*, const dc_weight*, const float*, int, float*) { return 0; }
+int main() {
+    for (int n = 1;; ++n) {
+        dc_ctx ctx;
+        dc_lora* l = nullptr;
+        fake::calls = 0, fake::fail_at = n;
+        const int st = dc_b200_lora_create(&ctx, 64, 32, 4, 8, DC_GGML_TYPE_BF16, &l);
+        const bool failed = fake::calls >= n;
+        if (failed != (st != 0) || failed != !l) return printf("call %d: status %d\n", n, st), 1;
+        dc_b200_lora_destroy(l);
+        if (fake::bad_frees || !fake::live.empty()) return printf("call %d: %d freed twice, %d lost\n", n, fake::bad_frees, (int)fake::live.size()), 1;
+        if (!failed) return printf("%d calls\n", n - 1), 0;
+    }
+}
+""")
+    r = run(exe)
+    assert r.returncode == 0 and int(r.stdout.split()[0]) == 6, r.stdout
