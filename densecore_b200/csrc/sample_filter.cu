@@ -772,11 +772,14 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
         constexpr int PER = 16 / sizeof(TX), IN_FLIGHT = 4;
         if (((uintptr_t)(src + at0) & 15) == 0) {
             for (int i0 = s.lane * PER; i0 < p.seg; i0 += IN_FLIGHT * 32 * PER) {
-                TX v[IN_FLIGHT][PER];
+                struct alignas(16) Piece {      // taken and stored as sixteen bytes
+                    TX x[PER];
+                } v[IN_FLIGHT];
+                static_assert(sizeof(v) == 16 * IN_FLIGHT && alignof(Piece) == 16, "pieces are loads of 16 bytes");
 #pragma unroll
                 for (int c = 0; c < IN_FLIGHT; ++c) {
                     const int i = i0 + c * 32 * PER;
-                    if (i < p.seg && at0 + i + PER <= p.V) *reinterpret_cast<uint4*>(v[c]) = __ldg(reinterpret_cast<const uint4*>(src + at0 + i));
+                    if (i < p.seg && at0 + i + PER <= p.V) *reinterpret_cast<uint4*>(v[c].x) = __ldg(reinterpret_cast<const uint4*>(src + at0 + i));
                 }
 #pragma unroll
                 for (int c = 0; c < IN_FLIGHT; ++c) {
@@ -785,14 +788,14 @@ __global__ void __launch_bounds__(SF_T, 2) k_sample_filter(const SampleParams p)
                     float f[PER];
                     if (at0 + i + PER <= p.V) {
 #pragma unroll
-                        for (int j = 0; j < PER; ++j) f[j] = take((float)v[c][j], i + j);
+                        for (int j = 0; j < PER; ++j) f[j] = take((float)v[c].x[j], i + j);
                     } else {
 #pragma unroll
                         for (int j = 0; j < PER; ++j) f[j] = take(at0 + i + j < p.V ? (float)src[at0 + i + j] : -INFINITY, i + j);
                     }
 #pragma unroll
-                    for (int j = 0; j < PER; ++j) v[c][j] = (TX)f[j];
-                    *reinterpret_cast<uint4*>(x + i) = *reinterpret_cast<const uint4*>(v[c]);
+                    for (int j = 0; j < PER; ++j) v[c].x[j] = (TX)f[j];
+                    *reinterpret_cast<uint4*>(x + i) = *reinterpret_cast<const uint4*>(v[c].x);
                 }
             }
         } else {
