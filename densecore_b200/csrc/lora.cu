@@ -397,6 +397,11 @@ int grow(dc_ctx* ctx, dc_lora* l, int64_t rows) {
     return DC_B200_OK;
 }
 
+constexpr int LORA_ROWS = 65535 * 16;      // of a call: a grid's second dimension
+
+// Room for the row sums of a call of M rows.
+int make_room(dc_ctx* ctx, dc_lora* l, int M) { return grow(ctx, l, M < tile_rows(l->Rp) ? M : (int64_t)M * parts_of(ctx, M, l->Kp)); }
+
 int check_set(dc_lora* l, int slot, int rank, const void* a, const void* b, float scale) {
     if (slot < 0 || slot >= l->slots || rank < 0 || rank > l->max_rank || (rank && (!a || !b)) || !isfinite(scale))
         return dc_fail(l->ctx, DC_B200_INVALID_ARGUMENT, "lora_set: slot %d of %d, rank %d of at most %d", slot, l->slots, rank, l->max_rank);
@@ -479,13 +484,13 @@ int dc_b200_lora_add_dev(dc_ctx* ctx, dc_lora* l, const float* x_dev, int64_t ld
     if (ld_x == 0) ld_x = l->K;
     if (ld_base == 0) ld_base = l->N;
     if (ld_y == 0) ld_y = l->N;
-    if (M < 0 || M > 65535 * 16 || ld_x < l->K || ld_base < l->N || ld_y < l->N)
+    if (M < 0 || M > LORA_ROWS || ld_x < l->K || ld_base < l->N || ld_y < l->N)
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: bad argument (%d rows, strides %lld, %lld, %lld)", M, (long long)ld_x, (long long)ld_base, (long long)ld_y);
     if (M == 0) return DC_B200_OK;
     if (!x_dev || !ids_dev || !y_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "lora_add: null buffer");
     if (!base_dev) base_dev = y_dev, ld_base = ld_y;
     cudaSetDevice(ctx->device);
-    DC_TRY(grow(ctx, l, M < tile_rows(l->Rp) ? M : (int64_t)M * parts_of(ctx, M, l->Kp)));
+    DC_TRY(make_room(ctx, l, M));
     const LoraParams p = {l->a, l->b, l->rank, l->scale, l->slots, l->Rp, l->K, l->N, l->Kp, l->Np, x_dev, ld_x, M, ids_dev, l->h, base_dev, y_dev, ld_base, ld_y, nullptr};
     return l->type == DC_TYPE_BF16 ? launch_add<true>(ctx, p, l->max_rank, l->order) : launch_add<false>(ctx, p, l->max_rank, l->order);
 }
@@ -494,10 +499,12 @@ int dc_b200_mul_mat_lora_dev(dc_ctx* ctx, const dc_weight* w, dc_lora* l, const 
     if (!ctx || !w || !l) return DC_B200_INVALID_ARGUMENT;
     if (w->K != l->K || w->N != l->N || w->E != 1)
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: adapters of %lld x %lld beside a matrix of %lld x %lld", (long long)l->K, (long long)l->N, (long long)w->K, (long long)w->N);
-    if (M < 1 || !x_dev || !ids_dev || !y_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: bad argument");
+    if (M < 1 || M > LORA_ROWS || !x_dev || !ids_dev || !y_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: bad argument (%d rows)", M);
     const uintptr_t x0 = (uintptr_t)x_dev, x1 = (uintptr_t)(x_dev + (size_t)M * l->K), y0 = (uintptr_t)y_dev, y1 = (uintptr_t)(y_dev + (size_t)M * l->N);
     if (!(x1 <= y0 || y1 <= x0)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: x and y overlap");
     if (l->ctx != ctx) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "mul_mat_lora: the adapters belong to another context");
+    cudaSetDevice(ctx->device);
+    DC_TRY(make_room(ctx, l, M));      // (ahead of the product: a refused call has enqueued nothing)
     DC_TRY(dc_b200_mul_mat_dev(ctx, w, x_dev, M, y_dev));
     return dc_b200_lora_add_dev(ctx, l, x_dev, 0, M, ids_dev, nullptr, 0, y_dev, 0);
 }

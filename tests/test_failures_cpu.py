@@ -81,3 +81,41 @@ int main() {
 """)
     r = run(exe)
     assert r.returncode == 0 and int(r.stdout.split()[0]) == 6, r.stdout
+
+
+def test_a_product_with_adapters_is_refused_before_any_of_it_runs(tmp_path):
+    """Too many rows, or a workspace that cannot grow (a capture, no memory): neither the product nor anything else has been enqueued."""
+    exe = program(tmp_path, ["lora"], r"""
+static int products = 0;
+extern "C" int dc_b200_mul_mat_dev(dc_ctx*, const dc_weight*, const float*, int, float*) { return ++products, 0; }
+int main() {
+    dc_ctx ctx;
+    dc_weight w = {};
+    w.K = 256, w.N = 32, w.E = 1;
+    dc_lora* l = nullptr;
+    if (dc_b200_lora_create(&ctx, 256, 32, 4, 8, DC_GGML_TYPE_BF16, &l)) return printf("create\n"), 1;
+    float* x = (float*)(size_t(1) << 40);      // (nothing reads them here)
+    float* y = (float*)(size_t(1) << 44);
+    const int* ids = (const int*)x;
+    auto refused = [&](int M, int status) {
+        fake::launches = products = 0;
+        const int st = dc_b200_mul_mat_lora_dev(&ctx, &w, l, x, M, ids, y);
+        if (st != status || products || fake::launches) printf("%d rows: status %d, %d products\n", M, st, products), exit(1);
+    };
+    refused(65535 * 16 + 1, DC_B200_INVALID_ARGUMENT);
+    fake::capturing = true;
+    refused(5, DC_B200_UNSUPPORTED);
+    fake::capturing = false;
+    fake::calls = 0, fake::fail_at = 1;
+    refused(5, DC_B200_OUT_OF_MEMORY);
+    fake::fail_at = 0;
+    if (dc_b200_mul_mat_lora_dev(&ctx, &w, l, x, 5, ids, y) || products != 1 || fake::launches != 2) return printf("five rows: %d products, %d launches\n", products, fake::launches), 1;
+    fake::capturing = true;
+    if (dc_b200_mul_mat_lora_dev(&ctx, &w, l, x, 5, ids, y) || products != 2) return printf("five rows, captured\n"), 1;
+    refused(4000, DC_B200_UNSUPPORTED);
+    dc_b200_lora_destroy(l);
+    return fake::bad_frees || !fake::live.empty();
+}
+""")
+    r = run(exe)
+    assert r.returncode == 0, r.stdout
