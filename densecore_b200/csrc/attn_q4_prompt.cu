@@ -8,7 +8,8 @@
 //   warps 8-15   pages by bulk copies, codes turned into fp16 rows of the operands' 128-byte swizzle (d c + m, rounded once: 2^-11 relative); a warp has the keys
 //                or the values of one page, values turned (rows are dimensions: products with keys along the rows took three times as long to issue)
 //   warps 16-17  issue a set's products each (one warp for both was the bound: some 50 cycles a product)
-// Queries are bf16 rows times a power of two (exact in fp16), weights fp16 (2^-11): together below a bf16 result's own 2^-8.
+// Queries are bf16 rows times a power of two (exact in fp16), weights fp16 (2^-11, the largest at 2^7: down to 2^-32 of it), keys and
+// values fp32(d c + m) rounded to fp16 (2^-11): together below a bf16 result's own 2^-8.
 // A value that is not a number (d = m = NaN) enters the tiles as 0, or the products would carry it to rows that do not see it; the CTA keeps the first
 // position of such a value per group of 64 dimensions, and rows that see it end as NaN there.
 // Bound: the weights' arithmetic and the chain scores, weights, answers of a tile, one CTA per SM: 2011 tokens, 32 query heads, 4 key heads of 128: 60 us, 555 TFLOP/s; the
@@ -222,8 +223,9 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
 #pragma unroll
                     for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s(i));
                 }
-                const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
-                // the reference follows the largest score once that is 2^8 above it: weights up to 256 are as exact, and the answers' factors are rare
+                const float m_new = fmaxf(m_run, fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sl2, -7.0f));
+                // the largest weight is 2^7, so that the others keep fp16's range down to 2^-32 of it: where its value is next to nothing, they are the answer.  The
+                // reference follows once the largest score is 2^8 above it: weights up to 2^15 are as exact, and the answers' factors are rare
                 if (__any_sync(0xffffffffu, m_new > m_run + 8.0f)) {
                     const float corr = ex2(m_run - m_new);
                     m_run = m_new;
