@@ -196,9 +196,12 @@ constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BY
 
 // One CTA per (item, key head): its warps take the item's pages in turn, each with a running maximum of its own, and join at the end; the last CTA of a tile joins
 // the tile's splits in their order, so that results do not depend on who comes last.
-// Bound: a step of few tokens by its launches (one request of 512 positions 11.7 us, sixteen of up to 2300 15 us, with the rows' writing); a long cache by the instructions that
-// turn codes and scales into operands (59 % of the issue slots): 48 bf16 requests of up to 32000 positions, 533 MB, 162 us, 3.3 TB/s.  Four warps a CTA beat eight (sixteen
-// requests 15 against 23 us): fewer parts to join.
+// Bound: a step of few tokens by its launches (one request of 512 positions 10.4 us, sixteen of up to 2300 14.5 us, with the rows' writing; captured ones the same within
+// 0.2 us); a long cache by the chain of a page (codes and scales into operands, scores, weights, answers) in 16 warps an SM, f32 12: 48 requests of up to 32000 positions, 533 MB, bf16
+// 161 us, 3.3 TB/s, 59 % of the issue slots, half of each score product's sixteen rows empty; f32 211 us.  Four CTAs an SM hold bf16 rows of heads of 128 to 128 registers, of
+// which 32 bytes spill.  Four warps a CTA beat eight (sixteen requests 15 against 23 us): fewer parts to join.
+// f32 prompts run here too, eight rows at a time, each tile of rows through all pages that it sees: 2011 tokens, 32 query heads, 4 key heads 452 us where k_q4_prompt takes 59
+// on bf16 rows (its operands are fp16: f32 rows would need two terms of each).
 // A lane has row h = lane / 4 of the tile and tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page (t = lane % 4).
 // CAPTURED: the arrays' places come from the header, and there may be more CTAs than items.
 template <int HD, typename TX, bool CAPTURED>

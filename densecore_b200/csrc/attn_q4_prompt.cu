@@ -12,7 +12,7 @@
 // values fp32(d c + m) rounded to fp16 (2^-11): together below a bf16 result's own 2^-8.
 // A value that is not a number (d = m = NaN) enters the tiles as 0, or the products would carry it to rows that do not see it; the CTA keeps the first
 // position of such a value per group of 64 dimensions, and rows that see it end as NaN there.
-// Bound: the weights' arithmetic and the chain scores, weights, answers of a tile, one CTA per SM: 2011 tokens, 32 query heads, 4 key heads of 128: 60 us, 555 TFLOP/s; the
+// Bound: the weights' arithmetic and the chain scores, weights, answers of a tile, one CTA per SM: 2011 tokens, 32 query heads, 4 key heads of 128: 59.3 us, 559 TFLOP/s; the
 // matrix pipe is busy for 28 % of the time, issue slots for 54 %.  Steps on the way: table entries read once a page, not one load after the other, and rows of queries and results
 // stored coalesced; two issuing warps; references that follow rarely.
 // Keys are split over CTAs where there are fewer row tiles than SMs (dc_q4_tiles); k_q4_join adds the parts up.

@@ -101,7 +101,7 @@ __device__ __forceinline__ float4 load_x4(const float* row, int64_t k, int64_t K
     return make_float4(row[k], k + 1 < K ? row[k + 1] : 0.f, k + 2 < K ? row[k + 2] : 0.f, k + 3 < K ? row[k + 3] : 0.f);
 }
 
-// Few rows: a warp per rank of a row.  Bound: three loads that wait for one another; with k_lora_up_rows 6.8 us for a row (K 2048, N 5120, rank 16), 9.1 for 64 of rank 32.
+// Few rows: a warp per rank of a row.  Bound: three loads that wait for one another; with k_lora_up_rows 6.4 us for a row (K 2048, N 5120, rank 16), 9.3 for 64 of rank 32.
 template <bool BF>
 __global__ void __launch_bounds__(256) k_lora_down(const LoraParams p, int vec) {
     const int row = blockIdx.x, r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -159,7 +159,9 @@ __global__ void __launch_bounds__(128) k_lora_up_rows(const LoraParams p) {
 }
 
 // Rows by adapter, those without one last, else as they come: a row's place is the number of rows before it.  One CTA, some 5 us with its launch.
-// A tile of several adapters takes a pass for each: 200 mixed rows of rank 64 40 us as they come, 27 in order; runs of prompts, where nothing is gained, 22 and 28 at 384 rows.
+// A tile of several adapters takes a pass for each: 200 mixed rows of rank 64 40 us as they come, 27 in order; runs, as prompts have them, gain nothing by an order, 22 and 28 us
+// at 384 rows.  Above 256 rows they are taken as they come, right for runs and slow for mixed rows (K 2048, N 6144, rank 64): 300 rows of 4 adapters 18 us in runs, 43 mixed,
+// of 48 21 and 135; 2011 rows 66 and 175, 70 and 484.
 constexpr int LORA_SORTED = 256;
 __global__ void __launch_bounds__(LORA_SORTED) k_lora_order(const LoraParams p, int32_t* order) {
     __shared__ __align__(16) int slot[LORA_SORTED];
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_down_tile(const LoraParams p, i
 }
 
 // Many rows: y = base + h B^T, a CTA per (16 rows, 256 columns), a warp has 32 columns.  h comes in `parts` sums, 128 ranks of it at a time; base is on its way
-// meanwhile.  Bound: base and y, and the two-term products beside them: 2011 rows, N 6144, K 2048, rank 64: some 45 of the call's 68 us, 2.2 TB/s; base and y without products would
+// meanwhile.  Bound: base and y, and the two-term products beside them: 2011 rows, N 6144, K 2048, rank 64: some 45 of the call's 61 to 68 us, 2.2 TB/s; base and y without products would
 // take 22.  (Several tiles a CTA with the matrix in shared memory and base fetched three tiles ahead: 73 us a call where this took 70; two CTAs an SM with more
 // loads on their way 74 against 68; four with 64 registers spill: 78.)
 constexpr int UP_R = 128;
@@ -369,7 +371,7 @@ int launch_add(dc_ctx* ctx, LoraParams p, int max_rank, int32_t* order) {
     }
     const int parts = parts_of(ctx, p.M, p.Kp);
     p.order = nullptr;
-    if (p.M <= LORA_SORTED) {      // (more rows than that are prompts' for the most part, which come in runs)
+    if (p.M <= LORA_SORTED) {
         DC_TRY(dc_launch(ctx, "k_lora_order", k_lora_order, dim3(1), dim3(LORA_SORTED), 0, p, order));
         p.order = order;
     }

@@ -10,10 +10,11 @@
 //   a cut by weight: a histogram of numbers (32-bit atomics; sums of 64 bits in shared memory took ten times as long) bounds the weights ahead of every bin from both
 //   sides, between which the cut lies;
 //   up to 1024 tokens down to there: they are sorted in one CTA, which applies all filters and draws;
-//   up to here all is bound by latency: one row of 151936 tokens 11.4 us, sixteen with settings of their own 27 us;
+//   up to here all is bound by latency: one row of 151936 tokens 10.9 us, sixteen with settings of their own 27 to 44 us, by the settings;
 //   else the bins between the bounds are refined until 1024 tokens or one value is left, and the part of the row with the draw is searched.
-// Bound for many rows by nucleus: issue slots (58 %) and waits for one another between passes over shared memory (weights twice, numbers once, the search): 256 bf16 rows with
-// their distributions 295 us, 790 GB/s.
+// Bound for many rows by nucleus: issue slots (58 %) and waits for one another between passes over shared memory (weights twice, numbers once, the search): 256 bf16 rows
+// 229 us, with their distributions 287 us, 810 GB/s.  By top-k 50 and top-p 0.95 90 and 139 us, by temperature alone 107 and 166.  Two CTAs of 512 threads an SM leave 64
+// registers a thread, of which 40 to 64 bytes spill.
 #include <cooperative_groups.h>
 #include <math.h>
 

@@ -229,7 +229,8 @@ DC_B200_API int dc_b200_kv_read_block(dc_kv_cache* kv, int layer, int block, voi
  * Head sizes 64 (36 bytes a row) and 128 (72).  n_head query heads share n_kv_head key heads evenly.  row_type: type
  * of queries, new rows and results, DC_GGML_TYPE_F32 or DC_GGML_TYPE_BF16; attention over F32 rows is exact to f32
  * rounding, over BF16 rows to bf16's: weights, and in portions of 64 rows or more (new tokens times query heads of a key head) values, have fp16's 11 bits on the
- * way, and what weighs less than 2^-25 of a row's largest weight (times scales; 2^-32 in such portions) may be lost.  All calls of the block manager above (sequences, fork, prefix cache, block
+ * way, and what weighs less than 2^-25 of a row's largest weight (both times their values' scales; F32 rows 2^-36; in such portions 2^-32 of the weight
+ * alone) may be lost.  All calls of the block manager above (sequences, fork, prefix cache, block
  * tables) serve such a cache; dc_b200_flash_attn_decode / _prefill and dc_b200_kv_read_block refuse it. */
 DC_B200_API int dc_b200_kv_create_q4(dc_ctx* ctx, int n_layer, int n_head, int n_kv_head, int head_dim, int row_type, int max_blocks, int max_seqs,
                                      int max_blocks_per_seq, dc_kv_cache** out);

@@ -119,3 +119,27 @@ int main() {
 """)
     r = run(exe)
     assert r.returncode == 0, r.stdout
+
+
+def test_a_cache_that_fails_to_be_made_leaves_nothing(tmp_path):
+    exe = program(tmp_path, ["attn_q4", "kv"], r"""
+#include "dc_kv.h"
+#include "dc_q4.h"
+int dc_launch_q4_prompt(dc_ctx*, const dc_q4_call&) { return 0; }
+int dc_launch_q4_join(dc_ctx*, const dc_q4_call&) { return 0; }
+int main() {
+    for (int n = 1;; ++n) {
+        dc_ctx ctx;
+        dc_kv_cache* kv = nullptr;
+        fake::calls = 0, fake::fail_at = n;
+        const int st = dc_b200_kv_create_q4(&ctx, 3, 8, 2, 64, DC_GGML_TYPE_F32, 60, 2, 40, &kv);
+        const bool failed = fake::calls >= n;
+        if (failed != (st != 0) || failed != !kv) return printf("call %d: status %d\n", n, st), 1;
+        dc_b200_kv_destroy(kv);
+        if (fake::bad_frees || !fake::live.empty()) return printf("call %d: %d freed twice, %d lost\n", n, fake::bad_frees, (int)fake::live.size()), 1;
+        if (!failed) return printf("%d calls\n", n - 1), 0;
+    }
+}
+""")
+    r = run(exe)
+    assert r.returncode == 0 and int(r.stdout.split()[0]) >= 6, r.stdout
