@@ -87,6 +87,7 @@ struct WriteParams {
     int ldkv, n_kv;
     uint8_t* arena;
     float *k_held, *v_held;      // [T][n_kv][HD], may be null
+    int few;                     // ahead of captured attention, which does not serve steps with prompt-sized entries: their rows may be more than its buffers hold
 };
 
 // rint(x / d) as the division rounds it, x within 16 d: by the reciprocal, and by the division itself where the product lies near a border
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(128) k_q4_write(const WriteParams p) {
     __shared__ uint8_t codes[4][2][HD];
     pdl_wait();
     pdl_launch_dependents();      // (not before the wait: what the next kernel reads ahead of its own wait has to be complete)
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = p.head->T * p.n_kv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, units = p.few && p.head->n_tiles > 0 ? 0 : p.head->T * p.n_kv;
     const dc_q4_token* tokens = p.tokens ? p.tokens : p.head->tokens;
     for (int u = blockIdx.x * 4 + warp; u < units; u += gridDim.x * 4) {
         const int t = u / p.n_kv, head = u - t * p.n_kv;
@@ -185,7 +186,6 @@ struct RowsParams {
     float scale;
     void* out;
     int early;      // dc_q4_call
-    int tiles;      // of the call: a replay on a plan with others would leave their rows out
     int* err;
 };
 
@@ -203,7 +203,7 @@ constexpr size_t rows_smem() { return (size_t)RW * RW_STAGES * dc_q4_rec<HD>::BY
 // f32 prompts run here too, eight rows at a time, each tile of rows through all pages that it sees: 2011 tokens, 32 query heads, 4 key heads 452 us where k_q4_prompt takes 59
 // on bf16 rows (its operands are fp16: f32 rows would need two terms of each).
 // A lane has row h = lane / 4 of the tile and tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a page (t = lane % 4).
-// CAPTURED: the arrays' places come from the header, and there may be more CTAs than items.
+// CAPTURED: the arrays' places come from the header, and there may be more CTAs than items.  A step with prompt-sized entries, which it does not serve, is reported.
 template <int HD, typename TX, bool CAPTURED>
 __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(const RowsParams p) {
     using R = dc_q4_rec<HD>;
@@ -228,8 +228,11 @@ __global__ void __launch_bounds__(RW * 32, sizeof(TX) == 2 ? 4 : 3) k_q4_rows(co
     pdl_launch_dependents();
     dc_q4_item im;
     if constexpr (!CAPTURED) im = p.items[blockIdx.x];      // (as many as CTAs: it need not wait for their number)
-    const int n_items = p.head->n_items;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && p.head->n_tiles > 0 && p.tiles == 0) atomicExch(p.err, DC_ERR_REPLAY);
+    int n_items = p.head->n_items;
+    if (CAPTURED && p.head->n_tiles > 0) {
+        n_items = 0;
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicExch(p.err, DC_ERR_REPLAY);
+    }
     uint32_t n_full = 0;      // pages that this warp has waited for
     for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
         if (CAPTURED || it != (int)blockIdx.x) im = (CAPTURED ? p.head->items : p.items)[it];
@@ -602,7 +605,7 @@ int launch_rows(dc_ctx* ctx, const dc_q4_call& c) {
     const dc_q4& z = *c.kv->q4;
     const auto kernel = c.captured ? k_q4_rows<HD, TX, true> : k_q4_rows<HD, TX, false>;
     DC_TRY(dc_kernel_setup(ctx, (const void*)kernel, (int)rows_smem<HD>(), "k_q4_rows"));
-    const RowsParams p = {z.head, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.early, z.n_tiles, ctx->d_err};
+    const RowsParams p = {z.head, (const dc_q4_item*)(z.plan + z.at[DC_Q4_ITEMS]), (int*)(z.plan + z.at[DC_Q4_TICKETS]), (float*)(z.plan + z.at[DC_Q4_WS]), c.q, c.ldq, c.ldo, z.heads, z.kv, c.kv->max_blocks_per_seq, c.kv->d_tables, c.arena, c.scale, c.out, c.early, ctx->d_err};
     // (a captured call's later plans may have more items: CTAs for all SMs)
     const int ctas = c.captured ? std::max(z.n_items, ((sizeof(TX) == 2 ? 4 : 3) * ctx->num_sms + z.kv - 1) / z.kv) : z.n_items;
     return dc_launch(ctx, "k_q4_rows", kernel, dim3(ctas, z.kv), dim3(RW * 32), rows_smem<HD>(), p);
@@ -744,9 +747,9 @@ int empty_step(dc_ctx* ctx, const char* name) {      // nothing to do; a capture
     return capturing(ctx) ? dc_fail(ctx, DC_B200_UNSUPPORTED, "%s: a step without tokens cannot be captured", name) : DC_B200_OK;
 }
 
-int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held, bool captured) {
+int write_rows(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k, const void* v, int ldkv, float* k_held, float* v_held, bool captured, bool few) {
     const dc_q4& z = *kv->q4;
-    const WriteParams p = {z.head, captured ? nullptr : (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), k, v, ldkv, z.kv, kv->planes[layer].arena, k_held, v_held};
+    const WriteParams p = {z.head, captured ? nullptr : (const dc_q4_token*)(z.plan + z.at[DC_Q4_TOKENS]), k, v, ldkv, z.kv, kv->planes[layer].arena, k_held, v_held, few};
     const int units = z.T * z.kv;
     if (z.dim == 128) return z.type == DC_TYPE_F32 ? launch_write<128, float>(ctx, p, units) : launch_write<128, __nv_bfloat16>(ctx, p, units);
     return z.type == DC_TYPE_F32 ? launch_write<64, float>(ctx, p, units) : launch_write<64, __nv_bfloat16>(ctx, p, units);
@@ -854,7 +857,7 @@ int dc_b200_kv_q4_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void*
     if (z.T == 0) return empty_step(ctx, "kv_q4_write_dev");
     if (!k_dev || !v_dev || ld_kv < z.kv * z.dim) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_q4_write_dev: bad argument (row stride %d)", ld_kv);
     cudaSetDevice(ctx->device);
-    return write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev, capturing(ctx));
+    return write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev, capturing(ctx), false);
 }
 
 int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_dev, int ld_q, const void* k_dev, const void* v_dev, int ld_kv, float scale,
@@ -871,7 +874,7 @@ int dc_b200_flash_attn_q4_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const voi
     if (z.n_tiles && captured) return dc_fail(ctx, DC_B200_UNSUPPORTED, "flash_attn_q4_dev: prompt-sized portions cannot be captured (their number of CTAs goes by the positions)");
     if (!isfinite(scale)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "flash_attn_q4_dev: scale is not finite");
     cudaSetDevice(ctx->device);
-    if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev, captured));
+    if (k_dev) DC_TRY(write_rows(ctx, kv, layer, k_dev, v_dev, ld_kv, k_held_dev, v_held_dev, captured, captured));
     dc_q4_call c = {kv, kv->planes[layer].arena, q_dev, ld_q, ld_out, scale, out_dev, k_dev ? 1 : 0, captured};
     DC_TRY(dc_launch_q4_prompt(ctx, c));
     if (z.n_tiles) c.early = 2;      // the SMs that prompt tiles leave idle take the single tokens meanwhile

@@ -242,7 +242,7 @@ DC_B200_API int dc_b200_kv_create_q4(dc_ctx* ctx, int n_layer, int n_head, int n
  * stream capture.  A call of dc_b200_kv_seq_free / _fork / _reserve / _prefix_* ends the step.  The calls below may
  * be captured into a graph while the step has tokens and no entry is prompt-sized (of BF16 rows, 64 or more new tokens times query heads of a
  * key head).  A replay, on the context's stream, works on the newest plan at that time, whatever its entries, their number and positions; the call's buffers have to hold
- * that step's rows, and it is subject to the same rules as a call.  On a plan with prompt-sized entries it leaves their rows out, which the next
+ * that step's rows, and it is subject to the same rules as a call.  On a plan with prompt-sized entries attention does nothing, which the next
  * dc_b200_synchronize reports. */
 DC_B200_API int dc_b200_kv_batch(dc_kv_cache* kv, int n_entries, const int32_t* seqs, const int32_t* pos0, const int32_t* counts);
 /* Writes the step's rows into one layer.  k_dev, v_dev: [T][n_kv_head][head_dim] rows ld_kv elements apart (0: dense),

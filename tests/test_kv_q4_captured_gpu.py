@@ -115,3 +115,47 @@ def test_captured_writes_alone(ctx, dtype):
             m.check_blocks(s)
             at += n
     del graph
+
+
+def test_a_step_that_a_capture_does_not_serve_leaves_cache_and_results(ctx):
+    """Prompt-sized entries beside a decoded token: rows behind those of the captured call are not read, nothing is written, and the status says so."""
+    rng = np.random.default_rng(4)
+    m = Mirror(ctx, "bf16", 8, 2, 128, 2, 40)
+    a, b = m.cache.seq_alloc(), m.cache.seq_alloc()
+    m.step(rng, [a, b], [0, 0], [100, 30])
+    q, k, v = (torch.full((60, h, 128), 3.0, device=GPU, dtype=torch.bfloat16) for h in (8, 2, 2))
+    out = torch.full_like(q, -7.0)
+    stream = torch.cuda.ExternalStream(dc._lib.lib().dc_b200_stream(ctx.handle))
+    m.cache.batch([b, a], [30, 100], [1, 1])
+    ctx.synchronize()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        m.cache.attend_dev(0, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0.1, out.data_ptr())
+    m.cache.batch([b, a], [30, 100], [1, 40])
+    half = torch.full((41, 2, 128), 0.5, device=GPU, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    m.cache.write_dev(0, half.data_ptr(), half.data_ptr())
+    ctx.synchronize()
+    with torch.cuda.stream(stream):
+        graph.replay()
+    with pytest.raises(dc.DcError) as e:
+        ctx.synchronize()
+    assert e.value.status == -6 and torch.all(out == -7.0)
+    for s, p, n in ((b, 30, 1), (a, 100, 40)):
+        for store in (m.k[0], m.v[0]):
+            store[s] = np.concatenate([store[s], np.full((n, 2, 128), 0.5, np.float32)])
+        m.check_blocks(s)
+    rows = m.rows(rng, 2)
+    m.cache.batch([b, a], [31, 140], [1, 1])
+    for to, x in zip((q, k, v), rows):
+        to[:2].copy_(_dev(x, "bf16"))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph.replay()
+    ctx.synchronize()
+    for i, (s, p) in enumerate(((b, 31), (a, 140))):
+        for store, x in ((m.k[0], rows[1]), (m.v[0], rows[2])):
+            store[s] = np.concatenate([store[s], held(x[i:i + 1])])
+        m.compare(out[i:i + 1].float().cpu().numpy(), rows[0][i:i + 1], s, p, 0.1)
+    del graph
