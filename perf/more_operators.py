@@ -406,9 +406,10 @@ def context():
 
 
 class On:
-    """An array of the library's as a tensor."""
+    """An array of the library's as a tensor, which keeps its owner."""
 
-    def __init__(self, address, shape):
+    def __init__(self, owner, address, shape):
+        self.owner = owner
         self.__cuda_array_interface__ = {"shape": shape, "typestr": "<i4", "data": (address, False), "version": 3}
 
 
@@ -419,7 +420,7 @@ def own_pool(s):
     kv.step_dev(s["before"].data_ptr(), max_count=s["max_count"])
     ctx.synchronize()
     at, n = kv.arrays(), case["slots"]
-    s["arrays"] = {k: torch.as_tensor(On(at[k], shape), device=GPU) for k, shape in
+    s["arrays"] = {k: torch.as_tensor(On(kv, at[k], shape), device=GPU) for k, shape in
                    {"lens": (n,), "counts": (n,), "starts": (n + 1,), "tables": (n, a_slot), "slots": (most,), "positions": (most,), "seqs": (most,), "free": (1,)}.items()}
     s["at"] = [(d.data_ptr(), c.data_ptr()) for d, c in s["steps"]]
 
