@@ -117,6 +117,7 @@ int dc_check_device_error(dc_ctx* ctx) {
     if (e != cudaSuccess) return dc_check_cuda(ctx, e, "reading device error word");
     if (err != 0) {
         cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream);
+        if (err == DC_ERR_STEP) return dc_fail(ctx, DC_B200_BACKEND_ERROR, "a captured attention call was replayed on a step with more new tokens of a sequence than its own allowed");
         if (err == DC_ERR_REPLAY) return dc_fail(ctx, DC_B200_BACKEND_ERROR, "a captured attention step was replayed on a batch with prompt-sized portions");
         return dc_fail(ctx, DC_B200_BACKEND_ERROR, "a kernel gave up a bounded wait (code %d)", err);
     }
@@ -170,6 +171,7 @@ void dc_b200_destroy(dc_ctx* ctx) {
         }
     }
     if (ctx->scratch) cudaFree(ctx->scratch);
+    if (ctx->verify_ws) cudaFree(ctx->verify_ws);
     if (ctx->pinned) cudaFreeHost(ctx->pinned);
     cudaFree(ctx->d_err);
     cudaStreamDestroy(ctx->stream);

@@ -30,6 +30,7 @@
 #define DC_WAIT_LIMIT (1u << 22)
 #define DC_ERR_MBAR_TIMEOUT 1
 #define DC_ERR_REPLAY 64   // a captured step met a plan that it does not serve
+#define DC_ERR_STEP 65     // attention met a step with more new tokens of a sequence than it was launched for
 
 namespace dc {
 

@@ -15,6 +15,7 @@ struct dc_kv_seq {
 };
 
 struct dc_q4;
+struct dc_kv_dev;
 struct dc_kv_cache {
     dc_ctx* ctx = nullptr;
     int n_layer = 0, n_kv = 0, head_dim = 0;
@@ -31,6 +32,7 @@ struct dc_kv_cache {
     uint8_t* state = nullptr;    // [max_seqs][state_bytes]
     size_t state_bytes = 0;
     struct dc_q4* q4 = nullptr;  // of a cache in 4 bits (planes of its layers)
+    struct dc_kv_dev* dev = nullptr;  // of a cache whose sequences are kept on the GPU (then all of the above is empty)
     uint64_t edits = 0;          // changes of sequences and their blocks
     std::vector<int> free_list;
     std::vector<int> ref;        // references per physical block (sequences sharing it after a fork)
@@ -52,6 +54,7 @@ int dc_kv_init_planes(dc_ctx* ctx, dc_kv_cache* kv, const std::vector<size_t>& r
                       int max_blocks_per_seq);
 void dc_kv_release(dc_kv_cache* kv);
 DC_PART void dc_q4_release(dc_kv_cache* kv);
+DC_PART void dc_kv_dev_release(dc_kv_cache* kv);
 int dc_kv_seq_alloc(dc_kv_cache* kv, int* out_seq);
 int dc_kv_seq_free(dc_kv_cache* kv, int seq);
 int dc_kv_seq_reserve(dc_kv_cache* kv, int seq, int n_tokens);

@@ -98,6 +98,7 @@ static int take_block(dc_kv_cache* kv) {
 
 void dc_kv_release(dc_kv_cache* kv) {
     if (dc_q4_release) dc_q4_release(kv);
+    if (dc_kv_dev_release) dc_kv_dev_release(kv);
     if (kv->k_arena) cudaFree(kv->k_arena);
     if (kv->v_arena) cudaFree(kv->v_arena);
     if (kv->d_tables) cudaFree(kv->d_tables);
@@ -111,6 +112,7 @@ void dc_kv_release(dc_kv_cache* kv) {
 }
 
 int dc_kv_seq_alloc(dc_kv_cache* kv, int* out_seq) {
+    if (kv->dev) return dc_fail(kv->ctx, DC_B200_UNSUPPORTED, "kv: the sequences of this cache are kept on the GPU (dc_b200_kv_step_dev)");
     for (int s = 0; s < kv->max_seqs; ++s) {
         if (!kv->seqs[s].used) {
             kv->seqs[s].used = true;
@@ -364,7 +366,7 @@ int dc_b200_kv_seq_fork(dc_kv_cache* kv, int src_seq, int* out_seq) {
 int dc_b200_kv_block_refcount(dc_kv_cache* kv, int block) {
     return (kv && block >= 0 && block < kv->max_blocks) ? kv->ref[block] : DC_B200_INVALID_ARGUMENT;
 }
-int dc_b200_kv_free_blocks(dc_kv_cache* kv) { return kv ? dc_kv_available_blocks(kv) : DC_B200_INVALID_ARGUMENT; }
+int dc_b200_kv_free_blocks(dc_kv_cache* kv) { return kv && !kv->dev ? dc_kv_available_blocks(kv) : DC_B200_INVALID_ARGUMENT; }
 int dc_b200_kv_prefix_attach(dc_kv_cache* kv, int seq, const int32_t* tokens, int n_tokens, int* cached_tokens) {
     if (!kv || !cached_tokens) return DC_B200_INVALID_ARGUMENT;
     cudaSetDevice(kv->ctx->device);

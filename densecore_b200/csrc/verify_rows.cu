@@ -1,0 +1,496 @@
+// Verification of the drafted tokens of many requests, and each one's next token, from given uniform numbers (no counterpart in DenseCore; the rule is dc_b200_verify_accept's).
+//
+//   p_i = softmax(x_i / T) (or given), draft i is accepted if u_i q_i(t_i) < p_i(t_i) and all before it are; with n accepted, the next token is the first, by index, up to which the
+//   sum of r = max(0, p_n - q_n) (of p_n behind the last draft, or where r is nothing) is above u_last times the whole
+//
+// k_verify_stats (logits alone): the rows' maxima and sums of weights, a row cut into parts where there are few; one pass.  k_verify_next: every CTA of a request decides
+// n from those for itself, then sums r over its part of row n in tiles of 2048 tokens; the last CTA of the request finds the tile that the draw falls into, and
+// in it the token.  So a row that is accepted is read once, and the one drawn from twice (the second time largely from L2).
+// Weights are 2^((x - max) log2(e) / T) in f32 (2^-22), sums in 64 bits, in an order that does not depend on timing.
+#include <math.h>
+
+#include <algorithm>
+
+#include "dc_common.cuh"
+#include "dc_internal.h"
+#include "dc_launch.cuh"
+
+using namespace dc;
+
+#define DC_TRY(expr)                       \
+    do {                                   \
+        int _st = (expr);                  \
+        if (_st != DC_B200_OK) return _st; \
+    } while (0)
+
+namespace {
+
+constexpr int VR_T = 256, VR_PER = 8, VR_TILE = VR_T * VR_PER, VR_DRAFTS = 64, VR_VOCAB = 389120, VR_TILES = VR_VOCAB / VR_TILE, VR_ROWS = 65536;
+constexpr int VR_STATS_CTAS = 16, VR_NEXT_CTAS = 4;      // an SM, where rows are cut into parts
+constexpr int VR_PROBS = -1;
+
+struct alignas(16) Stat {      // of a part of a row
+    double sum;      // of weights against the part's maximum
+    float most;
+    int first;       // index of the first largest
+};
+
+struct VerifyParams {
+    const void* target;
+    size_t ld;
+    int rows, V, R, D, parts, part_tiles;      // tiles of a part
+    const int32_t *starts, *n_drafts, *tokens;
+    const float *q, *temperature, *u;
+    int32_t *out, *accepted, *rejected;
+    Stat* stats;                               // [request][row][stat_parts]
+    int stat_parts;
+    double* sums;                              // [request][tile], where a request has several CTAs
+    int32_t* tickets;
+};
+
+// Drafts of a request and its first row; false: it takes no part.
+__device__ __forceinline__ bool request(const VerifyParams& p, int r, int& n, int& row0) {
+    n = p.n_drafts ? min(p.n_drafts[r], p.D) : p.D;
+    row0 = p.starts ? p.starts[r] : r * (p.D + 1);
+    return n >= 0 && row0 >= 0 && (long long)row0 + n < p.rows;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float value(float x) { return x; }
+__device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// log2(e) / T in two terms.  Differences are held to 1e35, at which a weight is 0 for every scale from 1e-30 on: so NaN and -inf have none, and no product overflows.
+struct Scale {
+    float hi, lo;
+    bool greedy;
+    __device__ __forceinline__ explicit Scale(float T) {
+        greedy = !(T > 0.0f);
+        const double c = greedy ? 1.0 : fmin(fmax(1.4426950408889634 / (double)T, 1e-30), 1e30);
+        hi = (float)c, lo = c < 1e10 ? (float)(c - (double)hi) : 0.0f;
+    }
+    __device__ __forceinline__ float operator()(float x, float most) const {      // x at or below `most`, which is finite
+        const float d = fmaxf(x - most, -1e35f);
+        return ex2(fmaf(d, hi, d * lo));
+    }
+};
+__device__ __forceinline__ float weight_inf(float x) { return x == INFINITY ? 1.0f : 0.0f; }      // beside an infinite largest
+
+// Eight neighbouring values of a row from index i on; `none` behind its end.
+template <typename TX>
+__device__ __forceinline__ void load8(const TX* row, int i, int V, float none, float (&x)[8]) {
+    if (i + 8 <= V && ((uintptr_t)(row + i) & 15) == 0) {
+        if constexpr (sizeof(TX) == 2) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + i));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[2 * k] = __uint_as_float(w[k] << 16), x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+        } else {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(row + i)), b = __ldg(reinterpret_cast<const float4*>(row + i) + 1);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = i + k < V ? value(row[i + k]) : none;
+    }
+}
+
+// Two parts of a row as one: sums against the larger maximum, the first largest.
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, const Scale& c) {
+    Stat s;
+    s.most = fmaxf(a.most, b.most);
+    s.first = a.most == b.most ? min(a.first, b.first) : a.most > b.most ? a.first : b.first;
+    // (the weight of a maximum against itself is 1, also of an infinite one; beside that others have none)
+    const float f = a.most == b.most ? 1.0f : s.most == INFINITY ? 0.0f : c(fminf(a.most, b.most), s.most);
+    s.sum = a.most == s.most ? a.sum + b.sum * (double)f : a.sum * (double)f + b.sum;
+    return s;
+}
+__device__ __forceinline__ Stat warp_join(Stat s, const Scale& c) {
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) {
+        Stat o;
+        o.sum = __shfl_xor_sync(0xffffffffu, s.sum, k), o.most = __shfl_xor_sync(0xffffffffu, s.most, k), o.first = __shfl_xor_sync(0xffffffffu, s.first, k);
+        s = join(s, o, c);      // (the same for both lanes: sums of two are commutative)
+    }
+    return s;
+}
+
+// One CTA per (row, part).  Bound: HBM for many rows.
+template <typename TX>
+__global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
+    constexpr int B = 4;      // tiles on their way at once
+    __shared__ Stat warps[VR_T / 32];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int unit = blockIdx.x / p.stat_parts, part = blockIdx.x % p.stat_parts, r = unit / (p.D + 1), i = unit % (p.D + 1);
+    int n, row0;
+    if (!request(p, r, n, row0) || i > n) return;
+    const TX* row = reinterpret_cast<const TX*>(p.target) + (size_t)(row0 + i) * p.ld;
+    const Scale c(p.temperature ? p.temperature[r] : 1.0f);
+    const int tiles = (p.V + VR_TILE - 1) / VR_TILE, first = part * ((tiles + p.stat_parts - 1) / p.stat_parts), last = min(tiles, first + (tiles + p.stat_parts - 1) / p.stat_parts);
+    float most = -INFINITY;
+    int where = 0x7fffffff;
+    double sum = 0.0;
+    for (int t0 = first; t0 < last; t0 += B) {
+        float x[B][8];
+#pragma unroll
+        for (int b = 0; b < B; ++b) load8(row, t0 + b < last ? (t0 + b) * VR_TILE + VR_PER * (int)threadIdx.x : p.V, p.V, -INFINITY, x[b]);
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, x[b][k]);
+        if (top > most) {
+            sum = most > -INFINITY && top < INFINITY ? sum * (double)c(most, top) : 0.0;
+            most = top;
+            where = 0x7fffffff;
+#pragma unroll
+            for (int b = B - 1; b >= 0; --b)
+#pragma unroll
+                for (int k = 7; k >= 0; --k)
+                    if (x[b][k] == top) where = (t0 + b) * VR_TILE + VR_PER * (int)threadIdx.x + k;
+        }
+        if (!(top > -INFINITY)) continue;      // nothing with a weight
+        float s[B] = {};
+        if (most == INFINITY) {
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[b] += weight_inf(x[b][k]);
+        } else {
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[b] += c(x[b][k], most);
+        }
+        sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+    }
+    Stat s;
+    s.sum = sum, s.most = most, s.first = where;
+    s = warp_join(s, c);
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x / 32] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < VR_T / 32; ++w) s = join(s, warps[w], c);
+        p.stats[(size_t)unit * p.stat_parts + part] = s;
+    }
+}
+
+// Exclusive sum over the CTA's threads.
+__device__ __forceinline__ double scan(double v, double* warps, double& all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double in = v;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, in, s);
+        if (lane >= s) in += o;
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = in;
+    __syncthreads();
+    double before = 0.0;
+    all = 0.0;
+#pragma unroll
+    for (int w = 0; w < VR_T / 32; ++w) {
+        if (w == warp) before = all;
+        all += warps[w];
+    }
+    const double ex = __shfl_up_sync(0xffffffffu, in, 1);
+    return before + (lane ? ex : 0.0);
+}
+
+// One CTA per (request, part of the row drawn from).  Bound: HBM for many requests (the row and its draft's probabilities, once; the draw's own tile again), latency for few: the rows'
+// statistics, the decisions, the part, the ticket and the draw's tile one after the other.
+template <typename TX, bool PROBS>
+__global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
+    __shared__ Stat rows[VR_DRAFTS + 1];
+    __shared__ int s_good[VR_DRAFTS], s_n, s_tile, s_last, s_token, s_at_most;
+    __shared__ double s_sums[VR_TILES], s_warps[VR_TILES][VR_T / 32], s_total, s_before;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int r = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int n, row0;
+    if (!request(p, r, n, row0)) {
+        if (part == 0) {
+            for (int i = tid; i <= p.D; i += VR_T) p.out[(size_t)r * (p.D + 1) + i] = -1;
+            if (tid == 0) {
+                p.accepted[r] = 0;
+                if (p.rejected) p.rejected[r] = 0;
+            }
+        }
+        return;
+    }
+    const TX* target = reinterpret_cast<const TX*>(p.target) + (size_t)row0 * p.ld;
+    const Scale c(PROBS ? 1.0f : p.temperature ? p.temperature[r] : 1.0f);
+    if constexpr (!PROBS) {
+        for (int i = warp; i <= n; i += VR_T / 32) {
+            Stat s;
+            s.sum = 0.0, s.most = -INFINITY, s.first = 0x7fffffff;
+            const Stat* from = p.stats + ((size_t)r * (p.D + 1) + i) * p.stat_parts;
+            for (int k = lane; k < p.stat_parts; k += 32) {
+                Stat o;
+                const int4 v = __ldcg(reinterpret_cast<const int4*>(from + k));
+                o.sum = __hiloint2double(v.y, v.x), o.most = __int_as_float(v.z), o.first = v.w;
+                s = join(s, o, c);
+            }
+            s = warp_join(s, c);
+            if (lane == 0) rows[i] = s;
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += VR_T) {
+        const int t = p.tokens[(size_t)i * p.R + r];
+        bool good = false;
+        if (t >= 0 && t < p.V) {
+            float q = p.q ? p.q[((size_t)i * p.R + r) * p.V + t] : 1.0f;
+            if (!(q > 0.0f && q <= 3.4028235e38f)) q = 0.0f;
+            const float x = value(target[(size_t)i * p.ld + t]);
+            const double uq = (double)p.u[(size_t)r * (p.D + 1) + i] * (double)q;
+            if constexpr (PROBS) {
+                good = uq < (x > 0.0f && x <= 3.4028235e38f ? (double)x : 0.0);
+            } else {
+                const Stat& s = rows[i];
+                if (s.most > -INFINITY)
+                    good = c.greedy ? uq < (t == s.first ? 1.0 : 0.0) : uq * s.sum < (double)(s.most == INFINITY ? weight_inf(x) : c(x, s.most));
+            }
+        }
+        s_good[i] = good;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int k = 0;
+        while (k < n && s_good[k]) ++k;
+        s_n = k;
+    }
+    __syncthreads();
+    // ---- what is drawn from, of eight neighbouring tokens
+    const int k = s_n, own = k < n ? p.tokens[(size_t)k * p.R + r] : -1;
+    const TX* row = target + (size_t)k * p.ld;
+    const float* qrow = k < n && p.q ? p.q + ((size_t)k * p.R + r) * p.V : nullptr;
+    Stat st;
+    st.sum = 1.0, st.most = 0.0f, st.first = 0;
+    if constexpr (!PROBS) st = rows[k];
+    const float inv = (float)(1.0 / st.sum);
+    const bool none = !PROBS && !(st.most > -INFINITY);
+    auto drawn_from = [&](int i, bool residual, float (&w)[8]) {
+        float q[8];
+        load8(row, i, p.V, PROBS ? 0.0f : -INFINITY, w);
+        if (residual && qrow) load8(qrow, i, p.V, 0.0f, q);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            if constexpr (PROBS) w[x] = w[x] > 0.0f && w[x] <= 3.4028235e38f ? w[x] : 0.0f;
+            else if (none) w[x] = 0.0f;
+            else if (c.greedy) w[x] = i + x == st.first ? 1.0f : 0.0f;
+            else w[x] = (st.most == INFINITY ? weight_inf(w[x]) : c(w[x], st.most)) * inv;
+            if (residual) {
+                if (qrow) {
+                    if (q[x] > 0.0f && q[x] <= 3.4028235e38f) w[x] = fmaxf(w[x] - q[x], 0.0f);
+                } else if (i + x == own) {
+                    w[x] = fmaxf(w[x] - 1.0f, 0.0f);
+                }
+            }
+        }
+    };
+    auto sum_of = [](const float (&w)[8]) {
+        double s = 0.0;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) s += (double)w[x];
+        return s;
+    };
+    const int tiles = (p.V + VR_TILE - 1) / VR_TILE, from = part * p.part_tiles, to = min(tiles, from + p.part_tiles);
+    auto sum_tiles = [&](int from, int to, bool residual) {      // every warp's share of each tile
+        for (int t = from; t < to; ++t) {
+            float w[8];
+            drawn_from(t * VR_TILE + VR_PER * tid, residual, w);
+            double s = sum_of(w);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            if (lane == 0) s_warps[t][warp] = s;
+        }
+        __syncthreads();
+    };
+    auto tile_sum = [&](int t) {
+        double s = 0.0;
+#pragma unroll
+        for (int w = 0; w < VR_T / 32; ++w) s += s_warps[t][w];
+        return s;
+    };
+    const float u = p.u[(size_t)r * (p.D + 1) + p.D], uc = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+    auto find_tile = [&]() {      // to everyone: the tile that the draw falls into, the sums ahead of it, the whole
+        __syncthreads();
+        if (warp == 0) {
+            const int per = (tiles + 31) / 32, a = min(tiles, lane * per), b = min(tiles, a + per);
+            double own = 0.0;
+            int last = -1;
+            for (int t = a; t < b; ++t) {
+                own += s_sums[t];
+                if (s_sums[t] > 0.0) last = t;
+            }
+            double upto = own;
+#pragma unroll
+            for (int x = 1; x < 32; x <<= 1) {
+                const double o = __shfl_up_sync(0xffffffffu, upto, x);
+                if (lane >= x) upto += o;
+            }
+            const double total = __shfl_sync(0xffffffffu, upto, 31), goal = (double)uc * total;
+            last = __reduce_max_sync(0xffffffffu, last);
+            const uint32_t there = __ballot_sync(0xffffffffu, upto > goal);
+            if (lane == (there ? __ffs(there) - 1 : 31)) {
+                double before = upto - own;
+                int t = a;
+                for (; t < b && !(before + s_sums[t] > goal); ++t) before += s_sums[t];
+                if (t >= b) {      // (rounding: the last tile with a weight)
+                    t = max(last, 0);
+                    before = 0.0;
+                    for (int x = 0; x < t; ++x) before += s_sums[x];
+                }
+                s_tile = t, s_before = before, s_total = total;
+            }
+        }
+        __syncthreads();
+    };
+    sum_tiles(from, to, k < n);
+    for (int t = from + tid; t < to; t += VR_T) {
+        const double s = tile_sum(t);
+        if (p.parts == 1) s_sums[t] = s;
+        else p.sums[(size_t)r * tiles + t] = s;
+    }
+    if (p.parts > 1) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            s_last = atomicAdd(p.tickets + r, 1) == p.parts - 1;
+            if (s_last) p.tickets[r] = 0;
+            __threadfence();
+        }
+        __syncthreads();
+        if (!s_last) return;
+        for (int t = tid; t < tiles; t += VR_T) s_sums[t] = __ldcg(p.sums + (size_t)r * tiles + t);
+    }
+    bool residual = k < n;
+    find_tile();
+    if (residual && !(s_total > 0.0)) {      // the draft is nowhere below the target: from the target itself
+        residual = false;
+        sum_tiles(0, tiles, false);
+        for (int t = tid; t < tiles; t += VR_T) s_sums[t] = tile_sum(t);
+        find_tile();
+    }
+    if (tid == 0) s_token = 0x7fffffff, s_at_most = -1;
+    __syncthreads();
+    if (s_total > 0.0) {
+        float w[8];
+        const int i0 = s_tile * VR_TILE + VR_PER * tid;
+        drawn_from(i0, residual, w);
+        double all, upto = scan(sum_of(w), s_warps[0], all);
+        const double goal = (double)uc * s_total - s_before;
+        int found = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            upto += (double)w[x];
+            if (w[x] > 0.0f) last = i0 + x;
+            if (upto > goal && w[x] > 0.0f) found = min(found, i0 + x);
+        }
+        found = __reduce_min_sync(0xffffffffu, found), last = __reduce_max_sync(0xffffffffu, last);
+        if (lane == 0) atomicMin(&s_token, found), atomicMax(&s_at_most, last);
+    }
+    __syncthreads();
+    const int token = s_token < p.V ? s_token : s_at_most;      // (rounding: the tile's last with a weight)
+    for (int i = tid; i <= p.D; i += VR_T) p.out[(size_t)r * (p.D + 1) + i] = i < k ? p.tokens[(size_t)i * p.R + r] : i == k ? token : -1;
+    if (tid == 0) {
+        p.accepted[r] = k;
+        if (p.rejected) p.rejected[r] = n - k;
+    }
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+template <typename TX, bool PROBS>
+int launch(dc_ctx* ctx, const VerifyParams& p) {
+    if constexpr (!PROBS)
+        DC_TRY(dc_launch(ctx, "k_verify_stats", k_verify_stats<TX>, dim3(p.R * (p.D + 1) * p.stat_parts), dim3(VR_T), 0, p));
+    return dc_launch(ctx, "k_verify_next", k_verify_next<TX, PROBS>, dim3(p.R * p.parts), dim3(VR_T), 0, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64_t ld, int rows, int vocab, int n_requests, int max_drafts, const int32_t* starts_dev,
+                            const int32_t* n_drafts_dev, const int32_t* draft_tokens_dev, const float* draft_probs_dev, const float* temperature_dev, const float* uniforms_dev,
+                            int32_t* tokens_dev, int32_t* accepted_dev, int32_t* rejected_dev) {
+    if (!ctx) return DC_B200_INVALID_ARGUMENT;
+    if (ld == 0) ld = vocab;
+    if (rows < 0 || vocab < 1 || ld < vocab || n_requests < 0 || max_drafts < 0)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: bad shape (%d requests of %d drafts, %d rows of %d, stride %lld)", n_requests, max_drafts, rows, vocab, (long long)ld);
+    if (type != DC_TYPE_F32 && type != DC_TYPE_BF16 && type != VR_PROBS)
+        return dc_fail(ctx, DC_B200_UNSUPPORTED, "verify_rows: rows of type %d (F32 and BF16 logits and f32 probabilities, -1, are supported)", type);
+    if (vocab > VR_VOCAB || max_drafts > VR_DRAFTS || (long long)n_requests * (max_drafts + 1) > VR_ROWS)
+        return dc_fail(ctx, DC_B200_UNSUPPORTED, "verify_rows: %d requests of %d drafts, %d tokens", n_requests, max_drafts, vocab);
+    if (n_requests == 0) return DC_B200_OK;
+    if (!target_dev || (max_drafts && !draft_tokens_dev) || !uniforms_dev || !tokens_dev || !accepted_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: null buffer");
+    if ((uintptr_t)target_dev % (type == DC_TYPE_BF16 ? 2 : 4) || (uintptr_t)draft_probs_dev % 4) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: a buffer is not aligned to its elements");
+    cudaSetDevice(ctx->device);
+    // rows are cut into parts where there are fewer than fill the GPU
+    const int tiles = (vocab + VR_TILE - 1) / VR_TILE, n_rows = n_requests * (max_drafts + 1), stat_ctas = VR_STATS_CTAS * ctx->num_sms, next_ctas = VR_NEXT_CTAS * ctx->num_sms;
+    int stat_parts = std::min(tiles, (stat_ctas + n_rows - 1) / n_rows), parts = std::min(tiles, (next_ctas + n_requests - 1) / n_requests);
+    const int part_tiles = (tiles + parts - 1) / parts;
+    parts = (tiles + part_tiles - 1) / part_tiles;
+    // a workspace of one size, which graphs that hold calls may go on using
+    const size_t stats = align256((size_t)(VR_ROWS + stat_ctas) * sizeof(Stat)), sums = align256((size_t)next_ctas * VR_TILES * sizeof(double)), tickets = align256((size_t)next_ctas * 4);
+    if (!ctx->verify_ws) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone)
+            return dc_fail(ctx, DC_B200_UNSUPPORTED, "verify_rows: a context's first call cannot be captured");
+        void* ws = nullptr;
+        DC_TRY(dc_check_cuda(ctx, cudaMalloc(&ws, stats + sums + tickets), "verify_rows: workspace"));
+        const cudaError_t e = cudaMemsetAsync((uint8_t*)ws + stats + sums, 0, tickets, ctx->stream);
+        if (e != cudaSuccess) {
+            cudaFree(ws);
+            return dc_check_cuda(ctx, e, "verify_rows: workspace");
+        }
+        ctx->verify_ws = (uint8_t*)ws;
+    }
+    const VerifyParams p = {target_dev, (size_t)ld, rows, vocab, n_requests, max_drafts, parts, part_tiles, starts_dev, n_drafts_dev, draft_tokens_dev, draft_probs_dev, temperature_dev,
+                            uniforms_dev, tokens_dev, accepted_dev, rejected_dev, (Stat*)ctx->verify_ws, stat_parts, (double*)(ctx->verify_ws + stats), (int32_t*)(ctx->verify_ws + stats + sums)};
+    return type == VR_PROBS ? launch<float, true>(ctx, p) : type == DC_TYPE_F32 ? launch<float, false>(ctx, p) : launch<__nv_bfloat16, false>(ctx, p);
+}
+
+int dc_b200_verify_rows(dc_ctx* ctx, const float* target_host, int n_requests, int vocab, int max_drafts, const int32_t* n_drafts, const int32_t* draft_tokens, const float* draft_probs,
+                        const float* temperature, int probs, const float* uniforms, int32_t* tokens_out, int32_t* accepted_out) {
+    if (!ctx) return DC_B200_INVALID_ARGUMENT;
+    if (!target_host || n_requests < 1 || vocab < 1 || max_drafts < 0 || (max_drafts && !draft_tokens) || !uniforms || !tokens_out || !accepted_out)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: bad argument");
+    if (vocab > VR_VOCAB || max_drafts > VR_DRAFTS || (long long)n_requests * (max_drafts + 1) > VR_ROWS)
+        return dc_fail(ctx, DC_B200_UNSUPPORTED, "verify_rows: %d requests of %d drafts, %d tokens", n_requests, max_drafts, vocab);
+    const size_t rows = (size_t)n_requests * (max_drafts + 1);
+    for (size_t i = 0; i < rows; ++i)
+        if (!(uniforms[i] >= 0.0f && uniforms[i] < 1.0f)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: uniform number %zu is out of range", i);
+    for (int r = 0; r < n_requests; ++r)
+        if ((temperature && !(temperature[r] >= 0.0f)) || (n_drafts && (n_drafts[r] < 0 || n_drafts[r] > max_drafts)))
+            return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: request %d has a setting out of range", r);
+    cudaSetDevice(ctx->device);
+    const size_t target = rows * vocab * 4, drafts = (size_t)n_requests * max_drafts, q = draft_probs ? drafts * vocab * 4 : 0;
+    uint8_t* at = dc_scratch(ctx, align256(target) + align256(q) + 6 * align256(rows * 4));
+    if (!at) return DC_B200_OUT_OF_MEMORY;
+    int st = DC_B200_OK;
+    auto up = [&](const void* from, size_t n) -> uint8_t* {      // (pageable sources: the copy is done with them when it returns)
+        uint8_t* to = at;
+        at += align256(n);
+        if (from && n && st == DC_B200_OK) st = dc_check_cuda(ctx, cudaMemcpyAsync(to, from, n, cudaMemcpyHostToDevice, ctx->stream), "verify_rows");
+        return from ? to : nullptr;
+    };
+    const uint8_t *x = up(target_host, target), *pq = up(draft_probs, q), *t = up(draft_tokens, drafts * 4), *nd = up(n_drafts, (size_t)n_requests * 4),
+                  *temp = up(temperature, (size_t)n_requests * 4), *u = up(uniforms, rows * 4);
+    DC_TRY(st);
+    int32_t *tokens = (int32_t*)at, *accepted = (int32_t*)(at + align256(rows * 4));
+    DC_TRY(dc_b200_verify_rows_dev(ctx, x, probs ? VR_PROBS : DC_TYPE_F32, 0, (int)rows, vocab, n_requests, max_drafts, nullptr, (const int32_t*)nd, (const int32_t*)t, (const float*)pq,
+                                   (const float*)temp, (const float*)u, tokens, accepted, nullptr));
+    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(tokens_out, tokens, rows * 4, cudaMemcpyDeviceToHost, ctx->stream), "verify_rows"));
+    DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(accepted_out, accepted, (size_t)n_requests * 4, cudaMemcpyDeviceToHost, ctx->stream), "verify_rows"));
+    return dc_b200_synchronize(ctx);
+}
+
+}  // extern "C"

@@ -234,6 +234,36 @@ class Context:
         self._check(_lib.lib().dc_b200_sample_rows(self.handle, _vp(logits), rows, vocab, *(_vp(x) for x in s), _vp(tokens), _vp(p), _vp(dist)))
         return (tokens, p, dist) if want_dist else (tokens, p)
 
+    def verify_rows_dev(self, target: int, requests: int, vocab: int, max_drafts: int, draft_tokens: int, draft_probs: int, uniforms: int, tokens: int, accepted: int, rejected: int = 0,
+                        starts: int = 0, n_drafts: int = 0, temperature: int = 0, rows: int = 0, ld: int = 0, dtype: str = "f32", probs: bool = False):
+        """Drafted tokens of many requests against device-resident rows of the target (logits, or probabilities); all device addresses, enqueue only."""
+        self._check(_lib.lib().dc_b200_verify_rows_dev(self.handle, _dev(target), -1 if probs else _row_type(dtype), ld, rows or requests * (max_drafts + 1), vocab, requests, max_drafts,
+                                                       _dev(starts), _dev(n_drafts), _dev(draft_tokens), _dev(draft_probs), _dev(temperature), _dev(uniforms), _dev(tokens), _dev(accepted),
+                                                       _dev(rejected)))
+
+    def verify_rows(self, target: np.ndarray, draft_tokens, draft_probs, uniforms, n_drafts=None, temperature=None, probs: bool = False):
+        """The same on host arrays: target [requests, drafts + 1, vocab], draft_tokens [drafts, requests], draft_probs [drafts, requests, vocab] or None, uniforms
+        [requests, drafts + 1].  Returns (tokens [requests, drafts + 1], accepted [requests])."""
+        target = np.ascontiguousarray(target, dtype=np.float32)
+        if target.ndim != 3:
+            raise ValueError(f"target rows of shape {target.shape}; [requests, drafts + 1, vocab] are wanted")
+        R, D, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+
+        def of(x, t, shape):
+            if x is None:
+                return None
+            x = np.asarray(x, dtype=t)
+            if x.shape != shape:
+                raise ValueError(f"an array of shape {x.shape} where {shape} is wanted")
+            return np.ascontiguousarray(x)
+
+        a = [of(draft_tokens, np.int32, (D, R)), of(draft_probs, np.float32, (D, R, V)),
+             of(None if temperature is None else np.broadcast_to(np.asarray(temperature, dtype=np.float32), (R,)), np.float32, (R,)), of(uniforms, np.float32, (R, D + 1))]
+        n = of(n_drafts, np.int32, (R,))
+        tokens, accepted = np.zeros((R, D + 1), dtype=np.int32), np.zeros(R, dtype=np.int32)
+        self._check(_lib.lib().dc_b200_verify_rows(self.handle, _vp(target), R, V, D, _vp(n), _vp(a[0]), _vp(a[1]), _vp(a[2]), int(probs), _vp(a[3]), _vp(tokens), _vp(accepted)))
+        return tokens, accepted
+
     # ---- adapters
     def lora(self, K: int, N: int, max_adapters: int, max_rank: int, dtype: str = "bf16") -> "LoraSet":
         """Low-rank adapters of a matrix of N x K; dtype: type of their matrices ("bf16", "f16")."""
@@ -256,6 +286,12 @@ class Context:
                     dtype: str = "f32") -> "KVCacheQ4":
         """Cache in 4 bits for layers of n_head query heads; dtype: rows of queries, keys, values and results ("f32", "bf16")."""
         return KVCacheQ4(self, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, dtype)
+
+
+    def kv_cache_dev(self, n_layer: int, n_head: int, n_kv_head: int, head_dim: int, max_blocks: int, max_seqs: int, max_blocks_per_seq: int, max_tokens: int,
+                     dtype: str = "bf16") -> "KVCacheDev":
+        """Cache of 16-bit rows whose sequences are kept on the GPU; dtype: rows of queries, keys, values and results ("f32": held as f16, "bf16", "f16")."""
+        return KVCacheDev(self, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, max_tokens, dtype)
 
 
 class LoraSet:
@@ -428,4 +464,63 @@ class KVCacheQ4(KVCache):
         k = np.zeros((16, self.n_kv, self.head_dim), dtype=np.float32)
         v = np.zeros_like(k)
         self.ctx._check(_lib.lib().dc_b200_kv_q4_read_block(self.handle, layer, block, _vp(k), _vp(v)))
+        return k, v
+
+
+class KVCacheDev:
+    """Paged cache of 16-bit rows whose sequences' lengths, pages and tables are device memory (dc_b200_kv_create_dev)."""
+
+    ARRAYS = ("lens", "counts", "starts", "tables", "slots", "positions", "seqs", "free")
+
+    def __init__(self, ctx: Context, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, max_tokens, dtype="bf16"):
+        self.handle = None
+        self.ctx, self.n_layer, self.n_head, self.n_kv, self.head_dim, self.dtype = ctx, n_layer, n_head, n_kv_head, head_dim, dtype
+        self.max_seqs, self.max_blocks_per_seq, self.max_tokens = max_seqs, max_blocks_per_seq, max_tokens
+        h = C.c_void_p()
+        ctx._check(_lib.lib().dc_b200_kv_create_dev(ctx.handle, n_layer, n_head, n_kv_head, head_dim, _row_type(dtype), max_blocks, max_seqs, max_blocks_per_seq, max_tokens, C.byref(h)))
+        self.handle = h
+
+    def close(self):
+        if self.handle:
+            _lib.lib().dc_b200_kv_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self.ctx.handle:
+                self.close()
+        except Exception:
+            pass
+
+    def arrays(self) -> dict:
+        """Device addresses of the sequences' arrays (all int32); they hold for the cache's life."""
+        a = (C.c_void_p * len(self.ARRAYS))()
+        self.ctx._check(_lib.lib().dc_b200_kv_dev_arrays(self.handle, a))
+        return dict(zip(self.ARRAYS, (int(x) for x in a)))
+
+    def read(self, name: str) -> np.ndarray:
+        """One of those arrays on the host."""
+        S = self.max_seqs
+        shape = {"lens": S, "counts": S, "starts": S + 1, "tables": (S, self.max_blocks_per_seq), "free": 1}.get(name, self.max_tokens)
+        self.ctx.synchronize()
+        return self.ctx.from_device(self.arrays()[name], np.empty(shape, dtype=np.int32))
+
+    def step_dev(self, count: int, drop: int = 0, max_count: int = 1):
+        """A step: every sequence loses its last drop[s] tokens and gets count[s] new ones (device addresses, 0: none), at most max_count; enqueue only."""
+        self.ctx._check(_lib.lib().dc_b200_kv_step_dev(self.ctx.handle, self.handle, _dev(drop), _dev(count), max_count))
+
+    def write_dev(self, layer: int, k: int, v: int, ld: int = 0):
+        """Writes the step's rows (device addresses) into one layer, enqueue only."""
+        self.ctx._check(_lib.lib().dc_b200_kv_dev_write_dev(self.ctx.handle, self.handle, layer, _dev(k), _dev(v), ld))
+
+    def attend_dev(self, layer: int, q: int, k: int, v: int, scale: float, out: int, window: int = 0, keep_first: int = 0, ld_q: int = 0, ld_kv: int = 0, ld_out: int = 0):
+        """Writes the step's rows (k = v = 0: they stand there already), then attends, over all earlier positions or the last `window` and the first `keep_first`;
+        device addresses, enqueue only."""
+        self.ctx._check(_lib.lib().dc_b200_flash_attn_kv_dev(self.ctx.handle, self.handle, layer, _dev(q), ld_q, _dev(k), _dev(v), ld_kv, scale, window, keep_first, _dev(out), ld_out))
+
+    def read_page(self, layer: int, page: int):
+        """The rows of one page, K and V, [16, n_kv, hd]: float16, or bits (uint16) of bf16."""
+        k = np.zeros((16, self.n_kv, self.head_dim), dtype=np.uint16 if self.dtype == "bf16" else np.float16)
+        v = np.zeros_like(k)
+        self.ctx._check(_lib.lib().dc_b200_kv_dev_read_page(self.handle, layer, page, _vp(k), _vp(v)))
         return k, v

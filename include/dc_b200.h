@@ -261,6 +261,46 @@ DC_B200_API int dc_b200_flash_attn_q4(dc_ctx* ctx, dc_kv_cache* kv, int layer, c
 /* The values that one block of one layer stands for: f32 [16][n_kv_head][head_dim] each (either may be NULL). */
 DC_B200_API int dc_b200_kv_q4_read_block(dc_kv_cache* kv, int layer, int block, float* k_host, float* v_host);
 
+/* ---- paged KV cache whose sequences are kept on the GPU + attention over it ----- */
+/* A cache of 16-bit rows for steps that follow one another without the host, as a run of speculative steps in a CUDA graph (no counterpart in
+ * DenseCore).  Slot s of max_seqs is a sequence; its length, pages and block table are device memory and change by dc_b200_kv_step_dev alone: pages are
+ * not shared, and the block manager's calls above refuse such a cache (dc_b200_kv_destroy takes it).  Head sizes 64 and 128; n_head query heads share
+ * n_kv_head key heads evenly.  row_type: type of queries, new rows and results, DC_GGML_TYPE_F32 (held as F16; what lies beyond F16's range becomes
+ * infinite), _F16 or _BF16.  At most 4096 sequences.  max_tokens: new tokens of a step at most, of all sequences together. */
+DC_B200_API int dc_b200_kv_create_dev(dc_ctx* ctx, int n_layer, int n_head, int n_kv_head, int head_dim, int row_type, int max_blocks, int max_seqs,
+                                      int max_blocks_per_seq, int max_tokens, dc_kv_cache** out);
+/* Device addresses that hold for the cache's life, to be read by the caller's kernels; written by dc_b200_kv_step_dev.  A step's new tokens lie sequence
+ * after sequence, by rising slot.  What lies behind a table's pages or behind the step's tokens is left as it was. */
+typedef struct dc_kv_dev_arrays {
+    const int32_t* lens;      /* [max_seqs] tokens of each sequence, the step's new ones included */
+    const int32_t* counts;    /* [max_seqs] the step's new tokens of each */
+    const int32_t* starts;    /* [max_seqs + 1] the step's new tokens ahead of each sequence's, and all */
+    const int32_t* tables;    /* [max_seqs][max_blocks_per_seq] pages */
+    const int32_t* slots;     /* [max_tokens] place in the cache of each new token: 16 page + place in the page */
+    const int32_t* positions; /* [max_tokens] position of each new token in its sequence */
+    const int32_t* seqs;      /* [max_tokens] its sequence */
+    const int32_t* free;      /* [1] free pages */
+} dc_kv_dev_arrays;
+DC_B200_API int dc_b200_kv_dev_arrays(dc_kv_cache* kv, struct dc_kv_dev_arrays* out);
+/* A step: every sequence loses its last drop_dev[s] tokens (NULL or below 0: none; all, where it has fewer: it is then empty) and gets count_dev[s] new ones
+ * (NULL: none).  A sequence frees the pages that it then needs no more, or asks for those it lacks.  Refused, and so without new tokens (counts says 0), is one
+ * that asks for less than 0 or more than max_count tokens or than its table holds; of the others those for whose pages the free ones and the freed ones do not
+ * suffice, by the sum of all that is asked for up to them, by rising slot; and those with which the sum of new tokens is above max_tokens.  A refused one
+ * keeps the pages that it would have used.  The j-th page granted, by rising slot and place, is the j-th one freed, and behind those the newest free one.  Only
+ * enqueues, may be captured; a replay is a step of its own.  What max_count says holds for the calls below up to the next step: a replayed
+ * one has to find a step of no more. */
+DC_B200_API int dc_b200_kv_step_dev(dc_ctx* ctx, dc_kv_cache* kv, const int32_t* drop_dev, const int32_t* count_dev, int max_count);
+/* Writes the step's rows into one layer: k_dev, v_dev [tokens][n_kv_head][head_dim], rows ld_kv elements apart (0: dense).  Only enqueues, may be captured. */
+DC_B200_API int dc_b200_kv_dev_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k_dev, const void* v_dev, int64_t ld_kv);
+/* Writes the step's rows (k_dev and v_dev both NULL: they stand there already), then attends: the token at position p of a sequence over its positions k <= p; with
+ * window > 0 over those of them with k > p - window or k < keep_first (window 0: all).  q_dev, out_dev: [tokens][n_head][head_dim], rows ld_q and ld_out
+ * elements apart (0: dense), any alignment of the elements' own size; out_dev must not overlap the inputs.  Rows behind the step's last token are left as they
+ * were.  A value that is infinite or NaN reaches no row that does not see it; one that is seen may make infinity NaN.  Only enqueues, may be captured. */
+DC_B200_API int dc_b200_flash_attn_kv_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_dev, int64_t ld_q, const void* k_dev, const void* v_dev, int64_t ld_kv, float scale,
+                                          int window, int keep_first, void* out_dev, int64_t ld_out);
+/* The rows of one page of one layer, in the type they are held in: [16][n_kv_head][head_dim] each (either may be NULL). */
+DC_B200_API int dc_b200_kv_dev_read_page(dc_kv_cache* kv, int layer, int block, void* k_host, void* v_host);
+
 /* ---- sampling / speculative verify ----------------------------------------- */
 /* Greedy pick, first maximum wins (ArgmaxScalar, core/src/sampler/sampler.cpp:42-57). */
 DC_B200_API int dc_b200_argmax(dc_ctx* ctx, const float* logits_host, int rows, int n, int32_t* out_ids);
@@ -311,6 +351,28 @@ DC_B200_API int dc_b200_sample_rows_dev(dc_ctx* ctx, const void* logits_dev, int
 DC_B200_API int dc_b200_sample_rows(dc_ctx* ctx, const float* logits_host, int rows, int vocab, const float* temperature, const int32_t* top_k,
                                     const float* top_p, const float* min_p, const float* uniforms, int32_t* tokens_out, float* p_out,
                                     float* dist_out);
+
+/* Verification of the drafted tokens of many requests at once, the answers left on the GPU (the rule of dc_b200_verify_accept).  Request r has n_drafts_dev[r]
+ * drafts (NULL: max_drafts; more are taken as max_drafts; below 0: the request takes no part) and that many rows of the target plus one from row starts_dev[r] on
+ * (NULL: r (max_drafts + 1)): row i is the target's behind the tokens ahead of draft i.  A request whose rows do not lie within the `rows` rows takes no part.
+ * target_dev: rows of vocab numbers ld elements apart (0: dense); type DC_GGML_TYPE_F32 or DC_GGML_TYPE_BF16: logits, p = softmax(logits / temperature), a temperature that
+ * is not above 0 (temperature_dev [n_requests], NULL: 1) puts all on the first largest; type -1: f32 probabilities as they are, of any sum, e.g. dc_b200_sample_rows_dev's dist behind
+ * top-k and top-p (what is not above 0 or not finite counts as 0).  -inf and NaN among logits have no weight.
+ * draft_tokens_dev [max_drafts][n_requests] and draft_probs_dev [max_drafts][n_requests][vocab], as max_drafts calls of dc_b200_sample_rows_dev leave them (draft_probs_dev
+ * NULL: all of q on the drafted token).  uniforms_dev [n_requests][max_drafts + 1] in [0, 1).  Draft i is accepted if u_i q_i(t_i) < p_i(t_i) and all
+ * before it are; a drafted token outside the vocabulary is not.  The next token is drawn from max(0, p - q) at the first draft that is not accepted (from p where that is
+ * nothing), from p behind the last: the first token, by index, up to which the sum is above the request's last uniform number times the whole; -1 if nothing has a weight.
+ * Results: tokens_dev [n_requests][max_drafts + 1]: the accepted ones, the next one, -1 behind it; accepted_dev [n_requests]; rejected_dev [n_requests] (may be NULL): drafts not accepted,
+ * what dc_b200_kv_step_dev takes as drop_dev.  A request without part: tokens -1, both 0.  At most 64 drafts, 389120 tokens of vocabulary, 65536 rows n_requests (max_drafts + 1).  Weights are f32 (2^-22), sums 64
+ * bits in an order of their own, the same every time.  Only enqueues; a context's first call makes its workspace (of some MB, whatever the call's sizes) and cannot be
+ * captured. */
+DC_B200_API int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64_t ld, int rows, int vocab, int n_requests, int max_drafts, const int32_t* starts_dev,
+                                        const int32_t* n_drafts_dev, const int32_t* draft_tokens_dev, const float* draft_probs_dev, const float* temperature_dev,
+                                        const float* uniforms_dev, int32_t* tokens_dev, int32_t* accepted_dev, int32_t* rejected_dev);
+/* The same on host arrays (dense f32 rows [n_requests][max_drafts + 1][vocab]; probabilities where `probs` is not 0); refuses settings out of range: temperature below 0, n_drafts outside
+ * 0 .. max_drafts, uniforms outside [0, 1), NaN. */
+DC_B200_API int dc_b200_verify_rows(dc_ctx* ctx, const float* target_host, int n_requests, int vocab, int max_drafts, const int32_t* n_drafts, const int32_t* draft_tokens,
+                                    const float* draft_probs, const float* temperature, int probs, const float* uniforms, int32_t* tokens_out, int32_t* accepted_out);
 
 /* ---- low-rank adapters beside a shared product -------------------------------- */
 /* A set of adapters of one matrix [N, K] for many requests at once (no counterpart in DenseCore): slot a holds A [rank, K]
