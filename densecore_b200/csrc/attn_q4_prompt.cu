@@ -266,9 +266,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(QP_P, 2 * u + (t & 1)));      // (two barriers: a warp may be done with the next tile before another is with this one)
             }
-            // (phase by phase: the parity of the last alone also stands for the one before the last but one; tile t's scores come behind phase t - 2)
-            if (ok && n_tiles > 1) ok = wait(bar(QP_O, u), (n_tiles - 2) & 1);
-            if (ok) ok = wait(bar(QP_O, u), (n_tiles - 1) & 1);
+            if (ok) ok = wait(bar(QP_DRAIN, u), 0);      // (a barrier of its own: of two phases of the tiles' one, both of which may be complete, the first cannot be told from the next)
             if (ok) {
                 tc_fence_after();
                 const float l = l_run[0] + l_run[1];
@@ -457,6 +455,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1) k_q4_prompt(const PromptParams 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) umma_f16_ts(t_unit + 128, w + 8 * i, v + 2 * i, id_o, 1);
                 umma_commit(bar(QP_O, u));
+                if (t == n_tiles - 1) umma_commit(bar(QP_DRAIN, u));
                 umma_commit(bar(QP_FREE, t % QP_STAGES));
             }
         };

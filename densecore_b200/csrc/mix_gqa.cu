@@ -894,7 +894,7 @@ __global__ void __launch_bounds__(2 * PQ, PQ == 128 ? 2 : 1) k_gqa_prompt(const 
 constexpr int TP_Q = 128, TP_STAGES = 4, TP_THREADS = 13 * 32;
 constexpr uint32_t TP_QHEAD = TP_Q * 256, TP_TILE = PK * 256;      // a head's queries, keys or values of a tile: two halves of 64 columns
 constexpr uint32_t TP_KV = 2 * TP_QHEAD, TP_BARS = TP_KV + TP_STAGES * 2 * TP_TILE;
-enum TpBar { TP_FULL = 0, TP_FREE = 4, TP_S = 8, TP_P = 12, TP_O = 16, TP_DRAIN = 18, TP_NBARS };
+enum TpBar { TP_FULL = 0, TP_FREE = 4, TP_S = 8, TP_P = 12, TP_O = 16, TP_DRAIN = 18, TP_DONE = 19, TP_NBARS = 21 };
 constexpr size_t TP_SMEM = TP_BARS + TP_NBARS * 8 + 1024;
 
 template <bool SIGMOID>
@@ -1037,9 +1037,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) k_gqa_prompt_tc(const PromptPar
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(TP_P, 2 * u + (t & 1)));      // (two barriers: a warp may be done with the next tile before another is with this one)
         }
-        // (phase by phase: the parity of the last alone also stands for the one before the last but one; tile t's scores come behind phase t - 2)
-        if (ok && n_tiles > 1) ok = wait(bar(TP_O, u), (n_tiles - 2) & 1);
-        if (ok) ok = wait(bar(TP_O, u), (n_tiles - 1) & 1);
+        if (ok) ok = wait(bar(TP_DONE, u), 0);      // (a barrier of its own: of two phases of the tiles' one, both of which may be complete, the first cannot be told from the next)
         if (ok) {
             tc_fence_after();
             const bool in = q0 + row < n;
@@ -1124,6 +1122,7 @@ __global__ void __launch_bounds__(TP_THREADS, 1) k_gqa_prompt_tc(const PromptPar
                     for (int i = 0; i < 4; ++i) umma_f16_ts_lanes(d, w + 8 * i, v + (16 * 128 * i) / 16, id_o, 1, off);
                 }
                 umma_commit(bar(TP_O, u));
+                if (t == n_tiles - 1) umma_commit(bar(TP_DONE, u));
             }
         };
         const int window = p.window > 0 ? p.window : 0x7fffffff;
