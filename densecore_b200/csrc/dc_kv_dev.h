@@ -34,8 +34,8 @@ struct dc_kv_dev {
     dc_kv_entry* entries = nullptr;
     uint8_t* memory = nullptr;     // all of the above but the arena
     // of attention: partial results and tickets of sequences that several CTAs work on (zero between calls)
-    float* parts = nullptr;
-    int32_t* tickets = nullptr;
+    float *parts = nullptr, *prompt_parts = nullptr;
+    int32_t *tickets = nullptr, *prompt_tickets = nullptr;
 };
 enum { DC_KV_FREE = 0, DC_KV_ENTRIES = 1, DC_KV_NUMBERS = 4 };
 
@@ -55,3 +55,5 @@ struct dc_kv16_call {
 };
 int dc_launch_kv16_write(dc_ctx* ctx, const dc_kv_cache* kv, uint8_t* arena, const void* k, const void* v, int64_t ld, bool prompts_only);
 int dc_launch_kv16_rows(dc_ctx* ctx, const dc_kv16_call& c, bool prompts);
+int dc_launch_kv16_prompt(dc_ctx* ctx, const dc_kv16_call& c);      // prompt-sized sequences of 16-bit rows
+size_t dc_kv16_prompt_parts(int num_sms, int n_kv, int dim);        // bytes of its partial results

@@ -300,15 +300,16 @@ int create(dc_ctx* ctx, dc_kv_cache* kv) {
     };
     const size_t slots4 = (size_t)z.slots * 4, tokens4 = (size_t)z.max_tokens * 4;
     const size_t lens = room(slots4), held = room(slots4), counts = room(slots4), starts = room(slots4 + 4), tables = room(slots4 * z.pages_per_seq), map = room(tokens4), positions = room(tokens4),
-                 seqs = room(tokens4), numbers = room(DC_KV_NUMBERS * 4), entries = room(slots4 * 4), tickets = room((size_t)ctas * z.kv * 4), stack = room((size_t)z.pages * 4), zeroed = at,
-                 parts = room((size_t)2 * ctas * z.kv * dc_kv16_rows(z.type) * (z.dim + 2) * 4);
+                 seqs = room(tokens4), numbers = room(DC_KV_NUMBERS * 4), entries = room(slots4 * 4), tickets = room((size_t)ctas * z.kv * 4), prompt_tickets = room((size_t)ctx->num_sms * 4), stack = room((size_t)z.pages * 4), zeroed = at,
+                 parts = room((size_t)2 * ctas * z.kv * dc_kv16_rows(z.type) * (z.dim + 2) * 4),
+                 prompt_parts = room(z.type == DC_TYPE_F32 ? 0 : dc_kv16_prompt_parts(ctx->num_sms, z.kv, z.dim));
     DC_TRY(dc_check_cuda(ctx, cudaMalloc(&z.arena, bytes), "kv_create_dev"));
     DC_TRY(dc_check_cuda(ctx, cudaMalloc(&z.memory, at), "kv_create_dev"));
     DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.arena, 0, bytes, ctx->stream), "kv_create_dev"));
     DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.memory, 0, zeroed, ctx->stream), "kv_create_dev"));
     auto ints = [&](size_t from) { return (int32_t*)(z.memory + from); };
     z.lens = ints(lens), z.held = ints(held), z.counts = ints(counts), z.starts = ints(starts), z.tables = ints(tables), z.slot_map = ints(map), z.positions = ints(positions), z.seqs = ints(seqs);
-    z.numbers = ints(numbers), z.entries = (dc_kv_entry*)(z.memory + entries), z.tickets = ints(tickets), z.stack = ints(stack), z.parts = (float*)(z.memory + parts);
+    z.numbers = ints(numbers), z.entries = (dc_kv_entry*)(z.memory + entries), z.tickets = ints(tickets), z.prompt_tickets = ints(prompt_tickets), z.stack = ints(stack), z.parts = (float*)(z.memory + parts), z.prompt_parts = (float*)(z.memory + prompt_parts);
     k_kv_stack<<<std::min((z.pages + 255) / 256, ctx->num_sms * 4), 256, 0, ctx->stream>>>(z.stack, z.pages);
     DC_TRY(dc_check_cuda(ctx, cudaGetLastError(), "k_kv_stack"));
     const int32_t free_pages = z.pages;
@@ -432,7 +433,7 @@ int dc_b200_flash_attn_kv_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const voi
     const dc_kv16_call c = {kv, z.arena + z.layer_bytes * layer, q_dev, k_dev, v_dev, ld_q, ld_kv, ld_out, scale, window, keep_first, out_dev};
     if ((long long)z.max_count * (z.heads / z.kv) > dc_kv16_rows(z.type)) {      // sequences with more rows than a CTA takes: their rows are written ahead of all
         if (k_dev) DC_TRY(dc_launch_kv16_write(ctx, kv, c.arena, k_dev, v_dev, ld_kv, true));
-        DC_TRY(dc_launch_kv16_rows(ctx, c, true));
+        DC_TRY(z.type == DC_TYPE_F32 ? dc_launch_kv16_rows(ctx, c, true) : dc_launch_kv16_prompt(ctx, c));
     }
     return dc_launch_kv16_rows(ctx, c, false);
 }

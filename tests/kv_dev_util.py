@@ -132,13 +132,16 @@ class Mirror:
     def compare(self, out, q, layer, window, keep, scale):
         """Row by row against 64 bits.  What a result may be off by, of the weighted sum A of its values' sizes: twice the relative error of a weight, and of f32 sums over as many
         steps of sixteen keys.  A weight's: that of its score (queries in two fp16 terms, 2^-22 of the row's largest, where rows are f32; f32 sums of HD products, 2^-21 of their sizes), of exp2
-        (2^-21) and of its two terms (fp16 2^-22, bf16 2^-18).  Then its own rounding."""
+        (2^-21) and of its two terms (fp16 2^-22, bf16 2^-18).  Then its own rounding.
+        Sequences of more than 64 rows of 16 bits have weights of one term (fp16 2^-12, bf16 2^-9), whose sum is that of the rounded ones: weights w (1 + d) with |d| <= 2^-9 give
+        sum w (1 + d) (v - y) / sum w (1 + d) off y, which is at most 2^-9 (A + |y|) and 2^-18 of that, so twice 2^-9 of A as |y| <= A."""
         out, q = out.double().numpy(), q.double().numpy()
-        terms = 2.0**-17 if self.dtype == "bf16" else 2.0**-20
         eps = torch.finfo(TYPES[self.dtype]).eps / 2
         G, t = self.heads // self.n_kv, 0
         for s, n in enumerate(self.steps.counts):
             K, V = self.k[layer][s], self.v[layer][s]
+            one = n * G > 64
+            terms = {"f32": 2.0**-20, "f16": 2.0**-11.99 if one else 2.0**-20, "bf16": 2.0**-8.99 if one else 2.0**-17}[self.dtype]
             for p in range(self.steps.lens[s] - n, self.steps.lens[s]):
                 at = np.arange(p + 1)
                 at = at[(at > p - window) | (at < keep)] if window else at
