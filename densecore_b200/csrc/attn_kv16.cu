@@ -17,7 +17,7 @@
 
 #include "dc_common.cuh"
 #include "dc_internal.h"
-#include "dc_kv_dev.h"
+#include "dc_kv16_tiles.cuh"
 #include "dc_launch.cuh"
 
 using namespace dc;
@@ -31,7 +31,7 @@ using namespace dc;
 namespace {
 
 constexpr int KR_WARPS = 4, KR_SLOTS = 8;      // page places of a CTA, shared out among the groups of warps that take pages in turn
-constexpr int KR_LEAST = 16;                   // pages of a CTA at least
+constexpr int KR_LEAST = 16, KR_EVEN = 48;     // pages of a CTA at least; at most, where sequences are cut into parts alike
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -96,24 +96,79 @@ struct RowsParams {
     int32_t* tickets;
     int part_floats;            // of a part
     bool all;                   // nobody else takes sequences with more rows: one is an error
+    const float* prompt_parts;  // of prompt-sized ones, to be added up: k_kv16_prompt of the same call, whose CTAs have begun, is the kernel before (else null)
+    int num_sms;
     int* err;
 };
 
-// Pages that new tokens j0 .. j1 of an entry see, numbered: the first `kept` ones, then those from `low` on.
-struct Pages {
-    int kept, low, n;
-    __device__ __forceinline__ int at(int i) const { return i < kept ? i : low + i - kept; }
-};
-__device__ __forceinline__ Pages pages_of(int first, int last, int window, int keep) {      // positions of the first and the last token
-    Pages g;
-    g.low = window ? max(0, first - window + 1) / DC_KV_BLOCK : 0;
-    g.kept = min((int)(((long long)keep + DC_KV_BLOCK - 1) / DC_KV_BLOCK), g.low);
-    g.n = g.kept + last / DC_KV_BLOCK - g.low + 1;
-    return g;
-}
-
 template <int HD>
 constexpr size_t rows_smem() { return (size_t)KR_SLOTS * dc_kv16_rec<HD>::BYTES + KR_SLOTS * 8 + 1024; }
+
+// The parts of prompt-sized sequences' rows whose keys were split, in their order: a warp per JR rows, a lane HD / 32 dimensions.
+template <int HD, typename TX>
+__device__ __forceinline__ void join_prompts(const RowsParams& p, int n_entries, int G) {
+    constexpr int D = HD / 32, JR = 4;
+    const int lane = threadIdx.x & 31;
+    const TileLine tiles(p.entries, n_entries, G, 64, p.n_kv, p.num_sms);
+    if (tiles.most == 1) return;
+    const size_t step = (size_t)p.n_kv * kp_part_floats<HD>();
+    const int warps = gridDim.x * gridDim.y * KR_WARPS, units = tiles.n_all * p.n_kv * (KP_TILE_ROWS / JR);
+    for (int x = (blockIdx.y * gridDim.x + blockIdx.x) * KR_WARPS + (threadIdx.x >> 5); x < units; x += warps) {
+        const int r0 = x % (KP_TILE_ROWS / JR) * JR, kvh = x / (KP_TILE_ROWS / JR) % p.n_kv, line = x / (KP_TILE_ROWS / JR) / p.n_kv;
+        const Tile tl(tiles, line, p.window, p.keep);
+        if (tl.n_parts == 1 || r0 >= tl.rows) continue;
+        const float* from = p.prompt_parts + ((size_t)line * tiles.most * p.n_kv + kvh) * kp_part_floats<HD>();
+        float M[JR], sum[JR], v[JR][D];
+#pragma unroll
+        for (int b = 0; b < JR; ++b) {
+            M[b] = -3e38f, sum[b] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[b][d] = 0.0f;
+        }
+#pragma unroll 2
+        for (int i = 0; i < tl.n_parts; ++i) {
+            float2 ml[JR];
+            float y[JR][D];
+#pragma unroll
+            for (int b = 0; b < JR; ++b) {
+                const float* at = from + (size_t)i * step + (size_t)min(r0 + b, tl.rows - 1) * (HD + 4);
+                ml[b] = __ldcg(reinterpret_cast<const float2*>(at + HD));
+                if constexpr (D == 4) {
+                    const float4 f = __ldcg(reinterpret_cast<const float4*>(at) + lane);
+                    y[b][0] = f.x, y[b][1] = f.y, y[b][2] = f.z, y[b][3] = f.w;
+                } else {
+                    const float2 f = __ldcg(reinterpret_cast<const float2*>(at) + lane);
+                    y[b][0] = f.x, y[b][1] = f.y;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < JR; ++b) {
+                const float m = fmaxf(M[b], ml[b].x), f0 = ex2(M[b] - m), f1 = ex2(ml[b].x - m);
+                M[b] = m, sum[b] = fmaf(sum[b], f0, ml[b].y * f1);
+#pragma unroll
+                for (int d = 0; d < D; ++d) v[b][d] = fmaf(v[b][d], f0, y[b][d] * f1);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < JR; ++b) {
+            if (r0 + b >= tl.rows) continue;
+            const float inv = 1.0f / sum[b];
+            const int rr = tl.row0 + r0 + b, j = rr / G;
+            TX* to = reinterpret_cast<TX*>(p.out) + (size_t)(tl.e.tok0 + j) * p.ldo + (size_t)(kvh * G + rr - j * G) * HD + D * lane;
+            struct alignas(D * sizeof(TX)) Piece {
+                TX x[D];
+            } y;
+#pragma unroll
+            for (int d = 0; d < D; ++d) y.x[d] = from_f32<TX>(v[b][d] * inv);
+            if (((uintptr_t)to & (sizeof(Piece) - 1)) == 0) {
+                *reinterpret_cast<Piece*>(to) = y;
+            } else {
+#pragma unroll
+                for (int d = 0; d < D; ++d) to[d] = y.x[d];
+            }
+        }
+    }
+}
 
 // PROMPTS: tiles of 32 NT rows of the sequences that have more, each whole by one CTA; else sequences of up to 32 NT rows, their pages shared out.
 template <int HD, typename TX, typename TC, int NT, bool PROMPTS>
@@ -136,7 +191,8 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         mbar_fence_init();
     }
     __syncthreads();
-    pdl_wait();
+    // (behind k_kv16_prompt, which has waited for all before it and shares nothing with this one's sequences, the SMs that it leaves idle take them meanwhile)
+    if (!p.prompt_parts) pdl_wait();
     pdl_launch_dependents();
     const int n_entries = p.numbers[DC_KV_ENTRIES];
     // ---- the line of work: entries' pages (tiles), a warp of entries at a time
@@ -153,18 +209,35 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         mine = weigh(own);
         if (!PROMPTS && p.all && (long long)own.count * G > RT) atomicExch(p.err, DC_ERR_STEP);
     };
-    int work = 0;
+    int work = 0, n_with = 0;
     for (int base = 0; base < n_entries; base += 32) {
         look_at(base);
-        work += mine;
+        work += mine, n_with += mine > 0;
     }
-    work = __reduce_add_sync(0xffffffffu, work);
-    const int share = PROMPTS ? 1 : max(KR_LEAST, (int)(((long long)work + gridDim.x - 1) / gridDim.x));
-    int at = PROMPTS ? (int)blockIdx.x : (int)min((long long)work, (long long)blockIdx.x * share);
-    const int end = PROMPTS ? work : min(work, at + share);
+    work = __reduce_add_sync(0xffffffffu, work), n_with = __reduce_add_sync(0xffffffffu, n_with);
+    // few pages: every CTA has one part of one sequence, all of a sequence's alike, so that nobody does two chains of loads one after the other; many: equal shares of the
+    // line, which end within a sequence where they may
+    const int ctas = gridDim.x;
+    int share = max(KR_LEAST, (int)(((long long)work + ctas - 1) / ctas));
+    bool even = false;
+    if (!PROMPTS && 2 * n_with <= ctas) {
+        const int s = max(KR_LEAST, (int)(((long long)work + ctas - n_with - 1) / (ctas - n_with)));
+        even = s <= KR_EVEN;
+        if (even) share = s;
+    }
+    int at = PROMPTS || even ? (int)blockIdx.x : (int)min((long long)work, (long long)blockIdx.x * share);
+    int end = PROMPTS ? work : even ? at + 1 : min(work, at + share);      // (even: of the parts' line, whose length is at most that of the grid)
+    if (even) {
+        int parts = 0;
+        for (int base = 0; base < n_entries; base += 32) {
+            if (base != chunk) look_at(base);
+            parts += (mine + share - 1) / share;
+        }
+        end = min(end, __reduce_add_sync(0xffffffffu, parts));
+    }
     auto begin_line = [&](int base) {
         if (base != chunk) look_at(base);
-        upto = mine;
+        upto = even ? (mine + share - 1) / share : mine;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
             const int o = __shfl_up_sync(0xffffffffu, upto, s);
@@ -183,11 +256,12 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         const int who = __ffs(there) - 1;
         const int seq = __shfl_sync(0xffffffffu, own.seq, who), pos0 = __shfl_sync(0xffffffffu, own.pos0, who), count = __shfl_sync(0xffffffffu, own.count, who),
                   tok0 = __shfl_sync(0xffffffffu, own.tok0, who);
-        const int e_end = __shfl_sync(0xffffffffu, upto, who), e_work = __shfl_sync(0xffffffffu, mine, who), e_at = e_end - e_work;
+        const int e_end = __shfl_sync(0xffffffffu, upto, who), e_work = __shfl_sync(0xffffffffu, mine, who), e_parts = (e_work + share - 1) / share, e_at = e_end - (even ? e_parts : e_work);
         // ---- the item: rows from row0 on, pages page0 .. page1 - 1 of those that they see
         const int row0 = PROMPTS ? (at - e_at) * RT : 0, rows = min(RT, count * G - row0), j_last = (row0 + rows - 1) / G;
         const Pages pages = pages_of(pos0 + row0 / G, pos0 + j_last, p.window, p.keep);
-        const int page0 = PROMPTS ? 0 : at - e_at, page1 = PROMPTS ? pages.n : min(end, e_end) - e_at;
+        const int page0 = PROMPTS ? 0 : even ? (int)((long long)e_work * (at - e_at) / e_parts) : at - e_at;
+        const int page1 = PROMPTS ? pages.n : even ? (int)((long long)e_work * (at - e_at + 1) / e_parts) : min(end, e_end) - e_at;
         const int tiles = (rows + RW - 1) / RW, WM = tiles <= 1 ? 1 : tiles <= 2 ? 2 : 4, WK = KR_WARPS / WM, depth = KR_SLOTS / WK;
         const int grp = warp / WM, r0 = row0 + (warp % WM) * RW, n_my = (page1 - page0 - grp + WK - 1) / WK;
         const int32_t* table = p.tables + (size_t)seq * p.pages_per_seq;
@@ -434,7 +508,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         }
         __syncthreads();
         // ---- the groups' parts joined: a thread has four neighbouring dimensions of a row at a time
-        const int c_first = PROMPTS ? 0 : e_at / share, n_parts = PROMPTS ? 1 : (e_end - 1) / share - c_first + 1, my_part = PROMPTS ? 0 : (int)blockIdx.x - c_first;
+        const int c_first = PROMPTS ? 0 : even ? e_at : e_at / share, n_parts = PROMPTS ? 1 : even ? e_parts : (e_end - 1) / share - c_first + 1, my_part = PROMPTS ? 0 : (int)blockIdx.x - c_first;
         const bool alone = n_parts == 1;
         auto place = [&](int i) -> float* {      // part i of the sequence
             const int c = c_first + i;
@@ -513,6 +587,12 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         __syncthreads();
         at = PROMPTS ? at + (int)gridDim.x : min(end, e_end);
     }
+    if constexpr (NT == 2 && !PROMPTS) {
+        if (p.prompt_parts) {
+            pdl_wait();
+            join_prompts<HD, TX>(p, n_entries, G);
+        }
+    }
 }
 
 template <int HD, typename TX, typename TC, int NT, bool PROMPTS>
@@ -538,6 +618,7 @@ int dc_launch_kv16_rows(dc_ctx* ctx, const dc_kv16_call& c, bool prompts) {
     const dc_kv_dev& z = *c.kv->dev;
     const long long rows = (long long)z.max_count * (z.heads / z.kv);
     const RowsParams p = {z.entries, z.numbers, z.tables, z.pages_per_seq, z.heads, z.kv, c.q, c.k, c.v, c.ldq, c.ldkv, c.ldo, c.arena, c.scale, c.window, c.keep, c.out, z.parts, z.tickets,
-                          dc_kv16_rows(z.type) * (z.dim + 2), rows <= dc_kv16_rows(z.type), ctx->d_err};
+                          dc_kv16_rows(z.type) * (z.dim + 2), rows <= dc_kv16_rows(z.type), z.type != DC_TYPE_F32 && !prompts && rows > dc_kv16_rows(z.type) ? z.prompt_parts : nullptr,
+                          ctx->num_sms, ctx->d_err};
     return z.dim == 128 ? launch_type<128>(ctx, c, p, prompts, rows <= 8) : launch_type<64>(ctx, c, p, prompts, rows <= 8);
 }

@@ -12,6 +12,7 @@
 // rounding, of a sum of many.  fp16 ones are 2^7 at the largest, down to 2^-31 of it.
 // A value that is infinite or NaN in a tile of which some row does not see all enters it as 0, or the products would carry it to rows that do not see it; rows that do see
 // it are NaN in that dimension.
+// Keys are split over CTAs where there are fewer tiles of rows than SMs; the rows kernel, which follows, adds the parts up.
 #include <math.h>
 
 #include <algorithm>
@@ -19,7 +20,7 @@
 
 #include "dc_common.cuh"
 #include "dc_internal.h"
-#include "dc_kv_dev.h"
+#include "dc_kv16_tiles.cuh"
 #include "dc_launch.cuh"
 #include "dc_tcgen05.cuh"
 
@@ -73,10 +74,9 @@ struct PromptParams {
     int window, keep;
     void* out;
     float* parts;
-    int32_t* tickets;
 };
 
-constexpr int KP_ROWS = 128, KP_KEYS = 64, KP_STAGES = 4, KP_THREADS = 12 * 32;
+constexpr int KP_KEYS = 64, KP_STAGES = 4, KP_THREADS = 12 * 32;
 enum KpBar { KP_FULL = 0, KP_PRE = 4, KP_FREE = 8, KP_S = 12, KP_P = 16, KP_O = 20, KP_DRAIN = 22, KP_QUERY = 24, KP_NBARS = 25 };
 template <int HD>
 struct Lay {
@@ -84,9 +84,6 @@ struct Lay {
     static constexpr uint32_t KV = 2 * SET, BAD = KV + KP_STAGES * 2 * TILE, SICK = BAD + KP_STAGES * HD * 8, BARS = SICK + 2 * KP_ROWS * HD / 8;
     static constexpr size_t SMEM = BARS + KP_NBARS * 8 + 1024;
 };
-template <int HD>
-constexpr int part_floats() { return 2 * KP_ROWS * (HD + 4); }
-
 template <int HD, typename TC>
 __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParams p, int* err) {
     using L = Lay<HD>;
@@ -95,52 +92,20 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
     constexpr uint32_t EXPONENTS = F16 ? 0x7C007C00u : 0x7F807F80u;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_bad[KP_STAGES], s_last;
+    __shared__ int s_bad[KP_STAGES];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv, G = p.heads / p.n_kv;
     pdl_wait();
-    // ---- the item: which sequence, tile of rows and part of its keys
-    const int n_entries = p.numbers[DC_KV_ENTRIES];
-    dc_kv_entry own = {0, 0, 0, 0};
-    auto tiles_of = [&](const dc_kv_entry& e) { return (long long)e.count * G > p.least ? (int)(((long long)e.count * G + 2 * KP_ROWS - 1) / (2 * KP_ROWS)) : 0; };
-    auto entry_at = [&](int i) { return i < n_entries ? p.entries[i] : dc_kv_entry{0, 0, 0, 0}; };
-    int n_all = 0;
-    for (int base = 0; base < n_entries; base += 32) {
-        own = entry_at(base + lane);
-        n_all += tiles_of(own);
-    }
-    n_all = __reduce_add_sync(0xffffffffu, n_all);
-    const int most = max(1, n_all ? p.num_sms / (int)min((long long)n_all * p.n_kv, (long long)p.num_sms) : 1);      // parts of a tile's keys at most
-    const int line = item / most, part = item % most;
-    if (blockIdx.x == 0 && tid == 0 && (long long)n_all * p.n_kv > gridDim.x) atomicExch(err, DC_ERR_STEP);      // (a step of more than the launch was made for)
-    if (line >= n_all) return;
-    int before = 0, tile = 0;
-    for (int base = 0;; base += 32) {
-        if (n_entries > 32) own = entry_at(base + lane);
-        const int mine = tiles_of(own);
-        int upto = mine;
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, upto, s);
-            if (lane >= s) upto += o;
-        }
-        const uint32_t there = __ballot_sync(0xffffffffu, before + upto > line);
-        if (there) {
-            const int who = __ffs(there) - 1;
-            tile = __shfl_sync(0xffffffffu, before + upto, who) - 1 - line;      // the last tile first: it sees most keys
-            own.seq = __shfl_sync(0xffffffffu, own.seq, who), own.pos0 = __shfl_sync(0xffffffffu, own.pos0, who), own.count = __shfl_sync(0xffffffffu, own.count, who);
-            own.tok0 = __shfl_sync(0xffffffffu, own.tok0, who);
-            break;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    const int row0 = tile * 2 * KP_ROWS, rows = min(2 * KP_ROWS, own.count * G - row0), sets = rows > KP_ROWS ? 2 : 1;
-    const int first = own.pos0 + row0 / G, last = own.pos0 + (row0 + rows - 1) / G, window = p.window ? p.window : 0x7fffffff;
-    // pages that the rows see, numbered: the first `kept` ones, then those from `low` on
-    const int low = p.window ? max(0, first - p.window + 1) / DC_KV_BLOCK : 0, kept = min((int)(((long long)p.keep + DC_KV_BLOCK - 1) / DC_KV_BLOCK), low), n_pages = kept + last / DC_KV_BLOCK - low + 1;
-    const int key_tiles = (n_pages + 3) / 4, n_parts = max(1, min(most, key_tiles / 8));
-    if (part >= n_parts) return;
-    const int tile0 = (int)((long long)key_tiles * part / n_parts), n_tiles = (int)((long long)key_tiles * (part + 1) / n_parts) - tile0;
-    auto page_at = [&](int i) { return i < kept ? i : low + i - kept; };
+    // ---- the item: which tile of rows, and which part of its keys
+    const TileLine tiles(p.entries, p.numbers[DC_KV_ENTRIES], G, p.least, p.n_kv, p.num_sms);
+    if (blockIdx.x == 0 && tid == 0 && (long long)tiles.n_all * p.n_kv > gridDim.x) atomicExch(err, DC_ERR_STEP);      // (a step of more than the launch was made for)
+    const int line = item / tiles.most, part = item % tiles.most;
+    if (line >= tiles.n_all) return;
+    const Tile tl(tiles, line, p.window, p.keep);
+    if (part >= tl.n_parts) return;
+    const dc_kv_entry own = tl.e;
+    const int row0 = tl.row0, rows = tl.rows, sets = rows > KP_ROWS ? 2 : 1, first = tl.first, last = tl.last, window = p.window ? p.window : 0x7fffffff, n_pages = tl.pages.n, n_parts = tl.n_parts;
+    const int tile0 = (int)((long long)tl.key_tiles * part / n_parts), n_tiles = (int)((long long)tl.key_tiles * (part + 1) / n_parts) - tile0;
+    auto page_at = [&](int i) { return tl.pages.at(i); };
     // position of the first key of page i of tile t; far behind the last token where there is none
     auto key_at = [&](int t, int i) { return 4 * (tile0 + t) + i < n_pages ? page_at(4 * (tile0 + t) + i) * DC_KV_BLOCK : 0x40000000; };
     auto whole = [&](int t, int least, int most_pos) {      // whether tokens at positions least .. most_pos see all of a tile
@@ -359,7 +324,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                         }
                     }
                 } else {
-                    float* to = p.parts + ((size_t)(line * most + part) * p.n_kv + kvh) * part_floats<HD>() + (KP_ROWS * u + 32 * (warp & 3)) * (HD + 4);
+                    float* to = p.parts + ((size_t)(line * tiles.most + part) * p.n_kv + kvh) * kp_part_floats<HD>() + (KP_ROWS * u + 32 * (warp & 3)) * (HD + 4);
                     if (lane < n_rows) *reinterpret_cast<float2*>(to + (size_t)lane * (HD + 4) + HD) = make_float2(m_run, l);
                     constexpr int LN = HD == 128 ? 16 : 8;      // lanes of a row: 64 dimensions of four bytes, or 32
 #pragma unroll 1
@@ -383,64 +348,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                             const int rr = row_at(i);
                             const uint4 v = lds128(place(rr, c8));
                             if (rr < n_rows) *reinterpret_cast<uint4*>(to + (size_t)rr * (HD + 4) + 4 * LN * g + 4 * c8) = v;
-                        }
-                    }
-                    // ---- the last CTA of the tile adds its parts up, in their order: a warp has its 32 rows, a lane HD / 32 dimensions
-                    __threadfence();
-                    asm volatile("bar.sync 1, %0;" ::"r"(sets * KP_ROWS) : "memory");
-                    int32_t* ticket = p.tickets + (size_t)line * p.n_kv + kvh;
-                    if (tid == 0) {
-                        s_last = atomicAdd(ticket, 1) == n_parts - 1;
-                        if (s_last) *ticket = 0;
-                        __threadfence();
-                    }
-                    asm volatile("bar.sync 1, %0;" ::"r"(sets * KP_ROWS) : "memory");
-                    if (s_last) {
-                        constexpr int D = HD / 32, B = 4;
-                        const float* from = p.parts + ((size_t)line * most * p.n_kv + kvh) * part_floats<HD>() + (KP_ROWS * u + 32 * (warp & 3)) * (HD + 4);
-                        const size_t step = (size_t)p.n_kv * part_floats<HD>();
-                        for (int r0 = 0; r0 < n_rows; r0 += B) {      // four rows' numbers on their way at once
-                            float M[B], sum[B], v[B][D];
-#pragma unroll
-                            for (int b = 0; b < B; ++b) {
-                                M[b] = -3e38f, sum[b] = 0.0f;
-#pragma unroll
-                                for (int d = 0; d < D; ++d) v[b][d] = 0.0f;
-                            }
-                            for (int i = 0; i < n_parts; ++i) {
-                                float2 ml[B];
-                                float y[B][D];
-#pragma unroll
-                                for (int b = 0; b < B; ++b) {
-                                    const float* at = from + (size_t)i * step + (size_t)min(r0 + b, n_rows - 1) * (HD + 4);
-                                    ml[b] = __ldcg(reinterpret_cast<const float2*>(at + HD));
-                                    if constexpr (D == 4) {
-                                        const float4 f = __ldcg(reinterpret_cast<const float4*>(at) + lane);
-                                        y[b][0] = f.x, y[b][1] = f.y, y[b][2] = f.z, y[b][3] = f.w;
-                                    } else {
-                                        const float2 f = __ldcg(reinterpret_cast<const float2*>(at) + lane);
-                                        y[b][0] = f.x, y[b][1] = f.y;
-                                    }
-                                }
-#pragma unroll
-                                for (int b = 0; b < B; ++b) {
-                                    const float m = fmaxf(M[b], ml[b].x), f0 = ex2(M[b] - m), f1 = ex2(ml[b].x - m);
-                                    M[b] = m, sum[b] = fmaf(sum[b], f0, ml[b].y * f1);
-#pragma unroll
-                                    for (int d = 0; d < D; ++d) v[b][d] = fmaf(v[b][d], f0, y[b][d] * f1);
-                                }
-                            }
-#pragma unroll
-                            for (int b = 0; b < B; ++b) {
-                                if (r0 + b >= n_rows) continue;
-                                const float inv = 1.0f / sum[b];
-                                uint16_t* at = reinterpret_cast<uint16_t*>(p.out) + element(r0 + b, p.ldo) + D * lane;
-#pragma unroll
-                                for (int d = 0; d < D; d += 2) {
-                                    const uint32_t w = pack<TC>(v[b][d] * inv, v[b][d + 1] * inv);
-                                    at[d] = (uint16_t)w, at[d + 1] = (uint16_t)(w >> 16);
-                                }
-                            }
                         }
                     }
                 }
@@ -570,17 +477,17 @@ int launch(dc_ctx* ctx, const PromptParams& p, int items) {
 
 }  // namespace
 
-// Parts and tickets: as many as CTAs where keys are split (a tile that is not split has neither), the tickets of all tiles of a key head ahead of them.
-size_t dc_kv16_prompt_parts(int num_sms, int n_kv, int dim) { return (size_t)std::max(1, num_sms / n_kv) * n_kv * 2 * KP_ROWS * (dim + 4) * 4; }
+// Parts: as many as CTAs where keys are split (a tile that is not split has none).
+size_t dc_kv16_prompt_parts(int num_sms, int n_kv, int dim) { return (size_t)std::max(1, num_sms / n_kv) * n_kv * KP_TILE_ROWS * (dim + 4) * 4; }
 
 int dc_launch_kv16_prompt(dc_ctx* ctx, const dc_kv16_call& c) {
     const dc_kv_dev& z = *c.kv->dev;
     const long long G = z.heads / z.kv, tokens = std::min((long long)z.max_tokens, (long long)z.slots * z.max_count);
     // tiles: at most one that is not full for every sequence with that many new tokens
-    const long long least = dc_kv16_rows(z.type) / G + 1, tiles = tokens * G / (2 * KP_ROWS) + std::min((long long)z.slots, tokens / least);
+    const long long least = dc_kv16_rows(z.type) / G + 1, tiles = tokens * G / KP_TILE_ROWS + std::min((long long)z.slots, tokens / least);
     const int items = (int)std::max(tiles, (long long)std::max(1, ctx->num_sms / z.kv));
     const PromptParams p = {z.entries, z.numbers, z.tables, z.pages_per_seq, z.heads, z.kv, dc_kv16_rows(z.type), ctx->num_sms, c.q, c.ldq, c.ldo, c.arena, c.scale, c.window, c.keep, c.out,
-                            z.prompt_parts, z.prompt_tickets};
+                            z.prompt_parts};
     if (z.type == DC_TYPE_F16) return z.dim == 128 ? launch<128, __half>(ctx, p, items) : launch<64, __half>(ctx, p, items);
     return z.dim == 128 ? launch<128, __nv_bfloat16>(ctx, p, items) : launch<64, __nv_bfloat16>(ctx, p, items);
 }

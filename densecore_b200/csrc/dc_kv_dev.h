@@ -31,11 +31,12 @@ struct dc_kv_dev {
     uint8_t* arena = nullptr;      // [layer][page][key head] records
     int32_t *lens = nullptr, *held = nullptr, *counts = nullptr, *starts = nullptr, *tables = nullptr, *slot_map = nullptr, *positions = nullptr, *seqs = nullptr, *stack = nullptr;
     int32_t* numbers = nullptr;    // free pages, entries
+    int32_t* scratch = nullptr;    // of a step
     dc_kv_entry* entries = nullptr;
     uint8_t* memory = nullptr;     // all of the above but the arena
     // of attention: partial results and tickets of sequences that several CTAs work on (zero between calls)
     float *parts = nullptr, *prompt_parts = nullptr;
-    int32_t *tickets = nullptr, *prompt_tickets = nullptr;
+    int32_t* tickets = nullptr;
 };
 enum { DC_KV_FREE = 0, DC_KV_ENTRIES = 1, DC_KV_NUMBERS = 4 };
 

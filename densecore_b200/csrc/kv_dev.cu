@@ -6,9 +6,10 @@
 // Free pages are a stack F[0 .. n).  With R pages freed and A granted, all in the order of slots and places, the j-th granted one is the j-th freed one, or
 // F[n - 1 - (j - R)] behind those; what is left of the freed ones goes onto the stack in falling order.  So a step and the one that takes it back leave the
 // tables and the stack as they were.
-// All of it is prefix sums over the slots: every CTA of a cluster makes them for itself (each slot's numbers are some bytes), then the CTAs share the pages that move and
-// the new tokens' places.
-// Bound: latency of a launch, the loads, two scans and two cluster barriers; the largest steps by their tokens' twelve bytes.
+// All of it is prefix sums over the slots (k_kv_step, one CTA, or each CTA of a cluster for itself: a slot's numbers are some bytes), behind which every page that new
+// tokens lie on is a unit of work of its own: it is looked up or granted, and its tokens' places are written.  The largest steps share the units out among all SMs
+// (k_kv_places).
+// Bound: latency of a launch, the loads and two scans; the largest steps by their tokens' twelve bytes.
 #include <cooperative_groups.h>
 #include <math.h>
 #include <string.h>
@@ -32,13 +33,16 @@ using namespace dc;
 
 namespace {
 
-constexpr int KS_T = 1024, KS_PER = 4, KS_SLOTS = KS_T * KS_PER;
+constexpr int KS_T = 1024, KS_PER = 4, KS_SLOTS = KS_T * KS_PER, KS_APART = 16 * KS_T;
 
 struct StepParams {
     int slots, pages_per_seq, max_tokens, max_count;
     const int32_t *drop, *count;
     int32_t *lens, *held, *counts, *starts, *tables, *slot_map, *positions, *seqs, *stack, *numbers;
     dc_kv_entry* entries;
+    bool apart;                 // units are k_kv_places', which finds what it needs here:
+    int32_t* scratch;
+    struct Totals* totals;
 };
 
 // Exclusive sums of three values a thread over the CTA, in place; the whole sums to `all`.
@@ -81,10 +85,55 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int x) {
     return lo;
 }
 
+// Of every slot, ahead of it: new tokens, pages that they lie on, freed pages, granted ones; its tokens and pages that stay.
+struct Slots {
+    int32_t *tok0, *unit0, *free0, *give0, *keep, *left;
+    __device__ __forceinline__ Slots(int32_t* at, int n) : tok0(at), unit0(at + n), free0(at + 2 * n), give0(at + 3 * n), keep(at + 4 * n), left(at + 5 * n) {}
+};
+enum { KS_ARRAYS = 6 };
+struct Totals {
+    int32_t tokens, units, freed, given, free;      // free: of the pool, before the step
+};
+
+// Unit i: a page that new tokens lie on, or (behind those) a freed one that nobody takes.
+__device__ __forceinline__ void place_unit(const StepParams& p, const Slots& z, const Totals& all, int i) {
+    auto freed_page = [&](int j) {
+        const int s = find(z.free0, p.slots, j);
+        return p.tables[(size_t)s * p.pages_per_seq + z.left[s] + (j - z.free0[s])];
+    };
+    if (i >= all.units) {
+        const int j = all.given + i - all.units;
+        p.stack[all.free + all.freed - 1 - j] = freed_page(j);
+        return;
+    }
+    const int s = find(z.unit0, p.slots, i), keep = z.keep[s], place = keep / DC_KV_BLOCK + i - z.unit0[s], tok0 = z.tok0[s];
+    const int n_tok = (s + 1 < p.slots ? z.tok0[s + 1] : all.tokens) - tok0, left = z.left[s];
+    int32_t* cell = p.tables + (size_t)s * p.pages_per_seq + place;
+    int page;
+    if (place < left) {
+        page = *cell;
+    } else {      // the j-th granted one
+        const int j = z.give0[s] + place - left;
+        page = j < all.freed ? freed_page(j) : p.stack[all.free - 1 - (j - all.freed)];
+        *cell = page;
+    }
+    const int first = max(keep, place * DC_KV_BLOCK), last = min(keep + n_tok, (place + 1) * DC_KV_BLOCK), t = tok0 + first - keep, n = last - first;
+    int32_t *to = p.slot_map + t, *pos = p.positions + t, *seq = p.seqs + t;
+    const int slot = page * DC_KV_BLOCK + first % DC_KV_BLOCK;
+    int x = 0;
+    for (; x < n && ((t + x) & 3); ++x) to[x] = slot + x, pos[x] = first + x, seq[x] = s;
+    for (; x + 4 <= n; x += 4) {
+        *reinterpret_cast<int4*>(to + x) = make_int4(slot + x, slot + x + 1, slot + x + 2, slot + x + 3);
+        *reinterpret_cast<int4*>(pos + x) = make_int4(first + x, first + x + 1, first + x + 2, first + x + 3);
+        *reinterpret_cast<int4*>(seq + x) = make_int4(s, s, s, s);
+    }
+    for (; x < n; ++x) to[x] = slot + x, pos[x] = first + x, seq[x] = s;
+}
+
 __global__ void __launch_bounds__(KS_T) k_kv_step(const StepParams p) {
     extern __shared__ int32_t sm[];
     __shared__ Three warps[32];
-    int32_t *tok0 = sm, *free0 = tok0 + p.slots, *give0 = free0 + p.slots, *keep = give0 + p.slots, *kept_pages = keep + p.slots;
+    const Slots z(sm, p.slots);
     cg::cluster_group cl = cg::this_cluster();
     const int rank = (int)cl.block_rank(), n_cta = (int)cl.num_blocks();
     pdl_wait();
@@ -110,7 +159,8 @@ __global__ void __launch_bounds__(KS_T) k_kv_step(const StepParams p) {
     scan3(x, warps, all);
     const int n_freed = all.b;
     // ---- what is granted
-    Three y = {0, 0, 0}, granted;
+    Three y = {0, 0, 0}, granted;      // a: new tokens and, 2^32 fold, pages that they lie on
+    auto units = [&](int i) { return cnt[i] ? (kp[i] + cnt[i] - 1) / DC_KV_BLOCK - kp[i] / DC_KV_BLOCK + 1 : 0; };
     {
         long long tokens = x.a;
         int asked = x.c;
@@ -118,59 +168,56 @@ __global__ void __launch_bounds__(KS_T) k_kv_step(const StepParams p) {
         for (int i = 0; i < KS_PER; ++i) {
             tokens += cnt[i], asked += asks[i];      // (at most the tables' places in all: below 2^31)
             if ((asks[i] && asked > n_free + n_freed) || tokens > p.max_tokens) cnt[i] = asks[i] = 0;
-            y.a += cnt[i], y.b += asks[i], y.c += cnt[i] > 0;
+            y.a += cnt[i] + ((long long)units(i) << 32), y.b += asks[i], y.c += cnt[i] > 0;
         }
     }
     scan3(y, warps, granted);
+    const Totals sum = {(int)granted.a, (int)(granted.a >> 32), n_freed, granted.b, n_free};
     {
-        int tok = (int)y.a, give = y.b, freed = x.b;
+        int tok = (int)y.a, unit = (int)(y.a >> 32), give = y.b, freed = x.b;
 #pragma unroll
         for (int i = 0; i < KS_PER; ++i) {
             const int s = s0 + i;
             if (i >= per || s >= p.slots) break;
-            tok0[s] = tok, give0[s] = give, free0[s] = freed, keep[s] = kp[i], kept_pages[s] = left[i];
-            tok += cnt[i], give += asks[i], freed += frees[i];
+            z.tok0[s] = tok, z.unit0[s] = unit, z.give0[s] = give, z.free0[s] = freed, z.keep[s] = kp[i], z.left[s] = left[i];
+            tok += cnt[i], unit += units(i), give += asks[i], freed += frees[i];
         }
     }
-    cl.sync();      // everybody has read the old numbers
-    const int n_tok = (int)granted.a, n_given = granted.b;
+    if (n_cta > 1) cl.sync();      // everybody has read the old numbers
+    else __syncthreads();
     if (rank == 0) {
         int entry = y.c;
+        const Slots out(p.scratch, p.slots);
 #pragma unroll
         for (int i = 0; i < KS_PER; ++i) {
             const int s = s0 + i;
             if (i >= per || s >= p.slots) break;
-            p.lens[s] = kp[i] + cnt[i], p.held[s] = left[i] + asks[i], p.counts[s] = cnt[i], p.starts[s] = tok0[s];
-            if (cnt[i]) p.entries[entry++] = {s, kp[i], cnt[i], tok0[s]};
+            p.lens[s] = kp[i] + cnt[i], p.held[s] = left[i] + asks[i], p.counts[s] = cnt[i], p.starts[s] = z.tok0[s];
+            if (cnt[i]) p.entries[entry++] = {s, kp[i], cnt[i], z.tok0[s]};
+            if (p.apart) out.tok0[s] = z.tok0[s], out.unit0[s] = z.unit0[s], out.free0[s] = z.free0[s], out.give0[s] = z.give0[s], out.keep[s] = kp[i], out.left[s] = left[i];
         }
         if (threadIdx.x == 0) {
-            p.starts[p.slots] = n_tok;
-            p.numbers[DC_KV_FREE] = n_free + n_freed - n_given;
+            p.starts[p.slots] = sum.tokens;
+            p.numbers[DC_KV_FREE] = n_free + n_freed - sum.given;
             p.numbers[DC_KV_ENTRIES] = granted.c;
+            if (p.apart) *p.totals = sum;
         }
     }
-    // ---- pages: the j-th granted one, then freed ones that nobody takes
-    const int me = rank * KS_T + threadIdx.x, threads = n_cta * KS_T;
-    auto freed_page = [&](int j) {
-        const int s = find(free0, p.slots, j);
-        return p.tables[(size_t)s * p.pages_per_seq + kept_pages[s] + (j - free0[s])];
-    };
-    for (int j = me; j < max(n_given, n_freed); j += threads) {
-        if (j < n_given) {
-            const int page = j < n_freed ? freed_page(j) : p.stack[n_free - 1 - (j - n_freed)];
-            const int s = find(give0, p.slots, j);
-            p.tables[(size_t)s * p.pages_per_seq + kept_pages[s] + (j - give0[s])] = page;
-        } else {
-            p.stack[n_free + n_freed - 1 - j] = freed_page(j);
-        }
-    }
-    cl.sync();      // the tables stand
-    for (int t = me; t < n_tok; t += threads) {
-        const int s = find(tok0, p.slots, t), pos = keep[s] + t - tok0[s];
-        p.slot_map[t] = __ldcg(p.tables + (size_t)s * p.pages_per_seq + pos / DC_KV_BLOCK) * DC_KV_BLOCK + pos % DC_KV_BLOCK;
-        p.positions[t] = pos;
-        p.seqs[t] = s;
-    }
+    if (p.apart) return;
+    for (int i = rank * KS_T + threadIdx.x; i < sum.units + max(0, n_freed - sum.given); i += n_cta * KS_T) place_unit(p, z, sum, i);
+}
+
+// The units of a large step.
+constexpr int KP_T = 512;
+__global__ void __launch_bounds__(KP_T) k_kv_places(const StepParams p) {
+    extern __shared__ int32_t sm[];
+    pdl_wait();
+    pdl_launch_dependents();
+    const Totals sum = *p.totals;
+    for (int i = threadIdx.x; i < KS_ARRAYS * p.slots; i += KP_T) sm[i] = p.scratch[i];
+    __syncthreads();
+    const Slots z(sm, p.slots);
+    for (int i = blockIdx.x * KP_T + threadIdx.x; i < sum.units + max(0, sum.freed - sum.given); i += gridDim.x * KP_T) place_unit(p, z, sum, i);
 }
 
 __global__ void k_kv_stack(int32_t* stack, int n) {      // so that pages are handed out from 0 on
@@ -300,7 +347,7 @@ int create(dc_ctx* ctx, dc_kv_cache* kv) {
     };
     const size_t slots4 = (size_t)z.slots * 4, tokens4 = (size_t)z.max_tokens * 4;
     const size_t lens = room(slots4), held = room(slots4), counts = room(slots4), starts = room(slots4 + 4), tables = room(slots4 * z.pages_per_seq), map = room(tokens4), positions = room(tokens4),
-                 seqs = room(tokens4), numbers = room(DC_KV_NUMBERS * 4), entries = room(slots4 * 4), tickets = room((size_t)ctas * z.kv * 4), prompt_tickets = room((size_t)ctx->num_sms * 4), stack = room((size_t)z.pages * 4), zeroed = at,
+                 seqs = room(tokens4), numbers = room(DC_KV_NUMBERS * 4), entries = room(slots4 * 4), scratch = room(slots4 * KS_ARRAYS + sizeof(Totals)), tickets = room((size_t)ctas * z.kv * 4), stack = room((size_t)z.pages * 4), zeroed = at,
                  parts = room((size_t)2 * ctas * z.kv * dc_kv16_rows(z.type) * (z.dim + 2) * 4),
                  prompt_parts = room(z.type == DC_TYPE_F32 ? 0 : dc_kv16_prompt_parts(ctx->num_sms, z.kv, z.dim));
     DC_TRY(dc_check_cuda(ctx, cudaMalloc(&z.arena, bytes), "kv_create_dev"));
@@ -309,7 +356,7 @@ int create(dc_ctx* ctx, dc_kv_cache* kv) {
     DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.memory, 0, zeroed, ctx->stream), "kv_create_dev"));
     auto ints = [&](size_t from) { return (int32_t*)(z.memory + from); };
     z.lens = ints(lens), z.held = ints(held), z.counts = ints(counts), z.starts = ints(starts), z.tables = ints(tables), z.slot_map = ints(map), z.positions = ints(positions), z.seqs = ints(seqs);
-    z.numbers = ints(numbers), z.entries = (dc_kv_entry*)(z.memory + entries), z.tickets = ints(tickets), z.prompt_tickets = ints(prompt_tickets), z.stack = ints(stack), z.parts = (float*)(z.memory + parts), z.prompt_parts = (float*)(z.memory + prompt_parts);
+    z.numbers = ints(numbers), z.entries = (dc_kv_entry*)(z.memory + entries), z.scratch = ints(scratch), z.tickets = ints(tickets), z.stack = ints(stack), z.parts = (float*)(z.memory + parts), z.prompt_parts = (float*)(z.memory + prompt_parts);
     k_kv_stack<<<std::min((z.pages + 255) / 256, ctx->num_sms * 4), 256, 0, ctx->stream>>>(z.stack, z.pages);
     DC_TRY(dc_check_cuda(ctx, cudaGetLastError(), "k_kv_stack"));
     const int32_t free_pages = z.pages;
@@ -393,13 +440,19 @@ int dc_b200_kv_step_dev(dc_ctx* ctx, dc_kv_cache* kv, const int32_t* drop_dev, c
     dc_kv_dev& z = *kv->dev;
     if (max_count < 0) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_step_dev: at most %d new tokens a sequence", max_count);
     cudaSetDevice(ctx->device);
+    // pages that new tokens may lie on, and that may be freed: a CTA of 1024 threads, a cluster of eight, or all SMs behind a launch of their own
+    const long long units = (long long)z.slots * std::min<long long>(max_count / DC_KV_BLOCK + 2, z.pages_per_seq);
+    const bool apart = units > KS_APART;
     const StepParams p = {z.slots, z.pages_per_seq, z.max_tokens, max_count, drop_dev, count_dev, z.lens, z.held, z.counts, z.starts, z.tables, z.slot_map, z.positions, z.seqs, z.stack,
-                          z.numbers, z.entries};
-    const size_t smem = (size_t)z.slots * 20;
-    DC_TRY(dc_kernel_setup(ctx, (const void*)k_kv_step, KS_SLOTS * 20, "k_kv_step"));
-    // eight CTAs where the tokens are more than one takes in four rounds
-    const int n_cta = (long long)z.slots * max_count > 4 * KS_T ? 8 : 1;
+                          z.numbers, z.entries, apart, z.scratch, (Totals*)(z.scratch + (size_t)KS_ARRAYS * z.slots)};
+    const size_t smem = (size_t)z.slots * KS_ARRAYS * 4;
+    DC_TRY(dc_kernel_setup(ctx, (const void*)k_kv_step, KS_SLOTS * KS_ARRAYS * 4, "k_kv_step"));
+    const int n_cta = !apart && (units > 4 * KS_T || (drop_dev && (long long)z.slots * z.pages_per_seq > 64 * KS_T)) ? 8 : 1;
     DC_TRY(dc_launch_cluster(ctx, "k_kv_step", k_kv_step, dim3(n_cta), dim3(KS_T), smem, n_cta, p));
+    if (apart) {
+        DC_TRY(dc_kernel_setup(ctx, (const void*)k_kv_places, KS_SLOTS * KS_ARRAYS * 4, "k_kv_places"));
+        DC_TRY(dc_launch(ctx, "k_kv_places", k_kv_places, dim3((unsigned)std::min<long long>((units + KP_T - 1) / KP_T, 2 * ctx->num_sms)), dim3(KP_T), smem, p));
+    }
     z.max_count = max_count;
     return DC_B200_OK;
 }
