@@ -31,7 +31,7 @@ using namespace dc;
 namespace {
 
 constexpr int KR_WARPS = 4, KR_SLOTS = 8;      // page places of a CTA, shared out among the groups of warps that take pages in turn
-constexpr int KR_LEAST = 16, KR_EVEN = 48;     // pages of a CTA at least; at most, where sequences are cut into parts alike
+constexpr int KR_LEAST = 16, KR_CTAS = 3;      // pages of a CTA at least; CTAs of an SM
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -85,7 +85,7 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 struct RowsParams {
     const dc_kv_entry* entries;
     const int32_t *numbers, *tables;
-    int pages_per_seq, heads, n_kv;
+    int pages_per_seq, heads, n_kv, slots;
     const void *q, *k, *v;      // k null: nothing to write
     int64_t ldq, ldkv, ldo;
     uint8_t* arena;
@@ -172,7 +172,7 @@ __device__ __forceinline__ void join_prompts(const RowsParams& p, int n_entries,
 
 // PROMPTS: tiles of 32 NT rows of the sequences that have more, each whole by one CTA; else sequences of up to 32 NT rows, their pages shared out.
 template <int HD, typename TX, typename TC, int NT, bool PROMPTS>
-__global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams p) {
+__global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const RowsParams p) {
     using R = dc_kv16_rec<HD>;
     using W2 = Two<TC>;
     constexpr bool TERMS = sizeof(TX) == 4;      // queries in two terms
@@ -194,20 +194,21 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
     // (behind k_kv16_prompt, which has waited for all before it and shares nothing with this one's sequences, the SMs that it leaves idle take them meanwhile)
     if (!p.prompt_parts) pdl_wait();
     pdl_launch_dependents();
+    const dc_kv_entry ahead_of = p.entries[min((int)(threadIdx.x & 31), p.slots - 1)];      // (on its way with their number)
     const int n_entries = p.numbers[DC_KV_ENTRIES];
     // ---- the line of work: entries' pages (tiles), a warp of entries at a time
     dc_kv_entry own = {0, 0, 0, 0};
     int chunk = -32, ahead = 0, mine = 0, upto = 0;      // of the chunk's entries: work, and the line's up to with it
     auto weigh = [&](const dc_kv_entry& e) -> int {
-        const long long rows = (long long)e.count * G;
-        if constexpr (PROMPTS) return rows > RT ? (int)((rows + RT - 1) / RT) : 0;
+        const int rows = e.count * G;      // (at most 2^30, as the whole step's)
+        if constexpr (PROMPTS) return rows > RT ? (rows + RT - 1) / RT : 0;
         else return rows <= RT && e.count > 0 ? pages_of(e.pos0, e.pos0 + e.count - 1, p.window, p.keep).n : 0;
     };
     auto look_at = [&](int base) {
         chunk = base;
-        own = base + lane < n_entries ? p.entries[base + lane] : dc_kv_entry{0, 0, 0, 0};
+        own = base + lane >= n_entries ? dc_kv_entry{0, 0, 0, 0} : base == 0 ? ahead_of : p.entries[base + lane];
         mine = weigh(own);
-        if (!PROMPTS && p.all && (long long)own.count * G > RT) atomicExch(p.err, DC_ERR_STEP);
+        if (!PROMPTS && p.all && own.count * G > RT) atomicExch(p.err, DC_ERR_STEP);
     };
     int work = 0, n_with = 0;
     for (int base = 0; base < n_entries; base += 32) {
@@ -215,26 +216,26 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         work += mine, n_with += mine > 0;
     }
     work = __reduce_add_sync(0xffffffffu, work), n_with = __reduce_add_sync(0xffffffffu, n_with);
-    // few pages: every CTA has one part of one sequence, all of a sequence's alike, so that nobody does two chains of loads one after the other; many: equal shares of the
-    // line, which end within a sequence where they may
-    const int ctas = gridDim.x;
-    int share = max(KR_LEAST, (int)(((long long)work + ctas - 1) / ctas));
+    // Either equal shares of the line, which end within a sequence where they may; or every CTA one part of one sequence, a sequence's parts alike, so that nobody does two
+    // chains of loads one after the other: where that leaves no SM with more than 5/4 of the pages.  (All are fewer than 2^31 less the grid's width.)
+    const uint32_t ctas = gridDim.x;
+    int share = max(KR_LEAST, (int)(((uint32_t)work + ctas - 1) / ctas)), parts = 0;
     bool even = false;
-    if (!PROMPTS && 2 * n_with <= ctas) {
-        const int s = max(KR_LEAST, (int)(((long long)work + ctas - n_with - 1) / (ctas - n_with)));
-        even = s <= KR_EVEN;
+    if (!PROMPTS && n_with < (int)ctas) {
+        const int s = max(KR_LEAST, (int)(((uint32_t)work + ctas - n_with - 1) / (ctas - n_with)));      // (with this many pages a part there are no more parts than CTAs)
+        int longest = 0;
+        for (int base = 0; base < n_entries; base += 32) {
+            if (base != chunk) look_at(base);
+            const int n = (mine + s - 1) / s;
+            parts += n;
+            if (n) longest = max(longest, (mine + n - 1) / n);
+        }
+        parts = __reduce_add_sync(0xffffffffu, parts), longest = __reduce_max_sync(0xffffffffu, longest);
+        even = 4 * ((parts * p.n_kv + p.num_sms - 1) / p.num_sms) * longest <= 5 * KR_CTAS * share;
         if (even) share = s;
     }
     int at = PROMPTS || even ? (int)blockIdx.x : (int)min((long long)work, (long long)blockIdx.x * share);
-    int end = PROMPTS ? work : even ? at + 1 : min(work, at + share);      // (even: of the parts' line, whose length is at most that of the grid)
-    if (even) {
-        int parts = 0;
-        for (int base = 0; base < n_entries; base += 32) {
-            if (base != chunk) look_at(base);
-            parts += (mine + share - 1) / share;
-        }
-        end = min(end, __reduce_add_sync(0xffffffffu, parts));
-    }
+    const int end = PROMPTS ? work : even ? min(at + 1, parts) : min(work, at + share);      // (even: of the parts' line)
     auto begin_line = [&](int base) {
         if (base != chunk) look_at(base);
         upto = even ? (mine + share - 1) / share : mine;
@@ -256,32 +257,37 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         const int who = __ffs(there) - 1;
         const int seq = __shfl_sync(0xffffffffu, own.seq, who), pos0 = __shfl_sync(0xffffffffu, own.pos0, who), count = __shfl_sync(0xffffffffu, own.count, who),
                   tok0 = __shfl_sync(0xffffffffu, own.tok0, who);
-        const int e_end = __shfl_sync(0xffffffffu, upto, who), e_work = __shfl_sync(0xffffffffu, mine, who), e_parts = (e_work + share - 1) / share, e_at = e_end - (even ? e_parts : e_work);
+        const int e_end = __shfl_sync(0xffffffffu, upto, who), e_work = __shfl_sync(0xffffffffu, mine, who), e_parts = even ? (e_work + share - 1) / share : 0, e_at = e_end - (even ? e_parts : e_work);
         // ---- the item: rows from row0 on, pages page0 .. page1 - 1 of those that they see
         const int row0 = PROMPTS ? (at - e_at) * RT : 0, rows = min(RT, count * G - row0), j_last = (row0 + rows - 1) / G;
         const Pages pages = pages_of(pos0 + row0 / G, pos0 + j_last, p.window, p.keep);
-        const int page0 = PROMPTS ? 0 : even ? (int)((long long)e_work * (at - e_at) / e_parts) : at - e_at;
-        const int page1 = PROMPTS ? pages.n : even ? (int)((long long)e_work * (at - e_at + 1) / e_parts) : min(end, e_end) - e_at;
-        const int tiles = (rows + RW - 1) / RW, WM = tiles <= 1 ? 1 : tiles <= 2 ? 2 : 4, WK = KR_WARPS / WM, depth = KR_SLOTS / WK;
-        const int grp = warp / WM, r0 = row0 + (warp % WM) * RW, n_my = (page1 - page0 - grp + WK - 1) / WK;
+        const int e_of = at - e_at, e_each = even ? e_work / e_parts : 0, e_more = even ? e_work - e_each * e_parts : 0;      // (even: part e_of; the first e_more have a page more)
+        const int page0 = PROMPTS ? 0 : even ? e_each * e_of + min(e_of, e_more) : e_of;
+        const int page1 = PROMPTS ? pages.n : even ? page0 + e_each + (e_of < e_more) : min(end, e_end) - e_at;
+        const int tiles = (rows + RW - 1) / RW, lm = tiles <= 1 ? 0 : tiles <= 2 ? 1 : 2, lk = 2 - lm, ld = 3 - lk;      // 2^lm warps share a page, 2^lk groups of them take turns, 2^ld places each
+        static_assert(KR_WARPS == 4 && KR_SLOTS == 8, "powers of two");
+        const int WM = 1 << lm, WK = 1 << lk, depth = 1 << ld;
+        const int grp = warp >> lm, sub = warp & (WM - 1), r0 = row0 + sub * RW, n_my = (page1 - page0 - grp + WK - 1) >> lk;
         const int32_t* table = p.tables + (size_t)seq * p.pages_per_seq;
         auto group_sync = [&]() {
             if (WM == 1) __syncwarp();
             else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "r"(32 * WM) : "memory");
         };
         int entry = 0;      // lane i: the page of this group's number i + a multiple of 32
-        auto issue = [&](int i) {
-            if (i % 32 == 0) entry = i + lane < n_my ? table[pages.at(page0 + grp + (i + lane) * WK)] : 0;
+        auto issue = [&](int i, int s) {      // page i of the group's into its place s
+            if (i % 32 == 0) entry = i + lane < n_my ? table[pages.at(page0 + grp + ((i + lane) << lk))] : 0;
             const int page = __shfl_sync(0xffffffffu, entry, i % 32);
             if (lane == 0) {
-                const int s = grp * depth + i % depth;
                 mbar_expect_tx(bars + 8 * s, R::BYTES);
                 bulk_g2s(ring + s * R::BYTES, p.arena + ((size_t)page * p.n_kv + kvh) * R::BYTES, R::BYTES, bars + 8 * s);
             }
         };
-        if (warp % WM == 0)
-            for (int i = 0; i < depth && i < n_my; ++i) issue(i);
-        // ---- queries
+        const int s0 = grp << ld;
+        auto issue_first = [&]() {
+            if (sub == 0)
+                for (int i = 0; i < depth && i < n_my; ++i) issue(i, s0 + i);
+        };
+        // ---- queries: their loads, the table's, the first pages', then what the queries become
         int qpos[NT];
         uint32_t qa[KS][4];
         float F = p.scale * 1.4426950408889634f;
@@ -309,8 +315,12 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
                             else f = make_float2(a[0], a[1]);
                         }
                         x[s][2 * i] = f.x, x[s][2 * i + 1] = f.y;
-                        most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
                     }
+                issue_first();
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[s][i]));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
                 // times 2^(10 - e), 2^e <= largest < 2^(e + 1)
@@ -335,6 +345,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
                         const uint16_t* a = reinterpret_cast<const uint16_t*>(src[i & 1]) + 16 * s + 8 * (i >> 1);
                         qa[s][i] = !in[i & 1] ? 0u : vec ? *reinterpret_cast<const uint32_t*>(a) : a[0] | (uint32_t)a[1] << 16;
                     }
+                issue_first();
             }
         }
         // positions between which every row of the warp sees all keys, but for the kept ones
@@ -350,14 +361,14 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         const uint32_t v_lane = R::VALUES + (lane & 15) * 32 + (((lane >> 4) ^ ((lane >> 2) & 1)) << 4);
 
         for (int i = 0; i < n_my; ++i) {
-            const int s = grp * depth + i % depth, page = pages.at(page0 + grp + i * WK), k0 = page * DC_KV_BLOCK;
+            const int s = s0 + (i & (depth - 1)), page = pages.at(page0 + grp + (i << lk)), k0 = page * DC_KV_BLOCK;
             const uint32_t to = ring + s * R::BYTES;
-            mbar_wait(bars + 8 * s, (phases >> s & 1) ^ (i / depth & 1), p.err);
+            mbar_wait(bars + 8 * s, ((phases >> s) ^ (i >> ld)) & 1, p.err);
             if (!PROMPTS && p.k && k0 + DC_KV_BLOCK > pos0) {
                 // ---- the step's own rows, into the copy and into the cache (no other CTA has this page)
                 const int j0 = max(0, k0 - pos0), n = (min(count, k0 + DC_KV_BLOCK - pos0) - j0) * (HD / 2), slot0 = pos0 + j0 - k0;
                 uint8_t* rec = p.arena + ((size_t)table[page] * p.n_kv + kvh) * R::BYTES;
-                for (int x = (warp % WM) * 32 + lane; x < n; x += 32 * WM) {
+                for (int x = sub * 32 + lane; x < n; x += 32 << lm) {
                     const int j = x / (HD / 2), d = 2 * (x % (HD / 2));
                     const size_t from = (size_t)(tok0 + j0 + j) * p.ldkv + (size_t)kvh * HD + d;
                     const TX *ks = reinterpret_cast<const TX*>(p.k) + from, *vs = reinterpret_cast<const TX*>(p.v) + from;
@@ -487,12 +498,12 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
                 }
             }
             group_sync();      // the page has been read
-            if (warp % WM == 0 && i + depth < n_my) issue(i + depth);
+            if (sub == 0 && i + depth < n_my) issue(i + depth, s);
         }
         // uses of each place in this item
         for (int g = 0; g < WK; ++g) {
-            const int n = (page1 - page0 - g + WK - 1) / WK;
-            for (int s = 0; s < depth; ++s) phases ^= (uint32_t)((max(0, n - s + depth - 1) / depth) & 1) << (g * depth + s);
+            const int n = (page1 - page0 - g + WK - 1) >> lk;
+            for (int s = 0; s < depth; ++s) phases ^= (uint32_t)((n - s + depth - 1) >> ld & 1) << ((g << ld) + s);
         }
         __syncthreads();      // all pages have been read: the parts take their place
 #pragma unroll
@@ -526,10 +537,10 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         for (int x4 = threadIdx.x; x4 < rows * (HD / 4); x4 += KR_WARPS * 32) {
             const int r = x4 / (HD / 4), d = 4 * (x4 % (HD / 4)), w0 = r / RW, rr = r % RW;
             float M = -3.4028235e38f, L = 0.0f;
-            for (int g = 0; g < WK; ++g) M = fmaxf(M, part_ml[2 * ((g * WM + w0) * RW + rr)]);
+            for (int g = 0; g < WK; ++g) M = fmaxf(M, part_ml[2 * (((g << lm) + w0) * RW + rr)]);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int g = 0; g < WK; ++g) {
-                const int at = (g * WM + w0) * RW + rr;
+                const int at = ((g << lm) + w0) * RW + rr;
                 const float f = ex2(part_ml[2 * at] - M);
                 const float4 x = *reinterpret_cast<const float4*>(part + at * PITCH + d);
                 L = fmaf(part_ml[2 * at + 1], f, L);
@@ -545,12 +556,12 @@ __global__ void __launch_bounds__(KR_WARPS * 32, 3) k_kv16_rows(const RowsParams
         }
         if (!alone) {
             int32_t* ticket = p.tickets + (size_t)kvh * gridDim.x + c_first;      // (a CTA is the first of one sequence at most that others have too)
-            __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) {
-                s_last = atomicAdd(ticket, 1) == n_parts - 1;
+            if (threadIdx.x == 0) {      // (releases what the CTA's threads have stored ahead of the barrier, and acquires what the others' have)
+                int before;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
+                s_last = before == n_parts - 1;
                 if (s_last) *ticket = 0;
-                __threadfence();
             }
             __syncthreads();
             if (s_last) {
@@ -617,7 +628,7 @@ int launch_type(dc_ctx* ctx, const dc_kv16_call& c, const RowsParams& p, bool pr
 int dc_launch_kv16_rows(dc_ctx* ctx, const dc_kv16_call& c, bool prompts) {
     const dc_kv_dev& z = *c.kv->dev;
     const long long rows = (long long)z.max_count * (z.heads / z.kv);
-    const RowsParams p = {z.entries, z.numbers, z.tables, z.pages_per_seq, z.heads, z.kv, c.q, c.k, c.v, c.ldq, c.ldkv, c.ldo, c.arena, c.scale, c.window, c.keep, c.out, z.parts, z.tickets,
+    const RowsParams p = {z.entries, z.numbers, z.tables, z.pages_per_seq, z.heads, z.kv, z.slots, c.q, c.k, c.v, c.ldq, c.ldkv, c.ldo, c.arena, c.scale, c.window, c.keep, c.out, z.parts, z.tickets,
                           dc_kv16_rows(z.type) * (z.dim + 2), rows <= dc_kv16_rows(z.type), z.type != DC_TYPE_F32 && !prompts && rows > dc_kv16_rows(z.type) ? z.prompt_parts : nullptr,
                           ctx->num_sms, ctx->d_err};
     return z.dim == 128 ? launch_type<128>(ctx, c, p, prompts, rows <= 8) : launch_type<64>(ctx, c, p, prompts, rows <= 8);

@@ -79,24 +79,36 @@ struct Scale {
 };
 __device__ __forceinline__ float weight_inf(float x) { return x == INFINITY ? 1.0f : 0.0f; }      // beside an infinite largest
 
-// Eight neighbouring values of a row from index i on; `none` behind its end.
+// Eight neighbouring values of a row from index i on, as they lie: one or two loads of sixteen bytes.
 template <typename TX>
-__device__ __forceinline__ void load8(const TX* row, int i, int V, float none, float (&x)[8]) {
-    if (i + 8 <= V && ((uintptr_t)(row + i) & 15) == 0) {
-        if constexpr (sizeof(TX) == 2) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + i));
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct Eight {
+    uint4 v[sizeof(TX) / 2];
+    __device__ __forceinline__ static bool fits(const TX* row, int i, int V) { return i + 8 <= V && ((uintptr_t)(row + i) & 15) == 0; }
+    // `none` behind the row's end
+    __device__ __forceinline__ void load(const TX* row, int i, int V, float none) {
+        if (fits(row, i, V)) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[2 * k] = __uint_as_float(w[k] << 16), x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+            for (int k = 0; k < (int)sizeof(TX) / 2; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(row + i) + k);
         } else {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(row + i)), b = __ldg(reinterpret_cast<const float4*>(row + i) + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        }
-    } else {
+            alignas(16) TX x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = i + k < V ? value(row[i + k]) : none;
+            for (int k = 0; k < 8; ++k) x[k] = i + k < V ? row[i + k] : (TX)none;
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(TX) / 2; ++k) v[k] = reinterpret_cast<const uint4*>(x)[k];
+        }
     }
-}
+    __device__ __forceinline__ void values(float (&x)[8]) const {
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(TX) / 2; ++k) {
+            const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(TX) == 2) x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                else x[4 * k + j] = __uint_as_float(w[j]);
+            }
+        }
+    }
+};
 
 // Two parts of a row as one: sums against the larger maximum, the first largest.
 __device__ __forceinline__ Stat join(const Stat& a, const Stat& b, const Scale& c) {
@@ -121,7 +133,7 @@ __device__ __forceinline__ Stat warp_join(Stat s, const Scale& c) {
 // One CTA per (row, part).  Bound: HBM for many rows.
 template <typename TX>
 __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
-    constexpr int B = 4;      // tiles on their way at once
+    constexpr int B = sizeof(TX) == 2 ? 4 : 2;      // tiles on their way at once
     __shared__ Stat warps[VR_T / 32];
     pdl_wait();
     pdl_launch_dependents();
@@ -134,10 +146,17 @@ __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
     float most = -INFINITY;
     int where = 0x7fffffff;
     double sum = 0.0;
+    Eight<TX> next[B];
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) next[b].load(row, t0 + b < last ? (t0 + b) * VR_TILE + VR_PER * (int)threadIdx.x : p.V, p.V, -INFINITY);
+    };
+    if (first < last) fetch(first);
     for (int t0 = first; t0 < last; t0 += B) {
         float x[B][8];
 #pragma unroll
-        for (int b = 0; b < B; ++b) load8(row, t0 + b < last ? (t0 + b) * VR_TILE + VR_PER * (int)threadIdx.x : p.V, p.V, -INFINITY, x[b]);
+        for (int b = 0; b < B; ++b) next[b].values(x[b]);
+        if (t0 + B < last) fetch(t0 + B);      // (on their way meanwhile)
         float top = -INFINITY;
 #pragma unroll
         for (int b = 0; b < B; ++b)
@@ -166,7 +185,10 @@ __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) s[b] += c(x[b][k], most);
         }
-        sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+        float all = s[0];
+#pragma unroll
+        for (int b = 1; b < B; ++b) all += s[b];
+        sum += (double)all;
     }
     Stat s;
     s.sum = sum, s.most = most, s.first = where;
@@ -275,10 +297,18 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
     if constexpr (!PROBS) st = rows[k];
     const float inv = (float)(1.0 / st.sum);
     const bool none = !PROBS && !(st.most > -INFINITY);
-    auto drawn_from = [&](int i, bool residual, float (&w)[8]) {
+    struct Loaded {
+        Eight<TX> x;
+        Eight<float> q;
+    };
+    auto fetch = [&](int i, bool residual, Loaded& z) {
+        z.x.load(row, i, p.V, PROBS ? 0.0f : -INFINITY);
+        if (residual && qrow) z.q.load(qrow, i, p.V, 0.0f);
+    };
+    auto drawn_from = [&](int i, bool residual, const Loaded& z, float (&w)[8]) {
         float q[8];
-        load8(row, i, p.V, PROBS ? 0.0f : -INFINITY, w);
-        if (residual && qrow) load8(qrow, i, p.V, 0.0f, q);
+        z.x.values(w);
+        if (residual && qrow) z.q.values(q);
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             if constexpr (PROBS) w[x] = w[x] > 0.0f && w[x] <= 3.4028235e38f ? w[x] : 0.0f;
@@ -302,9 +332,13 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
     };
     const int tiles = (p.V + VR_TILE - 1) / VR_TILE, from = part * p.part_tiles, to = min(tiles, from + p.part_tiles);
     auto sum_tiles = [&](int from, int to, bool residual) {      // every warp's share of each tile
+        Loaded next;
+        if (from < to) fetch(from * VR_TILE + VR_PER * tid, residual, next);
         for (int t = from; t < to; ++t) {
+            const Loaded z = next;
+            if (t + 1 < to) fetch((t + 1) * VR_TILE + VR_PER * tid, residual, next);      // (on its way meanwhile)
             float w[8];
-            drawn_from(t * VR_TILE + VR_PER * tid, residual, w);
+            drawn_from(t * VR_TILE + VR_PER * tid, residual, z, w);
             double s = sum_of(w);
 #pragma unroll
             for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
@@ -383,7 +417,9 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
     if (s_total > 0.0) {
         float w[8];
         const int i0 = s_tile * VR_TILE + VR_PER * tid;
-        drawn_from(i0, residual, w);
+        Loaded z;
+        fetch(i0, residual, z);
+        drawn_from(i0, residual, z, w);
         double all, upto = scan(sum_of(w), s_warps[0], all);
         const double goal = (double)uc * s_total - s_before;
         int found = 0x7fffffff, last = -1;
