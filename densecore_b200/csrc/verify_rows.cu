@@ -63,19 +63,23 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// log2(e) / T in two terms.  Differences are held to 1e35, at which a weight is 0 for every scale from 1e-30 on: so NaN and -inf have none, and no product overflows.
+// log2(e) / T, rounded: what all weights of a request go by.  Differences are held to 1e35, at which a weight is 0 for every scale from 1e-30 on: so NaN and -inf have none, and no
+// product overflows.
 struct Scale {
-    float hi, lo;
+    float c;
     bool greedy;
     __device__ __forceinline__ explicit Scale(float T) {
         greedy = !(T > 0.0f);
-        const double c = greedy ? 1.0 : fmin(fmax(1.4426950408889634 / (double)T, 1e-30), 1e30);
-        hi = (float)c, lo = c < 1e10 ? (float)(c - (double)hi) : 0.0f;
+        c = greedy ? 1.0f : (float)fmin(fmax(1.4426950408889634 / (double)T, 1e-30), 1e30);
     }
-    __device__ __forceinline__ float operator()(float x, float most) const {      // x at or below `most`, which is finite
-        const float d = fmaxf(x - most, -1e35f);
-        return ex2(fmaf(d, hi, d * lo));
-    }
+    __device__ __forceinline__ float operator()(float x, float most) const { return ex2(fmaxf(x - most, -1e35f) * c); }      // x at or below `most`, which is finite
+};
+// The same weights with one multiply-add each: 2^(c x - hi) where c most = hi + lo exactly, so that each is 2^lo fold.  For products that leave lo below 1/32; NaN stays NaN.
+struct Quick {
+    float hi, lo;
+    bool is;
+    __device__ __forceinline__ Quick(const Scale& c, float most) : hi(c.c * most), lo(fmaf(c.c, most, -hi)), is(fabsf(hi) < 1048576.0f) {}
+    __device__ __forceinline__ float operator()(const Scale& c, float x) const { return ex2(fmaf(c.c, x, -hi)); }
 };
 __device__ __forceinline__ float weight_inf(float x) { return x == INFINITY ? 1.0f : 0.0f; }      // beside an infinite largest
 
@@ -130,7 +134,7 @@ __device__ __forceinline__ Stat warp_join(Stat s, const Scale& c) {
     return s;
 }
 
-// One CTA per (row, part).  Bound: HBM for many rows.
+// One CTA per (row, part).
 template <typename TX>
 __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
     constexpr int B = sizeof(TX) == 2 ? 4 : 2;      // tiles on their way at once
@@ -144,7 +148,7 @@ __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
     const Scale c(p.temperature ? p.temperature[r] : 1.0f);
     const int tiles = (p.V + VR_TILE - 1) / VR_TILE, first = part * ((tiles + p.stat_parts - 1) / p.stat_parts), last = min(tiles, first + (tiles + p.stat_parts - 1) / p.stat_parts);
     float most = -INFINITY;
-    int where = 0x7fffffff;
+    int where = 0x7fffffff;      // of a request that goes by the largest alone
     double sum = 0.0;
     Eight<TX> next[B];
     auto fetch = [&](int t0) {
@@ -165,29 +169,34 @@ __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
         if (top > most) {
             sum = most > -INFINITY && top < INFINITY ? sum * (double)c(most, top) : 0.0;
             most = top;
-            where = 0x7fffffff;
+            if (c.greedy) {
 #pragma unroll
-            for (int b = B - 1; b >= 0; --b)
+                for (int b = B - 1; b >= 0; --b)
 #pragma unroll
-                for (int k = 7; k >= 0; --k)
-                    if (x[b][k] == top) where = (t0 + b) * VR_TILE + VR_PER * (int)threadIdx.x + k;
+                    for (int k = 7; k >= 0; --k)
+                        if (x[b][k] == top) where = (t0 + b) * VR_TILE + VR_PER * (int)threadIdx.x + k;
+            }
         }
-        if (!(top > -INFINITY)) continue;      // nothing with a weight
+        if (!(top > -INFINITY) || c.greedy) continue;      // nothing with a weight, or nobody asks for it
         float s[B] = {};
-        if (most == INFINITY) {
+        const Quick q(c, most);
+        if (q.is) {
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) s[b] += weight_inf(x[b][k]);
-        } else {
-#pragma unroll
-            for (int b = 0; b < B; ++b)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) s[b] += c(x[b][k], most);
+                for (int k = 0; k < 8; ++k) s[b] += q(c, x[b][k]);
         }
         float all = s[0];
 #pragma unroll
         for (int b = 1; b < B; ++b) all += s[b];
+        all *= ex2(q.lo);
+        if (!(q.is && all < INFINITY)) {      // an infinite largest, a product too large, or a NaN among them
+            all = 0.0f;
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) all += most == INFINITY ? weight_inf(x[b][k]) : c(x[b][k], most);
+        }
         sum += (double)all;
     }
     Stat s;
@@ -292,11 +301,24 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
     const int k = s_n, own = k < n ? p.tokens[(size_t)k * p.R + r] : -1;
     const TX* row = target + (size_t)k * p.ld;
     const float* qrow = k < n && p.q ? p.q + ((size_t)k * p.R + r) * p.V : nullptr;
+    auto answer = [&](int token) {      // by the whole CTA
+        for (int i = tid; i <= p.D; i += VR_T) p.out[(size_t)r * (p.D + 1) + i] = i < k ? p.tokens[(size_t)i * p.R + r] : i == k ? token : -1;
+        if (tid == 0) {
+            p.accepted[r] = k;
+            if (p.rejected) p.rejected[r] = n - k;
+        }
+    };
     Stat st;
     st.sum = 1.0, st.most = 0.0f, st.first = 0;
-    if constexpr (!PROBS) st = rows[k];
-    const float inv = (float)(1.0 / st.sum);
-    const bool none = !PROBS && !(st.most > -INFINITY);
+    if constexpr (!PROBS) {
+        st = rows[k];
+        if (c.greedy || !(st.most > -INFINITY)) {      // all on one token, which stays whatever the draft had on it; or nothing
+            if (part == 0) answer(st.most > -INFINITY ? st.first : -1);
+            return;
+        }
+    }
+    const Quick quick(c, st.most);
+    const float inv = (float)(1.0 / st.sum), quick_inv = inv * ex2(quick.lo);
     struct Loaded {
         Eight<TX> x;
         Eight<float> q;
@@ -305,44 +327,63 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
         z.x.load(row, i, p.V, PROBS ? 0.0f : -INFINITY);
         if (residual && qrow) z.q.load(qrow, i, p.V, 0.0f);
     };
+    // (a weight that is NaN is below 0 by fmaxf)
     auto drawn_from = [&](int i, bool residual, const Loaded& z, float (&w)[8]) {
-        float q[8];
+        float f = 1.0f, q[8] = {};
         z.x.values(w);
-        if (residual && qrow) z.q.values(q);
+        if constexpr (PROBS) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            if constexpr (PROBS) w[x] = w[x] > 0.0f && w[x] <= 3.4028235e38f ? w[x] : 0.0f;
-            else if (none) w[x] = 0.0f;
-            else if (c.greedy) w[x] = i + x == st.first ? 1.0f : 0.0f;
-            else w[x] = (st.most == INFINITY ? weight_inf(w[x]) : c(w[x], st.most)) * inv;
-            if (residual) {
-                if (qrow) {
-                    if (q[x] > 0.0f && q[x] <= 3.4028235e38f) w[x] = fmaxf(w[x] - q[x], 0.0f);
-                } else if (i + x == own) {
-                    w[x] = fmaxf(w[x] - 1.0f, 0.0f);
-                }
-            }
+            for (int x = 0; x < 8; ++x) w[x] = w[x] <= 3.4028235e38f ? w[x] : 0.0f;
+        } else if (quick.is) {
+            f = quick_inv;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) w[x] = quick(c, w[x]);
+        } else {
+            f = inv;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) w[x] = st.most == INFINITY ? weight_inf(w[x]) : c(w[x], st.most);
         }
-    };
-    auto sum_of = [](const float (&w)[8]) {
-        double s = 0.0;
+        if (residual && qrow) {
+            z.q.values(q);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) s += (double)w[x];
-        return s;
+            for (int x = 0; x < 8; ++x) q[x] = fmaxf(q[x] <= 3.4028235e38f ? q[x] : 0.0f, 0.0f);
+        } else if (residual && own >= i && own < i + 8) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) q[x] = i + x == own ? 1.0f : 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) w[x] = fmaxf(fmaf(w[x], f, -q[x]), 0.0f);
     };
+    auto sum_of = [](const float (&w)[8]) { return (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]))); };
     const int tiles = (p.V + VR_TILE - 1) / VR_TILE, from = part * p.part_tiles, to = min(tiles, from + p.part_tiles);
     auto sum_tiles = [&](int from, int to, bool residual) {      // every warp's share of each tile
-        Loaded next;
-        if (from < to) fetch(from * VR_TILE + VR_PER * tid, residual, next);
-        for (int t = from; t < to; ++t) {
-            const Loaded z = next;
-            if (t + 1 < to) fetch((t + 1) * VR_TILE + VR_PER * tid, residual, next);      // (on its way meanwhile)
-            float w[8];
-            drawn_from(t * VR_TILE + VR_PER * tid, residual, z, w);
-            double s = sum_of(w);
+        constexpr int B = 2;
+        Loaded next[B];
+        auto begin = [&](int t) {
 #pragma unroll
-            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            if (lane == 0) s_warps[t][warp] = s;
+            for (int b = 0; b < B; ++b)
+                if (t + b < to) fetch((t + b) * VR_TILE + VR_PER * tid, residual, next[b]);
+        };
+        begin(from);
+        for (int t = from; t < to; t += B) {
+            double s[B];
+            Loaded z[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) z[b] = next[b];
+            begin(t + B);      // (on their way meanwhile)
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                float w[8];
+                drawn_from((t + b) * VR_TILE + VR_PER * tid, residual, z[b], w);
+                s[b] = sum_of(w);
+            }
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1)
+#pragma unroll
+                for (int b = 0; b < B; ++b) s[b] += __shfl_xor_sync(0xffffffffu, s[b], x);
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (lane == 0 && t + b < to) s_warps[t + b][warp] = s[b];
         }
         __syncthreads();
     };
@@ -393,12 +434,12 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
         else p.sums[(size_t)r * tiles + t] = s;
     }
     if (p.parts > 1) {
-        __threadfence();
         __syncthreads();
-        if (tid == 0) {
-            s_last = atomicAdd(p.tickets + r, 1) == p.parts - 1;
+        if (tid == 0) {      // (releases what the CTA's threads have stored ahead of the barrier, and acquires what the others' have)
+            int before;
+            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.tickets + r) : "memory");
+            s_last = before == p.parts - 1;
             if (s_last) p.tickets[r] = 0;
-            __threadfence();
         }
         __syncthreads();
         if (!s_last) return;
@@ -420,8 +461,10 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
         Loaded z;
         fetch(i0, residual, z);
         drawn_from(i0, residual, z, w);
-        double all, upto = scan(sum_of(w), s_warps[0], all);
+        // (a thread's sum is of f32 sums, those up to each of its tokens are of 64 bits: where rounding leaves none of them above the goal, it is its last with a weight)
+        double all, own_sum = sum_of(w), upto = scan(own_sum, s_warps[0], all);
         const double goal = (double)uc * s_total - s_before;
+        const bool mine = upto + own_sum > goal;
         int found = 0x7fffffff, last = -1;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -429,16 +472,13 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
             if (w[x] > 0.0f) last = i0 + x;
             if (upto > goal && w[x] > 0.0f) found = min(found, i0 + x);
         }
+        if (!mine) found = 0x7fffffff;
+        else if (found == 0x7fffffff && last >= 0) found = last;
         found = __reduce_min_sync(0xffffffffu, found), last = __reduce_max_sync(0xffffffffu, last);
         if (lane == 0) atomicMin(&s_token, found), atomicMax(&s_at_most, last);
     }
     __syncthreads();
-    const int token = s_token < p.V ? s_token : s_at_most;      // (rounding: the tile's last with a weight)
-    for (int i = tid; i <= p.D; i += VR_T) p.out[(size_t)r * (p.D + 1) + i] = i < k ? p.tokens[(size_t)i * p.R + r] : i == k ? token : -1;
-    if (tid == 0) {
-        p.accepted[r] = k;
-        if (p.rejected) p.rejected[r] = n - k;
-    }
+    answer(s_token < p.V ? s_token : s_at_most);      // (rounding: the tile's last with a weight)
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
