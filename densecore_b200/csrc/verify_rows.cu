@@ -26,7 +26,7 @@ using namespace dc;
 namespace {
 
 constexpr int VR_T = 256, VR_PER = 8, VR_TILE = VR_T * VR_PER, VR_DRAFTS = 64, VR_VOCAB = 389120, VR_TILES = VR_VOCAB / VR_TILE, VR_ROWS = 65536;
-constexpr int VR_STATS_CTAS = 16, VR_NEXT_CTAS = 4;      // an SM, where rows are cut into parts
+constexpr int VR_STATS_CTAS = 16, VR_NEXT_CTAS = 2;      // an SM, where rows are cut into parts
 constexpr int VR_PROBS = -1;
 
 struct alignas(16) Stat {      // of a part of a row
@@ -59,6 +59,27 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// pairs of f32 in a register pair: two results an instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(a));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -136,7 +157,7 @@ __device__ __forceinline__ Stat warp_join(Stat s, const Scale& c) {
 
 // One CTA per (row, part).
 template <typename TX>
-__global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
+__global__ void __launch_bounds__(VR_T, 4) k_verify_stats(const VerifyParams p) {
     constexpr int B = sizeof(TX) == 2 ? 4 : 2;      // tiles on their way at once
     __shared__ Stat warps[VR_T / 32];
     pdl_wait();
@@ -157,15 +178,26 @@ __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
     };
     if (first < last) fetch(first);
     for (int t0 = first; t0 < last; t0 += B) {
-        float x[B][8];
+        float x[B][8], top = -INFINITY;
+        if constexpr (sizeof(TX) == 2) {      // (pairs as they lie)
+            __nv_bfloat162 m = __floats2bfloat162_rn(-INFINITY, -INFINITY);
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const uint32_t w[4] = {next[b].v[0].x, next[b].v[0].y, next[b].v[0].z, next[b].v[0].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(w + k));
+            }
+            top = fmaxf(__low2float(m), __high2float(m));
+        }
 #pragma unroll
         for (int b = 0; b < B; ++b) next[b].values(x[b]);
         if (t0 + B < last) fetch(t0 + B);      // (on their way meanwhile)
-        float top = -INFINITY;
+        if constexpr (sizeof(TX) == 4) {
 #pragma unroll
-        for (int b = 0; b < B; ++b)
+            for (int b = 0; b < B; ++b)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) top = fmaxf(top, x[b][k]);
+                for (int k = 0; k < 8; ++k) top = fmaxf(top, x[b][k]);
+        }
         if (top > most) {
             sum = most > -INFINITY && top < INFINITY ? sum * (double)c(most, top) : 0.0;
             most = top;
@@ -178,18 +210,21 @@ __global__ void __launch_bounds__(VR_T) k_verify_stats(const VerifyParams p) {
             }
         }
         if (!(top > -INFINITY) || c.greedy) continue;      // nothing with a weight, or nobody asks for it
-        float s[B] = {};
+        float all = 0.0f;
         const Quick q(c, most);
         if (q.is) {
+            uint64_t s[2] = {0, 0};      // (two sums of pairs)
+            const uint64_t c2 = pair(c.c, c.c), h2 = pair(-q.hi, -q.hi);
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) s[b] += q(c, x[b][k]);
+                for (int k = 0; k < 8; k += 2) {
+                    const float2 y = unpair(fma2(pair(x[b][k], x[b][k + 1]), c2, h2));
+                    s[k / 2 & 1] = add2(s[k / 2 & 1], pair(ex2(y.x), ex2(y.y)));
+                }
+            const float2 z = unpair(add2(s[0], s[1]));
+            all = (z.x + z.y) * ex2(q.lo);
         }
-        float all = s[0];
-#pragma unroll
-        for (int b = 1; b < B; ++b) all += s[b];
-        all *= ex2(q.lo);
         if (!(q.is && all < INFINITY)) {      // an infinite largest, a product too large, or a NaN among them
             all = 0.0f;
 #pragma unroll
@@ -255,6 +290,12 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
         return;
     }
     const TX* target = reinterpret_cast<const TX*>(p.target) + (size_t)row0 * p.ld;
+    // ---- the drafts, a thread each: what decides on them, but for the rows' statistics, is on its way meanwhile
+    static_assert(VR_DRAFTS <= VR_T, "a thread a draft");
+    const int my_token = tid < n ? p.tokens[(size_t)tid * p.R + r] : -1;
+    const bool inside = my_token >= 0 && my_token < p.V;
+    float my_q = inside && p.q ? p.q[((size_t)tid * p.R + r) * p.V + my_token] : 1.0f;
+    const float my_x = inside ? value(target[(size_t)tid * p.ld + my_token]) : 0.0f, my_u = tid < n ? p.u[(size_t)r * (p.D + 1) + tid] : 0.0f;
     const Scale c(PROBS ? 1.0f : p.temperature ? p.temperature[r] : 1.0f);
     if constexpr (!PROBS) {
         for (int i = warp; i <= n; i += VR_T / 32) {
@@ -272,23 +313,20 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
         }
         __syncthreads();
     }
-    for (int i = tid; i < n; i += VR_T) {
-        const int t = p.tokens[(size_t)i * p.R + r];
+    if (tid < n) {
         bool good = false;
-        if (t >= 0 && t < p.V) {
-            float q = p.q ? p.q[((size_t)i * p.R + r) * p.V + t] : 1.0f;
-            if (!(q > 0.0f && q <= 3.4028235e38f)) q = 0.0f;
-            const float x = value(target[(size_t)i * p.ld + t]);
-            const double uq = (double)p.u[(size_t)r * (p.D + 1) + i] * (double)q;
+        if (inside) {
+            if (!(my_q > 0.0f && my_q <= 3.4028235e38f)) my_q = 0.0f;
+            const double uq = (double)my_u * (double)my_q;
             if constexpr (PROBS) {
-                good = uq < (x > 0.0f && x <= 3.4028235e38f ? (double)x : 0.0);
+                good = uq < (my_x > 0.0f && my_x <= 3.4028235e38f ? (double)my_x : 0.0);
             } else {
-                const Stat& s = rows[i];
+                const Stat& s = rows[tid];
                 if (s.most > -INFINITY)
-                    good = c.greedy ? uq < (t == s.first ? 1.0 : 0.0) : uq * s.sum < (double)(s.most == INFINITY ? weight_inf(x) : c(x, s.most));
+                    good = c.greedy ? uq < (my_token == s.first ? 1.0 : 0.0) : uq * s.sum < (double)(s.most == INFINITY ? weight_inf(my_x) : c(my_x, s.most));
             }
         }
-        s_good[i] = good;
+        s_good[tid] = good;
     }
     __syncthreads();
     if (tid == 0) {

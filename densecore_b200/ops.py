@@ -237,9 +237,8 @@ class Context:
     def verify_rows_dev(self, target: int, requests: int, vocab: int, max_drafts: int, draft_tokens: int, draft_probs: int, uniforms: int, tokens: int, accepted: int, rejected: int = 0,
                         starts: int = 0, n_drafts: int = 0, temperature: int = 0, rows: int = 0, ld: int = 0, dtype: str = "f32", probs: bool = False):
         """Drafted tokens of many requests against device-resident rows of the target (logits, or probabilities); all device addresses, enqueue only."""
-        self._check(_lib.lib().dc_b200_verify_rows_dev(self.handle, _dev(target), -1 if probs else _row_type(dtype), ld, rows or requests * (max_drafts + 1), vocab, requests, max_drafts,
-                                                       _dev(starts), _dev(n_drafts), _dev(draft_tokens), _dev(draft_probs), _dev(temperature), _dev(uniforms), _dev(tokens), _dev(accepted),
-                                                       _dev(rejected)))
+        self._check(_lib.lib().dc_b200_verify_rows_dev(self.handle, target, -1 if probs else _row_type(dtype), ld, rows or requests * (max_drafts + 1), vocab, requests, max_drafts, starts or None,
+                                                       n_drafts or None, draft_tokens or None, draft_probs or None, temperature or None, uniforms, tokens, accepted, rejected or None))
 
     def verify_rows(self, target: np.ndarray, draft_tokens, draft_probs, uniforms, n_drafts=None, temperature=None, probs: bool = False):
         """The same on host arrays: target [requests, drafts + 1, vocab], draft_tokens [drafts, requests], draft_probs [drafts, requests, vocab] or None, uniforms
@@ -507,7 +506,7 @@ class KVCacheDev:
 
     def step_dev(self, count: int, drop: int = 0, max_count: int = 1):
         """A step: every sequence loses its last drop[s] tokens and gets count[s] new ones (device addresses, 0: none), at most max_count; enqueue only."""
-        self.ctx._check(_lib.lib().dc_b200_kv_step_dev(self.ctx.handle, self.handle, _dev(drop), _dev(count), max_count))
+        self.ctx._check(_lib.lib().dc_b200_kv_step_dev(self.ctx.handle, self.handle, drop or None, count or None, max_count))
 
     def write_dev(self, layer: int, k: int, v: int, ld: int = 0):
         """Writes the step's rows (device addresses) into one layer, enqueue only."""
@@ -516,7 +515,7 @@ class KVCacheDev:
     def attend_dev(self, layer: int, q: int, k: int, v: int, scale: float, out: int, window: int = 0, keep_first: int = 0, ld_q: int = 0, ld_kv: int = 0, ld_out: int = 0):
         """Writes the step's rows (k = v = 0: they stand there already), then attends, over all earlier positions or the last `window` and the first `keep_first`;
         device addresses, enqueue only."""
-        self.ctx._check(_lib.lib().dc_b200_flash_attn_kv_dev(self.ctx.handle, self.handle, layer, _dev(q), ld_q, _dev(k), _dev(v), ld_kv, scale, window, keep_first, _dev(out), ld_out))
+        self.ctx._check(_lib.lib().dc_b200_flash_attn_kv_dev(self.ctx.handle, self.handle, layer, q or None, ld_q, k or None, v or None, ld_kv, scale, window, keep_first, out or None, ld_out))
 
     def read_page(self, layer: int, page: int):
         """The rows of one page, K and V, [16, n_kv, hd]: float16, or bits (uint16) of bf16."""
