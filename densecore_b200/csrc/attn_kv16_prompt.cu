@@ -42,6 +42,27 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// pairs of f32 in a register pair: two results an instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(a));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 template <typename TC>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     if constexpr (std::is_same<TC, __half>::value) {
@@ -202,27 +223,21 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                     const int kp = k0[i >> 4] + (i & 15);
                     return kp <= qp && (kp > qp - window || kp < p.keep);
                 };
-                int x[2][16] = {};      // 32 scores at a time, once for their largest and once for the weights: all 64 would not stay in registers
+                int x[4][16];
                 auto s = [&](int i) -> float { return __int_as_float(x[i >> 4][i & 15]); };
-                auto load = [&](int h) {
-                    tmem_ld16(t_s + 32 * h, x[0]);
-                    tmem_ld16(t_s + 32 * h + 16, x[1]);
-                    tmem_ld_wait(x[0]);
-                    tmem_ld_wait(x[1]);
-                    if (masked) {
+                __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!sees(32 * h + i)) x[i >> 4][i & 15] = __float_as_int(-INFINITY);
-                    }
-                };
+                for (int i = 0; i < 4; ++i) tmem_ld16(t_s + 16 * i, x[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld_wait(x[i]);
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (!sees(i)) x[i >> 4][i & 15] = __float_as_int(-INFINITY);
+                }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    __syncwarp();
-                    load(h);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s(i));
-                }
+                for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s(i));
                 if (!whole(t, first, last)) {      // (as warp 11 goes by)
                     const int stage = t % KP_STAGES;
                     ok = wait(bar(KP_FULL, stage), (t / KP_STAGES) & 1);
@@ -263,19 +278,24 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                         }
                     }
                 }
+                const uint64_t sl2_2 = pair(sl2, sl2), m_2 = pair(-m_run, -m_run);
+                uint64_t l_2[2] = {pair(l_run[0], l_run[1]), 0};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t w[16];
-                    __syncwarp();      // masks are a lane's own, loads and stores are the whole warp's
-                    load(h);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        w[i] = pack<TC>(ex2(fmaf(s(2 * i), sl2, -m_run)), ex2(fmaf(s(2 * i + 1), sl2, -m_run)));
+                        const float2 y = unpair(fma2(pair(s(32 * h + 2 * i), s(32 * h + 2 * i + 1)), sl2_2, m_2));
+                        w[i] = pack<TC>(ex2(y.x), ex2(y.y));
                         const float2 f = unpack<TC>(w[i]);
-                        l_run[i & 1] += f.x + f.y;
+                        l_2[i & 1] = add2(l_2[i & 1], pair(f.x, f.y));
                     }
-                    __syncwarp();
+                    __syncwarp();      // masks are a lane's own, stores are the whole warp's
                     tmem_st16(t_s + 16 * h, w);      // (columns whose scores have been read)
+                }
+                {
+                    const float2 f = unpair(add2(l_2[0], l_2[1]));
+                    l_run[0] = f.x, l_run[1] = f.y;
                 }
                 tmem_st_wait();
                 tc_fence_before();
