@@ -106,10 +106,10 @@ constexpr size_t rows_smem() { return (size_t)KR_SLOTS * dc_kv16_rec<HD>::BYTES 
 
 // The parts of prompt-sized sequences' rows whose keys were split, in their order: a warp per JR rows, a lane HD / 32 dimensions.
 template <int HD, typename TX>
-__device__ __forceinline__ void join_prompts(const RowsParams& p, int n_entries, int G) {
+__device__ __forceinline__ void join_prompts(const RowsParams& p, int G) {
     constexpr int D = HD / 32, JR = 4;
     const int lane = threadIdx.x & 31;
-    const TileLine tiles(p.entries, n_entries, G, 64, p.n_kv, p.num_sms);
+    const TileLine tiles(p.entries, p.numbers + DC_KV_ENTRIES, p.slots, G, 64, p.n_kv, p.num_sms);
     if (tiles.most == 1) return;
     const size_t step = (size_t)p.n_kv * kp_part_floats<HD>();
     const int warps = gridDim.x * gridDim.y * KR_WARPS, units = tiles.n_all * p.n_kv * (KP_TILE_ROWS / JR);
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
     if constexpr (NT == 2 && !PROMPTS) {
         if (p.prompt_parts) {
             pdl_wait();
-            join_prompts<HD, TX>(p, n_entries, G);
+            join_prompts<HD, TX>(p, G);
         }
     }
 }

@@ -87,7 +87,7 @@ __device__ __forceinline__ uint64_t umma_desc_sw32(uint32_t saddr) {
 struct PromptParams {
     const dc_kv_entry* entries;
     const int32_t *numbers, *tables;
-    int pages_per_seq, heads, n_kv, least, num_sms;      // least: sequences of more rows than this
+    int pages_per_seq, slots, heads, n_kv, least, num_sms;      // least: sequences of more rows than this
     const void* q;
     int64_t ldq, ldo;
     const uint8_t* arena;
@@ -117,27 +117,30 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, kvh = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv, G = p.heads / p.n_kv;
     pdl_wait();
     // ---- the item: which tile of rows, and which part of its keys
-    const TileLine tiles(p.entries, p.numbers[DC_KV_ENTRIES], G, p.least, p.n_kv, p.num_sms);
+    const TileLine tiles(p.entries, p.numbers + DC_KV_ENTRIES, p.slots, G, p.least, p.n_kv, p.num_sms);
     if (blockIdx.x == 0 && tid == 0 && (long long)tiles.n_all * p.n_kv > gridDim.x) atomicExch(err, DC_ERR_STEP);      // (a step of more than the launch was made for)
     const int line = item / tiles.most, part = item % tiles.most;
     if (line >= tiles.n_all) return;
     const Tile tl(tiles, line, p.window, p.keep);
     if (part >= tl.n_parts) return;
     const dc_kv_entry own = tl.e;
-    const int row0 = tl.row0, rows = tl.rows, sets = rows > KP_ROWS ? 2 : 1, first = tl.first, last = tl.last, window = p.window ? p.window : 0x7fffffff, n_pages = tl.pages.n, n_parts = tl.n_parts;
+    const int row0 = tl.row0, rows = tl.rows, sets = rows > KP_ROWS ? 2 : 1, first = tl.first, last = tl.last, window = p.window ? p.window : 0x7fffffff, n_pages = tl.pages.n, n_parts = tl.n_parts, kept = tl.pages.kept, low = tl.pages.low;
     const int tile0 = (int)((long long)tl.key_tiles * part / n_parts), n_tiles = (int)((long long)tl.key_tiles * (part + 1) / n_parts) - tile0;
     auto page_at = [&](int i) { return tl.pages.at(i); };
     // position of the first key of page i of tile t; far behind the last token where there is none
     auto key_at = [&](int t, int i) { return 4 * (tile0 + t) + i < n_pages ? page_at(4 * (tile0 + t) + i) * DC_KV_BLOCK : 0x40000000; };
-    auto whole = [&](int t, int least, int most_pos) {      // whether tokens at positions least .. most_pos see all of a tile
-        bool all = true;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k0 = key_at(t, i);
-            all = all && k0 + DC_KV_BLOCK - 1 <= least && (k0 > most_pos - window || k0 + DC_KV_BLOCK <= p.keep);
-        }
-        return all;
+    // Tiles that tokens at positions least .. greatest see all of: a run of them, of those that have no kept page
+    struct Run {
+        int from;
+        uint32_t n;
+        __device__ __forceinline__ bool operator()(int t) const { return (uint32_t)(t - from) < n; }
     };
+    auto run_of = [&](int least, int greatest) -> Run {
+        const int seen_from = max(tl.pages.low * DC_KV_BLOCK, greatest - window + 1), pages_to = min((least + 1) / DC_KV_BLOCK, n_pages - kept + low);      // the first key, the first page behind
+        const int page_from = (seen_from + DC_KV_BLOCK - 1) / DC_KV_BLOCK, from = max(0, (page_from - low + kept + 3) / 4 - tile0), to = (pages_to - low + kept) / 4 - tile0;
+        return {from, (uint32_t)max(0, to - from)};
+    };
+    const Run whole = run_of(first, last);
     const uint32_t sm = (smem_u32(smem) + 1023u) & ~1023u;
     uint8_t* const base = smem + (sm - smem_u32(smem));
     auto bar = [sm](int which, int i = 0) -> uint32_t { return sm + L::BARS + 8u * (uint32_t)(which + i); };
@@ -167,32 +170,40 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
             const int warp_row = row0 + KP_ROWS * u + 32 * (warp & 3), n_own = own.count * G - warp_row;      // the warp's first row, rows from there on
             const int my_token = min((row0 + r) / G, own.count - 1), qp = own.pos0 + my_token;
             const int w_first = own.pos0 + min(warp_row / G, own.count - 1), w_last = own.pos0 + min((warp_row + 31) / G, own.count - 1);
+            const Run whole_here = run_of(w_first, w_last);
             // ---- the warp's queries, neighbouring lanes along a row; negated where the scale is negative
             const uint32_t area = sm + u * L::SET + 32 * (warp & 3) * 128;      // the warp's 32 rows; after the last product they hold its results
-            constexpr int LANES = HD / 8, PER = 32 / LANES, BATCH = 4;           // lanes of a row, rows at a time
+            constexpr int LANES = HD / 8, PER = 32 / LANES, ROUNDS = 32 / PER;      // lanes of a row, rows at a time, times
             const int c8 = lane % LANES;
             auto row_at = [&](int i) { return PER * i + lane / LANES; };        // (of the warp's 32)
             auto place = [&](int rr, int c) { return area + (c >> 3) * (KP_ROWS * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4); };
-            auto element = [&](int rr, int64_t ld) {
-                const int x = warp_row + rr, j = x / G;
-                return (size_t)(own.tok0 + j) * ld + (size_t)(kvh * G + x - j * G) * HD;
+            // the lane's rows in turn: where token and head of each lie in rows of queries or results
+            struct Walk {
+                int j, g;
             };
-            const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll 1
-            for (int i0 = 0; i0 < 32 / PER; i0 += BATCH) {
-                uint4 v[BATCH];
+            const Walk walk0 = {(warp_row + lane / LANES) / G, (warp_row + lane / LANES) % G};
+            auto on = [&](Walk& x) {
+                x.g += PER;
+                while (x.g >= G) x.g -= G, ++x.j;      // (once at most, but for G < PER)
+            };
+            auto element = [&](const Walk& x, int64_t ld) { return (size_t)(own.tok0 + x.j) * ld + (size_t)(kvh * G + x.g) * HD + 8 * c8; };
+            const int n_rows = min(n_own, rows - KP_ROWS * u - 32 * (warp & 3));      // rows that there are, of the warp's 32
+            {
+                const uint32_t sign = p.scale < 0.0f ? 0x80008000u : 0u;
+                uint4 v[ROUNDS];      // (all on their way at once)
+                Walk x = walk0;
 #pragma unroll
-                for (int i = 0; i < BATCH; ++i) {
-                    const int rr = row_at(i0 + i);
+                for (int i = 0; i < ROUNDS; ++i) {
                     v[i] = make_uint4(0, 0, 0, 0);
-                    if (rr < n_own && rr + 32 * (warp & 3) + KP_ROWS * u < rows) {
-                        const uint16_t* at = reinterpret_cast<const uint16_t*>(p.q) + element(rr, p.ldq) + 8 * c8;
+                    if (row_at(i) < n_rows) {
+                        const uint16_t* at = reinterpret_cast<const uint16_t*>(p.q) + element(x, p.ldq);
                         if (((uintptr_t)at & 15) == 0) v[i] = __ldg(reinterpret_cast<const uint4*>(at));
                         else v[i] = make_uint4(at[0] | (uint32_t)at[1] << 16, at[2] | (uint32_t)at[3] << 16, at[4] | (uint32_t)at[5] << 16, at[6] | (uint32_t)at[7] << 16);
                     }
+                    on(x);
                 }
 #pragma unroll
-                for (int i = 0; i < BATCH; ++i) sts128(place(row_at(i0 + i), c8), v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign);
+                for (int i = 0; i < ROUNDS; ++i) sts128(place(row_at(i), c8), v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign);
             }
             uint32_t* sick = reinterpret_cast<uint32_t*>(base + L::SICK) + r * (HD / 32);      // the row's dimensions that have met a value that is no number
 #pragma unroll
@@ -215,7 +226,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                 ok = wait(bar(KP_S, 2 * u + (t & 1)), (t >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
-                const bool masked = !whole(t, w_first, w_last);
+                const bool masked = !whole_here(t);
                 int k0[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) k0[i] = key_at(t, i);
@@ -223,7 +234,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                     const int kp = k0[i >> 4] + (i & 15);
                     return kp <= qp && (kp > qp - window || kp < p.keep);
                 };
-                int x[4][16];
+                int x[4][16] = {};
                 auto s = [&](int i) -> float { return __int_as_float(x[i >> 4][i & 15]); };
                 __syncwarp();
 #pragma unroll
@@ -238,7 +249,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s(i));
-                if (!whole(t, first, last)) {      // (as warp 11 goes by)
+                if (!whole(t)) {      // (as warp 11 goes by)
                     const int stage = t % KP_STAGES;
                     ok = wait(bar(KP_FULL, stage), (t / KP_STAGES) & 1);
                     if (!ok) break;
@@ -310,7 +321,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                 bool any_sick = false;
 #pragma unroll
                 for (int i = 0; i < HD / 32; ++i) any_sick = any_sick || sick[i];
-                const int n_rows = min(n_own, rows - KP_ROWS * u - 32 * (warp & 3));
                 // rows by way of shared memory, so that neighbouring lanes store along a row; f32 parts 64 dimensions at a time
                 if (n_parts == 1) {
                     const float mul = 1.0f / l;
@@ -331,17 +341,22 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                         for (int i = 0; i < 2; ++i) sts128(place(lane, 2 * c + i), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                     }
                     __syncwarp();
-#pragma unroll 8
-                    for (int i = 0; i < 32 / PER; ++i) {
-                        const int rr = row_at(i);
-                        const uint4 v = lds128(place(rr, c8));
-                        if (rr >= n_rows) continue;
-                        uint16_t* at = reinterpret_cast<uint16_t*>(p.out) + element(rr, p.ldo) + 8 * c8;
-                        if (((uintptr_t)at & 15) == 0) {
-                            *reinterpret_cast<uint4*>(at) = v;
-                        } else {
-                            at[0] = v.x & 0xFFFF, at[1] = v.x >> 16, at[2] = v.y & 0xFFFF, at[3] = v.y >> 16, at[4] = v.z & 0xFFFF, at[5] = v.z >> 16, at[6] = v.w & 0xFFFF, at[7] = v.w >> 16;
+                    uint4 v[ROUNDS];
+#pragma unroll
+                    for (int i = 0; i < ROUNDS; ++i) v[i] = lds128(place(row_at(i), c8));
+                    Walk x = walk0;
+#pragma unroll
+                    for (int i = 0; i < ROUNDS; ++i) {
+                        if (row_at(i) < n_rows) {
+                            uint16_t* at = reinterpret_cast<uint16_t*>(p.out) + element(x, p.ldo);
+                            if (((uintptr_t)at & 15) == 0) {
+                                *reinterpret_cast<uint4*>(at) = v[i];
+                            } else {
+                                const uint4 f = v[i];
+                                at[0] = f.x & 0xFFFF, at[1] = f.x >> 16, at[2] = f.y & 0xFFFF, at[3] = f.y >> 16, at[4] = f.z & 0xFFFF, at[5] = f.z >> 16, at[6] = f.w & 0xFFFF, at[7] = f.w >> 16;
+                            }
                         }
+                        on(x);
                     }
                 } else {
                     float* to = p.parts + ((size_t)(line * tiles.most + part) * p.n_kv + kvh) * kp_part_floats<HD>() + (KP_ROWS * u + 32 * (warp & 3)) * (HD + 4);
@@ -364,7 +379,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                         }
                         __syncwarp();
 #pragma unroll 4
-                        for (int i = 0; i < 32 / PER; ++i) {
+                        for (int i = 0; i < ROUNDS; ++i) {
                             const int rr = row_at(i);
                             const uint4 v = lds128(place(rr, c8));
                             if (rr < n_rows) *reinterpret_cast<uint4*>(to + (size_t)rr * (HD + 4) + 4 * LN * g + 4 * c8) = v;
@@ -384,7 +399,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
         for (int t = 0; t < n_tiles; ++t) {
             const int stage = t % KP_STAGES;
             if (t >= KP_STAGES && !wait(bar(KP_FREE, stage), (t / KP_STAGES - 1) & 1)) break;
-            const uint32_t b = whole(t, first, last) ? bar(KP_FULL, stage) : bar(KP_PRE, stage);
+            const uint32_t b = whole(t) ? bar(KP_FULL, stage) : bar(KP_PRE, stage);
             if (lane == 0) mbar_expect_tx(b, 2 * L::TILE);
             __syncwarp();
             if (lane < 4) {
@@ -399,7 +414,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
         // ------------------------------------------------------------------ values of tiles that not all rows see all of
         uint32_t uses = 0;      // of the stages' first barriers, odd or even
         for (int t = 0; t < n_tiles; ++t) {
-            if (whole(t, first, last)) continue;
+            if (whole(t)) continue;
             const int stage = t % KP_STAGES;
             if (!wait(bar(KP_PRE, stage), uses >> stage & 1)) break;
             uses ^= 1u << stage;
@@ -506,7 +521,7 @@ int dc_launch_kv16_prompt(dc_ctx* ctx, const dc_kv16_call& c) {
     // tiles: at most one that is not full for every sequence with that many new tokens
     const long long least = dc_kv16_rows(z.type) / G + 1, tiles = tokens * G / KP_TILE_ROWS + std::min((long long)z.slots, tokens / least);
     const int items = (int)std::max(tiles, (long long)std::max(1, ctx->num_sms / z.kv));
-    const PromptParams p = {z.entries, z.numbers, z.tables, z.pages_per_seq, z.heads, z.kv, dc_kv16_rows(z.type), ctx->num_sms, c.q, c.ldq, c.ldo, c.arena, c.scale, c.window, c.keep, c.out,
+    const PromptParams p = {z.entries, z.numbers, z.tables, z.pages_per_seq, z.slots, z.heads, z.kv, dc_kv16_rows(z.type), ctx->num_sms, c.q, c.ldq, c.ldo, c.arena, c.scale, c.window, c.keep, c.out,
                             z.prompt_parts};
     if (z.type == DC_TYPE_F16) return z.dim == 128 ? launch<128, __half>(ctx, p, items) : launch<64, __half>(ctx, p, items);
     return z.dim == 128 ? launch<128, __nv_bfloat16>(ctx, p, items) : launch<64, __nv_bfloat16>(ctx, p, items);

@@ -27,12 +27,19 @@ struct TileLine {
     const dc_kv_entry* entries;
     int n_entries, G, least, n_all, most;      // n_all: tiles; most: parts of a tile's keys at most, where there are fewer tiles than SMs
     __device__ __forceinline__ int tiles_of(const dc_kv_entry& e) const {
-        const long long rows = (long long)e.count * G;
-        return rows > least ? (int)((rows + KP_TILE_ROWS - 1) / KP_TILE_ROWS) : 0;
+        const int rows = e.count * G;      // (at most 2^30, as the whole step's)
+        return rows > least ? (rows + KP_TILE_ROWS - 1) / KP_TILE_ROWS : 0;
     }
-    __device__ __forceinline__ dc_kv_entry entry(int i) const { return i < n_entries ? entries[i] : dc_kv_entry{0, 0, 0, 0}; }
-    __device__ TileLine(const dc_kv_entry* e, int n, int G_, int least_, int n_kv, int num_sms) : entries(e), n_entries(n), G(G_), least(least_), n_all(0) {
-        for (int base = 0; base < n; base += 32) n_all += tiles_of(entry(base + (threadIdx.x & 31)));
+    dc_kv_entry early;      // the lane's of the first 32, on its way with their number
+    __device__ __forceinline__ dc_kv_entry entry(int base) const {
+        const int i = base + (threadIdx.x & 31);
+        return i >= n_entries ? dc_kv_entry{0, 0, 0, 0} : base == 0 ? early : entries[i];
+    }
+    // slots: room for entries
+    __device__ __forceinline__ TileLine(const dc_kv_entry* e, const int32_t* n, int slots, int G_, int least_, int n_kv, int num_sms) : entries(e), G(G_), least(least_), n_all(0) {
+        early = e[min((int)(threadIdx.x & 31), slots - 1)];
+        n_entries = *n;
+        for (int base = 0; base < n_entries; base += 32) n_all += tiles_of(entry(base));
         n_all = __reduce_add_sync(0xffffffffu, n_all);
         most = n_all ? max(1, num_sms / (int)min((long long)n_all * n_kv, (long long)num_sms)) : 1;
     }
@@ -43,11 +50,11 @@ struct Tile {
     Pages pages;
     int key_tiles, n_parts;
     // tile i of the line, i < n_all
-    __device__ Tile(const TileLine& z, int i, int window, int keep) {
+    __device__ __forceinline__ Tile(const TileLine& z, int i, int window, int keep) {
         const int lane = threadIdx.x & 31;
         int before = 0, tile = 0;
         for (int base = 0;; base += 32) {
-            e = z.entry(base + lane);
+            e = z.entry(base);
             const int mine = z.tiles_of(e);
             int upto = mine;
 #pragma unroll

@@ -226,8 +226,8 @@ __global__ void k_kv_stack(int32_t* stack, int n) {      // so that pages are ha
 
 // ---------------------------------------------------------------- new rows into the cache
 struct WriteParams {
-    const int32_t *starts, *counts, *slot_map, *positions, *seqs;
-    int slots, n_kv, more_than;      // counts that are not more than this are left out
+    const int32_t *starts, *counts, *slot_map, *seqs;
+    int slots, max_tokens, n_kv, more_than;      // counts that are not more than this are left out
     const void *k, *v;
     int64_t ld;
     uint8_t* arena;
@@ -242,9 +242,9 @@ __device__ __forceinline__ __half held_as<__half, __half>(__half x) { return x; 
 template <>
 __device__ __forceinline__ __nv_bfloat16 held_as<__nv_bfloat16, __nv_bfloat16>(__nv_bfloat16 x) { return x; }
 
-// A warp per (run of new tokens within a page, key head); a lane has HD / 32 neighbouring dimensions.  Values are turned in registers: a dimension's tokens leave in
-// sixteen-byte pieces where eight of them are new, one by one otherwise.
-// Bound: latency of one round of loads; a prompt's by its rows.
+// A warp per (half of a run of new tokens within a page, key head); a lane has HD / 32 neighbouring dimensions.  Values are turned in registers: a dimension's tokens leave
+// in sixteen-byte pieces where eight of them are new, one by one otherwise.
+// Bound: latency of two rounds of loads, the tokens' places and the rows; a prompt's by its rows.
 template <int HD, typename TX, typename TC>
 __global__ void __launch_bounds__(128) k_kv16_write(const WriteParams p) {
     using R = dc_kv16_rec<HD>;
@@ -254,63 +254,61 @@ __global__ void __launch_bounds__(128) k_kv16_write(const WriteParams p) {
     };
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, T = p.starts[p.slots], head = blockIdx.y, d0 = PER * lane;
+    const int lane = threadIdx.x & 31, head = blockIdx.y, half = blockIdx.z, d0 = PER * lane;
+    const bool vec = (((uintptr_t)p.k | (uintptr_t)p.v | (size_t)p.ld * sizeof(TX)) & (PER * sizeof(TX) - 1)) == 0;
+    int T = 0x7fffffff;
     for (int t0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * DC_KV_BLOCK; t0 < T; t0 += gridDim.x * 4 * DC_KV_BLOCK) {
-        // lane i: whether token t0 + i begins a run
-        int pos = 0, seq = -1;
-        const int t = t0 + lane;
-        bool begins = false;
-        if (lane < DC_KV_BLOCK && t < T) {
-            pos = p.positions[t], seq = p.seqs[t];
-            begins = (pos % DC_KV_BLOCK == 0 || t == p.starts[seq]) && p.counts[seq] > p.more_than;
-        }
-        for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo; todo &= todo - 1) {
-            const int from = __ffs(todo) - 1, tok = t0 + from, at = __shfl_sync(0xffffffffu, pos, from) % DC_KV_BLOCK, s = __shfl_sync(0xffffffffu, seq, from);
-            const int n = min(DC_KV_BLOCK - at, p.starts[s + 1] - tok), page = p.slot_map[tok] / DC_KV_BLOCK;
-            uint8_t* rec = p.arena + ((size_t)page * p.n_kv + head) * R::BYTES;
-            const bool vec = (((uintptr_t)p.k | (uintptr_t)p.v | (size_t)p.ld * sizeof(TX)) & (PER * sizeof(TX) - 1)) == 0;
+        // lane i: where token t0 + i lies, and whether it begins a run; the runs that begin with the first sixteen are the warp's
+        const int t = min(t0 + lane, p.max_tokens - 1), slot = p.slot_map[t], seq = p.seqs[t], before = p.seqs[max(t - 1, 0)];
+        T = p.starts[p.slots];
+        const bool there = t0 + lane < T, begins = there && (slot % DC_KV_BLOCK == 0 || t == 0 || before != seq);
+        const uint32_t all = __ballot_sync(0xffffffffu, begins), live = __ballot_sync(0xffffffffu, there);
+        for (uint32_t todo = all & 0xFFFFu; todo; todo &= todo - 1) {
+            const int from = __ffs(todo) - 1, tok = t0 + from, s = __shfl_sync(0xffffffffu, slot, from), at = s % DC_KV_BLOCK;
+            const uint32_t behind = (all & ~((2u << from) - 1u)) | ~live;      // what ends the run
+            const int n = (behind ? __ffs(behind) - 1 : 32) - from;
+            const bool wanted = p.more_than == 0 || p.counts[__shfl_sync(0xffffffffu, seq, from)] > p.more_than;
+            if (at >= 8 * half + 8 || at + n <= 8 * half) continue;
             const TX *k = reinterpret_cast<const TX*>(p.k) + (size_t)tok * p.ld + (size_t)head * HD + d0, *v = reinterpret_cast<const TX*>(p.v) + (size_t)tok * p.ld + (size_t)head * HD + d0;
+            alignas(16) TX x[2][8][PER] = {};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {      // tokens of the page's slots 8 half ..
-                if (at >= 8 * half + 8 || at + n <= 8 * half) continue;
-                alignas(16) TC kv[8][PER], vv[PER][8];
+            for (int i = 0; i < 8; ++i) {
+                const int j = 8 * half + i - at;
+                if (j < 0 || j >= n) continue;
+                const TX *ks = k + (int64_t)j * p.ld, *vs = v + (int64_t)j * p.ld;
+                if (vec) {
+                    *reinterpret_cast<Piece*>(x[0][i]) = *reinterpret_cast<const Piece*>(ks);
+                    *reinterpret_cast<Piece*>(x[1][i]) = *reinterpret_cast<const Piece*>(vs);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = 8 * half + i - at;
-                    const bool in = j >= 0 && j < n;
-                    alignas(16) TX x[2][PER] = {};
-                    if (in) {
-                        const TX *ks = k + (int64_t)j * p.ld, *vs = v + (int64_t)j * p.ld;
-                        if (vec) {
-                            *reinterpret_cast<Piece*>(x[0]) = *reinterpret_cast<const Piece*>(ks);
-                            *reinterpret_cast<Piece*>(x[1]) = *reinterpret_cast<const Piece*>(vs);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < PER; ++c) x[0][c] = ks[c], x[1][c] = vs[c];
-                        }
-                    }
-#pragma unroll
-                    for (int c = 0; c < PER; ++c) kv[i][c] = held_as<TC, TX>(x[0][c]), vv[c][i] = held_as<TC, TX>(x[1][c]);
+                    for (int c = 0; c < PER; ++c) x[0][i][c] = ks[c], x[1][i][c] = vs[c];
                 }
+            }
+            if (!wanted) continue;
+            uint8_t* rec = p.arena + ((size_t)(s / DC_KV_BLOCK) * p.n_kv + head) * R::BYTES;
+            alignas(16) TC kv[8][PER], vv[PER][8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < PER; ++c) kv[i][c] = held_as<TC, TX>(x[0][i][c]), vv[c][i] = held_as<TC, TX>(x[1][i][c]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = 8 * half + i - at;
+                if (j < 0 || j >= n) continue;
+                uint8_t* to = rec + R::key(8 * half + i, d0);
+                if constexpr (PER == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(kv[i]);
+                else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(kv[i]);
+            }
+            if (at <= 8 * half && at + n >= 8 * half + 8) {
+#pragma unroll
+                for (int c = 0; c < PER; ++c) *reinterpret_cast<uint4*>(rec + R::value(8 * half, d0 + c)) = *reinterpret_cast<const uint4*>(vv[c]);
+            } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int j = 8 * half + i - at;
                     if (j < 0 || j >= n) continue;
-                    uint8_t* to = rec + R::key(8 * half + i, d0);
-                    if constexpr (PER == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(kv[i]);
-                    else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(kv[i]);
-                }
-                if (at <= 8 * half && at + n >= 8 * half + 8) {
 #pragma unroll
-                    for (int c = 0; c < PER; ++c) *reinterpret_cast<uint4*>(rec + R::value(8 * half, d0 + c)) = *reinterpret_cast<const uint4*>(vv[c]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int j = 8 * half + i - at;
-                        if (j < 0 || j >= n) continue;
-#pragma unroll
-                        for (int c = 0; c < PER; ++c) *reinterpret_cast<TC*>(rec + R::value(8 * half + i, d0 + c)) = vv[c][i];
-                    }
+                    for (int c = 0; c < PER; ++c) *reinterpret_cast<TC*>(rec + R::value(8 * half + i, d0 + c)) = vv[c][i];
                 }
             }
         }
@@ -366,15 +364,16 @@ int create(dc_ctx* ctx, dc_kv_cache* kv) {
 
 template <int HD, typename TX, typename TC>
 int launch_write(dc_ctx* ctx, const dc_kv_dev& z, const WriteParams& p) {
-    const int ctas = std::min((z.max_tokens + 4 * DC_KV_BLOCK - 1) / (4 * DC_KV_BLOCK), ctx->num_sms * 8);
-    return dc_launch(ctx, "k_kv16_write", k_kv16_write<HD, TX, TC>, dim3(ctas, z.kv), dim3(128), 0, p);
+    const long long tokens = std::min<long long>(z.max_tokens, (long long)z.slots * z.max_count);
+    const int ctas = (int)std::min<long long>((tokens + 4 * DC_KV_BLOCK - 1) / (4 * DC_KV_BLOCK), ctx->num_sms * 4);
+    return dc_launch(ctx, "k_kv16_write", k_kv16_write<HD, TX, TC>, dim3(ctas, z.kv, 2), dim3(128), 0, p);
 }
 
 }  // namespace
 
 int dc_launch_kv16_write(dc_ctx* ctx, const dc_kv_cache* kv, uint8_t* arena, const void* k, const void* v, int64_t ld, bool prompts_only) {
     const dc_kv_dev& z = *kv->dev;
-    const WriteParams p = {z.starts, z.counts, z.slot_map, z.positions, z.seqs, z.slots, z.kv, prompts_only ? dc_kv16_rows(z.type) / (z.heads / z.kv) : 0, k, v, ld, arena};
+    const WriteParams p = {z.starts, z.counts, z.slot_map, z.seqs, z.slots, z.max_tokens, z.kv, prompts_only ? dc_kv16_rows(z.type) / (z.heads / z.kv) : 0, k, v, ld, arena};
     if (z.dim == 128)
         return z.type == DC_TYPE_F32 ? launch_write<128, float, __half>(ctx, z, p)
                : z.type == DC_TYPE_F16 ? launch_write<128, __half, __half>(ctx, z, p) : launch_write<128, __nv_bfloat16, __nv_bfloat16>(ctx, z, p);
@@ -463,6 +462,7 @@ int dc_b200_kv_dev_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void
     if (ld_kv == 0) ld_kv = (int64_t)z.kv * z.dim;
     if (!k_dev || !v_dev || ld_kv < (int64_t)z.kv * z.dim || ((uintptr_t)k_dev | (uintptr_t)v_dev) % element(z.type))
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_dev_write_dev: bad argument (row stride %lld)", (long long)ld_kv);
+    if (z.max_count == 0) return DC_B200_OK;
     cudaSetDevice(ctx->device);
     return dc_launch_kv16_write(ctx, kv, z.arena + z.layer_bytes * layer, k_dev, v_dev, ld_kv, false);
 }
