@@ -355,8 +355,7 @@ int create(dc_ctx* ctx, dc_kv_cache* kv) {
     auto ints = [&](size_t from) { return (int32_t*)(z.memory + from); };
     z.lens = ints(lens), z.held = ints(held), z.counts = ints(counts), z.starts = ints(starts), z.tables = ints(tables), z.slot_map = ints(map), z.positions = ints(positions), z.seqs = ints(seqs);
     z.numbers = ints(numbers), z.entries = (dc_kv_entry*)(z.memory + entries), z.scratch = ints(scratch), z.tickets = ints(tickets), z.stack = ints(stack), z.parts = (float*)(z.memory + parts), z.prompt_parts = (float*)(z.memory + prompt_parts);
-    k_kv_stack<<<std::min((z.pages + 255) / 256, ctx->num_sms * 4), 256, 0, ctx->stream>>>(z.stack, z.pages);
-    DC_TRY(dc_check_cuda(ctx, cudaGetLastError(), "k_kv_stack"));
+    DC_TRY(dc_launch_drained(ctx, "k_kv_stack", k_kv_stack, dim3(std::min((z.pages + 255) / 256, ctx->num_sms * 4)), dim3(256), 0, z.stack, z.pages));
     const int32_t free_pages = z.pages;
     DC_TRY(dc_check_cuda(ctx, cudaMemcpyAsync(z.numbers + DC_KV_FREE, &free_pages, 4, cudaMemcpyHostToDevice, ctx->stream), "kv_create_dev"));
     return dc_check_cuda(ctx, cudaStreamSynchronize(ctx->stream), "kv_create_dev");
