@@ -54,7 +54,7 @@ template <typename TC>
 struct Two;      // pairs of the cache's type in a word
 template <>
 struct Two<__half> {
-    static constexpr uint32_t EXPONENTS = 0x7C007C00u;
+    static constexpr uint32_t EXPONENTS = 0x7C007C00u, ONE = 0x04000400u;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -63,7 +63,7 @@ struct Two<__half> {
 };
 template <>
 struct Two<__nv_bfloat16> {
-    static constexpr uint32_t EXPONENTS = 0x7F807F80u;
+    static constexpr uint32_t EXPONENTS = 0x7F807F80u, ONE = 0x00800080u;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -446,17 +446,17 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
                     lo[x][a] = W2::pack(w0 - f.x, w1 - f.y);
                 }
             // ---- answers.  Where some row does not see some key, a value that is infinite or NaN there must not meet its weight of 0
-            bool odd = false;
+            uint32_t tops = 0;      // (a half that is infinite or NaN has an exponent of ones: its top bit in the sum with ONE)
             if (!whole) {
 #pragma unroll
                 for (int c = 0; c < VT; ++c) {
                     uint32_t a[4];
                     ldsm4(to + v_lane + 512 * c, a);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) odd = odd || __vcmpeq2(a[x] & W2::EXPONENTS, W2::EXPONENTS);
+                    for (int x = 0; x < 4; ++x) tops |= (a[x] & W2::EXPONENTS) + W2::ONE;
                 }
             }
-            if (!__any_sync(0xffffffffu, odd)) {
+            if (!__any_sync(0xffffffffu, tops & 0x80008000u)) {
 #pragma unroll
                 for (int c = 0; c < VT; ++c) {
                     uint32_t a[4];

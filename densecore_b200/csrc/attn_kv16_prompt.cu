@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
     using L = Lay<HD>;
     using R = dc_kv16_rec<HD>;
     constexpr bool F16 = std::is_same<TC, __half>::value;
-    constexpr uint32_t EXPONENTS = F16 ? 0x7C007C00u : 0x7F807F80u;
+    // (a half that is infinite or NaN has an exponent of ones: its top bit in (w & EXPONENTS) + ONE)
+    constexpr uint32_t EXPONENTS = F16 ? 0x7C007C00u : 0x7F807F80u, ONE = F16 ? 0x04000400u : 0x00800080u, TOPS = 0x80008000u;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_bad[KP_STAGES];
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
     const Tile tl(tiles, line, p.window, p.keep);
     if (part >= tl.n_parts) return;
     const dc_kv_entry own = tl.e;
-    const int row0 = tl.row0, rows = tl.rows, sets = rows > KP_ROWS ? 2 : 1, first = tl.first, last = tl.last, window = p.window ? p.window : 0x7fffffff, n_pages = tl.pages.n, n_parts = tl.n_parts, kept = tl.pages.kept, low = tl.pages.low;
+    const int row0 = tl.row0, rows = tl.rows, sets = rows > KP_ROWS ? 2 : 1, first = tl.first, last = tl.last, window = p.window ? min(p.window, 0x40000000) : 0x40000000 /* positions are below 2^30 */, n_pages = tl.pages.n, n_parts = tl.n_parts, kept = tl.pages.kept, low = tl.pages.low;
     const int tile0 = (int)((long long)tl.key_tiles * part / n_parts), n_tiles = (int)((long long)tl.key_tiles * (part + 1) / n_parts) - tile0;
     auto page_at = [&](int i) { return tl.pages.at(i); };
     // position of the first key of page i of tile t; far behind the last token where there is none
@@ -227,13 +228,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                 if (!ok) break;
                 tc_fence_after();
                 const bool masked = !whole_here(t);
-                int k0[4];
+                uint32_t seen[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};      // the tile's keys that the row sees
+                if (!whole(t)) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) k0[i] = key_at(t, i);
-                auto sees = [&](int i) {
-                    const int kp = k0[i >> 4] + (i & 15);
-                    return kp <= qp && (kp > qp - window || kp < p.keep);
-                };
+                    for (int i = 0; i < 4; ++i) {
+                        const int k0 = key_at(t, i);
+                        auto below = [](int n) { return (1u << min(max(n, 0), 16)) - 1u; };      // the page's first n keys
+                        const uint32_t is = below(qp + 1 - k0) & (~below(qp + 1 - window - k0) | below(p.keep - k0)) & 0xFFFFu;
+                        seen[i >> 1] = i & 1 ? (seen[i >> 1] & 0xFFFFu) | is << 16 : (seen[i >> 1] & 0xFFFF0000u) | is;
+                    }
+                }
                 int x[4][16] = {};
                 auto s = [&](int i) -> float { return __int_as_float(x[i >> 4][i & 15]); };
                 __syncwarp();
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 64; ++i)
-                        if (!sees(i)) x[i >> 4][i & 15] = __float_as_int(-INFINITY);
+                        if (!(seen[i >> 5] >> (i & 31) & 1u)) x[i >> 4][i & 15] = __float_as_int(-INFINITY);
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -254,11 +258,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                     ok = wait(bar(KP_FULL, stage), (t / KP_STAGES) & 1);
                     if (!ok) break;
                     if (s_bad[stage]) {
-                        uint32_t seen[2] = {0, 0};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll 1
-                            for (int j = 0; j < 16; ++j) seen[i >> 1] |= (uint32_t)sees(16 * i + j) << (16 * (i & 1) + j);
                         const uint2* bad = reinterpret_cast<const uint2*>(base + L::BAD) + stage * HD;
 #pragma unroll 1
                         for (int d = 0; d < HD; ++d)
@@ -419,13 +418,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
             if (!wait(bar(KP_PRE, stage), uses >> stage & 1)) break;
             uses ^= 1u << stage;
             const uint32_t values = sm + L::KV + stage * (2 * L::TILE) + L::TILE;
-            bool odd = false;
+            uint32_t tops = 0;
 #pragma unroll 8
             for (int i = lane; i < (int)L::TILE / 16; i += 32) {
                 const uint4 v = lds128(values + 16 * i);
-                odd = odd || __vcmpeq2(v.x & EXPONENTS, EXPONENTS) || __vcmpeq2(v.y & EXPONENTS, EXPONENTS) || __vcmpeq2(v.z & EXPONENTS, EXPONENTS) || __vcmpeq2(v.w & EXPONENTS, EXPONENTS);
+                tops |= ((v.x & EXPONENTS) + ONE) | ((v.y & EXPONENTS) + ONE) | ((v.z & EXPONENTS) + ONE) | ((v.w & EXPONENTS) + ONE);
             }
-            odd = __any_sync(0xffffffffu, odd);
+            const bool odd = __any_sync(0xffffffffu, tops & TOPS);
             if (odd) {      // which keys, by dimension; and 0 in their place
                 uint32_t* bad = reinterpret_cast<uint32_t*>(base + L::BAD) + stage * HD * 2;
                 for (int i = lane; i < 2 * HD; i += 32) bad[i] = 0;

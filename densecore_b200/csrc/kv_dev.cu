@@ -95,39 +95,46 @@ struct Totals {
     int32_t tokens, units, freed, given, free;      // free: of the pool, before the step
 };
 
-// Unit i: a page that new tokens lie on, or (behind those) a freed one that nobody takes.
-__device__ __forceinline__ void place_unit(const StepParams& p, const Slots& z, const Totals& all, int i) {
+// Units i .. i + 31, one a lane (a whole warp): pages that new tokens lie on, behind those freed ones that nobody takes.
+__device__ __forceinline__ void place_units(const StepParams& p, const Slots& z, const Totals& all, int i) {
+    const int lane = threadIdx.x & 31, n_units = all.units + max(0, all.freed - all.given);
     auto freed_page = [&](int j) {
         const int s = find(z.free0, p.slots, j);
         return p.tables[(size_t)s * p.pages_per_seq + z.left[s] + (j - z.free0[s])];
     };
-    if (i >= all.units) {
+    int s = 0, slot = 0, first = 0, t = 0, n = 0;
+    i += lane;
+    if (i < all.units) {
+        s = find(z.unit0, p.slots, i);
+        const int keep = z.keep[s], place = keep / DC_KV_BLOCK + i - z.unit0[s], tok0 = z.tok0[s], left = z.left[s];
+        const int n_tok = (s + 1 < p.slots ? z.tok0[s + 1] : all.tokens) - tok0;
+        int32_t* cell = p.tables + (size_t)s * p.pages_per_seq + place;
+        int page;
+        if (place < left) {
+            page = *cell;
+        } else {      // the j-th granted one
+            const int j = z.give0[s] + place - left;
+            page = j < all.freed ? freed_page(j) : p.stack[all.free - 1 - (j - all.freed)];
+            *cell = page;
+        }
+        first = max(keep, place * DC_KV_BLOCK), n = min(keep + n_tok, (place + 1) * DC_KV_BLOCK) - first, t = tok0 + first - keep;
+        slot = page * DC_KV_BLOCK + first % DC_KV_BLOCK;
+    } else if (i < n_units) {
         const int j = all.given + i - all.units;
         p.stack[all.free + all.freed - 1 - j] = freed_page(j);
-        return;
     }
-    const int s = find(z.unit0, p.slots, i), keep = z.keep[s], place = keep / DC_KV_BLOCK + i - z.unit0[s], tok0 = z.tok0[s];
-    const int n_tok = (s + 1 < p.slots ? z.tok0[s + 1] : all.tokens) - tok0, left = z.left[s];
-    int32_t* cell = p.tables + (size_t)s * p.pages_per_seq + place;
-    int page;
-    if (place < left) {
-        page = *cell;
-    } else {      // the j-th granted one
-        const int j = z.give0[s] + place - left;
-        page = j < all.freed ? freed_page(j) : p.stack[all.free - 1 - (j - all.freed)];
-        *cell = page;
+    // ---- the units' tokens, two units at a time, a lane each
+    const int x = lane & 15;
+    for (uint32_t todo = __ballot_sync(0xffffffffu, n > 0); todo;) {
+        const int a = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int b = todo ? __ffs(todo) - 1 : a, from = lane < 16 ? a : b;
+        const bool mine = lane < 16 || todo != 0;
+        todo &= todo - 1;
+        const int us = __shfl_sync(0xffffffffu, s, from), uslot = __shfl_sync(0xffffffffu, slot, from), ufirst = __shfl_sync(0xffffffffu, first, from), ut = __shfl_sync(0xffffffffu, t, from),
+                  un = __shfl_sync(0xffffffffu, n, from);
+        if (mine && x < un) p.slot_map[ut + x] = uslot + x, p.positions[ut + x] = ufirst + x, p.seqs[ut + x] = us;
     }
-    const int first = max(keep, place * DC_KV_BLOCK), last = min(keep + n_tok, (place + 1) * DC_KV_BLOCK), t = tok0 + first - keep, n = last - first;
-    int32_t *to = p.slot_map + t, *pos = p.positions + t, *seq = p.seqs + t;
-    const int slot = page * DC_KV_BLOCK + first % DC_KV_BLOCK;
-    int x = 0;
-    for (; x < n && ((t + x) & 3); ++x) to[x] = slot + x, pos[x] = first + x, seq[x] = s;
-    for (; x + 4 <= n; x += 4) {
-        *reinterpret_cast<int4*>(to + x) = make_int4(slot + x, slot + x + 1, slot + x + 2, slot + x + 3);
-        *reinterpret_cast<int4*>(pos + x) = make_int4(first + x, first + x + 1, first + x + 2, first + x + 3);
-        *reinterpret_cast<int4*>(seq + x) = make_int4(s, s, s, s);
-    }
-    for (; x < n; ++x) to[x] = slot + x, pos[x] = first + x, seq[x] = s;
 }
 
 __global__ void __launch_bounds__(KS_T) k_kv_step(const StepParams p) {
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(KS_T) k_kv_step(const StepParams p) {
         }
     }
     if (p.apart) return;
-    for (int i = rank * KS_T + threadIdx.x; i < sum.units + max(0, n_freed - sum.given); i += n_cta * KS_T) place_unit(p, z, sum, i);
+    for (int i = rank * KS_T + (threadIdx.x & ~31); i < sum.units + max(0, n_freed - sum.given); i += n_cta * KS_T) place_units(p, z, sum, i);
 }
 
 // The units of a large step.
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(KP_T) k_kv_places(const StepParams p) {
     for (int i = threadIdx.x; i < KS_ARRAYS * p.slots; i += KP_T) sm[i] = p.scratch[i];
     __syncthreads();
     const Slots z(sm, p.slots);
-    for (int i = blockIdx.x * KP_T + threadIdx.x; i < sum.units + max(0, sum.freed - sum.given); i += gridDim.x * KP_T) place_unit(p, z, sum, i);
+    for (int i = blockIdx.x * KP_T + (threadIdx.x & ~31); i < sum.units + max(0, sum.freed - sum.given); i += gridDim.x * KP_T) place_units(p, z, sum, i);
 }
 
 __global__ void k_kv_stack(int32_t* stack, int n) {      // so that pages are handed out from 0 on
