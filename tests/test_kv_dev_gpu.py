@@ -92,7 +92,6 @@ def test_long_sequences_shared_out(ctx, dtype):
     """Lengths of which many CTAs have a part, beside short ones; then drafted tokens at all offsets of a page."""
     m = Mirror(ctx, dtype, 8, 2, 128, 5, 1400, 700, 16000, seed=5)
     m.step([9000, 1, 3000, 40, 0])
-    m.cache.write_dev  # (written below, with what attends)
     T = len(m.steps.seqs)
     k, v = m.rows(T, 2), m.rows(T, 2)
     kd, vd = k.to(GPU), v.to(GPU)
@@ -301,3 +300,74 @@ def test_calls_that_are_refused(ctx):
     with pytest.raises(dc.DcError, match="kept on the GPU"):
         KVCache.seq_alloc(kv)
     kv.close()
+
+
+def test_pages_far_into_a_large_cache(ctx):
+    """Offsets beyond 2^32 bytes within a layer, and a second layer behind it."""
+    m = Mirror(ctx, "bf16", 16, 8, 128, 3, 84000, 82000, 1310000, layers=2, seed=37)      # 64 KB a page and layer
+    m.step([0, 1300000, 0])
+    m.step([70, 0, 9], [0, 0, 0])
+    assert min(m.steps.slots) // 16 * 65536 > 2**32
+    m.attend(1)
+    m.attend(0)
+    m.step([1, 0, 5])
+    m.attend(0)
+    m.attend(1, window=30, keep=3)
+    m.cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_a_captured_prompt_step(ctx, dtype):
+    """Prompts, drafted and single tokens of one graph, replayed on other mixtures of them: portions that are split over their keys, whole tiles, windows."""
+    m = Mirror(ctx, dtype, 8, 2, 64, 3, 900, 300, 900, seed=41)
+    room = 900
+    count, drop = ints([0] * 3), ints([0] * 3)
+    t = m.rows(1, 1).dtype
+    q, k, v = (torch.zeros(room, h, 64, dtype=t, device=GPU) for h in (8, 2, 2))
+    out = torch.zeros(room, 8, 64, dtype=t, device=GPU)
+
+    def call():
+        m.cache.step_dev(count.data_ptr(), drop=drop.data_ptr(), max_count=600)
+        m.cache.attend_dev(0, q.data_ptr(), k.data_ptr(), v.data_ptr(), 0.11, out.data_ptr(), window=700, keep_first=20)
+    torch.cuda.synchronize()
+    call()
+    ctx.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), stream_of(ctx)
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+    for c, d in (([600, 1, 17], [0, 0, 0]), ([1, 300, 5], [0, 0, 3]), ([600, 200, 64], [1, 1, 1]), ([0, 0, 0], [0, 0, 0]), ([1, 1, 1], [0, 0, 0]), ([33, 600, 0], [0, 0, ALL]), ([500, 1, 129], [40, 5, 0])):
+        count.copy_(ints(c)), drop.copy_(ints(d))
+        m.steps.step(c, d, 600)
+        T = len(m.steps.seqs)
+        new = [m.rows(T, h) for h in (8, 2, 2)]
+        for to, x in zip((q, k, v), new):
+            to[:T].copy_(x)
+        out.fill_(-7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.synchronize()
+        for rows in (m.k[0], m.v[0]):
+            for s in range(3):
+                rows[s] = rows[s][:m.steps.lens[s] - m.steps.counts[s]]
+        m.append(0, new[1], new[2])
+        m.steps.check(m.cache)
+        assert (out[T:] == -7).all()
+        m.compare(out[:T].cpu(), new[0], 0, 700, 20, 0.11)
+
+
+def test_prompts_behind_long_sequences(ctx):
+    """Few tiles of rows, so that their keys are split over CTAs and added up, beside single tokens; all the keys or a window of them."""
+    for dtype, hd in (("bf16", 128), ("f16", 64)):
+        m = Mirror(ctx, dtype, 4, 2, hd, 3, 900, 400, 12000, seed=43)
+        m.step([5000, 700, 20])
+        T = 5720
+        k, v = m.rows(T, 2), m.rows(T, 2)
+        kd, vd = k.to(GPU), v.to(GPU)
+        torch.cuda.synchronize()
+        m.cache.write_dev(0, kd.data_ptr(), vd.data_ptr())
+        ctx.synchronize()
+        m.append(0, k, v)
+        for count, window, keep in (([200, 1, 1], 0, 0), ([40, 3, 300], 0, 0), ([130, 1, 33], 2500, 40), ([65, 200, 0], 0, 0)):
+            m.step(count)
+            m.attend(window=window, keep=keep)
