@@ -323,8 +323,8 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
                     for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[s][i]));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                // times 2^(10 - e), 2^e <= largest < 2^(e + 1)
-                const int e = max(-100, min(100, (int)(__float_as_uint(most) >> 23) - 127));
+                // times 2^(10 - e), 2^e <= largest < 2^(e + 1); both factors are normal numbers
+                const int e = max(-116, min(127, (int)(__float_as_uint(most) >> 23) - 127));
                 const float up = __uint_as_float((uint32_t)(137 - e) << 23);
                 F *= __uint_as_float((uint32_t)(117 + e) << 23);
 #pragma unroll

@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
             fence_async_smem();
             mbar_arrive(bar(KP_QUERY));
             __syncwarp();
-            const float sl2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-35f);      // (above 0: minus infinity stays so)
+            const float sl2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-45f);      // (above 0, if only the least there is: minus infinity stays so)
             constexpr float LARGEST = F16 ? 7.0f : 0.0f;                                 // of a weight, in powers of two
             float m_run = -3e38f, l_run[2] = {0.0f, 0.0f};
             bool ok = true;

@@ -6,7 +6,8 @@
 // k_verify_stats (logits alone): the rows' maxima and sums of weights, a row cut into parts where there are few; one pass.  k_verify_next: every CTA of a request decides
 // n from those for itself, then sums r over its part of row n in tiles of 2048 tokens; the last CTA of the request finds the tile that the draw falls into, and
 // in it the token.  So a row that is accepted is read once, and the one drawn from twice (the second time largely from L2).
-// Weights are 2^((x - max) log2(e) / T) in f32 (2^-22), sums in 64 bits, in an order that does not depend on timing.
+// Weights are 2^((x - max) log2(e) / T) in f32: one of 2^-m is off by 2^-22 and, as scale and exponent are rounded once each, by m 2^-23.  Sums are of 64 bits (eight weights at a time in
+// 32), in an order that does not depend on timing.
 #include <math.h>
 
 #include <algorithm>

@@ -371,3 +371,23 @@ def test_prompts_behind_long_sequences(ctx):
         for count, window, keep in (([200, 1, 1], 0, 0), ([40, 3, 300], 0, 0), ([130, 1, 33], 2500, 40), ([65, 200, 0], 0, 0)):
             m.step(count)
             m.attend(window=window, keep=keep)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_queries_near_the_ends_of_their_range(ctx, dtype):
+    """Rows from 2^-115 to 2^123 under scales that undo it: results as those of rows around 1."""
+    m = Mirror(ctx, dtype, 4, 2, 64, 2, 40, 20, 320, seed=47)
+    for power in (-115, 0, 100, 115, 121):
+        m.step([1, 70] if power in (0, 115) else [2, 3])
+        T = len(m.steps.seqs)
+        m.attend(q=m.rows(T, 4) * 2.0**power, scale=64**-0.5 * 2.0**-power)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_more_query_heads_than_a_tile_has_rows(ctx, dtype):
+    """A single token has more rows of a key head than the rows kernel takes, or as many, or one fewer."""
+    for heads, kv, hd in ((96, 1, 64), (260, 1, 64), (130, 2, 128), (64, 1, 128), (66, 2, 64), (32, 1, 64)):
+        m = Mirror(ctx, dtype, heads, kv, hd, 3, 60, 20, 40, seed=53)
+        for count, window, keep in (([20, 1, 0], 0, 0), ([1, 1, 1], 0, 0), ([2, 0, 1], 9, 2), ([1, 1, 1], 3, 0)):
+            m.step(count)
+            m.attend(window=window, keep=keep)
