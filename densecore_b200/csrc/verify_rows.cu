@@ -44,7 +44,7 @@ struct VerifyParams {
     const float *q, *temperature, *u;
     int32_t *out, *accepted, *rejected;
     Stat* stats;                               // [request][row][stat_parts]
-    int stat_parts;
+    int stat_parts, stat_tiles;
     double* sums;                              // [request][tile], where a request has several CTAs
     int32_t* tickets;
 };
@@ -146,13 +146,14 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b, const Scale& 
     s.sum = a.most == s.most ? a.sum + b.sum * (double)f : a.sum * (double)f + b.sum;
     return s;
 }
-__device__ __forceinline__ Stat warp_join(Stat s, const Scale& c) {
+// Those of a warp's lanes, to all of them.
+__device__ __forceinline__ Stat warp_join(const Stat& a, const Scale& c) {
+    Stat s;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(s.most) : "f"(a.most));
+    s.first = c.greedy ? __reduce_min_sync(0xffffffffu, a.most == s.most ? a.first : 0x7fffffff) : 0x7fffffff;
+    s.sum = a.most == s.most ? a.sum : s.most == INFINITY ? 0.0 : a.sum * (double)c(a.most, s.most);
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) {
-        Stat o;
-        o.sum = __shfl_xor_sync(0xffffffffu, s.sum, k), o.most = __shfl_xor_sync(0xffffffffu, s.most, k), o.first = __shfl_xor_sync(0xffffffffu, s.first, k);
-        s = join(s, o, c);      // (the same for both lanes: sums of two are commutative)
-    }
+    for (int k = 16; k > 0; k >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, k);      // (the same in all lanes: sums of two are commutative)
     return s;
 }
 
@@ -163,12 +164,12 @@ __global__ void __launch_bounds__(VR_T, 4) k_verify_stats(const VerifyParams p) 
     __shared__ Stat warps[VR_T / 32];
     pdl_wait();
     pdl_launch_dependents();
-    const int unit = blockIdx.x / p.stat_parts, part = blockIdx.x % p.stat_parts, r = unit / (p.D + 1), i = unit % (p.D + 1);
+    const int r = blockIdx.x, i = blockIdx.y, part = blockIdx.z;
+    const float T = p.temperature ? p.temperature[r] : 1.0f;
     int n, row0;
     if (!request(p, r, n, row0) || i > n) return;
     const TX* row = reinterpret_cast<const TX*>(p.target) + (size_t)(row0 + i) * p.ld;
-    const Scale c(p.temperature ? p.temperature[r] : 1.0f);
-    const int tiles = (p.V + VR_TILE - 1) / VR_TILE, first = part * ((tiles + p.stat_parts - 1) / p.stat_parts), last = min(tiles, first + (tiles + p.stat_parts - 1) / p.stat_parts);
+    const int first = part * p.stat_tiles, last = min((p.V + VR_TILE - 1) / VR_TILE, first + p.stat_tiles);
     float most = -INFINITY;
     int where = 0x7fffffff;      // of a request that goes by the largest alone
     double sum = 0.0;
@@ -178,6 +179,7 @@ __global__ void __launch_bounds__(VR_T, 4) k_verify_stats(const VerifyParams p) 
         for (int b = 0; b < B; ++b) next[b].load(row, t0 + b < last ? (t0 + b) * VR_TILE + VR_PER * (int)threadIdx.x : p.V, p.V, -INFINITY);
     };
     if (first < last) fetch(first);
+    const Scale c(T);
     for (int t0 = first; t0 < last; t0 += B) {
         float x[B][8], top = -INFINITY;
         if constexpr (sizeof(TX) == 2) {      // (pairs as they lie)
@@ -240,9 +242,11 @@ __global__ void __launch_bounds__(VR_T, 4) k_verify_stats(const VerifyParams p) 
     s = warp_join(s, c);
     if ((threadIdx.x & 31) == 0) warps[threadIdx.x / 32] = s;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < VR_T / 32; ++w) s = join(s, warps[w], c);
-        p.stats[(size_t)unit * p.stat_parts + part] = s;
+    if (threadIdx.x < 32) {
+        s.sum = 0.0, s.most = -INFINITY, s.first = 0x7fffffff;
+        if (threadIdx.x < VR_T / 32) s = warps[threadIdx.x];
+        s = warp_join(s, c);
+        if (threadIdx.x == 0) p.stats[((size_t)r * (p.D + 1) + i) * p.stat_parts + part] = s;
     }
 }
 
@@ -525,7 +529,7 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 template <typename TX, bool PROBS>
 int launch(dc_ctx* ctx, const VerifyParams& p) {
     if constexpr (!PROBS)
-        DC_TRY(dc_launch(ctx, "k_verify_stats", k_verify_stats<TX>, dim3(p.R * (p.D + 1) * p.stat_parts), dim3(VR_T), 0, p));
+        DC_TRY(dc_launch(ctx, "k_verify_stats", k_verify_stats<TX>, dim3(p.R, p.D + 1, p.stat_parts), dim3(VR_T), 0, p));
     return dc_launch(ctx, "k_verify_next", k_verify_next<TX, PROBS>, dim3(p.R * p.parts), dim3(VR_T), 0, p);
 }
 
@@ -551,7 +555,8 @@ int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64
     // rows are cut into parts where there are fewer than fill the GPU
     const int tiles = (vocab + VR_TILE - 1) / VR_TILE, n_rows = n_requests * (max_drafts + 1), stat_ctas = VR_STATS_CTAS * ctx->num_sms, next_ctas = VR_NEXT_CTAS * ctx->num_sms;
     int stat_parts = std::min(tiles, (stat_ctas + n_rows - 1) / n_rows), parts = std::min(tiles, (next_ctas + n_requests - 1) / n_requests);
-    const int part_tiles = (tiles + parts - 1) / parts;
+    const int part_tiles = (tiles + parts - 1) / parts, stat_tiles = (tiles + stat_parts - 1) / stat_parts;
+    stat_parts = (tiles + stat_tiles - 1) / stat_tiles;
     parts = (tiles + part_tiles - 1) / part_tiles;
     // a workspace of one size, which graphs that hold calls may go on using
     const size_t stats = align256((size_t)(VR_ROWS + stat_ctas) * sizeof(Stat)), sums = align256((size_t)next_ctas * VR_TILES * sizeof(double)), tickets = align256((size_t)next_ctas * 4);
@@ -569,7 +574,7 @@ int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64
         ctx->verify_ws = (uint8_t*)ws;
     }
     const VerifyParams p = {target_dev, (size_t)ld, rows, vocab, n_requests, max_drafts, parts, part_tiles, starts_dev, n_drafts_dev, draft_tokens_dev, draft_probs_dev, temperature_dev,
-                            uniforms_dev, tokens_dev, accepted_dev, rejected_dev, (Stat*)ctx->verify_ws, stat_parts, (double*)(ctx->verify_ws + stats), (int32_t*)(ctx->verify_ws + stats + sums)};
+                            uniforms_dev, tokens_dev, accepted_dev, rejected_dev, (Stat*)ctx->verify_ws, stat_parts, stat_tiles, (double*)(ctx->verify_ws + stats), (int32_t*)(ctx->verify_ws + stats + sums)};
     return type == VR_PROBS ? launch<float, true>(ctx, p) : type == DC_TYPE_F32 ? launch<float, false>(ctx, p) : launch<__nv_bfloat16, false>(ctx, p);
 }
 
