@@ -27,7 +27,9 @@ using namespace dc;
 namespace {
 
 constexpr int VR_T = 256, VR_PER = 8, VR_TILE = VR_T * VR_PER, VR_DRAFTS = 64, VR_VOCAB = 389120, VR_TILES = VR_VOCAB / VR_TILE, VR_ROWS = 65536;
-constexpr int VR_STATS_CTAS = 16, VR_NEXT_CTAS = 2;      // an SM, where rows are cut into parts
+// CTAs an SM that rows are cut for.  128 requests of up to 4 drafts, bf16, 151936 tokens: statistics for 8 / 16 / 24 / 32 CTAs 60.5 / 58.7 / 64.5 / 65.3 us, drawing (three fit an SM) for 2 / 3 / 4 58.7 /
+// 56.5 / 60.2; 64 requests of 3 drafts, probabilities, drawing 19.5 / 19.9 / 20.8.
+constexpr int VR_STATS_CTAS = 16, VR_NEXT_CTAS = 3;
 constexpr int VR_PROBS = -1;
 
 struct alignas(16) Stat {      // of a part of a row
@@ -157,7 +159,8 @@ __device__ __forceinline__ Stat warp_join(const Stat& a, const Scale& c) {
     return s;
 }
 
-// One CTA per (row, part).
+// One CTA per (row, part).  Bound: issue slots (64 %, exponentials 53 % of their pipe's) ahead of HBM: 141 MB of bf16 rows in 40 us, 3.5 TB/s (a call of 63 us; without
+// divisions and with maxima joined at once 59).  Four tiles on their way at 64 registers (four CTAs an SM); two tiles and five or six CTAs 67 to 68 for 66.
 template <typename TX>
 __global__ void __launch_bounds__(VR_T, 4) k_verify_stats(const VerifyParams p) {
     constexpr int B = sizeof(TX) == 2 ? 4 : 2;      // tiles on their way at once
@@ -274,7 +277,8 @@ __device__ __forceinline__ double scan(double v, double* warps, double& all) {
 }
 
 // One CTA per (request, part of the row drawn from).  Bound: HBM for many requests (the row and its draft's probabilities, once; the draw's own tile again), latency for few: the rows'
-// statistics, the decisions, the part, the ticket and the draw's tile one after the other.
+// statistics, the decisions, the part, the ticket and the draw's tile one after the other.  78 MB of probabilities: 19.5 us (4.0 TB/s); held to 64 registers, so that four CTAs fit an SM,
+// it spills: 23 to 29.  One request's whole call, with the statistics: 11.6 us.
 template <typename TX, bool PROBS>
 __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
     __shared__ Stat rows[VR_DRAFTS + 1];
