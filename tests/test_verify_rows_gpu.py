@@ -122,6 +122,16 @@ def test_requests_against_64_bits(ctx, form, R, D, V):
     run(ctx, x, starts, n, tokens, None, u, T, probs=form == "probs", dtype="bf16" if form == "bf16" else "f32")
 
 
+@pytest.mark.parametrize("form", ["f32", "bf16", "probs"])
+def test_requests_that_share_rows(ctx, form):
+    """Several requests' rows may be the same ones, wholly or in part, and in any order."""
+    rng = np.random.default_rng(21)
+    D, V = 3, 2500
+    x, _, _, tokens, q, u, T = make(rng, 8, D, V, probs=form == "probs")
+    x, starts, n = x[:5], np.array([0, 0, 1, 1, 0, 1, 4, 0]), np.array([3, 3, 3, 2, 0, 3, 0, 1])
+    run(ctx, x, starts, n, tokens, q, u, T, probs=form == "probs", dtype="bf16" if form == "bf16" else "f32")
+
+
 @pytest.mark.parametrize("dtype,ld,shift", [("f32", 0, 1), ("f32", 3001, 0), ("f32", 3004, 4), ("bf16", 0, 3), ("bf16", 3007, 0), ("bf16", 3008, 8), ("probs", 3003, 2)])
 def test_rows_of_any_alignment(ctx, dtype, ld, shift):
     rng = np.random.default_rng(5)
