@@ -98,7 +98,7 @@ struct Scale {
     }
     __device__ __forceinline__ float operator()(float x, float most) const { return ex2(fmaxf(x - most, -1e35f) * c); }      // x at or below `most`, which is finite
 };
-// The same weights with one multiply-add each: 2^(c x - hi) where c most = hi + lo exactly, so that each is 2^lo fold.  For products that leave lo below 1/32; NaN stays NaN.
+// The same weights with one multiply-add each: 2^(c x - hi) where c most = hi + lo exactly, so that each is 2^lo fold, and 2^-lo undoes it.  For products that leave lo below 1/32; NaN stays NaN.
 struct Quick {
     float hi, lo;
     bool is;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(VR_T, 4) k_verify_stats(const VerifyParams p) 
                     s[k / 2 & 1] = add2(s[k / 2 & 1], pair(ex2(y.x), ex2(y.y)));
                 }
             const float2 z = unpair(add2(s[0], s[1]));
-            all = (z.x + z.y) * ex2(q.lo);
+            all = (z.x + z.y) * ex2(-q.lo);
         }
         if (!(q.is && all < INFINITY)) {      // an infinite largest, a product too large, or a NaN among them
             all = 0.0f;
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
         }
     }
     const Quick quick(c, st.most);
-    const float inv = (float)(1.0 / st.sum), quick_inv = inv * ex2(quick.lo);
+    const float inv = (float)(1.0 / st.sum), quick_inv = inv * ex2(-quick.lo);
     struct Loaded {
         Eight<TX> x;
         Eight<float> q;
