@@ -6,8 +6,15 @@
 // k_verify_stats (logits alone): the rows' maxima and sums of weights, a row cut into parts where there are few; one pass.  k_verify_next: every CTA of a request decides
 // n from those for itself, then sums r over its part of row n in tiles of 2048 tokens; the last CTA of the request finds the tile that the draw falls into, and
 // in it the token.  So a row that is accepted is read once, and the one drawn from twice (the second time largely from L2).
-// Weights are 2^((x - max) log2(e) / T) in f32: one of 2^-m is off by 2^-22 and, as scale and exponent are rounded once each, by m 2^-23.  Sums are of 64 bits (eight weights at a time in
-// 32), in an order that does not depend on timing.
+//
+// A token of a large vocabulary has a millionth of the whole or less, so what decides is of 64 bits.  The statistics' weights are not: 2^((x - max) log2(e) / T) in f32, of which one of 2^-m is off by
+// 2^-22 and, as scale and exponent are rounded once each, by m 2^-23 (32 bf16 or 16 f32 ones at a time are added in 32 bits, then in 64).  Weighted by themselves the m of up to 2^19 tokens are 15 at the
+// most, so that a sum is off by less than 2^-18.  Sums decide on drafts that are further than 2^-16 from their border alone; for another one (one in some 10^4) every CTA of the request
+// sums its row again, in 64 bits.
+// The row drawn from has 64-bit weights w, for which its sum S is not known before all of them are: with s, the statistics' S, the one pass sums w, the r' = w - s q that are above 0, and the q
+// of those, so that S and then sum max(0, w - S q) = sum r' - (S - s) sum q are known behind it.  That holds where r and r' are of one sign: a warp's tokens that have an r' within 2^-16 s q
+// of 0 (some eight of 600 groups), or all where S is further than 2^-17 from s, are summed again with S itself.  Weights of f32 and sums of eight in 32 bits took 56.5 us for the 128 requests below, and drew
+// one token in 1500 beside the one that 64 bits give; these take 81.
 #include <math.h>
 
 #include <algorithm>
@@ -27,8 +34,8 @@ using namespace dc;
 namespace {
 
 constexpr int VR_T = 256, VR_PER = 8, VR_TILE = VR_T * VR_PER, VR_DRAFTS = 64, VR_VOCAB = 389120, VR_TILES = VR_VOCAB / VR_TILE, VR_ROWS = 65536;
-// CTAs an SM that rows are cut for.  128 requests of up to 4 drafts, bf16, 151936 tokens: statistics for 8 / 16 / 24 / 32 CTAs 60.5 / 58.7 / 64.5 / 65.3 us, drawing (three fit an SM) for 2 / 3 / 4 58.7 /
-// 56.5 / 60.2; 64 requests of 3 drafts, probabilities, drawing 19.5 / 19.9 / 20.8.
+// CTAs an SM that rows are cut for.  128 requests of up to 4 drafts, bf16, 151936 tokens: statistics for 8 / 16 / 24 / 32 CTAs 60.5 / 58.7 / 64.5 / 65.3 us (with f32 weights in drawing); drawing for three CTAs, held
+// to 80 registers, so that three fit an SM, 81, for four at 64 registers 88.
 constexpr int VR_STATS_CTAS = 16, VR_NEXT_CTAS = 3;
 constexpr int VR_PROBS = -1;
 
@@ -36,6 +43,12 @@ struct alignas(16) Stat {      // of a part of a row
     double sum;      // of weights against the part's maximum
     float most;
     int first;       // index of the first largest
+};
+
+struct Tile {        // of a row drawn from
+    double w, r;     // sums of weights, of what is left above the draft
+    float q;         // of the draft's probabilities where something is
+    int again;       // warps whose share is not in r and q yet, since some of what is left may be of the other sign: a bit each
 };
 
 struct VerifyParams {
@@ -47,7 +60,7 @@ struct VerifyParams {
     int32_t *out, *accepted, *rejected;
     Stat* stats;                               // [request][row][stat_parts]
     int stat_parts, stat_tiles;
-    double* sums;                              // [request][tile], where a request has several CTAs
+    Tile* sums;                                // [request][tile], where a request has several CTAs
     int32_t* tickets;
 };
 
@@ -87,23 +100,45 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// log2(e) / T, rounded: what all weights of a request go by.  Differences are held to 1e35, at which a weight is 0 for every scale from 1e-30 on: so NaN and -inf have none, and no
+// log2(e) / T, rounded: what the statistics' weights of a request go by.  Differences are held to 1e35, at which a weight is 0 for every scale from 1e-30 on: so NaN and -inf have none, and no
 // product overflows.
 struct Scale {
     float c;
-    bool greedy;
+    bool greedy, bent;      // bent: held to another than it is
+    double exact;
     __device__ __forceinline__ explicit Scale(float T) {
-        greedy = !(T > 0.0f);
-        c = greedy ? 1.0f : (float)fmin(fmax(1.4426950408889634 / (double)T, 1e-30), 1e30);
+        greedy = !(T > 0.0f), bent = !(T > 2e-30f && T < 1e30f);
+        exact = 1.4426950408889634074 / (double)T;
+        c = greedy ? 1.0f : (float)fmin(fmax(exact, 1e-30), 1e30);
     }
     __device__ __forceinline__ float operator()(float x, float most) const { return ex2(fmaxf(x - most, -1e35f) * c); }      // x at or below `most`, which is finite
 };
-// The same weights with one multiply-add each: 2^(c x - hi) where c most = hi + lo exactly, so that each is 2^lo fold, and 2^-lo undoes it.  For products that leave lo below 1/32; NaN stays NaN.
+// The statistics' weights with one multiply-add each: 2^(c x - hi) where c most = hi + lo exactly, so that each is 2^lo fold and a sum of them to be taken 2^-lo fold.  For products that leave lo below 1/32;
+// NaN stays NaN.
 struct Quick {
     float hi, lo;
     bool is;
     __device__ __forceinline__ Quick(const Scale& c, float most) : hi(c.c * most), lo(fmaf(c.c, most, -hi)), is(fabsf(hi) < 1048576.0f) {}
-    __device__ __forceinline__ float operator()(const Scale& c, float x) const { return ex2(fmaf(c.c, x, -hi)); }
+};
+// Weights in 64 bits: t = (x - most) log2(e) / T is off by some 2^-52 of itself, so that a weight of 2^-m is by m 2^-52.  2^t as in P. T. P. Tang's table-driven method (1989): t = n / 32 + f, |f| <= 1/64,
+// 2^(n / 32) from a table of 32, which lie in a warp's lanes, 2^f by its Taylor polynomial of degree 5 (what is left out is below 2^-48).  NaN and -inf have no weight, nor has what is below
+// 2^-1021; beside an infinite largest only infinite ones have.
+struct Exact {
+    double c, most, mine;      // mine: 2^(lane / 32)
+    bool inf;
+    __device__ __forceinline__ Exact(double c_, float m) : c(c_), most(m), mine(exp2((threadIdx.x & 31) / 32.0)), inf(m == INFINITY) {}
+    // (by whole warps; beside a finite largest)
+    __device__ __forceinline__ double operator()(float x) const {
+        constexpr double MAGIC = 0x1.8p47, L = 0.69314718055994530942;
+        const double t = ((double)x - most) * c, z = t + MAGIC, f = t - (z - MAGIC);
+        const int n = __double2loint(z);
+        double y = fma(f, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
+        y = fma(f, y, L * L * L / 6.0);
+        y = fma(f, y, L * L / 2.0);
+        y = fma(f, y, L);
+        y = fma(f, y, 1.0) * __shfl_sync(0xffffffffu, mine, n & 31);
+        return t > -1021.0 ? __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y)) : 0.0;
+    }
 };
 __device__ __forceinline__ float weight_inf(float x) { return x == INFINITY ? 1.0f : 0.0f; }      // beside an infinite largest
 
@@ -276,14 +311,30 @@ __device__ __forceinline__ double scan(double v, double* warps, double& all) {
     return before + (lane ? ex : 0.0);
 }
 
-// One CTA per (request, part of the row drawn from).  Bound: HBM for many requests (the row and its draft's probabilities, once; the draw's own tile again), latency for few: the rows'
-// statistics, the decisions, the part, the ticket and the draw's tile one after the other.  78 MB of probabilities: 19.5 us (4.0 TB/s); held to 64 registers, so that four CTAs fit an SM,
-// it spills: 23 to 29.  One request's whole call, with the statistics: 11.6 us.
+// A double of every warp's lane, summed in the order of the warps; to all threads.
+__device__ __forceinline__ double cta_sum(double v, double* warps) {
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) v += __shfl_xor_sync(0xffffffffu, v, k);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < VR_T / 32; ++w) all += warps[w];
+    return all;
+}
+
+// One CTA per (request, part of the row drawn from).  Bound: issue slots for many requests' logits (some 40 instructions a token, 14 of them of 64 bits, at 60 % of the slots), HBM for probabilities; latency
+// for few: the rows' statistics, the decisions, the part, the ticket and the draw's tile one after the other.  One request's whole call, with the statistics: 15.5 us; 78 MB of
+// probabilities: 20.5.  Two tiles on their way: 84 us for the 128 requests; sums of w and r reduced one after the other: 84.
 template <typename TX, bool PROBS>
-__global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
+__global__ void __launch_bounds__(VR_T, 3) k_verify_next(const VerifyParams p) {
+    constexpr int WARPS = VR_T / 32;
     __shared__ Stat rows[VR_DRAFTS + 1];
     __shared__ int s_good[VR_DRAFTS], s_n, s_tile, s_last, s_token, s_at_most;
-    __shared__ double s_sums[VR_TILES], s_warps[VR_TILES][VR_T / 32], s_total, s_before;
+    __shared__ Tile s_sums[VR_TILES];
+    __shared__ double s_w[VR_TILES][WARPS], s_r[VR_TILES][WARPS], s_total, s_before, s_warps[WARPS];
+    __shared__ float s_q[VR_TILES][WARPS];      // below 0: some of what is left may be of the other sign
     pdl_wait();
     pdl_launch_dependents();
     const int r = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -305,9 +356,9 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
     const bool inside = my_token >= 0 && my_token < p.V;
     float my_q = inside && p.q ? p.q[((size_t)tid * p.R + r) * p.V + my_token] : 1.0f;
     const float my_x = inside ? value(target[(size_t)tid * p.ld + my_token]) : 0.0f, my_u = tid < n ? p.u[(size_t)r * (p.D + 1) + tid] : 0.0f;
-    const Scale c(PROBS ? 1.0f : p.temperature ? p.temperature[r] : 1.0f);
+    const Scale c(PROBS || !p.temperature ? 1.0f : p.temperature[r]);
     if constexpr (!PROBS) {
-        for (int i = warp; i <= n; i += VR_T / 32) {
+        for (int i = warp; i <= n; i += WARPS) {
             Stat s;
             s.sum = 0.0, s.most = -INFINITY, s.first = 0x7fffffff;
             const Stat* from = p.stats + ((size_t)r * (p.D + 1) + i) * p.stat_parts;
@@ -322,30 +373,66 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
         }
         __syncthreads();
     }
+    double my_w = 0.0, uq = 0.0;      // the draft's weight, or what is given
     if (tid < n) {
-        bool good = false;
+        int good = 0;      // 2: too close to tell by the statistics
         if (inside) {
             if (!(my_q > 0.0f && my_q <= 3.4028235e38f)) my_q = 0.0f;
-            const double uq = (double)my_u * (double)my_q;
+            uq = (double)my_u * (double)my_q;      // (exact)
             if constexpr (PROBS) {
                 good = uq < (my_x > 0.0f && my_x <= 3.4028235e38f ? (double)my_x : 0.0);
             } else {
                 const Stat& s = rows[tid];
-                if (s.most > -INFINITY)
-                    good = c.greedy ? uq < (my_token == s.first ? 1.0 : 0.0) : uq * s.sum < (double)(s.most == INFINITY ? weight_inf(my_x) : c(my_x, s.most));
+                if (s.most > -INFINITY) {
+                    if (c.greedy) {
+                        good = uq < (my_token == s.first ? 1.0 : 0.0);
+                    } else {
+                        if (s.most == INFINITY) my_w = weight_inf(my_x);
+                        else if (my_x > -INFINITY) my_w = exp2(((double)my_x - (double)s.most) * c.exact);
+                        good = uq * s.sum < my_w;
+                        if (s.most < INFINITY && uq > 0.0 && my_w > 0.0 && (c.bent || fabs(uq * s.sum - my_w) <= 0x1p-16 * my_w)) good = 2;
+                    }
+                }
             }
         }
         s_good[tid] = good;
     }
-    __syncthreads();
-    if (tid == 0) {
-        int k = 0;
-        while (k < n && s_good[k]) ++k;
-        s_n = k;
+    auto first_not_good = [&]() {      // to everyone
+        __syncthreads();
+        if (tid == 0) {
+            int k = 0;
+            while (k < n && s_good[k] == 1) ++k;
+            s_n = k;
+        }
+        __syncthreads();
+        return s_n;
+    };
+    int k = first_not_good();
+    struct Loaded {
+        Eight<TX> x;
+        Eight<float> q;
+    };
+    const int tiles = (p.V + VR_TILE - 1) / VR_TILE;
+    if constexpr (!PROBS) {
+        while (k < n && s_good[k] == 2) {
+            const Exact weight(c.exact, rows[k].most);
+            double sum = 0.0;
+#pragma unroll 1
+            for (int t = 0; t < tiles; ++t) {
+                Eight<TX> v;
+                float x[8];
+                v.load(target + (size_t)k * p.ld, t * VR_TILE + VR_PER * tid, p.V, -INFINITY);
+                v.values(x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += weight(x[i]);
+            }
+            sum = cta_sum(sum, s_warps);
+            if (tid == k) s_good[k] = uq * sum < my_w;
+            k = first_not_good();
+        }
     }
-    __syncthreads();
     // ---- what is drawn from, of eight neighbouring tokens
-    const int k = s_n, own = k < n ? p.tokens[(size_t)k * p.R + r] : -1;
+    const int own = k < n ? p.tokens[(size_t)k * p.R + r] : -1;
     const TX* row = target + (size_t)k * p.ld;
     const float* qrow = k < n && p.q ? p.q + ((size_t)k * p.R + r) * p.V : nullptr;
     auto answer = [&](int token) {      // by the whole CTA
@@ -364,92 +451,166 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
             return;
         }
     }
-    const Quick quick(c, st.most);
-    const float inv = (float)(1.0 / st.sum), quick_inv = inv * ex2(-quick.lo);
-    struct Loaded {
-        Eight<TX> x;
-        Eight<float> q;
-    };
+    const Exact weight(c.exact, st.most);
     auto fetch = [&](int i, bool residual, Loaded& z) {
         z.x.load(row, i, p.V, PROBS ? 0.0f : -INFINITY);
         if (residual && qrow) z.q.load(qrow, i, p.V, 0.0f);
     };
-    // (a weight that is NaN is below 0 by fmaxf)
-    auto drawn_from = [&](int i, bool residual, const Loaded& z, float (&w)[8]) {
-        float f = 1.0f, q[8] = {};
-        z.x.values(w);
-        if constexpr (PROBS) {
+    auto weigh = [&](const Loaded& z, double (&w)[8]) {
+        float x[8];
+        z.x.values(x);
+        if (PROBS || weight.inf) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = w[x] <= 3.4028235e38f ? w[x] : 0.0f;
-        } else if (quick.is) {
-            f = quick_inv;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = quick(c, w[x]);
+            for (int j = 0; j < 8; ++j) w[j] = !PROBS ? weight_inf(x[j]) : x[j] > 0.0f && x[j] <= 3.4028235e38f ? x[j] : 0.0f;
         } else {
-            f = inv;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = st.most == INFINITY ? weight_inf(w[x]) : c(w[x], st.most);
+            for (int j = 0; j < 8; ++j) w[j] = weight(x[j]);
         }
-        if (residual && qrow) {
-            z.q.values(q);
-#pragma unroll
-            for (int x = 0; x < 8; ++x) q[x] = fmaxf(q[x] <= 3.4028235e38f ? q[x] : 0.0f, 0.0f);
-        } else if (residual && own >= i && own < i + 8) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) q[x] = i + x == own ? 1.0f : 0.0f;
-        }
-#pragma unroll
-        for (int x = 0; x < 8; ++x) w[x] = fmaxf(fmaf(w[x], f, -q[x]), 0.0f);
     };
-    auto sum_of = [](const float (&w)[8]) { return (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]))); };
-    const int tiles = (p.V + VR_TILE - 1) / VR_TILE, from = part * p.part_tiles, to = min(tiles, from + p.part_tiles);
-    auto sum_tiles = [&](int from, int to, bool residual) {      // every warp's share of each tile
-        constexpr int B = 2;
-        Loaded next[B];
-        auto begin = [&](int t) {
+    auto drafted = [&](int i, const Loaded& z, float (&q)[8]) {
+        if (qrow) {
+            z.q.values(q);
+            uint32_t top = 0;
 #pragma unroll
-            for (int b = 0; b < B; ++b)
-                if (t + b < to) fetch((t + b) * VR_TILE + VR_PER * tid, residual, next[b]);
-        };
-        begin(from);
-        for (int t = from; t < to; t += B) {
-            double s[B];
-            Loaded z[B];
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(q[j]));
+            if (top > 0x7F7FFFFFu) {      // below 0, infinite or NaN
 #pragma unroll
-            for (int b = 0; b < B; ++b) z[b] = next[b];
-            begin(t + B);      // (on their way meanwhile)
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                float w[8];
-                drawn_from((t + b) * VR_TILE + VR_PER * tid, residual, z[b], w);
-                s[b] = sum_of(w);
+                for (int j = 0; j < 8; ++j) q[j] = fmaxf(q[j] <= 3.4028235e38f ? q[j] : 0.0f, 0.0f);
             }
+        } else {
 #pragma unroll
-            for (int x = 16; x > 0; x >>= 1)
+            for (int j = 0; j < 8; ++j) q[j] = i + j == own ? 1.0f : 0.0f;
+        }
+    };
+    const int from = part * p.part_tiles, to = min(tiles, from + p.part_tiles);
+    {      // every warp's share of each tile
+        const bool residual = k < n;
+        Loaded next;
+        if (from < to) fetch(from * VR_TILE + VR_PER * tid, residual, next);
+        for (int t = from; t < to; ++t) {
+            const Loaded z = next;
+            if (t + 1 < to) fetch((t + 1) * VR_TILE + VR_PER * tid, residual, next);      // (on its way meanwhile)
+            double w[8], sw = 0.0, sr = 0.0;
+            float sq = 0.0f;
+            int nearest = -0x7fffffff;
+            weigh(z, w);
+            if (!PROBS || !residual) {
 #pragma unroll
-                for (int b = 0; b < B; ++b) s[b] += __shfl_xor_sync(0xffffffffu, s[b], x);
+                for (int j = 0; j < 8; ++j) sw += w[j];
+            }
+            if (residual) {
+                float q[8];
+                drafted(t * VR_TILE + VR_PER * tid, z, q);
 #pragma unroll
-            for (int b = 0; b < B; ++b)
-                if (lane == 0 && t + b < to) s_warps[t + b][warp] = s[b];
+                for (int j = 0; j < 8; ++j) {
+                    const double left = fma(-st.sum, (double)q[j], w[j]);
+                    if (__double2hiint(left) >= 0) {
+                        sr += left;
+                        if (!PROBS) sq += q[j];
+                    }
+                    // (|left| <= 2^-16 s q is below 2^-15 w, which the upper halves show)
+                    if (!PROBS) nearest = max(nearest, __double2hiint(w[j]) - (__double2hiint(left) & 0x7fffffff));
+                }
+            }
+            if (!PROBS && residual) {      // the lower lanes go on with w, the others with r
+                const bool up = lane & 16;
+                double mine = up ? sr : sw;
+                mine += __shfl_xor_sync(0xffffffffu, up ? sw : sr, 16);
+#pragma unroll
+                for (int x = 8; x > 0; x >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, x);
+                sw = mine, sr = __shfl_down_sync(0xffffffffu, mine, 16);
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, x);
+            } else {      // (one of them)
+                double mine = residual ? sr : sw;
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, x);
+                sw = sr = mine;
+            }
+            const bool again = !PROBS && __any_sync(0xffffffffu, nearest >= 15 << 20);
+            if (lane == 0) s_w[t][warp] = sw, s_r[t][warp] = again ? 0.0 : sr, s_q[t][warp] = again ? -1.0f : sq;
         }
         __syncthreads();
-    };
-    auto tile_sum = [&](int t) {
-        double s = 0.0;
+    }
+    for (int t = from + tid; t < to; t += VR_T) {
+        Tile z = {0.0, 0.0, 0.0f, 0};
 #pragma unroll
-        for (int w = 0; w < VR_T / 32; ++w) s += s_warps[t][w];
-        return s;
+        for (int w = 0; w < WARPS; ++w) z.w += s_w[t][w], z.r += s_r[t][w], z.q += fmaxf(s_q[t][w], 0.0f), z.again |= (s_q[t][w] < 0.0f) << w;
+        if (p.parts == 1) s_sums[t] = z;
+        else p.sums[(size_t)r * tiles + t] = z;
+    }
+    __syncthreads();
+    if (p.parts > 1) {
+        if (tid == 0) {      // (releases what the CTA's threads have stored ahead of the barrier, and acquires what the others' have)
+            int before;
+            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.tickets + r) : "memory");
+            s_last = before == p.parts - 1;
+            if (s_last) p.tickets[r] = 0;
+        }
+        __syncthreads();
+        if (!s_last) return;
+        for (int i = tid; i < tiles * (int)(sizeof(Tile) / 8); i += VR_T) reinterpret_cast<double*>(s_sums)[i] = __ldcg(reinterpret_cast<const double*>(p.sums + (size_t)r * tiles) + i);
+        __syncthreads();
+    }
+    // ---- the last CTA of the request: the row's sum, and what is left above the draft by it
+    double S = 1.0;
+    bool residual = k < n;
+    auto left_of = [&](int t, double (&w)[8]) {      // the thread's tokens of a tile
+        const int i = t * VR_TILE + VR_PER * tid;
+        Loaded z;
+        fetch(i, residual, z);
+        weigh(z, w);
+        if (residual) {
+            float q[8];
+            drafted(i, z, q);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = fmax(fma(-S, (double)q[j], w[j]), 0.0);
+        }
     };
+    // shares of the warps that `which` names of every tile, anew
+    auto shares = [&](auto which) {
+        for (int t0 = 0; t0 < tiles; t0 += 32)
+            for (uint32_t todo = __ballot_sync(0xffffffffu, t0 + lane < tiles && (which(t0 + lane) >> warp & 1)); todo; todo &= todo - 1) {
+                const int t = t0 + __ffs(todo) - 1;
+                double w[8], sum = 0.0;
+                left_of(t, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += w[j];
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                if (lane == 0) s_r[t][warp] = sum;
+            }
+        __syncthreads();
+    };
+    if (!PROBS && residual) {
+        double s = 0.0;
+        for (int t = tid; t < tiles; t += VR_T) s += s_sums[t].w;
+        S = cta_sum(s, s_warps);
+        const double more = S - st.sum;
+        const bool all = fabs(more) > 0x1p-17 * st.sum;
+        auto which = [&](int t) { return all ? (1 << WARPS) - 1 : s_sums[t].again; };
+        shares(which);
+        for (int t = tid; t < tiles; t += VR_T) {
+            Tile& z = s_sums[t];
+            double sum = all ? 0.0 : z.r - more * (double)z.q;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+                if (which(t) >> w & 1) sum += s_r[t][w];
+            z.r = sum;
+        }
+    }
+    // the tile that the draw falls into, the sums ahead of it, the whole; to everyone
     const float u = p.u[(size_t)r * (p.D + 1) + p.D], uc = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-    auto find_tile = [&]() {      // to everyone: the tile that the draw falls into, the sums ahead of it, the whole
+    auto find_tile = [&]() {
         __syncthreads();
         if (warp == 0) {
             const int per = (tiles + 31) / 32, a = min(tiles, lane * per), b = min(tiles, a + per);
+            auto sum = [&](int t) { return residual ? s_sums[t].r : s_sums[t].w; };
             double own = 0.0;
             int last = -1;
             for (int t = a; t < b; ++t) {
-                own += s_sums[t];
-                if (s_sums[t] > 0.0) last = t;
+                own += sum(t);
+                if (sum(t) > 0.0) last = t;
             }
             double upto = own;
 #pragma unroll
@@ -463,61 +624,50 @@ __global__ void __launch_bounds__(VR_T) k_verify_next(const VerifyParams p) {
             if (lane == (there ? __ffs(there) - 1 : 31)) {
                 double before = upto - own;
                 int t = a;
-                for (; t < b && !(before + s_sums[t] > goal); ++t) before += s_sums[t];
+                for (; t < b && !(before + sum(t) > goal); ++t) before += sum(t);
                 if (t >= b) {      // (rounding: the last tile with a weight)
                     t = max(last, 0);
                     before = 0.0;
-                    for (int x = 0; x < t; ++x) before += s_sums[x];
+                    for (int x = 0; x < t; ++x) before += sum(x);
                 }
                 s_tile = t, s_before = before, s_total = total;
             }
         }
         __syncthreads();
     };
-    sum_tiles(from, to, k < n);
-    for (int t = from + tid; t < to; t += VR_T) {
-        const double s = tile_sum(t);
-        if (p.parts == 1) s_sums[t] = s;
-        else p.sums[(size_t)r * tiles + t] = s;
-    }
-    if (p.parts > 1) {
-        __syncthreads();
-        if (tid == 0) {      // (releases what the CTA's threads have stored ahead of the barrier, and acquires what the others' have)
-            int before;
-            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.tickets + r) : "memory");
-            s_last = before == p.parts - 1;
-            if (s_last) p.tickets[r] = 0;
-        }
-        __syncthreads();
-        if (!s_last) return;
-        for (int t = tid; t < tiles; t += VR_T) s_sums[t] = __ldcg(p.sums + (size_t)r * tiles + t);
-    }
-    bool residual = k < n;
     find_tile();
     if (residual && !(s_total > 0.0)) {      // the draft is nowhere below the target: from the target itself
         residual = false;
-        sum_tiles(0, tiles, false);
-        for (int t = tid; t < tiles; t += VR_T) s_sums[t] = tile_sum(t);
+        if constexpr (PROBS) {      // (weights have not been summed so far)
+            shares([](int) { return (1 << WARPS) - 1; });
+            for (int t = tid; t < tiles; t += VR_T) {
+                double sum = 0.0;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) sum += s_r[t][w];
+                s_sums[t].w = sum;
+            }
+        }
         find_tile();
     }
     if (tid == 0) s_token = 0x7fffffff, s_at_most = -1;
     __syncthreads();
     if (s_total > 0.0) {
-        float w[8];
+        double w[8];
         const int i0 = s_tile * VR_TILE + VR_PER * tid;
-        Loaded z;
-        fetch(i0, residual, z);
-        drawn_from(i0, residual, z, w);
-        // (a thread's sum is of f32 sums, those up to each of its tokens are of 64 bits: where rounding leaves none of them above the goal, it is its last with a weight)
-        double all, own_sum = sum_of(w), upto = scan(own_sum, s_warps[0], all);
+        left_of(s_tile, w);
+        double own_sum = 0.0, all;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) own_sum += w[x];
+        // (where rounding leaves none of a thread's tokens above the goal, but their sum is, it is its last with a weight)
+        double upto = scan(own_sum, s_warps, all);
         const double goal = (double)uc * s_total - s_before;
         const bool mine = upto + own_sum > goal;
         int found = 0x7fffffff, last = -1;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            upto += (double)w[x];
-            if (w[x] > 0.0f) last = i0 + x;
-            if (upto > goal && w[x] > 0.0f) found = min(found, i0 + x);
+            upto += w[x];
+            if (w[x] > 0.0) last = i0 + x;
+            if (upto > goal && w[x] > 0.0) found = min(found, i0 + x);
         }
         if (!mine) found = 0x7fffffff;
         else if (found == 0x7fffffff && last >= 0) found = last;
@@ -563,7 +713,7 @@ int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64
     stat_parts = (tiles + stat_tiles - 1) / stat_tiles;
     parts = (tiles + part_tiles - 1) / part_tiles;
     // a workspace of one size, which graphs that hold calls may go on using
-    const size_t stats = align256((size_t)(VR_ROWS + stat_ctas) * sizeof(Stat)), sums = align256((size_t)next_ctas * VR_TILES * sizeof(double)), tickets = align256((size_t)next_ctas * 4);
+    const size_t stats = align256((size_t)(VR_ROWS + stat_ctas) * sizeof(Stat)), sums = align256((size_t)next_ctas * VR_TILES * sizeof(Tile)), tickets = align256((size_t)next_ctas * 4);
     if (!ctx->verify_ws) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone)
@@ -578,7 +728,7 @@ int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64
         ctx->verify_ws = (uint8_t*)ws;
     }
     const VerifyParams p = {target_dev, (size_t)ld, rows, vocab, n_requests, max_drafts, parts, part_tiles, starts_dev, n_drafts_dev, draft_tokens_dev, draft_probs_dev, temperature_dev,
-                            uniforms_dev, tokens_dev, accepted_dev, rejected_dev, (Stat*)ctx->verify_ws, stat_parts, stat_tiles, (double*)(ctx->verify_ws + stats), (int32_t*)(ctx->verify_ws + stats + sums)};
+                            uniforms_dev, tokens_dev, accepted_dev, rejected_dev, (Stat*)ctx->verify_ws, stat_parts, stat_tiles, (Tile*)(ctx->verify_ws + stats), (int32_t*)(ctx->verify_ws + stats + sums)};
     return type == VR_PROBS ? launch<float, true>(ctx, p) : type == DC_TYPE_F32 ? launch<float, false>(ctx, p) : launch<__nv_bfloat16, false>(ctx, p);
 }
 
