@@ -29,7 +29,7 @@ struct dc_kv_dev {
     int max_count = -1;            // of the newest step; -1: none yet
     size_t layer_bytes = 0;
     uint8_t* arena = nullptr;      // [layer][page][key head] records
-    int32_t *lens = nullptr, *held = nullptr, *counts = nullptr, *starts = nullptr, *tables = nullptr, *slot_map = nullptr, *positions = nullptr, *seqs = nullptr, *stack = nullptr;
+    int32_t *lens = nullptr, *held = nullptr, *counts = nullptr, *starts = nullptr, *tables = nullptr, *slot_map = nullptr, *positions = nullptr, *seqs = nullptr, *drafts = nullptr, *stack = nullptr;
     int32_t* numbers = nullptr;    // free pages, entries
     int32_t* scratch = nullptr;    // of a step
     dc_kv_entry* entries = nullptr;

@@ -41,7 +41,7 @@ constexpr int KS_T = 1024, KS_PER = 4, KS_SLOTS = KS_T * KS_PER, KS_APART = 16 *
 struct StepParams {
     int slots, pages_per_seq, max_tokens, max_count;
     const int32_t *drop, *count;
-    int32_t *lens, *held, *counts, *starts, *tables, *slot_map, *positions, *seqs, *stack, *numbers;
+    int32_t *lens, *held, *counts, *starts, *tables, *slot_map, *positions, *seqs, *drafts, *stack, *numbers;
     dc_kv_entry* entries;
     bool apart;                 // units are k_kv_places', which finds what it needs here:
     int32_t* scratch;
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(KS_T) k_kv_step(const StepParams p) {
         for (int i = 0; i < KS_PER; ++i) {
             const int s = s0 + i;
             if (i >= per || s >= p.slots) break;
-            p.lens[s] = kp[i] + cnt[i], p.held[s] = left[i] + asks[i], p.counts[s] = cnt[i], p.starts[s] = z.tok0[s];
+            p.lens[s] = kp[i] + cnt[i], p.held[s] = left[i] + asks[i], p.counts[s] = cnt[i], p.drafts[s] = cnt[i] - 1, p.starts[s] = z.tok0[s];
             if (cnt[i]) p.entries[entry++] = {s, kp[i], cnt[i], z.tok0[s]};
             if (p.apart) out.tok0[s] = z.tok0[s], out.unit0[s] = z.unit0[s], out.free0[s] = z.free0[s], out.give0[s] = z.give0[s], out.keep[s] = kp[i], out.left[s] = left[i];
         }
@@ -355,15 +355,16 @@ int create(dc_ctx* ctx, dc_kv_cache* kv) {
     };
     const size_t slots4 = (size_t)z.slots * 4, tokens4 = (size_t)z.max_tokens * 4;
     const size_t lens = room(slots4), held = room(slots4), counts = room(slots4), starts = room(slots4 + 4), tables = room(slots4 * z.pages_per_seq), map = room(tokens4), positions = room(tokens4),
-                 seqs = room(tokens4), numbers = room(DC_KV_NUMBERS * 4), entries = room(slots4 * 4), scratch = room(slots4 * KS_ARRAYS + sizeof(Totals)), tickets = room((size_t)ctas * z.kv * 4), stack = room((size_t)z.pages * 4), zeroed = at,
+                 seqs = room(tokens4), drafts = room(slots4), numbers = room(DC_KV_NUMBERS * 4), entries = room(slots4 * 4), scratch = room(slots4 * KS_ARRAYS + sizeof(Totals)), tickets = room((size_t)ctas * z.kv * 4), stack = room((size_t)z.pages * 4), zeroed = at,
                  parts = room((size_t)2 * ctas * z.kv * dc_kv16_rows(z.type) * (z.dim + 2) * 4),
                  prompt_parts = room(z.type == DC_TYPE_F32 ? 0 : dc_kv16_prompt_parts(ctx->num_sms, z.kv, z.dim));
     DC_TRY(dc_check_cuda(ctx, cudaMalloc(&z.arena, bytes), "kv_create_dev"));
     DC_TRY(dc_check_cuda(ctx, cudaMalloc(&z.memory, at), "kv_create_dev"));
     DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.arena, 0, bytes, ctx->stream), "kv_create_dev"));
     DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.memory, 0, zeroed, ctx->stream), "kv_create_dev"));
+    DC_TRY(dc_check_cuda(ctx, cudaMemsetAsync(z.memory + drafts, 0xFF, slots4, ctx->stream), "kv_create_dev"));
     auto ints = [&](size_t from) { return (int32_t*)(z.memory + from); };
-    z.lens = ints(lens), z.held = ints(held), z.counts = ints(counts), z.starts = ints(starts), z.tables = ints(tables), z.slot_map = ints(map), z.positions = ints(positions), z.seqs = ints(seqs);
+    z.lens = ints(lens), z.held = ints(held), z.counts = ints(counts), z.starts = ints(starts), z.tables = ints(tables), z.slot_map = ints(map), z.positions = ints(positions), z.seqs = ints(seqs), z.drafts = ints(drafts);
     z.numbers = ints(numbers), z.entries = (dc_kv_entry*)(z.memory + entries), z.scratch = ints(scratch), z.tickets = ints(tickets), z.stack = ints(stack), z.parts = (float*)(z.memory + parts), z.prompt_parts = (float*)(z.memory + prompt_parts);
     DC_TRY(dc_launch_drained(ctx, "k_kv_stack", k_kv_stack, dim3(std::min((z.pages + 255) / 256, ctx->num_sms * 4)), dim3(256), 0, z.stack, z.pages));
     const int32_t free_pages = z.pages;
@@ -439,7 +440,7 @@ int dc_b200_kv_dev_arrays(dc_kv_cache* kv, dc_kv_dev_arrays* out) {
     if (!kv || !out) return DC_B200_INVALID_ARGUMENT;
     if (!kv->dev) return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv_dev_arrays: not a cache whose sequences are on the GPU");
     const dc_kv_dev& z = *kv->dev;
-    *out = {z.lens, z.counts, z.starts, z.tables, z.slot_map, z.positions, z.seqs, z.numbers + DC_KV_FREE};
+    *out = {z.lens, z.counts, z.starts, z.tables, z.slot_map, z.positions, z.seqs, z.numbers + DC_KV_FREE, z.drafts};
     return DC_B200_OK;
 }
 
@@ -451,7 +452,7 @@ int dc_b200_kv_step_dev(dc_ctx* ctx, dc_kv_cache* kv, const int32_t* drop_dev, c
     // pages that new tokens may lie on, and that may be freed: a CTA of 1024 threads, a cluster of eight, or all SMs behind a launch of their own
     const long long units = (long long)z.slots * std::min<long long>(max_count / DC_KV_BLOCK + 2, z.pages_per_seq);
     const bool apart = units > KS_APART;
-    const StepParams p = {z.slots, z.pages_per_seq, z.max_tokens, max_count, drop_dev, count_dev, z.lens, z.held, z.counts, z.starts, z.tables, z.slot_map, z.positions, z.seqs, z.stack,
+    const StepParams p = {z.slots, z.pages_per_seq, z.max_tokens, max_count, drop_dev, count_dev, z.lens, z.held, z.counts, z.starts, z.tables, z.slot_map, z.positions, z.seqs, z.drafts, z.stack,
                           z.numbers, z.entries, apart, z.scratch, (Totals*)(z.scratch + (size_t)KS_ARRAYS * z.slots)};
     const size_t smem = (size_t)z.slots * KS_ARRAYS * 4;
     DC_TRY(dc_kernel_setup(ctx, (const void*)k_kv_step, KS_SLOTS * KS_ARRAYS * 4, "k_kv_step"));

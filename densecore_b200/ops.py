@@ -236,7 +236,8 @@ class Context:
 
     def verify_rows_dev(self, target: int, requests: int, vocab: int, max_drafts: int, draft_tokens: int, draft_probs: int, uniforms: int, tokens: int, accepted: int, rejected: int = 0,
                         starts: int = 0, n_drafts: int = 0, temperature: int = 0, rows: int = 0, ld: int = 0, dtype: str = "f32", probs: bool = False):
-        """Drafted tokens of many requests against device-resident rows of the target (logits, or probabilities); all device addresses, enqueue only."""
+        """Drafted tokens of many requests against device-resident rows of the target (logits, or probabilities); all device addresses, enqueue only.  Behind a step of
+        KVCacheDev starts and n_drafts are its arrays "starts" and "drafts"."""
         self._check(_lib.lib().dc_b200_verify_rows_dev(self.handle, target, -1 if probs else _row_type(dtype), ld, rows or requests * (max_drafts + 1), vocab, requests, max_drafts, starts or None,
                                                        n_drafts or None, draft_tokens or None, draft_probs or None, temperature or None, uniforms, tokens, accepted, rejected or None))
 
@@ -469,7 +470,7 @@ class KVCacheQ4(KVCache):
 class KVCacheDev:
     """Paged cache of 16-bit rows whose sequences' lengths, pages and tables are device memory (dc_b200_kv_create_dev)."""
 
-    ARRAYS = ("lens", "counts", "starts", "tables", "slots", "positions", "seqs", "free")
+    ARRAYS = ("lens", "counts", "starts", "tables", "slots", "positions", "seqs", "free", "drafts")
 
     def __init__(self, ctx: Context, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, max_tokens, dtype="bf16"):
         self.handle = None
@@ -500,7 +501,7 @@ class KVCacheDev:
     def read(self, name: str) -> np.ndarray:
         """One of those arrays on the host."""
         S = self.max_seqs
-        shape = {"lens": S, "counts": S, "starts": S + 1, "tables": (S, self.max_blocks_per_seq), "free": 1}.get(name, self.max_tokens)
+        shape = {"lens": S, "counts": S, "drafts": S, "starts": S + 1, "tables": (S, self.max_blocks_per_seq), "free": 1}.get(name, self.max_tokens)
         self.ctx.synchronize()
         return self.ctx.from_device(self.arrays()[name], np.empty(shape, dtype=np.int32))
 
