@@ -7,11 +7,14 @@
 // cache holds values turned), so that no value changes lanes on the way.
 //   16-bit rows: queries as they are; f32 rows: queries as two fp16 terms (22 bits) of a row times a power of two, rows h and h + 8 of the operand
 //   weights as two terms of the cache's type (bf16 16 bits, fp16 22), so that a result is rounded once; scores, maxima, sums and answers are f32
-// The reference of a row's weights follows its maximum once that is 2^6 ahead: weights up to 64 are as exact, and the answers' factors are rare.
+// The reference of a row's weights follows its maximum once that is 2^6 ahead: weights up to 64 are as exact, and the answers' factors are rare.  fp16 ends at 2^-25, so its reference lies 2^14
+// below the maximum and follows from 2^15 on: a row's weights are off by 2^-22 of themselves or 2^-39 of the largest.  For f32 results, whose second terms are 2^11 fold and have answers of
+// their own, by 2^-22 of themselves or 2^-50 of the largest: the rest of a row beside a key that is far ahead of it.
 // Work is cut on the GPU, since lengths are there: the pages that all sequences' rows see stand in a line, of which every CTA of a key head takes an equal part; a
 // sequence that several CTAs have is joined by the last of them, in the order of its parts, so that results do not depend on who that is.
 // Bound: long caches by HBM (48 sequences of up to 32000 positions, bf16, 32 / 4 heads of 128: 1.90 GB in 293 to 305 us, 97 % of a copy's rate); short ones by one chain of loads and barriers, some
-// 17 thousand cycles: entries, table, queries and first page, pages, parts, ticket, join (one request of 512 positions 9.2 us, 16 f32 ones of 2300 15.5).  Windows of 1024 over 64 sequences (136 MB)
+// 17 thousand cycles: entries, table, queries and first page, pages, parts, ticket, join (one request of 512 positions 10.1 us, 16 f32 ones of 2300 17.0; 32 requests of 5 fp16 tokens 48.5:
+// 9.5, 15.8 and 47.2 while small fp16 weights were lost).  Windows of 1024 over 64 sequences (136 MB)
 // 32.5 us: 4.7 TB/s within the pages, the rest is that chain.  Two pages of a warp at a time: one request 9.9 -> 11.6, windows 36 -> 42; four CTAs an SM for heads of 64: 46.6 -> 47.0.
 #include <math.h>
 
@@ -179,6 +182,9 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
     using R = dc_kv16_rec<HD>;
     using W2 = Two<TC>;
     constexpr bool TERMS = sizeof(TX) == 4;      // queries in two terms
+    // The reference of weights lies this many powers of two below a row's maximum where it is taken anew, and follows once the maximum is LAG further ahead
+    constexpr float AHEAD = std::is_same<TC, __half>::value ? 14.0f : 0.0f, LAG = std::is_same<TC, __half>::value ? 1.0f : 6.0f;
+    static_assert(!std::is_same<TC, __half>::value || AHEAD + LAG <= 15.0f, "weights, and 2^11 times what fp16 leaves of them, are fp16 numbers");
     static_assert(!TERMS || NT == 1, "rows h + 8 of the operand are second terms");
     constexpr int RW = 8 * NT, RT = KR_WARPS * RW, KS = HD / 16, VT = HD / 16, PITCH = HD + 4;
     static_assert(KR_WARPS * RW * (PITCH + 2) * 4 <= KR_SLOTS * R::BYTES, "the warps' parts take the pages' place");
@@ -354,7 +360,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
         }
         // positions between which every row of the warp sees all keys, but for the kept ones
         const int p_least = pos0 + min(r0 / G, count - 1), p_most = pos0 + min((r0 + RW - 1) / G, count - 1), window = p.window ? p.window : 0x7fffffff;
-        float o[VT][NT][4], m_run[NT], l[NT];
+        float o[VT][NT][4], o_lo[TERMS ? VT : 1][4] = {}, m_run[NT], l[NT];      // o_lo: of the weights' second terms, 2^11 fold
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             m_run[x] = -3.4028235e38f, l[x] = 0.0f;
@@ -422,19 +428,22 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
                 }
                 mx[x] = fmaxf(fmaxf(sc[0][2 * x], sc[0][2 * x + 1]), fmaxf(sc[1][2 * x], sc[1][2 * x + 1]));
             }
-            bool follow = mx[0] > m_run[0] + 6.0f;
-            if constexpr (NT == 2) follow = follow || mx[1] > m_run[1] + 6.0f;
+            bool follow = mx[0] > m_run[0] + (AHEAD + LAG);
+            if constexpr (NT == 2) follow = follow || mx[1] > m_run[1] + (AHEAD + LAG);
             if (__any_sync(0xffffffffu, follow)) {
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
                     mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
                     mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-                    const float m_new = fmaxf(m_run[x], mx[x]), corr = ex2(m_run[x] - m_new);
+                    const float m_new = fmaxf(m_run[x], mx[x] - AHEAD), corr = ex2(m_run[x] - m_new);
                     m_run[x] = m_new;
                     l[x] *= corr;
                     const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t4), c1 = __shfl_sync(0xffffffffu, corr, 8 * t4 + 4);
 #pragma unroll
-                    for (int c = 0; c < VT; ++c) o[c][x][0] *= c0, o[c][x][1] *= c1, o[c][x][2] *= c0, o[c][x][3] *= c1;
+                    for (int c = 0; c < VT; ++c) {
+                        o[c][x][0] *= c0, o[c][x][1] *= c1, o[c][x][2] *= c0, o[c][x][3] *= c1;
+                        if constexpr (TERMS) o_lo[c][0] *= c0, o_lo[c][1] *= c1, o_lo[c][2] *= c0, o_lo[c][3] *= c1;
+                    }
                 }
             }
             // ---- weights in two terms
@@ -447,7 +456,8 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
                     l[x] += w0 + w1;
                     hi[x][a] = W2::pack(w0, w1);
                     const float2 f = W2::unpack(hi[x][a]);
-                    lo[x][a] = W2::pack(w0 - f.x, w1 - f.y);
+                    if constexpr (TERMS) lo[x][a] = W2::pack((w0 - f.x) * 2048.0f, (w1 - f.y) * 2048.0f);
+                    else lo[x][a] = W2::pack(w0 - f.x, w1 - f.y);
                 }
             // ---- answers.  Where some row does not see some key, a value that is infinite or NaN there must not meet its weight of 0
             uint32_t tops = 0;      // (a half that is infinite or NaN has an exponent of ones: its top bit in the sum with ONE)
@@ -468,7 +478,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
                         mma<TC>(o[c][x], a, hi[x][0], hi[x][1]);
-                        mma<TC>(o[c][x], a, lo[x][0], lo[x][1]);
+                        mma<TC>(TERMS ? o_lo[TERMS ? c : 0] : o[c][x], a, lo[x][0], lo[x][1]);
                     }
                 }
             } else {
@@ -490,8 +500,13 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
                         ldsm4(to + v_lane + 512 * c, a);
                         a[0] &= seen[0], a[1] &= seen[0], a[2] &= seen[1], a[3] &= seen[1];
                         float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (TERMS) {
+                            mma<TC>(y, a, b[2], b[3]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[i] *= 1.0f / 2048.0f;
+                        }
                         mma<TC>(y, a, b[0], b[1]);
-                        mma<TC>(y, a, b[2], b[3]);
+                        if constexpr (!TERMS) mma<TC>(y, a, b[2], b[3]);
 #pragma unroll
                         for (int z = 0; z < NT; ++z) {
                             if (z != x) continue;
@@ -517,6 +532,10 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
             if (t4 == 0) part_ml[2 * (warp * RW + 8 * x + h)] = m_run[x], part_ml[2 * (warp * RW + 8 * x + h) + 1] = l[x];
 #pragma unroll
             for (int c = 0; c < VT; ++c) {
+                if constexpr (TERMS) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[c][x][i] = fmaf(o_lo[c][i], 1.0f / 2048.0f, o[c][x][i]);
+                }
                 float* at = part + (warp * RW + 8 * x + 2 * t4) * PITCH + 16 * c + h;
                 at[0] = o[c][x][0], at[PITCH] = o[c][x][1], at[8] = o[c][x][2], at[PITCH + 8] = o[c][x][3];
             }
