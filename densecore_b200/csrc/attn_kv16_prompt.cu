@@ -9,7 +9,9 @@
 //   warps 9-10   issue a set's products each
 //   warp 11      looks over the values of tiles that not all rows see all of
 // Weights are rounded to the cache's type (bf16 2^-9, fp16 2^-12) and summed as rounded, so that a row's answer is an average of its values: an error like that of the result's own
-// rounding, of a sum of many.  fp16 ones are 2^7 at the largest, down to 2^-31 of it.
+// rounding, of a sum of many.  fp16 ends at 2^-25: the reference of a row's weights lies 2^14 below its maximum where it is taken anew and follows from 2^15 on, so that what is lost is below 2^-39 of the
+// largest (2^7 and 2^15 took 56 us for a prompt of 2011 tokens for 60 now, and were off by a twentieth in a row
+// whose answer is the rest's beside a key 22 natural units ahead).
 // A value that is infinite or NaN in a tile of which some row does not see all enters it as 0, or the products would carry it to rows that do not see it; rows that do see
 // it are NaN in that dimension.
 // Keys are split over CTAs where there are fewer tiles of rows than SMs; the rows kernel, which follows, adds the parts up (the last CTA of a tile alone took 160 us over a kernel of 30).
@@ -216,7 +218,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
             mbar_arrive(bar(KP_QUERY));
             __syncwarp();
             const float sl2 = fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1e-45f);      // (above 0, if only the least there is: minus infinity stays so)
-            constexpr float LARGEST = F16 ? 7.0f : 0.0f;                                 // of a weight, in powers of two
+            // A row's largest weight where its reference is taken anew, and how far the maximum goes ahead until it is, in powers of two: fp16 ends at 2^16
+            constexpr float LARGEST = F16 ? 14.0f : 0.0f, LAG = F16 ? 1.0f : 8.0f;
+            static_assert(!F16 || LARGEST + LAG <= 15.0f, "weights are fp16 numbers");
             float m_run = -3e38f, l_run[2] = {0.0f, 0.0f};
             bool ok = true;
             __syncwarp();
@@ -269,8 +273,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                     __syncwarp();
                 }
                 const float m_new = fmaxf(m_run, fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sl2, -LARGEST));
-                // the reference follows once the largest score is 2^8 above it: weights up to there are as exact, and the answers' factors are rare
-                if (__any_sync(0xffffffffu, m_new > m_run + 8.0f)) {
+                // the reference follows once the largest score is 2^LAG further above it: weights up to there are as exact, and the answers' factors are rare
+                if (__any_sync(0xffffffffu, m_new > m_run + LAG)) {
                     const float corr = ex2(m_run - m_new);
                     m_run = m_new;
 #pragma unroll

@@ -47,3 +47,10 @@ def run(ctx, dtype, spread, ahead, steps):
 def test_the_rest_beside_a_dominant_key(ctx, dtype, spread, ahead):
     """Single tokens and drafted ones; f32 prompts."""
     run(ctx, dtype, spread, ahead, (([1, 1], 0, 0), ([5, 0], 0, 0), ([1, 0], 20000, 1), ([34 if dtype == "f32" else 16, 0], 0, 0)))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("spread", [0.5, 0.0])
+@pytest.mark.parametrize("ahead", [12, 14, 16, 18, 22])
+def test_the_rest_beside_a_dominant_key_of_prompts(ctx, dtype, spread, ahead):
+    run(ctx, dtype, spread, ahead, (([34, 0], 0, 0), ([70, 1], 20000, 1)))
