@@ -10,8 +10,7 @@
 //   warp 11      looks over the values of tiles that not all rows see all of
 // Weights are rounded to the cache's type (bf16 2^-9, fp16 2^-12) and summed as rounded, so that a row's answer is an average of its values: an error like that of the result's own
 // rounding, of a sum of many.  fp16 ends at 2^-25: the reference of a row's weights lies 2^14 below its maximum where it is taken anew and follows from 2^15 on, so that what is lost is below 2^-39 of the
-// largest (2^7 and 2^15 took 56 us for a prompt of 2011 tokens for 60 now, and were off by a twentieth in a row
-// whose answer is the rest's beside a key 22 natural units ahead).
+// of the largest (from 2^7 on it took 56 us for a prompt of 2011 tokens for 60 now, and a row whose answer is the rest's beside a key 22 natural units ahead was off by three times its rounding).
 // A value that is infinite or NaN in a tile of which some row does not see all enters it as 0, or the products would carry it to rows that do not see it; rows that do see
 // it are NaN in that dimension.
 // Keys are split over CTAs where there are fewer tiles of rows than SMs; the rows kernel, which follows, adds the parts up (the last CTA of a tile alone took 160 us over a kernel of 30).
