@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
     constexpr float AHEAD = std::is_same<TC, __half>::value ? 14.0f : 0.0f, LAG = std::is_same<TC, __half>::value ? 1.0f : 6.0f;
     static_assert(!std::is_same<TC, __half>::value || AHEAD + LAG <= 15.0f, "weights, and 2^11 times what fp16 leaves of them, are fp16 numbers");
     static_assert(!TERMS || NT == 1, "rows h + 8 of the operand are second terms");
+    static_assert(TERMS || !PROMPTS, "prompts of 16-bit rows are k_kv16_prompt's");
     constexpr int RW = 8 * NT, RT = KR_WARPS * RW, KS = HD / 16, VT = HD / 16, PITCH = HD + 4;
     static_assert(KR_WARPS * RW * (PITCH + 2) * 4 <= KR_SLOTS * R::BYTES, "the warps' parts take the pages' place");
     extern __shared__ uint8_t smem_raw[];
@@ -640,10 +641,8 @@ template <int HD>
 int launch_type(dc_ctx* ctx, const dc_kv16_call& c, const RowsParams& p, bool prompts, bool few) {
     const int type = c.kv->dev->type;
     if (type == DC_TYPE_F32) return prompts ? launch<HD, float, __half, 1, true>(ctx, c, p) : launch<HD, float, __half, 1, false>(ctx, c, p);
-    if (type == DC_TYPE_F16)
-        return prompts ? launch<HD, __half, __half, 2, true>(ctx, c, p) : few ? launch<HD, __half, __half, 1, false>(ctx, c, p) : launch<HD, __half, __half, 2, false>(ctx, c, p);
-    return prompts ? launch<HD, __nv_bfloat16, __nv_bfloat16, 2, true>(ctx, c, p)
-           : few   ? launch<HD, __nv_bfloat16, __nv_bfloat16, 1, false>(ctx, c, p) : launch<HD, __nv_bfloat16, __nv_bfloat16, 2, false>(ctx, c, p);
+    if (type == DC_TYPE_F16) return few ? launch<HD, __half, __half, 1, false>(ctx, c, p) : launch<HD, __half, __half, 2, false>(ctx, c, p);
+    return few ? launch<HD, __nv_bfloat16, __nv_bfloat16, 1, false>(ctx, c, p) : launch<HD, __nv_bfloat16, __nv_bfloat16, 2, false>(ctx, c, p);
 }
 
 }  // namespace
