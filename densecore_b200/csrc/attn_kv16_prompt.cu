@@ -401,9 +401,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
             if (lane < 4 && t < n_tiles) page = table[page_at(min(4 * (tile0 + t) + lane, n_pages - 1))];
         };
         look_up(0);
-        for (int t = 0; t < n_tiles; ++t) {
+        uint32_t uses = 0;      // of the stages' first barriers, odd or even
+        int t = 0;
+        for (; t < n_tiles; ++t) {
             const int stage = t % KP_STAGES;
             if (t >= KP_STAGES && !wait(bar(KP_FREE, stage), (t / KP_STAGES - 1) & 1)) break;
+            uses ^= whole(t) ? 0u : 1u << stage;
             const uint32_t b = whole(t) ? bar(KP_FULL, stage) : bar(KP_PRE, stage);
             if (lane == 0) mbar_expect_tx(b, 2 * L::TILE);
             __syncwarp();
@@ -414,6 +417,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv16_prompt(const PromptParam
                 bulk_g2s(to + L::TILE, from + R::VALUES, R::VALUES, b);
             }
             look_up(t + 1);
+        }
+        // no copy may still be in flight when the CTA leaves (at once unless someone gave up)
+        for (int i = max(0, t - KP_STAGES); i < t; ++i) {
+            const int stage = i % KP_STAGES;
+            if (whole(i)) mbar_wait_warp(bar(KP_FULL, stage), (i / KP_STAGES) & 1);
+            else mbar_wait_warp(bar(KP_PRE, stage), ~(uses >> stage) & 1);
         }
     } else if (warp == 11) {
         // ------------------------------------------------------------------ values of tiles that not all rows see all of
