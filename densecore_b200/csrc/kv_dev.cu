@@ -448,6 +448,7 @@ int dc_b200_kv_step_dev(dc_ctx* ctx, dc_kv_cache* kv, const int32_t* drop_dev, c
     DC_TRY(check_call(ctx, kv, "kv_step_dev"));
     dc_kv_dev& z = *kv->dev;
     if (max_count < 0) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_step_dev: at most %d new tokens a sequence", max_count);
+    if (((uintptr_t)drop_dev | (uintptr_t)count_dev) % 4) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "kv_step_dev: an array is not aligned to its elements");
     cudaSetDevice(ctx->device);
     // pages that new tokens may lie on, and that may be freed: a CTA of 1024 threads, a cluster of eight, or all SMs behind a launch of their own
     const long long units = (long long)z.slots * std::min<long long>(max_count / DC_KV_BLOCK + 2, z.pages_per_seq);

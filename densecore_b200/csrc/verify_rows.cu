@@ -704,7 +704,9 @@ int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64
         return dc_fail(ctx, DC_B200_UNSUPPORTED, "verify_rows: %d requests of %d drafts, %d tokens", n_requests, max_drafts, vocab);
     if (n_requests == 0) return DC_B200_OK;
     if (!target_dev || (max_drafts && !draft_tokens_dev) || !uniforms_dev || !tokens_dev || !accepted_dev) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: null buffer");
-    if ((uintptr_t)target_dev % (type == DC_TYPE_BF16 ? 2 : 4) || (uintptr_t)draft_probs_dev % 4) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: a buffer is not aligned to its elements");
+    if ((uintptr_t)target_dev % (type == DC_TYPE_BF16 ? 2 : 4) || ((uintptr_t)draft_probs_dev | (uintptr_t)starts_dev | (uintptr_t)n_drafts_dev | (uintptr_t)draft_tokens_dev | (uintptr_t)temperature_dev |
+                                                                       (uintptr_t)uniforms_dev | (uintptr_t)tokens_dev | (uintptr_t)accepted_dev | (uintptr_t)rejected_dev) % 4)
+        return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: a buffer is not aligned to its elements");
     cudaSetDevice(ctx->device);
     // rows are cut into parts where there are fewer than fill the GPU
     const int tiles = (vocab + VR_TILE - 1) / VR_TILE, n_rows = n_requests * (max_drafts + 1), stat_ctas = VR_STATS_CTAS * ctx->num_sms, next_ctas = VR_NEXT_CTAS * ctx->num_sms;

@@ -1,0 +1,47 @@
+"""Buffers of the calls of steps on the GPU that no kernel may be given: numbers off their own size."""
+from host_util import program, run
+from test_kv_dev_cpu import STUBS
+
+
+def test_step_numbers_off_their_size(tmp_path):
+    exe = program(tmp_path, ["kv_dev", "kv"], STUBS + r"""
+int main() {
+    dc_ctx ctx;
+    dc_kv_cache* kv = nullptr;
+    char* x = (char*)(size_t(1) << 40);      // (nothing reads it here)
+    auto at = [&](int n) { return (const int32_t*)(x + n); };
+    if (dc_b200_kv_create_dev(&ctx, 1, 8, 2, 64, DC_GGML_TYPE_BF16, 60, 4, 40, 100, &kv)) return printf("create\n"), 1;
+    fake::launches = 0;
+    for (int n = 1; n < 4; ++n)
+        if (dc_b200_kv_step_dev(&ctx, kv, at(n), at(0), 3) != DC_B200_INVALID_ARGUMENT || dc_b200_kv_step_dev(&ctx, kv, nullptr, at(n), 3) != DC_B200_INVALID_ARGUMENT || fake::launches) return printf("off by %d\n", n), 1;
+    if (dc_b200_flash_attn_kv_dev(&ctx, kv, 0, x, 0, x, x, 0, 1, 0, 0, x, 0) >= 0) return printf("a refused step counts\n"), 1;
+    if (dc_b200_kv_step_dev(&ctx, kv, at(4), at(8), 3) || fake::launches != 1) return printf("aligned ones\n"), 1;
+    dc_b200_kv_destroy(kv);
+    return fake::bad_frees || !fake::live.empty();
+}
+""")
+    r = run(exe)
+    assert r.returncode == 0, r.stdout
+
+
+def test_verification_buffers(tmp_path):
+    exe = program(tmp_path, ["verify_rows"], r"""
+int main() {
+    dc_ctx ctx;
+    char* x = (char*)(size_t(1) << 40);
+    // target, draft probabilities, starts, numbers of drafts, draft tokens, temperatures, uniform numbers, tokens, accepted, rejected: a megabyte apart
+    auto call = [&](int which, long off) {
+        const char* a[10];
+        for (int i = 0; i < 10; ++i) a[i] = x + ((long)i << 20) + (i == which ? off : 0);
+        return dc_b200_verify_rows_dev(&ctx, a[0], DC_GGML_TYPE_F32, 0, 40, 50, 10, 3, (const int*)a[2], (const int*)a[3], (const int*)a[4], (const float*)a[1], (const float*)a[5], (const float*)a[6],
+                                       (int*)a[7], (int*)a[8], (int*)a[9]);
+    };
+    for (int i = 0; i < 10; ++i)
+        for (int off = 1; off < 4; ++off)
+            if (call(i, off) != DC_B200_INVALID_ARGUMENT || fake::launches || fake::calls) return printf("buffer %d off by %d\n", i, off), 1;
+    if (call(0, 0) || fake::launches != 2) return printf("buffers apart\n"), 1;
+    return 0;
+}
+""")
+    r = run(exe)
+    assert r.returncode == 0, r.stdout
