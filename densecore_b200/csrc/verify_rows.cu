@@ -707,6 +707,14 @@ int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64
     if ((uintptr_t)target_dev % (type == DC_TYPE_BF16 ? 2 : 4) || ((uintptr_t)draft_probs_dev | (uintptr_t)starts_dev | (uintptr_t)n_drafts_dev | (uintptr_t)draft_tokens_dev | (uintptr_t)temperature_dev |
                                                                        (uintptr_t)uniforms_dev | (uintptr_t)tokens_dev | (uintptr_t)accepted_dev | (uintptr_t)rejected_dev) % 4)
         return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: a buffer is not aligned to its elements");
+    // a request's CTAs read these while one of them may have stored its results already
+    const size_t each = (size_t)n_requests * 4, out = each * (max_drafts + 1);
+    auto meet = [](const void* a, size_t n, const void* b, size_t m) { return a && b && (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n; };
+    const void* const read[] = {starts_dev, n_drafts_dev, temperature_dev};
+    for (const void* x : read)
+        if (meet(tokens_dev, out, x, each) || meet(accepted_dev, each, x, each) || meet(rejected_dev, each, x, each))
+            return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: a result overlaps an input");
+    if (meet(rejected_dev, each, tokens_dev, out) || meet(rejected_dev, each, accepted_dev, each)) return dc_fail(ctx, DC_B200_INVALID_ARGUMENT, "verify_rows: results overlap");
     cudaSetDevice(ctx->device);
     // rows are cut into parts where there are fewer than fill the GPU
     const int tiles = (vocab + VR_TILE - 1) / VR_TILE, n_rows = n_requests * (max_drafts + 1), stat_ctas = VR_STATS_CTAS * ctx->num_sms, next_ctas = VR_NEXT_CTAS * ctx->num_sms;

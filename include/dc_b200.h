@@ -368,8 +368,8 @@ DC_B200_API int dc_b200_sample_rows(dc_ctx* ctx, const float* logits_host, int r
  * before it are; a drafted token outside the vocabulary is not.  The next token is drawn from max(0, p - q) at the first draft that is not accepted (from p where that is
  * nothing), from p behind the last: the first token, by index, up to which the sum is above the request's last uniform number times the whole; -1 if nothing has a weight.
  * Results: tokens_dev [n_requests][max_drafts + 1]: the accepted ones, the next one, -1 behind it; accepted_dev [n_requests]; rejected_dev [n_requests] (may be NULL): drafts not accepted,
- * what dc_b200_kv_step_dev takes as drop_dev.  A request without part: tokens -1, both 0.  At most 64 drafts, 389120 tokens of vocabulary, 65536 rows n_requests (max_drafts + 1).  What is decided is decided in 64
- * bits: weights that make up a sum are off by less than 2^-46 of themselves, sums are in an order of their own, the same every time.  Only enqueues; a context's first call makes its
+ * what dc_b200_kv_step_dev takes as drop_dev.  A request without part: tokens -1, both 0.  At most 64 drafts, 389120 tokens of vocabulary, 65536 rows n_requests (max_drafts + 1).  Results do not overlap each
+ * other or the inputs.  What is decided is decided in 64 bits: weights that make up a sum are off by less than 2^-46 of themselves, sums are in an order of their own, the same every time.  Only enqueues; a context's first call makes its
  * workspace (of some MB, whatever the call's sizes) and cannot be captured. */
 DC_B200_API int dc_b200_verify_rows_dev(dc_ctx* ctx, const void* target_dev, int type, int64_t ld, int rows, int vocab, int n_requests, int max_drafts, const int32_t* starts_dev,
                                         const int32_t* n_drafts_dev, const int32_t* draft_tokens_dev, const float* draft_probs_dev, const float* temperature_dev,

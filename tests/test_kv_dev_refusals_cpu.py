@@ -1,4 +1,4 @@
-"""Buffers of the calls of steps on the GPU that no kernel may be given: numbers off their own size."""
+"""Buffers of the calls of steps on the GPU that no kernel may be given: numbers off their own size, and results in the place of what the call's CTAs still read."""
 from host_util import program, run
 from test_kv_dev_cpu import STUBS
 
@@ -39,6 +39,16 @@ int main() {
     for (int i = 0; i < 10; ++i)
         for (int off = 1; off < 4; ++off)
             if (call(i, off) != DC_B200_INVALID_ARGUMENT || fake::launches || fake::calls) return printf("buffer %d off by %d\n", i, off), 1;
+    // ten requests' numbers are 40 bytes: results in, across and just beside those of starts, drafts and temperatures (buffers 2, 3, 5), rejected ones of the other results too
+    for (int result = 7; result < 10; ++result)
+        for (int other : {2, 3, 5, 7, 8, 9}) {
+            if (other >= 7 && (result != 9) == (other != 9)) continue;
+            const long to = ((long)(other - result) << 20), size = result == 7 ? 160 : 40, others = other == 7 ? 160 : 40;
+            for (long d : {0L, 36L, -36L})
+                if (call(result, to + d) != DC_B200_INVALID_ARGUMENT || fake::launches) return printf("buffer %d at %d, %ld bytes on\n", result, other, d), 1;
+            if (call(result, to + others) || call(result, to - size) || fake::launches != 4) return printf("buffer %d beside %d\n", result, other), 1;
+            fake::launches = 0;
+        }
     if (call(0, 0) || fake::launches != 2) return printf("buffers apart\n"), 1;
     return 0;
 }
