@@ -325,8 +325,8 @@ __device__ __forceinline__ double cta_sum(double v, double* warps) {
 }
 
 // One CTA per (request, part of the row drawn from).  Bound: issue slots for many requests' logits (some 40 instructions a token, 14 of them of 64 bits, at 60 % of the slots), HBM for probabilities; latency
-// for few: the rows' statistics, the decisions, the part, the ticket and the draw's tile one after the other.  One request's whole call, with the statistics: 15.5 us; 78 MB of
-// probabilities: 20.5.  Two tiles on their way: 84 us for the 128 requests; sums of w and r reduced one after the other: 84.
+// for few: the rows' statistics, the decisions, the part, the ticket and the draw's tile one after the other.  One request's whole call, with the statistics: 15 us; 78 MB of
+// probabilities: 19.3.  Sums of w and r reduced one after the other: 84 us for the 128 requests.
 template <typename TX, bool PROBS>
 __global__ void __launch_bounds__(VR_T, 3) k_verify_next(const VerifyParams p) {
     constexpr int WARPS = VR_T / 32;
@@ -485,11 +485,14 @@ __global__ void __launch_bounds__(VR_T, 3) k_verify_next(const VerifyParams p) {
     const int from = part * p.part_tiles, to = min(tiles, from + p.part_tiles);
     {      // every warp's share of each tile
         const bool residual = k < n;
-        Loaded next;
-        if (from < to) fetch(from * VR_TILE + VR_PER * tid, residual, next);
-        for (int t = from; t < to; ++t) {
-            const Loaded z = next;
-            if (t + 1 < to) fetch((t + 1) * VR_TILE + VR_PER * tid, residual, next);      // (on its way meanwhile)
+        constexpr int B = PROBS ? 2 : 1;      // tiles on their way at once (probabilities 19.3 us for 22.9 of one; 64-bit weights leave no registers for two: 84 for 81)
+        Loaded next[B];
+        auto begin = [&](int t) {
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (t + b < to) fetch((t + b) * VR_TILE + VR_PER * tid, residual, next[b]);
+        };
+        auto add_up = [&](int t, const Loaded& z) {
             double w[8], sw = 0.0, sr = 0.0;
             float sq = 0.0f;
             int nearest = -0x7fffffff;
@@ -529,6 +532,16 @@ __global__ void __launch_bounds__(VR_T, 3) k_verify_next(const VerifyParams p) {
             }
             const bool again = !PROBS && __any_sync(0xffffffffu, nearest >= 15 << 20);
             if (lane == 0) s_w[t][warp] = sw, s_r[t][warp] = again ? 0.0 : sr, s_q[t][warp] = again ? -1.0f : sq;
+        };
+        begin(from);
+        for (int t = from; t < to; t += B) {
+            Loaded z[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) z[b] = next[b];
+            begin(t + B);      // (meanwhile)
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (t + b < to) add_up(t + b, z[b]);
         }
         __syncthreads();
     }
