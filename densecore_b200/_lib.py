@@ -118,6 +118,7 @@ def _signatures() -> dict:
         "dc_b200_kv_q4_read_block": (i32, [vp, i32, i32, vp, vp]),
         "dc_b200_kv_create_dev": (i32, [vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, pp]),
         "dc_b200_kv_dev_arrays": (i32, [vp, vp]),
+        "dc_b200_kv_dev_drafts": (i32, [vp, vp]),
         "dc_b200_kv_step_dev": (i32, [vp, vp, vp, vp, i32]),
         "dc_b200_kv_dev_write_dev": (i32, [vp, vp, i32, vp, vp, i64]),
         "dc_b200_flash_attn_kv_dev": (i32, [vp, vp, i32, vp, i64, vp, vp, i64, f32, i32, i32, vp, i64]),

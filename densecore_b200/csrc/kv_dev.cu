@@ -440,7 +440,14 @@ int dc_b200_kv_dev_arrays(dc_kv_cache* kv, dc_kv_dev_arrays* out) {
     if (!kv || !out) return DC_B200_INVALID_ARGUMENT;
     if (!kv->dev) return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv_dev_arrays: not a cache whose sequences are on the GPU");
     const dc_kv_dev& z = *kv->dev;
-    *out = {z.lens, z.counts, z.starts, z.tables, z.slot_map, z.positions, z.seqs, z.numbers + DC_KV_FREE, z.drafts};
+    *out = {z.lens, z.counts, z.starts, z.tables, z.slot_map, z.positions, z.seqs, z.numbers + DC_KV_FREE};
+    return DC_B200_OK;
+}
+
+int dc_b200_kv_dev_drafts(dc_kv_cache* kv, const int32_t** drafts_dev_out) {
+    if (!kv || !drafts_dev_out) return DC_B200_INVALID_ARGUMENT;
+    if (!kv->dev) return dc_fail(kv->ctx, DC_B200_INVALID_ARGUMENT, "kv_dev_drafts: not a cache whose sequences are on the GPU");
+    *drafts_dev_out = kv->dev->drafts;
     return DC_B200_OK;
 }
 

@@ -470,7 +470,7 @@ class KVCacheQ4(KVCache):
 class KVCacheDev:
     """Paged cache of 16-bit rows whose sequences' lengths, pages and tables are device memory (dc_b200_kv_create_dev)."""
 
-    ARRAYS = ("lens", "counts", "starts", "tables", "slots", "positions", "seqs", "free", "drafts")
+    ARRAYS = ("lens", "counts", "starts", "tables", "slots", "positions", "seqs", "free")
 
     def __init__(self, ctx: Context, n_layer, n_head, n_kv_head, head_dim, max_blocks, max_seqs, max_blocks_per_seq, max_tokens, dtype="bf16"):
         self.handle = None
@@ -494,9 +494,10 @@ class KVCacheDev:
 
     def arrays(self) -> dict:
         """Device addresses of the sequences' arrays (all int32); they hold for the cache's life."""
-        a = (C.c_void_p * len(self.ARRAYS))()
+        a, drafts = (C.c_void_p * len(self.ARRAYS))(), C.c_void_p()
         self.ctx._check(_lib.lib().dc_b200_kv_dev_arrays(self.handle, a))
-        return dict(zip(self.ARRAYS, (int(x) for x in a)))
+        self.ctx._check(_lib.lib().dc_b200_kv_dev_drafts(self.handle, C.byref(drafts)))
+        return dict(zip(self.ARRAYS, (int(x) for x in a)), drafts=drafts.value)
 
     def read(self, name: str) -> np.ndarray:
         """One of those arrays on the host."""

@@ -280,9 +280,10 @@ typedef struct dc_kv_dev_arrays {
     const int32_t* positions; /* [max_tokens] position of each new token in its sequence */
     const int32_t* seqs;      /* [max_tokens] its sequence */
     const int32_t* free;      /* [1] free pages */
-    const int32_t* drafts;    /* [max_seqs] the step's new tokens of each less one: the n_drafts_dev of dc_b200_verify_rows_dev for a step of drafts behind a last token; -1 without any */
 } dc_kv_dev_arrays;
 DC_B200_API int dc_b200_kv_dev_arrays(dc_kv_cache* kv, struct dc_kv_dev_arrays* out);
+/* One more of them, [max_seqs]: the step's new tokens of each sequence less one, -1 without any: the n_drafts_dev of dc_b200_verify_rows_dev for a step of drafts behind a last token. */
+DC_B200_API int dc_b200_kv_dev_drafts(dc_kv_cache* kv, const int32_t** drafts_dev_out);
 /* A step: every sequence loses its last drop_dev[s] tokens (NULL or below 0: none; all, where it has fewer: it is then empty) and gets count_dev[s] new ones
  * (NULL: none).  A sequence frees the pages that it then needs no more, or asks for those it lacks.  Refused, and so without new tokens (counts says 0), is one
  * that asks for less than 0 or more than max_count tokens or than its table holds; of the others those for whose pages the free ones and the freed ones do not
@@ -357,7 +358,7 @@ DC_B200_API int dc_b200_sample_rows(dc_ctx* ctx, const float* logits_host, int r
 
 /* Verification of the drafted tokens of many requests at once, the answers left on the GPU (the rule of dc_b200_verify_accept).  Request r has n_drafts_dev[r]
  * drafts (NULL: max_drafts; more are taken as max_drafts; below 0: the request takes no part) and that many rows of the target plus one from row starts_dev[r] on
- * (NULL: r (max_drafts + 1)): row i is the target's behind the tokens ahead of draft i.  Behind dc_b200_kv_step_dev both are dc_kv_dev_arrays' own, starts and drafts: a sequence whose tokens the step
+ * (NULL: r (max_drafts + 1)): row i is the target's behind the tokens ahead of draft i.  Behind dc_b200_kv_step_dev both are the cache's own, dc_kv_dev_arrays' starts and dc_b200_kv_dev_drafts: a sequence whose tokens the step
  * refused has no rows, takes no part and so has 0 in rejected_dev; with the number of drafts that were asked for its rows would be the next sequence's.  A request whose rows
  * do not lie within the `rows` rows takes no part.
  * target_dev: rows of vocab numbers ld elements apart (0: dense); type DC_GGML_TYPE_F32 or DC_GGML_TYPE_BF16: logits, p = softmax(logits / temperature), a temperature that

@@ -55,3 +55,26 @@ int main() {
 """)
     r = run(exe)
     assert r.returncode == 0, r.stdout
+
+
+def test_the_arrays_struct_is_as_it_was(tmp_path):
+    """Programs hand over a struct of eight addresses; the numbers of drafts are had by a call of their own."""
+    exe = program(tmp_path, ["kv_dev", "kv"], STUBS + r"""
+int main() {
+    dc_ctx ctx;
+    dc_kv_cache *kv = nullptr, *plain = nullptr;
+    if (dc_b200_kv_create_dev(&ctx, 1, 8, 2, 64, DC_GGML_TYPE_BF16, 60, 4, 40, 100, &kv) || dc_b200_kv_create(&ctx, 1, 2, 128, 9, 2, 4, &plain)) return printf("create\n"), 1;
+    struct { dc_kv_dev_arrays a; const void* behind; } x = {{}, &ctx};
+    const int32_t* drafts = nullptr;
+    if (sizeof(x.a) != 8 * sizeof(void*) || dc_b200_kv_dev_arrays(kv, &x.a) || x.behind != &ctx) return printf("the struct\n"), 1;
+    if (dc_b200_kv_dev_drafts(kv, &drafts) || !drafts) return printf("drafts\n"), 1;
+    for (int s = 0; s < 4; ++s)
+        if (drafts[s] != -1 || x.a.counts[s] != 0) return printf("before a step\n"), 1;
+    if (dc_b200_kv_dev_drafts(kv, nullptr) != DC_B200_INVALID_ARGUMENT || dc_b200_kv_dev_drafts(nullptr, &drafts) != DC_B200_INVALID_ARGUMENT || dc_b200_kv_dev_drafts(plain, &drafts) != DC_B200_INVALID_ARGUMENT)
+        return printf("refusals\n"), 1;
+    dc_b200_kv_destroy(kv), dc_b200_kv_destroy(plain);
+    return fake::bad_frees || !fake::live.empty();
+}
+""")
+    r = run(exe)
+    assert r.returncode == 0, r.stdout
