@@ -10,7 +10,7 @@
 // tokens lie on is a unit of work of its own: it is looked up or granted, and its tokens' places are written.  The largest steps share the units out among all SMs
 // (k_kv_places).
 // Bound: latency of a launch, the loads and two scans (5 us a step of 16 sequences); the largest steps by their tokens' twelve bytes and by the chain of a unit, page, token.  A step of 512
-// sequences that brings a million tokens or takes them back: 13 us, 4 of them its floor at the rate of a copy.
+// sequences that brings two million tokens (up to 8192 each) or takes them back: 13 us, 4 of them its floor at the rate of a copy.
 #include <cooperative_groups.h>
 #include <math.h>
 #include <string.h>

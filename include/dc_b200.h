@@ -289,8 +289,8 @@ DC_B200_API int dc_b200_kv_dev_drafts(dc_kv_cache* kv, const int32_t** drafts_de
  * that asks for less than 0 or more than max_count tokens or than its table holds; of the others those for whose pages the free ones and the freed ones do not
  * suffice, by the sum of all that is asked for up to them, by rising slot; and those with which the sum of new tokens is above max_tokens.  A refused one
  * keeps the pages that it would have used.  The j-th page granted, by rising slot and place, is the j-th one freed, and behind those the newest free one.  Only
- * enqueues, may be captured; a replay is a step of its own.  What max_count says holds for the calls below up to the next step: a replayed
- * one has to find a step of no more. */
+ * enqueues, may be captured; a replay is a step of its own.  What the newest call's max_count says (replays do not count) holds for the
+ * calls below up to the next: each, and its replays, has to find a step of no more. */
 DC_B200_API int dc_b200_kv_step_dev(dc_ctx* ctx, dc_kv_cache* kv, const int32_t* drop_dev, const int32_t* count_dev, int max_count);
 /* Writes the step's rows into one layer: k_dev, v_dev [tokens][n_kv_head][head_dim], rows ld_kv elements apart (0: dense).  Only enqueues, may be captured. */
 DC_B200_API int dc_b200_kv_dev_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* k_dev, const void* v_dev, int64_t ld_kv);
