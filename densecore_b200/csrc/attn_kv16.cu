@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
         }
         // positions between which every row of the warp sees all keys, but for the kept ones
         const int p_least = pos0 + min(r0 / G, count - 1), p_most = pos0 + min((r0 + RW - 1) / G, count - 1), window = p.window ? p.window : 0x7fffffff;
-        float o[VT][NT][4], o_lo[TERMS ? VT : 1][4] = {}, m_run[NT], l[NT];      // o_lo: of the weights' second terms, 2^11 fold
+        float o[VT][NT][4], m_run[NT], l[NT];
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             m_run[x] = -3.4028235e38f, l[x] = 0.0f;
@@ -441,10 +441,7 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
                     l[x] *= corr;
                     const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t4), c1 = __shfl_sync(0xffffffffu, corr, 8 * t4 + 4);
 #pragma unroll
-                    for (int c = 0; c < VT; ++c) {
-                        o[c][x][0] *= c0, o[c][x][1] *= c1, o[c][x][2] *= c0, o[c][x][3] *= c1;
-                        if constexpr (TERMS) o_lo[c][0] *= c0, o_lo[c][1] *= c1, o_lo[c][2] *= c0, o_lo[c][3] *= c1;
-                    }
+                    for (int c = 0; c < VT; ++c) o[c][x][0] *= c0, o[c][x][1] *= c1, o[c][x][2] *= c0, o[c][x][3] *= c1;
                 }
             }
             // ---- weights in two terms
@@ -478,8 +475,16 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
                     ldsm4(to + v_lane + 512 * c, a);
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
-                        mma<TC>(o[c][x], a, hi[x][0], hi[x][1]);
-                        mma<TC>(TERMS ? o_lo[TERMS ? c : 0] : o[c][x], a, lo[x][0], lo[x][1]);
+                        if constexpr (TERMS) {      // (a page's own sums, added to the nearest: the tensor cores' sums are cut off)
+                            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma<TC>(y, a, hi[x][0], hi[x][1]);
+                            mma<TC>(z, a, lo[x][0], lo[x][1]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[c][x][i] += fmaf(z[i], 1.0f / 2048.0f, y[i]);
+                        } else {
+                            mma<TC>(o[c][x], a, hi[x][0], hi[x][1]);
+                            mma<TC>(o[c][x], a, lo[x][0], lo[x][1]);
+                        }
                     }
                 }
             } else {
@@ -533,10 +538,6 @@ __global__ void __launch_bounds__(KR_WARPS * 32, KR_CTAS) k_kv16_rows(const Rows
             if (t4 == 0) part_ml[2 * (warp * RW + 8 * x + h)] = m_run[x], part_ml[2 * (warp * RW + 8 * x + h) + 1] = l[x];
 #pragma unroll
             for (int c = 0; c < VT; ++c) {
-                if constexpr (TERMS) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[c][x][i] = fmaf(o_lo[c][i], 1.0f / 2048.0f, o[c][x][i]);
-                }
                 float* at = part + (warp * RW + 8 * x + 2 * t4) * PITCH + 16 * c + h;
                 at[0] = o[c][x][0], at[PITCH] = o[c][x][1], at[8] = o[c][x][2], at[PITCH + 8] = o[c][x][3];
             }
