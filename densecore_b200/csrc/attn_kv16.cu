@@ -7,6 +7,8 @@
 // cache holds values turned), so that no value changes lanes on the way.
 //   16-bit rows: queries as they are; f32 rows: queries as two fp16 terms (22 bits) of a row times a power of two, rows h and h + 8 of the operand
 //   weights as two terms of the cache's type (bf16 16 bits, fp16 22), so that a result is rounded once; scores, maxima, sums and answers are f32
+//   f32 results: a page's answers begin at 0 and are added to the nearest, as the tensor cores' sums are cut off, some 2^-22.7 of themselves an instruction and always towards 0 (one sum over 1875 pages
+//   was off by 1.7e-4; 16-bit ones leave it at that: 312 instructions of a warp are 5.6e-5)
 // The reference of a row's weights follows its maximum once that is 2^6 ahead: weights up to 64 are as exact, and the answers' factors are rare.  fp16 ends at 2^-25, so its reference lies 2^14
 // below the maximum and follows from 2^15 on: a row's weights are off by 2^-22 of themselves or 2^-39 of the largest.  For f32 results, whose second terms are 2^11 fold and have answers of
 // their own, by 2^-22 of themselves or 2^-50 of the largest: the rest of a row beside a key that is far ahead of it.

@@ -11,6 +11,8 @@
 // Weights are rounded to the cache's type (bf16 2^-9, fp16 2^-12) and summed as rounded, so that a row's answer is an average of its values: an error like that of the result's own
 // rounding, of a sum of many.  fp16 ends at 2^-25: the reference of a row's weights lies 2^14 below its maximum where it is taken anew and follows from 2^15 on, so that what is lost is below 2^-39 of the
 // of the largest (from 2^7 on it took 56 us for a prompt of 2011 tokens for 60 now, and a row whose answer is the rest's beside a key 22 natural units ahead was off by three times its rounding).
+// Answers are the tensor cores' f32 sums, which are cut off by some 2^-23 of themselves an instruction, always towards 0: 150000 keys of one CTA leave a row 1e-3 too small (2000 leave it 1.4e-5), which is
+// a quarter of bf16's rounding and twice fp16's.
 // A value that is infinite or NaN in a tile of which some row does not see all enters it as 0, or the products would carry it to rows that do not see it; rows that do see
 // it are NaN in that dimension.
 // Keys are split over CTAs where there are fewer tiles of rows than SMs; the rows kernel, which follows, adds the parts up (the last CTA of a tile alone took 160 us over a kernel of 30).

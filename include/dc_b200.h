@@ -299,7 +299,8 @@ DC_B200_API int dc_b200_kv_dev_write_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer
  * elements apart (0: dense), any alignment of the elements' own size; out_dev must not overlap the inputs.  Rows behind the step's last token are left as they
  * were.  A value that is infinite or NaN reaches no row that does not see it; one that is seen may make infinity NaN.  A row's weights are off by 2^-22 of themselves or, far below its largest, by 2^-50
  * (F32) or 2^-39 (F16) of that; BF16: by 2^-17 of themselves.  Those of sequences with more than 64 new tokens times query heads of a key head, of 16-bit rows, are rounded once: 2^-12 or 2^-39 of the
- * largest (F16), 2^-9 (BF16).  Only enqueues, may be captured. */
+ * largest (F16), 2^-9 (BF16).  Sums are f32, to the nearest for F32 rows; tensor cores' own for 16-bit ones, which are cut off by some 2^-23 of themselves for every sixteen keys that one CTA takes: within
+ * half a rounding of F16 up to some 30000 keys a CTA, of BF16 up to 250000.  Only enqueues, may be captured. */
 DC_B200_API int dc_b200_flash_attn_kv_dev(dc_ctx* ctx, dc_kv_cache* kv, int layer, const void* q_dev, int64_t ld_q, const void* k_dev, const void* v_dev, int64_t ld_kv, float scale,
                                           int window, int keep_first, void* out_dev, int64_t ld_out);
 /* The rows of one page of one layer, in the type they are held in: [16][n_kv_head][head_dim] each (either may be NULL). */
